@@ -26,6 +26,7 @@
 #include "chronos_lookahead.h"
 #include "chronos_moe.h"
 #include "common.cuh"
+#include "host.cuh"
 #include "attention.cuh"
 #include "ep.cuh"
 #include "lookahead.cuh"
@@ -38,31 +39,8 @@
 namespace chronos {
 namespace {
 
-thread_local std::string g_last_error;
-
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-int fail(int code, const char* fmt, ...) {
-    char buf[512];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof(buf), fmt, ap);
-    va_end(ap);
-    g_last_error = buf;
-    return code;
-}
-
-#define CHRONOS_CUDA_CHECK(expr)                                                              \
-    do {                                                                                      \
-        cudaError_t err_ = (expr);                                                            \
-        if (err_ != cudaSuccess)                                                              \
-            return fail(CHRONOS_ERR_CUDA, "%s failed: %s (%s:%d)", #expr,                     \
-                        cudaGetErrorString(err_), __FILE__, __LINE__);                        \
-    } while (0)
-
 constexpr int kDownWideMinTokens = 1024;  // batches from this size use token-major down tiles
 constexpr int kDmPass = 64;  // token-major down: output columns per epilogue pass
-
-std::atomic<uint64_t> g_kernel_launches{0};
 
 // Decode routing as one cluster launch (route_fused.cuh); off: the two-kernel
 // path.  Set by chronos_moe_set_option("fused_route", 0/1).
@@ -94,29 +72,6 @@ std::atomic<int> g_down_split_target{-1};
 // 196.3-196.9 without; 8-layer model 795 vs 785 us per step).  Set by
 // chronos_moe_set_option("select_plan_one_block", 0/1).
 std::atomic<bool> g_select_one_block{false};
-
-inline void count_launch() { g_kernel_launches.fetch_add(1, std::memory_order_relaxed); }
-
-// Launch with programmatic stream serialisation (`pdl`): the kernel may start
-// while its predecessor in the stream runs and waits for it with pdl_wait().
-// The first kernel of a call is launched without it, so a call never overlaps
-// the previous call's kernels.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                          cudaStream_t st, bool pdl, Args&&... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = pdl ? attr : nullptr;
-    cfg.numAttrs = pdl ? 1 : 0;
-    count_launch();
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-}
 
 // ---------------------------------------------------------------------------
 // stage profiling: CUDA events at the stage boundaries of profiled calls
@@ -176,8 +131,6 @@ std::atomic<int> g_gateup_prefetch_mb{128};
 // kernels; each waits for its predecessor before touching memory.  Off by
 // default: the 8-layer decode step measured 761.0 us with it, 758.7 without.
 std::atomic<bool> g_model_pdl{false};
-
-int sm_count();
 
 int gateup_splits(const ChronosMoeShape& s) {
     if (!g_gateup_split_enabled || s.num_tokens < 1 || s.num_tokens > kSelectPlanMaxTokens ||
@@ -274,25 +227,6 @@ int validate_shape(const ChronosMoeShape* s) {
 // TMA descriptors (cuTensorMapEncodeTiled through the runtime's driver entry
 // point), cached by (address, extents, box).
 // ---------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn get_encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-                cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-    });
-    return fn;
-}
-
 struct MapKey {
     uint64_t ptr, rows, cols, box_rows, dtype;
     bool operator==(const MapKey& o) const {
@@ -350,39 +284,6 @@ int make_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, u
         g_maps.emplace(key, m);
     }
     *out = m;
-    return CHRONOS_OK;
-}
-
-int sm_count() {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    static int cached[64] = {0};
-    if (dev < 64 && cached[dev] > 0) return cached[dev];
-    int n = 0;
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    if (n <= 0) n = 148;
-    if (dev < 64) cached[dev] = n;
-    return n;
-}
-
-template <typename K>
-int set_smem(K kernel, int bytes) {
-    // The attribute is a limit that sticks to the function on its device, and
-    // setting it costs host time on every layer call: raise it only when a launch
-    // needs more than the largest value set so far on this device (a smaller
-    // launch fits under a larger limit; lowering it would break a later larger
-    // launch that found its size "already set").
-    static std::mutex mu;
-    static std::map<std::pair<const void*, int>, int> limit;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const auto key = std::make_pair(reinterpret_cast<const void*>(kernel), dev);
-    std::lock_guard<std::mutex> lk(mu);
-    auto it = limit.find(key);
-    if (it != limit.end() && it->second >= bytes) return CHRONOS_OK;
-    CHRONOS_CUDA_CHECK(
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    limit[key] = bytes;
     return CHRONOS_OK;
 }
 

@@ -1,0 +1,121 @@
+// host.cuh — host-side helpers shared by the C ABI's translation units: the
+// calling thread's error text, kernel launches and their count, per-kernel
+// shared-memory limits, the driver's tensor-map encoder.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+#include <map>
+#include <mutex>
+#include <string>
+#include <utility>
+
+#include "chronos_moe.h"
+
+namespace chronos {
+
+inline thread_local std::string g_last_error;
+
+inline int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+inline int fail(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    g_last_error = buf;
+    return code;
+}
+
+#define CHRONOS_CUDA_CHECK(expr)                                                              \
+    do {                                                                                      \
+        cudaError_t err_ = (expr);                                                            \
+        if (err_ != cudaSuccess)                                                              \
+            return fail(CHRONOS_ERR_CUDA, "%s failed: %s (%s:%d)", #expr,                     \
+                        cudaGetErrorString(err_), __FILE__, __LINE__);                        \
+    } while (0)
+
+inline std::atomic<uint64_t> g_kernel_launches{0};
+
+inline void count_launch() { g_kernel_launches.fetch_add(1, std::memory_order_relaxed); }
+
+// Launch with programmatic stream serialisation (`pdl`): the kernel may start
+// while its predecessor in the stream runs and waits for it with pdl_wait().
+// The first kernel of a call is launched without it, so a call never overlaps
+// the previous call's kernels.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                          cudaStream_t st, bool pdl, Args&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = pdl ? attr : nullptr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    count_launch();
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// cuTensorMapEncodeTiled through the runtime's driver entry point.
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn get_encode_fn() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+                cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(p);
+    });
+    return fn;
+}
+
+inline int sm_count() {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    static int cached[64] = {0};
+    if (dev < 64 && cached[dev] > 0) return cached[dev];
+    int n = 0;
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (n <= 0) n = 148;
+    if (dev < 64) cached[dev] = n;
+    return n;
+}
+
+template <typename K>
+int set_smem(K kernel, int bytes) {
+    // The attribute is a limit that sticks to the function on its device, and
+    // setting it costs host time on every layer call: raise it only when a launch
+    // needs more than the largest value set so far on this device (a smaller
+    // launch fits under a larger limit; lowering it would break a later larger
+    // launch that found its size "already set").
+    static std::mutex mu;
+    static std::map<std::pair<const void*, int>, int> limit;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const auto key = std::make_pair(reinterpret_cast<const void*>(kernel), dev);
+    std::lock_guard<std::mutex> lk(mu);
+    auto it = limit.find(key);
+    if (it != limit.end() && it->second >= bytes) return CHRONOS_OK;
+    CHRONOS_CUDA_CHECK(
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    limit[key] = bytes;
+    return CHRONOS_OK;
+}
+
+}  // namespace chronos
