@@ -49,7 +49,10 @@ EXPORTS = ("chronos_moe_workspace_size", "chronos_moe_forward", "chronos_moe_rou
            "chronos_ep_dispatch", "chronos_ep_combine", "chronos_ep_dispatch_args_size",
            "chronos_ep_combine_args_size", "chronos_lookahead_forward", "chronos_lookahead_args_size",
            "chronos_mla_decode", "chronos_sw_decode", "chronos_add_rmsnorm", "chronos_attn_args_size",
-           "chronos_norm_args_size", "chronos_argmax_rows")
+           "chronos_norm_args_size", "chronos_argmax_rows", "chronos_paged_append", "chronos_paged_decode",
+           "chronos_paged_evict", "chronos_window_attention", "chronos_paged_decode_workspace",
+           "chronos_paged_evict_workspace", "chronos_paged_append_args_size", "chronos_paged_decode_args_size",
+           "chronos_paged_evict_args_size", "chronos_window_attn_args_size")
 
 EP_MAX_RANKS = 32  # CHRONOS_EP_MAX_RANKS
 
@@ -204,6 +207,129 @@ class ChronosNormArgs(ctypes.Structure):
     ]
 
 
+class ChronosPagedCache(ctypes.Structure):
+    """include/chronos_paged.h"""
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("table_width", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("k_page_stride", ctypes.c_int64),
+        ("k_slot_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_page_stride", ctypes.c_int64),
+        ("v_slot_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("page_table", ctypes.c_void_p),
+        ("page_table_stride", ctypes.c_int64),
+        ("lens", ctypes.c_void_p),
+    ]
+
+
+class ChronosPagedAppendArgs(ctypes.Structure):
+    """include/chronos_paged.h"""
+    _fields_ = [
+        ("cache", ChronosPagedCache),
+        ("num_tokens", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_row_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_row_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("seen", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("slot_cap", ctypes.c_int64),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class ChronosPagedDecodeArgs(ctypes.Structure):
+    """include/chronos_paged.h"""
+    _fields_ = [
+        ("cache", ChronosPagedCache),
+        ("heads", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("q", ctypes.c_void_p),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_row_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+        ("lse", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("weights_out", ctypes.c_void_p),
+        ("slot_cap", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class ChronosPagedEvictArgs(ctypes.Structure):
+    """include/chronos_paged.h"""
+    _fields_ = [
+        ("cache", ChronosPagedCache),
+        ("budget", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("recent", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("seen", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("weights_out", ctypes.c_void_p),
+        ("positions_out", ctypes.c_void_p),
+        ("slot_cap", ctypes.c_int64),
+        ("lens_out", ctypes.c_void_p),
+        ("src", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class ChronosWindowAttnArgs(ctypes.Structure):
+    """include/chronos_paged.h"""
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("num_q", ctypes.c_int64),
+        ("num_k", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("k_row_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_row_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("out_row_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+        ("cu_q", ctypes.c_void_p),
+        ("cu_k", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -272,6 +398,23 @@ def load_library(path: str = LIB_PATH):
         lib.chronos_attn_args_size.restype = ctypes.c_size_t
         lib.chronos_norm_args_size.argtypes = []
         lib.chronos_norm_args_size.restype = ctypes.c_size_t
+        for fn, st in (("chronos_paged_append", ChronosPagedAppendArgs), ("chronos_paged_decode", ChronosPagedDecodeArgs),
+                       ("chronos_paged_evict", ChronosPagedEvictArgs),
+                       ("chronos_window_attention", ChronosWindowAttnArgs)):
+            getattr(lib, fn).argtypes = [ctypes.POINTER(st), ctypes.c_void_p]
+            getattr(lib, fn).restype = ctypes.c_int
+        for fn, st in (("chronos_paged_decode_workspace", ChronosPagedDecodeArgs),
+                       ("chronos_paged_evict_workspace", ChronosPagedEvictArgs)):
+            getattr(lib, fn).argtypes = [ctypes.POINTER(st)]
+            getattr(lib, fn).restype = ctypes.c_size_t
+        for fn, st in (("chronos_paged_append_args_size", ChronosPagedAppendArgs),
+                       ("chronos_paged_decode_args_size", ChronosPagedDecodeArgs),
+                       ("chronos_paged_evict_args_size", ChronosPagedEvictArgs),
+                       ("chronos_window_attn_args_size", ChronosWindowAttnArgs)):
+            getattr(lib, fn).argtypes = []
+            getattr(lib, fn).restype = ctypes.c_size_t
+            if getattr(lib, fn)() != ctypes.sizeof(st):
+                raise RuntimeError("paged-cache args layout mismatch between the library and the binding")
         if (lib.chronos_attn_args_size() != ctypes.sizeof(ChronosAttnArgs)
                 or lib.chronos_norm_args_size() != ctypes.sizeof(ChronosNormArgs)):
             raise RuntimeError("attention args layout mismatch between the library and the binding")

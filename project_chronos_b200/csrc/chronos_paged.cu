@@ -1,0 +1,457 @@
+// chronos_paged.cu — the C ABI of include/chronos_paged.h: argument checks,
+// workspace layout, choice of kernel and launches.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "chronos_paged.h"
+#include "common.cuh"
+#include "host.cuh"
+#include "paged.cuh"
+#include "window_attention.cuh"
+
+namespace chronos {
+namespace {
+
+size_t elem_bytes(int dtype) { return dtype == CHRONOS_DTYPE_FP32 ? 4 : 2; }
+bool dtype_known(int d) { return d == CHRONOS_DTYPE_BF16 || d == CHRONOS_DTYPE_FP16 || d == CHRONOS_DTYPE_FP32; }
+size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+bool multiples(int64_t of, std::initializer_list<int64_t> v) {
+    return std::all_of(v.begin(), v.end(), [of](int64_t x) { return x % of == 0; });
+}
+
+int check_cache(const ChronosPagedCache& c, const char* what) {
+    if (c.batch < 0 || c.kv_heads < 1 || c.head_dim < 1 || c.head_dim > CHRONOS_PAGED_MAX_HEAD_DIM ||
+        !dtype_known(c.dtype))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: batch %d, kv_heads %d, head_dim %d (1..%d), dtype %d", what, c.batch,
+                    c.kv_heads, c.head_dim, CHRONOS_PAGED_MAX_HEAD_DIM, c.dtype);
+    if (c.num_pages < 0 || c.page_size < 1 || c.table_width < 0)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: num_pages %d, page_size %d (>= 1), table_width %d", what, c.num_pages,
+                    c.page_size, c.table_width);
+    if (static_cast<int64_t>(c.batch) * c.kv_heads > (1 << 20))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: batch %d * kv_heads %d too large", what, c.batch, c.kv_heads);
+    return CHRONOS_OK;
+}
+int check_cache_pointers(const ChronosPagedCache& c, const char* what) {
+    if (c.batch > 0 && (c.lens == nullptr || (c.table_width > 0 && c.page_table == nullptr) ||
+                        (c.num_pages > 0 && (c.k_pages == nullptr || c.v_pages == nullptr))))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: lens, page_table, k_pages and v_pages are required", what);
+    return CHRONOS_OK;
+}
+// Slots a sequence can have: what its table (and the per-slot arrays, when there are any) hold.
+int slot_limit(const ChronosPagedCache& c, int64_t slot_cap, bool has_cap) {
+    int64_t n = static_cast<int64_t>(c.table_width) * c.page_size;
+    if (has_cap) n = std::min(n, slot_cap);
+    return static_cast<int>(std::min<int64_t>(n, (1 << 30)));
+}
+
+// ---------------------------------------------------------------------------
+// one-token attention
+// ---------------------------------------------------------------------------
+struct DecodePlan {
+    bool mma;
+    int dp;              // padded head dimension of the tensor-core path
+    int rows, parts, grid, part_stride, max_vis;
+    int64_t score_stride;
+    size_t o_part_o, o_part_ml, o_lse2, o_scores, total;
+};
+
+int check_decode(const ChronosPagedDecodeArgs* a) {
+    const char* what = "chronos_paged_decode";
+    if (a == nullptr) return fail(CHRONOS_ERR_INVALID_ARG, "%s: args is NULL", what);
+    if (int rc = check_cache(a->cache, what)) return rc;
+    if (a->heads < 1 || a->heads % a->cache.kv_heads || a->heads / a->cache.kv_heads > kPdMaxRep)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: heads %d must be 1..%d times kv_heads %d", what, a->heads, kPdMaxRep,
+                    a->cache.kv_heads);
+    if (a->window < 0 || a->sinks < 0)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: window %d, sinks %d must not be negative", what, a->window, a->sinks);
+    if (!(a->scale > 0.0f) || !std::isfinite(a->scale))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: scale %g must be positive", what, a->scale);
+    if ((a->weights == nullptr) != (a->weights_out == nullptr))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: weights and weights_out go together", what);
+    if (a->weights != nullptr && a->slot_cap < 0)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: slot_cap %lld", what, static_cast<long long>(a->slot_cap));
+    return CHRONOS_OK;
+}
+
+// The tensor-core path: 16-bit types whose rows can be copied 16 bytes at a time.
+bool decode_uses_mma(const ChronosPagedDecodeArgs* a) {
+    const ChronosPagedCache& c = a->cache;
+    return c.dtype != CHRONOS_DTYPE_FP32 && c.head_dim % 8 == 0 && aligned(c.k_pages, 16) && aligned(c.v_pages, 16) &&
+           aligned(a->q, 4) && aligned(a->out, 4) &&
+           multiples(8, {c.k_page_stride, c.k_slot_stride, c.k_head_stride, c.v_page_stride, c.v_slot_stride,
+                         c.v_head_stride}) &&
+           multiples(2, {a->q_row_stride, a->q_head_stride, a->out_row_stride, a->out_head_stride});
+}
+
+DecodePlan decode_plan(const ChronosPagedDecodeArgs* a) {
+    const ChronosPagedCache& c = a->cache;
+    DecodePlan d{};
+    d.mma = decode_uses_mma(a);
+    d.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
+    d.rows = d.mma ? 16 : kPdSimtRows;
+    const int rep = a->heads / c.kv_heads;
+    d.parts = (rep + d.rows - 1) / d.rows;
+    const int limit = slot_limit(c, a->slot_cap, a->weights != nullptr);
+    d.max_vis = a->window > 0 ? static_cast<int>(std::min<int64_t>(limit, static_cast<int64_t>(a->window) + a->sinks)) : limit;
+    const int per_sm = d.mma ? (d.dp == 256 ? 1 : 2) : 4;
+    const int64_t blocks = (static_cast<int64_t>(d.max_vis) + kPdBlock - 1) / kPdBlock;
+    const int64_t units = std::max<int64_t>(1, blocks) * c.batch * c.kv_heads * d.parts;
+    d.grid = static_cast<int>(std::min<int64_t>({units, static_cast<int64_t>(per_sm) * sm_count(), kPdMaxGrid}));
+    d.part_stride = d.mma ? d.dp : static_cast<int>(round_up(c.head_dim, 4));
+    size_t at = 0;
+    auto take = [&at](size_t bytes) {
+        const size_t o = at;
+        at = round_up(at + bytes, 256);
+        return o;
+    };
+    const size_t slots = 2 * static_cast<size_t>(d.grid) * d.rows;
+    d.o_part_o = take(slots * d.part_stride * 4);
+    d.o_part_ml = take(slots * 8);
+    if (a->weights != nullptr) {
+        d.score_stride = round_up(d.max_vis, kPdBlock);
+        d.o_lse2 = take(static_cast<size_t>(c.batch) * a->heads * 4);
+        d.o_scores = take(static_cast<size_t>(c.batch) * a->heads * d.score_stride * 4);
+    }
+    d.total = std::max<size_t>(at, 256);
+    return d;
+}
+
+template <typename T, int DP>
+int launch_decode_mma(const PagedDecodeParams& p, cudaStream_t st) {
+    using S = PagedMma<DP>;
+    void (*kernel)(PagedDecodeParams) = p.rep > 8 ? paged_decode_mma_kernel<T, DP, true> : paged_decode_mma_kernel<T, DP, false>;
+    if (int rc = set_smem(kernel, S::kSmem)) return rc;
+    CHRONOS_CUDA_CHECK(launch_kernel(kernel, dim3(p.grid), dim3(kPdThreads), S::kSmem, st, false, p));
+    return CHRONOS_OK;
+}
+
+template <typename T>
+int launch_decode(const PagedDecodeParams& p, const DecodePlan& d, bool vec, cudaStream_t st) {
+    if constexpr (sizeof(T) == 2) {
+        if (d.mma) {
+            const int rc = d.dp == 64 ? launch_decode_mma<T, 64>(p, st)
+                                      : d.dp == 128 ? launch_decode_mma<T, 128>(p, st) : launch_decode_mma<T, 256>(p, st);
+            if (rc) return rc;
+        }
+    }
+    if (!d.mma)
+        CHRONOS_CUDA_CHECK(launch_kernel(vec ? paged_decode_simt_kernel<T, true> : paged_decode_simt_kernel<T, false>,
+                                         dim3(p.grid), dim3(kPdThreads), 0, st, false, p));
+    // rows of one unit are never cut: then there is nothing to join
+    const bool joins = d.max_vis > kPdBlock;
+    PagedDecodeParams j = p;
+    j.join_blocks = joins ? p.c.batch * p.heads : 0;
+    j.weight_chunks = (p.max_slots + kPdWeightSlots - 1) / kPdWeightSlots;
+    const int64_t blocks = j.join_blocks + (p.weights != nullptr ? static_cast<int64_t>(p.c.batch) * p.c.kv_heads * j.weight_chunks : 0);
+    if (blocks > 0)
+        CHRONOS_CUDA_CHECK(launch_kernel(paged_join_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(kPdJoinThreads), 0,
+                                         st, true, j));
+    return CHRONOS_OK;
+}
+
+// ---------------------------------------------------------------------------
+// eviction
+// ---------------------------------------------------------------------------
+struct EvictPlan {
+    int64_t max_moves;
+    size_t o_moves, o_counts, o_lens, total;
+};
+
+int check_evict(const ChronosPagedEvictArgs* a) {
+    const char* what = "chronos_paged_evict";
+    if (a == nullptr) return fail(CHRONOS_ERR_INVALID_ARG, "%s: args is NULL", what);
+    if (int rc = check_cache(a->cache, what)) return rc;
+    if (a->budget < 1 || a->sinks < 0 || a->recent < 0 ||
+        static_cast<int64_t>(a->sinks) + a->recent > a->budget)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: budget %d must be >= 1 and >= sinks %d + recent %d", what, a->budget,
+                    a->sinks, a->recent);
+    if (a->slot_cap < 0) return fail(CHRONOS_ERR_INVALID_ARG, "%s: slot_cap %lld", what, static_cast<long long>(a->slot_cap));
+    return CHRONOS_OK;
+}
+
+EvictPlan evict_plan(const ChronosPagedEvictArgs* a) {
+    EvictPlan e{};
+    const int limit = slot_limit(a->cache, a->slot_cap, true);
+    e.max_moves = std::max(0, std::min(a->budget, limit - a->budget));
+    const size_t rows = static_cast<size_t>(a->cache.batch) * a->cache.kv_heads;
+    e.o_moves = 0;
+    e.o_counts = round_up(rows * e.max_moves * 8, 256);
+    e.o_lens = e.o_counts + round_up(rows * 4, 256);
+    e.total = e.o_lens + round_up(static_cast<size_t>(a->cache.batch) * 4, 256) + 256;
+    return e;
+}
+
+// Bytes of the widest unit that every row can be copied in: 16, or one element.
+bool copies16(const ChronosPagedCache& c) {
+    const int64_t n = 16 / static_cast<int64_t>(elem_bytes(c.dtype));
+    return c.head_dim % n == 0 && aligned(c.k_pages, 16) && aligned(c.v_pages, 16) &&
+           multiples(n, {c.k_page_stride, c.k_slot_stride, c.k_head_stride, c.v_page_stride, c.v_slot_stride, c.v_head_stride});
+}
+
+// ---------------------------------------------------------------------------
+// prompt attention
+// ---------------------------------------------------------------------------
+template <typename T>
+int launch_window_simt(const WindowParams& p, cudaStream_t st) {
+    void (*kernel)(WindowParams) = p.dim <= 64 ? window_simt_kernel<T, 1>
+                                   : p.dim <= 128 ? window_simt_kernel<T, 2>
+                                   : p.dim <= 192 ? window_simt_kernel<T, 3> : window_simt_kernel<T, 4>;
+    const int smem = window_simt_smem(p.dim);
+    if (int rc = set_smem(kernel, smem)) return rc;
+    const int64_t tiles = (p.num_q + kWsRows - 1) / kWsRows + p.batch;
+    CHRONOS_CUDA_CHECK(launch_kernel(kernel, dim3(static_cast<unsigned>(tiles * p.heads)), dim3(kWsThreads), smem, st, false, p));
+    return CHRONOS_OK;
+}
+
+template <typename T>
+int window_impl(const WindowParams& p, cudaStream_t st) {
+    return launch_window_simt<T>(p, st);
+}
+
+}  // namespace
+}  // namespace chronos
+
+extern "C" size_t chronos_paged_decode_workspace(const ChronosPagedDecodeArgs* a) {
+    using namespace chronos;
+    g_last_error.clear();
+    if (check_decode(a)) return 0;
+    return decode_plan(a).total;
+}
+
+extern "C" int chronos_paged_decode(const ChronosPagedDecodeArgs* a, void* stream) {
+    using namespace chronos;
+    g_last_error.clear();
+    const char* what = "chronos_paged_decode";
+    if (int rc = check_decode(a)) return rc;
+    if (a->cache.batch == 0) return CHRONOS_OK;
+    if (int rc = check_cache_pointers(a->cache, what)) return rc;
+    if (a->q == nullptr || a->out == nullptr) return fail(CHRONOS_ERR_INVALID_ARG, "%s: q and out are required", what);
+    const DecodePlan d = decode_plan(a);
+    const int64_t units = (static_cast<int64_t>(d.max_vis) / kPdBlock + 1) * a->cache.batch * a->cache.kv_heads * d.parts;
+    const int limit = slot_limit(a->cache, a->slot_cap, a->weights != nullptr);
+    const int64_t adds = static_cast<int64_t>(a->cache.batch) * a->heads +
+                         static_cast<int64_t>(a->cache.batch) * a->cache.kv_heads * (limit / kPdWeightSlots + 1);
+    if (units >= INT32_MAX || adds >= INT32_MAX)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: batch %d * heads * slots %d too large", what, a->cache.batch, limit);
+    if (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < d.total)
+        return fail(CHRONOS_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes, %zu (256-byte aligned) needed", what,
+                    a->workspace == nullptr ? size_t{0} : a->workspace_bytes, d.total);
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    PagedDecodeParams p{};
+    p.c = a->cache;
+    p.heads = a->heads;
+    p.rep = a->heads / a->cache.kv_heads;
+    p.rows = d.rows;
+    p.parts = d.parts;
+    p.window = a->window;
+    p.sinks = a->window > 0 ? a->sinks : 0;
+    p.max_slots = limit;
+    p.sl2 = static_cast<float>(static_cast<double>(a->scale) * 1.4426950408889634);
+    p.q = a->q;
+    p.q_row = a->q_row_stride;
+    p.q_head = a->q_head_stride;
+    p.out = a->out;
+    p.out_row = a->out_row_stride;
+    p.out_head = a->out_head_stride;
+    p.lse = a->lse;
+    p.weights = a->weights;
+    p.weights_out = a->weights_out;
+    p.slot_cap = a->slot_cap;
+    p.grid = d.grid;
+    p.part_stride = d.part_stride;
+    p.part_o = reinterpret_cast<float*>(ws + d.o_part_o);
+    p.part_ml = reinterpret_cast<float*>(ws + d.o_part_ml);
+    if (a->weights != nullptr) {
+        p.lse2 = reinterpret_cast<float*>(ws + d.o_lse2);
+        p.scores = reinterpret_cast<float*>(ws + d.o_scores);
+        p.score_stride = d.score_stride;
+    }
+    p.status = a->status;
+    const int64_t ve = a->cache.dtype == CHRONOS_DTYPE_FP32 ? 16 : 8;
+    const bool vec = a->cache.head_dim % 4 == 0 && aligned(a->cache.k_pages, ve) && aligned(a->cache.v_pages, ve) &&
+                     multiples(4, {a->cache.k_page_stride, a->cache.k_slot_stride, a->cache.k_head_stride,
+                                   a->cache.v_page_stride, a->cache.v_slot_stride, a->cache.v_head_stride});
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (a->cache.dtype) {
+        case CHRONOS_DTYPE_BF16: return launch_decode<__nv_bfloat16>(p, d, vec, st);
+        case CHRONOS_DTYPE_FP16: return launch_decode<__half>(p, d, vec, st);
+        default: return launch_decode<float>(p, d, vec, st);
+    }
+}
+
+extern "C" int chronos_paged_append(const ChronosPagedAppendArgs* a, void* stream) {
+    using namespace chronos;
+    g_last_error.clear();
+    const char* what = "chronos_paged_append";
+    if (a == nullptr) return fail(CHRONOS_ERR_INVALID_ARG, "%s: args is NULL", what);
+    if (int rc = check_cache(a->cache, what)) return rc;
+    if (a->num_tokens < 0 || a->num_tokens > INT32_MAX)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: num_tokens %lld", what, static_cast<long long>(a->num_tokens));
+    if (a->cu_seqlens == nullptr && a->num_tokens != a->cache.batch)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: %lld rows for %d sequences without cu_seqlens", what,
+                    static_cast<long long>(a->num_tokens), a->cache.batch);
+    if (a->positions != nullptr && a->seen == nullptr)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: positions need seen", what);
+    const bool arrays = a->weights != nullptr || a->positions != nullptr;
+    if (arrays && a->slot_cap < 0)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: slot_cap %lld", what, static_cast<long long>(a->slot_cap));
+    if (a->num_tokens == 0 || a->cache.batch == 0) return CHRONOS_OK;
+    if (int rc = check_cache_pointers(a->cache, what)) return rc;
+    if (a->k == nullptr || a->v == nullptr) return fail(CHRONOS_ERR_INVALID_ARG, "%s: k and v are required", what);
+    PagedAppendParams p{};
+    p.c = a->cache;
+    p.tokens = a->num_tokens;
+    p.k = a->k;
+    p.v = a->v;
+    p.k_row = a->k_row_stride;
+    p.k_head = a->k_head_stride;
+    p.v_row = a->v_row_stride;
+    p.v_head = a->v_head_stride;
+    p.cu = a->cu_seqlens;
+    p.seen = a->seen;
+    p.weights = a->weights;
+    p.positions = a->positions;
+    p.slot_cap = a->slot_cap;
+    p.max_slots = slot_limit(a->cache, a->slot_cap, arrays);
+    p.status = a->status;
+    const int es = static_cast<int>(elem_bytes(a->cache.dtype));
+    const bool wide = copies16(a->cache) && aligned(a->k, 16) && aligned(a->v, 16) &&
+                      multiples(16 / es, {a->k_row_stride, a->k_head_stride, a->v_row_stride, a->v_head_stride});
+    const int per = wide ? 16 / es : 1;
+    const int units = a->cache.head_dim / per;
+    const int64_t blocks = (a->num_tokens + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 64 * static_cast<int64_t>(sm_count()))));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (wide) CHRONOS_CUDA_CHECK(launch_kernel(paged_append_kernel<uint4>, grid, dim3(kAppendThreads), 0, st, false, p, units, per));
+    else if (es == 2) CHRONOS_CUDA_CHECK(launch_kernel(paged_append_kernel<uint16_t>, grid, dim3(kAppendThreads), 0, st, false, p, units, per));
+    else CHRONOS_CUDA_CHECK(launch_kernel(paged_append_kernel<uint32_t>, grid, dim3(kAppendThreads), 0, st, false, p, units, per));
+    return CHRONOS_OK;
+}
+
+extern "C" size_t chronos_paged_evict_workspace(const ChronosPagedEvictArgs* a) {
+    using namespace chronos;
+    g_last_error.clear();
+    if (check_evict(a)) return 0;
+    return evict_plan(a).total;
+}
+
+extern "C" int chronos_paged_evict(const ChronosPagedEvictArgs* a, void* stream) {
+    using namespace chronos;
+    g_last_error.clear();
+    const char* what = "chronos_paged_evict";
+    if (int rc = check_evict(a)) return rc;
+    if (a->cache.batch == 0) return CHRONOS_OK;
+    if (int rc = check_cache_pointers(a->cache, what)) return rc;
+    if (a->seen == nullptr || a->weights == nullptr || a->positions == nullptr || a->weights_out == nullptr ||
+        a->positions_out == nullptr || a->lens_out == nullptr || a->src == nullptr)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: seen, weights, positions, their outputs, lens_out and src are required", what);
+    const int rows = a->cache.batch * a->cache.kv_heads;
+    if (rows > 65535) return fail(CHRONOS_ERR_INVALID_ARG, "%s: batch * kv_heads %d above 65535", what, rows);
+    const EvictPlan e = evict_plan(a);
+    if (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < e.total)
+        return fail(CHRONOS_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes, %zu (256-byte aligned) needed", what,
+                    a->workspace == nullptr ? size_t{0} : a->workspace_bytes, e.total);
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    PagedEvictParams p{};
+    p.c = a->cache;
+    p.budget = a->budget;
+    p.sinks = a->sinks;
+    p.recent = a->recent;
+    p.seen = a->seen;
+    p.weights = a->weights;
+    p.positions = a->positions;
+    p.weights_out = a->weights_out;
+    p.positions_out = a->positions_out;
+    p.slot_cap = a->slot_cap;
+    p.lens_out = a->lens_out;
+    p.src = a->src;
+    p.max_slots = slot_limit(a->cache, a->slot_cap, true);
+    p.moves = reinterpret_cast<int32_t*>(ws + e.o_moves);
+    p.counts = reinterpret_cast<int32_t*>(ws + e.o_counts);
+    p.lens_copy = reinterpret_cast<int32_t*>(ws + e.o_lens);
+    p.max_moves = e.max_moves;
+    p.status = a->status;
+    constexpr int kKeyBytes = 192 * 1024;
+    const int64_t key_bytes = static_cast<int64_t>(p.max_slots) * 4;
+    p.keys_in_smem = key_bytes <= kKeyBytes;
+    const int smem = p.keys_in_smem ? static_cast<int>(key_bytes) : 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (int rc = set_smem(paged_evict_select_kernel, kKeyBytes)) return rc;
+    CHRONOS_CUDA_CHECK(launch_kernel(paged_evict_select_kernel, dim3(rows), dim3(kEvictThreads), smem, st, false, p));
+    const int es = static_cast<int>(elem_bytes(a->cache.dtype));
+    const bool wide = copies16(a->cache);
+    const int per = wide ? 16 / es : 1;
+    const int units = a->cache.head_dim / per;
+    const int64_t bx = std::max<int64_t>(1, std::min<int64_t>((e.max_moves + kEvictMovesPerBlock - 1) / kEvictMovesPerBlock, 4096));
+    const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(rows)), block(kEvictMoveThreads);
+    if (wide) CHRONOS_CUDA_CHECK(launch_kernel(paged_evict_move_kernel<uint4>, grid, block, 0, st, true, p, units, per));
+    else if (es == 2) CHRONOS_CUDA_CHECK(launch_kernel(paged_evict_move_kernel<uint16_t>, grid, block, 0, st, true, p, units, per));
+    else CHRONOS_CUDA_CHECK(launch_kernel(paged_evict_move_kernel<uint32_t>, grid, block, 0, st, true, p, units, per));
+    return CHRONOS_OK;
+}
+
+extern "C" int chronos_window_attention(const ChronosWindowAttnArgs* a, void* stream) {
+    using namespace chronos;
+    g_last_error.clear();
+    const char* what = "chronos_window_attention";
+    if (a == nullptr) return fail(CHRONOS_ERR_INVALID_ARG, "%s: args is NULL", what);
+    if (a->batch < 0 || a->kv_heads < 1 || a->heads < 1 || a->heads % a->kv_heads || a->head_dim < 1 ||
+        a->head_dim > CHRONOS_PAGED_MAX_HEAD_DIM || !dtype_known(a->dtype))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: batch %d, heads %d, kv_heads %d (divides heads), head_dim %d (1..%d), dtype %d",
+                    what, a->batch, a->heads, a->kv_heads, a->head_dim, CHRONOS_PAGED_MAX_HEAD_DIM, a->dtype);
+    if (a->window < 0 || a->sinks < 0)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: window %d, sinks %d must not be negative", what, a->window, a->sinks);
+    if (!(a->scale > 0.0f) || !std::isfinite(a->scale))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: scale %g must be positive", what, a->scale);
+    if (a->num_q < 0 || a->num_k < 0 || a->num_q > (1 << 30) || a->num_k > (1 << 30) ||
+        ((a->num_q + kWsRows - 1) / kWsRows + a->batch) * a->heads >= INT32_MAX)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: %lld query rows, %lld key rows", what, static_cast<long long>(a->num_q),
+                    static_cast<long long>(a->num_k));
+    if (a->batch == 0 || a->num_q == 0) return CHRONOS_OK;
+    if (a->q == nullptr || a->out == nullptr || a->cu_q == nullptr || a->cu_k == nullptr ||
+        (a->num_k > 0 && (a->k == nullptr || a->v == nullptr)))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: q, k, v, out, cu_q and cu_k are required", what);
+    WindowParams p{};
+    p.batch = a->batch;
+    p.heads = a->heads;
+    p.kv_heads = a->kv_heads;
+    p.rep = a->heads / a->kv_heads;
+    p.dim = a->head_dim;
+    p.window = a->window;
+    p.sinks = a->window > 0 ? a->sinks : 0;
+    p.sl2 = static_cast<float>(static_cast<double>(a->scale) * 1.4426950408889634);
+    p.num_q = a->num_q;
+    p.num_k = a->num_k;
+    p.q = a->q;
+    p.k = a->k;
+    p.v = a->v;
+    p.out = a->out;
+    p.q_row = a->q_row_stride;
+    p.q_head = a->q_head_stride;
+    p.k_row = a->k_row_stride;
+    p.k_head = a->k_head_stride;
+    p.v_row = a->v_row_stride;
+    p.v_head = a->v_head_stride;
+    p.o_row = a->out_row_stride;
+    p.o_head = a->out_head_stride;
+    p.cu_q = a->cu_q;
+    p.cu_k = a->cu_k;
+    p.lse = a->lse;
+    p.status = a->status;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (a->dtype) {
+        case CHRONOS_DTYPE_BF16: return window_impl<__nv_bfloat16>(p, st);
+        case CHRONOS_DTYPE_FP16: return window_impl<__half>(p, st);
+        default: return window_impl<float>(p, st);
+    }
+}
+
+extern "C" size_t chronos_paged_append_args_size(void) { return sizeof(ChronosPagedAppendArgs); }
+extern "C" size_t chronos_paged_decode_args_size(void) { return sizeof(ChronosPagedDecodeArgs); }
+extern "C" size_t chronos_paged_evict_args_size(void) { return sizeof(ChronosPagedEvictArgs); }
+extern "C" size_t chronos_window_attn_args_size(void) { return sizeof(ChronosWindowAttnArgs); }

@@ -1,0 +1,1197 @@
+// paged.cuh — the paged key-value cache: attention of one new token per
+// sequence over its pages, the append that fills them and the eviction that
+// empties them (include/chronos_paged.h).
+//
+// One-token attention.  With x_j = scale * log2(e) * q.k_j over the visible
+// slots, any set of slots is summarised by
+//     m = max x_j,  l = sum 2^(x_j - m),  o = sum 2^(x_j - m) v_j
+// and two such triples join as m = max(m1, m2), l = l1 2^(m1-m) + l2 2^(m2-m),
+// o likewise.  So every warp runs once over its slots with a running (m, l, o)
+// in registers, warps join through shared memory, blocks through a workspace.
+//
+// Work split.  The visible slots of every (sequence, group of query heads) are
+// cut into blocks of 64, all blocks of all sequences are numbered in one list
+// and block c of the grid takes the c-th equal share of the list, read from the
+// lengths on the device (a captured graph replays while the lengths grow).  A
+// share holds whole rows, which it finishes itself, and at most two parts of
+// rows (its first and its last), which a second kernel joins in the order of
+// the list: the result does not depend on which block ran first.
+#pragma once
+
+#include "chronos_paged.h"
+#include "common.cuh"
+
+namespace chronos {
+
+constexpr int kPdWarps = 4;
+constexpr int kPdThreads = 32 * kPdWarps;
+constexpr int kPdTile = 16;                     // slots a warp takes at a time
+constexpr int kPdBlock = kPdTile * kPdWarps;    // slots of one unit of the work list
+constexpr int kPdMaxGrid = 1024;
+constexpr int kPdMaxRep = 256;                  // query heads per kv head
+
+struct PagedDecodeParams {
+    ChronosPagedCache c;
+    int heads, rep;        // query heads, query heads per kv head
+    int rows;              // query heads a unit computes at once (16 on the tensor cores, 8 without)
+    int parts;             // ceil(rep / rows): units per kv head
+    int window, sinks;
+    int max_slots;         // lengths are cut to this
+    float sl2;             // scale * log2(e)
+    const void* q;
+    int64_t q_row, q_head;
+    void* out;
+    int64_t out_row, out_head;
+    float* lse;
+    const float* weights;
+    float* weights_out;
+    int64_t slot_cap;
+    int grid;              // blocks of the first kernel
+    int part_stride;       // floats per head of a part
+    float* part_o;         // [2 * grid][rows][part_stride]
+    float* part_ml;        // [2 * grid][rows][2]
+    float* lse2;           // [B * H] log2 of the softmax sum (rows one block finished); weights only
+    float* scores;         // [B * H][score_stride] x_j by visible index, or NULL; weights only
+    int64_t score_stride;
+    int join_blocks;       // blocks of the second kernel that join rows (the others add weights)
+    int weight_chunks;     // blocks per (sequence, kv head) that add weights
+    int32_t* status;
+};
+
+// The visible slots of sequence b: [0, first) and [lo, len).
+struct PagedRow {
+    int len, lo, first, nvis, nblk;
+};
+__device__ __forceinline__ PagedRow paged_row(const PagedDecodeParams& p, int b) {
+    PagedRow r;
+    r.len = min(max(p.c.lens[b], 0), p.max_slots);
+    r.lo = p.window > 0 ? max(0, r.len - p.window) : 0;
+    r.first = min(p.sinks, r.lo);
+    r.nvis = r.len - r.lo + r.first;
+    r.nblk = max(1, (r.nvis + kPdBlock - 1) / kPdBlock);   // an empty row still has its zeros written
+    return r;
+}
+
+// A place in the work list: unit u is block `blk` of row (b, v), v = kv head and part.
+struct PagedIter {
+    int u, b, v, blk;
+    PagedRow r;
+    __device__ __forceinline__ void advance(const PagedDecodeParams& p, int end) {
+        ++u;
+        if (++blk < r.nblk) return;
+        blk = 0;
+        if (++v < p.c.kv_heads * p.parts) return;
+        v = 0;
+        ++b;
+        if (u < end) r = paged_row(p, b);
+    }
+};
+
+// Report lengths that the table (or the running sums) cannot hold; one block does.
+__device__ __forceinline__ void paged_check_lens(const PagedDecodeParams& p) {
+    for (int b = threadIdx.x; b < p.c.batch; b += blockDim.x)
+        if (p.c.lens[b] < 0 || p.c.lens[b] > p.max_slots) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
+}
+
+// Number of units of all sequences (every lane of a warp gets it).
+__device__ __forceinline__ int paged_total(const PagedDecodeParams& p, int lane) {
+    int s = 0;
+    for (int b = lane; b < p.c.batch; b += 32) s += paged_row(p, b).nblk;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s * p.c.kv_heads * p.parts;
+}
+// Units per block of the grid.
+__device__ __forceinline__ int paged_share(const PagedDecodeParams& p, int total) {
+    return max(1, (total + p.grid - 1) / p.grid);
+}
+// First unit of sequence b / the sequence that holds unit u (whole warps call these).
+__device__ __forceinline__ int paged_first_unit(const PagedDecodeParams& p, int b, int lane) {
+    int s = 0;
+    for (int i = lane; i < b; i += 32) s += paged_row(p, i).nblk;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s * p.c.kv_heads * p.parts;
+}
+__device__ __forceinline__ PagedIter paged_seek(const PagedDecodeParams& p, int u, int lane) {
+    const int per = p.c.kv_heads * p.parts;
+    PagedIter it{};
+    it.u = u;
+    int before = 0;
+    for (int base = 0; base < p.c.batch; base += 32) {
+        const int b = base + lane;
+        const int n = b < p.c.batch ? paged_row(p, b).nblk * per : 0;
+        int inc = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += t;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, before + inc > u);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            const int start = before + __shfl_sync(0xffffffffu, inc - n, l);
+            it.b = base + l;
+            it.r = paged_row(p, it.b);
+            it.v = (u - start) / it.r.nblk;
+            it.blk = (u - start) % it.r.nblk;
+            return it;
+        }
+        before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return it;   // not reached for u < total
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLn2 = 0.6931471805599453f;
+
+// Page and slot of the 16 visible indices a warp takes next (lane i and i + 16
+// hold index i); page -1 for an index behind the row or a page that is none.
+struct PagedLook {
+    int page, slot;
+};
+__device__ __forceinline__ PagedLook paged_look(const PagedDecodeParams& p, const PagedIter& it, int end, int warp,
+                                                int lane) {
+    PagedLook k{-1, 0};
+    const int idx = it.blk * kPdBlock + warp * kPdTile + (lane & 15);
+    if (it.u < end && idx < it.r.nvis) {
+        const int pos = idx < it.r.first ? idx : it.r.lo + idx - it.r.first;
+        k.page = p.c.page_table[it.b * p.c.page_table_stride + pos / p.c.page_size];
+        k.slot = pos % p.c.page_size;
+        if (k.page < 0 || k.page >= p.c.num_pages) {
+            report_status(p.status, CHRONOS_ERR_INVALID_ARG);
+            k.page = -1;
+        }
+    }
+    return k;
+}
+
+// ---------------------------------------------------------------------------
+// tensor-core path: bf16 / fp16, up to 16 query heads of a kv head at once
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                                         uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma_16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+    if (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(addr)
+                     : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(addr)
+                     : "memory");
+}
+// Two fp32 values rounded to T, `lo` in the low half.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// 16 bytes global -> shared, zeros instead where !valid (src is not read then).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+    const int n = valid ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// DP: the head dimension rounded up to 64, 128 or 256 (columns behind it are
+// zero); HI: more than 8 query heads per unit (rows 8..15 of the products in use).
+template <int DP>
+struct PagedMma {
+    static constexpr int kStages = DP == 64 ? 6 : 3;
+    static constexpr int kTileBytes = kPdTile * DP * 2;                       // K or V of one warp's tile
+    static constexpr int kStageBytes = kPdWarps * 2 * kTileBytes;
+    static constexpr int kOStride = DP + 8;                                   // fp32; keeps the rows off one bank
+    static constexpr int kMergeBytes = (kPdWarps - 1) * 8 * kOStride * 4;
+    static constexpr int kSmem = kStages * kStageBytes + kMergeBytes + kPdWarps * 16 * 2 * 4 + kStages * kPdWarps * 4;
+    static constexpr int kBlocksPerSm = DP == 256 ? 1 : 2;
+};
+
+// HBM bound: 2 * D * 2 bytes per visible slot and kv head against 4 * D flops per
+// query head.  The tensor cores take a slot's K row for all query heads of the
+// group at once (rows of the 16-row operand; unused rows are zero).  A warp owns
+// 16 slots at a time and its own ring of asynchronous copies (K and V rows go to
+// shared memory 16 bytes at a time, rows of 8 chunks swizzled against bank
+// conflicts), so warps never wait for each other inside a row.
+template <typename T, int DP, bool HI>
+__global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_decode_mma_kernel(
+    const __grid_constant__ PagedDecodeParams p) {
+    using S = PagedMma<DP>;
+    constexpr int NS = S::kStages;
+    constexpr int CPR = DP / 8;            // 16-byte chunks per row
+    constexpr int RPI = 32 / CPR;          // rows a warp copies per instruction
+    extern __shared__ __align__(128) uint8_t smem[];
+    float* s_o = reinterpret_cast<float*>(smem + NS * S::kStageBytes);
+    float* s_ml = s_o + S::kMergeBytes / 4;                                    // [warp][16][2]
+    uint32_t* s_vis = reinterpret_cast<uint32_t*>(s_ml + kPdWarps * 32);       // [stage][warp]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int quad = lane >> 2, qc = lane & 3;   // this lane's rows quad, quad + 8 and column pair of a product
+
+    const int total = paged_total(p, lane);
+    const int share = paged_share(p, total);
+    const int begin = static_cast<int>(blockIdx.x) * share, end = min(total, begin + share);
+    if (blockIdx.x == 0) paged_check_lens(p);
+    if (begin >= end) return;
+    PagedIter ld = paged_seek(p, begin, lane);
+    PagedIter cp = ld;
+    PagedLook look = paged_look(p, ld, end, warp, lane);
+
+    const T* kbase = static_cast<const T*>(p.c.k_pages);
+    const T* vbase = static_cast<const T*>(p.c.v_pages);
+    auto issue = [&](int stage) {
+        const uint32_t sk = smem_u32(smem + stage * S::kStageBytes + warp * 2 * S::kTileBytes);
+        const int64_t g = ld.v / p.parts;
+        const int ch = lane % CPR;
+        const bool col = ch * 8 < p.c.head_dim;
+#pragma unroll
+        for (int i = 0; i < kPdTile / RPI; ++i) {
+            const int r = i * RPI + lane / CPR;
+            const int page = __shfl_sync(0xffffffffu, look.page, r);
+            const int64_t slot = __shfl_sync(0xffffffffu, look.slot, r);
+            const bool ok = col && page >= 0;
+            const T* ks = kbase + (ok ? page * p.c.k_page_stride + slot * p.c.k_slot_stride + g * p.c.k_head_stride + ch * 8 : 0);
+            const T* vs = vbase + (ok ? page * p.c.v_page_stride + slot * p.c.v_slot_stride + g * p.c.v_head_stride + ch * 8 : 0);
+            const uint32_t off = static_cast<uint32_t>(r * DP * 2 + ((ch ^ (r & 7)) << 4));
+            cp_async16(sk + off, ks, ok);
+            cp_async16(sk + S::kTileBytes + off, vs, ok);
+        }
+        const uint32_t vis = __ballot_sync(0xffffffffu, look.page >= 0) & 0xffffu;
+        if (lane == 0) s_vis[stage * kPdWarps + warp] = vis;
+    };
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s) {
+        if (ld.u < end) {
+            issue(s);
+            ld.advance(p, end);
+            look = paged_look(p, ld, end, warp, lane);
+        }
+        cp_async_commit();
+    }
+
+    uint32_t qa[DP / 16][4];
+    float o[DP / 8][4];
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+    bool fresh = true;          // the next unit opens a new part or row
+    int part_blk = 0;           // the block it opened with
+    int stage = 0;
+    while (cp.u < end) {
+        if (ld.u < end) {
+            issue(stage == 0 ? NS - 1 : stage - 1);
+            ld.advance(p, end);
+            look = paged_look(p, ld, end, warp, lane);
+        }
+        cp_async_commit();
+        const int kvh = cp.v / p.parts, h0 = (cp.v % p.parts) * 16;
+        const int nh = min(16, p.rep - h0);             // query heads of this unit
+        if (fresh) {
+            fresh = false;
+            part_blk = cp.blk;
+            m0 = m1 = -INFINITY;
+            l0 = l1 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+            const T* q = static_cast<const T*>(p.q) + cp.b * p.q_row + static_cast<int64_t>(kvh * p.rep + h0) * p.q_head;
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int row = quad + (j & 1) * 8, d = kk * 16 + qc * 2 + (j >> 1) * 8;
+                    qa[kk][j] = (HI || !(j & 1)) && row < nh && d < p.c.head_dim
+                                    ? *reinterpret_cast<const uint32_t*>(q + row * p.q_head + d) : 0u;
+                }
+        }
+        cp_async_wait<NS - 1>();
+        __syncwarp();
+        const uint32_t sk = smem_u32(smem + stage * S::kStageBytes + warp * 2 * S::kTileBytes);
+        const uint32_t sv = sk + S::kTileBytes;
+        const uint32_t vis = s_vis[stage * kPdWarps + warp];
+        if (vis || p.scores != nullptr) {   // with running sums, hidden slots' scores are written too
+            float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+            {
+                const int r = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk) {
+                    uint32_t kb[4];
+                    ldmatrix_x4<false>(kb, sk + r * DP * 2 + (((kk * 2 + half) ^ (r & 7)) << 4));
+                    mma_16816<T>(s[0], qa[kk], kb[0], kb[1]);
+                    mma_16816<T>(s[1], qa[kk], kb[2], kb[3]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool on = (vis >> (t * 8 + qc * 2 + (j & 1))) & 1u;
+                    s[t][j] = on ? s[t][j] * p.sl2 : -INFINITY;
+                }
+            if (p.scores != nullptr) {
+                const int idx = cp.blk * kPdBlock + warp * kPdTile + qc * 2;
+                float* sc = p.scores + (static_cast<int64_t>(cp.b) * p.heads + kvh * p.rep + h0) * p.score_stride + idx;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (quad < nh)
+                        *reinterpret_cast<float2*>(sc + quad * p.score_stride + t * 8) = make_float2(s[t][0], s[t][1]);
+                    if (HI && quad + 8 < nh)
+                        *reinterpret_cast<float2*>(sc + (quad + 8) * p.score_stride + t * 8) =
+                            make_float2(s[t][2], s[t][3]);
+                }
+            }
+            float n0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+            float n1 = HI ? fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])) : -INFINITY;
+#pragma unroll
+            for (int x = 1; x < 4; x <<= 1) {
+                n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
+                if (HI) n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
+            }
+            if (__any_sync(0xffffffffu, n0 > m0 || (HI && n1 > m1))) {
+                n0 = fmaxf(n0, m0);
+                const float c0 = n0 == -INFINITY ? 1.0f : exp2_fast(m0 - n0);
+                m0 = n0;
+                l0 *= c0;
+                float c1 = 1.0f;
+                if (HI) {
+                    n1 = fmaxf(n1, m1);
+                    c1 = n1 == -INFINITY ? 1.0f : exp2_fast(m1 - n1);
+                    m1 = n1;
+                    l1 *= c1;
+                }
+#pragma unroll
+                for (int i = 0; i < DP / 8; ++i) {
+                    o[i][0] *= c0;
+                    o[i][1] *= c0;
+                    if (HI) {
+                        o[i][2] *= c1;
+                        o[i][3] *= c1;
+                    }
+                }
+            }
+            const float u0 = m0 == -INFINITY ? 0.0f : m0, u1 = m1 == -INFINITY ? 0.0f : m1;
+            uint32_t pa[4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const float a = exp2_fast(s[t][0] - u0), b = exp2_fast(s[t][1] - u0);
+                l0 += a + b;
+                pa[2 * t] = pack2<T>(a, b);   // weights in T for the second product; the sum keeps fp32
+                if (HI) {
+                    const float c = exp2_fast(s[t][2] - u1), d = exp2_fast(s[t][3] - u1);
+                    l1 += c + d;
+                    pa[2 * t + 1] = pack2<T>(c, d);
+                } else {
+                    pa[2 * t + 1] = 0u;
+                }
+            }
+            {
+                const int r = lane & 15, half = lane >> 4;
+#pragma unroll
+                for (int dd = 0; dd < DP / 16; ++dd) {
+                    uint32_t vb[4];
+                    ldmatrix_x4<true>(vb, sv + r * DP * 2 + (((dd * 2 + half) ^ (r & 7)) << 4));
+                    mma_16816<T>(o[2 * dd], pa, vb[0], vb[1]);
+                    mma_16816<T>(o[2 * dd + 1], pa, vb[2], vb[3]);
+                }
+            }
+        }
+        __syncwarp();   // every lane has read the tile before its stage is filled again
+        stage = stage == NS - 1 ? 0 : stage + 1;
+
+        if (cp.blk + 1 == cp.r.nblk || cp.u + 1 == end) {
+            // the row (or this block's part of it) is complete: join the four warps
+            fresh = true;
+            const bool whole = part_blk == 0 && cp.blk + 1 == cp.r.nblk;
+#pragma unroll
+            for (int x = 1; x < 4; x <<= 1) {
+                l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+                l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+            }
+            if (qc == 0) {
+                *reinterpret_cast<float2*>(s_ml + (warp * 16 + quad) * 2) = make_float2(m0, l0);
+                if (HI) *reinterpret_cast<float2*>(s_ml + (warp * 16 + quad + 8) * 2) = make_float2(m1, l1);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int hi = 0; hi < (HI ? 2 : 1); ++hi) {
+                if (hi) __syncthreads();
+                const int row = quad + 8 * hi;
+                float M = -INFINITY, L = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kPdWarps; ++w) M = fmaxf(M, s_ml[(w * 16 + row) * 2]);
+                const float u = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+                for (int w = 0; w < kPdWarps; ++w)
+                    L += s_ml[(w * 16 + row) * 2 + 1] * exp2_fast(s_ml[(w * 16 + row) * 2] - u);
+                const float c = exp2_fast((hi ? m1 : m0) - u);
+                if (warp > 0) {
+                    float* dst = s_o + ((warp - 1) * 8 + quad) * S::kOStride + qc * 2;
+#pragma unroll
+                    for (int i = 0; i < DP / 8; ++i)
+                        *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * hi] * c, o[i][2 * hi + 1] * c);
+                }
+                __syncthreads();
+                if (warp == 0 && row < nh) {
+                    const float* src = s_o + quad * S::kOStride + qc * 2;
+                    const float inv = whole ? (L > 0.0f ? 1.0f / L : L) : 1.0f;
+                    const int64_t part = (2 * static_cast<int64_t>(blockIdx.x) + (part_blk == 0 ? 1 : 0)) * 16 + row;
+                    const int head = kvh * p.rep + h0 + row;
+                    T* out = static_cast<T*>(p.out) + cp.b * p.out_row + head * p.out_head;
+                    float* po = p.part_o + part * p.part_stride;
+#pragma unroll
+                    for (int i = 0; i < DP / 8; ++i) {
+                        float a = o[i][2 * hi] * c, b = o[i][2 * hi + 1] * c;
+#pragma unroll
+                        for (int w = 0; w < kPdWarps - 1; ++w) {
+                            const float2 t = *reinterpret_cast<const float2*>(src + w * 8 * S::kOStride + i * 8);
+                            a += t.x;
+                            b += t.y;
+                        }
+                        const int d = i * 8 + qc * 2;
+                        if (!whole)
+                            *reinterpret_cast<float2*>(po + d) = make_float2(a, b);
+                        else if (d < p.c.head_dim)
+                            *reinterpret_cast<uint32_t*>(out + d) = pack2<T>(a * inv, b * inv);
+                    }
+                    if (qc == 0) {
+                        if (!whole) {
+                            *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(M, L);
+                        } else {
+                            const float lg = L != 0.0f ? u + log2f(L) : -INFINITY;
+                            if (p.lse != nullptr) p.lse[static_cast<int64_t>(cp.b) * p.heads + head] = lg * kLn2;
+                            if (p.scores != nullptr) p.lse2[static_cast<int64_t>(cp.b) * p.heads + head] = lg;
+                        }
+                    }
+                }
+            }
+        }
+        cp.advance(p, end);
+    }
+    cp_async_wait<0>();
+}
+
+// ---------------------------------------------------------------------------
+// general path: fp32 (no tensor-core product keeps its precision), head
+// dimensions or strides the copies above cannot take.  Same work list; 8 query
+// heads at once, fp32 products.  K: four lanes share a slot (their partial dot
+// products meet in two shuffles), two slots per lane in flight; V: the lanes
+// split the columns and run over the warp's 16 slots.
+// ---------------------------------------------------------------------------
+constexpr int kPdSimtRows = 8;
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load4(const T* p, int d, int dim, float (&v)[4]) {
+    if (VEC) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(p + d);
+            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+        } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(p + d);
+            const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = to_f32<T>(t[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = d + i < dim ? to_f32<T>(p[d + i]) : 0.0f;
+    }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kPdThreads) paged_decode_simt_kernel(const __grid_constant__ PagedDecodeParams p) {
+    constexpr int R = kPdSimtRows, MAXD = CHRONOS_PAGED_MAX_HEAD_DIM;
+    __shared__ __align__(16) float s_q[R][MAXD];
+    __shared__ __align__(16) float s_o[kPdWarps - 1][R][MAXD];
+    __shared__ __align__(16) float s_p[kPdWarps][kPdTile][R];
+    __shared__ float s_c[kPdWarps][R];
+    __shared__ float s_ml[kPdWarps][R][2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int D = p.c.head_dim, D4 = (D + 3) / 4;
+    const int slot_lane = lane >> 2, part = lane & 3;
+
+    const int total = paged_total(p, lane);
+    const int share = paged_share(p, total);
+    const int begin = static_cast<int>(blockIdx.x) * share, end = min(total, begin + share);
+    if (blockIdx.x == 0) paged_check_lens(p);
+    if (begin >= end) return;
+    PagedIter cp = paged_seek(p, begin, lane);
+    PagedLook look = paged_look(p, cp, end, warp, lane);
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};   // heads 2 * part, 2 * part + 1
+    float o[R][8];
+    bool fresh = true;
+    int part_blk = 0;
+    while (cp.u < end) {
+        const int kvh = cp.v / p.parts, h0 = (cp.v % p.parts) * R;
+        const int nh = min(R, p.rep - h0);
+        if (fresh) {
+            fresh = false;
+            part_blk = cp.blk;
+            m[0] = m[1] = -INFINITY;
+            l[0] = l[1] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < R; ++h)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[h][i] = 0.0f;
+            __syncthreads();
+            const T* q = static_cast<const T*>(p.q) + cp.b * p.q_row + static_cast<int64_t>(kvh * p.rep + h0) * p.q_head;
+            for (int i = threadIdx.x; i < R * MAXD; i += kPdThreads) {
+                const int h = i / MAXD, d = i % MAXD;
+                s_q[h][d] = h < nh && d < D ? to_f32<T>(q[h * p.q_head + d]) : 0.0f;
+            }
+            __syncthreads();
+        }
+        PagedIter nx = cp;
+        nx.advance(p, end);
+        const PagedLook cur = look;
+        look = paged_look(p, nx, end, warp, lane);
+        const uint32_t vis = __ballot_sync(0xffffffffu, cur.page >= 0) & 0xffffu;
+        if (vis || p.scores != nullptr) {
+            // scores of slots slot_lane and slot_lane + 8
+            const int pg0 = __shfl_sync(0xffffffffu, cur.page, slot_lane), pg1 = __shfl_sync(0xffffffffu, cur.page, slot_lane + 8);
+            const int64_t sl0 = __shfl_sync(0xffffffffu, cur.slot, slot_lane), sl1 = __shfl_sync(0xffffffffu, cur.slot, slot_lane + 8);
+            const T* kb = static_cast<const T*>(p.c.k_pages) + kvh * p.c.k_head_stride;
+            const T* k0 = kb + (pg0 >= 0 ? pg0 * p.c.k_page_stride + sl0 * p.c.k_slot_stride : 0);
+            const T* k1 = kb + (pg1 >= 0 ? pg1 * p.c.k_page_stride + sl1 * p.c.k_slot_stride : 0);
+            float s0[R], s1[R];
+#pragma unroll
+            for (int h = 0; h < R; ++h) s0[h] = s1[h] = 0.0f;
+#pragma unroll 4
+            for (int c = part; c < D4; c += 4) {
+                float a[4] = {0.0f, 0.0f, 0.0f, 0.0f}, b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (pg0 >= 0) load4<T, VEC>(k0, c * 4, D, a);
+                if (pg1 >= 0) load4<T, VEC>(k1, c * 4, D, b);
+#pragma unroll
+                for (int h = 0; h < R; ++h) {
+                    const float4 qv = *reinterpret_cast<const float4*>(&s_q[h][c * 4]);
+                    s0[h] = fmaf(a[0], qv.x, fmaf(a[1], qv.y, fmaf(a[2], qv.z, fmaf(a[3], qv.w, s0[h]))));
+                    s1[h] = fmaf(b[0], qv.x, fmaf(b[1], qv.y, fmaf(b[2], qv.z, fmaf(b[3], qv.w, s1[h]))));
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < R; ++h) {
+#pragma unroll
+                for (int x = 1; x < 4; x <<= 1) {
+                    s0[h] += __shfl_xor_sync(0xffffffffu, s0[h], x);
+                    s1[h] += __shfl_xor_sync(0xffffffffu, s1[h], x);
+                }
+            }
+            // lane `part` of a slot's four keeps heads 2 * part and 2 * part + 1
+            float x[2][2];
+#pragma unroll
+            for (int h = 0; h < R; ++h)
+                if ((h >> 1) == part) {
+                    x[h & 1][0] = pg0 >= 0 ? s0[h] * p.sl2 : -INFINITY;
+                    x[h & 1][1] = pg1 >= 0 ? s1[h] * p.sl2 : -INFINITY;
+                }
+            const int idx = cp.blk * kPdBlock + warp * kPdTile + slot_lane;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int h = 2 * part + j;
+                if (p.scores != nullptr && h < nh) {
+                    float* sc = p.scores + (static_cast<int64_t>(cp.b) * p.heads + kvh * p.rep + h0 + h) * p.score_stride + idx;
+                    sc[0] = x[j][0];
+                    sc[8] = x[j][1];
+                }
+                float n = fmaxf(x[j][0], x[j][1]);
+#pragma unroll
+                for (int t = 4; t < 32; t <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, t));
+                n = fmaxf(n, m[j]);
+                const float u = n == -INFINITY ? 0.0f : n;
+                const float c = exp2_fast(m[j] - u);
+                m[j] = n;
+                const float a = exp2_fast(x[j][0] - u), b = exp2_fast(x[j][1] - u);
+                l[j] = l[j] * c + a + b;
+                s_p[warp][slot_lane][h] = a;
+                s_p[warp][slot_lane + 8][h] = b;
+                if (slot_lane == 0) s_c[warp][h] = c;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < R; ++h) {
+                const float c = s_c[warp][h];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[h][i] *= c;
+            }
+            const T* vb = static_cast<const T*>(p.c.v_pages) + kvh * p.c.v_head_stride;
+#pragma unroll 8
+            for (int t = 0; t < kPdTile; ++t) {
+                const int page = __shfl_sync(0xffffffffu, cur.page, t);
+                const int64_t slot = __shfl_sync(0xffffffffu, cur.slot, t);
+                if (page < 0) continue;
+                const T* v = vb + page * p.c.v_page_stride + slot * p.c.v_slot_stride;
+                const float4 pa = *reinterpret_cast<const float4*>(&s_p[warp][t][0]);
+                const float4 pb = *reinterpret_cast<const float4*>(&s_p[warp][t][4]);
+                const float ph[R] = {pa.x, pa.y, pa.z, pa.w, pb.x, pb.y, pb.z, pb.w};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int d = lane * 4 + 128 * i;
+                    if (d < D) {
+                        float a[4];
+                        load4<T, VEC>(v, d, D, a);
+#pragma unroll
+                        for (int h = 0; h < R; ++h)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[h][i * 4 + e] = fmaf(ph[h], a[e], o[h][i * 4 + e]);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+        if (cp.blk + 1 == cp.r.nblk || cp.u + 1 == end) {
+            fresh = true;
+            const bool whole = part_blk == 0 && cp.blk + 1 == cp.r.nblk;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int t = 4; t < 32; t <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], t);
+                if (slot_lane == 0) {
+                    s_ml[warp][2 * part + j][0] = m[j];
+                    s_ml[warp][2 * part + j][1] = l[j];
+                }
+            }
+            __syncthreads();
+            float M[R], L[R];
+#pragma unroll
+            for (int h = 0; h < R; ++h) {
+                M[h] = -INFINITY;
+                L[h] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kPdWarps; ++w) M[h] = fmaxf(M[h], s_ml[w][h][0]);
+                const float u = M[h] == -INFINITY ? 0.0f : M[h];
+#pragma unroll
+                for (int w = 0; w < kPdWarps; ++w) L[h] += s_ml[w][h][1] * exp2_fast(s_ml[w][h][0] - u);
+                const float c = exp2_fast(s_ml[warp][h][0] - u);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[h][i] *= c;
+            }
+            if (warp > 0)
+#pragma unroll
+                for (int h = 0; h < R; ++h)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        *reinterpret_cast<float4*>(&s_o[warp - 1][h][lane * 4 + 128 * i]) =
+                            make_float4(o[h][4 * i], o[h][4 * i + 1], o[h][4 * i + 2], o[h][4 * i + 3]);
+            __syncthreads();
+            if (warp == 0) {
+#pragma unroll
+                for (int h = 0; h < R; ++h) {
+                    if (h >= nh) break;
+                    const float inv = whole ? (L[h] > 0.0f ? 1.0f / L[h] : L[h]) : 1.0f;
+                    const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (part_blk == 0 ? 1 : 0)) * R + h;
+                    const int head = kvh * p.rep + h0 + h;
+                    T* out = static_cast<T*>(p.out) + cp.b * p.out_row + head * p.out_head;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int d = lane * 4 + 128 * (i >> 2) + (i & 3);
+                        if (d < D) {
+                            float a = o[h][i];
+#pragma unroll
+                            for (int w = 0; w < kPdWarps - 1; ++w) a += s_o[w][h][d];
+                            if (whole) out[d] = from_f32<T>(a * inv);
+                            else p.part_o[slot * p.part_stride + d] = a;
+                        }
+                    }
+                    if (lane == 0) {
+                        if (!whole) {
+                            p.part_ml[slot * 2] = M[h];
+                            p.part_ml[slot * 2 + 1] = L[h];
+                        } else {
+                            const float lg = L[h] != 0.0f ? (M[h] == -INFINITY ? 0.0f : M[h]) + log2f(L[h]) : -INFINITY;
+                            if (p.lse != nullptr) p.lse[static_cast<int64_t>(cp.b) * p.heads + head] = lg * kLn2;
+                            if (p.scores != nullptr) p.lse2[static_cast<int64_t>(cp.b) * p.heads + head] = lg;
+                        }
+                    }
+                }
+            }
+        }
+        cp = nx;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// join of the parts, and the running sums of the attention weights
+// ---------------------------------------------------------------------------
+constexpr int kPdJoinThreads = 256;
+constexpr int kPdWeightSlots = 4 * kPdJoinThreads;   // slots per block that adds weights
+
+// The parts of row (b, v): blocks c0..c1 of the grid; part(c) its place in the workspace.
+struct PagedParts {
+    int c0, c1;
+    __device__ __forceinline__ int64_t part(int c) const { return 2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0); }
+};
+__device__ __forceinline__ PagedParts paged_parts(const PagedDecodeParams& p, int b, int v, int lane) {
+    const int share = paged_share(p, paged_total(p, lane));
+    const int nblk = paged_row(p, b).nblk;
+    const int s = paged_first_unit(p, b, lane) + v * nblk;
+    return PagedParts{s / share, (s + nblk - 1) / share};
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPdJoinThreads) paged_join_kernel(const __grid_constant__ PagedDecodeParams p) {
+    constexpr int W = kPdJoinThreads / 32;
+    __shared__ float s_w[kPdMaxGrid];
+    __shared__ float s_red[W];
+    __shared__ float s_o[W][CHRONOS_PAGED_MAX_HEAD_DIM];
+    __shared__ float s_lse[kPdMaxRep];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    if (static_cast<int>(blockIdx.x) < p.join_blocks) {
+        const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
+        const int kvh = head / p.rep, hr = head % p.rep;
+        const PagedParts pp = paged_parts(p, b, kvh * p.parts + hr / p.rows, lane);
+        if (pp.c0 == pp.c1) return;   // one block finished the row
+        const int n = pp.c1 - pp.c0 + 1, row = hr % p.rows;
+        float M = -INFINITY;
+        for (int i = threadIdx.x; i < n; i += kPdJoinThreads)
+            M = fmaxf(M, p.part_ml[(pp.part(pp.c0 + i) * p.rows + row) * 2]);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+        if (lane == 0) s_red[warp] = M;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) M = fmaxf(M, s_red[w]);
+        const float u = M == -INFINITY ? 0.0f : M;
+        float L = 0.0f;
+        for (int i = threadIdx.x; i < n; i += kPdJoinThreads) {
+            const float* ml = p.part_ml + (pp.part(pp.c0 + i) * p.rows + row) * 2;
+            const float c = exp2_fast(ml[0] - u);
+            s_w[i] = c;
+            L += ml[1] * c;
+        }
+        L = warp_sum(L);
+        __syncthreads();
+        if (lane == 0) s_red[warp] = L;
+        __syncthreads();
+        L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) L += s_red[w];
+        // warps take every W-th part, lanes 4 columns (twice for more than 128)
+        float acc[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+        const int D = p.c.head_dim;
+#pragma unroll 4
+        for (int i = warp; i < n; i += W) {
+            const float* po = p.part_o + (pp.part(pp.c0 + i) * p.rows + row) * p.part_stride;
+            const float c = s_w[i];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int d = lane * 4 + 128 * j;
+                if (d < D) {
+                    const float4 f = *reinterpret_cast<const float4*>(po + d);
+                    acc[4 * j] = fmaf(c, f.x, acc[4 * j]);
+                    acc[4 * j + 1] = fmaf(c, f.y, acc[4 * j + 1]);
+                    acc[4 * j + 2] = fmaf(c, f.z, acc[4 * j + 2]);
+                    acc[4 * j + 3] = fmaf(c, f.w, acc[4 * j + 3]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s_o[warp][lane * 4 + 128 * (i >> 2) + (i & 3)] = acc[i];
+        __syncthreads();
+        const float inv = L > 0.0f ? 1.0f / L : L;   // 0 where nothing was visible; NaN stays
+        T* out = static_cast<T*>(p.out) + b * p.out_row + head * p.out_head;
+        for (int d = threadIdx.x; d < D; d += kPdJoinThreads) {
+            float a = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) a += s_o[w][d];
+            out[d] = from_f32<T>(a * inv);
+        }
+        if (threadIdx.x == 0 && p.lse != nullptr)
+            p.lse[static_cast<int64_t>(b) * p.heads + head] = L != 0.0f ? (u + log2f(L)) * kLn2 : -INFINITY;
+        return;
+    }
+    // weights_out[b, g, j] = weights[b, g, j] + sum_h 2^(x_hj - lse2_h)
+    int i = static_cast<int>(blockIdx.x) - p.join_blocks;
+    const int chunk = i % p.weight_chunks;
+    i /= p.weight_chunks;
+    const int g = i % p.c.kv_heads, b = i / p.c.kv_heads;
+    const PagedRow r = paged_row(p, b);
+    if (chunk * kPdWeightSlots >= r.len) return;
+    const int64_t hb = static_cast<int64_t>(b) * p.heads + g * p.rep;
+    for (int h = warp; h < p.rep; h += W) {
+        const PagedParts pp = paged_parts(p, b, g * p.parts + h / p.rows, lane);
+        float lg;
+        if (pp.c0 == pp.c1) {
+            lg = p.lse2[hb + h];
+        } else {
+            const int row = h % p.rows;
+            float M = -INFINITY;
+            for (int c = pp.c0 + lane; c <= pp.c1; c += 32) M = fmaxf(M, p.part_ml[(pp.part(c) * p.rows + row) * 2]);
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+            const float u = M == -INFINITY ? 0.0f : M;
+            float L = 0.0f;
+            for (int c = pp.c0 + lane; c <= pp.c1; c += 32) {
+                const float* ml = p.part_ml + (pp.part(c) * p.rows + row) * 2;
+                L += ml[1] * exp2_fast(ml[0] - u);
+            }
+            L = warp_sum(L);
+            lg = L != 0.0f ? u + log2f(L) : INFINITY;   // nothing readable: weights of zero
+        }
+        if (lane == 0) s_lse[h] = lg == -INFINITY ? INFINITY : lg;
+    }
+    __syncthreads();
+    const int64_t wb = (static_cast<int64_t>(b) * p.c.kv_heads + g) * p.slot_cap;
+    const int j0 = chunk * kPdWeightSlots + threadIdx.x * 4;
+    const float* sc = p.scores + hb * p.score_stride;
+    const bool vec = r.first == r.lo && j0 + 4 <= r.len && (p.slot_cap & 3) == 0 &&
+                     ((reinterpret_cast<uintptr_t>(p.weights) | reinterpret_cast<uintptr_t>(p.weights_out)) & 15) == 0;
+    if (vec) {   // every slot visible: index = slot
+        float4 w = *reinterpret_cast<const float4*>(p.weights + wb + j0);
+        for (int h = 0; h < p.rep; ++h) {
+            const float4 x = *reinterpret_cast<const float4*>(sc + h * p.score_stride + j0);
+            const float lg = s_lse[h];
+            w.x += exp2_fast(x.x - lg);
+            w.y += exp2_fast(x.y - lg);
+            w.z += exp2_fast(x.z - lg);
+            w.w += exp2_fast(x.w - lg);
+        }
+        *reinterpret_cast<float4*>(p.weights_out + wb + j0) = w;
+    } else {
+        for (int j = j0; j < min(j0 + 4, r.len); ++j) {
+            float w = p.weights[wb + j];
+            const int idx = j < r.first ? j : j >= r.lo ? r.first + j - r.lo : -1;
+            if (idx >= 0)
+                for (int h = 0; h < p.rep; ++h) w += exp2_fast(sc[h * p.score_stride + idx] - s_lse[h]);
+            p.weights_out[wb + j] = w;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+struct PagedAppendParams {
+    ChronosPagedCache c;
+    int64_t tokens;
+    const void* k;
+    const void* v;
+    int64_t k_row, k_head, v_row, v_head;
+    const int32_t* cu;
+    const int32_t* seen;
+    float* weights;
+    int32_t* positions;
+    int64_t slot_cap;
+    int max_slots;
+    int32_t* status;
+};
+
+constexpr int kAppendThreads = 256;
+
+// Copies: 4 * G * D * size bytes of traffic per token.  One warp per token: it
+// finds the sequence with one ballot per 32 offsets, then its lanes copy the
+// token's K and V rows in units of V bytes (16, or one element where the
+// strides forbid more), four loads in flight before the first store.
+template <typename V>
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ PagedAppendParams p,
+                                                                      int units_per_head, int elems_per_unit) {
+    const int lane = threadIdx.x & 31;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * (kAppendThreads / 32);
+    const int G = p.c.kv_heads, n = G * units_per_head;
+    for (int64_t t = static_cast<int64_t>(blockIdx.x) * (kAppendThreads / 32) + (threadIdx.x >> 5); t < p.tokens; t += warps) {
+        int b = 0;
+        int64_t i = 0;
+        if (p.cu == nullptr) {
+            b = static_cast<int>(t);
+        } else {
+            // sequences whose end is <= t come before token t's (ends ascend)
+            for (int base = 0; base < p.c.batch; base += 32) {
+                const bool before = base + lane < p.c.batch && p.cu[base + lane + 1] <= t;
+                const int cnt = __popc(__ballot_sync(0xffffffffu, before));
+                b += cnt;
+                if (cnt < 32) break;
+            }
+            if (b >= p.c.batch) continue;   // a row behind the last sequence
+            i = t - p.cu[b];
+            if (i < 0) continue;
+        }
+        const int64_t slot = p.c.lens[b] + i;
+        const bool fits = slot >= 0 && slot < p.max_slots;
+        const int page = fits ? p.c.page_table[b * p.c.page_table_stride + slot / p.c.page_size] : -1;
+        if (page < 0 || page >= p.c.num_pages) {
+            if (lane == 0) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
+            continue;
+        }
+        const int64_t in_page = slot % p.c.page_size;
+        const char* ks = static_cast<const char*>(p.k);
+        const char* vs = static_cast<const char*>(p.v);
+        char* kd = static_cast<char*>(p.c.k_pages);
+        char* vd = static_cast<char*>(p.c.v_pages);
+        const int es = static_cast<int>(sizeof(V)) / elems_per_unit;
+        for (int u0 = lane; u0 < n; u0 += 64) {
+            V x[4];
+            int64_t dk[2], dv[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int u = u0 + 32 * j;
+                if (u < n) {
+                    const int64_t g = u / units_per_head, e = static_cast<int64_t>(u % units_per_head) * elems_per_unit;
+                    x[2 * j] = *reinterpret_cast<const V*>(ks + (t * p.k_row + g * p.k_head + e) * es);
+                    x[2 * j + 1] = *reinterpret_cast<const V*>(vs + (t * p.v_row + g * p.v_head + e) * es);
+                    dk[j] = (page * p.c.k_page_stride + in_page * p.c.k_slot_stride + g * p.c.k_head_stride + e) * es;
+                    dv[j] = (page * p.c.v_page_stride + in_page * p.c.v_slot_stride + g * p.c.v_head_stride + e) * es;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (u0 + 32 * j < n) {
+                    *reinterpret_cast<V*>(kd + dk[j]) = x[2 * j];
+                    *reinterpret_cast<V*>(vd + dv[j]) = x[2 * j + 1];
+                }
+        }
+        for (int g = lane; g < G; g += 32) {
+            const int64_t at = (static_cast<int64_t>(b) * G + g) * p.slot_cap + slot;
+            if (p.weights != nullptr) p.weights[at] = 0.0f;
+            if (p.positions != nullptr) p.positions[at] = static_cast<int32_t>(p.seen[b] + i);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// eviction
+// ---------------------------------------------------------------------------
+struct PagedEvictParams {
+    ChronosPagedCache c;
+    int budget, sinks, recent;
+    const int32_t* seen;
+    const float* weights;
+    const int32_t* positions;
+    float* weights_out;
+    int32_t* positions_out;
+    int64_t slot_cap;
+    int32_t* lens_out;
+    int32_t* src;
+    int max_slots;
+    int keys_in_smem;      // 1: a row's keys fit shared memory, else they are formed again from the inputs
+    int32_t* moves;        // [B * G][max_moves][2]: (slot given up, slot that moves there)
+    int32_t* counts;       // [B * G]
+    int32_t* lens_copy;    // [B] lens_out may be the caller's lens
+    int64_t max_moves;
+    int32_t* status;
+};
+
+constexpr int kEvictThreads = 1024;
+constexpr int kEvictWarps = kEvictThreads / 32;
+constexpr int kEvictBins = 2048;   // 11 + 11 + 10 bits of the key
+
+// A weight's place in the order of floats as an unsigned number: larger weights
+// first, -0 as 0, NaN above every number; what is kept anyway above all.
+__device__ __forceinline__ uint32_t evict_key(float w, int pos, int sinks, int64_t newest) {
+    if (pos < sinks || pos >= newest) return 0xffffffffu;
+    if (w != w) return 0xfffffffeu;
+    const uint32_t u = __float_as_uint(w + 0.0f);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+// One block per (sequence, kv head).  The budget-th largest key by radix
+// selection (three counting passes over 11, 11 and 10 bits, counters in shared
+// memory), then ordered passes over the slots: every warp owns a contiguous
+// piece, counts in it, and a scan over the warps gives each its first rank.
+__global__ void __launch_bounds__(kEvictThreads) paged_evict_select_kernel(const __grid_constant__ PagedEvictParams p) {
+    extern __shared__ uint32_t s_keys[];   // [max_slots] when keys_in_smem
+    __shared__ int s_hist[kEvictBins];
+    __shared__ int s_a[kEvictWarps], s_b[kEvictWarps];
+    __shared__ int s_digit, s_above;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row = blockIdx.x, b = row / p.c.kv_heads;
+    const int raw = p.c.lens[b];
+    const int n = min(max(raw, 0), p.max_slots);
+    if (threadIdx.x == 0 && raw != n) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
+    const int64_t base = row * p.slot_cap;
+    const float* w = p.weights + base;
+    const int32_t* pos = p.positions + base;
+    int32_t* src = p.src + static_cast<int64_t>(row) * p.budget;
+    if (row % p.c.kv_heads == 0 && threadIdx.x == 0) p.lens_copy[b] = n;
+    if (n <= p.budget) {
+        for (int j = threadIdx.x; j < p.budget; j += kEvictThreads) src[j] = j < n ? j : -1;
+        for (int j = threadIdx.x; j < n; j += kEvictThreads) {
+            const float a = w[j];
+            const int c = pos[j];
+            p.weights_out[base + j] = a;
+            p.positions_out[base + j] = c;
+        }
+        if (threadIdx.x == 0) p.counts[row] = 0;
+        return;
+    }
+    const int64_t newest = static_cast<int64_t>(p.seen[b]) - p.recent;
+    auto key = [&](int j) -> uint32_t {
+        return p.keys_in_smem ? s_keys[j] : evict_key(w[j], pos[j], p.sinks, newest);
+    };
+    if (p.keys_in_smem) {
+#pragma unroll 4
+        for (int j = threadIdx.x; j < n; j += kEvictThreads) s_keys[j] = evict_key(w[j], pos[j], p.sinks, newest);
+    }
+    // radix selection: `prefix` the digits found, `want` the rank still to find below it
+    uint32_t prefix = 0, known = 0;
+    int want = p.budget;
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        const uint32_t mask = (1u << bits) - 1u;
+        for (int i = threadIdx.x; i < kEvictBins; i += kEvictThreads) s_hist[i] = 0;
+        __syncthreads();
+        for (int j = threadIdx.x; j < n; j += kEvictThreads) {
+            const uint32_t k = key(j);
+            if ((k & known) == prefix) atomicAdd(&s_hist[(k >> shift) & mask], 1);
+        }
+        __syncthreads();
+        // digit d such that fewer than `want` keys lie above it, and with it at least `want`:
+        // thread i holds the two highest digits not yet held by threads before it
+        const int d0 = kEvictBins - 1 - 2 * threadIdx.x;
+        const int h0 = s_hist[d0], h1 = s_hist[d0 - 1];
+        int inc = h0 + h1;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, inc, x);
+            if (lane >= x) inc += t;
+        }
+        if (lane == 31) s_a[warp] = inc;
+        __syncthreads();
+        int above = inc - h0 - h1;
+        for (int i = 0; i < warp; ++i) above += s_a[i];
+        if (above < want && above + h0 >= want) {
+            s_digit = d0;
+            s_above = above;
+        } else if (above + h0 < want && above + h0 + h1 >= want) {
+            s_digit = d0 - 1;
+            s_above = above + h0;
+        }
+        __syncthreads();
+        prefix |= static_cast<uint32_t>(s_digit) << shift;
+        known |= mask << shift;
+        want -= s_above;
+        __syncthreads();
+    }
+    // kept: keys above `prefix`, and the first `want` slots whose key equals it
+    const int per = ((n + kEvictWarps - 1) / kEvictWarps + 31) / 32 * 32;
+    const int j0 = min(n, warp * per), j1 = min(n, j0 + per);
+    int eq = 0;
+    for (int j = j0 + lane; j - lane < j1; j += 32)
+        eq += __popc(__ballot_sync(0xffffffffu, j < j1 && key(min(j, n - 1)) == prefix));
+    if (lane == 0) s_a[warp] = eq;
+    __syncthreads();
+    int eq0 = 0;
+    for (int i = 0; i < warp; ++i) eq0 += s_a[i];
+    const uint32_t below = (1u << lane) - 1u;
+    // holes (slots below the budget given up) and movers (kept slots beyond it), counted, then listed
+    int holes = 0, movers = 0;
+    int32_t* mv = p.moves + static_cast<int64_t>(row) * p.max_moves * 2;
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+        int rank = eq0, h = holes, m = movers;
+        for (int j = j0 + lane; j - lane < j1; j += 32) {
+            const bool in = j < j1;
+            const uint32_t k = in ? key(j) : 0u;
+            const uint32_t eqs = __ballot_sync(0xffffffffu, in && k == prefix);
+            const bool keep = in && (k > prefix || (k == prefix && rank + __popc(eqs & below) < want));
+            rank += __popc(eqs);
+            const uint32_t hb = __ballot_sync(0xffffffffu, in && !keep && j < p.budget);
+            const uint32_t mb = __ballot_sync(0xffffffffu, keep && j >= p.budget);
+            if (pass) {
+                if (in && !keep && j < p.budget) mv[2 * (h + __popc(hb & below))] = j;
+                if (keep && j >= p.budget) mv[2 * (m + __popc(mb & below)) + 1] = j;
+            }
+            h += __popc(hb);
+            m += __popc(mb);
+        }
+        if (pass == 0) {
+            __syncthreads();
+            if (lane == 0) {
+                s_a[warp] = h;
+                s_b[warp] = m;
+            }
+            __syncthreads();
+            for (int i = 0; i < warp; ++i) {
+                holes += s_a[i];
+                movers += s_b[i];
+            }
+        }
+    }
+    int count = 0;
+    for (int i = 0; i < kEvictWarps; ++i) count += s_a[i];
+    for (int j = threadIdx.x; j < p.budget; j += kEvictThreads) {
+        src[j] = j;
+        if (p.weights_out != p.weights) p.weights_out[base + j] = w[j];
+        if (p.positions_out != p.positions) p.positions_out[base + j] = pos[j];
+    }
+    if (threadIdx.x == 0) p.counts[row] = count;
+    __syncthreads();   // the lists and the copies above are written
+    for (int i = threadIdx.x; i < count; i += kEvictThreads) {
+        const int to = mv[2 * i], from = mv[2 * i + 1];
+        src[to] = from;
+        p.weights_out[base + to] = w[from];
+        p.positions_out[base + to] = pos[from];
+    }
+}
+
+constexpr int kEvictMoveThreads = 256;
+constexpr int kEvictMovesPerBlock = 64;
+
+// The K and V rows of the moves: one warp per move, sources (slots >= budget)
+// and targets (slots < budget) never overlap, so the order does not matter.
+template <typename V>
+__global__ void __launch_bounds__(kEvictMoveThreads) paged_evict_move_kernel(const __grid_constant__ PagedEvictParams p,
+                                                                             int units, int elems_per_unit) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row = blockIdx.y, b = row / p.c.kv_heads, g = row % p.c.kv_heads;
+    pdl_wait();
+    if (g == 0 && blockIdx.x == 0 && threadIdx.x == 0) p.lens_out[b] = min(p.lens_copy[b], p.budget);
+    const int count = p.counts[row];
+    const int32_t* mv = p.moves + static_cast<int64_t>(row) * p.max_moves * 2;
+    const int32_t* table = p.c.page_table + b * p.c.page_table_stride;
+    const int es = static_cast<int>(sizeof(V)) / elems_per_unit;
+    char* kp = static_cast<char*>(p.c.k_pages);
+    char* vp = static_cast<char*>(p.c.v_pages);
+    for (int i0 = blockIdx.x * kEvictMovesPerBlock; i0 < count; i0 += gridDim.x * kEvictMovesPerBlock)
+        for (int i = i0 + warp; i < min(count, i0 + kEvictMovesPerBlock); i += kEvictMoveThreads / 32) {
+            const int to = mv[2 * i], from = mv[2 * i + 1];
+            const int tp = table[to / p.c.page_size], fp = table[from / p.c.page_size];
+            if (tp < 0 || tp >= p.c.num_pages || fp < 0 || fp >= p.c.num_pages) {
+                if (lane == 0) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
+                continue;
+            }
+            const int64_t ts = to % p.c.page_size, fs = from % p.c.page_size;
+            for (int u = lane; u < 2 * units; u += 32) {
+                const bool isv = u >= units;
+                const int64_t e = static_cast<int64_t>(isv ? u - units : u) * elems_per_unit;
+                char* base = isv ? vp : kp;
+                const int64_t ps = isv ? p.c.v_page_stride : p.c.k_page_stride;
+                const int64_t ss = isv ? p.c.v_slot_stride : p.c.k_slot_stride;
+                const int64_t hs = g * (isv ? p.c.v_head_stride : p.c.k_head_stride) + e;
+                *reinterpret_cast<V*>(base + (tp * ps + ts * ss + hs) * es) =
+                    *reinterpret_cast<const V*>(base + (fp * ps + fs * ss + hs) * es);
+            }
+        }
+}
+
+}  // namespace chronos

@@ -523,6 +523,275 @@ def attn_decode(kind: str, proj: torch.Tensor, pos: torch.Tensor, cos: torch.Ten
     return out
 
 
+# ---------------------------------------------------------------------------
+# paged key-value cache (include/chronos_paged.h)
+# ---------------------------------------------------------------------------
+
+def _forward_only(*ts: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("forward-only kernels: call under torch.no_grad() or detach the inputs")
+
+
+def _check_i32(name: str, t: torch.Tensor, shape: tuple, dev: torch.device) -> int:
+    if t.dtype != torch.int32 or t.device != dev or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor {shape} on {dev}, got {t.dtype} {tuple(t.shape)} "
+                         f"on {t.device}")
+    return t.data_ptr()
+
+
+def _check_rows(name: str, t: torch.Tensor, shape: tuple, dt: torch.dtype, dev: torch.device) -> None:
+    """Rows of vectors: the last dimension contiguous, the others by their strides."""
+    if t.dtype != dt or t.device != dev:
+        raise TypeError(f"{name}: {dt} on {dev} expected, got {t.dtype} on {t.device}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        raise ValueError(f"{name}'s last dimension must be contiguous")
+
+
+def _check_slots(name: str, t: torch.Tensor, shape: tuple, dt: torch.dtype, dev: torch.device) -> int:
+    """A per-slot array [B, kv heads, slots]."""
+    if t.dtype != dt or t.device != dev or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dt} tensor {shape} on {dev}, got {t.dtype} {tuple(t.shape)} "
+                         f"on {t.device}")
+    return t.data_ptr()
+
+
+def _written_once(name: str, t: torch.Tensor) -> None:
+    """Refuse a tensor that is written through and holds one element at several places."""
+    for n, s in zip(t.shape, t.stride()):
+        if n > 1 and s == 0:
+            raise ValueError(f"{name} is written: it must not be expanded")
+
+
+def _paged_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
+                 written: bool) -> N.ChronosPagedCache:
+    """The checked cache part of a paged call's arguments."""
+    if not k_pages.is_cuda:
+        raise RuntimeError(f"chronos paged kernels need CUDA tensors (no CPU path exists); got a tensor on {k_pages.device}")
+    dev, dt = k_pages.device, k_pages.dtype
+    if dt not in _DTYPES:
+        raise TypeError(f"unsupported dtype {dt}")
+    if k_pages.dim() != 4:
+        raise ValueError(f"k_pages must be [pages, page size, kv heads, head dim], got {tuple(k_pages.shape)}")
+    _check_rows("v_pages", v_pages, tuple(k_pages.shape), dt, dev)
+    if k_pages.stride(3) != 1 and k_pages.shape[3] != 1:
+        raise ValueError("k_pages' last dimension must be contiguous")
+    if written:
+        _written_once("k_pages", k_pages)
+        _written_once("v_pages", v_pages)
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != dev:
+        raise ValueError(f"page_table must be an int32 tensor [B, pages] on {dev}")
+    b, width = page_table.shape
+    if width > 1 and page_table.stride(1) != 1:
+        raise ValueError("page_table's rows must be contiguous")
+    pages, size, g, d = k_pages.shape
+    kp, ks, kh, _ = k_pages.stride()
+    vp, vs, vh, _ = v_pages.stride()
+    return N.ChronosPagedCache(b, g, d, _DTYPES[dt], pages, size, width, 0, k_pages.data_ptr(), v_pages.data_ptr(),
+                               kp, ks, kh, vp, vs, vh, page_table.data_ptr(), page_table.stride(0),
+                               _check_i32("lens", lens, (b,), dev))
+
+
+def _launch(fn, args, dev: torch.device) -> None:
+    """Call ``fn`` on ``dev``'s current stream (the device of the tensors, whatever
+    the current device is)."""
+    stream = ctypes.c_void_p(_raw_stream(dev.index))
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(ctypes.byref(args), stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(ctypes.byref(args), stream)
+    N.check(rc)
+
+
+def _workspace(fn, args, dev: torch.device) -> torch.Tensor:
+    """Workspace of one call from torch's allocator: a captured graph keeps its own."""
+    if torch.cuda.current_device() == dev.index:
+        nbytes = fn(ctypes.byref(args))
+    else:
+        with torch.cuda.device(dev):
+            nbytes = fn(ctypes.byref(args))
+    if nbytes == 0:
+        N.check(N.CHRONOS_ERR_INVALID_ARG)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+    return ws
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 page_table: torch.Tensor, lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
+                 seen: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,
+                 positions: Optional[torch.Tensor] = None) -> None:
+    """Write new key/value rows into the pages (include/chronos_paged.h).
+
+    k, v [T, kv heads, D]: one token per sequence (T = B), or packed sequences with
+    ``cu_seqlens`` int32 [B + 1]; k_pages, v_pages [pages, page size, kv heads, D];
+    page_table int32 [B, pages]; lens int32 [B], slots in use before the call (not
+    changed).  Sequence b's i-th token goes to slot lens[b] + i; where given,
+    ``weights`` fp32 [B, kv heads, slots] get 0 there and ``positions`` int32 of
+    that shape seen[b] + i (``seen`` int32 [B]: tokens seen before).  A page must
+    not belong to two sequences that are written."""
+    _forward_only(k, v, k_pages, v_pages)
+    cache = _paged_cache(k_pages, v_pages, page_table, lens, written=True)
+    dev, dt = k_pages.device, k_pages.dtype
+    b, g, d = cache.batch, cache.kv_heads, cache.head_dim
+    t = k.shape[0]
+    _check_rows("k", k, (t, g, d), dt, dev)
+    _check_rows("v", v, (t, g, d), dt, dev)
+    cap, wp, pp = 0, None, None
+    for name, x, want in (("weights", weights, torch.float32), ("positions", positions, torch.int32)):
+        if x is not None:
+            if cap and x.shape[-1] != cap:
+                raise ValueError("weights and positions must have the same number of slots")
+            cap = x.shape[-1]
+            ptr = _check_slots(name, x, (b, g, cap), want, dev)
+            wp, pp = (ptr, pp) if name == "weights" else (wp, ptr)
+    args = N.ChronosPagedAppendArgs(
+        cache, t, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+        None if cu_seqlens is None else _check_i32("cu_seqlens", cu_seqlens, (b + 1,), dev),
+        None if seen is None else _check_i32("seen", seen, (b,), dev), wp, pp, cap, status_word(dev).data_ptr())
+    _launch(N.load_library().chronos_paged_append, args, dev)
+
+
+def paged_attn_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                      lens: torch.Tensor, scale: Optional[float] = None, window: int = 0, sinks: int = 0,
+                      weights: Optional[torch.Tensor] = None, weights_out: Optional[torch.Tensor] = None,
+                      out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per sequence over its pages (include/chronos_paged.h).
+
+    q [B, heads, D] (heads a multiple of the pages' kv heads, keys stored rotated);
+    lens int32 [B] counts the slots to attend to, the new token's included.  With
+    ``window`` > 0 the last ``window`` slots and the first ``sinks`` are visible.
+    ``scale`` defaults to D ** -0.5.  Returns out [B, heads, D] (zeros for a
+    sequence of length 0); ``lse`` fp32 [B, heads] receives the log of each softmax
+    sum.  ``weights`` fp32 [B, kv heads, slots]: weights_out (default: in place)
+    receives weights plus every slot's attention weight summed over the group's
+    heads; slots at or behind lens are left as they are."""
+    _forward_only(q, k_pages, v_pages)
+    cache = _paged_cache(k_pages, v_pages, page_table, lens, written=False)
+    dev, dt = k_pages.device, k_pages.dtype
+    b, d = cache.batch, cache.head_dim
+    h = q.shape[1] if q.dim() == 3 else 0
+    _check_rows("q", q, (b, h, d), dt, dev)
+    if out is None:
+        out = torch.empty(b, h, d, dtype=dt, device=dev)
+    else:
+        _check_rows("out", out, (b, h, d), dt, dev)
+        _written_once("out", out)
+    cap, wp, wo = 0, None, None
+    if weights is not None:
+        cap = weights.shape[-1]
+        wp = _check_slots("weights", weights, (b, cache.kv_heads, cap), torch.float32, dev)
+        wo = wp if weights_out is None else _check_slots("weights_out", weights_out, tuple(weights.shape),
+                                                         torch.float32, dev)
+    elif weights_out is not None:
+        raise ValueError("weights_out needs weights")
+    if lse is not None and (lse.dtype != torch.float32 or lse.device != dev or tuple(lse.shape) != (b, h)
+                            or not lse.is_contiguous()):
+        raise ValueError(f"lse must be a contiguous fp32 tensor {(b, h)} on {dev}")
+    args = N.ChronosPagedDecodeArgs(
+        cache, h, int(window), int(sinks), d ** -0.5 if scale is None else float(scale), q.data_ptr(), q.stride(0),
+        q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse), wp, wo, cap, None, 0,
+        status_word(dev).data_ptr())
+    lib = N.load_library()
+    ws = _workspace(lib.chronos_paged_decode_workspace, args, dev)  # noqa: F841 (held until the launch)
+    _launch(lib.chronos_paged_decode, args, dev)
+    return out
+
+
+def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
+                seen: torch.Tensor, weights: torch.Tensor, positions: torch.Tensor, budget: int, sinks: int = 0,
+                recent: int = 0, weights_out: Optional[torch.Tensor] = None,
+                positions_out: Optional[torch.Tensor] = None, lens_out: Optional[torch.Tensor] = None) -> dict:
+    """Cut every (sequence, kv head) down to ``budget`` slots (include/chronos_paged.h).
+
+    Kept: positions below ``sinks``, the ``recent`` newest (>= seen - recent), then the
+    largest ``weights`` (fp32 [B, kv heads, slots], equal ones by the lower slot);
+    kept slots at or beyond the budget move into the slots given up below it, K and V
+    in the pages, weights and ``positions`` (int32) into ``weights_out`` /
+    ``positions_out`` (default: in place).  Returns dict(lens, weights, positions, src):
+    lens int32 [B] (``lens_out`` or new), src int32 [B, kv heads, budget], the slot
+    that now sits in each slot (-1 behind the length).  A page must not belong to two
+    sequences."""
+    _forward_only(k_pages, v_pages, weights)
+    cache = _paged_cache(k_pages, v_pages, page_table, lens, written=True)
+    dev = k_pages.device
+    b, g = cache.batch, cache.kv_heads
+    cap = weights.shape[-1]
+    shape = (b, g, cap)
+    wp = _check_slots("weights", weights, shape, torch.float32, dev)
+    pp = _check_slots("positions", positions, shape, torch.int32, dev)
+    weights_out = weights if weights_out is None else weights_out
+    positions_out = positions if positions_out is None else positions_out
+    wo = _check_slots("weights_out", weights_out, shape, torch.float32, dev)
+    po = _check_slots("positions_out", positions_out, shape, torch.int32, dev)
+    if lens_out is None:
+        lens_out = torch.empty(b, dtype=torch.int32, device=dev)
+    if int(budget) < 1:
+        raise ValueError(f"budget {budget} must be at least 1")
+    src = torch.empty(b, g, int(budget), dtype=torch.int32, device=dev)
+    args = N.ChronosPagedEvictArgs(
+        cache, int(budget), int(sinks), int(recent), 0, _check_i32("seen", seen, (b,), dev), wp, pp, wo, po, cap,
+        _check_i32("lens_out", lens_out, (b,), dev), src.data_ptr(), None, 0, status_word(dev).data_ptr())
+    lib = N.load_library()
+    ws = _workspace(lib.chronos_paged_evict_workspace, args, dev)  # noqa: F841 (held until the launch)
+    _launch(lib.chronos_paged_evict, args, dev)
+    return dict(lens=lens_out, weights=weights_out, positions=positions_out, src=src)
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                     cu_seqlens_k: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0,
+                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                     lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of packed prompts (include/chronos_paged.h).
+
+    q [Tq, heads, D], k and v [Tk, kv heads, D]; sequence b has the query rows
+    cu_seqlens[b]..cu_seqlens[b+1] and the key rows of ``cu_seqlens_k`` (int32 [B + 1],
+    default: the same).  Its queries are the newest of its keys: query i stands at
+    position t = lk - lq + i and sees the keys j <= t, under a ``window`` > 0 only
+    j > t - window and the first ``sinks``.  ``scale`` defaults to D ** -0.5.  Returns
+    out [Tq, heads, D]: zeros for a row that sees nothing, rows behind the last
+    sequence as they were (``out``) or undefined; ``lse`` fp32 [Tq, heads]."""
+    if not q.is_cuda:
+        raise RuntimeError(f"chronos paged kernels need CUDA tensors (no CPU path exists); got a tensor on {q.device}")
+    _forward_only(q, k, v)
+    dev, dt = q.device, q.dtype
+    if dt not in _DTYPES:
+        raise TypeError(f"unsupported dtype {dt}")
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"q and k must be [rows, heads, head dim], got {tuple(q.shape)} and {tuple(k.shape)}")
+    tq, h, d = q.shape
+    tk, g, _ = k.shape
+    _check_rows("q", q, (tq, h, d), dt, dev)
+    _check_rows("k", k, (tk, g, d), dt, dev)
+    _check_rows("v", v, (tk, g, d), dt, dev)
+    if cu_seqlens_k is None:
+        cu_seqlens_k = cu_seqlens
+        if tk != tq:
+            raise ValueError(f"{tq} query rows and {tk} key rows need cu_seqlens_k")
+    b = cu_seqlens.numel() - 1
+    if b < 0:
+        raise ValueError("cu_seqlens must have one more entry than there are sequences")
+    if out is None:
+        out = torch.empty(tq, h, d, dtype=dt, device=dev)
+    else:
+        _check_rows("out", out, (tq, h, d), dt, dev)
+        _written_once("out", out)
+    if lse is not None and (lse.dtype != torch.float32 or lse.device != dev or tuple(lse.shape) != (tq, h)
+                            or not lse.is_contiguous()):
+        raise ValueError(f"lse must be a contiguous fp32 tensor {(tq, h)} on {dev}")
+    args = N.ChronosWindowAttnArgs(
+        b, h, g, d, _DTYPES[dt], int(window), int(sinks), d ** -0.5 if scale is None else float(scale), tq, tk,
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+        v.stride(0), v.stride(1), out.stride(0), out.stride(1), _check_i32("cu_seqlens", cu_seqlens, (b + 1,), dev),
+        _check_i32("cu_seqlens_k", cu_seqlens_k, (b + 1,), dev), _ptr(lse), status_word(dev).data_ptr())
+    _launch(N.load_library().chronos_window_attention, args, dev)
+    return out
+
+
 def profile_begin(max_calls: int) -> None:
     """Record per-stage CUDA events for the next ``max_calls`` layer calls (this thread)."""
     lib = N.load_library()

@@ -1,0 +1,805 @@
+"""The paged key-value cache (include/chronos_paged.h): append, one-token attention,
+eviction by attention weight, and prompt attention with a window and first tokens.
+
+CPU: refusals of the torch-facing calls and of the C ABI.  GPU: every operator
+against its definition in 64 bits.  Tolerances follow from the arithmetic, with
+u = finfo(type).eps / 2 and A = sum_j p_j |v_j|:
+
+* a score is a sum of D products accumulated in fp32 (each addition off by at most
+  2^-23 of the running sum of magnitudes, also where the tensor core cuts instead of
+  rounding), so it is off by at most D 2^-23 S, S = max_j scale sum_d |q_d k_jd|; the
+  exponential adds 2^-21 of its value; a weight p_j is thus off by
+  f = D 2^-23 S + n 2^-24 + 2^-20 of itself (n: terms of its normalising sum);
+* 16-bit layers round the weights to the layer type before the second product (u A) and
+  the result once (u |out|); the second product adds n 2^-23 A.
+  So |error| <= u (A + |out|) + (f + n 2^-23) A, without the first u A for fp32;
+* lse is off by at most f + 2^-22 |lse|; a slot's summed weight by f sum p + rounding.
+"""
+import ctypes
+import math
+
+import pytest
+import torch
+
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+gpu = pytest.mark.gpu
+
+
+def _unit(dt):
+    return torch.finfo(dt).eps / 2
+
+
+# ---------------------------------------------------------------------------------------
+# refusals (no GPU)
+# ---------------------------------------------------------------------------------------
+
+@pytest.fixture(scope="module")
+def lib():
+    from project_chronos_b200 import _native, build
+    build.build()
+    return _native.load_library()
+
+
+def _cpu_cache(b=2, g=2, d=16, pages=4, size=4, width=2, dt=FP):
+    return (torch.zeros(pages, size, g, d, dtype=dt), torch.zeros(pages, size, g, d, dtype=dt),
+            torch.zeros(b, width, dtype=torch.int32), torch.ones(b, dtype=torch.int32))
+
+
+def test_cpu_tensors_are_refused():
+    from project_chronos_b200 import ops
+    kp, vp, table, lens = _cpu_cache()
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.paged_attn_decode(torch.zeros(2, 4, 16), kp, vp, table, lens)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.paged_append(torch.zeros(2, 2, 16), torch.zeros(2, 2, 16), kp, vp, table, lens)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.paged_evict(kp, vp, table, lens, lens, torch.zeros(2, 2, 8), torch.zeros(2, 2, 8, dtype=torch.int32), 4)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.window_attention(torch.zeros(3, 4, 16), torch.zeros(3, 2, 16), torch.zeros(3, 2, 16),
+                             torch.tensor([0, 3], dtype=torch.int32))
+
+
+def _native_cache(N, **kw):
+    f = dict(batch=2, kv_heads=2, head_dim=16, dtype=N.DTYPE_BF16, num_pages=4, page_size=4, table_width=2)
+    f.update(kw)
+    return N.ChronosPagedCache(**f)
+
+
+@pytest.mark.parametrize("change, text", [
+    (dict(cache=dict(head_dim=0)), b"head_dim"), (dict(cache=dict(head_dim=257)), b"head_dim"),
+    (dict(cache=dict(page_size=0)), b"page_size"), (dict(cache=dict(dtype=7)), b"dtype"),
+    (dict(cache=dict(batch=-1)), b"batch"), (dict(heads=3), b"heads"), (dict(heads=0), b"heads"),
+    (dict(heads=2 * 257), b"heads"), (dict(window=-1), b"window"), (dict(sinks=-1), b"sinks"),
+    (dict(scale=0.0), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(scale=float("inf")), b"scale"),
+    (dict(weights=256), b"weights_out"), ({}, b"required"),
+])
+def test_decode_refuses_before_touching_the_device(lib, change, text):
+    from project_chronos_b200 import _native as N
+    f = dict(heads=4, window=0, sinks=0, scale=0.25)
+    f.update({k: v for k, v in change.items() if k != "cache"})
+    a = N.ChronosPagedDecodeArgs(cache=_native_cache(N, **change.get("cache", {})), **f)
+    assert lib.chronos_paged_decode(ctypes.byref(a), None) == N.CHRONOS_ERR_INVALID_ARG
+    assert text in lib.chronos_moe_last_error()
+    if change:
+        assert lib.chronos_paged_decode_workspace(ctypes.byref(a)) == 0
+
+
+@pytest.mark.parametrize("f, text", [
+    (dict(budget=0), b"budget"), (dict(budget=4, sinks=3, recent=2), b"budget"), (dict(budget=4, sinks=-1), b"budget"),
+    (dict(budget=4, recent=-1), b"budget"), (dict(budget=4, slot_cap=-1), b"slot_cap"), (dict(budget=4), b"required"),
+])
+def test_evict_refuses_before_touching_the_device(lib, f, text):
+    from project_chronos_b200 import _native as N
+    a = N.ChronosPagedEvictArgs(cache=_native_cache(N), **f)
+    assert lib.chronos_paged_evict(ctypes.byref(a), None) == N.CHRONOS_ERR_INVALID_ARG
+    assert text in lib.chronos_moe_last_error()
+
+
+@pytest.mark.parametrize("f, text", [
+    (dict(num_tokens=-1), b"num_tokens"), (dict(num_tokens=3), b"cu_seqlens"),
+    (dict(num_tokens=2, positions=256), b"seen"), (dict(num_tokens=2, weights=256, slot_cap=-1), b"slot_cap"),
+    (dict(num_tokens=2), b"required"),
+])
+def test_append_refuses_before_touching_the_device(lib, f, text):
+    from project_chronos_b200 import _native as N
+    a = N.ChronosPagedAppendArgs(cache=_native_cache(N), **f)
+    assert lib.chronos_paged_append(ctypes.byref(a), None) == N.CHRONOS_ERR_INVALID_ARG
+    assert text in lib.chronos_moe_last_error()
+
+
+@pytest.mark.parametrize("change, text", [
+    (dict(heads=3), b"heads"), (dict(kv_heads=0), b"kv_heads"), (dict(head_dim=300), b"head_dim"),
+    (dict(dtype=-1), b"dtype"), (dict(window=-2), b"window"), (dict(scale=-1.0), b"scale"),
+    (dict(num_q=-1), b"query rows"), (dict(num_k=1 << 31), b"key rows"), ({}, b"required"),
+])
+def test_window_attention_refuses_before_touching_the_device(lib, change, text):
+    from project_chronos_b200 import _native as N
+    f = dict(batch=1, heads=4, kv_heads=2, head_dim=16, dtype=N.DTYPE_BF16, scale=0.25, num_q=4, num_k=4)
+    f.update(change)
+    a = N.ChronosWindowAttnArgs(**f)
+    assert lib.chronos_window_attention(ctypes.byref(a), None) == N.CHRONOS_ERR_INVALID_ARG
+    assert text in lib.chronos_moe_last_error()
+
+
+def test_empty_calls_return_without_a_device(lib):
+    from project_chronos_b200 import _native as N
+    d = N.ChronosPagedDecodeArgs(cache=_native_cache(N, batch=0), heads=4, scale=1.0)
+    assert lib.chronos_paged_decode(ctypes.byref(d), None) == N.CHRONOS_OK
+    e = N.ChronosPagedEvictArgs(cache=_native_cache(N, batch=0), budget=1)
+    assert lib.chronos_paged_evict(ctypes.byref(e), None) == N.CHRONOS_OK
+    p = N.ChronosPagedAppendArgs(cache=_native_cache(N, batch=0))
+    assert lib.chronos_paged_append(ctypes.byref(p), None) == N.CHRONOS_OK
+    w = N.ChronosWindowAttnArgs(batch=0, heads=2, kv_heads=2, head_dim=8, scale=1.0)
+    assert lib.chronos_window_attention(ctypes.byref(w), None) == N.CHRONOS_OK
+
+
+# ---------------------------------------------------------------------------------------
+# definitions in 64 bits
+# ---------------------------------------------------------------------------------------
+
+def _attend(q, k, v, scale, seen):
+    """q [H, D], k and v [n, G, D], seen [n] (or [H, n]): out, lse, p [H, n], and what the
+    tolerance needs: A [H, D], f."""
+    h, g = q.shape[0], k.shape[1]
+    k = k.double().repeat_interleave(h // g, dim=1)
+    v = v.double().repeat_interleave(h // g, dim=1)
+    seen = seen.expand(h, -1)
+    q = q.double()
+    x = torch.einsum("hd,nhd->hn", q, torch.where(seen.T[..., None], k, 0.0)) * scale
+    x = x.masked_fill(~seen, -math.inf)
+    lse = torch.logsumexp(x, dim=1)
+    p = torch.where(seen, torch.exp(x - lse[:, None]), 0.0)
+    v = torch.where(seen.T[..., None], v, 0.0)
+    out = torch.einsum("hn,nhd->hd", p, v)
+    a = torch.einsum("hn,nhd->hd", p, v.abs())
+    s = (torch.einsum("hd,nhd->hn", q.abs(), torch.where(seen.T[..., None], k, 0.0).abs()) * scale).amax(dim=1) \
+        if k.shape[0] else torch.zeros(h, dtype=torch.float64, device=q.device)
+    n = k.shape[0]
+    f = q.shape[1] * 2.0 ** -23 * s + n * 2.0 ** -24 + 2.0 ** -20
+    return out, lse, p, a, f
+
+
+def _check_out(got, out, a, f, n, dt):
+    u = _unit(dt)
+    tol = u * out.abs() + (f[:, None] + n * 2.0 ** -23) * a + (u * a if dt != FP else 0.0) + 1e-30
+    if dt == HF:
+        # below fp16's normal range the result and each of the n weights (relative to a sum of at least 1)
+        # step by 2^-24; the values are standard normal, below 6
+        tol = tol + 2.0 ** -25 * (1 + 6 * n)
+    err = (got.double() - out).abs()
+    assert bool((err <= tol).all()), f"off by {float((err / tol).max()):.2f} of the tolerance"
+
+
+def _check_lse(got, lse, f):
+    none = lse == -math.inf
+    assert bool((got.double()[none] == -math.inf).all())
+    err = (got.double() - lse).abs()[~none]
+    assert bool((err <= (f + 2.0 ** -22 * lse.abs())[~none]).all())
+
+
+def _visible(n, window, sinks, dev, at=None):
+    """Slots a query at the last position (or at position `at`) sees of n."""
+    t = n - 1 if at is None else at
+    j = torch.arange(n, device=dev)
+    seen = j <= t
+    if window:
+        seen = seen & ((j > t - window) | (j < sinks))
+    return seen
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _make_cache(lens, g, d, size, dt, seed, width=None, bad=float("nan")):
+    """Shuffled pages; what no sequence owns is `bad`."""
+    gen = _gen(seed)
+    width = width or max(1, -(-max(lens) // size)) + 1
+    b = len(lens)
+    pages = b * width + 2
+    table = torch.randperm(pages, generator=gen, device="cuda")[: b * width].view(b, width).to(torch.int32)
+    kp = torch.full((pages, size, g, d), bad, dtype=dt, device="cuda")
+    vp = torch.full((pages, size, g, d), bad, dtype=dt, device="cuda")
+    rows = []
+    for i, n in enumerate(lens):
+        k = torch.randn(n, g, d, generator=gen, device="cuda").to(dt)
+        v = torch.randn(n, g, d, generator=gen, device="cuda").to(dt)
+        s = torch.arange(n, device="cuda")
+        kp[table[i].long()[s // size], s % size] = k
+        vp[table[i].long()[s // size], s % size] = v
+        rows.append((k, v))
+    return kp, vp, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), rows
+
+
+# ---------------------------------------------------------------------------------------
+# one-token attention
+# ---------------------------------------------------------------------------------------
+
+LENS = [0, 1, 15, 16, 17, 63, 64, 65, 333, 1100]
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("h, g, d, size", [(8, 2, 128, 16), (4, 4, 64, 64), (10, 2, 80, 48), (9, 1, 96, 16), (17, 1, 128, 32),
+                                           (16, 2, 256, 16), (6, 3, 40, 7), (2, 1, 37, 5), (3, 3, 1, 1), (40, 1, 8, 16)])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (50, 0), (64, 4), (7, 100)])
+def test_decode_matches_its_definition(dt, h, g, d, size, window, sinks):
+    from project_chronos_b200 import ops
+    kp, vp, table, lens, rows = _make_cache(LENS, g, d, size, dt, seed=h * d + size)
+    q = (2 * torch.randn(len(LENS), h, d, generator=_gen(3), device="cuda")).to(dt)
+    lse = torch.full((len(LENS), h), 7.0, device="cuda")
+    out = ops.paged_attn_decode(q, kp, vp, table, lens, window=window, sinks=sinks, lse=lse)
+    ops.check_status(out.device)
+    for b, (k, v) in enumerate(rows):
+        n = LENS[b]
+        ref, rl, _, a, f = _attend(q[b], k, v, d ** -0.5, _visible(n, window, sinks, "cuda"))
+        _check_out(out[b], ref, a, f, n, dt)
+        _check_lse(lse[b], rl, f)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("h, g, lens", [(8, 1, [20011]), (4, 2, [1, 9000, 3, 0, 5000]), (24, 1, [7001, 64])])
+def test_decode_split_over_the_length(dt, h, g, lens):
+    from project_chronos_b200 import ops
+    d, size = 128, 16
+    kp, vp, table, ln, rows = _make_cache(lens, g, d, size, dt, seed=5)
+    q = (3 * torch.randn(len(lens), h, d, generator=_gen(6), device="cuda")).to(dt)
+    lse = torch.empty(len(lens), h, device="cuda")
+    out = ops.paged_attn_decode(q, kp, vp, table, ln, lse=lse)
+    again = ops.paged_attn_decode(q, kp, vp, table, ln)
+    assert torch.equal(out, again)
+    for b, (k, v) in enumerate(rows):
+        n = lens[b]
+        ref, rl, _, a, f = _attend(q[b], k, v, d ** -0.5, _visible(n, 0, 0, "cuda"))
+        _check_out(out[b], ref, a, f, n, dt)
+        _check_lse(lse[b], rl, f)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("h, g, d, window, sinks", [(8, 2, 128, 0, 0), (20, 2, 64, 100, 3), (6, 6, 36, 0, 0)])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_decode_adds_attention_weights(dt, h, g, d, window, sinks, in_place):
+    from project_chronos_b200 import ops
+    lens = [0, 1, 70, 2500, 130]
+    kp, vp, table, ln, rows = _make_cache(lens, g, d, 16, dt, seed=8)
+    cap = table.shape[1] * 16 + (0 if in_place else 3)
+    q = (2 * torch.randn(len(lens), h, d, generator=_gen(9), device="cuda")).to(dt)
+    w = torch.rand(len(lens), g, cap, generator=_gen(10), device="cuda")
+    before = w.clone()
+    to = w if in_place else torch.full_like(w, -5.0)
+    out = ops.paged_attn_decode(q, kp, vp, table, ln, window=window, sinks=sinks, weights=w,
+                                weights_out=None if in_place else to)
+    plain = ops.paged_attn_decode(q, kp, vp, table, ln, window=window, sinks=sinks)
+    assert torch.equal(out, plain)
+    for b, (k, v) in enumerate(rows):
+        n = lens[b]
+        _, _, p, _, f = _attend(q[b], k, v, d ** -0.5, _visible(n, window, sinks, "cuda"))
+        rep = h // g
+        add = p.view(g, rep, n).sum(1)
+        want = before[b, :, :n].double() + add
+        tol = f.view(g, rep).amax(1)[:, None] * add + (rep + 1) * 2.0 ** -24 * want
+        assert bool(((to[b, :, :n].double() - want).abs() <= tol).all())
+        behind = before[b, :, n:] if in_place else torch.full_like(before[b, :, n:], -5.0)
+        assert torch.equal(to[b, :, n:], behind)
+    if not in_place:
+        assert torch.equal(w, before)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("layout", ["interleaved", "heads first", "odd strides"])
+def test_decode_takes_strides(dt, layout):
+    from project_chronos_b200 import ops
+    lens, h, g, d, size = [33, 200, 5], 8, 2, 64, 16
+    kp, vp, table, ln, rows = _make_cache(lens, g, d, size, dt, seed=21)
+    if layout == "interleaved":
+        both = torch.stack([kp, vp], dim=1)
+        kp, vp = both[:, 0], both[:, 1]
+    elif layout == "heads first":
+        kp, vp = (x.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3) for x in (kp, vp))
+    else:   # rows of d + 1 elements: no 16-byte copies
+        kp, vp = (torch.cat([x, x[..., :1]], dim=-1)[..., :d] for x in (kp, vp))
+    fused = (2 * torch.randn(len(lens), h + 2 * g + 1, d, generator=_gen(4), device="cuda")).to(dt)
+    wide = torch.full((len(lens), h + 1, d + 2), 9.0, dtype=dt, device="cuda")
+    out = wide[:, :h, :d]
+    tall = torch.cat([table, table], dim=1)[:, : table.shape[1]]
+    ops.paged_attn_decode(fused[:, :h], kp, vp, tall, ln, out=out)
+    for b, (k, v) in enumerate(rows):
+        ref, _, _, a, f = _attend(fused[b, :h], k, v, d ** -0.5, _visible(lens[b], 0, 0, "cuda"))
+        _check_out(out[b], ref, a, f, lens[b], dt)
+    assert bool((wide[:, h:] == 9.0).all()) and bool((wide[..., d:] == 9.0).all())
+
+
+@gpu
+def test_decode_offsets_pass_32_bits():
+    from project_chronos_b200 import ops
+    g, d, size = 8, 128, 64
+    pages = (1 << 31) // (g * d * size) + 40      # elements of one of K, V beyond 2^31
+    kp = torch.empty(pages, size, g, d, dtype=BF, device="cuda")
+    vp = torch.empty(pages, size, g, d, dtype=BF, device="cuda")
+    table = torch.tensor([[pages - 1, 2, pages - 7]], dtype=torch.int32, device="cuda")
+    n = 150
+    k, v = torch.randn(n, g, d, device="cuda").to(BF), torch.randn(n, g, d, device="cuda").to(BF)
+    lens = torch.tensor([0], dtype=torch.int32, device="cuda")
+    ops.paged_append(k, v, kp, vp, table, lens, cu_seqlens=torch.tensor([0, n], dtype=torch.int32, device="cuda"))
+    s = torch.arange(n, device="cuda")
+    assert torch.equal(kp[table[0].long()[s // size], s % size], k)
+    q = torch.randn(1, 16, d, device="cuda").to(BF)
+    lens.fill_(n)
+    out = ops.paged_attn_decode(q, kp, vp, table, lens)
+    ref, _, _, a, f = _attend(q[0], k, v, d ** -0.5, _visible(n, 0, 0, "cuda"))
+    _check_out(out[0], ref, a, f, n, BF)
+    cap = 3 * size
+    r = ops.paged_evict(kp, vp, table, lens, lens, torch.rand(1, g, cap, device="cuda"),
+                        torch.arange(cap, dtype=torch.int32, device="cuda").expand(1, g, cap).contiguous(), 70)
+    for j in range(g):
+        src = r["src"][0, j].long()
+        assert torch.equal(kp[table[0].long()[s[:70] // size], s[:70] % size, j], k[src, j])
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_bad_pages_and_lengths_are_reported_and_stay_in_bounds(dt):
+    from project_chronos_b200 import _native as N
+    from project_chronos_b200 import ops
+    lens, h, g, d = [40, 100], 4, 2, 64
+    kp, vp, table, ln, rows = _make_cache(lens, g, d, 16, dt, seed=2)
+    q = torch.randn(2, h, d, device="cuda").to(dt)
+    dev = q.device
+    ref, _, _, a, f = _attend(q[0], *rows[0], d ** -0.5, _visible(40, 0, 0, "cuda"))
+    for page in (-1, kp.shape[0], 1 << 30):
+        t = table.clone()
+        t[1, 2] = page                            # slots 32..47 of sequence 1 lie nowhere
+        w = torch.zeros(2, g, 128, device="cuda")
+        out = ops.paged_attn_decode(q, kp, vp, t, ln, weights=w)
+        with pytest.raises(N.ChronosMoeError, match="INVALID_ARG"):
+            ops.check_status(dev)
+        _check_out(out[0], ref, a, f, 40, dt)
+        seen = _visible(100, 0, 0, "cuda")
+        seen[32:48] = False
+        r1, _, p1, a1, f1 = _attend(q[1], *rows[1], d ** -0.5, seen)
+        _check_out(out[1], r1, a1, f1, 100, dt)
+        assert bool((w[1, :, 32:48] == 0).all()) and bool(torch.isfinite(w).all())
+        ops.paged_append(q[:, :g].contiguous(), q[:, :g].contiguous(), kp, vp, t,
+                         torch.tensor([60, 33], dtype=torch.int32, device="cuda"))
+        with pytest.raises(N.ChronosMoeError, match="INVALID_ARG"):
+            ops.check_status(dev)
+    for n in (-3, 16 * table.shape[1] + 1, 1 << 30):
+        bad = torch.tensor([40, n], dtype=torch.int32, device="cuda")
+        out = ops.paged_attn_decode(q, kp, vp, table, bad)
+        with pytest.raises(N.ChronosMoeError, match="INVALID_ARG"):
+            ops.check_status(dev)
+        _check_out(out[0], ref, a, f, 40, dt)
+        ops.paged_append(q[:, :g].contiguous(), q[:, :g].contiguous(), kp, vp, table,
+                         torch.tensor([50, n], dtype=torch.int32, device="cuda"))
+        with pytest.raises(N.ChronosMoeError, match="INVALID_ARG"):
+            ops.check_status(dev)
+    ops.check_status(dev)
+
+
+@gpu
+def test_decode_refuses_wrong_tensors():
+    from project_chronos_b200 import ops
+    kp, vp, table, ln, _ = _make_cache([5, 6], 2, 64, 16, BF, seed=1)
+    q = torch.zeros(2, 4, 64, dtype=BF, device="cuda")
+    ok = dict(q=q, k_pages=kp, v_pages=vp, page_table=table, lens=ln)
+    for change in (dict(q=q.float()), dict(q=q[:1]), dict(q=q[..., :32]), dict(v_pages=vp.half()), dict(v_pages=vp[:2]),
+                   dict(page_table=table.long()), dict(lens=ln.long()), dict(lens=ln[:1]), dict(q=q.cpu()),
+                   dict(out=torch.zeros(2, 4, 32, dtype=BF, device="cuda")), dict(lse=torch.zeros(2, 5, device="cuda")),
+                   dict(out=torch.zeros(2, 1, 64, dtype=BF, device="cuda").expand(2, 4, 64)),
+                   dict(weights=torch.zeros(2, 3, 32, device="cuda")), dict(weights_out=torch.zeros(2, 2, 32, device="cuda")),
+                   dict(k_pages=kp.transpose(2, 3).contiguous().transpose(2, 3)), dict(q=q.transpose(1, 2).contiguous().transpose(1, 2))):
+        with pytest.raises((TypeError, ValueError)):
+            ops.paged_attn_decode(**{**ok, **change})
+    with pytest.raises(RuntimeError, match="heads"):
+        ops.paged_attn_decode(**{**ok, "q": q[:, :3]})
+    with pytest.raises(RuntimeError, match="forward-only"):
+        ops.paged_attn_decode(**{**ok, "q": q.clone().requires_grad_()})
+    with pytest.raises(ValueError, match="expanded"):
+        ops.paged_append(q[:, :2].contiguous(), q[:, :2].contiguous(), kp[:1].expand(4, -1, -1, -1),
+                         vp[:1].expand(4, -1, -1, -1), table, ln)
+
+
+@gpu
+def test_decode_graphs_keep_their_own_workspaces():
+    """Two captured calls replay at once on two streams while lengths grow."""
+    from project_chronos_b200 import ops
+    dt, h, g, d = BF, 8, 1, 128
+    state = []
+    for seed in (1, 2):
+        kp, vp, table, ln, rows = _make_cache([6000], g, d, 16, dt, seed=seed)
+        q = torch.randn(1, h, d, generator=_gen(seed), device="cuda").to(dt)
+        out = torch.empty_like(q)
+        w = torch.zeros(1, g, table.shape[1] * 16, device="cuda")
+        ln.fill_(100)
+        ops.paged_attn_decode(q, kp, vp, table, ln, weights=w, out=out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.paged_attn_decode(q, kp, vp, table, ln, weights=w, out=out)
+        state.append((kp, vp, table, ln, rows, q, out, w, graph))
+    streams = [torch.cuda.Stream() for _ in state]
+    for n in (101, 3000, 6000):
+        for s in state:
+            s[3].fill_(n)
+            s[7].zero_()
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for st, s in zip(streams, state):
+                with torch.cuda.stream(st):
+                    s[7].zero_()
+                    s[8].replay()
+        torch.cuda.synchronize()
+        for kp, vp, table, ln, rows, q, out, w, _ in state:
+            k, v = rows[0]
+            ref, _, p, a, f = _attend(q[0], k[:n], v[:n], d ** -0.5, _visible(n, 0, 0, "cuda"))
+            _check_out(out[0], ref, a, f, n, dt)
+            assert bool(((w[0, 0, :n].double() - p.sum(0)).abs() <= f.max() * p.sum(0) + h * 2.0 ** -23 * p.sum(0)).all())
+
+
+# ---------------------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("g, d, size", [(2, 128, 16), (3, 37, 5), (1, 8, 64), (16, 80, 48)])
+@pytest.mark.parametrize("new", [None, [3, 0, 40, 1, 0, 129], [0, 0, 0, 0, 0, 0]])
+def test_append_writes_exactly_its_slots(dt, g, d, size, new):
+    from project_chronos_b200 import ops
+    past = [0, 4, 17, 100, 31, 2]
+    b = len(past)
+    counts = new or [1] * b
+    kp, vp, table, _, _ = _make_cache([p + c for p, c in zip(past, counts)], g, d, size, dt, seed=d, bad=-3.0)
+    lens = torch.tensor(past, dtype=torch.int32, device="cuda")
+    seen = lens + 1000
+    cap = table.shape[1] * size + 1
+    w = torch.full((b, g, cap), 4.0, device="cuda")
+    pos = torch.full((b, g, cap), -9, dtype=torch.int32, device="cuda")
+    extra = 0 if new is None else 3                        # rows behind the last sequence
+    t = sum(counts) + extra
+    fused = torch.randn(t, 2 * g + 1, d, generator=_gen(d), device="cuda").to(dt)
+    k, v = fused[:, :g], fused[:, g: 2 * g]
+    cu = None if new is None else torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+    want = [x.clone() for x in (kp, vp, w, pos)]
+    at = 0
+    for i in range(b):
+        for j in range(counts[i]):
+            s = past[i] + j
+            page = int(table[i, s // size])
+            want[0][page, s % size], want[1][page, s % size] = k[at], v[at]
+            want[2][i, :, s], want[3][i, :, s] = 0.0, past[i] + 1000 + j
+            at += 1
+    ops.paged_append(k, v, kp, vp, table, lens, cu_seqlens=cu, seen=seen, weights=w, positions=pos)
+    ops.check_status(kp.device)
+    for got, ref in zip((kp, vp, w, pos), want):
+        assert torch.equal(got, ref)
+    assert lens.tolist() == past
+
+
+@gpu
+def test_append_takes_pages_of_any_strides():
+    from project_chronos_b200 import ops
+    g, d, size = 2, 64, 16
+    both = torch.zeros(6, 2, g, size, d, dtype=BF, device="cuda")
+    kp, vp = both[:, 0].permute(0, 2, 1, 3), both[:, 1].permute(0, 2, 1, 3)
+    table = torch.tensor([[4, 1], [3, 0]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([15, 30], dtype=torch.int32, device="cuda")
+    k, v = torch.randn(2, g, d, device="cuda").to(BF), torch.randn(2, g, d, device="cuda").to(BF)
+    ops.paged_append(k, v, kp, vp, table, lens)
+    assert torch.equal(both[4, 0, :, 15], k[0]) and torch.equal(both[0, 1, :, 14], v[1])
+    assert int((both != 0).any(-1).sum()) == 2 * 2 * g
+
+
+# ---------------------------------------------------------------------------------------
+# eviction
+# ---------------------------------------------------------------------------------------
+
+def _evict_plan(w, pos, n, seen, budget, sinks, recent):
+    """src of one (sequence, kv head), by the definition: NaN above every number, ties by the lower slot."""
+    if n <= budget:
+        return list(range(n)) + [-1] * (budget - n)
+
+    def rank(j):
+        if pos[j] < sinks or pos[j] >= seen - recent:
+            return (0, 0.0, j)
+        return (1, 0.0, j) if math.isnan(w[j]) else (2, -w[j], j)
+
+    kept = set(sorted(range(n), key=rank)[:budget])
+    movers = iter(sorted(j for j in kept if j >= budget))
+    return [j if j in kept else next(movers) for j in range(budget)]
+
+
+@gpu
+@pytest.mark.parametrize("lens, budget, sinks, recent", [
+    ([100, 1, 0, 64, 65, 300], 64, 4, 16), ([5, 3, 2], 1, 0, 0), ([5, 3, 2], 1, 1, 0), ([2049, 2050, 1000], 2048, 4, 256),
+    ([4000, 3500], 1000, 0, 1000), ([4000, 3500], 1000, 0, 0), ([777], 776, 4, 700), ([1030, 5000], 33, 16, 17)])
+@pytest.mark.parametrize("values", ["random", "ties", "special"])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_evict_keeps_the_largest_weights(lens, budget, sinks, recent, values, in_place):
+    from project_chronos_b200 import ops
+    g, d, size = 2, 16, 16
+    kp, vp, table, ln, rows = _make_cache(lens, g, d, size, BF, seed=budget, bad=-1.0)
+    b, cap = len(lens), table.shape[1] * size
+    gen = _gen(sinks + recent)
+    w = torch.exp(3 * torch.randn(b, g, cap, generator=gen, device="cuda"))
+    if values == "ties":
+        w = torch.randint(0, 3, w.shape, generator=gen, device="cuda").float() - 1.0
+        w = torch.where(w == 0, torch.where(torch.rand(w.shape, generator=gen, device="cuda") < 0.5, -0.0, 0.0), w)
+    elif values == "special":
+        x = torch.rand(w.shape, generator=gen, device="cuda")
+        for lo, val in ((0.0, math.nan), (0.1, math.inf), (0.2, -math.inf), (0.3, 1e-44), (0.4, -1.0), (0.5, 3e38)):
+            w = torch.where((x >= lo) & (x < lo + 0.05), torch.full_like(w, val), w)
+    # a permutation per head, as earlier evictions leave it, with gaps
+    pos = torch.stack([torch.stack([torch.randperm(cap, generator=gen, device="cuda") * 2 for _ in range(g)])
+                       for _ in range(b)]).to(torch.int32)
+    for i, n in enumerate(lens):   # the positions in use: below seen
+        for j in range(g):
+            pos[i, j, :n] = (torch.randperm(n, generator=gen, device="cuda") * 3 // 2).to(torch.int32) if n else pos[i, j, :n]
+    seen = torch.tensor([max(1, 3 * n // 2) for n in lens], dtype=torch.int32, device="cuda")
+    k0, v0, w0, p0 = kp.clone(), vp.clone(), w.clone(), pos.clone()
+    wo, po = (None, None) if in_place else (torch.full_like(w, 8.0), torch.full_like(pos, 8))
+    r = ops.paged_evict(kp, vp, table, ln, seen, w, pos, budget, sinks=sinks, recent=recent, weights_out=wo, positions_out=po,
+                        lens_out=ln if in_place else None)
+    ops.check_status(kp.device)
+    assert r["lens"].tolist() == [min(n, budget) for n in lens]
+    k_want, v_want = k0.clone(), v0.clone()
+    for i, n in enumerate(lens):
+        t = table[i].long()
+        for j in range(g):
+            src = _evict_plan(w0[i, j].tolist(), p0[i, j].tolist(), n, int(seen[i]), budget, sinks, recent)
+            assert r["src"][i, j].tolist() == src
+            m = min(n, budget)
+            s = torch.tensor(src[:m], device="cuda", dtype=torch.long)
+            to = torch.arange(m, device="cuda")
+            assert torch.equal(r["weights"][i, j, :m].view(torch.int32), w0[i, j][s].view(torch.int32))
+            assert torch.equal(r["positions"][i, j, :m], p0[i, j][s])
+            rest = (w0[i, j, m:], p0[i, j, m:]) if in_place else (torch.full_like(w0[i, j, m:], 8.0), torch.full_like(p0[i, j, m:], 8))
+            assert torch.equal(r["weights"][i, j, m:].view(torch.int32), rest[0].view(torch.int32))
+            assert torch.equal(r["positions"][i, j, m:], rest[1])
+            k_want[t[to // size], to % size, j] = k0[t[s // size], s % size, j]
+            v_want[t[to // size], to % size, j] = v0[t[s // size], s % size, j]
+    assert torch.equal(kp, k_want) and torch.equal(vp, v_want)
+    assert ln.tolist() == ([min(n, budget) for n in lens] if in_place else lens)
+
+
+@gpu
+@pytest.mark.parametrize("dt, d", [(BF, 37), (FP, 5), (FP, 64)])
+def test_evict_long_rows_and_any_row_width(dt, d):
+    """More slots than shared memory holds keys of; rows copied element by element."""
+    from project_chronos_b200 import ops
+    n, g, size, budget = 60001, 1, 64, 20000
+    width = -(-n // size)
+    table = torch.randperm(width, generator=_gen(1), device="cuda").view(1, width).to(torch.int32)
+    kp = torch.randn(width, size, g, d, generator=_gen(2), device="cuda").to(dt)
+    vp = torch.randn(width, size, g, d, generator=_gen(3), device="cuda").to(dt)
+    w = torch.rand(1, g, width * size, generator=_gen(4), device="cuda")
+    pos = torch.arange(width * size, dtype=torch.int32, device="cuda").view(1, 1, -1).contiguous()
+    ln = torch.tensor([n], dtype=torch.int32, device="cuda")
+    k0, v0 = kp.clone(), vp.clone()
+    r = ops.paged_evict(kp, vp, table, ln, ln, w, pos, budget, sinks=3, recent=99, weights_out=torch.empty_like(w),
+                        positions_out=torch.empty_like(pos))
+    src = _evict_plan(w[0, 0].tolist(), pos[0, 0].tolist(), n, n, budget, 3, 99)
+    assert r["src"][0, 0].tolist() == src
+    s, to, t = torch.tensor(src, device="cuda"), torch.arange(budget, device="cuda"), table[0].long()
+    assert torch.equal(kp[t[to // size], to % size], k0[t[s // size], s % size])
+    assert torch.equal(vp[t[to // size], to % size], v0[t[s // size], s % size])
+
+
+# ---------------------------------------------------------------------------------------
+# prompt attention
+# ---------------------------------------------------------------------------------------
+
+def _check_prompt(got, lse, q, k, v, lq, lk, cq, ck, window, sinks, dt, rows=None):
+    h, d = q.shape[1], q.shape[2]
+    for i in (range(lq) if rows is None else rows):
+        t = lk - lq + i
+        seen = _visible(lk, window, sinks, "cuda", at=t)
+        ref, rl, _, a, f = _attend(q[cq + i], k[ck: ck + lk], v[ck: ck + lk], d ** -0.5, seen)
+        _check_out(got[cq + i], ref, a, f, lk, dt)
+        if lse is not None:
+            _check_lse(lse[cq + i], rl, f)
+
+
+def _some_rows(n):
+    return sorted({i for i in (0, 1, 2, n // 3, n // 2, n - 2, n - 1, 31, 32, 63, 64, 127, 128, 129, 255, 256) if 0 <= i < n})
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("h, g, d", [(8, 2, 128), (4, 4, 64), (6, 2, 80), (5, 1, 128), (16, 1, 96), (2, 1, 256), (3, 1, 37),
+                                     (32, 2, 64), (4, 2, 8)])
+@pytest.mark.parametrize("lq, past", [([1, 130, 0, 64, 300], [0, 0, 0, 0, 0]), ([3, 129, 40], [500, 1, 127]), ([9, 200], [-4, -150])])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (50, 0), (130, 5), (1, 0), (40, 200)])
+def test_prompt_attention_matches_its_definition(dt, h, g, d, lq, past, window, sinks):
+    from project_chronos_b200 import ops
+    lk = [max(0, a + b) for a, b in zip(lq, past)]
+    pad = 3
+    tq, tk = sum(lq) + pad, sum(lk) + pad
+    gen = _gen(h + d)
+    q = (2 * torch.randn(tq, h, d, generator=gen, device="cuda")).to(dt)
+    k = torch.randn(tk, g, d, generator=gen, device="cuda").to(dt)
+    v = torch.randn(tk, g, d, generator=gen, device="cuda").to(dt)
+    q[sum(lq):], k[sum(lk):], v[sum(lk):] = math.nan, math.nan, math.inf
+    cq = [0] + torch.tensor(lq).cumsum(0).tolist()
+    ck = [0] + torch.tensor(lk).cumsum(0).tolist()
+    out = torch.full_like(q, 5.0)
+    lse = torch.full((tq, h), 5.0, device="cuda")
+    ops.window_attention(q, k, v, torch.tensor(cq, dtype=torch.int32, device="cuda"),
+                         cu_seqlens_k=torch.tensor(ck, dtype=torch.int32, device="cuda"), window=window, sinks=sinks,
+                         out=out, lse=lse)
+    ops.check_status(q.device)
+    assert bool((out[sum(lq):] == 5.0).all()) and bool((lse[sum(lq):] == 5.0).all())
+    for b in range(len(lq)):
+        _check_prompt(out, lse, q, k, v, lq[b], lk[b], cq[b], ck[b], window, sinks, dt, _some_rows(lq[b]))
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (300, 4), (1000, 130)])
+def test_long_prompt_every_tile(dt, window, sinks):
+    """Many key tiles per row; every row against the definition, in blocks."""
+    from project_chronos_b200 import ops
+    n, h, g, d = 2100, 4, 1, 128
+    gen = _gen(window)
+    qkv = torch.randn(n, h + 2 * g, d, generator=gen, device="cuda")
+    qkv[:, :h] *= 3
+    qkv = qkv.to(dt)
+    q, k, v = qkv[:, :h], qkv[:, h: h + g], qkv[:, h + g:]
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    lse = torch.empty(n, h, device="cuda")
+    out = ops.window_attention(q, k, v, cu, window=window, sinks=sinks, lse=lse)
+    assert torch.equal(out, ops.window_attention(q, k, v, cu, window=window, sinks=sinks))
+    t, j = torch.arange(n, device="cuda")[:, None], torch.arange(n, device="cuda")[None]
+    seen = j <= t
+    if window:
+        seen = seen & ((j > t - window) | (j < sinks))
+    kd, vd = k[:, 0].double(), v[:, 0].double()
+    for hh in range(h):
+        x = (q[:, hh].double() @ kd.T * d ** -0.5).masked_fill(~seen, -math.inf)
+        rl = torch.logsumexp(x, 1)
+        p = torch.exp(x - rl[:, None])
+        s = (q[:, hh].double().abs() @ kd.abs().T * d ** -0.5).amax(1)
+        f = d * 2.0 ** -23 * s + n * 2.0 ** -24 + 2.0 ** -20
+        _check_out(out[:, hh], p @ vd, p @ vd.abs(), f, n, dt)
+        _check_lse(lse[:, hh], rl, f)
+
+
+@gpu
+@pytest.mark.parametrize("dt, d", [(BF, 128), (HF, 64), (FP, 64)])
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_hidden_values_do_not_reach_a_row(dt, d, what):
+    """Keys and values that are not finite, at places that some rows see and others do not."""
+    from project_chronos_b200 import ops
+    n, h, g, window, sinks = 700, 4, 2, 200, 3
+    gen = _gen(d)
+    q = torch.randn(n, h, d, generator=gen, device="cuda").to(dt)
+    k = torch.randn(n, g, d, generator=gen, device="cuda").to(dt)
+    v = torch.randn(n, g, d, generator=gen, device="cuda").to(dt)
+    at = 300
+    v[at, :, 5] = what
+    k[at + 1, 0, 7] = math.nan
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    out = ops.window_attention(q, k, v, cu, window=window, sinks=sinks)
+    for i in (0, 100, 250, 298, 299):                     # before: finite and right
+        _check_prompt(out, None, q, k, v, n, n, 0, 0, window, sinks, dt, [i])
+    for i in (at + window + 1, 600, n - 1):               # behind the window again
+        _check_prompt(out, None, q, k, v, n, n, 0, 0, window, sinks, dt, [i])
+    for i in (at + 1, at + 60, at + 130, at + window - 1):   # they see it
+        group1 = out[i, h // g:]
+        assert bool(torch.isnan(out[i, : h // g]).all())
+        assert not bool(torch.isfinite(group1[:, 5]).any())
+        assert bool(torch.isfinite(group1[:, :5]).all()) and bool(torch.isfinite(group1[:, 6:]).all())
+
+
+@gpu
+def test_prompt_attention_refuses_wrong_tensors():
+    from project_chronos_b200 import _native as N
+    from project_chronos_b200 import ops
+    q, k = torch.zeros(9, 4, 64, dtype=BF, device="cuda"), torch.zeros(9, 2, 64, dtype=BF, device="cuda")
+    cu = torch.tensor([0, 9], dtype=torch.int32, device="cuda")
+    ok = dict(q=q, k=k, v=k, cu_seqlens=cu)
+    for change in (dict(k=k.half()), dict(v=k[:8]), dict(k=k[:8], v=k[:8]), dict(q=q[..., :32]), dict(cu_seqlens=cu.long()),
+                   dict(cu_seqlens_k=cu[:1]), dict(out=q.float()), dict(lse=torch.zeros(9, 3, device="cuda")),
+                   dict(v=k.cpu()), dict(cu_seqlens=cu[:0])):
+        with pytest.raises((TypeError, ValueError)):
+            ops.window_attention(**{**ok, **change})
+    with pytest.raises(RuntimeError, match="heads"):
+        ops.window_attention(**{**ok, "q": q[:, :3]})
+    with pytest.raises(RuntimeError, match="forward-only"):
+        ops.window_attention(**{**ok, "k": k.clone().requires_grad_()})
+    # offsets that leave the tensors: reported, nothing outside is read or written
+    for bad in ([0, 12], [5, 20], [-3, 6]):
+        ops.window_attention(q, k, k, torch.tensor(bad, dtype=torch.int32, device="cuda"))
+        with pytest.raises(N.ChronosMoeError, match="INVALID_ARG"):
+            ops.check_status(q.device)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_calls_follow_the_current_stream(dt):
+    from project_chronos_b200 import ops
+    n, h, g, d = 400, 4, 2, 64
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        torch.cuda._sleep(20_000_000)
+        q = torch.randn(n, h, d, device="cuda").to(dt)
+        k, v = torch.randn(n, g, d, device="cuda").to(dt), torch.randn(n, g, d, device="cuda").to(dt)
+        cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        out = ops.window_attention(q, k, v, cu)
+        kp, vp = torch.zeros(30, 16, g, d, dtype=dt, device="cuda"), torch.zeros(30, 16, g, d, dtype=dt, device="cuda")
+        table = torch.arange(30, dtype=torch.int32, device="cuda").view(1, 30)
+        ops.paged_append(k, v, kp, vp, table, torch.zeros(1, dtype=torch.int32, device="cuda"), cu_seqlens=cu)
+        one = ops.paged_attn_decode(q[n - 1:], kp, vp, table, torch.full((1,), n, dtype=torch.int32, device="cuda"))
+    st.synchronize()
+    _check_prompt(out, None, q, k, v, n, n, 0, 0, 0, 0, dt, [0, 200, n - 1])
+    ref, _, _, a, f = _attend(q[n - 1], k, v, d ** -0.5, _visible(n, 0, 0, "cuda"))
+    _check_out(one[0], ref, a, f, n, dt)
+
+
+# ---------------------------------------------------------------------------------------
+# together: prompt, append, decode steps with running sums, eviction, more steps
+# ---------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_a_serving_run(dt):
+    """A ragged batch is prefilled, decoded, evicted to a budget every few steps; a list
+    of the rows that should be there is kept per (sequence, kv head) in 64 bits."""
+    from project_chronos_b200 import ops
+    h, g, d, size, budget, sinks, recent = 8, 2, 64, 16, 48, 2, 16
+    prompts, steps = [70, 5, 33], 24
+    b = len(prompts)
+    gen = _gen(77)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device="cuda").to(dt)  # noqa: E731
+    width = 8
+    kp, vp = (torch.full((b * width, size, g, d), math.nan, dtype=dt, device="cuda") for _ in range(2))
+    table = torch.randperm(b * width, generator=gen, device="cuda").view(b, width).to(torch.int32)
+    w = torch.full((b, g, width * size), math.nan, device="cuda")
+    pos = torch.full((b, g, width * size), -1, dtype=torch.int32, device="cuda")
+    lens, seen = (torch.zeros(b, dtype=torch.int32, device="cuda") for _ in range(2))
+    t = sum(prompts)
+    cu = torch.tensor([0] + torch.tensor(prompts).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+    q, k, v = rnd(t, h, d), rnd(t, g, d), rnd(t, g, d)
+    out = ops.window_attention(q, k, v, cu)
+    for i, n in enumerate(prompts):
+        _check_prompt(out, None, q, k, v, n, n, int(cu[i]), int(cu[i]), 0, 0, dt, _some_rows(n))
+    ops.paged_append(k, v, kp, vp, table, lens, cu_seqlens=cu, seen=seen, weights=w, positions=pos)
+    lens += cu.diff()
+    seen += cu.diff()
+    book = [[[[k[int(cu[i]) + j, x], v[int(cu[i]) + j, x], 0.0, j] for j in range(prompts[i])] for x in range(g)]
+            for i in range(b)]
+    for step in range(steps):
+        q, k, v = rnd(b, h, d), rnd(b, g, d), rnd(b, g, d)
+        ops.paged_append(k, v, kp, vp, table, lens, seen=seen, weights=w, positions=pos)
+        lens += 1
+        seen += 1
+        out = ops.paged_attn_decode(q, kp, vp, table, lens, weights=w)
+        for i in range(b):
+            for x in range(g):
+                rows = book[i][x]
+                rows.append([k[i, x], v[i, x], 0.0, int(seen[i]) - 1])
+                ks, vs = torch.stack([r[0] for r in rows])[:, None], torch.stack([r[1] for r in rows])[:, None]
+                part = slice(x * h // g, (x + 1) * h // g)
+                ref, _, p, a, f = _attend(q[i, part], ks, vs, d ** -0.5, _visible(len(rows), 0, 0, "cuda"))
+                _check_out(out[i, part], ref, a, f, len(rows), dt)
+                for r, y in zip(rows, p.sum(0).tolist()):
+                    r[2] += y
+        if step % 5 == 4:
+            # the kernel's own sums decide (they differ from the 64-bit ones by rounding); they are checked first
+            for i in range(b):
+                for x in range(g):
+                    mine = torch.tensor([r[2] for r in book[i][x]], device="cuda", dtype=torch.float64)
+                    got = w[i, x, : len(mine)].double()
+                    assert bool(((got - mine).abs() <= 1e-3 * mine).all())   # up to 24 steps of f <= D 2^-23 S each
+            plans = [[_evict_plan(w[i, x].tolist(), pos[i, x].tolist(), int(lens[i]), int(seen[i]), budget, sinks, recent)
+                      for x in range(g)] for i in range(b)]
+            r = ops.paged_evict(kp, vp, table, lens, seen, w, pos, budget, sinks=sinks, recent=recent, lens_out=lens)
+            for i in range(b):
+                for x in range(g):
+                    assert r["src"][i, x].tolist() == plans[i][x]
+                    book[i][x] = [book[i][x][j] for j in plans[i][x] if j >= 0]
+                    assert [y[3] for y in book[i][x]] == pos[i, x, : len(book[i][x])].tolist()
+    ops.check_status(kp.device)
