@@ -208,8 +208,66 @@ int launch_window_simt(const WindowParams& p, cudaStream_t st) {
     return CHRONOS_OK;
 }
 
+// Tensor map of rows of 16-bit vectors: `dims` outermost last, `strides` in
+// elements (of dims[1..]), box of 64 elements by box[1..], 128-byte swizzle.
+bool encode_rows(CUtensorMap* m, int dtype, const void* base, int rank, const uint64_t* dims, const int64_t* strides,
+                 const uint32_t* box) {
+    EncodeTiledFn enc = get_encode_fn();
+    if (enc == nullptr) return false;
+    cuuint64_t d[4], s[3];
+    cuuint32_t b[4], e[4] = {1, 1, 1, 1};
+    for (int i = 0; i < rank; ++i) {
+        d[i] = dims[i];
+        b[i] = box[i];
+        if (i > 0) s[i - 1] = static_cast<cuuint64_t>(strides[i - 1]) * 2;
+    }
+    return enc(m, dtype == CHRONOS_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+               static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// What the loads and the 16-byte stores of the tensor-core path need.
+bool window_uses_tc(const WindowParams& p) {
+    return p.dim % 8 == 0 && p.dim <= 128 && p.num_k > 0 && aligned(p.q, 16) && aligned(p.k, 16) && aligned(p.v, 16) &&
+           aligned(p.out, 16) &&
+           multiples(8, {p.q_row, p.q_head, p.k_row, p.k_head, p.v_row, p.v_head, p.o_row, p.o_head});
+}
+
+template <typename T, int DP>
+int launch_window_tc(const WindowParams& p, int dtype, bool* taken, cudaStream_t st) {
+    // rows of a block: the query heads of a kv head side by side where their number divides a tile
+    int rp_log2 = 0;
+    if ((p.rep & (p.rep - 1)) == 0 && p.rep <= 16)
+        while ((1 << rp_log2) < p.rep) ++rp_log2;
+    const int rp = 1 << rp_log2, groups = p.heads / rp;
+    const uint64_t dq[4] = {static_cast<uint64_t>(p.dim), static_cast<uint64_t>(rp), static_cast<uint64_t>(groups),
+                            static_cast<uint64_t>(p.num_q)};
+    const uint64_t dk[3] = {static_cast<uint64_t>(p.dim), static_cast<uint64_t>(p.kv_heads), static_cast<uint64_t>(p.num_k)};
+    const int64_t sq[3] = {p.q_head, p.q_head * rp, p.q_row}, sk[2] = {p.k_head, p.k_row}, sv[2] = {p.v_head, p.v_row};
+    const uint32_t bq[4] = {64, static_cast<uint32_t>(rp), 1, static_cast<uint32_t>(128 / rp)}, bk[3] = {64, 1, kWtKeys};
+    CUtensorMap mq, mk, mv;
+    *taken = encode_rows(&mq, dtype, p.q, 4, dq, sq, bq) && encode_rows(&mk, dtype, p.k, 3, dk, sk, bk) &&
+             encode_rows(&mv, dtype, p.v, 3, dk, sv, bk);
+    if (!*taken) return CHRONOS_OK;   // strides the maps cannot hold
+    using C = WindowTc<DP>;
+    if (int rc = set_smem(window_tc_kernel<T, DP>, C::kSmem)) return rc;
+    const int tokens = 256 / rp;
+    const int64_t tiles = (p.num_q + tokens - 1) / tokens + p.batch;
+    CHRONOS_CUDA_CHECK(launch_kernel(window_tc_kernel<T, DP>, dim3(static_cast<unsigned>(tiles * groups)), dim3(kWtThreads),
+                                     C::kSmem, st, false, p, mq, mk, mv, rp_log2, groups));
+    return CHRONOS_OK;
+}
+
 template <typename T>
-int window_impl(const WindowParams& p, cudaStream_t st) {
+int window_impl(const WindowParams& p, int dtype, cudaStream_t st) {
+    if constexpr (sizeof(T) == 2) {
+        if (window_uses_tc(p)) {
+            bool taken = false;
+            const int rc = p.dim <= 64 ? launch_window_tc<T, 64>(p, dtype, &taken, st) : launch_window_tc<T, 128>(p, dtype, &taken, st);
+            if (rc || taken) return rc;
+        }
+    }
     return launch_window_simt<T>(p, st);
 }
 
@@ -445,9 +503,9 @@ extern "C" int chronos_window_attention(const ChronosWindowAttnArgs* a, void* st
     p.status = a->status;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (a->dtype) {
-        case CHRONOS_DTYPE_BF16: return window_impl<__nv_bfloat16>(p, st);
-        case CHRONOS_DTYPE_FP16: return window_impl<__half>(p, st);
-        default: return window_impl<float>(p, st);
+        case CHRONOS_DTYPE_BF16: return window_impl<__nv_bfloat16>(p, a->dtype, st);
+        case CHRONOS_DTYPE_FP16: return window_impl<__half>(p, a->dtype, st);
+        default: return window_impl<float>(p, a->dtype, st);
     }
 }
 

@@ -243,4 +243,466 @@ __global__ void __launch_bounds__(kWsThreads) window_simt_kernel(const __grid_co
     }
 }
 
+// ---------------------------------------------------------------------------
+// tensor-core path: bf16 / fp16, head_dim a multiple of 8 up to 128
+// ---------------------------------------------------------------------------
+// Bound: the tensor cores (4 D flops per visible pair and head) and, as closely,
+// the 16 exponentials a cycle of an SM's special-function units.  A block holds
+// 256 query rows as two tiles of 128, each with a warpgroup of its own, so one
+// tile's exponentials run while the other's products do.  Accumulators live in
+// TMEM: scores S (128 columns per tile), over which the weights P are written in
+// the layer type as the first operand of the second product, and the output O
+// (DP columns per tile).  A row belongs to one thread, so its maximum and sum
+// need no exchange.  With several query heads per kv head (a power of two up to
+// 16) the 256 rows are 256 / rep tokens times rep heads: keys and values are
+// loaded once for all of them, and a window has fewer tiles with hidden pairs.
+//
+//   warps 0-3, 4-7   softmax of tile 0 / 1, rescaling of O, output
+//   warp 8           TMA loads of Q, K, V (128-byte swizzle, no multicast)
+//   warp 9           tcgen05.mma issue, TMEM allocation
+//   warps 10, 11     V tiles with hidden keys: rows behind the sequence become
+//                    zero (0 * NaN would reach every row), and so do rows that
+//                    are not finite, in which case the block computes its rows
+//                    again pair by pair at the end
+//
+// O is rescaled only when a row's maximum grew by more than 2^8 in weight: until
+// then weights are taken against the older maximum, at most 256 times too large,
+// which the fp32 sums and both 16-bit formats hold without loss.
+constexpr int kWtThreads = 384;
+constexpr int kWtKeys = 128;
+constexpr float kWtRescaleLog2 = 8.0f;
+constexpr uint64_t kWtLimitNs = 2000000000ull;
+
+template <int DP>
+struct WindowTc {
+    static constexpr int kHalves = DP / 64;
+    static constexpr int kTileBytes = 128 * DP * 2;         // 128 rows of K, V or Q
+    static constexpr int kStages = DP == 64 ? 3 : 2;        // of K and of V
+    static constexpr int kBarriers = 1 + 5 * kStages + 2 + 2 + 2 + 1;
+    static constexpr int kSmem = 1024 + (2 + 2 * kStages) * kTileBytes + 8 * kBarriers + 32;
+    static constexpr int kSCol = 0, kOCol = 256;            // S of tile w at 128 w, O at 256 + DP w
+};
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+            "r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+}
+
+// D[tmem] (+)= A[tmem] * B[smem desc], kind::f16.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Descriptor of an operand stored along its N dimension (128-byte swizzle: rows
+// of 64 elements along N, one row per k, atoms of 8 rows = 1024 bytes): leading
+// byte offset between 64-element groups of N, stride byte offset between groups
+// of 8 k.
+__device__ __forceinline__ uint64_t sdesc_mn_sw128(uint32_t smem_addr, uint32_t group_bytes) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>((group_bytes >> 4) & 0x3FFFu) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One row pair by pair (a whole warp): only visible keys are touched.
+template <typename T>
+__device__ __noinline__ void window_row_exact(const WindowParams& p, const WindowTile& t, int token, int head, int lane) {
+    const int tr = t.lk - t.lq + token;
+    const T* q = static_cast<const T*>(p.q) + (t.q0 + token) * p.q_row + head * p.q_head;
+    const T* k = static_cast<const T*>(p.k) + t.k0 * p.k_row + (head / p.rep) * p.k_head;
+    const T* v = static_cast<const T*>(p.v) + t.k0 * p.v_row + (head / p.rep) * p.v_head;
+    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int lo = p.window > 0 ? max(0, tr - p.window + 1) : 0;
+    const int first = min(p.sinks, lo);
+    for (int i = 0; i < first + tr + 1 - lo; ++i) {
+        const int64_t j = i < first ? i : lo + i - first;
+        float x = 0.0f;
+        for (int d = lane; d < p.dim; d += 32) x = fmaf(to_f32<T>(q[d]), to_f32<T>(k[j * p.k_row + d]), x);
+        x = warp_sum(x) * p.sl2;
+        const float n = fmaxf(m, x), u = n == -INFINITY ? 0.0f : n;
+        const float c = exp2_fast(m - u), e = exp2_fast(x - u);
+        m = n;
+        l = l * c + e;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const int d = lane + 32 * a;
+            if (d < p.dim) o[a] = fmaf(e, to_f32<T>(v[j * p.v_row + d]), o[a] * c);
+        }
+    }
+    const float inv = l > 0.0f ? 1.0f / l : l;
+    T* out = static_cast<T*>(p.out) + (t.q0 + token) * p.o_row + head * p.o_head;
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+        if (lane + 32 * a < p.dim) out[lane + 32 * a] = from_f32<T>(o[a] * inv);
+    if (lane == 0 && p.lse != nullptr)
+        p.lse[(t.q0 + token) * p.heads + head] = l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+}
+
+template <typename T>
+__device__ __forceinline__ bool any_not_finite(const uint4& u) {
+    constexpr uint32_t E = sizeof(T) == 2 && AbFormat<T>::value == 1 ? 0x7f80u : 0x7c00u;
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (w[i] & E) == E || (w[i] & (E << 16)) == (E << 16);
+    return bad;
+}
+
+// rp: heads per row group (1 << rp_log2), the query heads of one kv head or 1.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_constant__ WindowParams p,
+                                                                  const __grid_constant__ CUtensorMap tm_q,
+                                                                  const __grid_constant__ CUtensorMap tm_k,
+                                                                  const __grid_constant__ CUtensorMap tm_v, int rp_log2,
+                                                                  int groups) {
+    using C = WindowTc<DP>;
+    constexpr int NS = C::kStages;
+    extern __shared__ uint8_t dyn[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int hg = blockIdx.x % groups;
+    const int tokens = 256 >> rp_log2;            // tokens of the block
+    WindowTile t;
+    if (!window_tile(p, blockIdx.x / groups, tokens, lane, t)) return;
+    const int rows = min(tokens, t.lq - t.m0);
+    const int t0 = t.lk - t.lq + t.m0;            // position of the first token
+    const int hi = min(t.lk, t0 + rows);          // keys [lo, hi) and the first ones
+    const int lo = p.window > 0 ? max(0, t0 - p.window + 1) : 0;
+    const int ns = p.window > 0 ? (max(0, min(p.sinks, hi)) + kWtKeys - 1) / kWtKeys : 0;
+    const int w0 = max(ns * kWtKeys, lo);
+    const int nt = ns + (hi > w0 ? (hi - w0 + kWtKeys - 1) / kWtKeys : 0);
+    auto tile_base = [&](int i) { return i < ns ? i * kWtKeys : w0 + (i - ns) * kWtKeys; };
+
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~uintptr_t{1023});
+    uint8_t* s_q = smem;
+    uint8_t* s_k = s_q + 2 * C::kTileBytes;
+    uint8_t* s_v = s_k + NS * C::kTileBytes;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + NS * C::kTileBytes);
+    uint64_t* q_full = bars;
+    uint64_t* k_full = q_full + 1;
+    uint64_t* k_empty = k_full + NS;
+    uint64_t* v_full = k_empty + NS;
+    uint64_t* v_ok = v_full + NS;
+    uint64_t* v_empty = v_ok + NS;
+    uint64_t* s_full = v_empty + NS;              // [2]
+    uint64_t* p_ready = s_full + 2;               // [2]
+    uint64_t* o_done = p_ready + 2;               // [2]
+    uint64_t* drained = o_done + 2;
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drained + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(s_tmem + 1);
+    volatile int* not_finite = abort_flag + 1;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(k_full + i, 1);
+            mbar_init(k_empty + i, 1);
+            mbar_init(v_full + i, 1);
+            mbar_init(v_ok + i, 2);
+            mbar_init(v_empty + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full + i, 1);
+            mbar_init(p_ready + i, 4);
+            mbar_init(o_done + i, 1);
+        }
+        mbar_init(drained, 1);
+        *abort_flag = 0;
+        *not_finite = 0;
+        fence_mbar_init();
+    }
+    if (warp == 9) {
+        tmem_alloc(s_tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (mbar_wait_bounded(bar, parity, kWtLimitNs, const_cast<volatile int*>(abort_flag))) return true;
+        *abort_flag = 1;
+        report_status(p.status, CHRONOS_ERR_PIPELINE_TIMEOUT);
+        return false;
+    };
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 8 && lane == 0 && nt > 0) {
+            // ------------------------------ loads ------------------------------
+            const int g = groups == p.kv_heads ? hg : hg / p.rep;
+            mbar_arrive_expect_tx(q_full, 2 * C::kTileBytes);
+            for (int w = 0; w < 2; ++w)
+                for (int h = 0; h < C::kHalves; ++h)
+                    tma_load_4d(s_q + w * C::kTileBytes + h * 16384, &tm_q, q_full, h * 64, 0, hg,
+                                static_cast<int>(t.q0 + t.m0 + w * (128 >> rp_log2)));
+            int i = 0;
+            for (; i < nt; ++i) {
+                const int st = i % NS;
+                const uint32_t ph = (i / NS) & 1;
+                const int row = static_cast<int>(t.k0 + tile_base(i));
+                if (!wait(k_empty + st, ph ^ 1u)) break;
+                mbar_arrive_expect_tx(k_full + st, C::kTileBytes);
+                for (int h = 0; h < C::kHalves; ++h)
+                    tma_load_3d(s_k + st * C::kTileBytes + h * 16384, &tm_k, k_full + st, h * 64, g, row);
+                if (!wait(v_empty + st, ph ^ 1u)) {
+                    ++i;   // this tile's K copy is in flight (its V barrier is not waited for below)
+                    break;
+                }
+                mbar_arrive_expect_tx(v_full + st, C::kTileBytes);
+                for (int h = 0; h < C::kHalves; ++h)
+                    tma_load_3d(s_v + st * C::kTileBytes + h * 16384, &tm_v, v_full + st, h * 64, g, row);
+            }
+            if (*abort_flag) {
+                // the copies in flight land before the block's shared memory is given up
+                volatile int go = 0;
+                mbar_wait_bounded(q_full, 0, kWtLimitNs, &go);
+                for (int j = max(0, i - NS); j < i; ++j) {
+                    mbar_wait_bounded(k_full + j % NS, (j / NS) & 1, kWtLimitNs, &go);
+                    mbar_wait_bounded(v_full + j % NS, (j / NS) & 1, kWtLimitNs, &go);
+                }
+            }
+        } else if (warp == 9 && lane == 0 && nt > 0) {
+            // ------------------------------ products ------------------------------
+            constexpr uint32_t ID_QK = idesc_f16(128, kWtKeys, AbFormat<T>::value);
+            constexpr uint32_t ID_PV = idesc_f16(128, DP, AbFormat<T>::value) | (1u << 16);   // B along N
+            auto qk = [&](int w, int st) {
+                const uint32_t a = smem_u32(s_q + w * C::kTileBytes), b = smem_u32(s_k + st * C::kTileBytes);
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk) {
+                    const uint32_t off = (kk / 4) * 16384 + (kk % 4) * 32;
+                    umma_f16(tmem + C::kSCol + 128 * w, sdesc_k_sw128(a + off), sdesc_k_sw128(b + off), ID_QK, kk > 0);
+                }
+                umma_commit(s_full + w);
+            };
+            auto pv = [&](int w, int st, bool first) {
+                const uint32_t b = smem_u32(s_v + st * C::kTileBytes);
+#pragma unroll
+                for (int kk = 0; kk < kWtKeys / 16; ++kk)
+                    umma_f16_ts(tmem + C::kOCol + DP * w, tmem + C::kSCol + 128 * w + kk * 8,
+                                sdesc_mn_sw128(b + kk * 2048, 16384), ID_PV, !first || kk > 0);
+            };
+            bool ok = wait(q_full, 0) && wait(k_full, 0);
+            if (ok) {
+                tc_fence_after();
+                qk(0, 0);
+                qk(1, 0);
+                umma_commit(k_empty);
+            }
+            // the weights of tile w overwrite its scores: the next scores are issued behind the product
+            // that reads them, and products of one thread run in order
+            for (int i = 0; i < nt && ok; ++i) {
+                const int st = i % NS, sn = (i + 1) % NS;
+                const bool more = i + 1 < nt;
+                ok = wait(v_ok + st, (i / NS) & 1) && (!more || wait(k_full + sn, ((i + 1) / NS) & 1));
+                for (int w = 0; w < 2 && ok; ++w) {
+                    ok = wait(p_ready + w, i & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    pv(w, st, i == 0);
+                    if (w == 1) umma_commit(v_empty + st);
+                    if (more) qk(w, sn);
+                    else umma_commit(o_done + w);
+                }
+                if (ok && more) umma_commit(k_empty + sn);
+            }
+            if (!ok) {
+                volatile int go = 0;
+                umma_commit(drained);
+                mbar_wait_bounded(drained, 0, kWtLimitNs, &go);
+            }
+        } else if (warp >= 10) {
+            // ------------------------------ V tiles with hidden keys ------------------------------
+            const int tl = hi - 1;   // position of the last token (or the last key)
+            for (int i = 0; i < nt; ++i) {
+                const int st = i % NS, base = tile_base(i);
+                if (!wait(v_full + st, (i / NS) & 1)) break;
+                if (base + kWtKeys - 1 > t0 || (p.window > 0 && base <= tl - p.window)) {
+                    const int n = t.lk - base;   // keys of the sequence in this tile
+                    for (int r = threadIdx.x - 320; r < kWtKeys; r += 64) {
+                        uint8_t* row = s_v + st * C::kTileBytes + r * 128;
+                        bool zero = r >= n;
+                        if (!zero) {
+                            bool bad = false;
+#pragma unroll 4
+                            for (int c = 0; c < 8 * C::kHalves; ++c)
+                                bad |= any_not_finite<T>(*reinterpret_cast<const uint4*>(
+                                    row + (c >> 3) * 16384 + (((c + r) & 7) << 4)));
+                            if (bad) *not_finite = 1;
+                            zero = bad;
+                        }
+                        if (zero)
+#pragma unroll 4
+                            for (int c = 0; c < 8 * C::kHalves; ++c)
+                                *reinterpret_cast<uint4*>(row + (c >> 3) * 16384 + (((c + r) & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_ok + st);
+            }
+            __syncwarp();
+            asm volatile("bar.arrive 2, 320;" ::: "memory");
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        // ------------------------------ softmax and output ------------------------------
+        const int w = warp >> 2;
+        const int r = (warp & 3) * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lanes + C::kSCol + 128 * w, to = tmem + lanes + C::kOCol + DP * w;
+        const int per = 128 >> rp_log2;
+        const int local = w * per + (r >> rp_log2);          // token within the block
+        const int head = (hg << rp_log2) + (r & ((1 << rp_log2) - 1));
+        const int tr = t0 + local;                            // this row's position
+        const int ta = t0 + w * per, tb = min(ta + per, hi) - 1;   // the tile's first and last positions
+        float m = -INFINITY, l = 0.0f;
+        bool ok = true;
+        for (int i = 0; i < nt; ++i) {
+            ok = wait(s_full + w, i & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            float s[kWtKeys];
+#pragma unroll
+            for (int c = 0; c < kWtKeys; c += 32) tmem_ld32(ts + c, s + c);
+            tmem_wait_ld();
+            const int base = tile_base(i);
+            if (base + kWtKeys - 1 > ta || (p.window > 0 && base <= tb - p.window)) {
+                const int last = tr - base, from = p.window > 0 ? last - p.window + 1 : 0, first = p.sinks - base;
+#pragma unroll
+                for (int c = 0; c < kWtKeys; ++c)
+                    s[c] = c <= last && (c >= from || c < first) ? s[c] : -INFINITY;
+            }
+            float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int c = 4; c < kWtKeys; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+            const float n = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+            if (i == 0) {
+                m = n;
+            } else {
+                const bool grow = n > m && !((n - m) * p.sl2 <= kWtRescaleLog2);
+                if (__any_sync(0xffffffffu, grow)) {
+                    // the scores' barrier also covers the second product before them: O is complete
+                    const float f = grow ? exp2_fast((m - n) * p.sl2) : 1.0f;
+                    if (grow) m = n;
+                    l *= f;
+#pragma unroll
+                    for (int c = 0; c < DP; c += 32) {
+                        float o[32];
+                        tmem_ld32(to + c, o);
+                        tmem_wait_ld();
+                        uint32_t x[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(o[e] * f);
+                        tmem_st32(to + c, x);
+                    }
+                }
+            }
+            const float u = m == -INFINITY ? 0.0f : m * p.sl2;
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < kWtKeys; c += 64) {
+                uint32_t x[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const float a = exp2_fast(fmaf(s[c + 2 * e], p.sl2, -u)), b = exp2_fast(fmaf(s[c + 2 * e + 1], p.sl2, -u));
+                    sum[0] += a;
+                    sum[1] += b;
+                    x[e] = pack2<T>(a, b);   // weights in T for the second product; the sum keeps fp32
+                }
+                tmem_st32(ts + c / 2, x);
+            }
+            l += sum[0] + sum[1];
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_ready + w);
+        }
+        if (nt > 0 && ok) ok = __all_sync(0xffffffffu, wait(o_done + w, 0));
+        tc_fence_after();
+        const bool mine = ok && local < rows;
+        const int64_t qrow = t.q0 + t.m0 + local;
+        const float inv = l > 0.0f ? 1.0f / l : l;
+        T* out = static_cast<T*>(p.out) + qrow * p.o_row + head * p.o_head;
+#pragma unroll
+        for (int c = 0; c < DP; c += 32) {
+            float o[32];
+            if (nt > 0) {
+                tmem_ld32(to + c, o);
+                tmem_wait_ld();
+            }
+            if (mine)
+#pragma unroll
+                for (int e = 0; e < 32; e += 8)
+                    if (c + e < p.dim) {
+                        float x[8];
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) x[y] = nt > 0 ? o[e + y] * inv : 0.0f;
+                        store8<T>(out + c + e, x);
+                    }
+        }
+        if (mine && p.lse != nullptr)
+            p.lse[qrow * p.heads + head] = l != 0.0f ? ((m == -INFINITY ? 0.0f : m * p.sl2) + log2f(l)) * kLn2 : -INFINITY;
+        asm volatile("bar.sync 2, 320;" ::: "memory");
+        if (*not_finite && ok)
+            for (int x = warp; x < 256; x += 8) {
+                const int tok = x >> rp_log2;
+                if (tok < rows) window_row_exact<T>(p, t, t.m0 + tok, (hg << rp_log2) + (x & ((1 << rp_log2) - 1)), lane);
+            }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
 }  // namespace chronos
