@@ -338,18 +338,50 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+        "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+
+// Two fp32 operations per instruction, and the larger of three.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Bits 0..n-1 set (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t ones_below(int n) {
+    return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+}
 
 // One row pair by pair (a whole warp): only visible keys are touched.
 template <typename T>
@@ -472,7 +504,8 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
     };
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        // the block launched with 384 * 168 registers: 256 * 216 + 128 * 72
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 8 && lane == 0 && nt > 0) {
             // ------------------------------ loads ------------------------------
             const int g = groups == p.kv_heads ? hg : hg / p.rep;
@@ -590,7 +623,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
             asm volatile("bar.arrive 2, 320;" ::: "memory");
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         // ------------------------------ softmax and output ------------------------------
         const int w = warp >> 2;
         const int r = (warp & 3) * 32 + lane;
@@ -616,13 +649,18 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
             if (base + kWtKeys - 1 > ta || (p.window > 0 && base <= tb - p.window)) {
                 const int last = tr - base, from = p.window > 0 ? last - p.window + 1 : 0, first = p.sinks - base;
 #pragma unroll
-                for (int c = 0; c < kWtKeys; ++c)
-                    s[c] = c <= last && (c >= from || c < first) ? s[c] : -INFINITY;
+                for (int c = 0; c < kWtKeys; c += 32) {
+                    const uint32_t on = ones_below(last + 1 - c) & (~ones_below(from - c) | ones_below(first - c));
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) s[c + e] = (on >> e) & 1u ? s[c + e] : -INFINITY;
+                }
             }
             float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int c = 4; c < kWtKeys; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-            const float n = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+            for (int c = 4; c < kWtKeys - 4; c += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
+            const float n = fmaxf(max3(m, mx[0], mx[1]), max3(fmaxf(mx[2], mx[3]), fmaxf(s[124], s[125]), fmaxf(s[126], s[127])));
             if (i == 0) {
                 m = n;
             } else {
@@ -633,32 +671,33 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
                     if (grow) m = n;
                     l *= f;
 #pragma unroll
-                    for (int c = 0; c < DP; c += 32) {
-                        float o[32];
-                        tmem_ld32(to + c, o);
+                    for (int c = 0; c < DP; c += 16) {   // 16 columns at a time beside the 128 scores
+                        float o[16];
+                        tmem_ld16(to + c, o);
                         tmem_wait_ld();
-                        uint32_t x[32];
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(o[e] * f);
-                        tmem_st32(to + c, x);
+                        for (int e = 0; e < 16; ++e) o[e] *= f;
+                        tmem_st16(to + c, o);
                     }
                 }
             }
             const float u = m == -INFINITY ? 0.0f : m * p.sl2;
-            float sum[2] = {0.0f, 0.0f};
+            const float2 scale = make_float2(p.sl2, p.sl2), shift = make_float2(-u, -u);
+            float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-            for (int c = 0; c < kWtKeys; c += 64) {
-                uint32_t x[32];
+            for (int c = 0; c < kWtKeys; c += 32) {
+                uint32_t x[16];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const float a = exp2_fast(fmaf(s[c + 2 * e], p.sl2, -u)), b = exp2_fast(fmaf(s[c + 2 * e + 1], p.sl2, -u));
-                    sum[0] += a;
-                    sum[1] += b;
-                    x[e] = pack2<T>(a, b);   // weights in T for the second product; the sum keeps fp32
+                for (int e = 0; e < 16; ++e) {
+                    float2 a = fma2(make_float2(s[c + 2 * e], s[c + 2 * e + 1]), scale, shift);
+                    a.x = exp2_fast(a.x);
+                    a.y = exp2_fast(a.y);
+                    sum[e & 1] = add2(sum[e & 1], a);
+                    x[e] = pack2<T>(a.x, a.y);   // weights in T for the second product; the sum keeps fp32
                 }
-                tmem_st32(ts + c / 2, x);
+                tmem_st16u(ts + c / 2, x);
             }
-            l += sum[0] + sum[1];
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
