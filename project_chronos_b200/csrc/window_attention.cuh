@@ -278,7 +278,7 @@ struct WindowTc {
     static constexpr int kHalves = DP / 64;
     static constexpr int kTileBytes = 128 * DP * 2;         // 128 rows of K, V or Q
     static constexpr int kStages = DP == 64 ? 3 : 2;        // of K and of V
-    static constexpr int kBarriers = 1 + 5 * kStages + 2 + 2 + 2 + 1;
+    static constexpr int kBarriers = 1 + 5 * kStages + 2 + 4 + 2 + 1;
     static constexpr int kSmem = 1024 + (2 + 2 * kStages) * kTileBytes + 8 * kBarriers + 32;
     static constexpr int kSCol = 0, kOCol = 256;            // S of tile w at 128 w, O at 256 + DP w
 };
@@ -357,7 +357,16 @@ __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t* v) {
         : "memory");
 }
 
-// Two fp32 operations per instruction, and the larger of three.
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(p));
+    return p != 0;
+}
+
+// Two fp32 operations per instruction, and the largest of three (NaN if one is).
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 d;
     asm("fma.rn.f32x2 %0, %1, %2, %3;"
@@ -374,7 +383,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 
@@ -437,7 +446,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
     using C = WindowTc<DP>;
     constexpr int NS = C::kStages;
     extern __shared__ uint8_t dyn[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int hg = blockIdx.x % groups;
     const int tokens = 256 >> rp_log2;            // tokens of the block
     WindowTile t;
@@ -463,8 +472,8 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
     uint64_t* v_ok = v_full + NS;
     uint64_t* v_empty = v_ok + NS;
     uint64_t* s_full = v_empty + NS;              // [2]
-    uint64_t* p_ready = s_full + 2;               // [2]
-    uint64_t* o_done = p_ready + 2;               // [2]
+    uint64_t* p_ready = s_full + 2;               // [2][2]: tile, half of its keys
+    uint64_t* o_done = p_ready + 4;               // [2]
     uint64_t* drained = o_done + 2;
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(s_tmem + 1);
@@ -480,7 +489,8 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + i, 1);
-            mbar_init(p_ready + i, 4);
+            mbar_init(p_ready + 2 * i, 4);
+            mbar_init(p_ready + 2 * i + 1, 4);
             mbar_init(o_done + i, 1);
         }
         mbar_init(drained, 1);
@@ -497,6 +507,9 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
+        // the timer of the bounded wait costs more than most of these waits: look at it late
+        for (int i = 0; i < 256; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
         if (mbar_wait_bounded(bar, parity, kWtLimitNs, const_cast<volatile int*>(abort_flag))) return true;
         *abort_flag = 1;
         report_status(p.status, CHRONOS_ERR_PIPELINE_TIMEOUT);
@@ -540,51 +553,82 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
                     mbar_wait_bounded(v_full + j % NS, (j / NS) & 1, kWtLimitNs, &go);
                 }
             }
-        } else if (warp == 9 && lane == 0 && nt > 0) {
+        } else if (warp == 9 && nt > 0) {
             // ------------------------------ products ------------------------------
+            // The whole warp walks the loop and one elected lane issues: descriptors are
+            // one addition to a warp-uniform base.  (One lane alone building each
+            // descriptor took longer than the products themselves.)
             constexpr uint32_t ID_QK = idesc_f16(128, kWtKeys, AbFormat<T>::value);
             constexpr uint32_t ID_PV = idesc_f16(128, DP, AbFormat<T>::value) | (1u << 16);   // B along N
+            const bool leader = elect_one();
+            const uint64_t dq = sdesc_k_sw128(smem_u32(s_q)), dk = sdesc_k_sw128(smem_u32(s_k));
+            const uint64_t dv = sdesc_mn_sw128(smem_u32(s_v), 16384);
+            constexpr uint32_t TILE = C::kTileBytes >> 4;   // descriptors count 16 bytes
             auto qk = [&](int w, int st) {
-                const uint32_t a = smem_u32(s_q + w * C::kTileBytes), b = smem_u32(s_k + st * C::kTileBytes);
+                const uint64_t a = dq + w * TILE, b = dk + st * TILE;
+                if (leader) {
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk) {
-                    const uint32_t off = (kk / 4) * 16384 + (kk % 4) * 32;
-                    umma_f16(tmem + C::kSCol + 128 * w, sdesc_k_sw128(a + off), sdesc_k_sw128(b + off), ID_QK, kk > 0);
+                    for (int kk = 0; kk < DP / 16; ++kk) {
+                        constexpr int H = 16384 >> 4;
+                        umma_f16(tmem + C::kSCol + 128 * w, a + (kk / 4) * H + (kk % 4) * 2, b + (kk / 4) * H + (kk % 4) * 2,
+                                 ID_QK, kk > 0);
+                    }
+                    umma_commit(s_full + w);
                 }
-                umma_commit(s_full + w);
             };
-            auto pv = [&](int w, int st, bool first) {
-                const uint32_t b = smem_u32(s_v + st * C::kTileBytes);
+            auto pv = [&](int w, int st, int half, bool first) {
+                const uint64_t b = dv + st * TILE;
+                if (leader)
 #pragma unroll
-                for (int kk = 0; kk < kWtKeys / 16; ++kk)
-                    umma_f16_ts(tmem + C::kOCol + DP * w, tmem + C::kSCol + 128 * w + kk * 8,
-                                sdesc_mn_sw128(b + kk * 2048, 16384), ID_PV, !first || kk > 0);
+                    for (int kk = 0; kk < kWtKeys / 32; ++kk) {
+                        const int k = half * (kWtKeys / 32) + kk;
+                        umma_f16_ts(tmem + C::kOCol + DP * w, tmem + C::kSCol + 128 * w + k * 8, b + k * (2048 >> 4), ID_PV,
+                                    !first || k > 0);
+                    }
             };
-            bool ok = wait(q_full, 0) && wait(k_full, 0);
-            if (ok) {
+            auto until = [&](uint64_t* bar, uint32_t parity) {
+                const bool ok = __all_sync(0xffffffffu, wait(bar, parity));
                 tc_fence_after();
+                return ok;
+            };
+            bool ok = until(q_full, 0) && until(k_full, 0);
+            if (ok) {
                 qk(0, 0);
                 qk(1, 0);
-                umma_commit(k_empty);
+                if (leader) umma_commit(k_empty);
             }
             // the weights of tile w overwrite its scores: the next scores are issued behind the product
             // that reads them, and products of one thread run in order
+            int st = 0;
+            uint32_t ph = 0;
+            ok = ok && until(v_ok, 0);
             for (int i = 0; i < nt && ok; ++i) {
-                const int st = i % NS, sn = (i + 1) % NS;
+                const int sn = st + 1 == NS ? 0 : st + 1;
+                const uint32_t pn = st + 1 == NS ? ph ^ 1u : ph;
                 const bool more = i + 1 < nt;
-                ok = wait(v_ok + st, (i / NS) & 1) && (!more || wait(k_full + sn, ((i + 1) / NS) & 1));
-                for (int w = 0; w < 2 && ok; ++w) {
-                    ok = wait(p_ready + w, i & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                    pv(w, st, i == 0);
-                    if (w == 1) umma_commit(v_empty + st);
-                    if (more) qk(w, sn);
-                    else umma_commit(o_done + w);
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    if (!(ok = until(p_ready + 2 * w, i & 1))) break;
+                    pv(w, st, 0, i == 0);   // the first half of the keys while the second is still exponentiated
+                    if (!(ok = until(p_ready + 2 * w + 1, i & 1))) break;
+                    pv(w, st, 1, false);
+                    if (w == 1 && leader) umma_commit(v_empty + st);
+                    if (more) {
+                        // waits for loads stand behind queued products
+                        if (w == 0 && !(ok = until(k_full + sn, pn))) break;
+                        qk(w, sn);
+                    } else if (leader) {
+                        umma_commit(o_done + w);
+                    }
                 }
-                if (ok && more) umma_commit(k_empty + sn);
+                if (ok && more) {
+                    if (leader) umma_commit(k_empty + sn);
+                    ok = until(v_ok + sn, pn);
+                }
+                st = sn;
+                ph = pn;
             }
-            if (!ok) {
+            if (!ok && leader) {
                 volatile int go = 0;
                 umma_commit(drained);
                 mbar_wait_bounded(drained, 0, kWtLimitNs, &go);
@@ -646,7 +690,8 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
             for (int c = 0; c < kWtKeys; c += 32) tmem_ld32(ts + c, s + c);
             tmem_wait_ld();
             const int base = tile_base(i);
-            if (base + kWtKeys - 1 > ta || (p.window > 0 && base <= tb - p.window)) {
+            const bool edge = base + kWtKeys - 1 > ta || (p.window > 0 && base <= tb - p.window);
+            if (edge) {
                 const int last = tr - base, from = p.window > 0 ? last - p.window + 1 : 0, first = p.sinks - base;
 #pragma unroll
                 for (int c = 0; c < kWtKeys; c += 32) {
@@ -655,16 +700,21 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
                     for (int e = 0; e < 32; ++e) s[c + e] = (on >> e) & 1u ? s[c + e] : -INFINITY;
                 }
             }
-            float mx[4] = {s[0], s[1], s[2], s[3]};
+            // the running maximum; a NaN score makes it NaN, and with it the whole row
+            float mx[8];
 #pragma unroll
-            for (int c = 4; c < kWtKeys - 4; c += 8)
+            for (int e = 0; e < 8; ++e) mx[e] = max3(s[e], s[8 + e], s[16 + e]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
-            const float n = fmaxf(max3(m, mx[0], mx[1]), max3(fmaxf(mx[2], mx[3]), fmaxf(s[124], s[125]), fmaxf(s[126], s[127])));
+            for (int c = 24; c < kWtKeys - 8; c += 16)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 8 + e]);
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) mx[e] = max3(mx[e], s[kWtKeys - 8 + e], max3(mx[e + 1], s[kWtKeys - 7 + e], m));
+            const float n = max3(max3(mx[0], mx[2], mx[4]), mx[6], m);
             if (i == 0) {
                 m = n;
             } else {
-                const bool grow = n > m && !((n - m) * p.sl2 <= kWtRescaleLog2);
+                const bool grow = n != m && !((n - m) * p.sl2 <= kWtRescaleLog2);
                 if (__any_sync(0xffffffffu, grow)) {
                     // the scores' barrier also covers the second product before them: O is complete
                     const float f = grow ? exp2_fast((m - n) * p.sl2) : 1.0f;
@@ -696,13 +746,16 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
                     x[e] = pack2<T>(a.x, a.y);   // weights in T for the second product; the sum keeps fp32
                 }
                 tmem_st16u(ts + c / 2, x);
+                if (c & 32) {
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_ready + 2 * w + c / 64);
+                }
             }
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_ready + w);
         }
+        if (m == INFINITY) l = NAN;   // inf - inf
         if (nt > 0 && ok) ok = __all_sync(0xffffffffu, wait(o_done + w, 0));
         tc_fence_after();
         const bool mine = ok && local < rows;
