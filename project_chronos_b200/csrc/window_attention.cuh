@@ -357,6 +357,13 @@ __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t* v) {
         : "memory");
 }
 
+// 32 bytes in one store (a whole DRAM sector; 32-byte aligned).
+__device__ __forceinline__ void store32(void* p, const uint32_t (&x)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(x[0]), "r"(x[1]), "r"(x[2]),
+                 "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+                 : "memory");
+}
+
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -696,8 +703,9 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
 #pragma unroll
                 for (int c = 0; c < kWtKeys; c += 32) {
                     const uint32_t on = ones_below(last + 1 - c) & (~ones_below(from - c) | ones_below(first - c));
+                    if (__any_sync(0xffffffffu, on != 0xffffffffu))
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) s[c + e] = (on >> e) & 1u ? s[c + e] : -INFINITY;
+                        for (int e = 0; e < 32; ++e) s[c + e] = (on >> e) & 1u ? s[c + e] : -INFINITY;
                 }
             }
             // the running maximum; a NaN score makes it NaN, and with it the whole row
@@ -762,6 +770,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
         const int64_t qrow = t.q0 + t.m0 + local;
         const float inv = l > 0.0f ? 1.0f / l : l;
         T* out = static_cast<T*>(p.out) + qrow * p.o_row + head * p.o_head;
+        const bool wide = (reinterpret_cast<uintptr_t>(out) & 31) == 0;
 #pragma unroll
         for (int c = 0; c < DP; c += 32) {
             float o[32];
@@ -771,13 +780,18 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
             }
             if (mine)
 #pragma unroll
-                for (int e = 0; e < 32; e += 8)
-                    if (c + e < p.dim) {
-                        float x[8];
+                for (int e = 0; e < 32; e += 16) {
+                    uint32_t x[8];
 #pragma unroll
-                        for (int y = 0; y < 8; ++y) x[y] = nt > 0 ? o[e + y] * inv : 0.0f;
-                        store8<T>(out + c + e, x);
+                    for (int y = 0; y < 8; ++y)
+                        x[y] = nt > 0 ? pack2<T>(o[e + 2 * y] * inv, o[e + 2 * y + 1] * inv) : 0u;
+                    if (wide && c + e + 16 <= p.dim) {
+                        store32(out + c + e, x);
+                    } else {
+                        if (c + e < p.dim) *reinterpret_cast<uint4*>(out + c + e) = make_uint4(x[0], x[1], x[2], x[3]);
+                        if (c + e + 8 < p.dim) *reinterpret_cast<uint4*>(out + c + e + 8) = make_uint4(x[4], x[5], x[6], x[7]);
                     }
+                }
         }
         if (mine && p.lse != nullptr)
             p.lse[qrow * p.heads + head] = l != 0.0f ? ((m == -INFINITY ? 0.0f : m * p.sl2) + log2f(l)) * kLn2 : -INFINITY;
