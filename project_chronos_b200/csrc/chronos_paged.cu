@@ -52,9 +52,13 @@ int slot_limit(const ChronosPagedCache& c, int64_t slot_cap, bool has_cap) {
 // ---------------------------------------------------------------------------
 // one-token attention
 // ---------------------------------------------------------------------------
+constexpr int kPdClusterBlocks = 6;   // blocks of 64 places that a block of a cluster takes at most
+
 struct DecodePlan {
     bool mma;
     int dp;              // padded head dimension of the tensor-core path
+    bool one_page;       // 16 consecutive aligned slots lie in one page
+    int cluster;         // blocks per row in one cluster; 0: the work list and a second kernel
     int rows, parts, grid, part_stride, max_vis;
     int64_t score_stride;
     size_t o_part_o, o_part_ml, o_lse2, o_scores, total;
@@ -88,6 +92,17 @@ bool decode_uses_mma(const ChronosPagedDecodeArgs* a) {
            multiples(2, {a->q_row_stride, a->q_head_stride, a->out_row_stride, a->out_head_stride});
 }
 
+// Blocks per row when a cluster joins them, 0 when the work list is cut evenly instead.
+int decode_cluster(const ChronosPagedDecodeArgs* a, const DecodePlan& d, int64_t blocks) {
+    if (!d.mma || a->weights != nullptr) return 0;
+    const int64_t rows = static_cast<int64_t>(a->cache.batch) * a->cache.kv_heads * d.parts;
+    const int64_t room = (d.dp == 256 ? 1 : 2) * static_cast<int64_t>(sm_count());
+    int size = 1;
+    while (size < 8 && size < blocks) size *= 2;
+    while (size > 1 && rows * size > room) size /= 2;
+    return rows * size <= room && blocks <= kPdClusterBlocks * size ? size : 0;
+}
+
 DecodePlan decode_plan(const ChronosPagedDecodeArgs* a) {
     const ChronosPagedCache& c = a->cache;
     DecodePlan d{};
@@ -97,11 +112,14 @@ DecodePlan decode_plan(const ChronosPagedDecodeArgs* a) {
     const int rep = a->heads / c.kv_heads;
     d.parts = (rep + d.rows - 1) / d.rows;
     const int limit = slot_limit(c, a->slot_cap, a->weights != nullptr);
-    d.max_vis = a->window > 0 ? static_cast<int>(std::min<int64_t>(limit, static_cast<int64_t>(a->window) + a->sinks)) : limit;
+    // places of a row: both runs of visible slots start at a multiple of 16
+    d.max_vis = a->window > 0 ? static_cast<int>(std::min<int64_t>(limit, static_cast<int64_t>(a->window) + a->sinks + 32)) : limit;
+    d.one_page = c.page_size % kPdTile == 0;
     const int per_sm = d.mma ? (d.dp == 256 ? 1 : 2) : 4;
     const int64_t blocks = (static_cast<int64_t>(d.max_vis) + kPdBlock - 1) / kPdBlock;
     const int64_t units = std::max<int64_t>(1, blocks) * c.batch * c.kv_heads * d.parts;
     d.grid = static_cast<int>(std::min<int64_t>({units, static_cast<int64_t>(per_sm) * sm_count(), kPdMaxGrid}));
+    d.cluster = decode_cluster(a, d, blocks);
     d.part_stride = d.mma ? d.dp : static_cast<int>(round_up(c.head_dim, 4));
     size_t at = 0;
     auto take = [&at](size_t bytes) {
@@ -109,7 +127,7 @@ DecodePlan decode_plan(const ChronosPagedDecodeArgs* a) {
         at = round_up(at + bytes, 256);
         return o;
     };
-    const size_t slots = 2 * static_cast<size_t>(d.grid) * d.rows;
+    const size_t slots = d.cluster > 0 ? 0 : 2 * static_cast<size_t>(d.grid) * d.rows;
     d.o_part_o = take(slots * d.part_stride * 4);
     d.o_part_ml = take(slots * 8);
     if (a->weights != nullptr) {
@@ -121,12 +139,36 @@ DecodePlan decode_plan(const ChronosPagedDecodeArgs* a) {
     return d;
 }
 
+using DecodeKernel = void (*)(PagedDecodeParams);
+template <typename T, int DP, int NT>
+DecodeKernel decode_kernel(bool one_page, bool cluster) {
+    if (cluster) return one_page ? paged_decode_mma_kernel<T, DP, NT, true, true> : paged_decode_mma_kernel<T, DP, NT, false, true>;
+    return one_page ? paged_decode_mma_kernel<T, DP, NT, true, false> : paged_decode_mma_kernel<T, DP, NT, false, false>;
+}
+
 template <typename T, int DP>
-int launch_decode_mma(const PagedDecodeParams& p, cudaStream_t st) {
+int launch_decode_mma(const PagedDecodeParams& p, const DecodePlan& d, cudaStream_t st) {
     using S = PagedMma<DP>;
-    void (*kernel)(PagedDecodeParams) = p.rep > 8 ? paged_decode_mma_kernel<T, DP, true> : paged_decode_mma_kernel<T, DP, false>;
+    const DecodeKernel kernel = p.rep > 8 ? decode_kernel<T, DP, 2>(d.one_page, d.cluster > 0) : decode_kernel<T, DP, 1>(d.one_page, d.cluster > 0);
     if (int rc = set_smem(kernel, S::kSmem)) return rc;
-    CHRONOS_CUDA_CHECK(launch_kernel(kernel, dim3(p.grid), dim3(kPdThreads), S::kSmem, st, false, p));
+    if (d.cluster == 0) {
+        CHRONOS_CUDA_CHECK(launch_kernel(kernel, dim3(p.grid), dim3(kPdThreads), S::kSmem, st, false, p));
+        return CHRONOS_OK;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(p.c.batch) * p.c.kv_heads * p.parts * d.cluster);
+    cfg.blockDim = dim3(kPdThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = d.cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    count_launch();
+    CHRONOS_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p));
     return CHRONOS_OK;
 }
 
@@ -134,9 +176,9 @@ template <typename T>
 int launch_decode(const PagedDecodeParams& p, const DecodePlan& d, bool vec, cudaStream_t st) {
     if constexpr (sizeof(T) == 2) {
         if (d.mma) {
-            const int rc = d.dp == 64 ? launch_decode_mma<T, 64>(p, st)
-                                      : d.dp == 128 ? launch_decode_mma<T, 128>(p, st) : launch_decode_mma<T, 256>(p, st);
-            if (rc) return rc;
+            const int rc = d.dp == 64 ? launch_decode_mma<T, 64>(p, d, st)
+                                      : d.dp == 128 ? launch_decode_mma<T, 128>(p, d, st) : launch_decode_mma<T, 256>(p, d, st);
+            if (rc || d.cluster > 0) return rc;
         }
     }
     if (!d.mma)
@@ -309,6 +351,10 @@ extern "C" int chronos_paged_decode(const ChronosPagedDecodeArgs* a, void* strea
     p.window = a->window;
     p.sinks = a->window > 0 ? a->sinks : 0;
     p.max_slots = limit;
+    p.page_shift = -1;
+    if ((a->cache.page_size & (a->cache.page_size - 1)) == 0)
+        for (p.page_shift = 0; (1 << p.page_shift) < a->cache.page_size;) ++p.page_shift;
+    p.cluster = d.cluster;
     p.sl2 = static_cast<float>(static_cast<double>(a->scale) * 1.4426950408889634);
     p.q = a->q;
     p.q_row = a->q_row_stride;

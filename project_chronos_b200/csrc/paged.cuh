@@ -18,6 +18,8 @@
 // the list: the result does not depend on which block ran first.
 #pragma once
 
+#include <cooperative_groups.h>
+
 #include "chronos_paged.h"
 #include "common.cuh"
 
@@ -30,6 +32,11 @@ constexpr int kPdBlock = kPdTile * kPdWarps;    // slots of one unit of the work
 constexpr int kPdMaxGrid = 1024;
 constexpr int kPdMaxRep = 256;                  // query heads per kv head
 
+// Bits 0..n-1 set (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t ones_below(int n) {
+    return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+}
+
 struct PagedDecodeParams {
     ChronosPagedCache c;
     int heads, rep;        // query heads, query heads per kv head
@@ -37,6 +44,8 @@ struct PagedDecodeParams {
     int parts;             // ceil(rep / rows): units per kv head
     int window, sinks;
     int max_slots;         // lengths are cut to this
+    int page_shift;        // log2(page_size), -1 where it is no power of two
+    int cluster;           // blocks per row (cluster kernels)
     float sl2;             // scale * log2(e)
     const void* q;
     int64_t q_row, q_head;
@@ -58,17 +67,26 @@ struct PagedDecodeParams {
     int32_t* status;
 };
 
-// The visible slots of sequence b: [0, first) and [lo, len).
+// The visible slots of sequence b, [0, first) and [lo, len), as a list of n places
+// that starts every run of slots at a multiple of 16: place i is slot i before
+// `front`, slot i + skip from there on.  Places before lo or at first.. are hidden.
 struct PagedRow {
-    int len, lo, first, nvis, nblk;
+    int len, lo, first, front, skip, n, nblk;
+    __device__ __forceinline__ int slot(int place) const { return place < front ? place : place + skip; }
+    // Which of the 16 slots from `slot0` on are visible.
+    __device__ __forceinline__ uint32_t visible16(int slot0) const {
+        return (ones_below(first - slot0) | (ones_below(len - slot0) & ~ones_below(lo - slot0))) & 0xffffu;
+    }
 };
 __device__ __forceinline__ PagedRow paged_row(const PagedDecodeParams& p, int b) {
     PagedRow r;
     r.len = min(max(p.c.lens[b], 0), p.max_slots);
     r.lo = p.window > 0 ? max(0, r.len - p.window) : 0;
     r.first = min(p.sinks, r.lo);
-    r.nvis = r.len - r.lo + r.first;
-    r.nblk = max(1, (r.nvis + kPdBlock - 1) / kPdBlock);   // an empty row still has its zeros written
+    r.front = (r.first + 15) & ~15;
+    r.skip = max(0, (r.lo & ~15) - r.front);
+    r.n = r.len - r.skip;
+    r.nblk = max(1, (r.n + kPdBlock - 1) / kPdBlock);   // an empty row still has its zeros written
     return r;
 }
 
@@ -149,22 +167,40 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Page and slot of the 16 visible indices a warp takes next (lane i and i + 16
-// hold index i); page -1 for an index behind the row or a page that is none.
+__device__ __forceinline__ void paged_split(const PagedDecodeParams& p, int slot, int& page, int& in_page) {
+    if (p.page_shift >= 0) {
+        page = slot >> p.page_shift;
+        in_page = slot & (p.c.page_size - 1);
+    } else {
+        page = slot / p.c.page_size;
+        in_page = slot - page * p.c.page_size;
+    }
+}
+
+// The 16 places a warp takes next: which are visible, and their page and slot (lane i
+// and i + 16 hold place i; all lanes hold place 0's where page_size is a multiple of
+// 16: then all 16 lie in one page).  A page that is none hides its places.
 struct PagedLook {
     int page, slot;
+    uint32_t vis;
 };
+template <bool ONE_PAGE>
 __device__ __forceinline__ PagedLook paged_look(const PagedDecodeParams& p, const PagedIter& it, int end, int warp,
                                                 int lane) {
-    PagedLook k{-1, 0};
-    const int idx = it.blk * kPdBlock + warp * kPdTile + (lane & 15);
-    if (it.u < end && idx < it.r.nvis) {
-        const int pos = idx < it.r.first ? idx : it.r.lo + idx - it.r.first;
-        k.page = p.c.page_table[it.b * p.c.page_table_stride + pos / p.c.page_size];
-        k.slot = pos % p.c.page_size;
-        if (k.page < 0 || k.page >= p.c.num_pages) {
-            report_status(p.status, CHRONOS_ERR_INVALID_ARG);
-            k.page = -1;
+    PagedLook k{-1, 0, 0u};
+    const int place = it.blk * kPdBlock + warp * kPdTile;
+    if (it.u < end && place < it.r.n) {
+        const int slot0 = it.r.slot(place);
+        k.vis = it.r.visible16(slot0);
+        const bool mine = ONE_PAGE || (k.vis >> (lane & 15)) & 1u;
+        int page = 0;
+        if (mine && k.vis) {
+            paged_split(p, slot0 + (ONE_PAGE ? 0 : lane & 15), page, k.slot);
+            k.page = p.c.page_table[it.b * p.c.page_table_stride + page];
+            if (k.page < 0 || k.page >= p.c.num_pages) {
+                report_status(p.status, CHRONOS_ERR_INVALID_ARG);
+                k.page = -1;
+            }
         }
     }
     return k;
@@ -227,264 +263,359 @@ __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// DP: the head dimension rounded up to 64, 128 or 256 (columns behind it are
-// zero); HI: more than 8 query heads per unit (rows 8..15 of the products in use).
+// The parts of a row's `nh` heads (from `head0` on) that the blocks of a cluster hold in
+// their shared memory, o [16][stride] fp32 and then (m, l) [16][2]: every block joins
+// its share of the heads, in the order of the blocks.
+template <typename T>
+__device__ __forceinline__ void paged_cluster_join(const PagedDecodeParams& p, void* part, int stride, int rank, int b,
+                                                   int head0, int nh, int warp, int lane) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    const float* mine = static_cast<const float*>(part);
+    for (int row = rank * kPdWarps + warp; row < nh; row += p.cluster * kPdWarps) {
+        float M = -INFINITY, L = 0.0f;
+        const float* peer = cl.map_shared_rank(mine, lane < p.cluster ? lane : 0) + 16 * stride + row * 2;
+        const float pm = lane < p.cluster ? peer[0] : -INFINITY, pl = lane < p.cluster ? peer[1] : 0.0f;
+        M = pm;
+#pragma unroll
+        for (int x = 4; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+        M = __shfl_sync(0xffffffffu, M, 0);
+        const float u = M == -INFINITY ? 0.0f : M;
+        const float c = exp2_fast(pm - u);
+        L = pl * c;
+#pragma unroll
+        for (int x = 4; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+        L = __shfl_sync(0xffffffffu, L, 0);
+        const float inv = L > 0.0f ? 1.0f / L : L;
+        T* out = static_cast<T*>(p.out) + b * p.out_row + (head0 + row) * p.out_head;
+        float acc[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+        for (int r = 0; r < p.cluster; ++r) {
+            const float* po = cl.map_shared_rank(mine, r) + row * stride;
+            const float w = __shfl_sync(0xffffffffu, c, r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (lane + 32 * i < p.c.head_dim) acc[i] = fmaf(w, po[lane + 32 * i], acc[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (lane + 32 * i < p.c.head_dim) out[lane + 32 * i] = from_f32<T>(acc[i] * inv);
+        if (lane == 0 && p.lse != nullptr)
+            p.lse[static_cast<int64_t>(b) * p.heads + head0 + row] = L != 0.0f ? (u + log2f(L)) * kLn2 : -INFINITY;
+    }
+    cl.sync();   // nobody leaves while its part is read
+}
+
+// Swaps rows and columns of an 8 x 8 matrix of 16-bit values held by a warp.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// DP: the head dimension rounded up to 64, 128 or 256 (columns behind it are zero).
 template <int DP>
 struct PagedMma {
     static constexpr int kStages = DP == 64 ? 6 : 3;
     static constexpr int kTileBytes = kPdTile * DP * 2;                       // K or V of one warp's tile
     static constexpr int kStageBytes = kPdWarps * 2 * kTileBytes;
-    static constexpr int kOStride = DP + 8;                                   // fp32; keeps the rows off one bank
-    static constexpr int kMergeBytes = (kPdWarps - 1) * 8 * kOStride * 4;
-    static constexpr int kSmem = kStages * kStageBytes + kMergeBytes + kPdWarps * 16 * 2 * 4 + kStages * kPdWarps * 4;
+    static constexpr int kOStride = DP + 4;                                   // fp32; four heads on different banks
+    static constexpr int kMergeBytes = kPdWarps * 8 * kOStride * 4;
+    static constexpr int kSmem = kStages * kStageBytes + kMergeBytes + kPdWarps * 8 * 2 * 4 + kStages * kPdWarps * 4;
     static constexpr int kBlocksPerSm = DP == 256 ? 1 : 2;
 };
 
 // HBM bound: 2 * D * 2 bytes per visible slot and kv head against 4 * D flops per
-// query head.  The tensor cores take a slot's K row for all query heads of the
-// group at once (rows of the 16-row operand; unused rows are zero).  A warp owns
-// 16 slots at a time and its own ring of asynchronous copies (K and V rows go to
-// shared memory 16 bytes at a time, rows of 8 chunks swizzled against bank
-// conflicts), so warps never wait for each other inside a row.
-template <typename T, int DP, bool HI>
+// query head.  Transposed products, S^T = K Q^T (16 slots x 8 heads) and
+// O^T = V^T P^T (16 columns x 8 heads), take the query heads of a kv head as the
+// 8-wide operand: no row of the 16-wide one is wasted, and one movmatrix turns the
+// weights from the first product's result into the second's operand.  A warp owns 16
+// slots at a time and its own ring of asynchronous copies (K and V rows go to shared
+// memory 16 bytes at a time, swizzled against bank conflicts), so warps never wait for
+// each other inside a row.  The maximum moves only when a score exceeds it by more
+// than 2^8 in weight, which one vote per tile finds out.
+//
+// NT: groups of 8 query heads (1 or 2).  CL: a cluster of p.cluster blocks per row
+// shares its blocks of 64 places and joins through distributed shared memory;
+// otherwise block c takes the c-th share of the work list.
+template <typename T, int DP, int NT, bool ONE_PAGE, bool CL>
 __global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_decode_mma_kernel(
     const __grid_constant__ PagedDecodeParams p) {
     using S = PagedMma<DP>;
     constexpr int NS = S::kStages;
     constexpr int CPR = DP / 8;            // 16-byte chunks per row
     constexpr int RPI = 32 / CPR;          // rows a warp copies per instruction
+    constexpr float kGrow = 8.0f;
     extern __shared__ __align__(128) uint8_t smem[];
-    float* s_o = reinterpret_cast<float*>(smem + NS * S::kStageBytes);
-    float* s_ml = s_o + S::kMergeBytes / 4;                                    // [warp][16][2]
-    uint32_t* s_vis = reinterpret_cast<uint32_t*>(s_ml + kPdWarps * 32);       // [stage][warp]
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int quad = lane >> 2, qc = lane & 3;   // this lane's rows quad, quad + 8 and column pair of a product
+    float* s_o = reinterpret_cast<float*>(smem + NS * S::kStageBytes);         // [warp][8 heads][kOStride]
+    float* s_ml = s_o + S::kMergeBytes / 4;                                    // [warp][8][2]
+    uint32_t* s_vis = reinterpret_cast<uint32_t*>(s_ml + kPdWarps * 16);       // [stage][warp]
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int quad = lane >> 2, qc = lane & 3;   // a product's row (slot, column of V) and pair of heads
 
-    const int total = paged_total(p, lane);
-    const int share = paged_share(p, total);
-    const int begin = static_cast<int>(blockIdx.x) * share, end = min(total, begin + share);
-    if (blockIdx.x == 0) paged_check_lens(p);
-    if (begin >= end) return;
-    PagedIter ld = paged_seek(p, begin, lane);
+    int end;
+    PagedIter ld;
+    const int rank = CL ? static_cast<int>(blockIdx.x) % p.cluster : 0;
+    if constexpr (CL) {
+        const int row = blockIdx.x / p.cluster, per = p.c.kv_heads * p.parts;
+        ld.u = 0;
+        ld.b = row / per;
+        ld.v = row % per;
+        ld.blk = rank;
+        ld.r = paged_row(p, ld.b);
+        end = ld.r.nblk > rank ? (ld.r.nblk - rank + p.cluster - 1) / p.cluster : 0;
+        if (blockIdx.x == 0) paged_check_lens(p);
+    } else {
+        const int total = paged_total(p, lane);
+        const int share = paged_share(p, total);
+        const int begin = static_cast<int>(blockIdx.x) * share;
+        end = min(total, begin + share);
+        if (blockIdx.x == 0) paged_check_lens(p);
+        if (begin >= end) return;
+        ld = paged_seek(p, begin, lane);
+    }
+    auto advance = [&](PagedIter& it) {
+        if constexpr (CL) {
+            ++it.u;
+            it.blk += p.cluster;
+        } else {
+            it.advance(p, end);
+        }
+    };
     PagedIter cp = ld;
-    PagedLook look = paged_look(p, ld, end, warp, lane);
+    PagedLook look = paged_look<ONE_PAGE>(p, ld, end, warp, lane);
 
-    const T* kbase = static_cast<const T*>(p.c.k_pages);
-    const T* vbase = static_cast<const T*>(p.c.v_pages);
+    const int ch = lane % CPR, lrow = lane / CPR;
+    const bool col = ch * 8 < p.c.head_dim;
     auto issue = [&](int stage) {
         const uint32_t sk = smem_u32(smem + stage * S::kStageBytes + warp * 2 * S::kTileBytes);
         const int64_t g = ld.v / p.parts;
-        const int ch = lane % CPR;
-        const bool col = ch * 8 < p.c.head_dim;
+        uint32_t vis = look.vis;
+        if (ONE_PAGE) {
+            if (look.page < 0) vis = 0u;
+            // one page: the rows stand a slot stride apart
+            const T* ks = static_cast<const T*>(p.c.k_pages) + g * p.c.k_head_stride + ch * 8;
+            const T* vs = static_cast<const T*>(p.c.v_pages) + g * p.c.v_head_stride + ch * 8;
+            if (vis) {
+                ks += look.page * p.c.k_page_stride + (look.slot + lrow) * p.c.k_slot_stride;
+                vs += look.page * p.c.v_page_stride + (look.slot + lrow) * p.c.v_slot_stride;
+            }
+            const int64_t kstep = vis ? RPI * p.c.k_slot_stride : 0, vstep = vis ? RPI * p.c.v_slot_stride : 0;
 #pragma unroll
-        for (int i = 0; i < kPdTile / RPI; ++i) {
-            const int r = i * RPI + lane / CPR;
-            const int page = __shfl_sync(0xffffffffu, look.page, r);
-            const int64_t slot = __shfl_sync(0xffffffffu, look.slot, r);
-            const bool ok = col && page >= 0;
-            const T* ks = kbase + (ok ? page * p.c.k_page_stride + slot * p.c.k_slot_stride + g * p.c.k_head_stride + ch * 8 : 0);
-            const T* vs = vbase + (ok ? page * p.c.v_page_stride + slot * p.c.v_slot_stride + g * p.c.v_head_stride + ch * 8 : 0);
-            const uint32_t off = static_cast<uint32_t>(r * DP * 2 + ((ch ^ (r & 7)) << 4));
-            cp_async16(sk + off, ks, ok);
-            cp_async16(sk + S::kTileBytes + off, vs, ok);
+            for (int i = 0; i < kPdTile / RPI; ++i) {
+                const int r = i * RPI + lrow;
+                const bool ok = col && ((vis >> r) & 1u);
+                const uint32_t off = static_cast<uint32_t>(r * DP * 2 + ((ch ^ (r & 7)) << 4));
+                cp_async16(sk + off, ok ? ks : p.c.k_pages, ok);
+                cp_async16(sk + S::kTileBytes + off, ok ? vs : p.c.v_pages, ok);
+                ks += kstep;
+                vs += vstep;
+            }
+        } else {
+            vis &= __ballot_sync(0xffffffffu, look.page >= 0) & 0xffffu;
+            const T* kb = static_cast<const T*>(p.c.k_pages) + g * p.c.k_head_stride + ch * 8;
+            const T* vb = static_cast<const T*>(p.c.v_pages) + g * p.c.v_head_stride + ch * 8;
+#pragma unroll
+            for (int i = 0; i < kPdTile / RPI; ++i) {
+                const int r = i * RPI + lrow;
+                const int page = __shfl_sync(0xffffffffu, look.page, r);
+                const int64_t slot = __shfl_sync(0xffffffffu, look.slot, r);
+                const bool ok = col && ((vis >> r) & 1u);
+                const uint32_t off = static_cast<uint32_t>(r * DP * 2 + ((ch ^ (r & 7)) << 4));
+                cp_async16(sk + off, ok ? kb + page * p.c.k_page_stride + slot * p.c.k_slot_stride : p.c.k_pages, ok);
+                cp_async16(sk + S::kTileBytes + off, ok ? vb + page * p.c.v_page_stride + slot * p.c.v_slot_stride : p.c.v_pages, ok);
+            }
         }
-        const uint32_t vis = __ballot_sync(0xffffffffu, look.page >= 0) & 0xffffu;
         if (lane == 0) s_vis[stage * kPdWarps + warp] = vis;
     };
 #pragma unroll
     for (int s = 0; s < NS - 1; ++s) {
         if (ld.u < end) {
             issue(s);
-            ld.advance(p, end);
-            look = paged_look(p, ld, end, warp, lane);
+            advance(ld);
+            look = paged_look<ONE_PAGE>(p, ld, end, warp, lane);
         }
         cp_async_commit();
     }
 
-    uint32_t qa[DP / 16][4];
-    float o[DP / 8][4];
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+    // where ldmatrix finds this lane's row of a 16 x 16 piece of K (rows: slots) or V
+    uint32_t koff[4], voff[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int kr = (lane & 7) + ((lane >> 3) & 1) * 8, vr = (lane & 7) + (lane >> 4) * 8;
+        koff[i] = static_cast<uint32_t>(kr * DP * 2 + (((2 * i + (lane >> 4)) ^ (lane & 7)) << 4));
+        voff[i] = static_cast<uint32_t>(S::kTileBytes + vr * DP * 2 + (((2 * i + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+    }
+    uint32_t qb[NT][DP / 16][2];
+    float o[NT][DP / 16][4];
+    float m[NT][2], l[NT][2];
     bool fresh = true;          // the next unit opens a new part or row
     int part_blk = 0;           // the block it opened with
     int stage = 0;
-    while (cp.u < end) {
-        if (ld.u < end) {
-            issue(stage == 0 ? NS - 1 : stage - 1);
-            ld.advance(p, end);
-            look = paged_look(p, ld, end, warp, lane);
-        }
-        cp_async_commit();
+    while (cp.u < end || (CL && fresh)) {
         const int kvh = cp.v / p.parts, h0 = (cp.v % p.parts) * 16;
         const int nh = min(16, p.rep - h0);             // query heads of this unit
         if (fresh) {
             fresh = false;
             part_blk = cp.blk;
-            m0 = m1 = -INFINITY;
-            l0 = l1 = 0.0f;
-#pragma unroll
-            for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
             const T* q = static_cast<const T*>(p.q) + cp.b * p.q_row + static_cast<int64_t>(kvh * p.rep + h0) * p.q_head;
 #pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk)
+            for (int t = 0; t < NT; ++t) {
+                m[t][0] = m[t][1] = -INFINITY;
+                l[t][0] = l[t][1] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int row = quad + (j & 1) * 8, d = kk * 16 + qc * 2 + (j >> 1) * 8;
-                    qa[kk][j] = (HI || !(j & 1)) && row < nh && d < p.c.head_dim
-                                    ? *reinterpret_cast<const uint32_t*>(q + row * p.q_head + d) : 0u;
-                }
-        }
-        cp_async_wait<NS - 1>();
-        __syncwarp();
-        const uint32_t sk = smem_u32(smem + stage * S::kStageBytes + warp * 2 * S::kTileBytes);
-        const uint32_t sv = sk + S::kTileBytes;
-        const uint32_t vis = s_vis[stage * kPdWarps + warp];
-        if (vis || p.scores != nullptr) {   // with running sums, hidden slots' scores are written too
-            float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-            {
-                const int r = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+                for (int i = 0; i < DP / 16; ++i) {
+                    o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.0f;
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk) {
-                    uint32_t kb[4];
-                    ldmatrix_x4<false>(kb, sk + r * DP * 2 + (((kk * 2 + half) ^ (r & 7)) << 4));
-                    mma_16816<T>(s[0], qa[kk], kb[0], kb[1]);
-                    mma_16816<T>(s[1], qa[kk], kb[2], kb[3]);
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const bool on = (vis >> (t * 8 + qc * 2 + (j & 1))) & 1u;
-                    s[t][j] = on ? s[t][j] * p.sl2 : -INFINITY;
-                }
-            if (p.scores != nullptr) {
-                const int idx = cp.blk * kPdBlock + warp * kPdTile + qc * 2;
-                float* sc = p.scores + (static_cast<int64_t>(cp.b) * p.heads + kvh * p.rep + h0) * p.score_stride + idx;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (quad < nh)
-                        *reinterpret_cast<float2*>(sc + quad * p.score_stride + t * 8) = make_float2(s[t][0], s[t][1]);
-                    if (HI && quad + 8 < nh)
-                        *reinterpret_cast<float2*>(sc + (quad + 8) * p.score_stride + t * 8) =
-                            make_float2(s[t][2], s[t][3]);
-                }
-            }
-            float n0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-            float n1 = HI ? fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])) : -INFINITY;
-#pragma unroll
-            for (int x = 1; x < 4; x <<= 1) {
-                n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
-                if (HI) n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
-            }
-            if (__any_sync(0xffffffffu, n0 > m0 || (HI && n1 > m1))) {
-                n0 = fmaxf(n0, m0);
-                const float c0 = n0 == -INFINITY ? 1.0f : exp2_fast(m0 - n0);
-                m0 = n0;
-                l0 *= c0;
-                float c1 = 1.0f;
-                if (HI) {
-                    n1 = fmaxf(n1, m1);
-                    c1 = n1 == -INFINITY ? 1.0f : exp2_fast(m1 - n1);
-                    m1 = n1;
-                    l1 *= c1;
-                }
-#pragma unroll
-                for (int i = 0; i < DP / 8; ++i) {
-                    o[i][0] *= c0;
-                    o[i][1] *= c0;
-                    if (HI) {
-                        o[i][2] *= c1;
-                        o[i][3] *= c1;
+                    for (int j = 0; j < 2; ++j) {
+                        const int row = t * 8 + quad, d = i * 16 + qc * 2 + j * 8;
+                        qb[t][i][j] = row < nh && d < p.c.head_dim
+                                          ? *reinterpret_cast<const uint32_t*>(q + row * p.q_head + d) : 0u;
                     }
                 }
             }
-            const float u0 = m0 == -INFINITY ? 0.0f : m0, u1 = m1 == -INFINITY ? 0.0f : m1;
-            uint32_t pa[4];
+        }
+        if (ld.u < end) {
+            issue(stage == 0 ? NS - 1 : stage - 1);
+            advance(ld);
+            look = paged_look<ONE_PAGE>(p, ld, end, warp, lane);
+        }
+        cp_async_commit();
+        cp_async_wait<NS - 1>();
+        __syncwarp();
+        const uint32_t st = smem_u32(smem + stage * S::kStageBytes + warp * 2 * S::kTileBytes);
+        const uint32_t vis = cp.u < end ? s_vis[stage * kPdWarps + warp] : 0u;
+        if (vis || (p.scores != nullptr && cp.u < end)) {   // with running sums, hidden slots' scores are written too
+            float s[NT][4];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const float a = exp2_fast(s[t][0] - u0), b = exp2_fast(s[t][1] - u0);
-                l0 += a + b;
-                pa[2 * t] = pack2<T>(a, b);   // weights in T for the second product; the sum keeps fp32
-                if (HI) {
-                    const float c = exp2_fast(s[t][2] - u1), d = exp2_fast(s[t][3] - u1);
-                    l1 += c + d;
-                    pa[2 * t + 1] = pack2<T>(c, d);
-                } else {
-                    pa[2 * t + 1] = 0u;
-                }
+            for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) {
+                uint32_t ka[4];
+                ldmatrix_x4<false>(ka, st + koff[kk & 3] + (kk >> 2) * 128);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) mma_16816<T>(s[t], ka, qb[t][kk][0], qb[t][kk][1]);
             }
-            {
-                const int r = lane & 15, half = lane >> 4;
+            // s[t][0..1]: slot quad, heads 8t + 2qc, + 1; s[t][2..3]: slot quad + 8
+            const bool on0 = (vis >> quad) & 1u, on1 = (vis >> (quad + 8)) & 1u;
+            bool grow = false;
 #pragma unroll
-                for (int dd = 0; dd < DP / 16; ++dd) {
-                    uint32_t vb[4];
-                    ldmatrix_x4<true>(vb, sv + r * DP * 2 + (((dd * 2 + half) ^ (r & 7)) << 4));
-                    mma_16816<T>(o[2 * dd], pa, vb[0], vb[1]);
-                    mma_16816<T>(o[2 * dd + 1], pa, vb[2], vb[3]);
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[t][j] = (j < 2 ? on0 : on1) ? s[t][j] * p.sl2 : -INFINITY;
+                    grow |= s[t][j] > m[t][j & 1] + kGrow;
                 }
+            if (p.scores != nullptr) {
+                const int idx = cp.blk * kPdBlock + warp * kPdTile + quad;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int h = t * 8 + qc * 2 + j;
+                        if (h < nh) {
+                            float* sc = p.scores + (static_cast<int64_t>(cp.b) * p.heads + kvh * p.rep + h0 + h) * p.score_stride + idx;
+                            sc[0] = s[t][j];
+                            sc[8] = s[t][2 + j];
+                        }
+                    }
+            }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float n = fmaxf(s[t][j], s[t][2 + j]);
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, x));
+                        n = fmaxf(n, m[t][j]);
+                        const float c = n == -INFINITY ? 1.0f : exp2_fast(m[t][j] - n);
+                        m[t][j] = n;
+                        l[t][j] *= c;
+#pragma unroll
+                        for (int i = 0; i < DP / 16; ++i) {
+                            o[t][i][j] *= c;
+                            o[t][i][2 + j] *= c;
+                        }
+                    }
+            }
+            uint32_t pb[NT][2];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const float u0 = m[t][0] == -INFINITY ? 0.0f : m[t][0], u1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
+                const float a = exp2_fast(s[t][0] - u0), b = exp2_fast(s[t][1] - u1);
+                const float c = exp2_fast(s[t][2] - u0), d = exp2_fast(s[t][3] - u1);
+                l[t][0] += a + c;
+                l[t][1] += b + d;
+                // weights in T for the second product; the sum keeps fp32
+                pb[t][0] = transpose8x8(pack2<T>(a, b));
+                pb[t][1] = transpose8x8(pack2<T>(c, d));
+            }
+#pragma unroll
+            for (int dd = 0; dd < DP / 16; ++dd) {
+                uint32_t va[4];
+                ldmatrix_x4<true>(va, st + voff[dd & 3] + (dd >> 2) * 128);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) mma_16816<T>(o[t][dd], va, pb[t][0], pb[t][1]);
             }
         }
         __syncwarp();   // every lane has read the tile before its stage is filled again
         stage = stage == NS - 1 ? 0 : stage + 1;
 
-        if (cp.blk + 1 == cp.r.nblk || cp.u + 1 == end) {
-            // the row (or this block's part of it) is complete: join the four warps
-            fresh = true;
-            const bool whole = part_blk == 0 && cp.blk + 1 == cp.r.nblk;
+        if (CL ? cp.u + 1 >= end : (cp.blk + 1 == cp.r.nblk || cp.u + 1 == end)) {
+            // the row (or this block's part of it) is complete: join the four warps, 8 heads at a time
+            fresh = !CL;
+            const bool whole = CL ? p.cluster == 1 : part_blk == 0 && cp.blk + 1 == cp.r.nblk;
 #pragma unroll
-            for (int x = 1; x < 4; x <<= 1) {
-                l0 += __shfl_xor_sync(0xffffffffu, l0, x);
-                l1 += __shfl_xor_sync(0xffffffffu, l1, x);
-            }
-            if (qc == 0) {
-                *reinterpret_cast<float2*>(s_ml + (warp * 16 + quad) * 2) = make_float2(m0, l0);
-                if (HI) *reinterpret_cast<float2*>(s_ml + (warp * 16 + quad + 8) * 2) = make_float2(m1, l1);
-            }
-            __syncthreads();
+            for (int t = 0; t < NT; ++t) {
+                if (t * 8 >= nh) break;
 #pragma unroll
-            for (int hi = 0; hi < (HI ? 2 : 1); ++hi) {
-                if (hi) __syncthreads();
-                const int row = quad + 8 * hi;
-                float M = -INFINITY, L = 0.0f;
+                for (int j = 0; j < 2; ++j) {
 #pragma unroll
-                for (int w = 0; w < kPdWarps; ++w) M = fmaxf(M, s_ml[(w * 16 + row) * 2]);
-                const float u = M == -INFINITY ? 0.0f : M;
+                    for (int x = 4; x < 32; x <<= 1) l[t][j] += __shfl_xor_sync(0xffffffffu, l[t][j], x);
+                    if (quad == 0)
+                        *reinterpret_cast<float2*>(s_ml + (warp * 8 + qc * 2 + j) * 2) = make_float2(m[t][j], l[t][j]);
 #pragma unroll
-                for (int w = 0; w < kPdWarps; ++w)
-                    L += s_ml[(w * 16 + row) * 2 + 1] * exp2_fast(s_ml[(w * 16 + row) * 2] - u);
-                const float c = exp2_fast((hi ? m1 : m0) - u);
-                if (warp > 0) {
-                    float* dst = s_o + ((warp - 1) * 8 + quad) * S::kOStride + qc * 2;
-#pragma unroll
-                    for (int i = 0; i < DP / 8; ++i)
-                        *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * hi] * c, o[i][2 * hi + 1] * c);
+                    for (int i = 0; i < DP / 16; ++i) {
+                        float* dst = s_o + (warp * 8 + qc * 2 + j) * S::kOStride + i * 16 + quad;
+                        dst[0] = o[t][i][j];
+                        dst[8] = o[t][i][2 + j];
+                    }
                 }
                 __syncthreads();
-                if (warp == 0 && row < nh) {
-                    const float* src = s_o + quad * S::kOStride + qc * 2;
-                    const float inv = whole ? (L > 0.0f ? 1.0f / L : L) : 1.0f;
-                    const int64_t part = (2 * static_cast<int64_t>(blockIdx.x) + (part_blk == 0 ? 1 : 0)) * 16 + row;
-                    const int head = kvh * p.rep + h0 + row;
-                    T* out = static_cast<T*>(p.out) + cp.b * p.out_row + head * p.out_head;
-                    float* po = p.part_o + part * p.part_stride;
+                for (int h = warp; h < 8 && t * 8 + h < nh; h += kPdWarps) {
+                    float M = -INFINITY, L = 0.0f, c[kPdWarps];
 #pragma unroll
-                    for (int i = 0; i < DP / 8; ++i) {
-                        float a = o[i][2 * hi] * c, b = o[i][2 * hi + 1] * c;
+                    for (int w = 0; w < kPdWarps; ++w) M = fmaxf(M, s_ml[(w * 8 + h) * 2]);
+                    const float u = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-                        for (int w = 0; w < kPdWarps - 1; ++w) {
-                            const float2 t = *reinterpret_cast<const float2*>(src + w * 8 * S::kOStride + i * 8);
-                            a += t.x;
-                            b += t.y;
-                        }
-                        const int d = i * 8 + qc * 2;
-                        if (!whole)
-                            *reinterpret_cast<float2*>(po + d) = make_float2(a, b);
-                        else if (d < p.c.head_dim)
-                            *reinterpret_cast<uint32_t*>(out + d) = pack2<T>(a * inv, b * inv);
+                    for (int w = 0; w < kPdWarps; ++w) {
+                        c[w] = exp2_fast(s_ml[(w * 8 + h) * 2] - u);
+                        L += s_ml[(w * 8 + h) * 2 + 1] * c[w];
                     }
-                    if (qc == 0) {
+                    const float inv = whole ? (L > 0.0f ? 1.0f / L : L) : 1.0f;
+                    const int row = t * 8 + h, head = kvh * p.rep + h0 + row;
+                    const int64_t part = (2 * static_cast<int64_t>(blockIdx.x) + (part_blk == 0 ? 1 : 0)) * 16 + row;
+                    T* out = static_cast<T*>(p.out) + cp.b * p.out_row + head * p.out_head;
+                    // a cluster's block leaves its part where the copies were (they are all consumed)
+                    float* po = CL ? reinterpret_cast<float*>(smem) + row * DP : p.part_o + part * p.part_stride;
+                    for (int d = lane * 2; d < DP; d += 64) {
+                        float a = 0.0f, b = 0.0f;
+#pragma unroll
+                        for (int w = 0; w < kPdWarps; ++w) {
+                            const float2 v = *reinterpret_cast<const float2*>(s_o + (w * 8 + h) * S::kOStride + d);
+                            a = fmaf(v.x, c[w], a);
+                            b = fmaf(v.y, c[w], b);
+                        }
+                        if (!whole) *reinterpret_cast<float2*>(po + d) = make_float2(a, b);
+                        else if (d < p.c.head_dim) *reinterpret_cast<uint32_t*>(out + d) = pack2<T>(a * inv, b * inv);
+                    }
+                    if (lane == 0) {
                         if (!whole) {
-                            *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(M, L);
+                            float* ml = CL ? reinterpret_cast<float*>(smem) + 16 * DP + row * 2 : p.part_ml + part * 2;
+                            *reinterpret_cast<float2*>(ml) = make_float2(M, L);
                         } else {
                             const float lg = L != 0.0f ? u + log2f(L) : -INFINITY;
                             if (p.lse != nullptr) p.lse[static_cast<int64_t>(cp.b) * p.heads + head] = lg * kLn2;
@@ -492,11 +623,18 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_
                         }
                     }
                 }
+                if (NT > 1 || !CL) __syncthreads();
             }
+            if (CL) break;
         }
-        cp.advance(p, end);
+        advance(cp);
     }
     cp_async_wait<0>();
+    if constexpr (CL)
+        if (p.cluster > 1) {
+            const int kvh = cp.v / p.parts, h0 = (cp.v % p.parts) * 16;
+            paged_cluster_join<T>(p, smem, DP, rank, cp.b, kvh * p.rep + h0, min(16, p.rep - h0), warp, lane);
+        }
 }
 
 // ---------------------------------------------------------------------------
@@ -544,7 +682,7 @@ __global__ void __launch_bounds__(kPdThreads) paged_decode_simt_kernel(const __g
     if (blockIdx.x == 0) paged_check_lens(p);
     if (begin >= end) return;
     PagedIter cp = paged_seek(p, begin, lane);
-    PagedLook look = paged_look(p, cp, end, warp, lane);
+    PagedLook look = paged_look<false>(p, cp, end, warp, lane);
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};   // heads 2 * part, 2 * part + 1
     float o[R][8];
     bool fresh = true;
@@ -572,7 +710,7 @@ __global__ void __launch_bounds__(kPdThreads) paged_decode_simt_kernel(const __g
         PagedIter nx = cp;
         nx.advance(p, end);
         const PagedLook cur = look;
-        look = paged_look(p, nx, end, warp, lane);
+        look = paged_look<false>(p, nx, end, warp, lane);
         const uint32_t vis = __ballot_sync(0xffffffffu, cur.page >= 0) & 0xffffu;
         if (vis || p.scores != nullptr) {
             // scores of slots slot_lane and slot_lane + 8
@@ -864,7 +1002,7 @@ __global__ void __launch_bounds__(kPdJoinThreads) paged_join_kernel(const __grid
     const int64_t wb = (static_cast<int64_t>(b) * p.c.kv_heads + g) * p.slot_cap;
     const int j0 = chunk * kPdWeightSlots + threadIdx.x * 4;
     const float* sc = p.scores + hb * p.score_stride;
-    const bool vec = r.first == r.lo && j0 + 4 <= r.len && (p.slot_cap & 3) == 0 &&
+    const bool vec = r.skip == 0 && r.first == r.lo && j0 + 4 <= r.len && (p.slot_cap & 3) == 0 &&
                      ((reinterpret_cast<uintptr_t>(p.weights) | reinterpret_cast<uintptr_t>(p.weights_out)) & 15) == 0;
     if (vec) {   // every slot visible: index = slot
         float4 w = *reinterpret_cast<const float4*>(p.weights + wb + j0);
@@ -880,8 +1018,8 @@ __global__ void __launch_bounds__(kPdJoinThreads) paged_join_kernel(const __grid
     } else {
         for (int j = j0; j < min(j0 + 4, r.len); ++j) {
             float w = p.weights[wb + j];
-            const int idx = j < r.first ? j : j >= r.lo ? r.first + j - r.lo : -1;
-            if (idx >= 0)
+            const int idx = j < r.front ? j : j - r.skip;   // its place, if it has one
+            if (j < r.first || j >= r.lo)
                 for (int h = 0; h < p.rep; ++h) w += exp2_fast(sc[h * p.score_stride + idx] - s_lse[h]);
             p.weights_out[wb + j] = w;
         }

@@ -394,11 +394,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-// Bits 0..n-1 set (none for n <= 0, all for n >= 32).
-__device__ __forceinline__ uint32_t ones_below(int n) {
-    return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
-}
-
 // One row pair by pair (a whole warp): only visible keys are touched.
 template <typename T>
 __device__ __noinline__ void window_row_exact(const WindowParams& p, const WindowTile& t, int token, int head, int lane) {
