@@ -82,13 +82,14 @@ int check_decode(const ChronosPagedDecodeArgs* a) {
     return CHRONOS_OK;
 }
 
-// The tensor-core path: 16-bit types whose rows can be copied 16 bytes at a time.
+// The tensor-core path: rows that can be copied 16 bytes at a time (fp32: up to 128
+// columns, what shared memory holds three stages of), q and out in pairs.
 bool decode_uses_mma(const ChronosPagedDecodeArgs* a) {
     const ChronosPagedCache& c = a->cache;
-    return c.dtype != CHRONOS_DTYPE_FP32 && c.head_dim % 8 == 0 && aligned(c.k_pages, 16) && aligned(c.v_pages, 16) &&
-           aligned(a->q, 4) && aligned(a->out, 4) &&
-           multiples(8, {c.k_page_stride, c.k_slot_stride, c.k_head_stride, c.v_page_stride, c.v_slot_stride,
-                         c.v_head_stride}) &&
+    const int64_t n = 16 / static_cast<int64_t>(elem_bytes(c.dtype));
+    return (c.dtype != CHRONOS_DTYPE_FP32 || c.head_dim <= 128) && c.head_dim % n == 0 && aligned(c.k_pages, 16) &&
+           aligned(c.v_pages, 16) && aligned(a->q, 8) && aligned(a->out, 8) &&
+           multiples(n, {c.k_page_stride, c.k_slot_stride, c.k_head_stride, c.v_page_stride, c.v_slot_stride, c.v_head_stride}) &&
            multiples(2, {a->q_row_stride, a->q_head_stride, a->out_row_stride, a->out_head_stride});
 }
 
@@ -96,7 +97,7 @@ bool decode_uses_mma(const ChronosPagedDecodeArgs* a) {
 int decode_cluster(const ChronosPagedDecodeArgs* a, const DecodePlan& d, int64_t blocks) {
     if (!d.mma || a->weights != nullptr) return 0;
     const int64_t rows = static_cast<int64_t>(a->cache.batch) * a->cache.kv_heads * d.parts;
-    const int64_t room = (d.dp == 256 ? 1 : 2) * static_cast<int64_t>(sm_count());
+    const int64_t room = (d.dp * elem_bytes(a->cache.dtype) == 512 ? 1 : 2) * static_cast<int64_t>(sm_count());
     int size = 1;
     while (size < 8 && size < blocks) size *= 2;
     while (size > 1 && rows * size > room) size /= 2;
@@ -108,14 +109,15 @@ DecodePlan decode_plan(const ChronosPagedDecodeArgs* a) {
     DecodePlan d{};
     d.mma = decode_uses_mma(a);
     d.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
-    d.rows = d.mma ? 16 : kPdSimtRows;
+    const bool one_block = d.dp * elem_bytes(c.dtype) == 512;   // rows of 512 bytes: one block per SM
+    d.rows = d.mma && c.dtype != CHRONOS_DTYPE_FP32 ? 16 : 8;
     const int rep = a->heads / c.kv_heads;
     d.parts = (rep + d.rows - 1) / d.rows;
     const int limit = slot_limit(c, a->slot_cap, a->weights != nullptr);
     // places of a row: both runs of visible slots start at a multiple of 16
     d.max_vis = a->window > 0 ? static_cast<int>(std::min<int64_t>(limit, static_cast<int64_t>(a->window) + a->sinks + 32)) : limit;
     d.one_page = c.page_size % kPdTile == 0;
-    const int per_sm = d.mma ? (d.dp == 256 ? 1 : 2) : 4;
+    const int per_sm = d.mma ? (one_block ? 1 : 2) : 4;
     const int64_t blocks = (static_cast<int64_t>(d.max_vis) + kPdBlock - 1) / kPdBlock;
     const int64_t units = std::max<int64_t>(1, blocks) * c.batch * c.kv_heads * d.parts;
     d.grid = static_cast<int>(std::min<int64_t>({units, static_cast<int64_t>(per_sm) * sm_count(), kPdMaxGrid}));
@@ -148,8 +150,10 @@ DecodeKernel decode_kernel(bool one_page, bool cluster) {
 
 template <typename T, int DP>
 int launch_decode_mma(const PagedDecodeParams& p, const DecodePlan& d, cudaStream_t st) {
-    using S = PagedMma<DP>;
-    const DecodeKernel kernel = p.rep > 8 ? decode_kernel<T, DP, 2>(d.one_page, d.cluster > 0) : decode_kernel<T, DP, 1>(d.one_page, d.cluster > 0);
+    using S = PagedMma<T, DP>;
+    DecodeKernel kernel = decode_kernel<T, DP, 1>(d.one_page, d.cluster > 0);
+    if constexpr (sizeof(T) == 2)
+        if (p.rep > 8) kernel = decode_kernel<T, DP, 2>(d.one_page, d.cluster > 0);
     if (int rc = set_smem(kernel, S::kSmem)) return rc;
     if (d.cluster == 0) {
         CHRONOS_CUDA_CHECK(launch_kernel(kernel, dim3(p.grid), dim3(kPdThreads), S::kSmem, st, false, p));
@@ -174,12 +178,14 @@ int launch_decode_mma(const PagedDecodeParams& p, const DecodePlan& d, cudaStrea
 
 template <typename T>
 int launch_decode(const PagedDecodeParams& p, const DecodePlan& d, bool vec, cudaStream_t st) {
-    if constexpr (sizeof(T) == 2) {
-        if (d.mma) {
-            const int rc = d.dp == 64 ? launch_decode_mma<T, 64>(p, d, st)
-                                      : d.dp == 128 ? launch_decode_mma<T, 128>(p, d, st) : launch_decode_mma<T, 256>(p, d, st);
-            if (rc || d.cluster > 0) return rc;
-        }
+    if (d.mma) {
+        int rc;
+        if constexpr (sizeof(T) == 2)
+            rc = d.dp == 64 ? launch_decode_mma<T, 64>(p, d, st)
+                            : d.dp == 128 ? launch_decode_mma<T, 128>(p, d, st) : launch_decode_mma<T, 256>(p, d, st);
+        else
+            rc = d.dp == 64 ? launch_decode_mma<T, 64>(p, d, st) : launch_decode_mma<T, 128>(p, d, st);
+        if (rc || d.cluster > 0) return rc;
     }
     if (!d.mma)
         CHRONOS_CUDA_CHECK(launch_kernel(vec ? paged_decode_simt_kernel<T, true> : paged_decode_simt_kernel<T, false>,

@@ -226,6 +226,34 @@ __device__ __forceinline__ void mma_16816<__half>(float (&d)[4], const uint32_t 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// fp32 operands by two tf32 terms each, x = hi + lo: hi is x rounded to 11 bits, lo the
+// rest, of which the tensor core takes the first 11 bits, so hi + lo is off by 2^-21 |x|
+// at most, and hi hi + hi lo + lo hi leaves out a term below 2^-22.  What is not finite
+// has no rest.
+struct Tf32Pair {
+    uint32_t hi, lo;
+};
+__device__ __forceinline__ Tf32Pair tf32_split(float x) {
+    Tf32Pair r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r.hi) : "f"(x));
+    const float lo = x - __uint_as_float(r.hi);
+    r.lo = lo == lo ? __float_as_uint(lo) : 0u;
+    return r;
+}
+__device__ __forceinline__ void mma_1688_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// d += a * (b0, b1) for a 16 x 8 piece of K or V^T and the two rows of a split operand.
+__device__ __forceinline__ void mma_fp32(float (&d)[4], const float (&a)[4], const Tf32Pair& b0, const Tf32Pair& b1) {
+    const Tf32Pair x0 = tf32_split(a[0]), x1 = tf32_split(a[1]), x2 = tf32_split(a[2]), x3 = tf32_split(a[3]);
+    mma_1688_tf32(d, x0.hi, x1.hi, x2.hi, x3.hi, b0.hi, b1.hi);
+    mma_1688_tf32(d, x0.hi, x1.hi, x2.hi, x3.hi, b0.lo, b1.lo);
+    mma_1688_tf32(d, x0.lo, x1.lo, x2.lo, x3.lo, b0.hi, b1.hi);
+}
 template <bool TRANS>
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
     if (TRANS)
@@ -316,19 +344,21 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 }
 
 // DP: the head dimension rounded up to 64, 128 or 256 (columns behind it are zero).
-template <int DP>
+template <typename T, int DP>
 struct PagedMma {
-    static constexpr int kStages = DP == 64 ? 6 : 3;
-    static constexpr int kTileBytes = kPdTile * DP * 2;                       // K or V of one warp's tile
+    static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
+    static constexpr int kStages = kRowBytes == 128 ? 6 : 3;
+    static constexpr int kTileBytes = kPdTile * kRowBytes;                    // K or V of one warp's tile
     static constexpr int kStageBytes = kPdWarps * 2 * kTileBytes;
     static constexpr int kOStride = DP + 4;                                   // fp32; four heads on different banks
     static constexpr int kMergeBytes = kPdWarps * 8 * kOStride * 4;
     static constexpr int kSmem = kStages * kStageBytes + kMergeBytes + kPdWarps * 8 * 2 * 4 + kStages * kPdWarps * 4;
-    static constexpr int kBlocksPerSm = DP == 256 ? 1 : 2;
+    static constexpr int kBlocksPerSm = kRowBytes == 512 ? 1 : 2;
+    static constexpr int kRows = sizeof(T) == 4 ? 8 : 16;                     // query heads of a unit at most
 };
 
-// HBM bound: 2 * D * 2 bytes per visible slot and kv head against 4 * D flops per
-// query head.  Transposed products, S^T = K Q^T (16 slots x 8 heads) and
+// HBM bound: 2 * D elements per visible slot and kv head against 4 * D flops per query
+// head (fp32 layers by three tf32 products each).  Transposed products, S^T = K Q^T (16 slots x 8 heads) and
 // O^T = V^T P^T (16 columns x 8 heads), take the query heads of a kv head as the
 // 8-wide operand: no row of the 16-wide one is wasted, and one movmatrix turns the
 // weights from the first product's result into the second's operand.  A warp owns 16
@@ -341,11 +371,13 @@ struct PagedMma {
 // shares its blocks of 64 places and joins through distributed shared memory;
 // otherwise block c takes the c-th share of the work list.
 template <typename T, int DP, int NT, bool ONE_PAGE, bool CL>
-__global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_decode_mma_kernel(
+__global__ void __launch_bounds__(kPdThreads, PagedMma<T, DP>::kBlocksPerSm) paged_decode_mma_kernel(
     const __grid_constant__ PagedDecodeParams p) {
-    using S = PagedMma<DP>;
+    using S = PagedMma<T, DP>;
     constexpr int NS = S::kStages;
-    constexpr int CPR = DP / 8;            // 16-byte chunks per row
+    constexpr int EPC = 16 / static_cast<int>(sizeof(T));   // elements of a 16-byte chunk
+    constexpr int CPR = DP / EPC;          // chunks per row
+    constexpr int RB = S::kRowBytes;
     constexpr int RPI = 32 / CPR;          // rows a warp copies per instruction
     constexpr float kGrow = 8.0f;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -388,7 +420,7 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_
     PagedLook look = paged_look<ONE_PAGE>(p, ld, end, warp, lane);
 
     const int ch = lane % CPR, lrow = lane / CPR;
-    const bool col = ch * 8 < p.c.head_dim;
+    const bool col = ch * EPC < p.c.head_dim;
     auto issue = [&](int stage) {
         const uint32_t sk = smem_u32(smem + stage * S::kStageBytes + warp * 2 * S::kTileBytes);
         const int64_t g = ld.v / p.parts;
@@ -396,8 +428,8 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_
         if (ONE_PAGE) {
             if (look.page < 0) vis = 0u;
             // one page: the rows stand a slot stride apart
-            const T* ks = static_cast<const T*>(p.c.k_pages) + g * p.c.k_head_stride + ch * 8;
-            const T* vs = static_cast<const T*>(p.c.v_pages) + g * p.c.v_head_stride + ch * 8;
+            const T* ks = static_cast<const T*>(p.c.k_pages) + g * p.c.k_head_stride + ch * EPC;
+            const T* vs = static_cast<const T*>(p.c.v_pages) + g * p.c.v_head_stride + ch * EPC;
             if (vis) {
                 ks += look.page * p.c.k_page_stride + (look.slot + lrow) * p.c.k_slot_stride;
                 vs += look.page * p.c.v_page_stride + (look.slot + lrow) * p.c.v_slot_stride;
@@ -407,7 +439,7 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_
             for (int i = 0; i < kPdTile / RPI; ++i) {
                 const int r = i * RPI + lrow;
                 const bool ok = col && ((vis >> r) & 1u);
-                const uint32_t off = static_cast<uint32_t>(r * DP * 2 + ((ch ^ (r & 7)) << 4));
+                const uint32_t off = static_cast<uint32_t>(r * RB + ((ch ^ (r & 7)) << 4));
                 cp_async16(sk + off, ok ? ks : p.c.k_pages, ok);
                 cp_async16(sk + S::kTileBytes + off, ok ? vs : p.c.v_pages, ok);
                 ks += kstep;
@@ -415,15 +447,15 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_
             }
         } else {
             vis &= __ballot_sync(0xffffffffu, look.page >= 0) & 0xffffu;
-            const T* kb = static_cast<const T*>(p.c.k_pages) + g * p.c.k_head_stride + ch * 8;
-            const T* vb = static_cast<const T*>(p.c.v_pages) + g * p.c.v_head_stride + ch * 8;
+            const T* kb = static_cast<const T*>(p.c.k_pages) + g * p.c.k_head_stride + ch * EPC;
+            const T* vb = static_cast<const T*>(p.c.v_pages) + g * p.c.v_head_stride + ch * EPC;
 #pragma unroll
             for (int i = 0; i < kPdTile / RPI; ++i) {
                 const int r = i * RPI + lrow;
                 const int page = __shfl_sync(0xffffffffu, look.page, r);
                 const int64_t slot = __shfl_sync(0xffffffffu, look.slot, r);
                 const bool ok = col && ((vis >> r) & 1u);
-                const uint32_t off = static_cast<uint32_t>(r * DP * 2 + ((ch ^ (r & 7)) << 4));
+                const uint32_t off = static_cast<uint32_t>(r * RB + ((ch ^ (r & 7)) << 4));
                 cp_async16(sk + off, ok ? kb + page * p.c.k_page_stride + slot * p.c.k_slot_stride : p.c.k_pages, ok);
                 cp_async16(sk + S::kTileBytes + off, ok ? vb + page * p.c.v_page_stride + slot * p.c.v_slot_stride : p.c.v_pages, ok);
             }
@@ -445,18 +477,21 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int kr = (lane & 7) + ((lane >> 3) & 1) * 8, vr = (lane & 7) + (lane >> 4) * 8;
-        koff[i] = static_cast<uint32_t>(kr * DP * 2 + (((2 * i + (lane >> 4)) ^ (lane & 7)) << 4));
-        voff[i] = static_cast<uint32_t>(S::kTileBytes + vr * DP * 2 + (((2 * i + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+        koff[i] = static_cast<uint32_t>(kr * RB + (((2 * i + (lane >> 4)) ^ (lane & 7)) << 4));
+        voff[i] = static_cast<uint32_t>(S::kTileBytes + vr * RB + (((2 * i + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
     }
-    uint32_t qb[NT][DP / 16][2];
+    constexpr bool F32 = sizeof(T) == 4;
+    static_assert(!F32 || NT == 1, "fp32 units have 8 heads");
+    uint32_t qb[NT][F32 ? 1 : DP / 16][2];
+    Tf32Pair qf[F32 ? DP / 8 : 1][2];
     float o[NT][DP / 16][4];
     float m[NT][2], l[NT][2];
     bool fresh = true;          // the next unit opens a new part or row
     int part_blk = 0;           // the block it opened with
     int stage = 0;
     while (cp.u < end || (CL && fresh)) {
-        const int kvh = cp.v / p.parts, h0 = (cp.v % p.parts) * 16;
-        const int nh = min(16, p.rep - h0);             // query heads of this unit
+        const int kvh = cp.v / p.parts, h0 = (cp.v % p.parts) * S::kRows;
+        const int nh = min(S::kRows, p.rep - h0);             // query heads of this unit
         if (fresh) {
             fresh = false;
             part_blk = cp.blk;
@@ -469,13 +504,21 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_
                 for (int i = 0; i < DP / 16; ++i) {
                     o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
+                    for (int j = 0; j < 2 && !F32; ++j) {
                         const int row = t * 8 + quad, d = i * 16 + qc * 2 + j * 8;
                         qb[t][i][j] = row < nh && d < p.c.head_dim
                                           ? *reinterpret_cast<const uint32_t*>(q + row * p.q_head + d) : 0u;
                     }
                 }
             }
+            if constexpr (F32)
+#pragma unroll
+                for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int d = i * 8 + qc + j * 4;
+                        qf[i][j] = tf32_split(quad < nh && d < p.c.head_dim ? to_f32<T>(q[quad * p.q_head + d]) : 0.0f);
+                    }
         }
         if (ld.u < end) {
             issue(stage == 0 ? NS - 1 : stage - 1);
@@ -492,11 +535,17 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_
 #pragma unroll
             for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
 #pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk) {
+            for (int kk = 0; kk < RB / 32; ++kk) {   // 32 bytes of every slot's row at a time
                 uint32_t ka[4];
                 ldmatrix_x4<false>(ka, st + koff[kk & 3] + (kk >> 2) * 128);
+                if constexpr (F32) {
+                    const float a[4] = {__uint_as_float(ka[0]), __uint_as_float(ka[1]), __uint_as_float(ka[2]),
+                                        __uint_as_float(ka[3])};
+                    mma_fp32(s[0], a, qf[kk][0], qf[kk][1]);
+                } else {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) mma_16816<T>(s[t], ka, qb[t][kk][0], qb[t][kk][1]);
+                    for (int t = 0; t < NT; ++t) mma_16816<T>(s[t], ka, qb[t][kk][0], qb[t][kk][1]);
+                }
             }
             // s[t][0..1]: slot quad, heads 8t + 2qc, + 1; s[t][2..3]: slot quad + 8
             const bool on0 = (vis >> quad) & 1u, on1 = (vis >> (quad + 8)) & 1u;
@@ -542,6 +591,7 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_
                     }
             }
             uint32_t pb[NT][2];
+            Tf32Pair pf[F32 ? 4 : 1];   // [8 slots][2 rows of 4]
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const float u0 = m[t][0] == -INFINITY ? 0.0f : m[t][0], u1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
@@ -549,16 +599,42 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_
                 const float c = exp2_fast(s[t][2] - u0), d = exp2_fast(s[t][3] - u1);
                 l[t][0] += a + c;
                 l[t][1] += b + d;
+                if constexpr (F32) {
+                    // row k of 8 slots, head quad: held by the lane of slot k and pair quad / 2
+                    const float w[4] = {a, b, c, d};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int src = (qc + (i & 1) * 4) * 4 + (quad >> 1);
+                        const float x = __shfl_sync(0xffffffffu, w[(i >> 1) * 2], src);
+                        const float y = __shfl_sync(0xffffffffu, w[(i >> 1) * 2 + 1], src);
+                        pf[i] = tf32_split((quad & 1) ? y : x);
+                    }
+                    continue;
+                }
                 // weights in T for the second product; the sum keeps fp32
                 pb[t][0] = transpose8x8(pack2<T>(a, b));
                 pb[t][1] = transpose8x8(pack2<T>(c, d));
             }
 #pragma unroll
             for (int dd = 0; dd < DP / 16; ++dd) {
-                uint32_t va[4];
-                ldmatrix_x4<true>(va, st + voff[dd & 3] + (dd >> 2) * 128);
+                if constexpr (F32) {
+                    const uint8_t* v = smem + stage * S::kStageBytes + warp * 2 * S::kTileBytes + S::kTileBytes;
 #pragma unroll
-                for (int t = 0; t < NT; ++t) mma_16816<T>(o[t][dd], va, pb[t][0], pb[t][1]);
+                    for (int k = 0; k < 2; ++k) {   // slots 8k .. 8k + 7
+                        float a[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int slot = k * 8 + qc + (i >> 1) * 4, d = dd * 16 + quad + (i & 1) * 8;
+                            a[i] = *reinterpret_cast<const float*>(v + slot * RB + (((d >> 2) ^ (slot & 7)) << 4) + (d & 3) * 4);
+                        }
+                        mma_fp32(o[0][dd], a, pf[2 * k], pf[2 * k + 1]);
+                    }
+                } else {
+                    uint32_t va[4];
+                    ldmatrix_x4<true>(va, st + voff[dd & 3] + (dd >> 2) * 128);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) mma_16816<T>(o[t][dd], va, pb[t][0], pb[t][1]);
+                }
             }
         }
         __syncwarp();   // every lane has read the tile before its stage is filled again
@@ -597,7 +673,7 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_
                     }
                     const float inv = whole ? (L > 0.0f ? 1.0f / L : L) : 1.0f;
                     const int row = t * 8 + h, head = kvh * p.rep + h0 + row;
-                    const int64_t part = (2 * static_cast<int64_t>(blockIdx.x) + (part_blk == 0 ? 1 : 0)) * 16 + row;
+                    const int64_t part = (2 * static_cast<int64_t>(blockIdx.x) + (part_blk == 0 ? 1 : 0)) * S::kRows + row;
                     T* out = static_cast<T*>(p.out) + cp.b * p.out_row + head * p.out_head;
                     // a cluster's block leaves its part where the copies were (they are all consumed)
                     float* po = CL ? reinterpret_cast<float*>(smem) + row * DP : p.part_o + part * p.part_stride;
@@ -610,7 +686,10 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_
                             b = fmaf(v.y, c[w], b);
                         }
                         if (!whole) *reinterpret_cast<float2*>(po + d) = make_float2(a, b);
-                        else if (d < p.c.head_dim) *reinterpret_cast<uint32_t*>(out + d) = pack2<T>(a * inv, b * inv);
+                        else if (d < p.c.head_dim) {
+                            if constexpr (F32) *reinterpret_cast<float2*>(out + d) = make_float2(a * inv, b * inv);
+                            else *reinterpret_cast<uint32_t*>(out + d) = pack2<T>(a * inv, b * inv);
+                        }
                     }
                     if (lane == 0) {
                         if (!whole) {
@@ -632,14 +711,14 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<DP>::kBlocksPerSm) paged_
     cp_async_wait<0>();
     if constexpr (CL)
         if (p.cluster > 1) {
-            const int kvh = cp.v / p.parts, h0 = (cp.v % p.parts) * 16;
-            paged_cluster_join<T>(p, smem, DP, rank, cp.b, kvh * p.rep + h0, min(16, p.rep - h0), warp, lane);
+            const int kvh = cp.v / p.parts, h0 = (cp.v % p.parts) * S::kRows;
+            paged_cluster_join<T>(p, smem, DP, rank, cp.b, kvh * p.rep + h0, min(S::kRows, p.rep - h0), warp, lane);
         }
 }
 
 // ---------------------------------------------------------------------------
-// general path: fp32 (no tensor-core product keeps its precision), head
-// dimensions or strides the copies above cannot take.  Same work list; 8 query
+// general path: head dimensions or strides the copies above cannot take, fp32 heads
+// of more than 128.  Same work list; 8 query
 // heads at once, fp32 products.  K: four lanes share a slot (their partial dot
 // products meet in two shuffles), two slots per lane in flight; V: the lanes
 // split the columns and run over the warp's 16 slots.
