@@ -58,6 +58,7 @@ struct DecodePlan {
     bool mma;
     int dp;              // padded head dimension of the tensor-core path
     bool one_page;       // 16 consecutive aligned slots lie in one page
+    int per_sm;          // blocks an SM holds
     int cluster;         // blocks per row in one cluster; 0: the work list and a second kernel
     int rows, parts, grid, part_stride, max_vis;
     int64_t score_stride;
@@ -97,7 +98,7 @@ bool decode_uses_mma(const ChronosPagedDecodeArgs* a) {
 int decode_cluster(const ChronosPagedDecodeArgs* a, const DecodePlan& d, int64_t blocks) {
     if (!d.mma || a->weights != nullptr) return 0;
     const int64_t rows = static_cast<int64_t>(a->cache.batch) * a->cache.kv_heads * d.parts;
-    const int64_t room = (d.dp * elem_bytes(a->cache.dtype) == 512 ? 1 : 2) * static_cast<int64_t>(sm_count());
+    const int64_t room = static_cast<int64_t>(d.per_sm) * sm_count();
     int size = 1;
     while (size < 8 && size < blocks) size *= 2;
     while (size > 1 && rows * size > room) size /= 2;
@@ -109,7 +110,7 @@ DecodePlan decode_plan(const ChronosPagedDecodeArgs* a) {
     DecodePlan d{};
     d.mma = decode_uses_mma(a);
     d.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
-    const bool one_block = d.dp * elem_bytes(c.dtype) == 512;   // rows of 512 bytes: one block per SM
+    d.per_sm = !d.mma ? 4 : d.dp * elem_bytes(c.dtype) == 128 ? 3 : 2;   // PagedMma::kBlocksPerSm
     d.rows = d.mma && c.dtype != CHRONOS_DTYPE_FP32 ? 16 : 8;
     const int rep = a->heads / c.kv_heads;
     d.parts = (rep + d.rows - 1) / d.rows;
@@ -117,10 +118,9 @@ DecodePlan decode_plan(const ChronosPagedDecodeArgs* a) {
     // places of a row: both runs of visible slots start at a multiple of 16
     d.max_vis = a->window > 0 ? static_cast<int>(std::min<int64_t>(limit, static_cast<int64_t>(a->window) + a->sinks + 32)) : limit;
     d.one_page = c.page_size % kPdTile == 0;
-    const int per_sm = d.mma ? (one_block ? 1 : 2) : 4;
     const int64_t blocks = (static_cast<int64_t>(d.max_vis) + kPdBlock - 1) / kPdBlock;
     const int64_t units = std::max<int64_t>(1, blocks) * c.batch * c.kv_heads * d.parts;
-    d.grid = static_cast<int>(std::min<int64_t>({units, static_cast<int64_t>(per_sm) * sm_count(), kPdMaxGrid}));
+    d.grid = static_cast<int>(std::min<int64_t>({units, static_cast<int64_t>(d.per_sm) * sm_count(), kPdMaxGrid}));
     d.cluster = decode_cluster(a, d, blocks);
     d.part_stride = d.mma ? d.dp : static_cast<int>(round_up(c.head_dim, 4));
     size_t at = 0;
