@@ -52,7 +52,11 @@ int slot_limit(const ChronosPagedCache& c, int64_t slot_cap, bool has_cap) {
 // ---------------------------------------------------------------------------
 // one-token attention
 // ---------------------------------------------------------------------------
-constexpr int kPdClusterBlocks = 6;   // blocks of 64 places that a block of a cluster takes at most
+// Blocks of 64 places that a block of a cluster takes at most, where the clusters leave
+// more than half of the grid idle / where they do not.  (8 each: one row set of 4096 slots
+// on 64 of 296 blocks 16.4 us, 12.3 us by the work list; 64 rows up to 2048 slots on 256
+// blocks 16.4 us, 18.4 us by the list; 256 rows up to 512 slots 12.4 and 20.5 us.)
+constexpr int kPdClusterBlocks = 6, kPdClusterBlocksFull = 8;
 
 struct DecodePlan {
     bool mma;
@@ -102,7 +106,8 @@ int decode_cluster(const ChronosPagedDecodeArgs* a, const DecodePlan& d, int64_t
     int size = 1;
     while (size < 8 && size < blocks) size *= 2;
     while (size > 1 && rows * size > room) size /= 2;
-    return rows * size <= room && blocks <= kPdClusterBlocks * size ? size : 0;
+    const int64_t most = 2 * rows * size > room ? kPdClusterBlocksFull : kPdClusterBlocks;
+    return rows * size <= room && blocks <= most * size ? size : 0;
 }
 
 DecodePlan decode_plan(const ChronosPagedDecodeArgs* a) {

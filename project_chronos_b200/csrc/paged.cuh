@@ -349,7 +349,7 @@ struct PagedMma {
     static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
     // Rows of 512 bytes have one stage, K and V of which are filled again separately as
     // soon as each is read: two blocks per SM then hide each other's waits (three stages
-    // and one block per SM: 168 against 118 us for 16 x 16384 slots in fp32).
+    // and one block per SM: 168 against 117 us for 16 x 16384 slots in fp32).
     static constexpr int kStages = kRowBytes == 512 ? 1 : 3;
     static constexpr int kTileBytes = kPdTile * kRowBytes;                    // K or V of one warp's tile
     static constexpr int kStageBytes = kPdWarps * 2 * kTileBytes;
@@ -1270,18 +1270,35 @@ __device__ __forceinline__ uint32_t evict_key(float w, int pos, int sinks, int64
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+// Sum of the values that the warps before this one left in x[kEvictWarps] (whole warps
+// call it; `total`: of all warps).
+__device__ __forceinline__ int evict_before(const int* x, int warp, int lane, int* total = nullptr) {
+    const int v = x[lane];
+    int inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += t;
+    }
+    if (total != nullptr) *total = __shfl_sync(0xffffffffu, inc, 31);
+    return __shfl_sync(0xffffffffu, inc - v, warp);
+}
+
 // One block per (sequence, kv head).  The budget-th largest key by radix
 // selection (three counting passes over 11, 11 and 10 bits, counters in shared
-// memory), then ordered passes over the slots: every warp owns a contiguous
-// piece, counts in it, and a scan over the warps gives each its first rank.
+// memory, the first pass while the keys are formed), then ordered passes over the
+// slots: every warp owns a contiguous piece, counts in it, and a scan over the
+// warps gives each its first rank.  Bound by latency: a row's 8 bytes per slot
+// pass one SM (2049 slots 6 us, 32768 slots 25 us).
 __global__ void __launch_bounds__(kEvictThreads) paged_evict_select_kernel(const __grid_constant__ PagedEvictParams p) {
     extern __shared__ uint32_t s_keys[];   // [max_slots] when keys_in_smem
-    __shared__ int s_hist[kEvictBins];
-    __shared__ int s_a[kEvictWarps], s_b[kEvictWarps];
-    __shared__ int s_digit, s_above;
+    __shared__ int s_hist[3][kEvictBins];
+    __shared__ int s_a[3][kEvictWarps], s_b[kEvictWarps];
+    __shared__ int s_digit[3], s_above[3];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row = blockIdx.x, b = row / p.c.kv_heads;
     const int raw = p.c.lens[b];
+    const int64_t newest = static_cast<int64_t>(p.seen[b]) - p.recent;
     const int n = min(max(raw, 0), p.max_slots);
     if (threadIdx.x == 0 && raw != n) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
     const int64_t base = row * p.slot_cap;
@@ -1300,14 +1317,29 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_select_kernel(const
         if (threadIdx.x == 0) p.counts[row] = 0;
         return;
     }
-    const int64_t newest = static_cast<int64_t>(p.seen[b]) - p.recent;
     auto key = [&](int j) -> uint32_t {
         return p.keys_in_smem ? s_keys[j] : evict_key(w[j], pos[j], p.sinks, newest);
     };
-    if (p.keys_in_smem) {
+    for (int i = threadIdx.x; i < 3 * kEvictBins; i += kEvictThreads) (&s_hist[0][0])[i] = 0;
+    __syncthreads();
+    auto first = [&](int j, float a, int c) {
+        const uint32_t k = evict_key(a, c, p.sinks, newest);
+        if (p.keys_in_smem) s_keys[j] = k;
+        atomicAdd(&s_hist[0][k >> 21], 1);
+    };
+    const bool vec = (p.slot_cap & 3) == 0 &&
+                     ((reinterpret_cast<uintptr_t>(p.weights) | reinterpret_cast<uintptr_t>(p.positions)) & 15) == 0;
+    const int whole = vec ? n / 4 : 0;
 #pragma unroll 4
-        for (int j = threadIdx.x; j < n; j += kEvictThreads) s_keys[j] = evict_key(w[j], pos[j], p.sinks, newest);
+    for (int i = threadIdx.x; i < whole; i += kEvictThreads) {
+        const float4 a = reinterpret_cast<const float4*>(w)[i];
+        const int4 c = reinterpret_cast<const int4*>(pos)[i];
+        first(4 * i, a.x, c.x);
+        first(4 * i + 1, a.y, c.y);
+        first(4 * i + 2, a.z, c.z);
+        first(4 * i + 3, a.w, c.w);
     }
+    for (int j = 4 * whole + threadIdx.x; j < n; j += kEvictThreads) first(j, w[j], pos[j]);
     // radix selection: `prefix` the digits found, `want` the rank still to find below it
     uint32_t prefix = 0, known = 0;
     int want = p.budget;
@@ -1315,87 +1347,81 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_select_kernel(const
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
         const uint32_t mask = (1u << bits) - 1u;
-        for (int i = threadIdx.x; i < kEvictBins; i += kEvictThreads) s_hist[i] = 0;
-        __syncthreads();
-        for (int j = threadIdx.x; j < n; j += kEvictThreads) {
-            const uint32_t k = key(j);
-            if ((k & known) == prefix) atomicAdd(&s_hist[(k >> shift) & mask], 1);
-        }
+        if (pass > 0)
+            for (int j = threadIdx.x; j < n; j += kEvictThreads) {
+                const uint32_t k = key(j);
+                if ((k & known) == prefix) atomicAdd(&s_hist[pass][(k >> shift) & mask], 1);
+            }
         __syncthreads();
         // digit d such that fewer than `want` keys lie above it, and with it at least `want`:
         // thread i holds the two highest digits not yet held by threads before it
         const int d0 = kEvictBins - 1 - 2 * threadIdx.x;
-        const int h0 = s_hist[d0], h1 = s_hist[d0 - 1];
+        const int h0 = s_hist[pass][d0], h1 = s_hist[pass][d0 - 1];
         int inc = h0 + h1;
 #pragma unroll
         for (int x = 1; x < 32; x <<= 1) {
             const int t = __shfl_up_sync(0xffffffffu, inc, x);
             if (lane >= x) inc += t;
         }
-        if (lane == 31) s_a[warp] = inc;
+        if (lane == 31) s_a[pass][warp] = inc;
         __syncthreads();
-        int above = inc - h0 - h1;
-        for (int i = 0; i < warp; ++i) above += s_a[i];
+        const int above = inc - h0 - h1 + evict_before(s_a[pass], warp, lane);
         if (above < want && above + h0 >= want) {
-            s_digit = d0;
-            s_above = above;
+            s_digit[pass] = d0;
+            s_above[pass] = above;
         } else if (above + h0 < want && above + h0 + h1 >= want) {
-            s_digit = d0 - 1;
-            s_above = above + h0;
+            s_digit[pass] = d0 - 1;
+            s_above[pass] = above + h0;
         }
         __syncthreads();
-        prefix |= static_cast<uint32_t>(s_digit) << shift;
+        prefix |= static_cast<uint32_t>(s_digit[pass]) << shift;
         known |= mask << shift;
-        want -= s_above;
-        __syncthreads();
+        want -= s_above[pass];
     }
     // kept: keys above `prefix`, and the first `want` slots whose key equals it
     const int per = ((n + kEvictWarps - 1) / kEvictWarps + 31) / 32 * 32;
     const int j0 = min(n, warp * per), j1 = min(n, j0 + per);
     int eq = 0;
+#pragma unroll 4
     for (int j = j0 + lane; j - lane < j1; j += 32)
         eq += __popc(__ballot_sync(0xffffffffu, j < j1 && key(min(j, n - 1)) == prefix));
-    if (lane == 0) s_a[warp] = eq;
+    if (lane == 0) s_a[0][warp] = eq;
     __syncthreads();
-    int eq0 = 0;
-    for (int i = 0; i < warp; ++i) eq0 += s_a[i];
+    const int eq0 = evict_before(s_a[0], warp, lane);
     const uint32_t below = (1u << lane) - 1u;
     // holes (slots below the budget given up) and movers (kept slots beyond it), counted, then listed
-    int holes = 0, movers = 0;
+    int holes = 0, movers = 0, count = 0;
     int32_t* mv = p.moves + static_cast<int64_t>(row) * p.max_moves * 2;
 #pragma unroll
     for (int pass = 0; pass < 2; ++pass) {
         int rank = eq0, h = holes, m = movers;
+#pragma unroll 2
         for (int j = j0 + lane; j - lane < j1; j += 32) {
             const bool in = j < j1;
-            const uint32_t k = in ? key(j) : 0u;
+            const uint32_t k = key(min(j, n - 1));
             const uint32_t eqs = __ballot_sync(0xffffffffu, in && k == prefix);
             const bool keep = in && (k > prefix || (k == prefix && rank + __popc(eqs & below) < want));
             rank += __popc(eqs);
-            const uint32_t hb = __ballot_sync(0xffffffffu, in && !keep && j < p.budget);
-            const uint32_t mb = __ballot_sync(0xffffffffu, keep && j >= p.budget);
+            const bool hole = in && !keep && j < p.budget, mover = keep && j >= p.budget;
+            const uint32_t hb = __ballot_sync(0xffffffffu, hole), mb = __ballot_sync(0xffffffffu, mover);
             if (pass) {
-                if (in && !keep && j < p.budget) mv[2 * (h + __popc(hb & below))] = j;
-                if (keep && j >= p.budget) mv[2 * (m + __popc(mb & below)) + 1] = j;
+                if (hole) mv[2 * (h + __popc(hb & below))] = j;
+                if (mover) mv[2 * (m + __popc(mb & below)) + 1] = j;
             }
             h += __popc(hb);
             m += __popc(mb);
         }
         if (pass == 0) {
-            __syncthreads();
             if (lane == 0) {
-                s_a[warp] = h;
+                s_a[1][warp] = h;
                 s_b[warp] = m;
             }
             __syncthreads();
-            for (int i = 0; i < warp; ++i) {
-                holes += s_a[i];
-                movers += s_b[i];
-            }
+            holes = evict_before(s_a[1], warp, lane, &count);
+            movers = evict_before(s_b, warp, lane);
         }
     }
-    int count = 0;
-    for (int i = 0; i < kEvictWarps; ++i) count += s_a[i];
+#pragma unroll 4
     for (int j = threadIdx.x; j < p.budget; j += kEvictThreads) {
         src[j] = j;
         if (p.weights_out != p.weights) p.weights_out[base + j] = w[j];
@@ -1403,22 +1429,25 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_select_kernel(const
     }
     if (threadIdx.x == 0) p.counts[row] = count;
     __syncthreads();   // the lists and the copies above are written
+#pragma unroll 4
     for (int i = threadIdx.x; i < count; i += kEvictThreads) {
-        const int to = mv[2 * i], from = mv[2 * i + 1];
-        src[to] = from;
-        p.weights_out[base + to] = w[from];
-        p.positions_out[base + to] = pos[from];
+        const int2 move = reinterpret_cast<const int2*>(mv)[i];
+        src[move.x] = move.y;
+        p.weights_out[base + move.x] = w[move.y];
+        p.positions_out[base + move.x] = pos[move.y];
     }
 }
 
 constexpr int kEvictMoveThreads = 256;
-constexpr int kEvictMovesPerBlock = 64;
+constexpr int kEvictMovesPerBlock = kEvictMoveThreads / 32 * 4;
 
-// The K and V rows of the moves: one warp per move, sources (slots >= budget)
-// and targets (slots < budget) never overlap, so the order does not matter.
+// The K and V rows of the moves, read once and written once: a warp takes four moves at
+// a time (all four rows' loads in flight before the first store).  Sources (slots >=
+// budget) and targets (slots < budget) never overlap, so the order does not matter.
 template <typename V>
 __global__ void __launch_bounds__(kEvictMoveThreads) paged_evict_move_kernel(const __grid_constant__ PagedEvictParams p,
                                                                              int units, int elems_per_unit) {
+    constexpr int M = 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row = blockIdx.y, b = row / p.c.kv_heads, g = row % p.c.kv_heads;
     pdl_wait();
@@ -1429,26 +1458,42 @@ __global__ void __launch_bounds__(kEvictMoveThreads) paged_evict_move_kernel(con
     const int es = static_cast<int>(sizeof(V)) / elems_per_unit;
     char* kp = static_cast<char*>(p.c.k_pages);
     char* vp = static_cast<char*>(p.c.v_pages);
-    for (int i0 = blockIdx.x * kEvictMovesPerBlock; i0 < count; i0 += gridDim.x * kEvictMovesPerBlock)
-        for (int i = i0 + warp; i < min(count, i0 + kEvictMovesPerBlock); i += kEvictMoveThreads / 32) {
-            const int to = mv[2 * i], from = mv[2 * i + 1];
-            const int tp = table[to / p.c.page_size], fp = table[from / p.c.page_size];
-            if (tp < 0 || tp >= p.c.num_pages || fp < 0 || fp >= p.c.num_pages) {
-                if (lane == 0) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
-                continue;
-            }
-            const int64_t ts = to % p.c.page_size, fs = from % p.c.page_size;
-            for (int u = lane; u < 2 * units; u += 32) {
-                const bool isv = u >= units;
-                const int64_t e = static_cast<int64_t>(isv ? u - units : u) * elems_per_unit;
-                char* base = isv ? vp : kp;
-                const int64_t ps = isv ? p.c.v_page_stride : p.c.k_page_stride;
-                const int64_t ss = isv ? p.c.v_slot_stride : p.c.k_slot_stride;
-                const int64_t hs = g * (isv ? p.c.v_head_stride : p.c.k_head_stride) + e;
-                *reinterpret_cast<V*>(base + (tp * ps + ts * ss + hs) * es) =
-                    *reinterpret_cast<const V*>(base + (fp * ps + fs * ss + hs) * es);
-            }
+    const int step = gridDim.x * (kEvictMoveThreads / 32) * M;
+    for (int i0 = (blockIdx.x * (kEvictMoveThreads / 32) + warp) * M; i0 < count; i0 += step) {
+        // lanes 2m and 2m + 1: target and source of move m, as offsets of their K and V rows
+        int64_t ko = 0, vo = 0;
+        bool ok = false;
+        if (lane < 2 * M && i0 + lane / 2 < count) {
+            const int slot = mv[2 * i0 + lane];
+            const int page = table[slot / p.c.page_size];
+            const int64_t in = slot % p.c.page_size;
+            ok = page >= 0 && page < p.c.num_pages;
+            if (!ok) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
+            ko = (page * p.c.k_page_stride + in * p.c.k_slot_stride + g * p.c.k_head_stride) * es;
+            vo = (page * p.c.v_page_stride + in * p.c.v_slot_stride + g * p.c.v_head_stride) * es;
         }
+        const uint32_t good = __ballot_sync(0xffffffffu, ok);
+        for (int u0 = 0; u0 < 2 * units; u0 += 32) {
+            const int u = u0 + lane;
+            const bool isv = u >= units;
+            const int64_t e = static_cast<int64_t>(isv ? u - units : u) * elems_per_unit * es;
+            V x[M];
+            char* to[M];
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                const int64_t kt = __shfl_sync(0xffffffffu, ko, 2 * m), kf = __shfl_sync(0xffffffffu, ko, 2 * m + 1);
+                const int64_t vt = __shfl_sync(0xffffffffu, vo, 2 * m), vf = __shfl_sync(0xffffffffu, vo, 2 * m + 1);
+                to[m] = nullptr;
+                if (u < 2 * units && ((good >> (2 * m)) & 3u) == 3u) {
+                    to[m] = (isv ? vp + vt : kp + kt) + e;
+                    x[m] = *reinterpret_cast<const V*>((isv ? vp + vf : kp + kf) + e);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+                if (to[m] != nullptr) *reinterpret_cast<V*>(to[m]) = x[m];
+        }
+    }
 }
 
 }  // namespace chronos
