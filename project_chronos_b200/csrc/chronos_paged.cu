@@ -210,9 +210,13 @@ int launch_decode(const PagedDecodeParams& p, const DecodePlan& d, bool vec, cud
 // ---------------------------------------------------------------------------
 // eviction
 // ---------------------------------------------------------------------------
+constexpr int kEvictKeyBytes = 192 * 1024;   // of shared memory for the keys of a row
+static_assert(kEvictKeyBytes / 4 / 32 <= 3 * kEvictBins / 2, "the bits of such a row fit the counters' place");
+
 struct EvictPlan {
     int64_t max_moves;
-    size_t o_moves, o_counts, o_lens, total;
+    int64_t bit_words;      // 0 where a row's keys (and then its bits) fit shared memory
+    size_t o_moves, o_counts, o_lens, o_bits, total;
 };
 
 int check_evict(const ChronosPagedEvictArgs* a) {
@@ -235,7 +239,9 @@ EvictPlan evict_plan(const ChronosPagedEvictArgs* a) {
     e.o_moves = 0;
     e.o_counts = round_up(rows * e.max_moves * 8, 256);
     e.o_lens = e.o_counts + round_up(rows * 4, 256);
-    e.total = e.o_lens + round_up(static_cast<size_t>(a->cache.batch) * 4, 256) + 256;
+    e.o_bits = e.o_lens + round_up(static_cast<size_t>(a->cache.batch) * 4, 256);
+    e.bit_words = static_cast<int64_t>(limit) * 4 <= kEvictKeyBytes ? 0 : (limit + 31) / 32;
+    e.total = e.o_bits + rows * e.bit_words * 8 + 256;
     return e;
 }
 
@@ -491,12 +497,13 @@ extern "C" int chronos_paged_evict(const ChronosPagedEvictArgs* a, void* stream)
     p.lens_copy = reinterpret_cast<int32_t*>(ws + e.o_lens);
     p.max_moves = e.max_moves;
     p.status = a->status;
-    constexpr int kKeyBytes = 192 * 1024;
     const int64_t key_bytes = static_cast<int64_t>(p.max_slots) * 4;
-    p.keys_in_smem = key_bytes <= kKeyBytes;
+    p.keys_in_smem = key_bytes <= kEvictKeyBytes;
+    p.bits = reinterpret_cast<uint32_t*>(ws + e.o_bits);
+    p.bit_words = e.bit_words;
     const int smem = p.keys_in_smem ? static_cast<int>(key_bytes) : 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (int rc = set_smem(paged_evict_select_kernel, kKeyBytes)) return rc;
+    if (int rc = set_smem(paged_evict_select_kernel, kEvictKeyBytes)) return rc;
     CHRONOS_CUDA_CHECK(launch_kernel(paged_evict_select_kernel, dim3(rows), dim3(kEvictThreads), smem, st, false, p));
     const int es = static_cast<int>(elem_bytes(a->cache.dtype));
     const bool wide = copies16(a->cache);

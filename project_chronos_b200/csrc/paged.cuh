@@ -1250,6 +1250,8 @@ struct PagedEvictParams {
     int32_t* src;
     int max_slots;
     int keys_in_smem;      // 1: a row's keys fit shared memory, else they are formed again from the inputs
+    uint32_t* bits;        // [B * G][2][bit_words] for rows whose keys do not fit
+    int64_t bit_words;
     int32_t* moves;        // [B * G][max_moves][2]: (slot given up, slot that moves there)
     int32_t* counts;       // [B * G]
     int32_t* lens_copy;    // [B] lens_out may be the caller's lens
@@ -1286,9 +1288,9 @@ __device__ __forceinline__ int evict_before(const int* x, int warp, int lane, in
 
 // One block per (sequence, kv head).  The budget-th largest key by radix
 // selection (three counting passes over 11, 11 and 10 bits, counters in shared
-// memory, the first pass while the keys are formed), then ordered passes over the
-// slots: every warp owns a contiguous piece, counts in it, and a scan over the
-// warps gives each its first rank.  Bound by latency: a row's 8 bytes per slot
+// memory, the first pass while the keys are formed), then one bit per slot for
+// what is kept, and scans of their counts, which give every hole and every slot that
+// moves its rank.  Bound by latency: a row's 8 bytes per slot
 // pass one SM (2049 slots 6 us, 32768 slots 25 us).
 __global__ void __launch_bounds__(kEvictThreads) paged_evict_select_kernel(const __grid_constant__ PagedEvictParams p) {
     extern __shared__ uint32_t s_keys[];   // [max_slots] when keys_in_smem
@@ -1378,48 +1380,57 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_select_kernel(const
         known |= mask << shift;
         want -= s_above[pass];
     }
-    // kept: keys above `prefix`, and the first `want` slots whose key equals it
-    const int per = ((n + kEvictWarps - 1) / kEvictWarps + 31) / 32 * 32;
-    const int j0 = min(n, warp * per), j1 = min(n, j0 + per);
-    int eq = 0;
+    // kept: keys above `prefix`, and the first `want` slots whose key equals it.  One pass over
+    // the keys leaves both as bits; from there on a thread owns contiguous words of 32 slots.
+    const int words = (n + 31) / 32;
+    uint32_t* more = p.keys_in_smem ? reinterpret_cast<uint32_t*>(&s_hist[0][0])
+                                    : p.bits + static_cast<int64_t>(row) * 2 * p.bit_words;
+    uint32_t* same = more + (p.keys_in_smem ? 3 * kEvictBins / 2 : p.bit_words);
 #pragma unroll 4
-    for (int j = j0 + lane; j - lane < j1; j += 32)
-        eq += __popc(__ballot_sync(0xffffffffu, j < j1 && key(min(j, n - 1)) == prefix));
-    if (lane == 0) s_a[0][warp] = eq;
+    for (int j = warp * 32 + lane; j - lane < n; j += kEvictThreads) {
+        const bool in = j < n;
+        const uint32_t k = key(min(j, n - 1));
+        const uint32_t gt = __ballot_sync(0xffffffffu, in && k > prefix), eq = __ballot_sync(0xffffffffu, in && k == prefix);
+        if (lane == 0) {
+            more[j >> 5] = gt;
+            same[j >> 5] = eq;
+        }
+    }
     __syncthreads();
-    const int eq0 = evict_before(s_a[0], warp, lane);
-    const uint32_t below = (1u << lane) - 1u;
-    // holes (slots below the budget given up) and movers (kept slots beyond it), counted, then listed
-    int holes = 0, movers = 0, count = 0;
-    int32_t* mv = p.moves + static_cast<int64_t>(row) * p.max_moves * 2;
+    const int per = (words + kEvictThreads - 1) / kEvictThreads;
+    const int w0 = min(words, static_cast<int>(threadIdx.x) * per), w1 = min(words, w0 + per);
+    // exclusive prefix of a thread's count, over the block
+    auto before = [&](int mine, int* x, int* total) {
+        int inc = mine;
 #pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {
-        int rank = eq0, h = holes, m = movers;
-#pragma unroll 2
-        for (int j = j0 + lane; j - lane < j1; j += 32) {
-            const bool in = j < j1;
-            const uint32_t k = key(min(j, n - 1));
-            const uint32_t eqs = __ballot_sync(0xffffffffu, in && k == prefix);
-            const bool keep = in && (k > prefix || (k == prefix && rank + __popc(eqs & below) < want));
-            rank += __popc(eqs);
-            const bool hole = in && !keep && j < p.budget, mover = keep && j >= p.budget;
-            const uint32_t hb = __ballot_sync(0xffffffffu, hole), mb = __ballot_sync(0xffffffffu, mover);
-            if (pass) {
-                if (hole) mv[2 * (h + __popc(hb & below))] = j;
-                if (mover) mv[2 * (m + __popc(mb & below)) + 1] = j;
-            }
-            h += __popc(hb);
-            m += __popc(mb);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += t;
         }
-        if (pass == 0) {
-            if (lane == 0) {
-                s_a[1][warp] = h;
-                s_b[warp] = m;
-            }
-            __syncthreads();
-            holes = evict_before(s_a[1], warp, lane, &count);
-            movers = evict_before(s_b, warp, lane);
-        }
+        if (lane == 31) x[warp] = inc;
+        __syncthreads();
+        return inc - mine + evict_before(x, warp, lane, total);
+    };
+    int eq = 0;
+    for (int i = w0; i < w1; ++i) eq += __popc(same[i]);
+    int rank = before(eq, s_a[0], nullptr);
+    int holes = 0, movers = 0, count = 0;
+    for (int i = w0; i < w1; ++i) {
+        uint32_t take = same[i];
+        const int room = max(0, want - rank);
+        rank += __popc(take);
+        while (__popc(take) > room) take &= ~(0x80000000u >> __clz(take));   // the lower slots first
+        const uint32_t keep = more[i] | take, low = ones_below(p.budget - 32 * i);
+        more[i] = keep;
+        holes += __popc(~keep & low & ones_below(n - 32 * i));
+        movers += __popc(keep & ~low);
+    }
+    int h = before(holes, s_a[1], &count), m = before(movers, s_b, nullptr);
+    int32_t* mv = p.moves + static_cast<int64_t>(row) * p.max_moves * 2;
+    for (int i = w0; i < w1; ++i) {
+        const uint32_t keep = more[i], low = ones_below(p.budget - 32 * i);
+        for (uint32_t x = ~keep & low & ones_below(n - 32 * i); x; x &= x - 1) mv[2 * h++] = 32 * i + __ffs(x) - 1;
+        for (uint32_t x = keep & ~low; x; x &= x - 1) mv[2 * m++ + 1] = 32 * i + __ffs(x) - 1;
     }
 #pragma unroll 4
     for (int j = threadIdx.x; j < p.budget; j += kEvictThreads) {
