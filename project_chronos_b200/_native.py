@@ -343,6 +343,8 @@ class ChronosMoeError(RuntimeError):
 def load_library(path: str = LIB_PATH):
     """Load (once) and return the extension; raises if it is missing or stale."""
     global _lib
+    if _lib is not None:   # loaded: no lock on the way of every call
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

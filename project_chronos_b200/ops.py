@@ -527,97 +527,98 @@ def attn_decode(kind: str, proj: torch.Tensor, pos: torch.Tensor, cos: torch.Ten
 # paged key-value cache (include/chronos_paged.h)
 # ---------------------------------------------------------------------------
 
-def _forward_only(*ts: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled():
-        for t in ts:
-            if t is not None and t.requires_grad:
-                raise RuntimeError("forward-only kernels: call under torch.no_grad() or detach the inputs")
-
-
-def _check_i32(name: str, t: torch.Tensor, shape: tuple, dev: torch.device) -> int:
-    if t.dtype != torch.int32 or t.device != dev or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor {shape} on {dev}, got {t.dtype} {tuple(t.shape)} "
-                         f"on {t.device}")
-    return t.data_ptr()
-
-
-def _check_rows(name: str, t: torch.Tensor, shape: tuple, dt: torch.dtype, dev: torch.device) -> None:
-    """Rows of vectors: the last dimension contiguous, the others by their strides."""
+def _refuse(name: str, t: torch.Tensor, shape, dt: torch.dtype, dev: torch.device, contiguous: bool) -> None:
+    """Say what is wrong with a tensor that a paged call cannot take."""
     if t.dtype != dt or t.device != dev:
         raise TypeError(f"{name}: {dt} on {dev} expected, got {t.dtype} on {t.device}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
     if t.stride(-1) != 1 and t.shape[-1] != 1:
         raise ValueError(f"{name}'s last dimension must be contiguous")
+    if t.requires_grad:
+        raise RuntimeError("forward-only kernels: call under torch.no_grad() or detach the inputs")
 
 
-def _check_slots(name: str, t: torch.Tensor, shape: tuple, dt: torch.dtype, dev: torch.device) -> int:
-    """A per-slot array [B, kv heads, slots]."""
-    if t.dtype != dt or t.device != dev or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dt} tensor {shape} on {dev}, got {t.dtype} {tuple(t.shape)} "
-                         f"on {t.device}")
+def _rows(name: str, t: torch.Tensor, shape: tuple, dt: torch.dtype, index: int, dev: torch.device, grad: bool) -> tuple:
+    """Strides of a tensor of vectors: the last dimension contiguous, the others by their strides."""
+    st = t.stride()
+    if (t.dtype is not dt or t.get_device() != index or t.shape != shape or (st[-1] != 1 and shape[-1] != 1)
+            or (grad and t.requires_grad)):
+        _refuse(name, t, shape, dt, dev, False)
+    return st
+
+
+def _dense(name: str, t: torch.Tensor, shape: tuple, dt: torch.dtype, index: int, dev: torch.device) -> int:
+    """Address of a contiguous tensor."""
+    if t.dtype is not dt or t.get_device() != index or t.shape != shape or not t.is_contiguous():
+        _refuse(name, t, shape, dt, dev, True)
     return t.data_ptr()
 
 
-def _written_once(name: str, t: torch.Tensor) -> None:
+def _written_once(name: str, shape, strides) -> None:
     """Refuse a tensor that is written through and holds one element at several places."""
-    for n, s in zip(t.shape, t.stride()):
-        if n > 1 and s == 0:
-            raise ValueError(f"{name} is written: it must not be expanded")
+    if 0 in strides:
+        for n, s in zip(shape, strides):
+            if n > 1 and s == 0:
+                raise ValueError(f"{name} is written: it must not be expanded")
+
+
+def _no_cpu(t: torch.Tensor) -> None:
+    raise RuntimeError(f"chronos paged kernels need CUDA tensors (no CPU path exists); got a tensor on {t.device}")
 
 
 def _paged_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
-                 written: bool) -> N.ChronosPagedCache:
+                 written: bool, dev: torch.device, index: int, grad: bool) -> N.ChronosPagedCache:
     """The checked cache part of a paged call's arguments."""
-    if not k_pages.is_cuda:
-        raise RuntimeError(f"chronos paged kernels need CUDA tensors (no CPU path exists); got a tensor on {k_pages.device}")
-    dev, dt = k_pages.device, k_pages.dtype
-    if dt not in _DTYPES:
+    dt = k_pages.dtype
+    code = _DTYPES.get(dt)
+    if code is None:
         raise TypeError(f"unsupported dtype {dt}")
-    if k_pages.dim() != 4:
-        raise ValueError(f"k_pages must be [pages, page size, kv heads, head dim], got {tuple(k_pages.shape)}")
-    _check_rows("v_pages", v_pages, tuple(k_pages.shape), dt, dev)
-    if k_pages.stride(3) != 1 and k_pages.shape[3] != 1:
-        raise ValueError("k_pages' last dimension must be contiguous")
+    shape = k_pages.shape
+    if len(shape) != 4:
+        raise ValueError(f"k_pages must be [pages, page size, kv heads, head dim], got {tuple(shape)}")
+    pages, size, g, d = shape
+    ks = _rows("k_pages", k_pages, shape, dt, index, dev, grad)
+    vs = _rows("v_pages", v_pages, shape, dt, index, dev, grad)
     if written:
-        _written_once("k_pages", k_pages)
-        _written_once("v_pages", v_pages)
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != dev:
-        raise ValueError(f"page_table must be an int32 tensor [B, pages] on {dev}")
+        _written_once("k_pages", shape, ks)
+        _written_once("v_pages", shape, vs)
+    ts = page_table.stride()
+    if page_table.dtype is not torch.int32 or page_table.get_device() != index or len(ts) != 2 \
+            or (ts[1] != 1 and page_table.shape[1] > 1):
+        raise ValueError(f"page_table must be an int32 tensor [B, pages] on {dev} with contiguous rows")
     b, width = page_table.shape
-    if width > 1 and page_table.stride(1) != 1:
-        raise ValueError("page_table's rows must be contiguous")
-    pages, size, g, d = k_pages.shape
-    kp, ks, kh, _ = k_pages.stride()
-    vp, vs, vh, _ = v_pages.stride()
-    return N.ChronosPagedCache(b, g, d, _DTYPES[dt], pages, size, width, 0, k_pages.data_ptr(), v_pages.data_ptr(),
-                               kp, ks, kh, vp, vs, vh, page_table.data_ptr(), page_table.stride(0),
-                               _check_i32("lens", lens, (b,), dev))
+    return N.ChronosPagedCache(b, g, d, code, pages, size, width, 0, k_pages.data_ptr(), v_pages.data_ptr(),
+                               ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], page_table.data_ptr(), ts[0],
+                               _dense("lens", lens, (b,), torch.int32, index, dev))
 
 
-def _launch(fn, args, dev: torch.device) -> None:
-    """Call ``fn`` on ``dev``'s current stream (the device of the tensors, whatever
-    the current device is)."""
-    stream = ctypes.c_void_p(_raw_stream(dev.index))
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(ctypes.byref(args), stream)
+def _launch(fn, args, index: int) -> None:
+    """Call ``fn`` on the current stream of device ``index`` (the tensors' device,
+    whatever the current device is)."""
+    if torch.cuda.current_device() == index:
+        rc = fn(args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(ctypes.byref(args), stream)
-    N.check(rc)
+        with torch.cuda.device(index):
+            rc = fn(args, _raw_stream(index))
+    if rc:
+        N.check(rc)
 
 
-def _workspace(fn, args, dev: torch.device) -> torch.Tensor:
+def _workspace(fn, args, dev: torch.device, index: int) -> torch.Tensor:
     """Workspace of one call from torch's allocator: a captured graph keeps its own."""
-    if torch.cuda.current_device() == dev.index:
-        nbytes = fn(ctypes.byref(args))
+    if torch.cuda.current_device() == index:
+        nbytes = fn(args)
     else:
-        with torch.cuda.device(dev):
-            nbytes = fn(ctypes.byref(args))
+        with torch.cuda.device(index):
+            nbytes = fn(args)
     if nbytes == 0:
         N.check(N.CHRONOS_ERR_INVALID_ARG)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+    args.workspace = ws.data_ptr()
+    args.workspace_bytes = nbytes
     return ws
 
 
@@ -634,26 +635,29 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     ``weights`` fp32 [B, kv heads, slots] get 0 there and ``positions`` int32 of
     that shape seen[b] + i (``seen`` int32 [B]: tokens seen before).  A page must
     not belong to two sequences that are written."""
-    _forward_only(k, v, k_pages, v_pages)
-    cache = _paged_cache(k_pages, v_pages, page_table, lens, written=True)
-    dev, dt = k_pages.device, k_pages.dtype
-    b, g, d = cache.batch, cache.kv_heads, cache.head_dim
+    if not k_pages.is_cuda:
+        _no_cpu(k_pages)
+    dev, index, grad = k_pages.device, k_pages.get_device(), torch.is_grad_enabled()
+    cache = _paged_cache(k_pages, v_pages, page_table, lens, True, dev, index, grad)
+    b, g, d, dt = cache.batch, cache.kv_heads, cache.head_dim, k_pages.dtype
     t = k.shape[0]
-    _check_rows("k", k, (t, g, d), dt, dev)
-    _check_rows("v", v, (t, g, d), dt, dev)
+    ks = _rows("k", k, (t, g, d), dt, index, dev, grad)
+    vs = _rows("v", v, (t, g, d), dt, index, dev, grad)
     cap, wp, pp = 0, None, None
-    for name, x, want in (("weights", weights, torch.float32), ("positions", positions, torch.int32)):
-        if x is not None:
-            if cap and x.shape[-1] != cap:
-                raise ValueError("weights and positions must have the same number of slots")
-            cap = x.shape[-1]
-            ptr = _check_slots(name, x, (b, g, cap), want, dev)
-            wp, pp = (ptr, pp) if name == "weights" else (wp, ptr)
+    if weights is not None:
+        cap = weights.shape[-1]
+        wp = _dense("weights", weights, (b, g, cap), torch.float32, index, dev)
+    if positions is not None:
+        if weights is not None and positions.shape[-1] != cap:
+            raise ValueError("weights and positions must have the same number of slots")
+        cap = positions.shape[-1]
+        pp = _dense("positions", positions, (b, g, cap), torch.int32, index, dev)
     args = N.ChronosPagedAppendArgs(
-        cache, t, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-        None if cu_seqlens is None else _check_i32("cu_seqlens", cu_seqlens, (b + 1,), dev),
-        None if seen is None else _check_i32("seen", seen, (b,), dev), wp, pp, cap, status_word(dev).data_ptr())
-    _launch(N.load_library().chronos_paged_append, args, dev)
+        cache, t, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
+        None if cu_seqlens is None else _dense("cu_seqlens", cu_seqlens, (b + 1,), torch.int32, index, dev),
+        None if seen is None else _dense("seen", seen, (b,), torch.int32, index, dev), wp, pp, cap,
+        status_word(dev).data_ptr())
+    _launch(N.load_library().chronos_paged_append, args, index)
 
 
 def paged_attn_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -670,35 +674,35 @@ def paged_attn_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     sum.  ``weights`` fp32 [B, kv heads, slots]: weights_out (default: in place)
     receives weights plus every slot's attention weight summed over the group's
     heads; slots at or behind lens are left as they are."""
-    _forward_only(q, k_pages, v_pages)
-    cache = _paged_cache(k_pages, v_pages, page_table, lens, written=False)
-    dev, dt = k_pages.device, k_pages.dtype
-    b, d = cache.batch, cache.head_dim
+    if not k_pages.is_cuda:
+        _no_cpu(k_pages)
+    dev, index, grad = k_pages.device, k_pages.get_device(), torch.is_grad_enabled()
+    cache = _paged_cache(k_pages, v_pages, page_table, lens, False, dev, index, grad)
+    b, d, dt = cache.batch, cache.head_dim, k_pages.dtype
     h = q.shape[1] if q.dim() == 3 else 0
-    _check_rows("q", q, (b, h, d), dt, dev)
+    shape = (b, h, d)
+    qs = _rows("q", q, shape, dt, index, dev, grad)
     if out is None:
-        out = torch.empty(b, h, d, dtype=dt, device=dev)
+        out = torch.empty(shape, dtype=dt, device=dev)
+        os = out.stride()
     else:
-        _check_rows("out", out, (b, h, d), dt, dev)
-        _written_once("out", out)
+        os = _rows("out", out, shape, dt, index, dev, grad)
+        _written_once("out", shape, os)
     cap, wp, wo = 0, None, None
     if weights is not None:
         cap = weights.shape[-1]
-        wp = _check_slots("weights", weights, (b, cache.kv_heads, cap), torch.float32, dev)
-        wo = wp if weights_out is None else _check_slots("weights_out", weights_out, tuple(weights.shape),
-                                                         torch.float32, dev)
+        slots = (b, cache.kv_heads, cap)
+        wp = _dense("weights", weights, slots, torch.float32, index, dev)
+        wo = wp if weights_out is None else _dense("weights_out", weights_out, slots, torch.float32, index, dev)
     elif weights_out is not None:
         raise ValueError("weights_out needs weights")
-    if lse is not None and (lse.dtype != torch.float32 or lse.device != dev or tuple(lse.shape) != (b, h)
-                            or not lse.is_contiguous()):
-        raise ValueError(f"lse must be a contiguous fp32 tensor {(b, h)} on {dev}")
     args = N.ChronosPagedDecodeArgs(
-        cache, h, int(window), int(sinks), d ** -0.5 if scale is None else float(scale), q.data_ptr(), q.stride(0),
-        q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse), wp, wo, cap, None, 0,
+        cache, h, window, sinks, d ** -0.5 if scale is None else scale, q.data_ptr(), qs[0], qs[1], out.data_ptr(),
+        os[0], os[1], None if lse is None else _dense("lse", lse, (b, h), torch.float32, index, dev), wp, wo, cap, None, 0,
         status_word(dev).data_ptr())
     lib = N.load_library()
-    ws = _workspace(lib.chronos_paged_decode_workspace, args, dev)  # noqa: F841 (held until the launch)
-    _launch(lib.chronos_paged_decode, args, dev)
+    ws = _workspace(lib.chronos_paged_decode_workspace, args, dev, index)  # noqa: F841 (held until the launch)
+    _launch(lib.chronos_paged_decode, args, index)
     return out
 
 
@@ -716,29 +720,34 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.
     lens int32 [B] (``lens_out`` or new), src int32 [B, kv heads, budget], the slot
     that now sits in each slot (-1 behind the length).  A page must not belong to two
     sequences."""
-    _forward_only(k_pages, v_pages, weights)
-    cache = _paged_cache(k_pages, v_pages, page_table, lens, written=True)
-    dev = k_pages.device
+    if not k_pages.is_cuda:
+        _no_cpu(k_pages)
+    dev, index, grad = k_pages.device, k_pages.get_device(), torch.is_grad_enabled()
+    cache = _paged_cache(k_pages, v_pages, page_table, lens, True, dev, index, grad)
     b, g = cache.batch, cache.kv_heads
     cap = weights.shape[-1]
     shape = (b, g, cap)
-    wp = _check_slots("weights", weights, shape, torch.float32, dev)
-    pp = _check_slots("positions", positions, shape, torch.int32, dev)
-    weights_out = weights if weights_out is None else weights_out
-    positions_out = positions if positions_out is None else positions_out
-    wo = _check_slots("weights_out", weights_out, shape, torch.float32, dev)
-    po = _check_slots("positions_out", positions_out, shape, torch.int32, dev)
+    wp = _dense("weights", weights, shape, torch.float32, index, dev)
+    pp = _dense("positions", positions, shape, torch.int32, index, dev)
+    if weights_out is None:
+        weights_out, wo = weights, wp
+    else:
+        wo = _dense("weights_out", weights_out, shape, torch.float32, index, dev)
+    if positions_out is None:
+        positions_out, po = positions, pp
+    else:
+        po = _dense("positions_out", positions_out, shape, torch.int32, index, dev)
     if lens_out is None:
         lens_out = torch.empty(b, dtype=torch.int32, device=dev)
-    if int(budget) < 1:
+    if budget < 1:
         raise ValueError(f"budget {budget} must be at least 1")
-    src = torch.empty(b, g, int(budget), dtype=torch.int32, device=dev)
+    src = torch.empty((b, g, budget), dtype=torch.int32, device=dev)
     args = N.ChronosPagedEvictArgs(
-        cache, int(budget), int(sinks), int(recent), 0, _check_i32("seen", seen, (b,), dev), wp, pp, wo, po, cap,
-        _check_i32("lens_out", lens_out, (b,), dev), src.data_ptr(), None, 0, status_word(dev).data_ptr())
+        cache, budget, sinks, recent, 0, _dense("seen", seen, (b,), torch.int32, index, dev), wp, pp, wo, po, cap,
+        _dense("lens_out", lens_out, (b,), torch.int32, index, dev), src.data_ptr(), None, 0, status_word(dev).data_ptr())
     lib = N.load_library()
-    ws = _workspace(lib.chronos_paged_evict_workspace, args, dev)  # noqa: F841 (held until the launch)
-    _launch(lib.chronos_paged_evict, args, dev)
+    ws = _workspace(lib.chronos_paged_evict_workspace, args, dev, index)  # noqa: F841 (held until the launch)
+    _launch(lib.chronos_paged_evict, args, index)
     return dict(lens=lens_out, weights=weights_out, positions=positions_out, src=src)
 
 
@@ -756,39 +765,40 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     out [Tq, heads, D]: zeros for a row that sees nothing, rows behind the last
     sequence as they were (``out``) or undefined; ``lse`` fp32 [Tq, heads]."""
     if not q.is_cuda:
-        raise RuntimeError(f"chronos paged kernels need CUDA tensors (no CPU path exists); got a tensor on {q.device}")
-    _forward_only(q, k, v)
-    dev, dt = q.device, q.dtype
-    if dt not in _DTYPES:
+        _no_cpu(q)
+    dev, index, grad = q.device, q.get_device(), torch.is_grad_enabled()
+    dt = q.dtype
+    code = _DTYPES.get(dt)
+    if code is None:
         raise TypeError(f"unsupported dtype {dt}")
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"q and k must be [rows, heads, head dim], got {tuple(q.shape)} and {tuple(k.shape)}")
-    tq, h, d = q.shape
+    shape = tq, h, d = tuple(q.shape)
     tk, g, _ = k.shape
-    _check_rows("q", q, (tq, h, d), dt, dev)
-    _check_rows("k", k, (tk, g, d), dt, dev)
-    _check_rows("v", v, (tk, g, d), dt, dev)
-    if cu_seqlens_k is None:
-        cu_seqlens_k = cu_seqlens
-        if tk != tq:
-            raise ValueError(f"{tq} query rows and {tk} key rows need cu_seqlens_k")
-    b = cu_seqlens.numel() - 1
-    if b < 0:
+    qs = _rows("q", q, shape, dt, index, dev, grad)
+    ks = _rows("k", k, (tk, g, d), dt, index, dev, grad)
+    vs = _rows("v", v, (tk, g, d), dt, index, dev, grad)
+    n = cu_seqlens.numel()
+    if n < 1:
         raise ValueError("cu_seqlens must have one more entry than there are sequences")
-    if out is None:
-        out = torch.empty(tq, h, d, dtype=dt, device=dev)
+    cq = _dense("cu_seqlens", cu_seqlens, (n,), torch.int32, index, dev)
+    if cu_seqlens_k is not None:
+        ck = _dense("cu_seqlens_k", cu_seqlens_k, (n,), torch.int32, index, dev)
+    elif tk != tq:
+        raise ValueError(f"{tq} query rows and {tk} key rows need cu_seqlens_k")
     else:
-        _check_rows("out", out, (tq, h, d), dt, dev)
-        _written_once("out", out)
-    if lse is not None and (lse.dtype != torch.float32 or lse.device != dev or tuple(lse.shape) != (tq, h)
-                            or not lse.is_contiguous()):
-        raise ValueError(f"lse must be a contiguous fp32 tensor {(tq, h)} on {dev}")
+        ck = cq
+    if out is None:
+        out = torch.empty(shape, dtype=dt, device=dev)
+        os = out.stride()
+    else:
+        os = _rows("out", out, shape, dt, index, dev, grad)
+        _written_once("out", shape, os)
     args = N.ChronosWindowAttnArgs(
-        b, h, g, d, _DTYPES[dt], int(window), int(sinks), d ** -0.5 if scale is None else float(scale), tq, tk,
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-        v.stride(0), v.stride(1), out.stride(0), out.stride(1), _check_i32("cu_seqlens", cu_seqlens, (b + 1,), dev),
-        _check_i32("cu_seqlens_k", cu_seqlens_k, (b + 1,), dev), _ptr(lse), status_word(dev).data_ptr())
-    _launch(N.load_library().chronos_window_attention, args, dev)
+        n - 1, h, g, d, code, window, sinks, d ** -0.5 if scale is None else scale, tq, tk, q.data_ptr(), k.data_ptr(),
+        v.data_ptr(), out.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], cq, ck,
+        None if lse is None else _dense("lse", lse, (tq, h), torch.float32, index, dev), status_word(dev).data_ptr())
+    _launch(N.load_library().chronos_window_attention, args, index)
     return out
 
 
