@@ -99,7 +99,7 @@ typedef struct ChronosPagedDecodeArgs {
     const float* weights;      /* [B, G, slot_cap] or NULL */
     float* weights_out;
     int64_t slot_cap;
-    void* workspace;           /* chronos_paged_decode_workspace bytes, 256-byte aligned */
+    void* workspace;           /* chronos_paged_decode_workspace bytes, 256-byte aligned; NULL for 0 */
     size_t workspace_bytes;
     int32_t* status;
 } ChronosPagedDecodeArgs;
@@ -165,8 +165,9 @@ CHRONOS_API int chronos_paged_decode(const ChronosPagedDecodeArgs* args, void* c
 CHRONOS_API int chronos_paged_evict(const ChronosPagedEvictArgs* args, void* cuda_stream);
 CHRONOS_API int chronos_window_attention(const ChronosWindowAttnArgs* args, void* cuda_stream);
 
-/* Workspace bytes of a call, from its shapes (the buffers need not be set);
- * 0 with chronos_moe_last_error set for an invalid shape. */
+/* Workspace bytes of a call, from its shapes and the alignment of its buffers (set
+ * them as for the call); 0 where it needs none, and, with chronos_moe_last_error
+ * set, for an invalid shape. */
 CHRONOS_API size_t chronos_paged_decode_workspace(const ChronosPagedDecodeArgs* args);
 CHRONOS_API size_t chronos_paged_evict_workspace(const ChronosPagedEvictArgs* args);
 

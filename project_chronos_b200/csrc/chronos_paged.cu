@@ -142,7 +142,7 @@ DecodePlan decode_plan(const ChronosPagedDecodeArgs* a) {
         d.o_lse2 = take(static_cast<size_t>(c.batch) * a->heads * 4);
         d.o_scores = take(static_cast<size_t>(c.batch) * a->heads * d.score_stride * 4);
     }
-    d.total = std::max<size_t>(at, 256);
+    d.total = d.cluster > 0 ? 0 : std::max<size_t>(at, 256);   // a cluster needs none
     return d;
 }
 
@@ -255,11 +255,19 @@ bool copies16(const ChronosPagedCache& c) {
 // ---------------------------------------------------------------------------
 // prompt attention
 // ---------------------------------------------------------------------------
+template <typename T, bool VEC>
+auto window_simt_pick(int dim) -> void (*)(WindowParams) {
+    return dim <= 64 ? window_simt_kernel<T, 1, VEC>
+           : dim <= 128 ? window_simt_kernel<T, 2, VEC>
+           : dim <= 192 ? window_simt_kernel<T, 3, VEC> : window_simt_kernel<T, 4, VEC>;
+}
+
 template <typename T>
 int launch_window_simt(const WindowParams& p, cudaStream_t st) {
-    void (*kernel)(WindowParams) = p.dim <= 64 ? window_simt_kernel<T, 1>
-                                   : p.dim <= 128 ? window_simt_kernel<T, 2>
-                                   : p.dim <= 192 ? window_simt_kernel<T, 3> : window_simt_kernel<T, 4>;
+    const size_t four = 4 * sizeof(T);
+    const bool vec = p.dim % 4 == 0 && aligned(p.q, four) && aligned(p.k, four) && aligned(p.v, four) &&
+                     multiples(4, {p.q_row, p.q_head, p.k_row, p.k_head, p.v_row, p.v_head});
+    void (*kernel)(WindowParams) = vec ? window_simt_pick<T, true>(p.dim) : window_simt_pick<T, false>(p.dim);
     const int smem = window_simt_smem(p.dim);
     if (int rc = set_smem(kernel, smem)) return rc;
     const int64_t tiles = (p.num_q + kWsRows - 1) / kWsRows + p.batch;
@@ -355,7 +363,7 @@ extern "C" int chronos_paged_decode(const ChronosPagedDecodeArgs* a, void* strea
                          static_cast<int64_t>(a->cache.batch) * a->cache.kv_heads * (limit / kPdWeightSlots + 1);
     if (units >= INT32_MAX || adds >= INT32_MAX)
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: batch %d * heads * slots %d too large", what, a->cache.batch, limit);
-    if (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < d.total)
+    if (d.total > 0 && (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < d.total))
         return fail(CHRONOS_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes, %zu (256-byte aligned) needed", what,
                     a->workspace == nullptr ? size_t{0} : a->workspace_bytes, d.total);
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
@@ -504,11 +512,17 @@ extern "C" int chronos_paged_evict(const ChronosPagedEvictArgs* a, void* stream)
     const int smem = p.keys_in_smem ? static_cast<int>(key_bytes) : 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (int rc = set_smem(paged_evict_select_kernel, kEvictKeyBytes)) return rc;
-    CHRONOS_CUDA_CHECK(launch_kernel(paged_evict_select_kernel, dim3(rows), dim3(kEvictThreads), smem, st, false, p));
     const int es = static_cast<int>(elem_bytes(a->cache.dtype));
     const bool wide = copies16(a->cache);
     const int per = wide ? 16 / es : 1;
     const int units = a->cache.head_dim / per;
+    // Few moves per row (a cache that gives up a page's slots at a time): the selecting block
+    // makes them, without the second kernel.  Not where lens_out is lens, which the other kv
+    // heads' blocks still read.
+    p.move_here = wide && e.max_moves <= kEvictMovesHere &&
+                  (a->lens_out + a->cache.batch <= a->cache.lens || a->cache.lens + a->cache.batch <= a->lens_out);
+    CHRONOS_CUDA_CHECK(launch_kernel(paged_evict_select_kernel, dim3(rows), dim3(kEvictThreads), smem, st, false, p, units, per));
+    if (p.move_here) return CHRONOS_OK;
     const int64_t bx = std::max<int64_t>(1, std::min<int64_t>((e.max_moves + kEvictMovesPerBlock - 1) / kEvictMovesPerBlock, 4096));
     const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(rows)), block(kEvictMoveThreads);
     if (wide) CHRONOS_CUDA_CHECK(launch_kernel(paged_evict_move_kernel<uint4>, grid, block, 0, st, true, p, units, per));

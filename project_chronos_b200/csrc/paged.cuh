@@ -1256,9 +1256,13 @@ struct PagedEvictParams {
     int32_t* counts;       // [B * G]
     int32_t* lens_copy;    // [B] lens_out may be the caller's lens
     int64_t max_moves;
+    int move_here;         // 1: the selecting block moves the rows (16-byte units) and writes lens_out
     int32_t* status;
 };
 
+// Slots beyond the budget up to which the selecting block moves the rows itself: 32 warps
+// with four rows each.
+constexpr int kEvictMovesHere = 128;
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictBins = 2048;   // 11 + 11 + 10 bits of the key
@@ -1270,6 +1274,54 @@ __device__ __forceinline__ uint32_t evict_key(float w, int pos, int sinks, int64
     if (w != w) return 0xfffffffeu;
     const uint32_t u = __float_as_uint(w + 0.0f);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+// The K and V rows of the moves, read once and written once: a warp takes four moves at
+// a time (all four rows' loads in flight before the first store).  Sources (slots >=
+// budget) and targets (slots < budget) never overlap, so the order does not matter.
+template <typename V>
+__device__ __forceinline__ void paged_move_rows(const PagedEvictParams& p, int b, int g, const int32_t* mv, int count,
+                                                int warp, int warps, int lane, int units, int elems_per_unit) {
+    constexpr int M = 4;
+    const int32_t* table = p.c.page_table + b * p.c.page_table_stride;
+    const int es = static_cast<int>(sizeof(V)) / elems_per_unit;
+    char* kp = static_cast<char*>(p.c.k_pages);
+    char* vp = static_cast<char*>(p.c.v_pages);
+    for (int i0 = warp * M; i0 < count; i0 += warps * M) {
+        // lanes 2m and 2m + 1: target and source of move m, as offsets of their K and V rows
+        int64_t ko = 0, vo = 0;
+        bool ok = false;
+        if (lane < 2 * M && i0 + lane / 2 < count) {
+            const int slot = mv[2 * i0 + lane];
+            const int page = table[slot / p.c.page_size];
+            const int64_t in = slot % p.c.page_size;
+            ok = page >= 0 && page < p.c.num_pages;
+            if (!ok) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
+            ko = (page * p.c.k_page_stride + in * p.c.k_slot_stride + g * p.c.k_head_stride) * es;
+            vo = (page * p.c.v_page_stride + in * p.c.v_slot_stride + g * p.c.v_head_stride) * es;
+        }
+        const uint32_t good = __ballot_sync(0xffffffffu, ok);
+        for (int u0 = 0; u0 < 2 * units; u0 += 32) {
+            const int u = u0 + lane;
+            const bool isv = u >= units;
+            const int64_t e = static_cast<int64_t>(isv ? u - units : u) * elems_per_unit * es;
+            V x[M];
+            char* to[M];
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                const int64_t kt = __shfl_sync(0xffffffffu, ko, 2 * m), kf = __shfl_sync(0xffffffffu, ko, 2 * m + 1);
+                const int64_t vt = __shfl_sync(0xffffffffu, vo, 2 * m), vf = __shfl_sync(0xffffffffu, vo, 2 * m + 1);
+                to[m] = nullptr;
+                if (u < 2 * units && ((good >> (2 * m)) & 3u) == 3u) {
+                    to[m] = (isv ? vp + vt : kp + kt) + e;
+                    x[m] = *reinterpret_cast<const V*>((isv ? vp + vf : kp + kf) + e);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+                if (to[m] != nullptr) *reinterpret_cast<V*>(to[m]) = x[m];
+        }
+    }
 }
 
 // Sum of the values that the warps before this one left in x[kEvictWarps] (whole warps
@@ -1292,7 +1344,8 @@ __device__ __forceinline__ int evict_before(const int* x, int warp, int lane, in
 // what is kept, and scans of their counts, which give every hole and every slot that
 // moves its rank.  Bound by latency: a row's 8 bytes per slot
 // pass one SM (2049 slots 6 us, 32768 slots 25 us).
-__global__ void __launch_bounds__(kEvictThreads) paged_evict_select_kernel(const __grid_constant__ PagedEvictParams p) {
+__global__ void __launch_bounds__(kEvictThreads) paged_evict_select_kernel(const __grid_constant__ PagedEvictParams p,
+                                                                              int units, int elems_per_unit) {
     extern __shared__ uint32_t s_keys[];   // [max_slots] when keys_in_smem
     __shared__ int s_hist[3][kEvictBins];
     __shared__ int s_a[3][kEvictWarps], s_b[kEvictWarps];
@@ -1307,7 +1360,10 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_select_kernel(const
     const float* w = p.weights + base;
     const int32_t* pos = p.positions + base;
     int32_t* src = p.src + static_cast<int64_t>(row) * p.budget;
-    if (row % p.c.kv_heads == 0 && threadIdx.x == 0) p.lens_copy[b] = n;
+    if (row % p.c.kv_heads == 0 && threadIdx.x == 0) {
+        if (p.move_here) p.lens_out[b] = min(n, p.budget);
+        else p.lens_copy[b] = n;
+    }
     if (n <= p.budget) {
         for (int j = threadIdx.x; j < p.budget; j += kEvictThreads) src[j] = j < n ? j : -1;
         for (int j = threadIdx.x; j < n; j += kEvictThreads) {
@@ -1447,64 +1503,21 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_select_kernel(const
         p.weights_out[base + move.x] = w[move.y];
         p.positions_out[base + move.x] = pos[move.y];
     }
+    if (p.move_here) paged_move_rows<uint4>(p, b, row % p.c.kv_heads, mv, count, warp, kEvictWarps, lane, units, elems_per_unit);
 }
 
 constexpr int kEvictMoveThreads = 256;
 constexpr int kEvictMovesPerBlock = kEvictMoveThreads / 32 * 4;
 
-// The K and V rows of the moves, read once and written once: a warp takes four moves at
-// a time (all four rows' loads in flight before the first store).  Sources (slots >=
-// budget) and targets (slots < budget) never overlap, so the order does not matter.
 template <typename V>
 __global__ void __launch_bounds__(kEvictMoveThreads) paged_evict_move_kernel(const __grid_constant__ PagedEvictParams p,
                                                                              int units, int elems_per_unit) {
-    constexpr int M = 4;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row = blockIdx.y, b = row / p.c.kv_heads, g = row % p.c.kv_heads;
     pdl_wait();
     if (g == 0 && blockIdx.x == 0 && threadIdx.x == 0) p.lens_out[b] = min(p.lens_copy[b], p.budget);
-    const int count = p.counts[row];
-    const int32_t* mv = p.moves + static_cast<int64_t>(row) * p.max_moves * 2;
-    const int32_t* table = p.c.page_table + b * p.c.page_table_stride;
-    const int es = static_cast<int>(sizeof(V)) / elems_per_unit;
-    char* kp = static_cast<char*>(p.c.k_pages);
-    char* vp = static_cast<char*>(p.c.v_pages);
-    const int step = gridDim.x * (kEvictMoveThreads / 32) * M;
-    for (int i0 = (blockIdx.x * (kEvictMoveThreads / 32) + warp) * M; i0 < count; i0 += step) {
-        // lanes 2m and 2m + 1: target and source of move m, as offsets of their K and V rows
-        int64_t ko = 0, vo = 0;
-        bool ok = false;
-        if (lane < 2 * M && i0 + lane / 2 < count) {
-            const int slot = mv[2 * i0 + lane];
-            const int page = table[slot / p.c.page_size];
-            const int64_t in = slot % p.c.page_size;
-            ok = page >= 0 && page < p.c.num_pages;
-            if (!ok) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
-            ko = (page * p.c.k_page_stride + in * p.c.k_slot_stride + g * p.c.k_head_stride) * es;
-            vo = (page * p.c.v_page_stride + in * p.c.v_slot_stride + g * p.c.v_head_stride) * es;
-        }
-        const uint32_t good = __ballot_sync(0xffffffffu, ok);
-        for (int u0 = 0; u0 < 2 * units; u0 += 32) {
-            const int u = u0 + lane;
-            const bool isv = u >= units;
-            const int64_t e = static_cast<int64_t>(isv ? u - units : u) * elems_per_unit * es;
-            V x[M];
-            char* to[M];
-#pragma unroll
-            for (int m = 0; m < M; ++m) {
-                const int64_t kt = __shfl_sync(0xffffffffu, ko, 2 * m), kf = __shfl_sync(0xffffffffu, ko, 2 * m + 1);
-                const int64_t vt = __shfl_sync(0xffffffffu, vo, 2 * m), vf = __shfl_sync(0xffffffffu, vo, 2 * m + 1);
-                to[m] = nullptr;
-                if (u < 2 * units && ((good >> (2 * m)) & 3u) == 3u) {
-                    to[m] = (isv ? vp + vt : kp + kt) + e;
-                    x[m] = *reinterpret_cast<const V*>((isv ? vp + vf : kp + kf) + e);
-                }
-            }
-#pragma unroll
-            for (int m = 0; m < M; ++m)
-                if (to[m] != nullptr) *reinterpret_cast<V*>(to[m]) = x[m];
-        }
-    }
+    paged_move_rows<V>(p, b, g, p.moves + static_cast<int64_t>(row) * p.max_moves * 2, p.counts[row],
+                       blockIdx.x * (kEvictMoveThreads / 32) + (threadIdx.x >> 5), gridDim.x * (kEvictMoveThreads / 32),
+                       threadIdx.x & 31, units, elems_per_unit);
 }
 
 }  // namespace chronos

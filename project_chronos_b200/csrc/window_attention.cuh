@@ -87,8 +87,9 @@ __host__ __device__ constexpr int window_simt_smem(int dim) {
     return (kWsRows + 2 * kWsKeys) * (window_simt_dim(dim) + 4) * 4 + kWsRows * (kWsKeys + 4) * 4;
 }
 
-// NC: groups of 64 output columns (head_dim <= 64 * NC).
-template <typename T, int NC>
+// NC: groups of 64 output columns (head_dim <= 64 * NC); VEC: rows of 4 elements on
+// boundaries of 4.
+template <typename T, int NC, bool VEC>
 __global__ void __launch_bounds__(kWsThreads) window_simt_kernel(const __grid_constant__ WindowParams p) {
     constexpr int DP = 64 * NC, LD = DP + 4;      // row stride: float4 reads of 16 rows on different banks
     extern __shared__ __align__(16) float wsm[];
@@ -111,9 +112,12 @@ __global__ void __launch_bounds__(kWsThreads) window_simt_kernel(const __grid_co
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
 
     auto stage = [&](float* dst, const T* src, int64_t row_stride, int n) {
-        for (int i = threadIdx.x; i < kWsRows * DP; i += kWsThreads) {
-            const int r = i / DP, d = i % DP;
-            dst[r * LD + d] = r < n && d < p.dim ? to_f32<T>(src[r * row_stride + d]) : 0.0f;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < kWsRows * (DP / 4); i += kWsThreads) {
+            const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (r < n && d < p.dim) load4<T, VEC>(src + r * row_stride, d, p.dim, v);
+            *reinterpret_cast<float4*>(dst + r * LD + d) = make_float4(v[0], v[1], v[2], v[3]);
         }
     };
     stage(s_q, static_cast<const T*>(p.q) + (t.q0 + t.m0) * p.q_row + head * p.q_head, p.q_row, rows);

@@ -607,15 +607,18 @@ def _launch(fn, args, index: int) -> None:
         N.check(rc)
 
 
-def _workspace(fn, args, dev: torch.device, index: int) -> torch.Tensor:
-    """Workspace of one call from torch's allocator: a captured graph keeps its own."""
+def _workspace(fn, args, dev: torch.device, index: int) -> Optional[torch.Tensor]:
+    """Workspace of one call from torch's allocator: a captured graph keeps its own.  None
+    where the call needs none."""
     if torch.cuda.current_device() == index:
         nbytes = fn(args)
     else:
         with torch.cuda.device(index):
             nbytes = fn(args)
     if nbytes == 0:
-        N.check(N.CHRONOS_ERR_INVALID_ARG)
+        if N.load_library().chronos_moe_last_error():
+            N.check(N.CHRONOS_ERR_INVALID_ARG)
+        return None
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     args.workspace = ws.data_ptr()
     args.workspace_bytes = nbytes
