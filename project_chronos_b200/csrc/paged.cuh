@@ -226,8 +226,8 @@ __device__ __forceinline__ void mma_16816<__half>(float (&d)[4], const uint32_t 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// fp32 operands by two tf32 terms each, x = hi + lo: hi is x rounded to 11 bits, lo the
-// rest, of which the tensor core takes the first 11 bits, so hi + lo is off by 2^-21 |x|
+// fp32 operands by two tf32 terms each, x = hi + lo, both rounded to 11 bits (lo by half
+// a step before the tensor core drops the bits behind it), so hi + lo is off by 2^-23 |x|
 // at most, and hi hi + hi lo + lo hi leaves out a term below 2^-22.  What is not finite
 // has no rest.
 struct Tf32Pair {
@@ -237,7 +237,7 @@ __device__ __forceinline__ Tf32Pair tf32_split(float x) {
     Tf32Pair r;
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r.hi) : "f"(x));
     const float lo = x - __uint_as_float(r.hi);
-    r.lo = lo == lo ? __float_as_uint(lo) : 0u;
+    r.lo = lo == lo ? __float_as_uint(lo) + 0x1000u : 0u;
     return r;
 }
 __device__ __forceinline__ void mma_1688_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -248,11 +248,17 @@ __device__ __forceinline__ void mma_1688_tf32(float (&d)[4], uint32_t a0, uint32
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // d += a * (b0, b1) for a 16 x 8 piece of K or V^T and the two rows of a split operand.
+// The tensor core cuts its sums instead of rounding them: each piece is summed from
+// zero, small terms first, and added to d in fp32 (a running sum on the tensor core was
+// 2.8e-6 off where this is 4e-7).
 __device__ __forceinline__ void mma_fp32(float (&d)[4], const float (&a)[4], const Tf32Pair& b0, const Tf32Pair& b1) {
     const Tf32Pair x0 = tf32_split(a[0]), x1 = tf32_split(a[1]), x2 = tf32_split(a[2]), x3 = tf32_split(a[3]);
-    mma_1688_tf32(d, x0.hi, x1.hi, x2.hi, x3.hi, b0.hi, b1.hi);
-    mma_1688_tf32(d, x0.hi, x1.hi, x2.hi, x3.hi, b0.lo, b1.lo);
-    mma_1688_tf32(d, x0.lo, x1.lo, x2.lo, x3.lo, b0.hi, b1.hi);
+    float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    mma_1688_tf32(t, x0.hi, x1.hi, x2.hi, x3.hi, b0.lo, b1.lo);
+    mma_1688_tf32(t, x0.lo, x1.lo, x2.lo, x3.lo, b0.hi, b1.hi);
+    mma_1688_tf32(t, x0.hi, x1.hi, x2.hi, x3.hi, b0.hi, b1.hi);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] += t[i];
 }
 template <bool TRANS>
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
