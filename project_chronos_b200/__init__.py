@@ -13,6 +13,10 @@ Public API (mirrors chronos/model/moe_chronos.py of FonaTech/Project_Chronos):
   chronos/runtime/cache_manager.py and chronos/io/async_prefetcher.py);
 * ``LookaheadRouter`` (``lookahead``) — the lookahead routing predictor
   (chronos/model/lookahead_router.py) as one fused kernel;
+* ``PagedCache`` (``paged``) and ``ops.paged_append`` / ``paged_attn_decode`` /
+  ``paged_evict`` / ``window_attention`` — a paged key-value cache for rows of
+  different lengths and the attention that serves prompts and single tokens
+  from it (include/chronos_paged.h);
 * ``synthetic`` — seeded workloads of the benchmark configurations.
 
 Importing the package does not load the CUDA library; the first layer call
@@ -22,6 +26,7 @@ from .moe import ChronosMOEFeedForward, FeedForward, LazyExpertPlaceholder  # no
 from .expert_store import ExpertStore, LRUCache, ResidencySet, SlotTable, WarmTier  # noqa: F401
 from .cache_manager import CacheManager, WarmLoader  # noqa: F401
 from .lookahead import LookaheadRouter  # noqa: F401
+from .paged import PagedCache  # noqa: F401
 
 __all__ = ["ChronosMOEFeedForward", "FeedForward", "LazyExpertPlaceholder", "ExpertStore", "LRUCache",
-           "ResidencySet", "SlotTable", "WarmTier", "CacheManager", "WarmLoader", "LookaheadRouter"]
+           "ResidencySet", "SlotTable", "WarmTier", "CacheManager", "WarmLoader", "LookaheadRouter", "PagedCache"]

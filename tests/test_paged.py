@@ -133,6 +133,31 @@ def test_empty_calls_return_without_a_device(lib):
     assert lib.chronos_window_attention(ctypes.byref(w), None) == N.CHRONOS_OK
 
 
+def test_page_bookkeeping_on_the_host():
+    from project_chronos_b200 import PagedCache
+    c = PagedCache(2, 5, 1, 8, 4, "cpu", torch.float32, page_size=4)
+    c.reserve(0, 9)
+    c.reserve(1, 1)
+    assert c.page_table.tolist() == [[0, 1, 2, -1], [3, -1, -1, -1]] and c.free_pages() == 1
+    c.reserve(0, 12)                                     # covered already
+    with pytest.raises(RuntimeError, match="at most 4"):
+        c.reserve(0, 17)
+    with pytest.raises(RuntimeError, match="out of pages"):
+        c.reserve(1, 12)
+    assert c.page_table.tolist()[1] == [3, -1, -1, -1] and c.free_pages() == 1   # nothing half done
+    c.trim(0, 5)
+    assert c.page_table.tolist()[0] == [0, 1, -1, -1] and c.free_pages() == 2
+    c.reserve(1, 12)
+    assert sorted(c.page_table[1, :3].tolist()) == [2, 3, 4]
+    c.lens[1] = 12
+    c.release(1)
+    assert c.page_table.tolist()[1] == [-1] * 4 and c.free_pages() == 3 and c.lens.tolist() == [0, 0]
+    with pytest.raises(RuntimeError, match="track_weights"):
+        c.evict(3)
+    with pytest.raises(ValueError):
+        PagedCache(0, 5, 1, 8, 4, "cpu")
+
+
 # ---------------------------------------------------------------------------------------
 # definitions in 64 bits
 # ---------------------------------------------------------------------------------------
@@ -802,3 +827,171 @@ def test_a_serving_run(dt):
                     book[i][x] = [book[i][x][j] for j in plans[i][x] if j >= 0]
                     assert [y[3] for y in book[i][x]] == pos[i, x, : len(book[i][x])].tolist()
     ops.check_status(kp.device)
+
+
+@gpu
+def test_paged_cache_rows_come_and_go():
+    """The cache object: a row ends, its pages serve another one; a row without pages is
+    refused on the device; a captured step replays while the rows grow."""
+    from project_chronos_b200 import PagedCache, ops
+    from project_chronos_b200 import _native as N
+    h, g, d, dt = 8, 2, 64, BF
+    gen = _gen(5)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device="cuda").to(dt)  # noqa: E731
+    c = PagedCache(2, 12, g, d, 8, "cuda", dt, page_size=16, track_weights=True)
+    book = [[], []]
+
+    def step(one):
+        k, v, q = rnd(2, g, d), rnd(2, g, d), rnd(2, h, d)
+        c.append(k, v)
+        out = one(q)
+        for b in range(2):
+            book[b].append((k[b], v[b]))
+            ks, vs = (torch.stack([r[i] for r in book[b]]) for i in (0, 1))
+            ref, _, _, a, f = _attend(q[b], ks, vs, d ** -0.5, _visible(len(ks), 0, 0, "cuda"))
+            _check_out(out[b], ref, a, f, len(ks), dt)
+
+    for b, n in enumerate((40, 7)):
+        c.reserve(b, n + 40)
+    k, v = rnd(47, g, d), rnd(47, g, d)
+    c.append(k, v, torch.tensor([0, 40, 47], dtype=torch.int32, device="cuda"))
+    book[0] = [(k[i], v[i]) for i in range(40)]
+    book[1] = [(k[i], v[i]) for i in range(40, 47)]
+    step(c.attend)
+    static_q, static_out = rnd(2, h, d), torch.empty(2, h, d, dtype=dt, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.attend(static_q, out=static_out)
+
+    def replay(q):
+        static_q.copy_(q)
+        graph.replay()
+        return static_out
+
+    for _ in range(20):
+        step(replay)
+    # row 0 ends; its pages go to row 1, which goes on, and a new row 0 starts
+    c.release(0)
+    book[0] = []
+    c.reserve(1, 100)
+    c.reserve(0, 60)
+    for _ in range(25):
+        step(replay)
+    ops.check_status(c.lens.device)
+    assert c.positions[0, 0, :25].tolist() == list(range(25))
+    c.release(0)
+    with pytest.raises(RuntimeError, match="at most 8"):
+        c.reserve(1, 128 * 2)
+    c.append(rnd(2, g, d), rnd(2, g, d))                 # row 0 has no pages
+    with pytest.raises(N.ChronosMoeError, match="INVALID_ARG"):
+        ops.check_status(c.lens.device)
+
+
+# ---------------------------------------------------------------------------------------
+# many rows, other strides, captured evictions
+# ---------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dt, d", [(BF, 128), (BF, 64), (FP, 128), (HF, 256)])
+@pytest.mark.parametrize("b, most", [(400, 60), (400, 200), (150, 500), (70, 1500)])
+def test_decode_of_many_rows(dt, d, b, most):
+    """Around the choice between clusters and the work list: more rows than blocks, rows of
+    one to many blocks, none at all."""
+    from project_chronos_b200 import ops
+    gen = torch.Generator().manual_seed(b + most)
+    lens = torch.randint(0, most + 1, (b,), generator=gen).tolist()
+    lens[:3] = [0, most, 1]
+    h, g = 6, 2
+    kp, vp, table, ln, rows = _make_cache(lens, g, d, 16, dt, seed=d)
+    q = (2 * torch.randn(b, h, d, generator=_gen(1), device="cuda")).to(dt)
+    lse = torch.empty(b, h, device="cuda")
+    out = ops.paged_attn_decode(q, kp, vp, table, ln, scale=0.11, lse=lse)
+    for i in list(range(0, b, 17)) + [1, 2, b - 1]:
+        k, v = rows[i]
+        ref, rl, _, a, f = _attend(q[i], k, v, 0.11, _visible(lens[i], 0, 0, "cuda"))
+        _check_out(out[i], ref, a, f, lens[i], dt)
+        _check_lse(lse[i], rl, f)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_many_short_sequences(dt):
+    from project_chronos_b200 import ops
+    b, h, g, d, size = 1100, 4, 2, 64, 16
+    gen = torch.Generator().manual_seed(3)
+    new = torch.randint(0, 9, (b,), generator=gen).tolist()
+    t = sum(new)
+    cu = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+    q = torch.randn(t, h, d, generator=_gen(1), device="cuda").to(dt)
+    k, v = (torch.randn(t, g, d, generator=_gen(2 + i), device="cuda").to(dt) for i in range(2))
+    out = ops.window_attention(q, k, v, cu, window=3, sinks=1)
+    kp, vp = (torch.zeros(b, size, g, d, dtype=dt, device="cuda") for _ in range(2))
+    table = torch.randperm(b, generator=_gen(9), device="cuda").to(torch.int32).view(b, 1)
+    ops.paged_append(k, v, kp, vp, table, torch.zeros(b, dtype=torch.int32, device="cuda"), cu_seqlens=cu)
+    last = torch.tensor([max(0, int(cu[i + 1]) - 1) for i in range(b)], device="cuda")
+    one = ops.paged_attn_decode(q[last].contiguous(), kp, vp, table, cu.diff().contiguous(), window=3, sinks=1)
+    ops.check_status(q.device)
+    for i in range(0, b, 29):
+        n, c0 = new[i], int(cu[i])
+        _check_prompt(out, None, q, k, v, n, n, c0, c0, 3, 1, dt)
+        if n:
+            assert torch.equal(kp[int(table[i, 0]), :n], k[c0: c0 + n])
+            ref, _, _, a, f = _attend(q[c0 + n - 1], k[c0: c0 + n], v[c0: c0 + n], d ** -0.5, _visible(n, 3, 1, "cuda"))
+            _check_out(one[i], ref, a, f, n, dt)
+        else:
+            assert bool((one[i] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("layout", ["fused", "heads first", "odd strides"])
+def test_prompt_attention_takes_strides(dt, layout):
+    from project_chronos_b200 import ops
+    n, h, g, d = 300, 6, 2, 64
+    x = torch.randn(n, h + 2 * g, d, generator=_gen(4), device="cuda").to(dt)
+    if layout == "heads first":
+        x = x.transpose(0, 1).contiguous().transpose(0, 1)
+    elif layout == "odd strides":
+        x = torch.cat([x, x[..., :1]], dim=-1)[..., :d]
+    q, k, v = x[:, :h], x[:, h: h + g], x[:, h + g:]
+    wide = torch.full((n, h + 1, d + (1 if layout == "odd strides" else 8)), 3.0, dtype=dt, device="cuda")
+    cu = torch.tensor([0, 100, n], dtype=torch.int32, device="cuda")
+    ops.window_attention(q, k, v, cu, out=wide[:, :h, :d], window=90, sinks=2)
+    for c0, m in ((0, 100), (100, 200)):
+        _check_prompt(wide[:, :h, :d], None, q, k, v, m, m, c0, c0, 90, 2, dt, _some_rows(m))
+    assert bool((wide[:, h:] == 3.0).all()) and bool((wide[..., d:] == 3.0).all())
+
+
+@gpu
+@pytest.mark.parametrize("n, budget", [(900, 820), (900, 300)])
+def test_captured_evictions(n, budget):
+    """One kernel (few slots) and two, replayed on new contents; a row shorter than the budget."""
+    from project_chronos_b200 import ops
+    g, d, size = 2, 32, 16
+    kp, vp, table, ln, _ = _make_cache([n, 20], g, d, size, BF, seed=1, width=-(-n // size), bad=0.0)
+    cap = table.shape[1] * size
+    w = torch.zeros(2, g, cap, device="cuda")
+    pos = torch.arange(cap, dtype=torch.int32, device="cuda").expand(2, g, cap).contiguous()
+    wo, po = torch.zeros_like(w), torch.zeros_like(pos)
+    call = lambda: ops.paged_evict(kp, vp, table, ln, ln, w, pos, budget, sinks=2, recent=9, weights_out=wo, positions_out=po)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        r = call()
+    for seed in range(3):
+        kp.copy_(torch.randn(kp.shape, generator=_gen(seed), device="cuda"))
+        vp.copy_(torch.randn(vp.shape, generator=_gen(seed + 9), device="cuda"))
+        w.copy_(torch.rand(w.shape, generator=_gen(seed + 20), device="cuda"))
+        k0, v0 = kp.clone(), vp.clone()
+        graph.replay()
+        assert r["lens"].tolist() == [budget, 20]
+        t = table[0].long()
+        for j in range(g):
+            src = _evict_plan(w[0, j].tolist(), pos[0, j].tolist(), n, n, budget, 2, 9)
+            assert r["src"][0, j].tolist() == src
+            s, to = torch.tensor(src, device="cuda"), torch.arange(budget, device="cuda")
+            assert torch.equal(kp[t[to // size], to % size, j], k0[t[s // size], s % size, j])
+            assert torch.equal(vp[t[to // size], to % size, j], v0[t[s // size], s % size, j])
+        assert torch.equal(kp[table[1].long()], k0[table[1].long()])
