@@ -31,7 +31,7 @@ struct WindowParams {
 // The row tile a block works on: `rows` queries of sequence b from its query m0 on.
 struct WindowTile {
     int b, m0;
-    int64_t q0, k0;     // first rows of the sequence in q and k
+    int q0, k0;         // first rows of the sequence in q and k
     int lq, lk;
 };
 
@@ -61,7 +61,8 @@ __device__ __forceinline__ bool window_tile(const WindowParams& p, int64_t x, in
             t.k0 = p.cu_k[t.b];
             t.lq = p.cu_q[t.b + 1] - p.cu_q[t.b];
             t.lk = p.cu_k[t.b + 1] - p.cu_k[t.b];
-            if (t.q0 < 0 || t.q0 + t.lq > p.num_q || t.k0 < 0 || t.lk < 0 || t.k0 + t.lk > p.num_k) {
+            if (t.q0 < 0 || static_cast<int64_t>(t.q0) + t.lq > p.num_q || t.k0 < 0 || t.lk < 0 ||
+                static_cast<int64_t>(t.k0) + t.lk > p.num_k) {
                 if (lane == 0) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
                 return false;
             }
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(kWsThreads) window_simt_kernel(const __grid_co
             *reinterpret_cast<float4*>(dst + r * LD + d) = make_float4(v[0], v[1], v[2], v[3]);
         }
     };
-    stage(s_q, static_cast<const T*>(p.q) + (t.q0 + t.m0) * p.q_row + head * p.q_head, p.q_row, rows);
+    stage(s_q, static_cast<const T*>(p.q) + static_cast<int64_t>(t.q0 + t.m0) * p.q_row + head * p.q_head, p.q_row, rows);
     float m[4], l[4], o[4][NC * 4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -133,8 +134,8 @@ __global__ void __launch_bounds__(kWsThreads) window_simt_kernel(const __grid_co
         const int j0 = it < ns ? it * kWsKeys : w0 + (it - ns) * kWsKeys;
         const int n = min(kWsKeys, t.lk - j0);
         __syncthreads();
-        stage(s_k, static_cast<const T*>(p.k) + (t.k0 + j0) * p.k_row + g * p.k_head, p.k_row, n);
-        stage(s_v, static_cast<const T*>(p.v) + (t.k0 + j0) * p.v_row + g * p.v_head, p.v_row, n);
+        stage(s_k, static_cast<const T*>(p.k) + static_cast<int64_t>(t.k0 + j0) * p.k_row + g * p.k_head, p.k_row, n);
+        stage(s_v, static_cast<const T*>(p.v) + static_cast<int64_t>(t.k0 + j0) * p.v_row + g * p.v_head, p.v_row, n);
         __syncthreads();
         float s[4][4];
 #pragma unroll
@@ -236,14 +237,14 @@ __global__ void __launch_bounds__(kWsThreads) window_simt_kernel(const __grid_co
         const int row = ty * 4 + r;
         if (row >= rows) continue;
         const float inv = l[r] > 0.0f ? 1.0f / l[r] : l[r];   // 0 for a row that saw nothing; NaN stays
-        T* out = static_cast<T*>(p.out) + (t.q0 + t.m0 + row) * p.o_row + head * p.o_head;
+        T* out = static_cast<T*>(p.out) + static_cast<int64_t>(t.q0 + t.m0 + row) * p.o_row + head * p.o_head;
 #pragma unroll
         for (int c = 0; c < NC * 4; ++c) {
             const int d = (c >> 2) * 64 + tx * 4 + (c & 3);
             if (d < p.dim) out[d] = from_f32<T>(o[r][c] * inv);
         }
         if (tx == 0 && p.lse != nullptr)
-            p.lse[(t.q0 + t.m0 + row) * p.heads + head] = l[r] != 0.0f ? (m[r] + log2f(l[r])) * kLn2 : -INFINITY;
+            p.lse[static_cast<int64_t>(t.q0 + t.m0 + row) * p.heads + head] = l[r] != 0.0f ? (m[r] + log2f(l[r])) * kLn2 : -INFINITY;
     }
 }
 
@@ -282,7 +283,7 @@ struct WindowTc {
     static constexpr int kHalves = DP / 64;
     static constexpr int kTileBytes = 128 * DP * 2;         // 128 rows of K, V or Q
     static constexpr int kStages = DP == 64 ? 3 : 2;        // of K and of V
-    static constexpr int kBarriers = 1 + 5 * kStages + 2 + 4 + 2 + 1;
+    static constexpr int kBarriers = 2 + 5 * kStages + 2 + 4 + 2 + 1;
     static constexpr int kSmem = 1024 + (2 + 2 * kStages) * kTileBytes + 8 * kBarriers + 32;
     static constexpr int kSCol = 0, kOCol = 256;            // S of tile w at 128 w, O at 256 + DP w
 };
@@ -402,9 +403,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 template <typename T>
 __device__ __noinline__ void window_row_exact(const WindowParams& p, const WindowTile& t, int token, int head, int lane) {
     const int tr = t.lk - t.lq + token;
-    const T* q = static_cast<const T*>(p.q) + (t.q0 + token) * p.q_row + head * p.q_head;
-    const T* k = static_cast<const T*>(p.k) + t.k0 * p.k_row + (head / p.rep) * p.k_head;
-    const T* v = static_cast<const T*>(p.v) + t.k0 * p.v_row + (head / p.rep) * p.v_head;
+    const T* q = static_cast<const T*>(p.q) + static_cast<int64_t>(t.q0 + token) * p.q_row + head * p.q_head;
+    const T* k = static_cast<const T*>(p.k) + static_cast<int64_t>(t.k0) * p.k_row + (head / p.rep) * p.k_head;
+    const T* v = static_cast<const T*>(p.v) + static_cast<int64_t>(t.k0) * p.v_row + (head / p.rep) * p.v_head;
     float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const int lo = p.window > 0 ? max(0, tr - p.window + 1) : 0;
     const int first = min(p.sinks, lo);
@@ -424,12 +425,12 @@ __device__ __noinline__ void window_row_exact(const WindowParams& p, const Windo
         }
     }
     const float inv = l > 0.0f ? 1.0f / l : l;
-    T* out = static_cast<T*>(p.out) + (t.q0 + token) * p.o_row + head * p.o_head;
+    T* out = static_cast<T*>(p.out) + static_cast<int64_t>(t.q0 + token) * p.o_row + head * p.o_head;
 #pragma unroll
     for (int a = 0; a < 4; ++a)
         if (lane + 32 * a < p.dim) out[lane + 32 * a] = from_f32<T>(o[a] * inv);
     if (lane == 0 && p.lse != nullptr)
-        p.lse[(t.q0 + token) * p.heads + head] = l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        p.lse[static_cast<int64_t>(t.q0 + token) * p.heads + head] = l != 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
 }
 
 template <typename T>
@@ -453,6 +454,11 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
     constexpr int NS = C::kStages;
     extern __shared__ uint8_t dyn[];
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    if (warp == 8 && lane == 0) {
+        prefetch_tmap(&tm_q);
+        prefetch_tmap(&tm_k);
+        prefetch_tmap(&tm_v);
+    }
     const int hg = blockIdx.x % groups;
     const int tokens = 256 >> rp_log2;            // tokens of the block
     WindowTile t;
@@ -472,7 +478,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
     uint8_t* s_v = s_k + NS * C::kTileBytes;
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + NS * C::kTileBytes);
     uint64_t* q_full = bars;
-    uint64_t* k_full = q_full + 1;
+    uint64_t* k_full = q_full + 2;                // q_full [2]: by tile
     uint64_t* k_empty = k_full + NS;
     uint64_t* v_full = k_empty + NS;
     uint64_t* v_ok = v_full + NS;
@@ -486,6 +492,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
     volatile int* not_finite = abort_flag + 1;
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
+        mbar_init(q_full + 1, 1);
         for (int i = 0; i < NS; ++i) {
             mbar_init(k_full + i, 1);
             mbar_init(k_empty + i, 1);
@@ -523,25 +530,29 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
     };
 
     if (warp >= 8) {
-        // the block launched with 384 * 168 registers: 256 * 216 + 128 * 72
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        // the block launched with 384 * 168 registers: 256 * 200 + 128 * 104 (the issuing warp
+        // spills with fewer: 72 cost 2 %, 56 cost 7 %)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         if (warp == 8 && lane == 0 && nt > 0) {
             // ------------------------------ loads ------------------------------
             const int g = groups == p.kv_heads ? hg : hg / p.rep;
-            mbar_arrive_expect_tx(q_full, 2 * C::kTileBytes);
-            for (int w = 0; w < 2; ++w)
+            auto load_q = [&](int w) {
+                mbar_arrive_expect_tx(q_full + w, C::kTileBytes);
                 for (int h = 0; h < C::kHalves; ++h)
-                    tma_load_4d(s_q + w * C::kTileBytes + h * 16384, &tm_q, q_full, h * 64, 0, hg,
-                                static_cast<int>(t.q0 + t.m0 + w * (128 >> rp_log2)));
+                    tma_load_4d(s_q + w * C::kTileBytes + h * 16384, &tm_q, q_full + w, h * 64, 0, hg,
+                                t.q0 + t.m0 + w * (128 >> rp_log2));
+            };
+            load_q(0);
             int i = 0;
             for (; i < nt; ++i) {
                 const int st = i % NS;
                 const uint32_t ph = (i / NS) & 1;
-                const int row = static_cast<int>(t.k0 + tile_base(i));
+                const int row = t.k0 + tile_base(i);
                 if (!wait(k_empty + st, ph ^ 1u)) break;
                 mbar_arrive_expect_tx(k_full + st, C::kTileBytes);
                 for (int h = 0; h < C::kHalves; ++h)
                     tma_load_3d(s_k + st * C::kTileBytes + h * 16384, &tm_k, k_full + st, h * 64, g, row);
+                if (i == 0) load_q(1);
                 if (!wait(v_empty + st, ph ^ 1u)) {
                     ++i;   // this tile's K copy is in flight (its V barrier is not waited for below)
                     break;
@@ -554,6 +565,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
                 // the copies in flight land before the block's shared memory is given up
                 volatile int go = 0;
                 mbar_wait_bounded(q_full, 0, kWtLimitNs, &go);
+                mbar_wait_bounded(q_full + 1, 0, kWtLimitNs, &go);
                 for (int j = max(0, i - NS); j < i; ++j) {
                     mbar_wait_bounded(k_full + j % NS, (j / NS) & 1, kWtLimitNs, &go);
                     mbar_wait_bounded(v_full + j % NS, (j / NS) & 1, kWtLimitNs, &go);
@@ -598,8 +610,9 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
                 return ok;
             };
             bool ok = until(q_full, 0) && until(k_full, 0);
+            if (ok) qk(0, 0);
+            ok = ok && until(q_full + 1, 0);
             if (ok) {
-                qk(0, 0);
                 qk(1, 0);
                 if (leader) umma_commit(k_empty);
             }
@@ -673,7 +686,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
             asm volatile("bar.arrive 2, 320;" ::: "memory");
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         // ------------------------------ softmax and output ------------------------------
         const int w = warp >> 2;
         const int r = (warp & 3) * 32 + lane;
