@@ -42,6 +42,9 @@ int check_cache_pointers(const ChronosPagedCache& c, const char* what) {
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: lens, page_table, k_pages and v_pages are required", what);
     return CHRONOS_OK;
 }
+// A window (or number of first tokens) as the kernels take it: rows have at most 2^30
+// keys, so a longer one hides nothing, and positions minus it stay within 32 bits.
+int cut_window(int window) { return std::min(window, 1 << 30); }
 // Slots a sequence can have: what its table (and the per-slot arrays, when there are any) hold.
 int slot_limit(const ChronosPagedCache& c, int64_t slot_cap, bool has_cap) {
     int64_t n = static_cast<int64_t>(c.table_width) * c.page_size;
@@ -373,8 +376,8 @@ extern "C" int chronos_paged_decode(const ChronosPagedDecodeArgs* a, void* strea
     p.rep = a->heads / a->cache.kv_heads;
     p.rows = d.rows;
     p.parts = d.parts;
-    p.window = a->window;
-    p.sinks = a->window > 0 ? a->sinks : 0;
+    p.window = cut_window(a->window);
+    p.sinks = a->window > 0 ? cut_window(a->sinks) : 0;
     p.max_slots = limit;
     p.page_shift = -1;
     if ((a->cache.page_size & (a->cache.page_size - 1)) == 0)
@@ -558,8 +561,8 @@ extern "C" int chronos_window_attention(const ChronosWindowAttnArgs* a, void* st
     p.kv_heads = a->kv_heads;
     p.rep = a->heads / a->kv_heads;
     p.dim = a->head_dim;
-    p.window = a->window;
-    p.sinks = a->window > 0 ? a->sinks : 0;
+    p.window = cut_window(a->window);
+    p.sinks = a->window > 0 ? cut_window(a->sinks) : 0;
     p.sl2 = static_cast<float>(static_cast<double>(a->scale) * 1.4426950408889634);
     p.num_q = a->num_q;
     p.num_k = a->num_k;

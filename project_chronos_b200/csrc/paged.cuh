@@ -229,15 +229,27 @@ __device__ __forceinline__ void mma_16816<__half>(float (&d)[4], const uint32_t 
 // fp32 operands by two tf32 terms each, x = hi + lo, both rounded to 11 bits (lo by half
 // a step before the tensor core drops the bits behind it), so hi + lo is off by 2^-23 |x|
 // at most, and hi hi + hi lo + lo hi leaves out a term below 2^-22.  What is not finite
-// has no rest.
+// has no rest and stays out of the small terms (infinity times a rest of zero).
 struct Tf32Pair {
     uint32_t hi, lo;
+};
+struct Tf32Value : Tf32Pair {
+    uint32_t cross;   // hi in the small terms
 };
 __device__ __forceinline__ Tf32Pair tf32_split(float x) {
     Tf32Pair r;
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r.hi) : "f"(x));
     const float lo = x - __uint_as_float(r.hi);
     r.lo = lo == lo ? __float_as_uint(lo) + 0x1000u : 0u;
+    return r;
+}
+__device__ __forceinline__ Tf32Value tf32_value(float x) {
+    Tf32Value r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r.hi) : "f"(x));
+    const float lo = x - __uint_as_float(r.hi);
+    const bool finite = lo == lo;
+    r.lo = finite ? __float_as_uint(lo) + 0x1000u : 0u;
+    r.cross = finite ? r.hi : 0u;
     return r;
 }
 __device__ __forceinline__ void mma_1688_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -252,9 +264,9 @@ __device__ __forceinline__ void mma_1688_tf32(float (&d)[4], uint32_t a0, uint32
 // zero, small terms first, and added to d in fp32 (a running sum on the tensor core was
 // 2.8e-6 off where this is 4e-7).
 __device__ __forceinline__ void mma_fp32(float (&d)[4], const float (&a)[4], const Tf32Pair& b0, const Tf32Pair& b1) {
-    const Tf32Pair x0 = tf32_split(a[0]), x1 = tf32_split(a[1]), x2 = tf32_split(a[2]), x3 = tf32_split(a[3]);
+    const Tf32Value x0 = tf32_value(a[0]), x1 = tf32_value(a[1]), x2 = tf32_value(a[2]), x3 = tf32_value(a[3]);
     float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    mma_1688_tf32(t, x0.hi, x1.hi, x2.hi, x3.hi, b0.lo, b1.lo);
+    mma_1688_tf32(t, x0.cross, x1.cross, x2.cross, x3.cross, b0.lo, b1.lo);
     mma_1688_tf32(t, x0.lo, x1.lo, x2.lo, x3.lo, b0.hi, b1.hi);
     mma_1688_tf32(t, x0.hi, x1.hi, x2.hi, x3.hi, b0.hi, b1.hi);
 #pragma unroll

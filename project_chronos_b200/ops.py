@@ -565,6 +565,13 @@ def _written_once(name: str, shape, strides) -> None:
                 raise ValueError(f"{name} is written: it must not be expanded")
 
 
+def _int32(**values: int) -> None:
+    """Refuse what the argument structs' 32-bit fields would cut."""
+    for name, v in values.items():
+        if not -0x80000000 <= v <= 0x7FFFFFFF:
+            raise ValueError(f"{name} {v} does not fit 32 bits")
+
+
 def _no_cpu(t: torch.Tensor) -> None:
     raise RuntimeError(f"chronos paged kernels need CUDA tensors (no CPU path exists); got a tensor on {t.device}")
 
@@ -699,6 +706,8 @@ def paged_attn_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
         wo = wp if weights_out is None else _dense("weights_out", weights_out, slots, torch.float32, index, dev)
     elif weights_out is not None:
         raise ValueError("weights_out needs weights")
+    if (window | sinks) >> 31:
+        _int32(window=window, sinks=sinks)
     args = N.ChronosPagedDecodeArgs(
         cache, h, window, sinks, d ** -0.5 if scale is None else scale, q.data_ptr(), qs[0], qs[1], out.data_ptr(),
         os[0], os[1], None if lse is None else _dense("lse", lse, (b, h), torch.float32, index, dev), wp, wo, cap, None, 0,
@@ -744,6 +753,8 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.
         lens_out = torch.empty(b, dtype=torch.int32, device=dev)
     if budget < 1:
         raise ValueError(f"budget {budget} must be at least 1")
+    if (budget | sinks | recent) >> 31:
+        _int32(budget=budget, sinks=sinks, recent=recent)
     src = torch.empty((b, g, budget), dtype=torch.int32, device=dev)
     args = N.ChronosPagedEvictArgs(
         cache, budget, sinks, recent, 0, _dense("seen", seen, (b,), torch.int32, index, dev), wp, pp, wo, po, cap,
@@ -797,6 +808,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     else:
         os = _rows("out", out, shape, dt, index, dev, grad)
         _written_once("out", shape, os)
+    if (window | sinks) >> 31:
+        _int32(window=window, sinks=sinks)
     args = N.ChronosWindowAttnArgs(
         n - 1, h, g, d, code, window, sinks, d ** -0.5 if scale is None else scale, tq, tk, q.data_ptr(), k.data_ptr(),
         v.data_ptr(), out.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], cq, ck,

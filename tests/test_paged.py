@@ -10,6 +10,9 @@ u = finfo(type).eps / 2 and A = sum_j p_j |v_j|:
   rounding), so it is off by at most D 2^-23 S, S = max_j scale sum_d |q_d k_jd|; the
   exponential adds 2^-21 of its value; a weight p_j is thus off by
   f = D 2^-23 S + n 2^-24 + 2^-20 of itself (n: terms of its normalising sum);
+* fp32 layers of the tensor-core path split every operand into two tf32 terms: a product is
+  off by 2^-21 of its magnitude, which D 2^-23 S (D >= 8 here) and the 2^-20 of f cover
+  beside their fewer additions;
 * 16-bit layers round the weights to the layer type before the second product (u A) and
   the result once (u |out|); the second product adds n 2^-23 A.
   So |error| <= u (A + |out|) + (f + n 2^-23) A, without the first u A for fp32;
@@ -995,3 +998,85 @@ def test_captured_evictions(n, budget):
             assert torch.equal(kp[t[to // size], to % size, j], k0[t[s // size], s % size, j])
             assert torch.equal(vp[t[to // size], to % size, j], v0[t[s // size], s % size, j])
         assert torch.equal(kp[table[1].long()], k0[table[1].long()])
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_the_longest_windows(dt):
+    """A window of 2^31 - 1 hides nothing, whatever the position; more is refused."""
+    from project_chronos_b200 import ops
+    big = 2 ** 31 - 1
+    h, g, d = 4, 2, 64
+    gen = _gen(1)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device="cuda").to(dt)  # noqa: E731
+    q, k, v = rnd(370, h, d), rnd(270, g, d), rnd(270, g, d)   # the first 100 rows see nothing
+    cq, ck = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 300, 370], [0, 200, 270]))
+    for window, sinks in ((big, 0), (big, big), (3, big)):
+        out = ops.window_attention(q, k, v, cq, cu_seqlens_k=ck, window=window, sinks=sinks)
+        _check_prompt(out, None, q, k, v, 300, 200, 0, 0, 0, 0, dt, [0, 99, 100, 101, 299])
+        _check_prompt(out, None, q, k, v, 70, 70, 300, 200, 0, 0, dt, [0, 69])
+    kp, vp, table, ln, rows = _make_cache([90, 1], g, d, 16, dt, seed=3)
+    q1 = rnd(2, h, d)
+    for window, sinks in ((big, 0), (big, big), (3, big)):
+        out = ops.paged_attn_decode(q1, kp, vp, table, ln, window=window, sinks=sinks)
+        for b, (kk, vv) in enumerate(rows):
+            ref, _, _, a, f = _attend(q1[b], kk, vv, d ** -0.5, _visible(len(kk), 0, 0, "cuda"))
+            _check_out(out[b], ref, a, f, len(kk), dt)
+    for bad in (dict(window=2 ** 31), dict(window=2 ** 32 + 3), dict(sinks=2 ** 40), dict(window=-2 ** 31 - 1)):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.paged_attn_decode(q1, kp, vp, table, ln, **bad)
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.window_attention(q, k, v, cq, cu_seqlens_k=ck, **bad)
+    with pytest.raises(RuntimeError, match="negative"):
+        ops.paged_attn_decode(q1, kp, vp, table, ln, window=-5)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("d", [64, 36])
+def test_decode_passes_on_what_is_not_finite(dt, d):
+    """A visible NaN or infinity reaches the heads (columns) that read it, a hidden one none."""
+    from project_chronos_b200 import ops
+    h, g = 4, 2
+    kp, vp, table, ln, rows = _make_cache([200, 200, 200], g, d, 16, dt, seed=3)
+    q = torch.randn(3, h, d, generator=_gen(1), device="cuda").to(dt)
+    at = lambda b, s: (int(table[b, s // 16]), s % 16)  # noqa: E731
+    kp[at(0, 77)][0, 3] = math.nan
+    vp[at(1, 77)][1, 5] = math.inf
+    vp[at(2, 10)][:, :] = math.nan                    # hidden by the window
+    kp[at(2, 11)][:, :] = math.inf
+    out = ops.paged_attn_decode(q, kp, vp, table, ln, window=150, sinks=4)
+    assert bool(torch.isnan(out[0, :2]).all()) and bool(torch.isfinite(out[0, 2:]).all())
+    assert bool((out[1, 2:, 5] == math.inf).all())
+    assert bool(torch.isfinite(out[1, :2]).all()) and bool(torch.isfinite(out[1, 2:, :5]).all())
+    k, v = rows[2]
+    ref, _, _, a, f = _attend(q[2], k, v, d ** -0.5, _visible(200, 150, 4, "cuda"))
+    _check_out(out[2], ref, a, f, 200, dt)
+
+
+@gpu
+def test_empty_calls_on_the_device():
+    from project_chronos_b200 import ops
+    z = dict(dtype=BF, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    kp = torch.zeros(3, 16, 2, 64, **z)
+    none = ops.paged_attn_decode(torch.zeros(0, 4, 64, **z), kp, kp, torch.zeros(0, 2, **i32), torch.zeros(0, **i32))
+    assert none.shape == (0, 4, 64)
+    # no pages at all: every row is empty
+    no = torch.zeros(0, 16, 2, 64, **z)
+    out = ops.paged_attn_decode(torch.ones(2, 4, 64, **z), no, no, torch.zeros(2, 0, **i32), torch.zeros(2, **i32))
+    assert bool((out == 0).all())
+    assert ops.window_attention(torch.zeros(0, 4, 64, **z), torch.zeros(5, 2, 64, **z), torch.zeros(5, 2, 64, **z),
+                                torch.zeros(2, **i32), cu_seqlens_k=torch.zeros(2, **i32)).shape == (0, 4, 64)
+    # queries without keys see nothing
+    lse = torch.zeros(3, 4, device="cuda")
+    out = ops.window_attention(torch.ones(3, 4, 64, **z), torch.zeros(0, 2, 64, **z), torch.zeros(0, 2, 64, **z),
+                               torch.tensor([0, 3], **i32), cu_seqlens_k=torch.zeros(2, **i32), lse=lse)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    ops.paged_append(torch.zeros(0, 2, 64, **z), torch.zeros(0, 2, 64, **z), kp, kp.clone(), torch.zeros(1, 1, **i32),
+                     torch.zeros(1, **i32), cu_seqlens=torch.zeros(2, **i32))
+    w = torch.zeros(1, 2, 16, device="cuda")
+    r = ops.paged_evict(kp, kp.clone(), torch.zeros(1, 1, **i32), torch.zeros(1, **i32), torch.zeros(1, **i32), w,
+                        torch.zeros(1, 2, 16, **i32), 40)
+    assert r["lens"].tolist() == [0] and bool((r["src"] == -1).all())
+    ops.check_status(kp.device)
