@@ -226,8 +226,8 @@ __device__ __forceinline__ void mma_16816<__half>(float (&d)[4], const uint32_t 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// fp32 operands by two tf32 terms each, x = hi + lo, both rounded to 11 bits (lo by half
-// a step before the tensor core drops the bits behind it), so hi + lo is off by 2^-23 |x|
+// fp32 operands by two tf32 terms each, x = hi + lo: hi is x rounded to 11 bits, lo the
+// rest, of which the tensor core takes the first 11 bits, so hi + lo is off by 2^-21 |x|
 // at most, and hi hi + hi lo + lo hi leaves out a term below 2^-22.  What is not finite
 // has no rest and stays out of the small terms (infinity times a rest of zero).
 struct Tf32Pair {
@@ -240,7 +240,7 @@ __device__ __forceinline__ Tf32Pair tf32_split(float x) {
     Tf32Pair r;
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r.hi) : "f"(x));
     const float lo = x - __uint_as_float(r.hi);
-    r.lo = lo == lo ? __float_as_uint(lo) + 0x1000u : 0u;
+    r.lo = lo == lo ? __float_as_uint(lo) : 0u;
     return r;
 }
 __device__ __forceinline__ Tf32Value tf32_value(float x) {
@@ -248,7 +248,7 @@ __device__ __forceinline__ Tf32Value tf32_value(float x) {
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r.hi) : "f"(x));
     const float lo = x - __uint_as_float(r.hi);
     const bool finite = lo == lo;
-    r.lo = finite ? __float_as_uint(lo) + 0x1000u : 0u;
+    r.lo = finite ? __float_as_uint(lo) : 0u;
     r.cross = finite ? r.hi : 0u;
     return r;
 }
