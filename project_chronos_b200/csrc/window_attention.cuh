@@ -7,6 +7,8 @@
 // sum: out = sum 2^(x_j - m) v_j / sum 2^(x_j - m), x_j = scale log2(e) q.k_j.
 #pragma once
 
+#include <cooperative_groups.h>
+
 #include "chronos_paged.h"
 #include "common.cuh"
 #include "paged.cuh"
@@ -280,6 +282,10 @@ __global__ void __launch_bounds__(kWsThreads) window_simt_kernel(const __grid_co
 // cycles, then both products 1400 (1040 by themselves), and two such chains per SM
 // overlap to 3500 cycles per 128 keys where either unit alone needs 2050.
 //
+// Few row tiles and many keys (SPLIT): a thread-block cluster shares a row tile, block r
+// of it the r-th part of the key tiles; every block leaves its rows' (m, l, O) in its
+// shared memory and joins its share of the rows through distributed shared memory.
+//
 // O is rescaled only when a row's maximum grew by more than 2^8 in weight: until
 // then weights are taken against the older maximum, at most 256 times too large,
 // which the fp32 sums and both 16-bit formats hold without loss.
@@ -295,6 +301,8 @@ struct WindowTc {
     static constexpr int kStages = DP == 64 ? 3 : 2;        // of K and of V
     static constexpr int kBarriers = 2 + 5 * kStages + 2 + 4 + 2 + 1;
     static constexpr int kSmem = 1024 + (2 + 2 * kStages) * kTileBytes + 8 * kBarriers + 32;
+    static constexpr int kSplitSmem = kSmem + 256 * 8;      // and (m, l) of every row
+    static_assert(256 * DP * 4 <= (2 + kStages) * kTileBytes, "fp32 rows fit the buffers of Q and K");
     static constexpr int kSCol = 0, kOCol = 256;            // S of tile w at 128 w, O at 256 + DP w
 };
 
@@ -453,13 +461,82 @@ __device__ __forceinline__ bool any_not_finite(const uint4& u) {
     return bad;
 }
 
-// rp: heads per row group (1 << rp_log2), the query heads of one kv head or 1.
+// The rows of a split row tile (256, fp32 and swizzled in every block's `part`, (m, l) in
+// `ml`) that fall to this block, eight warps.  Lane x holds what the x-th of the warp's rows
+// needs of every part; then four rows at a time are read and joined, in the order of the
+// keys.  A function of its own: inlined, its registers made the main loop spill.
 template <typename T, int DP>
+__device__ __noinline__ void window_cluster_join(const WindowParams& p, const WindowTile& t, float* s_part, float* s_ml,
+                                                 const int* not_finite, int hg, int rows, int rp_log2, int rank,
+                                                 int splits, int warp, int lane) {
+    cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
+    constexpr int NV = DP / 32, R = 4;
+    bool again = false;
+    for (int q = 0; q < splits; ++q) again |= *static_cast<const volatile int*>(cl.map_shared_rank(not_finite, q)) != 0;
+    auto row_of = [&](int x) { return (x * splits + rank) * 8 + warp; };
+    const int n = 32 / splits;
+    float c[8], M = -INFINITY, L = 0.0f;
+    const int mine = min(row_of(lane), 255);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        c[q] = q < splits ? cl.map_shared_rank(s_ml, q)[mine * 2] : -INFINITY;
+        M = max3(M, c[q], M);
+    }
+    const float u = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        c[q] = exp2_fast(c[q] - u);
+        if (q < splits) L += cl.map_shared_rank(s_ml, q)[mine * 2 + 1] * c[q];
+    }
+    const float inv = L > 0.0f ? 1.0f / L : L, lg = L != 0.0f ? (u + log2f(L)) * kLn2 : -INFINITY;
+    for (int x0 = 0; x0 < n && (row_of(x0) >> rp_log2) < rows; x0 += R) {
+        float acc[R][NV];
+#pragma unroll
+        for (int y = 0; y < R; ++y)
+#pragma unroll
+            for (int e = 0; e < NV; ++e) acc[y][e] = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            if (q >= splits) break;
+            const float* part = cl.map_shared_rank(s_part, q);
+#pragma unroll
+            for (int y = 0; y < R; ++y) {
+                const int row = row_of(x0 + y);
+                const float w = __shfl_sync(0xffffffffu, c[q], x0 + y);
+#pragma unroll
+                for (int e = 0; e < NV; ++e) {
+                    const int d = lane + 32 * e;
+                    acc[y][e] = fmaf(w, part[row * DP + ((d / 4) ^ (row & 7)) * 4 + (d & 3)], acc[y][e]);
+                }
+            }
+        }
+#pragma unroll
+        for (int y = 0; y < R; ++y) {
+            const int row = row_of(x0 + y);
+            const int token = row >> rp_log2, head = (hg << rp_log2) + (row & ((1 << rp_log2) - 1));
+            const float f = __shfl_sync(0xffffffffu, inv, x0 + y), e0 = __shfl_sync(0xffffffffu, lg, x0 + y);
+            if (token >= rows) continue;
+            if (again) {
+                window_row_exact<T>(p, t, t.m0 + token, head, lane);
+                continue;
+            }
+            const int64_t qrow = t.q0 + t.m0 + token;
+            T* out = static_cast<T*>(p.out) + qrow * p.o_row + head * p.o_head;
+#pragma unroll
+            for (int e = 0; e < NV; ++e)
+                if (lane + 32 * e < p.dim) out[lane + 32 * e] = from_f32<T>(acc[y][e] * f);
+            if (lane == 0 && p.lse != nullptr) p.lse[qrow * p.heads + head] = e0;
+        }
+    }
+}
+
+// rp: heads per row group (1 << rp_log2), the query heads of one kv head or 1.
+template <typename T, int DP, bool SPLIT>
 __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_constant__ WindowParams p,
                                                                   const __grid_constant__ CUtensorMap tm_q,
                                                                   const __grid_constant__ CUtensorMap tm_k,
                                                                   const __grid_constant__ CUtensorMap tm_v, int rp_log2,
-                                                                  int groups) {
+                                                                  int groups, int splits) {
     using C = WindowTc<DP>;
     constexpr int NS = C::kStages;
     extern __shared__ uint8_t dyn[];
@@ -469,18 +546,25 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
         prefetch_tmap(&tm_k);
         prefetch_tmap(&tm_v);
     }
-    const int hg = blockIdx.x % groups;
+    const int block = SPLIT ? static_cast<int>(blockIdx.x) / splits : static_cast<int>(blockIdx.x);
+    const int hg = block % groups;
     const int tokens = 256 >> rp_log2;            // tokens of the block
     WindowTile t;
-    if (!window_tile(p, blockIdx.x / groups, tokens, lane, t)) return;
+    if (!window_tile(p, block / groups, tokens, lane, t)) return;
     const int rows = min(tokens, t.lq - t.m0);
     const int t0 = t.lk - t.lq + t.m0;            // position of the first token
     const int hi = min(t.lk, t0 + rows);          // keys [lo, hi) and the first ones
     const int lo = p.window > 0 ? max(0, t0 - p.window + 1) : 0;
     const int ns = p.window > 0 ? (max(0, min(p.sinks, hi)) + kWtKeys - 1) / kWtKeys : 0;
     const int w0 = max(ns * kWtKeys, lo);
-    const int nt = ns + (hi > w0 ? (hi - w0 + kWtKeys - 1) / kWtKeys : 0);
-    auto tile_base = [&](int i) { return i < ns ? i * kWtKeys : w0 + (i - ns) * kWtKeys; };
+    const int all = ns + (hi > w0 ? (hi - w0 + kWtKeys - 1) / kWtKeys : 0);
+    // this block's key tiles
+    const int rank = SPLIT ? static_cast<int>(blockIdx.x) % splits : 0;
+    const int i0 = SPLIT ? all * rank / splits : 0, nt = SPLIT ? all * (rank + 1) / splits - i0 : all;
+    auto tile_base = [&](int i) {
+        if (SPLIT) i += i0;
+        return i < ns ? i * kWtKeys : w0 + (i - ns) * kWtKeys;
+    };
 
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~uintptr_t{1023});
     uint8_t* s_q = smem;
@@ -500,6 +584,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(s_tmem + 1);
     volatile int* not_finite = abort_flag + 1;
+    float* s_ml = reinterpret_cast<float*>(bars + C::kBarriers + 4);   // [256][2], SPLIT only
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
         mbar_init(q_full + 1, 1);
@@ -788,7 +873,25 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
         if (m == INFINITY) l = NAN;   // inf - inf
         if (nt > 0 && ok) ok = __all_sync(0xffffffffu, wait(o_done + w, 0));
         tc_fence_after();
-        const bool mine = ok && local < rows;
+        if constexpr (SPLIT) {
+            // unnormalised, in fp32, 16-byte chunks swizzled by row; the products with Q and K are complete
+            float* part = reinterpret_cast<float*>(s_q) + (w * 128 + r) * DP;
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+                float o[32];
+                if (nt > 0) {
+                    tmem_ld32(to + c, o);
+                    tmem_wait_ld();
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    *reinterpret_cast<float4*>(part + (((c + e) / 4) ^ (r & 7)) * 4) =
+                        nt > 0 ? make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+            s_ml[(w * 128 + r) * 2] = m == -INFINITY ? m : m * p.sl2;
+            s_ml[(w * 128 + r) * 2 + 1] = l;
+        }
+        const bool mine = !SPLIT && ok && local < rows;
         const int64_t qrow = t.q0 + t.m0 + local;
         const float inv = l > 0.0f ? 1.0f / l : l;
         T* out = static_cast<T*>(p.out) + qrow * p.o_row + head * p.o_head;
@@ -796,7 +899,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
 #pragma unroll
         for (int c = 0; c < DP; c += 32) {
             float o[32];
-            if (nt > 0) {
+            if (!SPLIT && nt > 0) {
                 tmem_ld32(to + c, o);
                 tmem_wait_ld();
             }
@@ -818,7 +921,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
         if (mine && p.lse != nullptr)
             p.lse[qrow * p.heads + head] = l != 0.0f ? ((m == -INFINITY ? 0.0f : m * p.sl2) + log2f(l)) * kLn2 : -INFINITY;
         asm volatile("bar.sync 2, 320;" ::: "memory");
-        if (*not_finite && ok)
+        if (!SPLIT && *not_finite && ok)
             for (int x = warp; x < 256; x += 8) {
                 const int tok = x >> rp_log2;
                 if (tok < rows) window_row_exact<T>(p, t, t.m0 + tok, (hg << rp_log2) + (x & ((1 << rp_log2) - 1)), lane);
@@ -830,6 +933,15 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
     if (warp == 9) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
+    }
+    if constexpr (SPLIT) {
+        cooperative_groups::this_cluster().sync();
+        // (the softmax warps: the others gave their registers up)
+        if (warp < 8)
+            window_cluster_join<T, DP>(p, t, reinterpret_cast<float*>(s_q), s_ml, const_cast<const int*>(not_finite), hg, rows,
+                                       rp_log2, rank, splits, warp, lane);
+        __syncwarp();
+        cooperative_groups::this_cluster().sync();   // nobody leaves while its part is read
     }
 }
 

@@ -1080,3 +1080,54 @@ def test_empty_calls_on_the_device():
                         torch.zeros(1, 2, 16, **i32), 40)
     assert r["lens"].tolist() == [0] and bool((r["src"] == -1).all())
     ops.check_status(kp.device)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("h, g, d", [(8, 2, 128), (4, 4, 64), (6, 1, 80)])
+@pytest.mark.parametrize("lq, past", [([1], [3000]), ([64], [5000]), ([130], [2500]), ([3, 3], [9000, 2]), ([5, 0, 200], [1700, 4000, 1500])])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (1900, 150), (60, 3)])
+def test_few_queries_on_many_keys(dt, h, g, d, lq, past, window, sinks):
+    """Row tiles whose keys a cluster shares; blocks of it without keys."""
+    from project_chronos_b200 import ops
+    lk = [a + b for a, b in zip(lq, past)]
+    gen = _gen(h + lq[0])
+    q = (2 * torch.randn(sum(lq) + 2, h, d, generator=gen, device="cuda")).to(dt)
+    k = torch.randn(sum(lk), g, d, generator=gen, device="cuda").to(dt)
+    v = torch.randn(sum(lk), g, d, generator=gen, device="cuda").to(dt)
+    cq, ck = ([0] + torch.tensor(x).cumsum(0).tolist() for x in (lq, lk))
+    out = torch.full_like(q, 5.0)
+    lse = torch.full(q.shape[:2], 5.0, device="cuda")
+    call = lambda o, e: ops.window_attention(  # noqa: E731
+        q, k, v, torch.tensor(cq, dtype=torch.int32, device="cuda"), cu_seqlens_k=torch.tensor(ck, dtype=torch.int32, device="cuda"),
+        window=window, sinks=sinks, out=o, lse=e)
+    call(out, lse)
+    again = torch.full_like(q, 5.0)
+    call(again, None)
+    ops.check_status(q.device)
+    assert torch.equal(out, again)
+    assert bool((out[sum(lq):] == 5.0).all()) and bool((lse[sum(lq):] == 5.0).all())
+    for b in range(len(lq)):
+        _check_prompt(out, lse, q, k, v, lq[b], lk[b], cq[b], ck[b], window, sinks, dt, _some_rows(lq[b]))
+
+
+@gpu
+def test_hidden_values_do_not_reach_a_split_row():
+    from project_chronos_b200 import ops
+    n, past, h, g, d, window = 90, 4000, 8, 2, 128, 3000
+    gen = _gen(2)
+    q, k, v = (torch.randn(r, x, d, generator=gen, device="cuda").to(BF) for r, x in ((n, h), (n + past, g), (n + past, g)))
+    first = past - window + 40                        # seen by the rows up to 39 - 1 only
+    v[first, 1, 7] = math.nan
+    v[past + 50, :, 3] = math.inf                     # seen from row 50 on
+    cq, ck = (torch.tensor([0, x], dtype=torch.int32, device="cuda") for x in (n, n + past))
+    out = ops.window_attention(q, k, v, cq, cu_seqlens_k=ck, window=window)
+    clean = v.clone()
+    clean[first], clean[past + 50] = 0.0, 0.0
+    for i in (39, 40, 45, 49):                        # row i sees keys past + i - window + 1 .. past + i
+        sees_first = past + i - window < first
+        assert sees_first == (i < 40)
+        if not sees_first:
+            _check_prompt(out, None, q, k, clean, n, n + past, 0, 0, window, 0, BF, [i])
+    assert bool(torch.isnan(out[20, 4:, 7]).all()) and bool(torch.isfinite(out[20, :4]).all())
+    assert bool((out[60, :, 3] == math.inf).all()) and bool(torch.isfinite(out[60, :, 4:]).all())
