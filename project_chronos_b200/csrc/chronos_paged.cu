@@ -367,7 +367,7 @@ extern "C" int chronos_paged_decode(const ChronosPagedDecodeArgs* a, void* strea
     const int limit = slot_limit(a->cache, a->slot_cap, a->weights != nullptr);
     const int64_t adds = static_cast<int64_t>(a->cache.batch) * a->heads +
                          static_cast<int64_t>(a->cache.batch) * a->cache.kv_heads * (limit / kPdWeightSlots + 1);
-    if (units >= INT32_MAX || adds >= INT32_MAX)
+    if (units >= (1 << 30) || adds >= INT32_MAX)
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: batch %d * heads * slots %d too large", what, a->cache.batch, limit);
     if (d.total > 0 && (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < d.total))
         return fail(CHRONOS_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes, %zu (256-byte aligned) needed", what,

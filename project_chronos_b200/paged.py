@@ -56,6 +56,7 @@ class PagedCache:
             slots = (batch, kv_heads, table_width * page_size)
             self.weights = torch.zeros(slots, dtype=torch.float32, device=device)
             self.positions = torch.zeros(slots, dtype=torch.int32, device=device)
+        self._evicted = False    # slots and positions are no longer the same
         self._free: List[int] = list(range(num_pages - 1, -1, -1))
         self._pages: List[List[int]] = [[] for _ in range(batch)]
 
@@ -115,7 +116,9 @@ class PagedCache:
                out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of each row's newest token (already appended) over its slots, q
         [B, heads, D] -> [B, heads, D]; adds to ``weights`` where they are tracked.
-        A window counts slots: it belongs to rows nothing was evicted from."""
+        A window counts slots: it is refused once the cache was evicted from."""
+        if window and self._evicted:
+            raise RuntimeError("a window counts slots, which an eviction has reordered: attend without one")
         return ops.paged_attn_decode(q, self.k_pages, self.v_pages, self.page_table, self.lens, scale=scale,
                                      window=window, sinks=sinks, weights=self.weights, out=out, lse=lse)
 
@@ -124,5 +127,6 @@ class PagedCache:
         place.  Returns src int32 [B, kv_heads, budget]: where each slot came from."""
         if self.weights is None:
             raise RuntimeError("evict needs a cache with track_weights=True")
+        self._evicted = True
         return ops.paged_evict(self.k_pages, self.v_pages, self.page_table, self.lens, self.seen, self.weights,
                                self.positions, budget, sinks=sinks, recent=recent, lens_out=self.lens)["src"]

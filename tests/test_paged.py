@@ -883,6 +883,12 @@ def test_paged_cache_rows_come_and_go():
         step(replay)
     ops.check_status(c.lens.device)
     assert c.positions[0, 0, :25].tolist() == list(range(25))
+    q = rnd(2, h, d)
+    assert bool(torch.isfinite(c.attend(q, window=20, sinks=2)).all())
+    src = c.evict(20, sinks=2, recent=8)
+    assert c.lens.tolist() == [20, 20] and sorted(src[0, 0].tolist())[:2] == [0, 1]
+    with pytest.raises(RuntimeError, match="window"):
+        c.attend(q, window=20)
     c.release(0)
     with pytest.raises(RuntimeError, match="at most 8"):
         c.reserve(1, 128 * 2)
