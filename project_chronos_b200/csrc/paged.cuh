@@ -391,7 +391,7 @@ struct PagedMma {
 // Measured, 32 / 8 heads of 128: 4 rows of 100003 to 131072 slots in fp16 300 us, 6.6 TB/s
 // (16-wide rows of heads, maxima and page lookups per row of slots: 418 us); 16 rows of
 // 16384 slots, 8 / 2 heads: 105 us with head_dim 64, 89 us with 256 (bf16, 5.1 and 6.0
-// TB/s), 119 us in fp32 (4.5 TB/s, bound by the splitting into tf32).
+// TB/s), 127 us in fp32 (4.2 TB/s, bound by the splitting into tf32).
 //
 // NT: groups of 8 query heads (1 or 2).  CL: a cluster of p.cluster blocks per row
 // shares its blocks of 64 places and joins through distributed shared memory;
