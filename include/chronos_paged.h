@@ -63,7 +63,9 @@ typedef struct ChronosPagedCache {
  * rows, in order; without cu_seqlens one token per sequence) goes to slot
  * lens[b] + i.  With `weights`, weights[b, g, slot] = 0; with `positions`,
  * positions[b, g, slot] = seen[b] + i.  Rows behind the last sequence are not
- * read. */
+ * read.  With `lens_out`, lens_out[b] = lens[b] + the tokens of sequence b stored
+ * before its first dropped one, and seen_out[b] = seen[b] + the same number;
+ * lens_out may be lens and seen_out may be seen, any other overlap is refused. */
 typedef struct ChronosPagedAppendArgs {
     ChronosPagedCache cache;
     int64_t num_tokens;        /* rows of k and v */
@@ -75,6 +77,8 @@ typedef struct ChronosPagedAppendArgs {
     float* weights;            /* [B, G, slot_cap] or NULL */
     int32_t* positions;        /* [B, G, slot_cap] or NULL */
     int64_t slot_cap;
+    int32_t* lens_out;         /* [B] or NULL */
+    int32_t* seen_out;         /* [B] or NULL (needs seen) */
     int32_t* status;           /* device status word, or NULL */
 } ChronosPagedAppendArgs;
 

@@ -248,6 +248,8 @@ class ChronosPagedAppendArgs(ctypes.Structure):
         ("weights", ctypes.c_void_p),
         ("positions", ctypes.c_void_p),
         ("slot_cap", ctypes.c_int64),
+        ("lens_out", ctypes.c_void_p),
+        ("seen_out", ctypes.c_void_p),
         ("status", ctypes.c_void_p),
     ]
 

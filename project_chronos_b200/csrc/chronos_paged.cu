@@ -42,6 +42,10 @@ int check_cache_pointers(const ChronosPagedCache& c, const char* what) {
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: lens, page_table, k_pages and v_pages are required", what);
     return CHRONOS_OK;
 }
+// Whether two arrays of n numbers overlap (`same`: other than as one).
+bool cross(const int32_t* a, const int32_t* b, int n, bool same) {
+    return a != nullptr && b != nullptr && a < b + n && b < a + n && !(same && a == b);
+}
 // A window (or number of first tokens) as the kernels take it: rows have at most 2^30
 // keys, so a longer one hides nothing, and positions minus it stay within 32 bits.
 int cut_window(int window) { return std::min(window, 1 << 30); }
@@ -435,9 +439,17 @@ extern "C" int chronos_paged_append(const ChronosPagedAppendArgs* a, void* strea
     const bool arrays = a->weights != nullptr || a->positions != nullptr;
     if (arrays && a->slot_cap < 0)
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: slot_cap %lld", what, static_cast<long long>(a->slot_cap));
-    if (a->num_tokens == 0 || a->cache.batch == 0) return CHRONOS_OK;
+    if (a->seen_out != nullptr && a->seen == nullptr)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: seen_out needs seen", what);
+    const int n = a->cache.batch;
+    if (cross(a->lens_out, a->cache.lens, n, true) || cross(a->seen_out, a->seen, n, true) ||
+        cross(a->lens_out, a->seen, n, false) || cross(a->seen_out, a->cache.lens, n, false) ||
+        cross(a->lens_out, a->seen_out, n, false))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: lens_out may be lens, seen_out may be seen, and they overlap nothing else", what);
+    const bool counts = a->lens_out != nullptr || a->seen_out != nullptr;
+    if (a->cache.batch == 0 || (a->num_tokens == 0 && !counts)) return CHRONOS_OK;
     if (int rc = check_cache_pointers(a->cache, what)) return rc;
-    if (a->k == nullptr || a->v == nullptr) return fail(CHRONOS_ERR_INVALID_ARG, "%s: k and v are required", what);
+    if (a->num_tokens > 0 && (a->k == nullptr || a->v == nullptr)) return fail(CHRONOS_ERR_INVALID_ARG, "%s: k and v are required", what);
     PagedAppendParams p{};
     p.c = a->cache;
     p.tokens = a->num_tokens;
@@ -453,6 +465,8 @@ extern "C" int chronos_paged_append(const ChronosPagedAppendArgs* a, void* strea
     p.positions = a->positions;
     p.slot_cap = a->slot_cap;
     p.max_slots = slot_limit(a->cache, a->slot_cap, arrays);
+    p.lens_out = a->lens_out;
+    p.seen_out = a->seen_out;
     p.status = a->status;
     const int es = static_cast<int>(elem_bytes(a->cache.dtype));
     const bool wide = copies16(a->cache) && aligned(a->k, 16) && aligned(a->v, 16) &&
@@ -462,9 +476,14 @@ extern "C" int chronos_paged_append(const ChronosPagedAppendArgs* a, void* strea
     const int64_t blocks = (a->num_tokens + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 64 * static_cast<int64_t>(sm_count()))));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (wide) CHRONOS_CUDA_CHECK(launch_kernel(paged_append_kernel<uint4>, grid, dim3(kAppendThreads), 0, st, false, p, units, per));
-    else if (es == 2) CHRONOS_CUDA_CHECK(launch_kernel(paged_append_kernel<uint16_t>, grid, dim3(kAppendThreads), 0, st, false, p, units, per));
-    else CHRONOS_CUDA_CHECK(launch_kernel(paged_append_kernel<uint32_t>, grid, dim3(kAppendThreads), 0, st, false, p, units, per));
+    if (a->num_tokens > 0) {
+        if (wide) CHRONOS_CUDA_CHECK(launch_kernel(paged_append_kernel<uint4>, grid, dim3(kAppendThreads), 0, st, false, p, units, per));
+        else if (es == 2) CHRONOS_CUDA_CHECK(launch_kernel(paged_append_kernel<uint16_t>, grid, dim3(kAppendThreads), 0, st, false, p, units, per));
+        else CHRONOS_CUDA_CHECK(launch_kernel(paged_append_kernel<uint32_t>, grid, dim3(kAppendThreads), 0, st, false, p, units, per));
+    }
+    if (counts && a->cu_seqlens != nullptr)
+        CHRONOS_CUDA_CHECK(launch_kernel(paged_advance_kernel, dim3((n + kAppendThreads / 32 - 1) / (kAppendThreads / 32)),
+                                         dim3(kAppendThreads), 0, st, a->num_tokens > 0, p));
     return CHRONOS_OK;
 }
 

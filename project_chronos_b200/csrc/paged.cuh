@@ -1183,16 +1183,26 @@ struct PagedAppendParams {
     int32_t* positions;
     int64_t slot_cap;
     int max_slots;
+    int32_t* lens_out;
+    int32_t* seen_out;
     int32_t* status;
 };
 
 constexpr int kAppendThreads = 256;
+
+// Sequence b's new length: `stored` tokens were.  One lane calls it, after the whole warp
+// has read the sequence's old ones.
+__device__ __forceinline__ void paged_advance(const PagedAppendParams& p, int b, int stored) {
+    if (p.lens_out != nullptr) p.lens_out[b] = p.c.lens[b] + stored;
+    if (p.seen_out != nullptr) p.seen_out[b] = p.seen[b] + stored;
+}
 
 // Copies: 4 * G * D * size bytes of traffic per token.  One warp per token: it
 // finds the sequence with one ballot per 32 offsets, then its lanes copy the
 // token's K and V rows in units of V bytes (16, or one element where the
 // strides forbid more), four loads in flight before the first store.  8 prompts of up
 // to 8192 tokens, 8 heads of 128 in bf16: 57 us, 5.6 TB/s read and written.
+// Without offsets a warp has a sequence to itself and advances its length, too.
 template <typename V>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ PagedAppendParams p,
                                                                       int units_per_head, int elems_per_unit) {
@@ -1220,7 +1230,11 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
         const bool fits = slot >= 0 && slot < p.max_slots;
         const int page = fits ? p.c.page_table[b * p.c.page_table_stride + slot / p.c.page_size] : -1;
         if (page < 0 || page >= p.c.num_pages) {
-            if (lane == 0) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
+            if (p.cu == nullptr) __syncwarp();
+            if (lane == 0) {
+                report_status(p.status, CHRONOS_ERR_INVALID_ARG);
+                if (p.cu == nullptr) paged_advance(p, b, 0);
+            }
             continue;
         }
         const int64_t in_page = slot % p.c.page_size;
@@ -1255,7 +1269,40 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
             if (p.weights != nullptr) p.weights[at] = 0.0f;
             if (p.positions != nullptr) p.positions[at] = static_cast<int32_t>(p.seen[b] + i);
         }
+        if (p.cu == nullptr) {
+            __syncwarp();
+            if (lane == 0) paged_advance(p, b, 1);
+        }
     }
+}
+
+// The lengths after a packed append, one warp per sequence: its tokens up to the first that
+// had no slot or no page (the pages its new slots lie in, 32 at a time).
+__global__ void __launch_bounds__(kAppendThreads) paged_advance_kernel(const __grid_constant__ PagedAppendParams p) {
+    const int lane = threadIdx.x & 31;
+    const int b = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
+    if (b >= p.c.batch) return;
+    pdl_wait();   // the rows are stored by the old lengths
+    const int64_t first = p.cu[b], last = min(static_cast<int64_t>(p.cu[b + 1]), p.tokens);
+    if (lane == 0 && (first < 0 || p.cu[b + 1] < first || p.cu[b + 1] > p.tokens)) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
+    const int64_t from = p.c.lens[b], size = p.c.page_size;
+    int64_t n = from >= 0 && first >= 0 ? max(int64_t{0}, min(last - first, p.max_slots - from)) : 0;
+    if (n > 0)
+        for (int64_t p0 = from / size; p0 * size < from + n; p0 += 32) {
+            const int64_t at = p0 + lane;
+            bool none = false;
+            if (at * size < from + n) {
+                const int page = p.c.page_table[b * p.c.page_table_stride + at];
+                none = page < 0 || page >= p.c.num_pages;
+            }
+            const uint32_t gone = __ballot_sync(0xffffffffu, none);
+            if (gone) {
+                n = max(int64_t{0}, (p0 + __ffs(gone) - 1) * size - from);
+                break;
+            }
+        }
+    __syncwarp();
+    if (lane == 0) paged_advance(p, b, static_cast<int>(n));
 }
 
 // ---------------------------------------------------------------------------

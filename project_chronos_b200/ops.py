@@ -635,16 +635,20 @@ def _workspace(fn, args, dev: torch.device, index: int) -> Optional[torch.Tensor
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                  page_table: torch.Tensor, lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
                  seen: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,
-                 positions: Optional[torch.Tensor] = None) -> None:
+                 positions: Optional[torch.Tensor] = None, lens_out: Optional[torch.Tensor] = None,
+                 seen_out: Optional[torch.Tensor] = None) -> None:
     """Write new key/value rows into the pages (include/chronos_paged.h).
 
     k, v [T, kv heads, D]: one token per sequence (T = B), or packed sequences with
     ``cu_seqlens`` int32 [B + 1]; k_pages, v_pages [pages, page size, kv heads, D];
-    page_table int32 [B, pages]; lens int32 [B], slots in use before the call (not
-    changed).  Sequence b's i-th token goes to slot lens[b] + i; where given,
+    page_table int32 [B, pages]; lens int32 [B], slots in use before the call.
+    Sequence b's i-th token goes to slot lens[b] + i; where given,
     ``weights`` fp32 [B, kv heads, slots] get 0 there and ``positions`` int32 of
-    that shape seen[b] + i (``seen`` int32 [B]: tokens seen before).  A page must
-    not belong to two sequences that are written."""
+    that shape seen[b] + i (``seen`` int32 [B]: tokens seen before).  ``lens_out`` and
+    ``seen_out`` int32 [B] (lens and seen themselves, or others) receive lens and seen
+    plus the tokens stored: one without a slot or a page is dropped and recorded as
+    CHRONOS_ERR_INVALID_ARG in the status word, and neither it nor what follows it in
+    its sequence counts.  A page must not belong to two sequences that are written."""
     if not k_pages.is_cuda:
         _no_cpu(k_pages)
     dev, index, grad = k_pages.device, k_pages.get_device(), torch.is_grad_enabled()
@@ -666,6 +670,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         cache, t, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
         None if cu_seqlens is None else _dense("cu_seqlens", cu_seqlens, (b + 1,), torch.int32, index, dev),
         None if seen is None else _dense("seen", seen, (b,), torch.int32, index, dev), wp, pp, cap,
+        None if lens_out is None else _dense("lens_out", lens_out, (b,), torch.int32, index, dev),
+        None if seen_out is None else _dense("seen_out", seen_out, (b,), torch.int32, index, dev),
         status_word(dev).data_ptr())
     _launch(N.load_library().chronos_paged_append, args, index)
 

@@ -11,7 +11,7 @@ rotated, which makes attention independent of the order of the slots and lets
     cache.reserve(row, slots)                       # host: pages for a row
     out = ops.window_attention(q, k, v, cu)         # a packed batch of prompts
     cache.append(k, v, cu)                          # ... into the pages
-    cache.append(k1, v1)                            # one token per row
+    cache.append(k1, v1)                            # one token per row (idle rows: with offsets, none)
     out = cache.attend(q1)                          # attention of those tokens
     cache.evict(budget, sinks=4, recent=256)        # least attention goes
 
@@ -103,14 +103,12 @@ class PagedCache:
 
     def append(self, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None) -> None:
         """Append one token per row (k, v [B, kv_heads, D]) or packed sequences
-        (``cu_seqlens`` int32 [B + 1]).  A row whose pages do not reach drops the tokens
-        behind them and records CHRONOS_ERR_INVALID_ARG in the status word."""
+        (``cu_seqlens`` int32 [B + 1]; no tokens for a row that is idle).  A row whose
+        pages do not reach drops the tokens behind them, does not count them and records
+        CHRONOS_ERR_INVALID_ARG in the status word."""
         ops.paged_append(k, v, self.k_pages, self.v_pages, self.page_table, self.lens, cu_seqlens=cu_seqlens,
-                         seen=None if self.positions is None else self.seen, weights=self.weights,
-                         positions=self.positions)
-        grown = 1 if cu_seqlens is None else cu_seqlens[1:] - cu_seqlens[:-1]
-        self.lens += grown
-        self.seen += grown
+                         seen=self.seen, weights=self.weights, positions=self.positions, lens_out=self.lens,
+                         seen_out=self.seen)
 
     def attend(self, q: torch.Tensor, scale: Optional[float] = None, window: int = 0, sinks: int = 0,
                out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -1137,3 +1137,141 @@ def test_hidden_values_do_not_reach_a_split_row():
             _check_prompt(out, None, q, k, clean, n, n + past, 0, 0, window, 0, BF, [i])
     assert bool(torch.isnan(out[20, 4:, 7]).all()) and bool(torch.isfinite(out[20, :4]).all())
     assert bool((out[60, :, 3] == math.inf).all()) and bool(torch.isfinite(out[60, :, 4:]).all())
+
+
+# ---------------------------------------------------------------------------------------
+# lengths that the append counts
+# ---------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("track", [True, False])
+def test_dropped_tokens_are_not_counted(track):
+    """A row without pages, or with too few, keeps the length of what it stored: what comes
+    after it gets pages again lands right behind, and nothing stale is attended to."""
+    from project_chronos_b200 import PagedCache, ops
+    from project_chronos_b200 import _native as N
+    h, g, d, dt = 8, 2, 64, BF
+    gen = _gen(15)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device="cuda").to(dt)  # noqa: E731
+    c = PagedCache(2, 12, g, d, 8, "cuda", dt, page_size=16, track_weights=track)
+    dev = c.lens.device
+    book = [[], []]
+
+    def put(counts, stored):
+        t = sum(counts)
+        k, v = rnd(t, g, d), rnd(t, g, d)
+        cu = torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+        c.append(k, v, None if counts == [1, 1] else cu)
+        at = 0
+        for b, n in enumerate(counts):
+            book[b] += [(k[at + i], v[at + i]) for i in range(stored[b])]
+            at += n
+        if list(counts) != list(stored):
+            with pytest.raises(N.ChronosMoeError, match="INVALID_ARG"):
+                ops.check_status(dev)
+        look()
+
+    def look():
+        assert c.lens.tolist() == [len(x) for x in book] and c.seen.tolist() == c.lens.tolist()
+        q = rnd(2, h, d)
+        out = c.attend(q)
+        ops.check_status(dev)
+        for b in range(2):
+            if track:
+                assert c.positions[b, 0, : len(book[b])].tolist() == list(range(len(book[b])))
+            if not book[b]:
+                assert bool((out[b] == 0).all())
+                continue
+            ks, vs = (torch.stack([r[i] for r in book[b]]) for i in (0, 1))
+            ref, _, _, a, f = _attend(q[b], ks, vs, d ** -0.5, _visible(len(ks), 0, 0, "cuda"))
+            _check_out(out[b], ref, a, f, len(ks), dt)
+
+    c.reserve(0, 40)
+    c.reserve(1, 60)
+    put([40, 20], [40, 20])
+    c.release(0)
+    book[0] = []
+    for _ in range(5):
+        put([1, 1], [0, 1])                           # row 0 is idle
+    c.reserve(0, 33)                                  # 48 slots, pages used before
+    put([33, 0], [33, 0])
+    for i in range(18):                               # row 0 is full after 15
+        put([1, 1], [int(i < 15), 1])
+    c.reserve(0, 64)
+    put([1, 1], [1, 1])
+    put([40, 2], [15, 2])                             # the first 15 of a packed row fit
+    c.reserve(0, 70)
+    put([3, 0], [3, 0])
+
+
+@gpu
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("dt, d", [(BF, 64), (FP, 5)])
+def test_append_counts_what_it_stored(dt, d, in_place):
+    """Lengths and tokens seen after packed and one-token calls: rows that are full, have a hole in
+    their table, none of it, a bad length, no tokens."""
+    from project_chronos_b200 import _native as N
+    from project_chronos_b200 import ops
+    g, size, width = 2, 4, 70
+    b = 45
+    gen = torch.Generator().manual_seed(d)
+    have = torch.randint(0, width + 1, (b,), generator=gen)     # pages of each row
+    have[:4] = torch.tensor([width, width, 0, 40])
+    past = (torch.rand(b, generator=gen) * (have * size + 1)).long().clamp(max=width * size)
+    new = torch.randint(0, 60, (b,), generator=gen)
+    new[:6] = torch.tensor([width * size, 0, 5, 200, 0, 1])
+    past[0], past[3] = 0, 9
+    table = torch.full((b, width), -1, dtype=torch.int32)
+    pages = int(have.sum())
+    order = torch.randperm(pages, generator=gen).to(torch.int32)
+    at = 0
+    for i in range(b):
+        table[i, : have[i]] = order[at: at + int(have[i])]
+        at += int(have[i])
+    table[3, 35] = pages                                        # a page that is none, its neighbours are
+    past[7] = -1
+    room = have * size
+    room[3], room[7] = 35 * size, -1
+    to = dict(dtype=torch.int32, device="cuda")
+    for counts in (new, torch.ones(b, dtype=torch.long)):
+        kp, vp = (torch.zeros(pages, size, g, d, dtype=dt, device="cuda") for _ in range(2))
+        lens, seen = past.to(**to), (past + 1000).to(**to)
+        t = int(counts.sum())
+        k, v = (torch.randn(t, g, d, generator=_gen(i), device="cuda").to(dt) for i in (1, 2))
+        cu = None if counts is not new else torch.tensor([0] + counts.cumsum(0).tolist(), **to)
+        lo, so = (lens, seen) if in_place else (torch.full_like(lens, 77), torch.full_like(seen, 77))
+        ops.paged_append(k, v, kp, vp, table.cuda(), lens, cu_seqlens=cu, seen=seen, lens_out=lo, seen_out=so)
+        with pytest.raises(N.ChronosMoeError, match="INVALID_ARG"):
+            ops.check_status(kp.device)
+        stored = torch.minimum(counts, (room - past).clamp(min=0))
+        stored[7] = 0
+        assert lo.tolist() == (past + stored).tolist() and so.tolist() == (past + 1000 + stored).tolist()
+        if not in_place:
+            assert lens.tolist() == past.tolist()
+        first = 0
+        for i in range(b):
+            for j in range(int(stored[i])):
+                s = int(past[i]) + j
+                assert torch.equal(kp[int(table[i, s // size]), s % size], k[first + j])
+            first += int(counts[i])
+    # offsets beyond the rows count what is there; without rows the lengths are copied
+    ops.paged_append(k[:3], v[:3], kp, vp, table[:2].cuda(), torch.zeros(2, **to), cu_seqlens=torch.tensor([0, 2, 9], **to),
+                     lens_out=lo[:2])
+    with pytest.raises(N.ChronosMoeError, match="INVALID_ARG"):
+        ops.check_status(kp.device)
+    assert lo[:2].tolist() == [2, 1]
+    ops.paged_append(k[:0], v[:0], kp, vp, table[:2].cuda(), torch.tensor([5, 6], **to), cu_seqlens=torch.zeros(3, **to),
+                     lens_out=lo[:2])
+    assert lo[:2].tolist() == [5, 6]
+    ops.check_status(kp.device)
+
+
+def test_append_refuses_lengths_that_overlap(lib):
+    from project_chronos_b200 import _native as N
+    for f, text in ((dict(seen_out=4096), b"seen_out needs seen"), (dict(lens_out=1028), b"overlap"),
+                    (dict(seen=2048, seen_out=2052), b"overlap"), (dict(seen=2048, lens_out=2048), b"overlap"),
+                    (dict(seen=2048, seen_out=1024), b"overlap"), (dict(seen=2048, seen_out=4096, lens_out=4100), b"overlap"),
+                    (dict(seen=2048, seen_out=2048, lens_out=1024), b"required")):
+        a = N.ChronosPagedAppendArgs(cache=_native_cache(N, lens=1024), num_tokens=2, **f)
+        assert lib.chronos_paged_append(ctypes.byref(a), None) == N.CHRONOS_ERR_INVALID_ARG
+        assert text in lib.chronos_moe_last_error()
