@@ -288,7 +288,8 @@ __global__ void __launch_bounds__(kWsThreads) window_simt_kernel(const __grid_co
 //
 // O is rescaled only when a row's maximum grew by more than 2^8 in weight: until
 // then weights are taken against the older maximum, at most 256 times too large,
-// which the fp32 sums and both 16-bit formats hold without loss.
+// which the fp32 sums and both 16-bit formats hold without loss (fp16 weights also
+// carry 2^7, see WeightLift).
 constexpr int kWtThreads = 384;
 constexpr int kWtKeys = 128;
 constexpr float kWtRescaleLog2 = 8.0f;
@@ -792,6 +793,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
         const int head = (hg << rp_log2) + (r & ((1 << rp_log2) - 1));
         const int tr = t0 + local;                            // this row's position
         const int ta = t0 + w * per, tb = min(ta + per, hi) - 1;   // the tile's first and last positions
+        constexpr float kLift = WeightLift<T>::value;
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
         for (int i = 0; i < nt; ++i) {
@@ -846,7 +848,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
                     }
                 }
             }
-            const float u = m == -INFINITY ? 0.0f : m * p.sl2;
+            const float u = m == -INFINITY ? 0.0f : m * p.sl2 - kLift;
             const float2 scale = make_float2(p.sl2, p.sl2), shift = make_float2(-u, -u);
             float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
@@ -888,7 +890,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
                     *reinterpret_cast<float4*>(part + (((c + e) / 4) ^ (r & 7)) * 4) =
                         nt > 0 ? make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
-            s_ml[(w * 128 + r) * 2] = m == -INFINITY ? m : m * p.sl2;
+            s_ml[(w * 128 + r) * 2] = m == -INFINITY ? m : m * p.sl2 - kLift;
             s_ml[(w * 128 + r) * 2 + 1] = l;
         }
         const bool mine = !SPLIT && ok && local < rows;
@@ -919,7 +921,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
                 }
         }
         if (mine && p.lse != nullptr)
-            p.lse[qrow * p.heads + head] = l != 0.0f ? ((m == -INFINITY ? 0.0f : m * p.sl2) + log2f(l)) * kLn2 : -INFINITY;
+            p.lse[qrow * p.heads + head] = l != 0.0f ? ((m == -INFINITY ? 0.0f : m * p.sl2 - kLift) + log2f(l)) * kLn2 : -INFINITY;
         asm volatile("bar.sync 2, 320;" ::: "memory");
         if (!SPLIT && *not_finite && ok)
             for (int x = warp; x < 256; x += 8) {

@@ -1275,3 +1275,106 @@ def test_append_refuses_lengths_that_overlap(lib):
         a = N.ChronosPagedAppendArgs(cache=_native_cache(N, lens=1024), num_tokens=2, **f)
         assert lib.chronos_paged_append(ctypes.byref(a), None) == N.CHRONOS_ERR_INVALID_ARG
         assert text in lib.chronos_moe_last_error()
+
+
+# ---------------------------------------------------------------------------------------
+# fp16 weights far below the largest
+# ---------------------------------------------------------------------------------------
+
+def _fp16_terms(n, v):
+    """What rounding to fp16 adds where weights are taken against a maximum 2^7 below: the result's
+    last place below the normal range, and the weights' (2^-25 of 2^7, relative to a sum of at least 1)."""
+    return 2.0 ** -25 + n * 2.0 ** -32 * float(v.abs().max())
+
+
+def _check_tight(got, ref, a, f, n, v):
+    u = _unit(HF)
+    tol = u * ref.abs() + (u + f[:, None] + n * 2.0 ** -23) * a + _fp16_terms(n, v)
+    err = (got.double() - ref).abs()
+    assert bool((err <= tol).all()), f"off by {float((err / tol).max()):.2f} of the tolerance"
+
+
+def _some_heavy(n, g, d, gap, at):
+    """Keys and values of which the slots `at` outweigh each other one by 2^gap, for a query whose first
+    16 elements sum to `gap`; their values are zero, so the result is what the light ones leave."""
+    k = torch.zeros(n, g, d, dtype=HF, device="cuda")
+    k[at, :, :16] = math.log(2.0)
+    v = (64.0 + 64.0 * torch.rand(n, g, d, generator=_gen(gap), device="cuda")).to(HF)
+    v[at] = 0.0
+    return k, v
+
+
+@gpu
+@pytest.mark.parametrize("gap", [20, 25, 26, 29])
+@pytest.mark.parametrize("b, n, h, g, d", [(1, 131072, 8, 2, 128), (300, 4001, 16, 2, 64), (140, 500, 20, 2, 256), (140, 500, 4, 2, 128),
+                                           (2, 9000, 6, 2, 36)])
+def test_fp16_light_slots_count_next_to_heavy_ones(b, n, h, g, d, gap):
+    """One heavy slot for each of a block's warps; fewer and more rows than blocks."""
+    from project_chronos_b200 import ops
+    size = 16
+    k, v = _some_heavy(n, g, d, gap, [5, 21, 37, 53])
+    width = -(-n // size)
+    table = torch.arange(width, dtype=torch.int32, device="cuda").expand(b, width).contiguous()
+    kp, vp = (torch.zeros(width * size, g, d, dtype=HF, device="cuda") for _ in range(2))
+    kp[:n], vp[:n] = k, v
+    kp, vp = kp.view(width, size, g, d), vp.view(width, size, g, d)
+    q = torch.zeros(b, h, d, dtype=HF, device="cuda")
+    q[..., :16] = gap / 16
+    lens = torch.full((b,), n, dtype=torch.int32, device="cuda")
+    w = torch.zeros(b, g, width * size, device="cuda")
+    lse, lse2 = torch.empty(b, h, device="cuda"), torch.empty(b, h, device="cuda")
+    out = ops.paged_attn_decode(q, kp, vp, table, lens, scale=1.0, lse=lse)
+    out2 = ops.paged_attn_decode(q, kp, vp, table, lens, scale=1.0, lse=lse2, weights=w)
+    ref, rl, p, a, f = _attend(q[0], k, v, 1.0, _visible(n, 0, 0, "cuda"))
+    want = p.view(g, h // g, n).sum(1)
+    for i in (0, b // 2, b - 1):
+        for o, e in ((out, lse), (out2, lse2)):
+            _check_tight(o[i], ref, a, f, n, v)
+            _check_lse(e[i], rl, f)
+        assert bool(((w[i, :, :n].double() - want).abs() <= (f.max() + (h + 1) * 2.0 ** -24) * want).all())
+
+
+@gpu
+@pytest.mark.parametrize("gap", [20, 25, 26, 29])
+@pytest.mark.parametrize("h, g, d, lq, lk", [(8, 2, 128, 40, 9000), (4, 4, 64, 600, 4000), (4, 1, 128, 1, 20000), (4, 2, 80, 4000, 4000)])
+def test_fp16_light_keys_count_next_to_a_heavy_one(h, g, d, lq, lk, gap):
+    from project_chronos_b200 import ops
+    k, v = _some_heavy(lk, g, d, gap, [5])
+    q = torch.zeros(lq, h, d, dtype=HF, device="cuda")
+    q[..., :16] = gap / 16
+    cq, ck = (torch.tensor([0, x], dtype=torch.int32, device="cuda") for x in (lq, lk))
+    lse = torch.empty(lq, h, device="cuda")
+    out = ops.window_attention(q, k, v, cq, cu_seqlens_k=ck, scale=1.0, lse=lse)
+    for i in _some_rows(lq):
+        if lk - lq + i < 6:
+            continue
+        ref, rl, _, a, f = _attend(q[i], k, v, 1.0, _visible(lk, 0, 0, "cuda", at=lk - lq + i))
+        _check_tight(out[i], ref, a, f, lk, v)
+        _check_lse(lse[i], rl, f)
+
+
+@gpu
+@pytest.mark.parametrize("step", [7.9, 8.0, 8.1, 15.0])
+def test_fp16_scores_that_climb(step):
+    """Maxima that lag behind by up to 2^8 in weight, every 128 keys a step higher."""
+    from project_chronos_b200 import ops
+    n, h, g, d, size = 1000, 8, 2, 64, 16
+    k = torch.zeros(n, g, d, dtype=HF, device="cuda")
+    k[:, :, 0] = (torch.arange(n, device="cuda") // 128).to(HF)[:, None]
+    v = torch.randn(n, g, d, generator=_gen(1), device="cuda").to(HF)
+    q = torch.zeros(n, h, d, dtype=HF, device="cuda")
+    q[..., 0] = step
+    scale = math.log(2.0)
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    lse = torch.empty(n, h, device="cuda")
+    out = ops.window_attention(q, k, v, cu, scale=scale, lse=lse)
+    kp, vp = (torch.zeros(63 * size, g, d, dtype=HF, device="cuda") for _ in range(2))
+    kp[:n], vp[:n] = k, v
+    table = torch.arange(63, dtype=torch.int32, device="cuda").view(1, 63)
+    one = ops.paged_attn_decode(q[n - 1:], kp.view(63, size, g, d), vp.view(63, size, g, d), table, cu[1:], scale=scale)
+    for i in _some_rows(n) + [400, 700]:
+        ref, rl, _, a, f = _attend(q[i], k, v, scale, _visible(n, 0, 0, "cuda", at=i))
+        _check_tight(out[i], ref, a, f, n, v)
+        _check_lse(lse[i], rl, f)
+        if i == n - 1:
+            _check_tight(one[0], ref, a, f, n, v)
