@@ -88,7 +88,11 @@ typedef struct ChronosPagedAppendArgs {
  * A sequence of length 0 gets zeros and lse = -inf.  With `weights`,
  *     weights_out[b, g, j] = weights[b, g, j] + sum over the group's heads of p_j
  * for every j < len (hidden ones add nothing); slots behind are left as they
- * are; weights_out may be weights. */
+ * are; weights_out may be weights.  The workspace of a call with weights then
+ * holds 4 bytes per query head and slot that a row can see (by table_width and
+ * slot_cap, or window), up to 2^28 bytes or one sequence's: beyond that the call
+ * runs over groups of sequences.  The choice of kernel and grid goes by the same
+ * sizes: a table far wider than the rows costs a second kernel. */
 typedef struct ChronosPagedDecodeArgs {
     ChronosPagedCache cache;
     int32_t heads;             /* H, a multiple of G */

@@ -65,7 +65,14 @@ int slot_limit(const ChronosPagedCache& c, int64_t slot_cap, bool has_cap) {
 // blocks 16.4 us, 18.4 us by the list; 256 rows up to 512 slots 12.4 and 20.5 us.)
 constexpr int kPdClusterBlocks = 6, kPdClusterBlocksFull = 8;
 
+// Bytes of scores that a call with running sums keeps at a time (or one sequence's, where
+// those are more): it runs over groups of sequences.  64 rows under a table of 131072 slots,
+// 32 / 8 heads of 128 in bf16: with 500 slots each 123 us in four groups, 91 us at once with
+// 1.07 GB of scores; with 8000 slots each 468 and 427 us.
+constexpr size_t kPdScoreBytes = size_t{1} << 28;
+
 struct DecodePlan {
+    int group;           // sequences at a time
     bool mma;
     int dp;              // padded head dimension of the tensor-core path
     bool one_page;       // 16 consecutive aligned slots lie in one page
@@ -108,7 +115,7 @@ bool decode_uses_mma(const ChronosPagedDecodeArgs* a) {
 // Blocks per row when a cluster joins them, 0 when the work list is cut evenly instead.
 int decode_cluster(const ChronosPagedDecodeArgs* a, const DecodePlan& d, int64_t blocks) {
     if (!d.mma || a->weights != nullptr) return 0;
-    const int64_t rows = static_cast<int64_t>(a->cache.batch) * a->cache.kv_heads * d.parts;
+    const int64_t rows = static_cast<int64_t>(d.group) * a->cache.kv_heads * d.parts;
     const int64_t room = static_cast<int64_t>(d.per_sm) * sm_count();
     int size = 1;
     while (size < 8 && size < blocks) size *= 2;
@@ -117,7 +124,8 @@ int decode_cluster(const ChronosPagedDecodeArgs* a, const DecodePlan& d, int64_t
     return rows * size <= room && blocks <= most * size ? size : 0;
 }
 
-DecodePlan decode_plan(const ChronosPagedDecodeArgs* a) {
+// The plan of a group of `group` sequences (0: as many as the call takes at a time).
+DecodePlan decode_plan(const ChronosPagedDecodeArgs* a, int group = 0) {
     const ChronosPagedCache& c = a->cache;
     DecodePlan d{};
     d.mma = decode_uses_mma(a);
@@ -130,8 +138,16 @@ DecodePlan decode_plan(const ChronosPagedDecodeArgs* a) {
     // places of a row: both runs of visible slots start at a multiple of 16
     d.max_vis = a->window > 0 ? static_cast<int>(std::min<int64_t>(limit, static_cast<int64_t>(a->window) + a->sinks + 32)) : limit;
     d.one_page = c.page_size % kPdTile == 0;
+    d.score_stride = a->weights != nullptr ? round_up(d.max_vis, kPdBlock) : 0;
+    d.group = group > 0 ? group : c.batch;
+    const size_t scores = static_cast<size_t>(a->heads) * d.score_stride * 4;   // of a sequence
+    if (group == 0 && scores > 0 && scores * c.batch > kPdScoreBytes) {
+        const int most = static_cast<int>(std::max<size_t>(1, kPdScoreBytes / scores));
+        const int groups = (c.batch + most - 1) / most;
+        d.group = (c.batch + groups - 1) / groups;
+    }
     const int64_t blocks = (static_cast<int64_t>(d.max_vis) + kPdBlock - 1) / kPdBlock;
-    const int64_t units = std::max<int64_t>(1, blocks) * c.batch * c.kv_heads * d.parts;
+    const int64_t units = std::max<int64_t>(1, blocks) * d.group * c.kv_heads * d.parts;
     d.grid = static_cast<int>(std::min<int64_t>({units, static_cast<int64_t>(d.per_sm) * sm_count(), kPdMaxGrid}));
     d.cluster = decode_cluster(a, d, blocks);
     d.part_stride = d.mma ? d.dp : static_cast<int>(round_up(c.head_dim, 4));
@@ -145,9 +161,8 @@ DecodePlan decode_plan(const ChronosPagedDecodeArgs* a) {
     d.o_part_o = take(slots * d.part_stride * 4);
     d.o_part_ml = take(slots * 8);
     if (a->weights != nullptr) {
-        d.score_stride = round_up(d.max_vis, kPdBlock);
-        d.o_lse2 = take(static_cast<size_t>(c.batch) * a->heads * 4);
-        d.o_scores = take(static_cast<size_t>(c.batch) * a->heads * d.score_stride * 4);
+        d.o_lse2 = take(static_cast<size_t>(d.group) * a->heads * 4);
+        d.o_scores = take(scores * d.group);
     }
     d.total = d.cluster > 0 ? 0 : std::max<size_t>(at, 256);   // a cluster needs none
     return d;
@@ -200,6 +215,61 @@ int launch_decode(const PagedDecodeParams& p, const DecodePlan& d, bool vec, cud
         CHRONOS_CUDA_CHECK(launch_kernel(paged_join_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(kPdJoinThreads), 0,
                                          st, true, j));
     return CHRONOS_OK;
+}
+
+// The sequences from b0 on that plan `d` is of.
+int decode_group(const ChronosPagedDecodeArgs* a, const DecodePlan& d, int b0, int limit, cudaStream_t st) {
+    const int64_t es = static_cast<int64_t>(elem_bytes(a->cache.dtype));
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    PagedDecodeParams p{};
+    p.c = a->cache;
+    p.c.batch = d.group;
+    p.c.lens += b0;
+    p.c.page_table += b0 * a->cache.page_table_stride;
+    p.heads = a->heads;
+    p.rep = a->heads / a->cache.kv_heads;
+    p.rows = d.rows;
+    p.parts = d.parts;
+    p.window = cut_window(a->window);
+    p.sinks = a->window > 0 ? cut_window(a->sinks) : 0;
+    p.max_slots = limit;
+    p.page_shift = -1;
+    if ((a->cache.page_size & (a->cache.page_size - 1)) == 0)
+        for (p.page_shift = 0; (1 << p.page_shift) < a->cache.page_size;) ++p.page_shift;
+    p.cluster = d.cluster;
+    p.sl2 = static_cast<float>(static_cast<double>(a->scale) * 1.4426950408889634);
+    p.q = static_cast<const uint8_t*>(a->q) + b0 * a->q_row_stride * es;
+    p.q_row = a->q_row_stride;
+    p.q_head = a->q_head_stride;
+    p.out = static_cast<uint8_t*>(a->out) + b0 * a->out_row_stride * es;
+    p.out_row = a->out_row_stride;
+    p.out_head = a->out_head_stride;
+    if (a->lse != nullptr) p.lse = a->lse + static_cast<int64_t>(b0) * a->heads;
+    if (a->weights != nullptr) {
+        const int64_t at = static_cast<int64_t>(b0) * a->cache.kv_heads * a->slot_cap;
+        p.weights = a->weights + at;
+        p.weights_out = a->weights_out + at;
+    }
+    p.slot_cap = a->slot_cap;
+    p.grid = d.grid;
+    p.part_stride = d.part_stride;
+    p.part_o = reinterpret_cast<float*>(ws + d.o_part_o);
+    p.part_ml = reinterpret_cast<float*>(ws + d.o_part_ml);
+    if (a->weights != nullptr) {
+        p.lse2 = reinterpret_cast<float*>(ws + d.o_lse2);
+        p.scores = reinterpret_cast<float*>(ws + d.o_scores);
+        p.score_stride = d.score_stride;
+    }
+    p.status = a->status;
+    const int64_t ve = a->cache.dtype == CHRONOS_DTYPE_FP32 ? 16 : 8;
+    const bool vec = a->cache.head_dim % 4 == 0 && aligned(a->cache.k_pages, ve) && aligned(a->cache.v_pages, ve) &&
+                     multiples(4, {a->cache.k_page_stride, a->cache.k_slot_stride, a->cache.k_head_stride,
+                                   a->cache.v_page_stride, a->cache.v_slot_stride, a->cache.v_head_stride});
+    switch (a->cache.dtype) {
+        case CHRONOS_DTYPE_BF16: return launch_decode<__nv_bfloat16>(p, d, vec, st);
+        case CHRONOS_DTYPE_FP16: return launch_decode<__half>(p, d, vec, st);
+        default: return launch_decode<float>(p, d, vec, st);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -376,51 +446,11 @@ extern "C" int chronos_paged_decode(const ChronosPagedDecodeArgs* a, void* strea
     if (d.total > 0 && (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < d.total))
         return fail(CHRONOS_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes, %zu (256-byte aligned) needed", what,
                     a->workspace == nullptr ? size_t{0} : a->workspace_bytes, d.total);
-    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-    PagedDecodeParams p{};
-    p.c = a->cache;
-    p.heads = a->heads;
-    p.rep = a->heads / a->cache.kv_heads;
-    p.rows = d.rows;
-    p.parts = d.parts;
-    p.window = cut_window(a->window);
-    p.sinks = a->window > 0 ? cut_window(a->sinks) : 0;
-    p.max_slots = limit;
-    p.page_shift = -1;
-    if ((a->cache.page_size & (a->cache.page_size - 1)) == 0)
-        for (p.page_shift = 0; (1 << p.page_shift) < a->cache.page_size;) ++p.page_shift;
-    p.cluster = d.cluster;
-    p.sl2 = static_cast<float>(static_cast<double>(a->scale) * 1.4426950408889634);
-    p.q = a->q;
-    p.q_row = a->q_row_stride;
-    p.q_head = a->q_head_stride;
-    p.out = a->out;
-    p.out_row = a->out_row_stride;
-    p.out_head = a->out_head_stride;
-    p.lse = a->lse;
-    p.weights = a->weights;
-    p.weights_out = a->weights_out;
-    p.slot_cap = a->slot_cap;
-    p.grid = d.grid;
-    p.part_stride = d.part_stride;
-    p.part_o = reinterpret_cast<float*>(ws + d.o_part_o);
-    p.part_ml = reinterpret_cast<float*>(ws + d.o_part_ml);
-    if (a->weights != nullptr) {
-        p.lse2 = reinterpret_cast<float*>(ws + d.o_lse2);
-        p.scores = reinterpret_cast<float*>(ws + d.o_scores);
-        p.score_stride = d.score_stride;
+    for (int b0 = 0; b0 < a->cache.batch; b0 += d.group) {
+        const int n = std::min(d.group, a->cache.batch - b0);
+        if (int rc = decode_group(a, n == d.group ? d : decode_plan(a, n), b0, limit, static_cast<cudaStream_t>(stream))) return rc;
     }
-    p.status = a->status;
-    const int64_t ve = a->cache.dtype == CHRONOS_DTYPE_FP32 ? 16 : 8;
-    const bool vec = a->cache.head_dim % 4 == 0 && aligned(a->cache.k_pages, ve) && aligned(a->cache.v_pages, ve) &&
-                     multiples(4, {a->cache.k_page_stride, a->cache.k_slot_stride, a->cache.k_head_stride,
-                                   a->cache.v_page_stride, a->cache.v_slot_stride, a->cache.v_head_stride});
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    switch (a->cache.dtype) {
-        case CHRONOS_DTYPE_BF16: return launch_decode<__nv_bfloat16>(p, d, vec, st);
-        case CHRONOS_DTYPE_FP16: return launch_decode<__half>(p, d, vec, st);
-        default: return launch_decode<float>(p, d, vec, st);
-    }
+    return CHRONOS_OK;
 }
 
 extern "C" int chronos_paged_append(const ChronosPagedAppendArgs* a, void* stream) {

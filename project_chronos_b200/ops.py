@@ -689,7 +689,8 @@ def paged_attn_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     sequence of length 0); ``lse`` fp32 [B, heads] receives the log of each softmax
     sum.  ``weights`` fp32 [B, kv heads, slots]: weights_out (default: in place)
     receives weights plus every slot's attention weight summed over the group's
-    heads; slots at or behind lens are left as they are."""
+    heads; slots at or behind lens are left as they are.  It takes a workspace of 4 bytes
+    per head and slot of the table, 256 MB (or one sequence's) at most."""
     if not k_pages.is_cuda:
         _no_cpu(k_pages)
     dev, index, grad = k_pages.device, k_pages.get_device(), torch.is_grad_enabled()

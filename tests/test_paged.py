@@ -1378,3 +1378,61 @@ def test_fp16_scores_that_climb(step):
         _check_lse(lse[i], rl, f)
         if i == n - 1:
             _check_tight(one[0], ref, a, f, n, v)
+
+
+# ---------------------------------------------------------------------------------------
+# running sums under a table far wider than the rows
+# ---------------------------------------------------------------------------------------
+
+def test_score_workspace_is_bounded(lib):
+    """Running sums keep scores of a bounded number of sequences at a time, however wide the table is."""
+    from project_chronos_b200 import _native as N
+    for batch, width in ((64, 2048), (4096, 512), (256, 1 << 14)):
+        c = N.ChronosPagedCache(batch=batch, kv_heads=8, head_dim=128, dtype=N.DTYPE_BF16, num_pages=99, page_size=64,
+                                table_width=width)
+        a = N.ChronosPagedDecodeArgs(cache=c, heads=32, scale=1.0, weights=256, weights_out=256, slot_cap=64 * width)
+        n = lib.chronos_paged_decode_workspace(ctypes.byref(a))
+        one = 32 * 64 * width * 4                     # a sequence's
+        assert 0 < n <= max(1 << 28, one) + (1 << 24)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_summed_weights_under_a_wide_table(dt):
+    """Rows far shorter than their table: the call runs over groups of sequences."""
+    from project_chronos_b200 import _native as N
+    from project_chronos_b200 import ops
+    b, h, g, d, size, width = 150, 16, 2, 64, 16, 2048
+    gen = torch.Generator().manual_seed(1)
+    lens = torch.randint(0, 400, (b,), generator=gen).tolist()
+    kp, vp, _, ln, rows = _make_cache(lens, g, d, size, dt, seed=11)
+    narrow = _make_cache(lens, g, d, size, dt, seed=11)[2]
+    table = torch.full((b, 2 * width), -1, dtype=torch.int32, device="cuda")[:, :width]
+    table[:, : narrow.shape[1]] = narrow
+    q = (2 * torch.randn(b, h + 1, d, generator=_gen(9), device="cuda")).to(dt)[:, :h]
+    w0 = torch.rand(b, g, width * size, generator=_gen(10), device="cuda")
+    for window, sinks in ((0, 0), (90, 3)):
+        w = w0.clone()
+        lse = torch.empty(b, h, device="cuda")
+        wide = torch.full((b, h + 1, d), 9.0, dtype=dt, device="cuda")
+        ops.paged_attn_decode(q, kp, vp, table, ln, window=window, sinks=sinks, weights=w, lse=lse, out=wide[:, :h])
+        ops.check_status(kp.device)
+        assert bool((wide[:, h] == 9.0).all())
+        again = w0.clone()
+        assert torch.equal(wide[:, :h], ops.paged_attn_decode(q, kp, vp, table, ln, window=window, sinks=sinks, weights=again))
+        assert torch.equal(w, again)
+        for i in range(b):
+            k, v = rows[i]
+            n = lens[i]
+            ref, rl, p, a, f = _attend(q[i], k, v, d ** -0.5, _visible(n, window, sinks, "cuda"))
+            _check_out(wide[i, :h], ref, a, f, n, dt)
+            _check_lse(lse[i], rl, f)
+            add = p.view(g, h // g, n).sum(1)
+            want = w0[i, :, :n].double() + add
+            tol = f.view(g, h // g).amax(1)[:, None] * add + (h // g + 1) * 2.0 ** -24 * want
+            assert bool(((w[i, :, :n].double() - want).abs() <= tol).all())
+            assert torch.equal(w[i, :, n:], w0[i, :, n:])
+    ln[b - 1] = width * size + 5
+    ops.paged_attn_decode(q, kp, vp, table, ln, weights=w0)
+    with pytest.raises(N.ChronosMoeError, match="INVALID_ARG"):
+        ops.check_status(kp.device)
