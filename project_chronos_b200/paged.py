@@ -17,8 +17,9 @@ rotated, which makes attention independent of the order of the slots and lets
 
 The kernels behind it are ``ops.paged_append``, ``ops.paged_attn_decode`` and
 ``ops.paged_evict`` (include/chronos_paged.h).  append, attend and evict run on
-the current stream, read lengths on the device and copy nothing to the host;
-attend can be captured in a CUDA graph and replayed while the rows grow.
+the current stream, read lengths on the device and copy nothing to the host (but
+for a window asked for after an eviction, see attend); attend can be captured in
+a CUDA graph and replayed while the rows grow.
 """
 from __future__ import annotations
 
@@ -56,7 +57,8 @@ class PagedCache:
             slots = (batch, kv_heads, table_width * page_size)
             self.weights = torch.zeros(slots, dtype=torch.float32, device=device)
             self.positions = torch.zeros(slots, dtype=torch.int32, device=device)
-        self._evicted = False    # slots and positions are no longer the same
+        self._evicted = False    # since the rows were last seen uncut
+        self._replays = False    # an eviction was captured: a graph may run it at any time
         self._free: List[int] = list(range(num_pages - 1, -1, -1))
         self._pages: List[List[int]] = [[] for _ in range(batch)]
 
@@ -114,17 +116,30 @@ class PagedCache:
                out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of each row's newest token (already appended) over its slots, q
         [B, heads, D] -> [B, heads, D]; adds to ``weights`` where they are tracked.
-        A window counts slots: it is refused once the cache was evicted from."""
-        if window and self._evicted:
-            raise RuntimeError("a window counts slots, which an eviction has reordered: attend without one")
+        A window counts slots: it is refused while a row lives that an eviction has cut
+        (after an eviction a call with a window reads that from the device, once if no row
+        was cut; a graph that was captured with a window must not be replayed then)."""
+        if window and (self._evicted or self._replays):
+            self._refuse_cut_rows()
         return ops.paged_attn_decode(q, self.k_pages, self.v_pages, self.page_table, self.lens, scale=scale,
                                      window=window, sinks=sinks, weights=self.weights, out=out, lse=lse)
+
+    def _refuse_cut_rows(self) -> None:
+        if self.lens.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a window cannot be captured after an eviction: it counts slots, which may be reordered")
+        lens, seen = torch.stack([self.lens, self.seen]).tolist()
+        cut = [row for row in range(self.batch) if lens[row] != seen[row]]
+        if cut:
+            raise RuntimeError(f"a window counts slots, which an eviction has reordered in rows {cut}: attend without one")
+        self._evicted = False
 
     def evict(self, budget: int, sinks: int = 0, recent: int = 0) -> torch.Tensor:
         """Cut every row and kv head down to ``budget`` slots (``ops.paged_evict``), in
         place.  Returns src int32 [B, kv_heads, budget]: where each slot came from."""
         if self.weights is None:
             raise RuntimeError("evict needs a cache with track_weights=True")
+        src = ops.paged_evict(self.k_pages, self.v_pages, self.page_table, self.lens, self.seen, self.weights,
+                              self.positions, budget, sinks=sinks, recent=recent, lens_out=self.lens)["src"]
         self._evicted = True
-        return ops.paged_evict(self.k_pages, self.v_pages, self.page_table, self.lens, self.seen, self.weights,
-                               self.positions, budget, sinks=sinks, recent=recent, lens_out=self.lens)["src"]
+        self._replays = self._replays or torch.cuda.is_current_stream_capturing()
+        return src

@@ -1436,3 +1436,80 @@ def test_summed_weights_under_a_wide_table(dt):
     ops.paged_attn_decode(q, kp, vp, table, ln, weights=w0)
     with pytest.raises(N.ChronosMoeError, match="INVALID_ARG"):
         ops.check_status(kp.device)
+
+
+# ---------------------------------------------------------------------------------------
+# windows and evictions
+# ---------------------------------------------------------------------------------------
+
+def test_a_refused_eviction_leaves_the_window():
+    from project_chronos_b200 import PagedCache
+    c = PagedCache(1, 4, 1, 8, 4, "cpu", torch.float32, page_size=4, track_weights=True)
+    c.reserve(0, 9)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        c.evict(4)
+    with pytest.raises(RuntimeError, match="CUDA"):   # not "a window counts slots"
+        c.attend(torch.zeros(1, 1, 8), window=3)
+
+
+@gpu
+def test_windows_come_back_after_evictions():
+    """A window is refused while a row that an eviction cut lives, and only then."""
+    from project_chronos_b200 import PagedCache, ops
+    h, g, d, dt, window, sinks = 8, 2, 64, BF, 20, 2
+    gen = _gen(6)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device="cuda").to(dt)  # noqa: E731
+    c = PagedCache(2, 20, g, d, 8, "cuda", dt, page_size=16, track_weights=True)
+    lens = [50, 9]
+
+    def fill():
+        k, v = rnd(sum(lens), g, d), rnd(sum(lens), g, d)
+        c.append(k, v, torch.tensor([0, lens[0], sum(lens)], dtype=torch.int32, device="cuda"))
+        return [(k[: lens[0]], v[: lens[0]]), (k[lens[0]:], v[lens[0]:])]
+
+    def look(rows):
+        q = rnd(2, h, d)
+        out = c.attend(q, window=window, sinks=sinks)
+        for b, (k, v) in enumerate(rows):
+            ref, _, _, a, f = _attend(q[b], k, v, d ** -0.5, _visible(lens[b], window, sinks, "cuda"))
+            _check_out(out[b], ref, a, f, lens[b], dt)
+
+    for b in range(2):
+        c.reserve(b, 100)
+    rows = fill()
+    look(rows)
+    with pytest.raises(RuntimeError, match="budget"):
+        c.evict(4, sinks=3, recent=2)                 # refused
+    look(rows)
+    c.evict(60, sinks=2, recent=5)                    # every row is within it
+    look(rows)
+    c.evict(30, sinks=2, recent=5)                    # cuts row 0
+    with pytest.raises(RuntimeError, match="window"):
+        c.attend(rnd(2, h, d), window=window)
+    c.attend(rnd(2, h, d))
+    c.release(1)                                      # was not cut
+    with pytest.raises(RuntimeError, match="window"):
+        c.attend(rnd(2, h, d), window=window)
+    c.release(0)
+    for b in range(2):
+        c.reserve(b, 100)
+    rows = fill()
+    look(rows)
+    # a captured eviction may be replayed at any time
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.evict(30, sinks=2, recent=5)
+    look(rows)
+    graph.replay()
+    with pytest.raises(RuntimeError, match="window"):
+        c.attend(rnd(2, h, d), window=window)
+    for b in range(2):
+        c.release(b)
+        c.reserve(b, 100)
+    rows = fill()
+    look(rows)
+    graph.replay()
+    with pytest.raises(RuntimeError, match="window"):
+        c.attend(rnd(2, h, d), window=window)
+    ops.check_status(c.lens.device)
