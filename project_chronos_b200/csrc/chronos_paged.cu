@@ -535,7 +535,6 @@ extern "C" int chronos_paged_evict(const ChronosPagedEvictArgs* a, void* stream)
         a->positions_out == nullptr || a->lens_out == nullptr || a->src == nullptr)
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: seen, weights, positions, their outputs, lens_out and src are required", what);
     const int rows = a->cache.batch * a->cache.kv_heads;
-    if (rows > 65535) return fail(CHRONOS_ERR_INVALID_ARG, "%s: batch * kv_heads %d above 65535", what, rows);
     const EvictPlan e = evict_plan(a);
     if (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < e.total)
         return fail(CHRONOS_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes, %zu (256-byte aligned) needed", what,
@@ -579,7 +578,8 @@ extern "C" int chronos_paged_evict(const ChronosPagedEvictArgs* a, void* stream)
     CHRONOS_CUDA_CHECK(launch_kernel(paged_evict_select_kernel, dim3(rows), dim3(kEvictThreads), smem, st, false, p, units, per));
     if (p.move_here) return CHRONOS_OK;
     const int64_t bx = std::max<int64_t>(1, std::min<int64_t>((e.max_moves + kEvictMovesPerBlock - 1) / kEvictMovesPerBlock, 4096));
-    const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(rows)), block(kEvictMoveThreads);
+    const unsigned by = std::min(rows, 32768), bz = (rows + by - 1) / by;   // rows, up to 2^20
+    const dim3 grid(static_cast<unsigned>(bx), by, bz), block(kEvictMoveThreads);
     if (wide) CHRONOS_CUDA_CHECK(launch_kernel(paged_evict_move_kernel<uint4>, grid, block, 0, st, true, p, units, per));
     else if (es == 2) CHRONOS_CUDA_CHECK(launch_kernel(paged_evict_move_kernel<uint16_t>, grid, block, 0, st, true, p, units, per));
     else CHRONOS_CUDA_CHECK(launch_kernel(paged_evict_move_kernel<uint32_t>, grid, block, 0, st, true, p, units, per));

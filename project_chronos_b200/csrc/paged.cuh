@@ -1596,7 +1596,8 @@ constexpr int kEvictMovesPerBlock = kEvictMoveThreads / 32 * 4;
 template <typename V>
 __global__ void __launch_bounds__(kEvictMoveThreads) paged_evict_move_kernel(const __grid_constant__ PagedEvictParams p,
                                                                              int units, int elems_per_unit) {
-    const int row = blockIdx.y, b = row / p.c.kv_heads, g = row % p.c.kv_heads;
+    const int row = blockIdx.z * gridDim.y + blockIdx.y, b = row / p.c.kv_heads, g = row % p.c.kv_heads;
+    if (b >= p.c.batch) return;
     pdl_wait();
     if (g == 0 && blockIdx.x == 0 && threadIdx.x == 0) p.lens_out[b] = min(p.lens_copy[b], p.budget);
     paged_move_rows<V>(p, b, g, p.moves + static_cast<int64_t>(row) * p.max_moves * 2, p.counts[row],

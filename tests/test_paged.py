@@ -1513,3 +1513,35 @@ def test_windows_come_back_after_evictions():
     with pytest.raises(RuntimeError, match="window"):
         c.attend(rnd(2, h, d), window=window)
     ops.check_status(c.lens.device)
+
+
+# ---------------------------------------------------------------------------------------
+# evictions: many rows, lengths written over what the call reads
+# ---------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("d, budget", [(8, 3), (8, 200), (5, 3)])
+def test_evict_of_very_many_rows(d, budget):
+    from project_chronos_b200 import ops
+    b, g, n = 70000, 1, 4
+    size = 4
+    kp = torch.randn(b, size, g, d, generator=_gen(1), device="cuda").to(BF)
+    vp = torch.randn(b, size, g, d, generator=_gen(2), device="cuda").to(BF)
+    table = torch.randperm(b, generator=_gen(3), device="cuda").to(torch.int32).view(b, 1)
+    w = torch.rand(b, g, size, generator=_gen(4), device="cuda")
+    pos = torch.arange(size, dtype=torch.int32, device="cuda").expand(b, g, size).contiguous()
+    ln = torch.full((b,), n, dtype=torch.int32, device="cuda")
+    k0, v0 = kp[table[:, 0].long()].clone(), vp[table[:, 0].long()].clone()
+    r = ops.paged_evict(kp, vp, table, ln, ln, w.clone(), pos, budget)
+    ops.check_status(kp.device)
+    m = min(n, budget)
+    assert bool((r["lens"] == m).all()) and r["src"].shape == (b, g, budget)
+    src = torch.arange(m, device="cuda").expand(b, m).clone()
+    if budget < n:                                    # the smallest goes, the last slot fills its place
+        low = w[:, 0].argmin(dim=1)
+        gone = low < m
+        src[gone, low[gone]] = n - 1
+    assert torch.equal(r["src"][:, 0, :m].long(), src)
+    at = src[:, :, None].expand(b, m, d)
+    assert torch.equal(kp[table[:, 0].long()][:, :m, 0], k0[:, :, 0].gather(1, at))
+    assert torch.equal(vp[table[:, 0].long()][:, :m, 0], v0[:, :, 0].gather(1, at))
