@@ -133,7 +133,7 @@ typedef struct ChronosPagedEvictArgs {
     float* weights_out;
     int32_t* positions_out;
     int64_t slot_cap;
-    int32_t* lens_out;         /* [B]; may be cache.lens */
+    int32_t* lens_out;         /* [B]; may be cache.lens or seen */
     int32_t* src;              /* [B, G, budget] */
     void* workspace;           /* chronos_paged_evict_workspace bytes, 256-byte aligned */
     size_t workspace_bytes;

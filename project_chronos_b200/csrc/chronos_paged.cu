@@ -571,10 +571,10 @@ extern "C" int chronos_paged_evict(const ChronosPagedEvictArgs* a, void* stream)
     const int per = wide ? 16 / es : 1;
     const int units = a->cache.head_dim / per;
     // Few moves per row (a cache that gives up a page's slots at a time): the selecting block
-    // makes them, without the second kernel.  Not where lens_out is lens, which the other kv
-    // heads' blocks still read.
-    p.move_here = wide && e.max_moves <= kEvictMovesHere &&
-                  (a->lens_out + a->cache.batch <= a->cache.lens || a->cache.lens + a->cache.batch <= a->lens_out);
+    // makes them, without the second kernel.  Not where lens_out lies over lens or seen, which
+    // the other kv heads' blocks still read.
+    p.move_here = wide && e.max_moves <= kEvictMovesHere && !cross(a->lens_out, a->cache.lens, a->cache.batch, false) &&
+                  !cross(a->lens_out, a->seen, a->cache.batch, false);
     CHRONOS_CUDA_CHECK(launch_kernel(paged_evict_select_kernel, dim3(rows), dim3(kEvictThreads), smem, st, false, p, units, per));
     if (p.move_here) return CHRONOS_OK;
     const int64_t bx = std::max<int64_t>(1, std::min<int64_t>((e.max_moves + kEvictMovesPerBlock - 1) / kEvictMovesPerBlock, 4096));

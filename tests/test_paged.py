@@ -1545,3 +1545,21 @@ def test_evict_of_very_many_rows(d, budget):
     at = src[:, :, None].expand(b, m, d)
     assert torch.equal(kp[table[:, 0].long()][:, :m, 0], k0[:, :, 0].gather(1, at))
     assert torch.equal(vp[table[:, 0].long()][:, :m, 0], v0[:, :, 0].gather(1, at))
+
+
+@gpu
+@pytest.mark.parametrize("lens_is", ["seen", "lens"])
+def test_evict_writes_lengths_over_its_inputs(lens_is):
+    """One slot too many in rows of many kv heads: the new lengths may take the place of what the call reads."""
+    from project_chronos_b200 import ops
+    lens, g, d, budget = [65] * 30 + [40, 64], 16, 16, 64
+    kp, vp, table, ln, _ = _make_cache(lens, g, d, 16, BF, seed=1, bad=0.0)
+    cap = table.shape[1] * 16
+    w = torch.rand(len(lens), g, cap, generator=_gen(2), device="cuda")
+    pos = torch.arange(cap, dtype=torch.int32, device="cuda").expand(len(lens), g, cap).contiguous()
+    seen = ln.clone()
+    ref = ops.paged_evict(kp.clone(), vp.clone(), table, ln, seen, w.clone(), pos.clone(), budget, sinks=2, recent=9)
+    k, v = kp.clone(), vp.clone()
+    r = ops.paged_evict(k, v, table, ln, seen, w, pos, budget, sinks=2, recent=9, lens_out=seen if lens_is == "seen" else ln)
+    for key in ("lens", "src", "weights", "positions"):
+        assert torch.equal(r[key], ref[key])
