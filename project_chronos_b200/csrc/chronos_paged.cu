@@ -359,8 +359,12 @@ bool encode_rows(CUtensorMap* m, int dtype, const void* base, int rank, const ui
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// What the loads and the 16-byte stores of the tensor-core path need.
+// What the loads and the 16-byte stores of the tensor-core path need.  A tensor map steps by
+// at least one element: rows or heads read several times (a stride of zero) have no map.
 bool window_uses_tc(const WindowParams& p) {
+    if ((p.num_q > 1 && p.q_row == 0) || (p.heads > 1 && p.q_head == 0) || (p.num_k > 1 && (p.k_row == 0 || p.v_row == 0)) ||
+        (p.kv_heads > 1 && (p.k_head == 0 || p.v_head == 0)))
+        return false;
     return p.dim % 8 == 0 && p.dim <= 128 && p.num_k > 0 && aligned(p.q, 16) && aligned(p.k, 16) && aligned(p.v, 16) &&
            aligned(p.out, 16) &&
            multiples(8, {p.q_row, p.q_head, p.k_row, p.k_head, p.v_row, p.v_head, p.o_row, p.o_head});
@@ -407,9 +411,14 @@ int launch_window_tc(const WindowParams& p, int dtype, bool* taken, cudaStream_t
 }
 
 template <typename T>
-int window_impl(const WindowParams& p, int dtype, cudaStream_t st) {
+int window_impl(WindowParams p, int dtype, cudaStream_t st) {
     if constexpr (sizeof(T) == 2) {
         if (window_uses_tc(p)) {
+            // no step is ever taken in a dimension of one: any stride will do
+            if (p.num_q == 1) p.q_row = p.dim;
+            if (p.heads == 1) p.q_head = p.dim;
+            if (p.num_k == 1) p.k_row = p.v_row = p.dim;
+            if (p.kv_heads == 1) p.k_head = p.v_head = p.dim;
             bool taken = false;
             const int rc = p.dim <= 64 ? launch_window_tc<T, 64>(p, dtype, &taken, st) : launch_window_tc<T, 128>(p, dtype, &taken, st);
             if (rc || taken) return rc;
@@ -634,6 +643,10 @@ extern "C" int chronos_window_attention(const ChronosWindowAttnArgs* a, void* st
     p.cu_k = a->cu_k;
     p.lse = a->lse;
     p.status = a->status;
+    if (p.k_head == 0 && p.v_head == 0) {   // one kv head read as several
+        p.kv_heads = 1;
+        p.rep = p.heads;
+    }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (a->dtype) {
         case CHRONOS_DTYPE_BF16: return window_impl<__nv_bfloat16>(p, a->dtype, st);

@@ -1563,3 +1563,24 @@ def test_evict_writes_lengths_over_its_inputs(lens_is):
     r = ops.paged_evict(k, v, table, ln, seen, w, pos, budget, sinks=2, recent=9, lens_out=seen if lens_is == "seen" else ln)
     for key in ("lens", "src", "weights", "positions"):
         assert torch.equal(r[key], ref[key])
+
+
+# ---------------------------------------------------------------------------------------
+# prompts: expanded heads, results over the queries, offsets
+# ---------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("which", ["q", "k", "v", "k and v", "all"])
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_prompt_attention_takes_expanded_heads(which, dt):
+    """One row of heads read as several: strides of zero."""
+    from project_chronos_b200 import ops
+    n, h, g, d = 300, 8, 4, 64
+    gen = _gen(4)
+    make = lambda heads, name: torch.randn(n, 1 if name in which or which == "all" else heads, d, generator=gen,  # noqa: E731
+                                           device="cuda").to(dt).expand(n, heads, d)
+    q, k, v = make(h, "q"), make(g, "k"), make(g, "v")
+    cu = torch.tensor([0, 100, n], dtype=torch.int32, device="cuda")
+    out = ops.window_attention(q, k, v, cu, window=90, sinks=2)
+    for c0, m in ((0, 100), (100, 200)):
+        _check_prompt(out, None, q, k, v, m, m, c0, c0, 90, 2, dt, _some_rows(m))
