@@ -778,8 +778,6 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
                 __syncwarp();
                 if (lane == 0) mbar_arrive(v_ok + st);
             }
-            __syncwarp();
-            asm volatile("bar.arrive 2, 320;" ::: "memory");
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
@@ -873,7 +871,14 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         }
         if (m == INFINITY) l = NAN;   // inf - inf
-        if (nt > 0 && ok) ok = __all_sync(0xffffffffu, wait(o_done + w, 0));
+        // every V tile has been looked through when the last one has; a row is either stored here or
+        // computed again from q, which out may be (seen while the last product runs)
+        bool again = false;
+        if (!SPLIT && nt > 0 && ok) {
+            ok = wait(v_ok + (nt - 1) % NS, ((nt - 1) / NS) & 1);
+            again = *not_finite != 0;
+        }
+        if (nt > 0) ok = __all_sync(0xffffffffu, ok && wait(o_done + w, 0));
         tc_fence_after();
         if constexpr (SPLIT) {
             // unnormalised, in fp32, 16-byte chunks swizzled by row; the products with Q and K are complete
@@ -893,7 +898,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
             s_ml[(w * 128 + r) * 2] = m == -INFINITY ? m : m * p.sl2 - kLift;
             s_ml[(w * 128 + r) * 2 + 1] = l;
         }
-        const bool mine = !SPLIT && ok && local < rows;
+        const bool mine = !SPLIT && ok && !again && local < rows;
         const int64_t qrow = t.q0 + t.m0 + local;
         const float inv = l > 0.0f ? 1.0f / l : l;
         T* out = static_cast<T*>(p.out) + qrow * p.o_row + head * p.o_head;
@@ -922,8 +927,7 @@ __global__ void __launch_bounds__(kWtThreads, 1) window_tc_kernel(const __grid_c
         }
         if (mine && p.lse != nullptr)
             p.lse[qrow * p.heads + head] = l != 0.0f ? ((m == -INFINITY ? 0.0f : m * p.sl2 - kLift) + log2f(l)) * kLn2 : -INFINITY;
-        asm volatile("bar.sync 2, 320;" ::: "memory");
-        if (!SPLIT && *not_finite && ok)
+        if (again && ok)
             for (int x = warp; x < 256; x += 8) {
                 const int tok = x >> rp_log2;
                 if (tok < rows) window_row_exact<T>(p, t, t.m0 + tok, (hg << rp_log2) + (x & ((1 << rp_log2) - 1)), lane);

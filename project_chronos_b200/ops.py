@@ -784,7 +784,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     position t = lk - lq + i and sees the keys j <= t, under a ``window`` > 0 only
     j > t - window and the first ``sinks``.  ``scale`` defaults to D ** -0.5.  Returns
     out [Tq, heads, D]: zeros for a row that sees nothing, rows behind the last
-    sequence as they were (``out``) or undefined; ``lse`` fp32 [Tq, heads]."""
+    sequence as they were (``out``, which may be ``q``) or undefined; ``lse`` fp32
+    [Tq, heads]."""
     if not q.is_cuda:
         _no_cpu(q)
     dev, index, grad = q.device, q.get_device(), torch.is_grad_enabled()

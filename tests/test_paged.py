@@ -1584,3 +1584,21 @@ def test_prompt_attention_takes_expanded_heads(which, dt):
     out = ops.window_attention(q, k, v, cu, window=90, sinks=2)
     for c0, m in ((0, 100), (100, 200)):
         _check_prompt(out, None, q, k, v, m, m, c0, c0, 90, 2, dt, _some_rows(m))
+
+
+@gpu
+@pytest.mark.parametrize("lq, lk", [(300, 300), (40, 4000)])
+@pytest.mark.parametrize("bad", [False, True])
+def test_prompt_attention_over_its_queries(lq, lk, bad):
+    """out may be q, also where a value that is not finite sends rows through a second computation."""
+    from project_chronos_b200 import ops
+    h, g, d, window = 8, 2, 128, 200
+    gen = _gen(1)
+    q, k, v = (torch.randn(r, x, d, generator=gen, device="cuda").to(BF) for r, x in ((lq, h), (lk, g), (lk, g)))
+    if bad:
+        v[lk - 20, :, 3] = math.inf
+    cq, ck = (torch.tensor([0, x], dtype=torch.int32, device="cuda") for x in (lq, lk))
+    want = ops.window_attention(q, k, v, cq, cu_seqlens_k=ck, window=window)
+    got = q.clone()
+    ops.window_attention(got, k, v, cq, cu_seqlens_k=ck, window=window, out=got)
+    assert torch.equal(got.view(torch.int16), want.view(torch.int16))
