@@ -144,7 +144,10 @@ typedef struct ChronosPagedEvictArgs {
  * [cu_k[b], cu_k[b+1]); its i-th query stands at position t = lk - lq + i and sees
  *     key j <= t with (window == 0 or j > t - window or j < sinks).
  * A row that sees nothing (t < 0) gets zeros and lse = -inf.  Query rows behind
- * the last sequence are left as they are, key rows behind it are not used. */
+ * the last sequence are left as they are, key rows behind it are not used.
+ * Offsets that do not ascend or leave the rows are reported as
+ * CHRONOS_ERR_INVALID_ARG in the status word; what the results are is not said then.
+ * out may be q. */
 typedef struct ChronosWindowAttnArgs {
     int32_t batch;
     int32_t heads;             /* H, a multiple of kv_heads */

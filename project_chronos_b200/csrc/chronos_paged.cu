@@ -335,7 +335,7 @@ int launch_window_simt(const WindowParams& p, cudaStream_t st) {
     void (*kernel)(WindowParams) = vec ? window_simt_pick<T, true>(p.dim) : window_simt_pick<T, false>(p.dim);
     const int smem = window_simt_smem(p.dim);
     if (int rc = set_smem(kernel, smem)) return rc;
-    const int64_t tiles = (p.num_q + kWsRows - 1) / kWsRows + p.batch;
+    const int64_t tiles = (p.num_q + kWsRows - 1) / kWsRows + p.batch;   // one more than there are, at least
     CHRONOS_CUDA_CHECK(launch_kernel(kernel, dim3(static_cast<unsigned>(tiles * p.heads)), dim3(kWsThreads), smem, st, false, p));
     return CHRONOS_OK;
 }
@@ -396,16 +396,16 @@ int launch_window_tc(const WindowParams& p, int dtype, bool* taken, cudaStream_t
     // on 8064 keys 119 us, split over 8 blocks 36).
     const int64_t mean = p.num_k / p.batch;
     const int64_t keys = p.window > 0 ? std::min<int64_t>(mean, static_cast<int64_t>(p.window) + p.sinks + tokens) : mean;
-    int splits = 1;
+    int splits = 1;   // (and one tile's blocks that check the offsets)
     while (splits < 8 && blocks * splits * 2 <= sm_count() && keys >= std::max(8, 4 * splits) * kWtKeys) splits *= 2;
     if (splits == 1) {
         if (int rc = set_smem(window_tc_kernel<T, DP, false>, C::kSmem)) return rc;
-        CHRONOS_CUDA_CHECK(launch_kernel(window_tc_kernel<T, DP, false>, dim3(static_cast<unsigned>(blocks)), dim3(kWtThreads),
+        CHRONOS_CUDA_CHECK(launch_kernel(window_tc_kernel<T, DP, false>, dim3(static_cast<unsigned>(blocks + 1)), dim3(kWtThreads),
                                          C::kSmem, st, false, p, mq, mk, mv, rp_log2, groups, 1));
         return CHRONOS_OK;
     }
     if (int rc = set_smem(window_tc_kernel<T, DP, true>, C::kSplitSmem)) return rc;
-    CHRONOS_CUDA_CHECK(launch_cluster(window_tc_kernel<T, DP, true>, dim3(static_cast<unsigned>(blocks * splits)), dim3(kWtThreads),
+    CHRONOS_CUDA_CHECK(launch_cluster(window_tc_kernel<T, DP, true>, dim3(static_cast<unsigned>((blocks + 1) * splits)), dim3(kWtThreads),
                                       C::kSplitSmem, st, splits, p, mq, mk, mv, rp_log2, groups, splits));
     return CHRONOS_OK;
 }

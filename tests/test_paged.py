@@ -1602,3 +1602,16 @@ def test_prompt_attention_over_its_queries(lq, lk, bad):
     got = q.clone()
     ops.window_attention(got, k, v, cq, cu_seqlens_k=ck, window=window, out=got)
     assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_offsets_that_do_not_ascend_are_reported(dt):
+    from project_chronos_b200 import _native as N
+    from project_chronos_b200 import ops
+    q, k = torch.zeros(9, 4, 64, dtype=dt, device="cuda"), torch.zeros(9, 2, 64, dtype=dt, device="cuda")
+    for cu in ([0, 9, 3], [0, 4, 4, 9, 2], list(range(9)) + [9] * 60 + [5], [9, 3], [3, 2, 1, 0]):
+        cu = torch.tensor(cu, dtype=torch.int32, device="cuda")
+        ops.window_attention(q, k, k, cu)
+        with pytest.raises(N.ChronosMoeError, match="INVALID_ARG"):
+            ops.check_status(q.device)
