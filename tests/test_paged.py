@@ -1615,3 +1615,17 @@ def test_offsets_that_do_not_ascend_are_reported(dt):
         ops.window_attention(q, k, k, cu)
         with pytest.raises(N.ChronosMoeError, match="INVALID_ARG"):
             ops.check_status(q.device)
+
+
+@gpu
+def test_sums_that_require_grad_are_refused():
+    from project_chronos_b200 import ops
+    kp, vp, table, ln, _ = _make_cache([5, 6], 2, 64, 16, BF, seed=1)
+    q = torch.zeros(2, 4, 64, dtype=BF, device="cuda")
+    w = torch.zeros(2, 2, 32, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="forward-only"):
+        ops.paged_attn_decode(q, kp, vp, table, ln, weights=w)
+    with pytest.raises(RuntimeError, match="forward-only"):
+        ops.paged_attn_decode(q, kp, vp, table, ln, lse=torch.zeros(2, 4, device="cuda", requires_grad=True))
+    with torch.no_grad():
+        ops.paged_attn_decode(q, kp, vp, table, ln, weights=w)
