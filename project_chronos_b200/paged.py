@@ -69,11 +69,16 @@ class PagedCache:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def _pages_of(self, slots: int) -> int:
+        if slots < 0:
+            raise ValueError(f"slots must not be negative, got {slots}")
+        return -(-int(slots) // self.page_size)
+
     def reserve(self, row: int, slots: int) -> None:
         """Give ``row`` the pages it lacks for ``slots`` slots (host bookkeeping and one
         copy of its table row)."""
         have = self._pages[row]
-        need = -(-int(slots) // self.page_size)
+        need = self._pages_of(slots)
         if need > self.table_width:
             raise RuntimeError(f"{slots} slots need {need} pages, a row has at most {self.table_width}")
         if need - len(have) > len(self._free):
@@ -85,7 +90,7 @@ class PagedCache:
     def trim(self, row: int, slots: int) -> None:
         """Give back the pages of ``row`` behind its first ``slots`` slots (after an
         eviction to at most that many: the caller knows the budget)."""
-        keep = -(-int(slots) // self.page_size)
+        keep = self._pages_of(slots)
         gone = self._pages[row][keep:]
         if gone:
             del self._pages[row][keep:]

@@ -1629,3 +1629,13 @@ def test_sums_that_require_grad_are_refused():
         ops.paged_attn_decode(q, kp, vp, table, ln, lse=torch.zeros(2, 4, device="cuda", requires_grad=True))
     with torch.no_grad():
         ops.paged_attn_decode(q, kp, vp, table, ln, weights=w)
+
+
+def test_trim_refuses_negative_slots():
+    from project_chronos_b200 import PagedCache
+    c = PagedCache(1, 5, 1, 8, 4, "cpu", torch.float32, page_size=4)
+    c.reserve(0, 12)
+    for call in (c.trim, c.reserve):
+        with pytest.raises(ValueError, match="negative"):
+            call(0, -5)
+    assert c.page_table.tolist() == [[0, 1, 2, -1]] and c.free_pages() == 2
