@@ -89,13 +89,15 @@ class PagedCache:
 
     def trim(self, row: int, slots: int) -> None:
         """Give back the pages of ``row`` behind its first ``slots`` slots (after an
-        eviction to at most that many: the caller knows the budget)."""
+        eviction to at most that many: the caller knows the budget).  What lies in them
+        is lost: a longer row is cut to the pages it keeps."""
         keep = self._pages_of(slots)
         gone = self._pages[row][keep:]
         if gone:
             del self._pages[row][keep:]
             self._free.extend(reversed(gone))
             self._write_row(row)
+            self.lens[row].clamp_(max=keep * self.page_size)
 
     def release(self, row: int) -> None:
         """End ``row``'s sequence: its pages return to the pool, its length becomes 0."""

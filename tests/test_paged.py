@@ -1639,3 +1639,18 @@ def test_trim_refuses_negative_slots():
         with pytest.raises(ValueError, match="negative"):
             call(0, -5)
     assert c.page_table.tolist() == [[0, 1, 2, -1]] and c.free_pages() == 2
+
+
+def test_trim_cuts_the_length():
+    """Slots whose pages were given back do not come back with other pages."""
+    from project_chronos_b200 import PagedCache
+    c = PagedCache(2, 8, 1, 8, 4, "cpu", torch.float32, page_size=4)
+    for row, slots in ((0, 14), (1, 6)):
+        c.reserve(row, slots)
+        c.lens[row], c.seen[row] = slots, slots
+    c.trim(0, 5)
+    assert c.lens.tolist() == [8, 6] and c.seen.tolist() == [14, 6]
+    c.reserve(0, 16)
+    assert c.lens.tolist() == [8, 6]
+    c.trim(1, 8)                                      # nothing behind it
+    assert c.lens.tolist() == [8, 6]
