@@ -88,7 +88,7 @@ typedef struct ChronosPagedAppendArgs {
  * A sequence of length 0 gets zeros and lse = -inf.  With `weights`,
  *     weights_out[b, g, j] = weights[b, g, j] + sum over the group's heads of p_j
  * for every j < len (hidden ones add nothing); slots behind are left as they
- * are; weights_out may be weights.  The workspace of a call with weights then
+ * are; weights_out may be weights, any other overlap of the two is refused.  The workspace of a call with weights then
  * holds 4 bytes per query head and slot that a row can see (by table_width and
  * slot_cap, or window), up to 2^28 bytes or one sequence's: beyond that the call
  * runs over groups of sequences.  The choice of kernel and grid goes by the same
@@ -117,7 +117,8 @@ typedef struct ChronosPagedDecodeArgs {
  * above every number, -0 = 0, equal ones by the lower slot).  Kept slots below
  * `budget` stay where they are; the i-th kept slot at or beyond it moves into
  * the i-th slot below it that was given up: K and V rows in the pages, weight
- * and position into weights_out / positions_out (which may be the inputs).
+ * and position into weights_out / positions_out (which may be the inputs, but not
+ * overlap them otherwise).
  *     src[b, g, j] = slot that now sits in slot j (j itself where it stayed),
  *     -1 for j >= min(n, budget);  lens_out[b] = min(n, budget)
  * Slots of weights_out / positions_out from lens_out on are left as they are. */
@@ -147,7 +148,7 @@ typedef struct ChronosPagedEvictArgs {
  * the last sequence are left as they are, key rows behind it are not used.
  * Offsets that do not ascend or leave the rows are reported as
  * CHRONOS_ERR_INVALID_ARG in the status word; what the results are is not said then.
- * out may be q. */
+ * out may be q, but not k or v. */
 typedef struct ChronosWindowAttnArgs {
     int32_t batch;
     int32_t heads;             /* H, a multiple of kv_heads */

@@ -43,9 +43,12 @@ int check_cache_pointers(const ChronosPagedCache& c, const char* what) {
     return CHRONOS_OK;
 }
 // Whether two arrays of n numbers overlap (`same`: other than as one).
-bool cross(const int32_t* a, const int32_t* b, int n, bool same) {
+template <typename T>
+bool cross(const T* a, const T* b, int64_t n, bool same) {
     return a != nullptr && b != nullptr && a < b + n && b < a + n && !(same && a == b);
 }
+// Numbers of a per-slot array.
+int64_t slots_of(const ChronosPagedCache& c, int64_t slot_cap) { return static_cast<int64_t>(c.batch) * c.kv_heads * slot_cap; }
 // A window (or number of first tokens) as the kernels take it: rows have at most 2^30
 // keys, so a longer one hides nothing, and positions minus it stay within 32 bits.
 int cut_window(int window) { return std::min(window, 1 << 30); }
@@ -98,6 +101,8 @@ int check_decode(const ChronosPagedDecodeArgs* a) {
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: weights and weights_out go together", what);
     if (a->weights != nullptr && a->slot_cap < 0)
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: slot_cap %lld", what, static_cast<long long>(a->slot_cap));
+    if (cross<float>(a->weights, a->weights_out, slots_of(a->cache, a->slot_cap), true))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: weights_out overlaps weights other than as the same array", what);
     return CHRONOS_OK;
 }
 
@@ -293,6 +298,10 @@ int check_evict(const ChronosPagedEvictArgs* a) {
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: budget %d must be >= 1 and >= sinks %d + recent %d", what, a->budget,
                     a->sinks, a->recent);
     if (a->slot_cap < 0) return fail(CHRONOS_ERR_INVALID_ARG, "%s: slot_cap %lld", what, static_cast<long long>(a->slot_cap));
+    const int64_t n = slots_of(a->cache, a->slot_cap);
+    if (cross<float>(a->weights, a->weights_out, n, true) || cross<int32_t>(a->positions, a->positions_out, n, true))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: weights_out and positions_out overlap their inputs other than as the same arrays",
+                    what);
     return CHRONOS_OK;
 }
 
@@ -616,6 +625,8 @@ extern "C" int chronos_window_attention(const ChronosWindowAttnArgs* a, void* st
     if (a->q == nullptr || a->out == nullptr || a->cu_q == nullptr || a->cu_k == nullptr ||
         (a->num_k > 0 && (a->k == nullptr || a->v == nullptr)))
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: q, k, v, out, cu_q and cu_k are required", what);
+    if (a->num_k > 0 && (a->out == a->k || a->out == a->v))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: out may be q, but not k or v", what);
     WindowParams p{};
     p.batch = a->batch;
     p.heads = a->heads;

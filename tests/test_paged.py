@@ -1654,3 +1654,25 @@ def test_trim_cuts_the_length():
     assert c.lens.tolist() == [8, 6]
     c.trim(1, 8)                                      # nothing behind it
     assert c.lens.tolist() == [8, 6]
+
+
+def test_results_that_overlap_other_inputs_are_refused(lib):
+    from project_chronos_b200 import _native as N
+    cap = 8                                           # 2 * 2 * 8 numbers
+    for at in (4096 - 4, 4096 + 4, 4096 + 127):
+        d = N.ChronosPagedDecodeArgs(cache=_native_cache(N), heads=4, scale=1.0, weights=4096, weights_out=at, slot_cap=cap)
+        assert lib.chronos_paged_decode(ctypes.byref(d), None) == N.CHRONOS_ERR_INVALID_ARG
+        assert b"overlaps" in lib.chronos_moe_last_error()
+        for f in (dict(weights_out=at, positions_out=8192), dict(weights_out=4096, positions_out=at + 4096)):
+            e = N.ChronosPagedEvictArgs(cache=_native_cache(N), budget=4, weights=4096, positions=8192, slot_cap=cap, **f)
+            assert lib.chronos_paged_evict(ctypes.byref(e), None) == N.CHRONOS_ERR_INVALID_ARG
+            assert b"overlap" in lib.chronos_moe_last_error()
+    for at in (4096, 4096 + 128, 4096 - 128):         # the same, side by side
+        d = N.ChronosPagedDecodeArgs(cache=_native_cache(N), heads=4, scale=1.0, weights=4096, weights_out=at, slot_cap=cap)
+        assert lib.chronos_paged_decode(ctypes.byref(d), None) == N.CHRONOS_ERR_INVALID_ARG
+        assert b"required" in lib.chronos_moe_last_error()
+    for f in (dict(k=4096, v=8192), dict(k=8192, v=4096)):
+        w = N.ChronosWindowAttnArgs(batch=1, heads=2, kv_heads=2, head_dim=8, scale=1.0, num_q=4, num_k=4, q=1024, out=4096,
+                                    cu_q=512, cu_k=512, **f)
+        assert lib.chronos_window_attention(ctypes.byref(w), None) == N.CHRONOS_ERR_INVALID_ARG
+        assert b"not k or v" in lib.chronos_moe_last_error()
