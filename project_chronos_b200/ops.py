@@ -553,7 +553,7 @@ def _rows(name: str, t: torch.Tensor, shape: tuple, dt: torch.dtype, index: int,
 def _dense(name: str, t: torch.Tensor, shape: tuple, dt: torch.dtype, index: int, dev: torch.device) -> int:
     """Address of a contiguous tensor."""
     if (t.dtype is not dt or t.get_device() != index or t.shape != shape or not t.is_contiguous()
-            or (t.requires_grad and torch.is_grad_enabled())):
+            or (dt is torch.float32 and t.requires_grad and torch.is_grad_enabled())):
         _refuse(name, t, shape, dt, dev, True)
     return t.data_ptr()
 
