@@ -107,7 +107,7 @@ int check_decode(const ChronosPagedDecodeArgs* a) {
 }
 
 // The tensor-core path: rows that can be copied 16 bytes at a time (fp32: up to 128
-// columns, what shared memory holds three stages of), q and out in pairs.
+// columns), q and out in pairs.
 bool decode_uses_mma(const ChronosPagedDecodeArgs* a) {
     const ChronosPagedCache& c = a->cache;
     const int64_t n = 16 / static_cast<int64_t>(elem_bytes(c.dtype));

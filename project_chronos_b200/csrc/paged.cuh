@@ -400,10 +400,12 @@ struct PagedMma {
 // each other inside a row.  The maximum moves only when a score exceeds it by more
 // than 2^8 in weight, which one vote per tile finds out.
 //
-// Measured, 32 / 8 heads of 128: 4 rows of 100003 to 131072 slots in fp16 300 us, 6.6 TB/s
-// (16-wide rows of heads, maxima and page lookups per row of slots: 418 us); 16 rows of
-// 16384 slots, 8 / 2 heads: 105 us with head_dim 64, 89 us with 256 (bf16, 5.1 and 6.0
-// TB/s), 127 us in fp32 (4.2 TB/s, bound by the splitting into tf32).
+// Measured, 32 / 8 heads of 128: 4 rows of 100003 to 131072 slots in fp16 291 to 310 us on
+// different boxes, 6.4 to 6.8 TB/s (16-wide rows of heads, maxima and page lookups per row of
+// slots: 418 us).  16 rows of 16384 slots in bf16: 32 / 8 heads of 64 105 us (5.1 TB/s), of 128
+// 172 us (6.2), of 256 311 us (6.9); 8 / 2 heads of 64 35 us (3.8), of 128 54 us (5.0), of 256
+// 89 us (6.0).  In fp32, heads of 128: 8 / 2 126 us (4.2 TB/s), 32 / 8 460 us (4.7), bound by
+// the splitting into tf32.
 //
 // NT: groups of 8 query heads (1 or 2).  CL: a cluster of p.cluster blocks per row
 // shares its blocks of 64 places and joins through distributed shared memory;

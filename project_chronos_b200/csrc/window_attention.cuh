@@ -289,12 +289,13 @@ __global__ void __launch_bounds__(kWsThreads) window_simt_kernel(const __grid_co
 //   warps 10, 11     V tiles with hidden keys: rows behind the sequence become
 //                    zero (0 * NaN would reach every row), and so do rows that
 //                    are not finite, in which case the block computes its rows
-//                    again pair by pair at the end
+//                    again pair by pair at the end (right, not fast: one infinity near
+//                    the end of 8192 keys takes 4 x 2048 queries from 0.77 to 141 ms)
 //
-// Measured, bf16, 32 / 8 heads of 128: 4 x 2048 queries on 8192 keys 673 us, 1180 TFLOP/s
-// (71 % of the library product's burst rate; 780 us once the power cap holds the
-// clock); one prompt of 8192 under a window of 1024 with 4 first tokens 195 us.  A
-// tile's chain bounds it: maximum and exponentials of its 128 x 128 scores about 2000
+// Measured, 32 / 8 heads of 128: 4 x 1793 to 2048 queries on up to 8192 keys in bf16 770 to
+// 788 us in long runs, which the power cap holds (1020 TFLOP/s, 73 % of the library product's
+// sustained rate), 673 us in short ones (71 % of its burst rate); one prompt of 8191 under a
+// window of 1024 with 4 first tokens in fp16 203 to 209 us.  A tile's chain bounds it: maximum and exponentials of its 128 x 128 scores about 2000
 // cycles, then both products 1400 (1040 by themselves), and two such chains per SM
 // overlap to 3500 cycles per 128 keys where either unit alone needs 2050.
 //
