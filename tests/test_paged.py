@@ -1676,3 +1676,53 @@ def test_results_that_overlap_other_inputs_are_refused(lib):
                                     cu_q=512, cu_k=512, **f)
         assert lib.chronos_window_attention(ctypes.byref(w), None) == N.CHRONOS_ERR_INVALID_ARG
         assert b"not k or v" in lib.chronos_moe_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("packed", [False, True])
+def test_a_captured_step_counts_what_it_stored(packed):
+    """Append and attention in one graph, replayed while a row grows, fills up and gets more pages."""
+    from project_chronos_b200 import _native as N
+    from project_chronos_b200 import PagedCache, ops
+    h, g, d, dt = 8, 2, 64, BF
+    c = PagedCache(2, 12, g, d, 6, "cuda", dt, page_size=16, track_weights=True)
+    k, v = (torch.zeros(2, g, d, dtype=dt, device="cuda") for _ in range(2))
+    q, out = torch.zeros(2, h, d, dtype=dt, device="cuda"), torch.zeros(2, h, d, dtype=dt, device="cuda")
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda") if packed else None
+    for b in range(2):
+        c.reserve(b, 16 + 32 * b)
+
+    def step():
+        c.append(k, v, cu)
+        c.attend(q, out=out)
+
+    step()                                            # a first call outside the capture
+    for b in range(2):
+        c.release(b)
+        c.reserve(b, 16 + 32 * b)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    assert c.lens.tolist() == [0, 0]                  # captured, not run
+    book = [[], []]
+    gen = _gen(3)
+    for i in range(40):
+        if i == 20:
+            c.reserve(0, 40)
+        for x in (k, v, q):
+            x.copy_(torch.randn(x.shape, generator=gen, device="cuda"))
+        graph.replay()
+        full = 16 <= i < 20
+        for b in range(2):
+            if b == 1 or not full:
+                book[b].append((k[b].clone(), v[b].clone()))
+            ks, vs = (torch.stack([r[j] for r in book[b]]) for j in (0, 1))
+            ref, _, _, a, f = _attend(q[b], ks, vs, d ** -0.5, _visible(len(ks), 0, 0, "cuda"))
+            _check_out(out[b], ref, a, f, len(ks), dt)
+        assert c.lens.tolist() == [len(x) for x in book] == c.seen.tolist()
+        if full:
+            with pytest.raises(N.ChronosMoeError, match="INVALID_ARG"):
+                ops.check_status(out.device)
+        else:
+            ops.check_status(out.device)
