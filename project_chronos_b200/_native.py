@@ -52,7 +52,11 @@ EXPORTS = ("chronos_moe_workspace_size", "chronos_moe_forward", "chronos_moe_rou
            "chronos_norm_args_size", "chronos_argmax_rows", "chronos_paged_append", "chronos_paged_decode",
            "chronos_paged_evict", "chronos_window_attention", "chronos_paged_decode_workspace",
            "chronos_paged_evict_workspace", "chronos_paged_append_args_size", "chronos_paged_decode_args_size",
-           "chronos_paged_evict_args_size", "chronos_window_attn_args_size")
+           "chronos_paged_evict_args_size", "chronos_window_attn_args_size", "chronos_paged_append_rope",
+           "chronos_paged_gather", "chronos_paged_decode4", "chronos_paged_bounds", "chronos_paged_select",
+           "chronos_paged_sparse", "chronos_paged_decode4_workspace", "chronos_paged_select_workspace",
+           "chronos_paged_rope_args_size", "chronos_paged_gather_args_size", "chronos_paged_decode4_args_size",
+           "chronos_paged_bounds_args_size", "chronos_paged_select_args_size", "chronos_paged_sparse_args_size")
 
 EP_MAX_RANKS = 32  # CHRONOS_EP_MAX_RANKS
 
@@ -332,6 +336,153 @@ class ChronosWindowAttnArgs(ctypes.Structure):
     ]
 
 
+class ChronosPagedRopeArgs(ctypes.Structure):
+    """include/chronos_paged4.h"""
+    _fields_ = [
+        ("cache", ChronosPagedCache),
+        ("packed", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("rope_dim", ctypes.c_int32),
+        ("rope_start", ctypes.c_int32),
+        ("table_len", ctypes.c_int32),
+        ("table_dtype", ctypes.c_int32),
+        ("k_scale", ctypes.c_float),
+        ("v_scale", ctypes.c_float),
+        ("num_tokens", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("q", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("k_row_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_row_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("q_out_row_stride", ctypes.c_int64),
+        ("q_out_head_stride", ctypes.c_int64),
+        ("k_out_row_stride", ctypes.c_int64),
+        ("k_out_head_stride", ctypes.c_int64),
+        ("cos", ctypes.c_void_p),
+        ("sin", ctypes.c_void_p),
+        ("cos_row_stride", ctypes.c_int64),
+        ("sin_row_stride", ctypes.c_int64),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("seen", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("slot_cap", ctypes.c_int64),
+        ("lens_out", ctypes.c_void_p),
+        ("seen_out", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class ChronosPagedGatherArgs(ctypes.Structure):
+    """include/chronos_paged4.h"""
+    _fields_ = [
+        ("cache", ChronosPagedCache),
+        ("packed", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("k_scale", ctypes.c_float),
+        ("v_scale", ctypes.c_float),
+        ("num_tokens", ctypes.c_int64),
+        ("k_out", ctypes.c_void_p),
+        ("v_out", ctypes.c_void_p),
+        ("k_row_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_row_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("first", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class ChronosPagedDecode4Args(ctypes.Structure):
+    """include/chronos_paged4.h"""
+    _fields_ = [
+        ("cache", ChronosPagedCache),
+        ("heads", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("k_scale", ctypes.c_float),
+        ("v_scale", ctypes.c_float),
+        ("q", ctypes.c_void_p),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_row_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+        ("lse", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class ChronosPagedBoundsArgs(ctypes.Structure):
+    """include/chronos_paged4.h"""
+    _fields_ = [
+        ("cache", ChronosPagedCache),
+        ("packed", ctypes.c_int32),
+        ("full", ctypes.c_int32),
+        ("k_scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int64),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("bounds", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class ChronosPagedSelectArgs(ctypes.Structure):
+    """include/chronos_paged4.h"""
+    _fields_ = [
+        ("cache", ChronosPagedCache),
+        ("heads", ctypes.c_int32),
+        ("topk", ctypes.c_int32),
+        ("first", ctypes.c_int32),
+        ("last", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("bounds", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("pages", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class ChronosPagedSparseArgs(ctypes.Structure):
+    """include/chronos_paged4.h"""
+    _fields_ = [
+        ("cache", ChronosPagedCache),
+        ("packed", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("topk", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("k_scale", ctypes.c_float),
+        ("v_scale", ctypes.c_float),
+        ("num_tokens", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_row_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+        ("lse", ctypes.c_void_p),
+        ("pages", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -418,6 +569,21 @@ def load_library(path: str = LIB_PATH):
             getattr(lib, fn).argtypes = []
             getattr(lib, fn).restype = ctypes.c_size_t
             if getattr(lib, fn)() != ctypes.sizeof(st):
+                raise RuntimeError("paged-cache args layout mismatch between the library and the binding")
+        for name, st in (("append_rope", ChronosPagedRopeArgs), ("gather", ChronosPagedGatherArgs),
+                         ("decode4", ChronosPagedDecode4Args), ("bounds", ChronosPagedBoundsArgs),
+                         ("select", ChronosPagedSelectArgs), ("sparse", ChronosPagedSparseArgs)):
+            fn = getattr(lib, "chronos_paged_" + name)
+            fn.argtypes = [ctypes.POINTER(st), ctypes.c_void_p]
+            fn.restype = ctypes.c_int
+            if name in ("decode4", "select"):
+                fn = getattr(lib, "chronos_paged_" + name + "_workspace")
+                fn.argtypes = [ctypes.POINTER(st)]
+                fn.restype = ctypes.c_size_t
+            fn = getattr(lib, "chronos_paged_" + name.replace("append_", "") + "_args_size")
+            fn.argtypes = []
+            fn.restype = ctypes.c_size_t
+            if fn() != ctypes.sizeof(st):
                 raise RuntimeError("paged-cache args layout mismatch between the library and the binding")
         if (lib.chronos_attn_args_size() != ctypes.sizeof(ChronosAttnArgs)
                 or lib.chronos_norm_args_size() != ctypes.sizeof(ChronosNormArgs)):

@@ -1,0 +1,62 @@
+// paged4_host.cuh — argument checks that the calls of include/chronos_paged4.h share.
+#pragma once
+
+#include "chronos_paged4.h"
+#include "paged_host.cuh"
+
+namespace chronos {
+
+constexpr int kPaged4MaxRep = 256;   // query heads per kv head
+
+inline int check_heads(int heads, const ChronosPagedCache& c, const char* what) {
+    if (heads < 1 || heads % c.kv_heads || heads / c.kv_heads > kPaged4MaxRep)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: heads %d must be 1..%d times kv_heads %d", what, heads, kPaged4MaxRep, c.kv_heads);
+    return CHRONOS_OK;
+}
+inline int check_positive(const char* name, float x, const char* what) {
+    if (!(x > 0.0f) || !std::isfinite(x)) return fail(CHRONOS_ERR_INVALID_ARG, "%s: %s %g must be positive", what, name, x);
+    return CHRONOS_OK;
+}
+inline int check_tokens(int64_t tokens, const int32_t* cu, const ChronosPagedCache& c, const char* what) {
+    if (tokens < 0 || tokens * c.kv_heads > INT32_MAX / 16)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: num_tokens %lld", what, static_cast<long long>(tokens));
+    if (cu == nullptr && tokens != c.batch)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: %lld rows for %d sequences without cu_seqlens", what, static_cast<long long>(tokens), c.batch);
+    return CHRONOS_OK;
+}
+// Rows of heads, strides in bytes.
+struct RowsOf {
+    const void* at;
+    int64_t rows, row, heads, head, bytes;
+};
+inline RowsOf rows_of(const void* at, int dtype, int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t dim) {
+    const int64_t es = static_cast<int64_t>(elem_bytes(dtype));
+    return RowsOf{at, at == nullptr ? 0 : rows, row * es, heads, head * es, dim * es};
+}
+// Whether the two may share a byte.  Rows side by side in one array (parts of a projection,
+// heads in turn) do not.
+inline bool rows_meet(const RowsOf& a, const RowsOf& b) {
+    if (a.rows <= 0 || b.rows <= 0 || a.heads <= 0 || b.heads <= 0) return false;
+    const int64_t ea = (a.heads - 1) * a.head + a.bytes, eb = (b.heads - 1) * b.head + b.bytes;
+    const int64_t at_a = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.at)), at_b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.at));
+    if (at_a + (a.rows - 1) * a.row + ea <= at_b || at_b + (b.rows - 1) * b.row + eb <= at_a) return false;
+    const auto apart = [&](int64_t step, int64_t na, int64_t nb) {   // all of a lies in [0, na) modulo step, b in [d, d + nb)
+        const int64_t d = ((at_b - at_a) % step + step) % step;
+        return d >= na && d + nb <= step;
+    };
+    if (a.row == b.row && a.row > 0 && apart(a.row, ea, eb)) return false;
+    return !(a.row == b.row && a.head == b.head && a.head > 0 && a.row % a.head == 0 && apart(a.head, a.bytes, b.bytes));
+}
+// Whether rows that are written meet an input other than as the rows that they are made from.
+inline bool rows_same(const RowsOf& a, const RowsOf& b) { return a.at == b.at && a.row == b.row && a.head == b.head; }
+
+// Pages of 4-bit values.
+inline int check_packed(const ChronosPagedCache& c, float k_scale, float v_scale, const char* what) {
+    if (c.page_size % 16) return fail(CHRONOS_ERR_INVALID_ARG, "%s: 4-bit pages need a page_size that is a multiple of 16, got %d", what, c.page_size);
+    if (!multiples(16, {c.k_page_stride, c.k_head_stride, c.v_page_stride, c.v_head_stride}) || !aligned(c.k_pages, 16) || !aligned(c.v_pages, 16))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: 4-bit pages and their strides must be multiples of 16 bytes", what);
+    if (int rc = check_positive("k_scale", k_scale, what)) return rc;
+    return check_positive("v_scale", v_scale, what);
+}
+
+}  // namespace chronos
