@@ -44,8 +44,7 @@ int launch_rope(PagedRopeParams p, bool packed, bool vec, cudaStream_t st) {
     const int lanes = vec ? fp4_columns(p.c.head_dim) / 8 : 32, rows = 2 * p.c.kv_heads + p.heads;
     // Warps per token: more while SMs would be idle and every one has rows of its own.
     p.slices = 1;
-    const int at_once = 2 * (32 / lanes);
-    while (p.slices < kRopeWarps && p.slices * at_once < rows && p.tokens * p.slices < 16 * static_cast<int64_t>(sm_count())) p.slices *= 2;
+    while (p.slices < kRopeWarps && p.slices * (32 / lanes) < rows && p.tokens * p.slices < 16 * static_cast<int64_t>(sm_count())) p.slices *= 2;
     const int per = kRopeWarps / p.slices;
     auto kernel = packed ? rope_kernel<T, TT, true>(lanes, vec) : rope_kernel<T, TT, false>(lanes, vec);
     if (p.tokens > 0)

@@ -54,34 +54,59 @@ struct PagedRopeParams {
 constexpr int kRopeThreads = 256;
 constexpr int kRopeWarps = kRopeThreads / 32;
 
-// A lane's 8 columns of a row and, where they are rotated, the columns they turn with.
-struct RopeRow {
-    float x[8], with[8];
-};
 // Column that column d turns with (d itself where it is not rotated).
 __device__ __forceinline__ int rope_partner(int d, int start, int dim) {
     const int j = d - start;
     return j < 0 || j >= dim ? d : j < dim / 2 ? d + dim / 2 : d - dim / 2;
 }
 
+// A lane's 8 columns of a row as they are loaded.  VEC: 16-byte words (the columns they turn
+// with come from the lane that has them); else numbers, with those columns beside them.
 template <typename T, bool VEC>
-__device__ __forceinline__ void rope_load(RopeRow& r, const T* row, int col, bool on, bool turns, int D, int start, int dim) {
+struct RopeRow {
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* row, int col, bool on, int, int, int) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r.x[j] = r.with[j] = 0.0f;
-    if (!on) return;
-    if constexpr (VEC) {
-        load8<T>(row + col, r.x);
-        if (turns) load8<T>(row + rope_partner(col, start, dim), r.with);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (col + j < D) {
-                r.x[j] = to_f32<T>(row[col + j]);
-                const int w = rope_partner(col + j, start, dim);
-                if (turns && w != col + j) r.with[j] = to_f32<T>(row[w]);
-            }
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+            w[i] = on ? reinterpret_cast<const uint4*>(row + col)[i] : make_uint4(0u, 0u, 0u, 0u);
     }
-}
+    __device__ __forceinline__ void values(float (&x)[8]) const { load8<T>(reinterpret_cast<const T*>(w), x); }
+    // Whole warps call it.
+    __device__ __forceinline__ void partner(float (&x)[8], int lane) const {
+        RopeRow r;
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) {
+            r.w[i].x = __shfl_sync(0xffffffffu, w[i].x, lane);
+            r.w[i].y = __shfl_sync(0xffffffffu, w[i].y, lane);
+            r.w[i].z = __shfl_sync(0xffffffffu, w[i].z, lane);
+            r.w[i].w = __shfl_sync(0xffffffffu, w[i].w, lane);
+        }
+        r.values(x);
+    }
+};
+template <typename T>
+struct RopeRow<T, false> {
+    float x[8], with[8];
+    __device__ __forceinline__ void load(const T* row, int col, bool on, int D, int start, int dim) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[j] = with[j] = 0.0f;
+            if (on && col + j < D) {
+                x[j] = to_f32<T>(row[col + j]);
+                const int w = rope_partner(col + j, start, dim);
+                if (w != col + j) with[j] = to_f32<T>(row[w]);
+            }
+        }
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = x[j];
+    }
+    __device__ __forceinline__ void partner(float (&v)[8], int) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = with[j];
+    }
+};
 template <typename T, bool VEC>
 __device__ __forceinline__ void rope_store(T* row, const float (&y)[8], int col, int D) {
     if constexpr (VEC) {
@@ -93,12 +118,54 @@ __device__ __forceinline__ void rope_store(T* row, const float (&y)[8], int col,
     }
 }
 
+// What a lane's 8 values are made of, for the computation in 64 bits: the row (NULL: zeros)
+// and the angles of its position (NULL: not rotated).
+template <typename T, typename TT>
+struct RopeSource {
+    const T* row;
+    const TT* cos;
+    const TT* sin;
+    int col, D, start, dim;
+    float scale;   // the cache's factor
+    __device__ __forceinline__ double value(int j) const {
+        const int d = col + j;
+        if (row == nullptr || d >= D) return 0.0;
+        double v = to_f32<T>(row[d]);
+        const int w = cos != nullptr ? rope_partner(d, start, dim) : d;
+        if (w != d) {
+            const double turned = static_cast<double>(to_f32<T>(row[w])) * to_f32<TT>(sin[d - start]);
+            v = v * to_f32<TT>(cos[d - start]) + (w > d ? -turned : turned);
+        }
+        return v / static_cast<double>(scale);
+    }
+};
+// Codes and scale in 64 bits.  two: the scale's candidates, the lower one in the low byte.
+// Whole warps call it.  Not inlined: its registers stay out of the common path.
+template <typename T, typename TT>
+__device__ __noinline__ uint32_t fp4_block_exact(const RopeSource<T, TT> src, uint32_t two, uint32_t* scale) {
+    double t = 0.0;
+    for (int j = 0; j < 8; ++j) t = fmax(t, fabs(src.value(j)));
+    t = fmax(t, __shfl_xor_sync(0xffffffffu, t, 1));
+    uint32_t lo = two & 0xffu;
+    if (lo != two >> 8) lo = fp8_scales(static_cast<float>(t / 6.0), 0.0f) & 0xffu;
+    *scale = lo;
+    const double z = fp8_value(lo);
+    uint32_t c = 0;
+    for (int j = 0; j < 8; ++j) {
+        const double d = src.value(j), m = fabs(d);
+        const uint32_t level = (m > 0.25 * z) + (m >= 0.75 * z) + (m > 1.25 * z) + (m >= 1.75 * z) + (m > 2.5 * z) +
+                               (m >= 3.5 * z) + (m > 5.0 * z);
+        c |= (level | (signbit(d) ? 8u : 0u)) << (4 * j);
+    }
+    return c;
+}
+
 // Codes of a lane's 8 values and the scale of its block of 16 (two lanes).  y: the values in
 // units of the cache's factor; off: what y may be off by at most, in 2^-20 (rotated or
-// divided values; `exact` ones are what they are); wide(j): the j-th value in 64 bits.
-// Whole warps call it.
-template <bool SIXTEEN, typename F>
-__device__ __forceinline__ uint32_t fp4_block(const float (&y)[8], const float (&off)[8], bool exact, uint32_t& scale, F wide) {
+// divided values; `exact` ones are what they are).  Whole warps call it.
+template <typename T, typename TT>
+__device__ __forceinline__ uint32_t fp4_block(const float (&y)[8], const float (&off)[8], bool exact, uint32_t& scale,
+                                              const RopeSource<T, TT>& src) {
     constexpr float kOff = 0x1p-20f;
     uint32_t top = 0;
     float most = 0.0f;
@@ -108,73 +175,73 @@ __device__ __forceinline__ uint32_t fp4_block(const float (&y)[8], const float (
         most = fmaxf(most, off[j]);
     }
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    const bool all = __shfl_xor_sync(0xffffffffu, exact ? 1 : 0, 1) && exact;
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));   // 0: all 16 are exact
     const bool finite = top < 0x7f800000u;
     const float a = finite ? __uint_as_float(top) : 0.0f;
     // exact magnitudes are divided as they are; the others open the scale where a little more or
     // less of them gives another one
-    uint32_t lo, hi;
-    if (all) {
-        lo = hi = fp8_scales(a / 6.0f, 0.0f) & 0xffu;
+    uint32_t two;
+    if (most == 0.0f) {
+        const float a6 = a / 6.0f;
+        two = fp8_scales(a6, a6);
     } else {
         const float a6 = a * (1.0f / 6.0f), d6 = fmaxf(most, a) * (kOff / 2);
-        const uint32_t two = fp8_scales(fmaxf(a6 - d6, 0.0f), a6 + d6);
-        lo = two & 0xffu;
-        hi = two >> 8;
+        two = fp8_scales(fmaxf(a6 - d6, 0.0f), a6 + d6);
     }
-    float s = fp8_value(lo);
+    const float s = fp8_value(two);
     const float r = s > 0.0f ? __frcp_rn(s) : 0.0f;
-    float u[8], w[8];
+    uint32_t codes;
+    bool open = (two & 0xffu) != two >> 8;
+    float u[8];
+    if (sizeof(T) == 2 && exact) {
+        // 96 + 2^-17 z: values of 64 to 128 have 17 bits behind the point
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float v = y[j] * r;
-        if (SIXTEEN && exact) {
-            // 96 + 2^-17 z: values of 64 to 128 have 17 bits behind the point
-            u[j] = w[j] = copysignf(fmaf(y[j], r, 96.0f) - 96.0f, y[j]);
-        } else {
-            const float d = (exact ? fabsf(y[j]) : off[j]) * r * kOff;
-            u[j] = v - d;
-            w[j] = v + d;
-        }
+        for (int j = 0; j < 8; ++j) u[j] = copysignf(fmaf(y[j], r, 96.0f) - 96.0f, y[j]);
+        codes = fp4_codes(u);
+    } else {
+        const float d = r * kOff;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = fmaf(exact ? fabsf(y[j]) : off[j], -d, y[j] * r);
+        codes = fp4_codes(u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = fmaf(exact ? fabsf(y[j]) : off[j], d, y[j] * r);
+        open |= codes != fp4_codes(u);
     }
-    uint32_t codes = fp4_codes(u);
-    const uint32_t other = fp4_codes(w);
-    const bool open = finite && (lo != hi || codes != other);
-    if (__any_sync(0xffffffffu, open)) {
-        double d[8], t = 0.0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            d[j] = wide(j);
-            t = fmax(t, fabs(d[j]));
-        }
-        t = fmax(t, __shfl_xor_sync(0xffffffffu, t, 1));
-        if (lo != hi) lo = fp8_scales(static_cast<float>(t / 6.0), 0.0f) & 0xffu;
-        s = fp8_value(lo);
-        uint32_t c = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const double m = fabs(d[j]), z = s;
-            const uint32_t level = (m > 0.25 * z) + (m >= 0.75 * z) + (m > 1.25 * z) + (m >= 1.75 * z) + (m > 2.5 * z) +
-                                   (m >= 3.5 * z) + (m > 5.0 * z);
-            c |= (level | (signbit(d[j]) ? 8u : 0u)) << (4 * j);
-        }
-        codes = c;
-    }
-    scale = finite ? lo : kFp8Nan;
-    return finite && s > 0.0f ? codes : 0u;
+    scale = two & 0xffu;
+    open &= finite;
+    if (__any_sync(0xffffffffu, open)) codes = fp4_block_exact<T, TT>(src, two, &scale);
+    codes = finite && scale != 0u ? codes : 0u;
+    if (!finite) scale = kFp8Nan;
+    return codes;
 }
 
 // LPR lanes hold a row (8 columns each).  VEC: rows, halves and tables can be read 8
 // columns at a time.
 template <typename T, typename TT, int LPR, bool VEC, bool PACKED>
-__global__ void __launch_bounds__(kRopeThreads) paged_rope_kernel(const __grid_constant__ PagedRopeParams p) {
-    constexpr int RPW = 32 / LPR;   // rows of a warp at once
-    constexpr int U = 2;            // ... and as many again in flight
+__global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED || sizeof(T) == 4 ? 2 : 3) paged_rope_kernel(const __grid_constant__ PagedRopeParams p) {
+    constexpr int RPW = 32 / LPR;                       // rows of a warp at once
+    constexpr int U = sizeof(T) == 2 && VEC ? 4 : 2;    // ... and so many times that in flight
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int slice = warp % p.slices;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * (kRopeWarps / p.slices) + warp / p.slices;
-    const int G = p.c.kv_heads, D = p.c.head_dim;
+    const int G = p.c.kv_heads, D = p.c.head_dim, rows = 2 * G + p.heads;
+    const int sub = lane / LPR, col = lane % LPR * 8;
+    const bool on = col < D;
+    const int stride = p.slices * RPW;
+    auto source = [&](int r) {
+        return r < G ? static_cast<const T*>(p.k) + t * p.k_row + r * p.k_head
+                     : r < 2 * G ? static_cast<const T*>(p.v) + t * p.v_row + (r - G) * p.v_head
+                                 : static_cast<const T*>(p.q) + t * p.q_row + (r - 2 * G) * p.q_head;
+    };
+    // the first rows are on their way while the token's place is looked up
+    RopeRow<T, VEC> x[U];
+    int r0 = slice * RPW;
+#pragma unroll
+    for (int n = 0; n < U; ++n) {
+        const int r = r0 + n * stride + sub;
+        x[n].load(source(r), col, on && r < rows && t < p.tokens, D, p.start, p.dim);
+    }
+
     int b = -1, page = -1;
     int64_t i = 0, slot = 0, at = 0;
     bool placed = false;    // at a position of the tables
@@ -212,25 +279,23 @@ __global__ void __launch_bounds__(kRopeThreads) paged_rope_kernel(const __grid_c
             if (p.positions != nullptr) p.positions[w] = static_cast<int32_t>(at);
         }
 
-    const int sub = lane / LPR, col = lane % LPR * 8;
-    const bool on = col < D;
     // angles of this lane's columns; the sine carries the sign of its half
     float cs[8], sn[8];
     bool turns = false;
+    const TT* cos = static_cast<const TT*>(p.cos) + at * p.cos_row;
+    const TT* sin = static_cast<const TT*>(p.sin) + at * p.sin_row;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         cs[j] = 1.0f;
         sn[j] = 0.0f;
     }
     if (on && p.dim > 0 && placed) {
-        const TT* c = static_cast<const TT*>(p.cos) + at * p.cos_row;
-        const TT* s = static_cast<const TT*>(p.sin) + at * p.sin_row;
         if constexpr (VEC) {
             const int j = col - p.start;
             turns = j >= 0 && j < p.dim;
             if (turns) {
-                load8<TT>(c + j, cs);
-                load8<TT>(s + j, sn);
+                load8<TT>(cos + j, cs);
+                load8<TT>(sin + j, sn);
                 if (j < p.dim / 2)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) sn[e] = -sn[e];
@@ -241,46 +306,64 @@ __global__ void __launch_bounds__(kRopeThreads) paged_rope_kernel(const __grid_c
                 const int j = col + e - p.start;
                 if (col + e < D && j >= 0 && j < p.dim) {
                     turns = true;
-                    cs[e] = to_f32<TT>(c[j]);
-                    sn[e] = to_f32<TT>(s[j]);
+                    cs[e] = to_f32<TT>(cos[j]);
+                    sn[e] = to_f32<TT>(sin[j]);
                     if (j < p.dim / 2) sn[e] = -sn[e];
                 }
             }
         }
     }
+    const int from = VEC ? lane - lane % LPR + rope_partner(col, p.start, turns ? p.dim : 0) / 8 : lane;   // the lane that has what these turn with
 
-    const int rows = 2 * G + p.heads;
-    for (int r0 = slice * RPW * U; r0 < rows; r0 += p.slices * RPW * U) {
-        RopeRow x[U];
+    for (; r0 < rows; r0 += stride * U) {
+        if (r0 != slice * RPW)
 #pragma unroll
-        for (int n = 0; n < U; ++n) {
-            const int r = r0 + n * RPW + sub;
-            const T* src = r < G ? static_cast<const T*>(p.k) + t * p.k_row + r * p.k_head
-                                 : r < 2 * G ? static_cast<const T*>(p.v) + t * p.v_row + (r - G) * p.v_head
-                                             : static_cast<const T*>(p.q) + t * p.q_row + (r - 2 * G) * p.q_head;
-            rope_load<T, VEC>(x[n], src, col, on && r < rows, turns && (r < G || r >= 2 * G), D, p.start, p.dim);
-        }
+            for (int n = 0; n < U; ++n) {
+                const int r = r0 + n * stride + sub;
+                x[n].load(source(r), col, on && r < rows, D, p.start, p.dim);
+            }
         __syncwarp();   // q_out may be q, k_out k: a row is read before it is written over
 #pragma unroll
         for (int n = 0; n < U; ++n) {
-            const int r = r0 + n * RPW + sub;
+            const int base = r0 + n * stride, r = base + sub;
+            if (base >= rows) break;
             const bool is_k = r < G, is_v = !is_k && r < 2 * G, turned = turns && !is_v;
-            float y[8];
+            float y[8], w[8];
+            x[n].values(y);
+            x[n].partner(w, from);
+            float off[PACKED ? 8 : 1];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = turned ? fmaf(x[n].x[j], cs[j], x[n].with[j] * sn[j]) : x[n].x[j];
-            if (on && r < rows) {
-                if (!is_k && !is_v) {
-                    T* to = static_cast<T*>(p.q_out) + t * p.qo_row + (r - 2 * G) * p.qo_head;
-                    if (!placed)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) y[j] = 0.0f;
-                    rope_store<T, VEC>(to, y, col, D);
-                } else if (is_k && p.k_out != nullptr) {
+            for (int j = 0; j < 8; ++j) {
+                w[j] *= sn[j];
+                if constexpr (PACKED) off[j] = turned ? fmaf(fabsf(y[j]), fabsf(cs[j]), fabsf(w[j])) : fabsf(y[j]);
+                y[j] = turned ? fmaf(y[j], cs[j], w[j]) : y[j];
+            }
+            uint32_t codes = 0, scale = 0;
+            const bool store4 = PACKED && page >= 0 && base < 2 * G;   // a row of the group is one of K or V
+            if constexpr (PACKED) {
+                if (store4) {
+                    const float unit = is_k ? p.k_unit : p.v_unit;
+                    const bool exact = !turned && (is_k ? p.k_exact : p.v_exact);
                     float z[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) z[j] = placed ? y[j] : 0.0f;
-                    rope_store<T, VEC>(static_cast<T*>(p.k_out) + t * p.ko_row + r * p.ko_head, z, col, D);
+                    for (int j = 0; j < 8; ++j) {
+                        z[j] = y[j] * unit;
+                        off[j] = exact ? 0.0f : off[j] * unit;
+                    }
+                    const RopeSource<T, TT> src{r < 2 * G ? source(r) : nullptr, turned ? cos : nullptr, sin, col, D, p.start, p.dim,
+                                                is_k ? p.k_scale : p.v_scale};
+                    codes = fp4_block<T, TT>(z, off, exact, scale, src);
+                    __syncwarp();   // the rows may be read there
                 }
+            }
+            if (on && r < rows) {
+                if (!placed)   // stored nowhere: q_out and k_out are zeros
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) y[j] = 0.0f;
+                if (!is_k && !is_v)
+                    rope_store<T, VEC>(static_cast<T*>(p.q_out) + t * p.qo_row + (r - 2 * G) * p.qo_head, y, col, D);
+                else if (is_k && p.k_out != nullptr)
+                    rope_store<T, VEC>(static_cast<T*>(p.k_out) + t * p.ko_row + r * p.ko_head, y, col, D);
                 if (!PACKED && page >= 0) {
                     if (is_k)
                         rope_store<T, VEC>(static_cast<T*>(p.c.k_pages) + page * p.c.k_page_stride + in_page * p.c.k_slot_stride +
@@ -290,30 +373,13 @@ __global__ void __launch_bounds__(kRopeThreads) paged_rope_kernel(const __grid_c
                                                (r - G) * p.c.v_head_stride, y, col, D);
                 }
             }
-            if (PACKED && page >= 0 && r0 + n * RPW < 2 * G) {   // a row of the group is one of K or V
-                const float unit = is_k ? p.k_unit : p.v_unit;
-                const bool exact = !turned && (is_k ? p.k_exact : p.v_exact);
-                float off[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    off[j] = exact ? 0.0f
-                                   : (turned ? fmaf(fabsf(x[n].x[j]), fabsf(cs[j]), fabsf(x[n].with[j] * sn[j])) : fabsf(y[j])) * unit;
-                    y[j] *= unit;
-                }
-                uint32_t scale;
-                const uint32_t codes = fp4_block<sizeof(T) == 2>(y, off, exact, scale, [&](int j) {
-                    const double v = turned ? static_cast<double>(x[n].x[j]) * cs[j] + static_cast<double>(x[n].with[j]) * sn[j]
-                                            : static_cast<double>(x[n].x[j]);
-                    return v / static_cast<double>(is_k ? p.k_scale : p.v_scale);
-                });
-                if (r < 2 * G && col < p.columns) {
-                    const int g = is_k ? r : r - G, line = in_page & 15;
-                    uint8_t* record = static_cast<uint8_t*>(is_k ? p.c.k_pages : p.c.v_pages) +
-                                      page * (is_k ? p.c.k_page_stride : p.c.v_page_stride) +
-                                      g * (is_k ? p.c.k_head_stride : p.c.v_head_stride) + (in_page >> 4) * fp4_record(p.columns);
-                    *reinterpret_cast<uint32_t*>(record + line * (p.columns / 2) + col / 2) = codes;
-                    if ((col & 8) == 0) record[8 * p.columns + line * (p.columns / 16) + col / 16] = static_cast<uint8_t>(scale);
-                }
+            if (store4 && r < 2 * G && col < p.columns) {
+                const int g = is_k ? r : r - G, line = in_page & 15;
+                uint8_t* record = static_cast<uint8_t*>(is_k ? p.c.k_pages : p.c.v_pages) +
+                                  page * (is_k ? p.c.k_page_stride : p.c.v_page_stride) +
+                                  g * (is_k ? p.c.k_head_stride : p.c.v_head_stride) + (in_page >> 4) * fp4_record(p.columns);
+                *reinterpret_cast<uint32_t*>(record + line * (p.columns / 2) + col / 2) = codes;
+                if ((col & 8) == 0) record[8 * p.columns + line * (p.columns / 16) + col / 16] = static_cast<uint8_t>(scale);
             }
         }
     }
