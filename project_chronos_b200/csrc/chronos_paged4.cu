@@ -248,7 +248,9 @@ extern "C" int chronos_paged_gather(const ChronosPagedGatherArgs* a, void* strea
     const int dt = a->cache.dtype;
     const bool vec = a->cache.head_dim % 8 == 0 && (a->packed || pages8(a->cache)) &&
                      rows8(dt, {p.k, p.v}, {p.k_row, p.k_head, p.v_row, p.v_head});
-    const dim3 grid(static_cast<unsigned>((p.tokens + kRopeWarps - 1) / kRopeWarps));
+    // as many tokens per block as leave every SM four blocks
+    p.block = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kGatherTokens, p.tokens / (4 * sm_count()))));
+    const dim3 grid(static_cast<unsigned>((p.tokens + p.block - 1) / p.block));
     return by_dtype(dt, [&](auto x) {
         using T = decltype(x);
         auto kernel = a->packed ? gather_kernel<T, true>(p.columns / 8, vec) : gather_kernel<T, false>(p.columns / 8, vec);

@@ -57,5 +57,17 @@ __device__ __forceinline__ uint32_t mul_halves(uint32_t a, uint32_t b) {
     return r;
 }
 constexpr uint32_t kFp8Nan = 0x7fu;
+// max(a, |b|), NaN where one of the two is.
+__device__ __forceinline__ float max_magnitude(float a, float b) {
+    float r;
+    asm("{\n\t.reg .f32 m;\n\tabs.f32 m, %2;\n\tmax.NaN.f32 %0, %1, m;\n\t}" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// 1 / x to 2^-22.
+__device__ __forceinline__ float reciprocal(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 
 }  // namespace chronos

@@ -71,16 +71,15 @@ struct RopeRow {
             w[i] = on ? reinterpret_cast<const uint4*>(row + col)[i] : make_uint4(0u, 0u, 0u, 0u);
     }
     __device__ __forceinline__ void values(float (&x)[8]) const { load8<T>(reinterpret_cast<const T*>(w), x); }
-    // Whole warps call it.
-    __device__ __forceinline__ void partner(float (&x)[8], int lane) const {
+    // Zeros for columns that do not turn.  Whole warps call it.
+    __device__ __forceinline__ void partner(float (&x)[8], int lane, bool turns) const {
         RopeRow r;
+        auto take = [&](uint32_t v) {
+            const uint32_t g = __shfl_sync(0xffffffffu, v, lane);
+            return turns ? g : 0u;
+        };
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) {
-            r.w[i].x = __shfl_sync(0xffffffffu, w[i].x, lane);
-            r.w[i].y = __shfl_sync(0xffffffffu, w[i].y, lane);
-            r.w[i].z = __shfl_sync(0xffffffffu, w[i].z, lane);
-            r.w[i].w = __shfl_sync(0xffffffffu, w[i].w, lane);
-        }
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.w[i] = make_uint4(take(w[i].x), take(w[i].y), take(w[i].z), take(w[i].w));
         r.values(x);
     }
 };
@@ -102,7 +101,7 @@ struct RopeRow<T, false> {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = x[j];
     }
-    __device__ __forceinline__ void partner(float (&v)[8], int) const {
+    __device__ __forceinline__ void partner(float (&v)[8], int, bool) const {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = with[j];
     }
@@ -139,17 +138,24 @@ struct RopeSource {
         return v / static_cast<double>(scale);
     }
 };
-// Codes and scale in 64 bits.  two: the scale's candidates, the lower one in the low byte.
-// Whole warps call it.  Not inlined: its registers stay out of the common path.
+// Codes and scale in 64 bits.  Whole warps call it.  Not inlined: its registers stay out of
+// the common path.
 template <typename T, typename TT>
-__device__ __noinline__ uint32_t fp4_block_exact(const RopeSource<T, TT> src, uint32_t two, uint32_t* scale) {
+__device__ __noinline__ uint32_t fp4_block_exact(const RopeSource<T, TT> src, uint32_t* scale) {
     double t = 0.0;
-    for (int j = 0; j < 8; ++j) t = fmax(t, fabs(src.value(j)));
+    bool bad = false;
+    for (int j = 0; j < 8; ++j) {
+        const double d = fabs(src.value(j));
+        bad |= !(d < INFINITY);
+        t = fmax(t, d);
+    }
     t = fmax(t, __shfl_xor_sync(0xffffffffu, t, 1));
-    uint32_t lo = two & 0xffu;
-    if (lo != two >> 8) lo = fp8_scales(static_cast<float>(t / 6.0), 0.0f) & 0xffu;
-    *scale = lo;
-    const double z = fp8_value(lo);
+    bad |= __shfl_xor_sync(0xffffffffu, bad ? 1 : 0, 1) != 0;
+    const float t6 = static_cast<float>(t / 6.0);
+    const uint32_t e = bad ? kFp8Nan : fp8_scales(t6, t6) & 0xffu;
+    *scale = e;
+    if (bad || e == 0u) return 0u;
+    const double z = fp8_value(e);
     uint32_t c = 0;
     for (int j = 0; j < 8; ++j) {
         const double d = src.value(j), m = fabs(d);
@@ -160,38 +166,33 @@ __device__ __noinline__ uint32_t fp4_block_exact(const RopeSource<T, TT> src, ui
     return c;
 }
 
-// Codes of a lane's 8 values and the scale of its block of 16 (two lanes).  y: the values in
-// units of the cache's factor; off: what y may be off by at most, in 2^-20 (rotated or
-// divided values; `exact` ones are what they are).  Whole warps call it.
-template <typename T, typename TT>
-__device__ __forceinline__ uint32_t fp4_block(const float (&y)[8], const float (&off)[8], bool exact, uint32_t& scale,
-                                              const RopeSource<T, TT>& src) {
-    constexpr float kOff = 0x1p-20f;
-    uint32_t top = 0;
-    float most = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        top = max(top, __float_as_uint(y[j]) & 0x7fffffffu);
-        most = fmaxf(most, off[j]);
-    }
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));   // 0: all 16 are exact
-    const bool finite = top < 0x7f800000u;
-    const float a = finite ? __uint_as_float(top) : 0.0f;
-    // exact magnitudes are divided as they are; the others open the scale where a little more or
-    // less of them gives another one
+// Codes of a lane's 8 values y (in units of the cache's factor; top: the largest magnitude, NaN
+// where one is) and the scale of its block of 16 (two lanes).  off: no value of the lane is off by more than 2^-22 off; 0 where all are
+// what they are.  open: the block has to be decided in 64 bits.  Whole warps call it.
+template <typename T>
+__device__ __forceinline__ uint32_t fp4_block(const float (&y)[8], float top, float off, uint32_t& scale, bool& open) {
+    // here and in what follows: NaN where one of the 16 is
+    const float a = max_magnitude(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    const bool exact = off == 0.0f;
+    off = fmaxf(off, __shfl_xor_sync(0xffffffffu, off, 1));
+    const bool finite = a < INFINITY;
+    // exact magnitudes are divided as they are (16-bit ones lie on the middle of two scales or at
+    // least 2^-12 of it away: rounding the quotient to 15 bits restores what lay there); the others
+    // open the scale where a little more or less of them gives another one
     uint32_t two;
-    if (most == 0.0f) {
-        const float a6 = a / 6.0f;
-        two = fp8_scales(a6, a6);
-    } else {
-        const float a6 = a * (1.0f / 6.0f), d6 = fmaxf(most, a) * (kOff / 2);
+    if (off != 0.0f) {
+        const float a6 = a * (1.0f / 6.0f), d6 = fmaxf(off, a) * 0x1p-21f;
         two = fp8_scales(fmaxf(a6 - d6, 0.0f), a6 + d6);
+    } else {
+        float a6;
+        if constexpr (sizeof(T) == 2) a6 = __uint_as_float((__float_as_uint(a * (1.0f / 6.0f)) + 0x80u) & 0xffffff00u);
+        else a6 = a / 6.0f;
+        two = fp8_scales(a6, a6);
     }
     const float s = fp8_value(two);
-    const float r = s > 0.0f ? __frcp_rn(s) : 0.0f;
+    const float r = s > 0.0f ? reciprocal(s) : 0.0f;
     uint32_t codes;
-    bool open = (two & 0xffu) != two >> 8;
+    open = (two & 0xffu) != two >> 8;
     float u[8];
     if (sizeof(T) == 2 && exact) {
         // 96 + 2^-17 z: values of 64 to 128 have 17 bits behind the point
@@ -199,17 +200,17 @@ __device__ __forceinline__ uint32_t fp4_block(const float (&y)[8], const float (
         for (int j = 0; j < 8; ++j) u[j] = copysignf(fmaf(y[j], r, 96.0f) - 96.0f, y[j]);
         codes = fp4_codes(u);
     } else {
-        const float d = r * kOff;
+        const float d = exact ? 0.0f : fmaxf(off, a) * r * 0x1p-21f;   // with what r and the product are off 7 of these 8 times 2^-24; exact: zeros
 #pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] = fmaf(exact ? fabsf(y[j]) : off[j], -d, y[j] * r);
+        for (int j = 0; j < 8; ++j) u[j] = fmaf(y[j], r, -d);
         codes = fp4_codes(u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] = fmaf(exact ? fabsf(y[j]) : off[j], d, y[j] * r);
+        for (int j = 0; j < 8; ++j) u[j] = fmaf(y[j], r, d);
+        // a sign that differs is one of values next to zero: decided like the codes
         open |= codes != fp4_codes(u);
     }
     scale = two & 0xffu;
     open &= finite;
-    if (__any_sync(0xffffffffu, open)) codes = fp4_block_exact<T, TT>(src, two, &scale);
     codes = finite && scale != 0u ? codes : 0u;
     if (!finite) scale = kFp8Nan;
     return codes;
@@ -218,31 +219,33 @@ __device__ __forceinline__ uint32_t fp4_block(const float (&y)[8], const float (
 // LPR lanes hold a row (8 columns each).  VEC: rows, halves and tables can be read 8
 // columns at a time.
 template <typename T, typename TT, int LPR, bool VEC, bool PACKED>
-__global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED || sizeof(T) == 4 ? 2 : 3) paged_rope_kernel(const __grid_constant__ PagedRopeParams p) {
+__global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) == 4 ? 2 : 3) paged_rope_kernel(const __grid_constant__ PagedRopeParams p) {
     constexpr int RPW = 32 / LPR;                       // rows of a warp at once
-    constexpr int U = sizeof(T) == 2 && VEC ? 4 : 2;    // ... and so many times that in flight
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int U = sizeof(T) == 2 && VEC && !PACKED ? 4 : 2;    // ... and so many times that in flight
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int slice = warp % p.slices;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * (kRopeWarps / p.slices) + warp / p.slices;
-    const int G = p.c.kv_heads, D = p.c.head_dim, rows = 2 * G + p.heads;
+    const int G = p.c.kv_heads, D = p.c.head_dim;
     const int sub = lane / LPR, col = lane % LPR * 8;
     const bool on = col < D;
-    const int stride = p.slices * RPW;
-    auto source = [&](int r) {
-        return r < G ? static_cast<const T*>(p.k) + t * p.k_row + r * p.k_head
-                     : r < 2 * G ? static_cast<const T*>(p.v) + t * p.v_row + (r - G) * p.v_head
-                                 : static_cast<const T*>(p.q) + t * p.q_row + (r - 2 * G) * p.q_head;
+    // units of RPW rows of one kind: first those of K, then V, then the queries
+    const int uk = (G + RPW - 1) / RPW, units = 2 * uk + (p.heads + RPW - 1) / RPW;
+    const T* src_k = static_cast<const T*>(p.k) + t * p.k_row + sub * p.k_head;
+    const T* src_v = static_cast<const T*>(p.v) + t * p.v_row + sub * p.v_head;
+    const T* src_q = static_cast<const T*>(p.q) + t * p.q_row + sub * p.q_head;
+    auto fetch = [&](RopeRow<T, VEC>& x, int u) {
+        const bool is_k = u < uk, is_q = u >= 2 * uk;
+        const int row = (is_k ? u : is_q ? u - 2 * uk : u - uk) * RPW;
+        const T* src = is_k ? src_k + row * p.k_head : is_q ? src_q + row * p.q_head : src_v + row * p.v_head;
+        x.load(src, col, on && u < units && row + sub < (is_q ? p.heads : G) && t < p.tokens, D, p.start, p.dim);
     };
     // the first rows are on their way while the token's place is looked up
     RopeRow<T, VEC> x[U];
-    int r0 = slice * RPW;
+    int u0 = slice;
 #pragma unroll
-    for (int n = 0; n < U; ++n) {
-        const int r = r0 + n * stride + sub;
-        x[n].load(source(r), col, on && r < rows && t < p.tokens, D, p.start, p.dim);
-    }
+    for (int n = 0; n < U; ++n) fetch(x[n], u0 + n * p.slices);
 
-    int b = -1, page = -1;
+    int b = -1, page = -1, in_page = 0;
     int64_t i = 0, slot = 0, at = 0;
     bool placed = false;    // at a position of the tables
     if (t < p.tokens) {
@@ -257,7 +260,11 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED || sizeof(T) =
         slot = p.c.lens[b] + i;
         at = p.seen != nullptr ? p.seen[b] + i : 0;
         placed = p.dim == 0 || (at >= 0 && at < p.table_len);
-        if (placed && slot >= 0 && slot < p.max_slots) page = p.c.page_table[b * p.c.page_table_stride + slot / p.c.page_size];
+        if (placed && slot >= 0 && slot < p.max_slots) {
+            const int size = p.c.page_size, j = static_cast<int>(slot) / size;
+            in_page = static_cast<int>(slot) - j * size;
+            page = p.c.page_table[b * p.c.page_table_stride + j];
+        }
         if (page < 0 || page >= p.c.num_pages) {
             page = -1;
             if (lane == 0) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
@@ -271,7 +278,6 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED || sizeof(T) =
         }
     }
     if (b < 0) return;
-    const int in_page = static_cast<int>(slot % p.c.page_size);
     if (slice == 0 && page >= 0)
         for (int g = lane; g < G; g += 32) {
             const int64_t w = (static_cast<int64_t>(b) * G + g) * p.slot_cap + slot;
@@ -287,7 +293,7 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED || sizeof(T) =
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         cs[j] = 1.0f;
-        sn[j] = 0.0f;
+        sn[j] = -0.0f;   // x c - 0 is x, its sign included
     }
     if (on && p.dim > 0 && placed) {
         if constexpr (VEC) {
@@ -315,71 +321,117 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED || sizeof(T) =
     }
     const int from = VEC ? lane - lane % LPR + rope_partner(col, p.start, turns ? p.dim : 0) / 8 : lane;   // the lane that has what these turn with
 
-    for (; r0 < rows; r0 += stride * U) {
-        if (r0 != slice * RPW)
+    auto rotate = [&](const RopeRow<T, VEC>& x, float (&y)[8], float& most) {
+        float w[8];
+        x.values(y);
+        x.partner(w, from, turns);
+        most = 0.0f;
 #pragma unroll
-            for (int n = 0; n < U; ++n) {
-                const int r = r0 + n * stride + sub;
-                x[n].load(source(r), col, on && r < rows, D, p.start, p.dim);
-            }
+        for (int j = 0; j < 8; ++j) {
+            w[j] *= sn[j];
+            if constexpr (PACKED) most = fmaxf(most, fabsf(w[j]));
+            y[j] = fmaf(y[j], cs[j], w[j]);
+        }
+    };
+    // where this lane's codes and (every other lane's) scales of K and V rows lie
+    const int line = in_page & 15;
+    const int64_t rec = static_cast<int64_t>(in_page >> 4) * fp4_record(p.columns);
+    uint8_t* kp = static_cast<uint8_t*>(p.c.k_pages) + page * p.c.k_page_stride + rec + sub * p.c.k_head_stride;
+    uint8_t* vp = static_cast<uint8_t*>(p.c.v_pages) + page * p.c.v_page_stride + rec + sub * p.c.v_head_stride;
+    const int at_codes = line * (p.columns / 2) + col / 2, at_scale = 8 * p.columns + line * (p.columns / 16) + col / 16;
+    auto put4 = [&](uint32_t codes, uint32_t scale, bool is_k, int base) {
+        uint8_t* record = is_k ? kp + base * p.c.k_head_stride : vp + base * p.c.v_head_stride;
+        if (base + sub < G && col < p.columns) {
+            *reinterpret_cast<uint32_t*>(record + at_codes) = codes;
+            if ((col & 8) == 0) record[at_scale] = static_cast<uint8_t>(scale);
+        }
+    };
+    // rows base.. of K or V into their records; true where one has to be done in 64 bits
+    auto store4 = [&](float (&y)[8], float most, bool turned, bool is_k, int base) {
+        const float unit = is_k ? p.k_unit : p.v_unit;
+        if (unit != 1.0f) {
+            most *= unit;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] *= unit;
+        }
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max_magnitude(top, y[j]);
+        // |x c| + |x' s| <= |y| + 2 |x' s|; fp32 values that are exact need the room of r and the product only
+        const float off = turned || !(is_k ? p.k_exact : p.v_exact) || sizeof(T) == 4 ? fmaf(2.0f, most, top) : 0.0f;
+        uint32_t scale;
+        bool open;
+        const uint32_t codes = fp4_block<T>(y, top, off, scale, open);
+        put4(codes, scale, is_k, base);
+        return __any_sync(0xffffffffu, open && base + sub < G) != 0;
+    };
+    for (; u0 < units; u0 += p.slices * U) {
+        if (u0 != slice)
+#pragma unroll
+            for (int n = 0; n < U; ++n) fetch(x[n], u0 + n * p.slices);
         __syncwarp();   // q_out may be q, k_out k: a row is read before it is written over
+        uint32_t again = 0;
 #pragma unroll
         for (int n = 0; n < U; ++n) {
-            const int base = r0 + n * stride, r = base + sub;
-            if (base >= rows) break;
-            const bool is_k = r < G, is_v = !is_k && r < 2 * G, turned = turns && !is_v;
-            float y[8], w[8];
-            x[n].values(y);
-            x[n].partner(w, from);
-            float off[PACKED ? 8 : 1];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                w[j] *= sn[j];
-                if constexpr (PACKED) off[j] = turned ? fmaf(fabsf(y[j]), fabsf(cs[j]), fabsf(w[j])) : fabsf(y[j]);
-                y[j] = turned ? fmaf(y[j], cs[j], w[j]) : y[j];
-            }
-            uint32_t codes = 0, scale = 0;
-            const bool store4 = PACKED && page >= 0 && base < 2 * G;   // a row of the group is one of K or V
-            if constexpr (PACKED) {
-                if (store4) {
-                    const float unit = is_k ? p.k_unit : p.v_unit;
-                    const bool exact = !turned && (is_k ? p.k_exact : p.v_exact);
-                    float z[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        z[j] = y[j] * unit;
-                        off[j] = exact ? 0.0f : off[j] * unit;
-                    }
-                    const RopeSource<T, TT> src{r < 2 * G ? source(r) : nullptr, turned ? cos : nullptr, sin, col, D, p.start, p.dim,
-                                                is_k ? p.k_scale : p.v_scale};
-                    codes = fp4_block<T, TT>(z, off, exact, scale, src);
-                    __syncwarp();   // the rows may be read there
-                }
-            }
-            if (on && r < rows) {
-                if (!placed)   // stored nowhere: q_out and k_out are zeros
+            const int u = u0 + n * p.slices;
+            if (u >= units) break;
+            float y[8], most;
+            if (u >= 2 * uk) {
+                const int row = (u - 2 * uk) * RPW + sub;
+                rotate(x[n], y, most);
+                if (!placed)   // stored nowhere: zeros
 #pragma unroll
                     for (int j = 0; j < 8; ++j) y[j] = 0.0f;
-                if (!is_k && !is_v)
-                    rope_store<T, VEC>(static_cast<T*>(p.q_out) + t * p.qo_row + (r - 2 * G) * p.qo_head, y, col, D);
-                else if (is_k && p.k_out != nullptr)
-                    rope_store<T, VEC>(static_cast<T*>(p.k_out) + t * p.ko_row + r * p.ko_head, y, col, D);
-                if (!PACKED && page >= 0) {
-                    if (is_k)
+                if (on && row < p.heads) rope_store<T, VEC>(static_cast<T*>(p.q_out) + t * p.qo_row + row * p.qo_head, y, col, D);
+            } else if (u < uk) {
+                const int row = u * RPW + sub;
+                rotate(x[n], y, most);
+                if (!placed)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) y[j] = 0.0f;
+                T* out = static_cast<T*>(p.k_out) + t * p.ko_row + row * p.ko_head;
+                if constexpr (PACKED) {
+                    float z[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) z[j] = y[j];
+                    if (page >= 0 && store4(z, most, turns, true, u * RPW)) again |= 1u << n;   // k_out may be k: written then
+                    else if (p.k_out != nullptr && on && row < G) rope_store<T, VEC>(out, y, col, D);
+                } else if (on && row < G) {
+                    if (page >= 0)
                         rope_store<T, VEC>(static_cast<T*>(p.c.k_pages) + page * p.c.k_page_stride + in_page * p.c.k_slot_stride +
-                                               r * p.c.k_head_stride, y, col, D);
-                    else if (is_v)
-                        rope_store<T, VEC>(static_cast<T*>(p.c.v_pages) + page * p.c.v_page_stride + in_page * p.c.v_slot_stride +
-                                               (r - G) * p.c.v_head_stride, y, col, D);
+                                               row * p.c.k_head_stride, y, col, D);
+                    if (p.k_out != nullptr) rope_store<T, VEC>(out, y, col, D);
+                }
+            } else if (page >= 0) {
+                const int row = (u - uk) * RPW + sub;
+                x[n].values(y);
+                if constexpr (PACKED) {
+                    if (store4(y, 0.0f, false, false, (u - uk) * RPW)) again |= 1u << n;
+                } else if (on && row < G) {
+                    rope_store<T, VEC>(static_cast<T*>(p.c.v_pages) + page * p.c.v_page_stride + in_page * p.c.v_slot_stride +
+                                           row * p.c.v_head_stride, y, col, D);
                 }
             }
-            if (store4 && r < 2 * G && col < p.columns) {
-                const int g = is_k ? r : r - G, line = in_page & 15;
-                uint8_t* record = static_cast<uint8_t*>(is_k ? p.c.k_pages : p.c.v_pages) +
-                                  page * (is_k ? p.c.k_page_stride : p.c.v_page_stride) +
-                                  g * (is_k ? p.c.k_head_stride : p.c.v_head_stride) + (in_page >> 4) * fp4_record(p.columns);
-                *reinterpret_cast<uint32_t*>(record + line * (p.columns / 2) + col / 2) = codes;
-                if ((col & 8) == 0) record[8 * p.columns + line * (p.columns / 16) + col / 16] = static_cast<uint8_t>(scale);
+        }
+        if constexpr (PACKED) {
+            while (again != 0u) {   // a warp in some thousand
+                const int u = u0 + (__ffs(again) - 1) * p.slices;
+                again &= again - 1;
+                const bool is_k = u < uk;
+                const int row = (is_k ? u : u - uk) * RPW + sub;
+                const RopeSource<T, TT> src{row < G ? (is_k ? src_k + u * RPW * p.k_head : src_v + (u - uk) * RPW * p.v_head) : nullptr,
+                                            is_k && turns ? cos : nullptr, sin, col, D, p.start, p.dim, is_k ? p.k_scale : p.v_scale};
+                uint32_t scale;
+                const uint32_t codes = fp4_block_exact<T, TT>(src, &scale);
+                put4(codes, scale, is_k, row - sub);
+                if (is_k && p.k_out != nullptr) {
+                    RopeRow<T, VEC> r;
+                    fetch(r, u);
+                    __syncwarp();
+                    float y[8], most;
+                    rotate(r, y, most);
+                    if (on && row < G) rope_store<T, VEC>(static_cast<T*>(p.k_out) + t * p.ko_row + row * p.ko_head, y, col, D);
+                }
             }
         }
     }
@@ -432,81 +484,120 @@ struct PagedGatherParams {
     const int32_t* cu;
     const int32_t* first;
     int max_slots;
+    int block;                  // tokens of a block, up to kGatherTokens
     int32_t* status;
 };
 
-// The 8 values that a stored slot of 4 bits has from column `col` on.
-__device__ __forceinline__ void fp4_load8(const uint8_t* record, int line, int col, int columns, float unit, float (&v)[8]) {
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(record + line * (columns / 2) + col / 2);
-    const float s = fp8_value(record[8 * columns + line * (columns / 16) + col / 16]);
+// The 8 values of codes with their scale.
+__device__ __forceinline__ void fp4_values8(uint32_t codes, uint32_t scale, float unit, float (&v)[8]) {
+    const uint32_t s = fp8_halves(scale | scale << 8);
     uint32_t h[4];
     fp4_halves(codes, h);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+        h[j] = mul_halves(h[j], s);   // 6 bits of at most 2688: exact in halves
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-        v[2 * j] = f.x * s * unit;   // code * scale is exact
-        v[2 * j + 1] = f.y * s * unit;
+        v[2 * j] = f.x;
+        v[2 * j + 1] = f.y;
     }
+    if (unit != 1.0f)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= unit;
+}
+// The 8 values that a stored slot of 4 bits has from column `col` on.
+__device__ __forceinline__ void fp4_load8(const uint8_t* record, int line, int col, int columns, float unit, float (&v)[8]) {
+    fp4_values8(*reinterpret_cast<const uint32_t*>(record + line * (columns / 2) + col / 2),
+                record[8 * columns + line * (columns / 16) + col / 16], unit, v);
 }
 
-// A warp per token, 8 columns per lane; rows that are none are zeros.
+// A block takes p.block consecutive tokens (up to 32): one lane of each warp looks up where a
+// token's slot lies, then the warps take its rows in turn, 8 columns per lane and several
+// rows' loads in flight.  Rows that are none are zeros.  A warp per token left HBM idle for
+// the chain of look-ups (40 us for 19528 tokens of 8 heads of 128).
+constexpr int kGatherTokens = 32;
+
 template <typename T, int LPR, bool VEC, bool PACKED>
 __global__ void __launch_bounds__(kRopeThreads) paged_gather_kernel(const __grid_constant__ PagedGatherParams p) {
-    constexpr int RPW = 32 / LPR, U = 4;
-    const int lane = threadIdx.x & 31;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * kRopeWarps + (threadIdx.x >> 5);
-    if (t >= p.tokens) return;
-    const int b = paged_sequence(p.cu, p.c.batch, t, lane);
-    if (b >= p.c.batch) return;
-    const int64_t i = t - p.cu[b];
-    if (i < 0) return;
-    const int64_t len = min(p.c.lens[b], p.max_slots);
-    const int64_t slot = p.first != nullptr ? p.first[b] + i : p.c.lens[b] - (static_cast<int64_t>(p.cu[b + 1]) - t);
-    int page = -1;
-    if (slot >= 0 && slot < len) page = p.c.page_table[b * p.c.page_table_stride + slot / p.c.page_size];
-    if (page < 0 || page >= p.c.num_pages) {
-        page = -1;
-        if (lane == 0) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
-    }
-    const int in_page = page >= 0 ? static_cast<int>(slot % p.c.page_size) : 0;
+    constexpr int RPW = 32 / LPR, U = sizeof(T) == 2 && VEC ? 4 : 2;
+    __shared__ int64_t s_k[kGatherTokens], s_v[kGatherTokens];   // where the token's slot lies, -1: nowhere, -2: no row
+    __shared__ int s_line[kGatherTokens];
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.block;
     const int G = p.c.kv_heads, D = p.c.head_dim;
     const int sub = lane / LPR, col = lane % LPR * 8;
-    if (col >= D) return;
-    for (int r0 = 0; r0 < 2 * G; r0 += RPW * U) {
-        float x[U][8];
-#pragma unroll
-        for (int n = 0; n < U; ++n) {
-            const int r = r0 + n * RPW + sub;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[n][j] = 0.0f;
-            if (r >= 2 * G || page < 0) continue;
-            const bool is_k = r < G;
-            const int g = is_k ? r : r - G;
-            if constexpr (PACKED) {
-                const uint8_t* record = static_cast<const uint8_t*>(is_k ? p.c.k_pages : p.c.v_pages) +
-                                        page * (is_k ? p.c.k_page_stride : p.c.v_page_stride) +
-                                        g * (is_k ? p.c.k_head_stride : p.c.v_head_stride) + (in_page >> 4) * fp4_record(p.columns);
-                fp4_load8(record, in_page & 15, col, p.columns, is_k ? p.k_scale : p.v_scale, x[n]);
-            } else {
-                const T* row = is_k ? static_cast<const T*>(p.c.k_pages) + page * p.c.k_page_stride + in_page * p.c.k_slot_stride + g * p.c.k_head_stride
-                                    : static_cast<const T*>(p.c.v_pages) + page * p.c.v_page_stride + in_page * p.c.v_slot_stride + g * p.c.v_head_stride;
-                if constexpr (VEC) {
-                    load8<T>(row + col, x[n]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (col + j < D) x[n][j] = to_f32<T>(row[col + j]);
-                }
+    for (int n = warp; n < p.block; n += kRopeWarps) {
+        const int64_t t = t0 + n;
+        int64_t k = -2, v = -2;
+        int line = 0;
+        const int b = t < p.tokens ? paged_sequence(p.cu, p.c.batch, t, lane) : p.c.batch;
+        if (b < p.c.batch && t >= p.cu[b]) {
+            k = v = -1;
+            const int64_t len = min(p.c.lens[b], p.max_slots);
+            const int64_t slot = p.first != nullptr ? p.first[b] + t - p.cu[b] : p.c.lens[b] - (static_cast<int64_t>(p.cu[b + 1]) - t);
+            int page = -1;
+            int in = 0;
+            if (slot >= 0 && slot < len) {
+                const int j = static_cast<int>(slot) / p.c.page_size;
+                in = static_cast<int>(slot) - j * p.c.page_size;
+                page = p.c.page_table[b * p.c.page_table_stride + j];
+            }
+            if (page >= 0 && page < p.c.num_pages) {
+                k = page * p.c.k_page_stride + (PACKED ? static_cast<int64_t>(in >> 4) * fp4_record(p.columns) : in * p.c.k_slot_stride);
+                v = page * p.c.v_page_stride + (PACKED ? static_cast<int64_t>(in >> 4) * fp4_record(p.columns) : in * p.c.v_slot_stride);
+                line = in & 15;
+            } else if (lane == 0) {
+                report_status(p.status, CHRONOS_ERR_INVALID_ARG);
             }
         }
-#pragma unroll
-        for (int n = 0; n < U; ++n) {
-            const int r = r0 + n * RPW + sub;
-            if (r >= 2 * G) continue;
-            T* to = r < G ? static_cast<T*>(p.k) + t * p.k_row + r * p.k_head : static_cast<T*>(p.v) + t * p.v_row + (r - G) * p.v_head;
-            rope_store<T, VEC>(to, x[n], col, D);
+        if (lane == 0) {
+            s_k[n] = k;
+            s_v[n] = v;
+            s_line[n] = line;
         }
     }
+    __syncthreads();
+    if (col >= D) return;
+    // a token's K rows, then its V rows, RPW at a time
+    const int uk = (G + RPW - 1) / RPW;
+    auto rows = [&](int n, bool is_k) {
+        const int64_t at = is_k ? s_k[n] : s_v[n];
+        if (at == -2) return;
+        const int64_t head = is_k ? p.c.k_head_stride : p.c.v_head_stride;
+        const float unit = is_k ? p.k_scale : p.v_scale;
+        T* to = is_k ? static_cast<T*>(p.k) + (t0 + n) * p.k_row + sub * p.k_head : static_cast<T*>(p.v) + (t0 + n) * p.v_row + sub * p.v_head;
+        const int64_t to_head = is_k ? p.k_head : p.v_head;
+        const int line = s_line[n];
+        const uint8_t* record = static_cast<const uint8_t*>(is_k ? p.c.k_pages : p.c.v_pages) + at + sub * head;   // packed
+        const T* row = static_cast<const T*>(is_k ? p.c.k_pages : p.c.v_pages) + at + sub * head;                  // not
+        for (int u0 = 0; u0 < uk; u0 += U) {
+            uint32_t codes[PACKED ? U : 1], scale[PACKED ? U : 1];
+            RopeRow<T, VEC> x[PACKED ? 1 : U];
+#pragma unroll
+            for (int m = 0; m < U; ++m) {
+                const int g = (u0 + m) * RPW;
+                const bool live = at >= 0 && g + sub < G;
+                if constexpr (PACKED) {
+                    codes[m] = scale[m] = 0u;
+                    if (live) {
+                        codes[m] = *reinterpret_cast<const uint32_t*>(record + g * head + line * (p.columns / 2) + col / 2);
+                        scale[m] = record[g * head + 8 * p.columns + line * (p.columns / 16) + col / 16];
+                    }
+                } else {
+                    x[m].load(row + g * head, col, live, D, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < U; ++m) {
+                const int g = (u0 + m) * RPW;
+                if (g + sub >= G) break;
+                float y[8];
+                if constexpr (PACKED) fp4_values8(codes[m], scale[m], unit, y);
+                else x[m].values(y);
+                rope_store<T, VEC>(to + g * to_head, y, col, D);
+            }
+        }
+    };
+    for (int n = warp; n < 2 * p.block; n += kRopeWarps) rows(n >> 1, (n & 1) == 0);
 }
 
 }  // namespace chronos
