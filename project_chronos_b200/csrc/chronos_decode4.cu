@@ -13,6 +13,8 @@ namespace {
 
 // Blocks of 64 slots that a block of a cluster takes at most (see chronos_paged_decode).
 constexpr int kP4ClusterBlocks = 6, kP4ClusterBlocksFull = 8;
+// Tiles of 16 slots that a warp takes of a unit of the work list.
+constexpr int kP4ListTiles = 4;
 
 struct Decode4Plan {
     int dp, parts, grid, cluster, max_vis;
@@ -51,7 +53,8 @@ Decode4Plan decode4_plan(const ChronosPagedDecode4Args* a) {
     d.max_vis = a->window > 0 ? static_cast<int>(std::min<int64_t>(limit, static_cast<int64_t>(a->window) + a->sinks + 32)) : limit;
     const int64_t blocks = (static_cast<int64_t>(d.max_vis) + kPdBlock - 1) / kPdBlock;
     const int64_t rows = static_cast<int64_t>(c.batch) * c.kv_heads * d.parts, room = static_cast<int64_t>(per_sm) * sm_count();
-    d.grid = static_cast<int>(std::min<int64_t>({std::max<int64_t>(1, blocks) * rows, room, kPdMaxGrid}));
+    const int64_t units = std::max<int64_t>(1, (blocks + kP4ListTiles - 1) / kP4ListTiles) * rows;
+    d.grid = static_cast<int>(std::min<int64_t>({units, room, kPdMaxGrid}));
     int size = 1;
     while (size < 8 && size < blocks) size *= 2;
     while (size > 1 && rows * size > room) size /= 2;
@@ -67,17 +70,17 @@ template <typename T, int DP, int NT>
 int launch_decode4(const PagedDecodeParams& p, const Decode4Plan& d, cudaStream_t st) {
     using S = Paged4<T, DP, NT>;
     if (d.cluster > 0) {
-        auto kernel = paged_decode4_kernel<T, DP, NT, true, false>;
+        auto kernel = paged_decode4_kernel<T, DP, NT, 1, true, false>;
         if (int rc = set_smem(kernel, S::kSmem)) return rc;
         CHRONOS_CUDA_CHECK(launch_cluster(kernel, dim3(static_cast<unsigned>(p.c.batch) * p.c.kv_heads * p.parts * d.cluster),
                                           dim3(kPdThreads), S::kSmem, st, d.cluster, p));
         return CHRONOS_OK;
     }
-    auto kernel = paged_decode4_kernel<T, DP, NT, false, false>;
+    auto kernel = paged_decode4_kernel<T, DP, NT, kP4ListTiles, false, false>;
     if (int rc = set_smem(kernel, S::kSmem)) return rc;
     CHRONOS_CUDA_CHECK(launch_kernel(kernel, dim3(p.grid), dim3(kPdThreads), S::kSmem, st, false, p));
     if (p.join_blocks > 0)   // rows of one unit are never cut: then there is nothing to join
-        CHRONOS_CUDA_CHECK(launch_kernel(paged_join_kernel<T>, dim3(static_cast<unsigned>(p.join_blocks)), dim3(kPdJoinThreads), 0, st, true, p));
+        CHRONOS_CUDA_CHECK(launch_kernel(paged_join_kernel<T, kP4ListTiles * kPdBlock>, dim3(static_cast<unsigned>(p.join_blocks)), dim3(kPdJoinThreads), 0, st, true, p));
     return CHRONOS_OK;
 }
 template <typename T>
@@ -139,7 +142,7 @@ extern "C" int chronos_paged_decode4(const ChronosPagedDecode4Args* a, void* str
     p.part_stride = d.dp;
     p.part_o = reinterpret_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float*>(ws + d.o_part_ml);
-    p.join_blocks = d.max_vis > kPdBlock ? a->cache.batch * a->heads : 0;
+    p.join_blocks = d.max_vis > kP4ListTiles * kPdBlock ? a->cache.batch * a->heads : 0;
     p.status = a->status;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (a->cache.dtype) {

@@ -33,7 +33,7 @@ int launch_sparse_kernel(K kernel, int smem, int per_sm, PagedDecodeParams p, in
 template <typename T, int DP, int NT>
 int launch_sparse4(const PagedDecodeParams& p, int64_t tokens, cudaStream_t st) {
     using S = Paged4<T, DP, NT>;
-    return launch_sparse_kernel(paged_decode4_kernel<T, DP, NT, true, true>, S::kSmem, S::kBlocksPerSm, p, tokens, st);
+    return launch_sparse_kernel(paged_decode4_kernel<T, DP, NT, 1, true, true>, S::kSmem, S::kBlocksPerSm, p, tokens, st);
 }
 template <typename T>
 int launch_sparse4(const PagedDecodeParams& p, int dp, int64_t tokens, cudaStream_t st) {

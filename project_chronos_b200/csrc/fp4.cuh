@@ -56,6 +56,29 @@ __device__ __forceinline__ uint32_t mul_halves(uint32_t a, uint32_t b) {
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
+// Halves of one operand twice (an operand of the multiplication itself, no instruction of its
+// own): a * (s.low, s.low), a * (s.high, s.high).
+__device__ __forceinline__ uint32_t mul_low(uint32_t a, uint32_t s) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 l, h;\n\t.reg .b32 t;\n\tmov.b32 {l, h}, %2;\n\tmov.b32 t, {l, l};\n\tmul.rn.f16x2 %0, %1, t;\n\t}" : "=r"(r) : "r"(a), "r"(s));
+    return r;
+}
+__device__ __forceinline__ uint32_t mul_high(uint32_t a, uint32_t s) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 l, h;\n\t.reg .b32 t;\n\tmov.b32 {l, h}, %2;\n\tmov.b32 t, {h, h};\n\tmul.rn.f16x2 %0, %1, t;\n\t}" : "=r"(r) : "r"(a), "r"(s));
+    return r;
+}
+// (a.low * s.low, b.low * t.high) and (a.high * s.low, b.high * t.high) for s = (s, 0), t = (0, t).
+__device__ __forceinline__ void pair_scaled(uint32_t a, uint32_t b, uint32_t s, uint32_t t, uint32_t& low, uint32_t& high) {
+    asm("{\n\t.reg .b16 al, ah, bl, bh;\n\t.reg .b32 x, y, z;\n\t"
+        "mov.b32 {al, ah}, %2;\n\tmov.b32 {bl, bh}, %3;\n\t"
+        "mov.b32 x, {al, al};\n\tmov.b32 y, {bl, bl};\n\t"
+        "mul.rn.f16x2 z, x, %4;\n\tfma.rn.f16x2 %0, y, %5, z;\n\t"
+        "mov.b32 x, {ah, ah};\n\tmov.b32 y, {bh, bh};\n\t"
+        "mul.rn.f16x2 z, x, %4;\n\tfma.rn.f16x2 %1, y, %5, z;\n\t}"
+        : "=&r"(low), "=&r"(high)
+        : "r"(a), "r"(b), "r"(s), "r"(t));
+}
 constexpr uint32_t kFp8Nan = 0x7fu;
 // max(a, |b|), NaN where one of the two is.
 __device__ __forceinline__ float max_magnitude(float a, float b) {

@@ -95,6 +95,7 @@ struct PagedRow {
         return (ones_below(first - slot0) | (ones_below(len - slot0) & ~ones_below(lo - slot0))) & 0xffffu;
     }
 };
+template <int BLOCK = kPdBlock>   // places of a unit
 __device__ __forceinline__ PagedRow paged_row(const PagedDecodeParams& p, int b) {
     PagedRow r;
     r.len = min(max(p.c.lens[b], 0), p.max_slots);
@@ -103,7 +104,7 @@ __device__ __forceinline__ PagedRow paged_row(const PagedDecodeParams& p, int b)
     r.front = (r.first + 15) & ~15;
     r.skip = max(0, (r.lo & ~15) - r.front);
     r.n = r.len - r.skip;
-    r.nblk = max(1, (r.n + kPdBlock - 1) / kPdBlock);   // an empty row still has its zeros written
+    r.nblk = max(1, (r.n + BLOCK - 1) / BLOCK);   // an empty row still has its zeros written
     return r;
 }
 
@@ -111,6 +112,7 @@ __device__ __forceinline__ PagedRow paged_row(const PagedDecodeParams& p, int b)
 struct PagedIter {
     int u, b, v, blk;
     PagedRow r;
+    template <int BLOCK = kPdBlock>
     __device__ __forceinline__ void advance(const PagedDecodeParams& p, int end) {
         ++u;
         if (++blk < r.nblk) return;
@@ -118,7 +120,7 @@ struct PagedIter {
         if (++v < p.c.kv_heads * p.parts) return;
         v = 0;
         ++b;
-        if (u < end) r = paged_row(p, b);
+        if (u < end) r = paged_row<BLOCK>(p, b);
     }
 };
 
@@ -129,9 +131,10 @@ __device__ __forceinline__ void paged_check_lens(const PagedDecodeParams& p) {
 }
 
 // Number of units of all sequences (every lane of a warp gets it).
+template <int BLOCK = kPdBlock>
 __device__ __forceinline__ int paged_total(const PagedDecodeParams& p, int lane) {
     int s = 0;
-    for (int b = lane; b < p.c.batch; b += 32) s += paged_row(p, b).nblk;
+    for (int b = lane; b < p.c.batch; b += 32) s += paged_row<BLOCK>(p, b).nblk;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s * p.c.kv_heads * p.parts;
@@ -141,13 +144,15 @@ __device__ __forceinline__ int paged_share(const PagedDecodeParams& p, int total
     return max(1, (total + p.grid - 1) / p.grid);
 }
 // First unit of sequence b / the sequence that holds unit u (whole warps call these).
+template <int BLOCK = kPdBlock>
 __device__ __forceinline__ int paged_first_unit(const PagedDecodeParams& p, int b, int lane) {
     int s = 0;
-    for (int i = lane; i < b; i += 32) s += paged_row(p, i).nblk;
+    for (int i = lane; i < b; i += 32) s += paged_row<BLOCK>(p, i).nblk;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s * p.c.kv_heads * p.parts;
 }
+template <int BLOCK = kPdBlock>
 __device__ __forceinline__ PagedIter paged_seek(const PagedDecodeParams& p, int u, int lane) {
     const int per = p.c.kv_heads * p.parts;
     PagedIter it{};
@@ -155,7 +160,7 @@ __device__ __forceinline__ PagedIter paged_seek(const PagedDecodeParams& p, int 
     int before = 0;
     for (int base = 0; base < p.c.batch; base += 32) {
         const int b = base + lane;
-        const int n = b < p.c.batch ? paged_row(p, b).nblk * per : 0;
+        const int n = b < p.c.batch ? paged_row<BLOCK>(p, b).nblk * per : 0;
         int inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -167,7 +172,7 @@ __device__ __forceinline__ PagedIter paged_seek(const PagedDecodeParams& p, int 
             const int l = __ffs(past) - 1;
             const int start = before + __shfl_sync(0xffffffffu, inc - n, l);
             it.b = base + l;
-            it.r = paged_row(p, it.b);
+            it.r = paged_row<BLOCK>(p, it.b);
             it.v = (u - start) / it.r.nblk;
             it.blk = (u - start) % it.r.nblk;
             return it;
@@ -214,11 +219,9 @@ struct PagedLook {
     uint32_t vis;
 };
 template <bool ONE_PAGE>
-__device__ __forceinline__ PagedLook paged_look(const PagedDecodeParams& p, const PagedIter& it, int end, int warp,
-                                                int lane) {
+__device__ __forceinline__ PagedLook paged_look_place(const PagedDecodeParams& p, const PagedIter& it, bool live, int place, int lane) {
     PagedLook k{-1, 0, 0u};
-    const int place = it.blk * kPdBlock + warp * kPdTile;
-    if (it.u < end && place < it.r.n) {
+    if (live && place < it.r.n) {
         const int slot0 = it.r.slot(place);
         k.vis = it.r.visible16(slot0);
         const bool mine = ONE_PAGE || (k.vis >> (lane & 15)) & 1u;
@@ -234,10 +237,16 @@ __device__ __forceinline__ PagedLook paged_look(const PagedDecodeParams& p, cons
     }
     return k;
 }
+template <bool ONE_PAGE>
+__device__ __forceinline__ PagedLook paged_look(const PagedDecodeParams& p, const PagedIter& it, int end, int warp,
+                                                int lane) {
+    return paged_look_place<ONE_PAGE>(p, it, it.u < end, it.blk * kPdBlock + warp * kPdTile, lane);
+}
 
 // Selected pages.  Token t sees the slots below `len` that lie in its pages; the places are
 // the slots of the list's entries, one page after the other.  seq = -1: a token behind the
 // last sequence.  Whole warps call it.
+template <int BLOCK = kPdBlock>
 __device__ __forceinline__ PagedRow paged_row_sel(const PagedDecodeParams& p, int t, int lane) {
     PagedRow r{};
     r.seq = p.cu == nullptr ? t : paged_sequence(p.cu, p.c.batch, t, lane);
@@ -250,14 +259,14 @@ __device__ __forceinline__ PagedRow paged_row_sel(const PagedDecodeParams& p, in
     r.len = min(max(raw, 0), p.max_slots) - (p.cu == nullptr ? 0 : p.cu[r.seq + 1] - 1 - t);
     r.len = max(r.len, 0);
     r.n = p.topk * p.c.page_size;
-    r.nblk = max(1, (r.n + kPdBlock - 1) / kPdBlock);
+    r.nblk = max(1, (r.n + BLOCK - 1) / BLOCK);
     return r;
 }
 template <bool ONE_PAGE>
-__device__ __forceinline__ PagedLook paged_look_sel(const PagedDecodeParams& p, const PagedIter& it, int end, int warp, int lane) {
+__device__ __forceinline__ PagedLook paged_look_sel(const PagedDecodeParams& p, const PagedIter& it, bool live, int place, int lane) {
     PagedLook k{-1, 0, 0u};
-    const int place = it.blk * kPdBlock + warp * kPdTile + (ONE_PAGE ? 0 : lane & 15);
-    if (it.u < end && place < it.r.n) {
+    if (!ONE_PAGE) place += lane & 15;
+    if (live && place < it.r.n) {
         int i;
         paged_split(p, place, i, k.slot);
         const int64_t head = static_cast<int64_t>(it.b) * p.c.kv_heads + it.v / p.parts;
@@ -278,7 +287,7 @@ __device__ __forceinline__ PagedLook paged_look_sel(const PagedDecodeParams& p, 
 }
 template <bool SEL, bool ONE_PAGE>
 __device__ __forceinline__ PagedLook paged_look_at(const PagedDecodeParams& p, const PagedIter& it, int end, int warp, int lane) {
-    if constexpr (SEL) return paged_look_sel<ONE_PAGE>(p, it, end, warp, lane);
+    if constexpr (SEL) return paged_look_sel<ONE_PAGE>(p, it, it.u < end, it.blk * kPdBlock + warp * kPdTile, lane);
     else return paged_look<ONE_PAGE>(p, it, end, warp, lane);
 }
 
@@ -1124,14 +1133,15 @@ struct PagedParts {
     int c0, c1;
     __device__ __forceinline__ int64_t part(int c) const { return 2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0); }
 };
+template <int BLOCK>
 __device__ __forceinline__ PagedParts paged_parts(const PagedDecodeParams& p, int b, int v, int lane) {
-    const int share = paged_share(p, paged_total(p, lane));
-    const int nblk = paged_row(p, b).nblk;
-    const int s = paged_first_unit(p, b, lane) + v * nblk;
+    const int share = paged_share(p, paged_total<BLOCK>(p, lane));
+    const int nblk = paged_row<BLOCK>(p, b).nblk;
+    const int s = paged_first_unit<BLOCK>(p, b, lane) + v * nblk;
     return PagedParts{s / share, (s + nblk - 1) / share};
 }
 
-template <typename T>
+template <typename T, int BLOCK = kPdBlock>
 __global__ void __launch_bounds__(kPdJoinThreads) paged_join_kernel(const __grid_constant__ PagedDecodeParams p) {
     constexpr int W = kPdJoinThreads / 32;
     __shared__ float s_w[kPdMaxGrid];
@@ -1143,7 +1153,7 @@ __global__ void __launch_bounds__(kPdJoinThreads) paged_join_kernel(const __grid
     if (static_cast<int>(blockIdx.x) < p.join_blocks) {
         const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
         const int kvh = head / p.rep, hr = head % p.rep;
-        const PagedParts pp = paged_parts(p, b, kvh * p.parts + hr / p.rows, lane);
+        const PagedParts pp = paged_parts<BLOCK>(p, b, kvh * p.parts + hr / p.rows, lane);
         if (pp.c0 == pp.c1) return;   // one block finished the row
         const int n = pp.c1 - pp.c0 + 1, row = hr % p.rows;
         float M = -INFINITY;
@@ -1215,7 +1225,7 @@ __global__ void __launch_bounds__(kPdJoinThreads) paged_join_kernel(const __grid
     if (chunk * kPdWeightSlots >= r.len) return;
     const int64_t hb = static_cast<int64_t>(b) * p.heads + g * p.rep;
     for (int h = warp; h < p.rep; h += W) {
-        const PagedParts pp = paged_parts(p, b, g * p.parts + h / p.rows, lane);
+        const PagedParts pp = paged_parts<BLOCK>(p, b, g * p.parts + h / p.rows, lane);
         float lg;
         if (pp.c0 == pp.c1) {
             lg = p.lse2[hb + h];

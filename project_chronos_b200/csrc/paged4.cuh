@@ -25,7 +25,7 @@ struct Paged4 {
     static constexpr int kStageBytes = kPdWarps * 2 * kRecord;
     static constexpr int kOStride = DP + 4;
     static constexpr int kMergeBytes = kPdWarps * 8 * kOStride * 4;
-    static constexpr int kSmem = kStages * kStageBytes + kMergeBytes + kPdWarps * 16 * 4 + kStages * kPdWarps * 4;
+    static constexpr int kSmem = kStages * kStageBytes + kMergeBytes + kPdWarps * 16 * 4;
     static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;      // halves that a query or weight is split into
     static constexpr int kBlocksPerSm = DP == 256 || (DP == 128 && NT * kTerms > 2) ? 2 : DP == 128 && NT * kTerms > 1 ? 3 : 4;
     static constexpr int kPartBytes = (16 * DP + 32) * 4;      // what a cluster's block leaves for the join
@@ -52,366 +52,443 @@ __device__ __forceinline__ void paged4_halves(float a, float b, uint32_t (&r)[TE
 // 2^-14 of the largest), weights of up to 2^15.  fp32 layers split queries and weights
 // into two halves each (22 bits).  The order of the columns inside a product is free: a
 // lane takes a contiguous quarter of a K slot and a contiguous eighth of a V slot, so a
-// tile's codes are read by one wide load per slot.  V's halves come in pairs of columns and
-// are paired by slots with one byte permutation each.
-template <typename T, int DP, int NT, bool CL, bool SEL>
+// tile's codes are read by one wide load per slot.  V's halves come in pairs of columns; the
+// multiplications by two slots' scales pair them by slots.
+//
+// A warp takes TILES tiles of 16 slots of a unit (4 * TILES tiles), one after the other; its lanes
+// look up the pages of a unit's tiles at once, a unit ahead.
+template <typename T, int DP, int NT, int TILES, bool CL, bool SEL>
 __global__ void __launch_bounds__(kPdThreads, Paged4<T, DP, NT>::kBlocksPerSm) paged_decode4_kernel(
     const __grid_constant__ PagedDecodeParams p) {
     using S = Paged4<T, DP, NT>;
-    constexpr int NS = S::kStages, RB = S::kSlotBytes, REC = S::kRecord, TERMS = S::kTerms;
-    constexpr int PIECES = 2 * REC / 16, PER = (PIECES + 31) / 32;   // 16-byte copies of a tile, per lane
+    constexpr int NS = S::kStages, RB = S::kSlotBytes, REC = S::kRecord, TERMS = S::kTerms, BLOCK = TILES * kPdBlock;
     constexpr int KW = DP / 32, VW = DP / 64;                        // words of 8 codes per slot and lane
     constexpr float kGrow = 8.0f, kLift = 7.0f;                      // see WeightLift
     static_assert(!SEL || CL, "selected pages: a cluster per row");
     extern __shared__ __align__(128) uint8_t smem[];
     float* s_o = reinterpret_cast<float*>(smem + NS * S::kStageBytes);   // [warp][8 heads][kOStride]
     float* s_ml = s_o + S::kMergeBytes / 4;                              // [warp][8][2]
-    uint32_t* s_vis = reinterpret_cast<uint32_t*>(s_ml + kPdWarps * 16); // [stage][warp]
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int quad = lane >> 2, qc = lane & 3;
 
     int end;
-    PagedIter ld;
+    PagedIter pf;   // the unit that is looked up next
     const int rank = CL ? static_cast<int>(blockIdx.x) % p.cluster : 0;
     if constexpr (CL) {
         const int row = blockIdx.x / p.cluster, per = p.c.kv_heads * p.parts;
-        ld.u = 0;
-        ld.b = row / per;
-        ld.v = row % per;
-        ld.blk = rank;
+        pf.u = 0;
+        pf.b = row / per;
+        pf.v = row % per;
+        pf.blk = rank;
         if constexpr (SEL) {
-            ld.r = paged_row_sel(p, ld.b, lane);
-            if (ld.r.seq < 0) return;
+            pf.r = paged_row_sel<BLOCK>(p, pf.b, lane);
+            if (pf.r.seq < 0) return;
         } else {
-            ld.r = paged_row(p, ld.b);
+            pf.r = paged_row<BLOCK>(p, pf.b);
         }
-        end = ld.r.nblk > rank ? (ld.r.nblk - rank + p.cluster - 1) / p.cluster : 0;
+        end = pf.r.nblk > rank ? (pf.r.nblk - rank + p.cluster - 1) / p.cluster : 0;
         if (!SEL && blockIdx.x == 0) paged_check_lens(p);
     } else {
-        const int total = paged_total(p, lane);
+        const int total = paged_total<BLOCK>(p, lane);
         const int share = paged_share(p, total);
         const int begin = static_cast<int>(blockIdx.x) * share;
         end = min(total, begin + share);
         if (blockIdx.x == 0) paged_check_lens(p);
         if (begin >= end) return;
-        ld = paged_seek(p, begin, lane);
+        pf = paged_seek<BLOCK>(p, begin, lane);
     }
     auto advance = [&](PagedIter& it) {
         if constexpr (CL) {
             ++it.u;
             it.blk += p.cluster;
         } else {
-            it.advance(p, end);
+            it.template advance<BLOCK>(p, end);
         }
     };
-    PagedIter cp = ld;
-    PagedLook look = paged_look_at<SEL, true>(p, ld, end, warp, lane);
+    auto kv_head = [&](int v) { return p.parts == 1 ? v : v / p.parts; };
+    // lane j (and j + TILES, ...) has tile j of the unit
+    auto look_up = [&]() {
+        const int place = pf.blk * BLOCK + (warp * TILES + (lane & (TILES - 1))) * kPdTile;
+        if constexpr (SEL) return paged_look_sel<true>(p, pf, pf.u < end, place, lane);
+        else return paged_look_place<true>(p, pf, pf.u < end, place, lane);
+    };
+    PagedIter cp = pf;
+    PagedLook look = look_up();
+    int head = kv_head(pf.v), left = end - pf.u;   // the unit that is being copied, units left
+    advance(pf);
+    PagedLook ahead = look_up();
+    int head_ahead = kv_head(pf.v);
 
-    // a tile: K's record, V's record, as they lie in the pages but for the turned pieces
-    uint32_t to[PER];
+    // a tile: K's record, V's record, as they lie in the pages but for the turned pieces: codes
+    // (CODES pieces of 16 bytes each) by all lanes, both scales (DP / 16 pieces each) by DP / 8 lanes
+    constexpr int CODES = DP / 2, SCALES = DP / 16;
+    const uint32_t ring = smem_u32(smem) + warp * 2 * REC;
+    uint32_t to[CODES / 32];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int n = lane + 32 * i, c = n < REC / 16 ? n : n - REC / 16;
-        const int slot = c / (RB / 16), piece = c % (RB / 16);
-        to[i] = static_cast<uint32_t>((n - c) * 16 + (c < RB ? slot * RB + ((piece ^ paged4_turn<DP>(slot)) << 4) : c * 16));
+    for (int i = 0; i < CODES / 32; ++i) {
+        const int n = lane + 32 * i, slot = n / (RB / 16), piece = n % (RB / 16);
+        to[i] = ring + static_cast<uint32_t>(slot * RB + ((piece ^ paged4_turn<DP>(slot)) << 4));
     }
-    auto issue = [&](int stage) {
-        uint32_t vis = look.vis;
-        if (look.page < 0) vis = 0u;
-        if (vis) {
-            const int64_t g = ld.v / p.parts, at = static_cast<int64_t>(look.slot >> 4) * REC;
-            const uint8_t* k = static_cast<const uint8_t*>(p.c.k_pages) + look.page * p.c.k_page_stride + g * p.c.k_head_stride + at;
-            const uint8_t* v = static_cast<const uint8_t*>(p.c.v_pages) + look.page * p.c.v_page_stride + g * p.c.v_head_stride + at;
-            const uint32_t st = smem_u32(smem + stage * S::kStageBytes + warp * 2 * REC);
+    const bool of_v = (lane & (SCALES - 1)) != lane;   // the scales of V
+    const uint32_t to_scale = ring + static_cast<uint32_t>((of_v ? REC : 0) + 16 * (CODES + (lane & (SCALES - 1))));
+    const uint8_t *k_row = nullptr, *v_row = nullptr;
+    auto row_pointers = [&]() {
+        k_row = static_cast<const uint8_t*>(p.c.k_pages) + head * p.c.k_head_stride + lane * 16;
+        v_row = static_cast<const uint8_t*>(p.c.v_pages) + head * p.c.v_head_stride + lane * 16;
+    };
+    row_pointers();
+    uint32_t shows[NS];   // which slots of the tile in a stage are visible
+    // Copies tile `tile` of the unit `look` is of into a stage (both known at compile time).
+    auto issue = [&](int stage, int tile) {
+        shows[stage] = 0u;
+        if (left > 0) {
+            int page = look.page;
+            uint32_t at = static_cast<uint32_t>(look.slot >> 4) * REC, vis = look.vis;   // of a page: 32 bits
+            if constexpr (TILES > 1) {
+                page = __shfl_sync(0xffffffffu, page, tile);
+                at = __shfl_sync(0xffffffffu, at, tile);
+                vis = __shfl_sync(0xffffffffu, vis, tile);
+            }
+            if (page >= 0 && vis != 0u) {
+                shows[stage] = vis;
+                // page strides fit 32 bits (the host sees to it): one multiplication per pointer
+                const uint8_t* k = k_row + static_cast<uint64_t>(static_cast<uint32_t>(page)) * static_cast<uint32_t>(p.c.k_page_stride) + at;
+                const uint8_t* v = v_row + static_cast<uint64_t>(static_cast<uint32_t>(page)) * static_cast<uint32_t>(p.c.v_page_stride) + at;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int n = lane + 32 * i;
-                if (n < PIECES) cp_async16(st + to[i], n < REC / 16 ? k + n * 16 : v + (n * 16 - REC), true);
+                for (int i = 0; i < CODES / 32; ++i) {
+                    cp_async16(to[i] + stage * S::kStageBytes, k + i * 512, true);
+                    cp_async16(to[i] + stage * S::kStageBytes + REC, v + i * 512, true);
+                }
+                const uint8_t* s = of_v ? v - SCALES * 16 : k;
+                if (lane < 2 * SCALES) cp_async16(to_scale + stage * S::kStageBytes, s + CODES * 16, true);
+            }
+            if (tile == TILES - 1) {   // on to the next unit
+                --left;
+                look = ahead;
+                if (head != head_ahead) {
+                    head = head_ahead;
+                    row_pointers();
+                }
+                advance(pf);
+                ahead = look_up();
+                head_ahead = kv_head(pf.v);
             }
         }
-        if (lane == 0) s_vis[stage * kPdWarps + warp] = vis;
+        cp_async_commit();
     };
 #pragma unroll
-    for (int s = 0; s < NS - 1; ++s) {
-        if (ld.u < end) {
-            issue(s);
-            advance(ld);
-            look = paged_look_at<SEL, true>(p, ld, end, warp, lane);
-        }
-        cp_async_commit();
-    }
+    for (int s = 0; s < NS - 1; ++s) issue(s, s % TILES);
 
     const int kslot = paged4_place(quad);            // and 8 on
     const int v0 = paged4_place(2 * qc), v1 = paged4_place(2 * qc + 1);
     uint32_t qb[NT][DP / 16][2][TERMS];
-    float unit[NT][2];          // of the scores of heads 2 qc and 2 qc + 1
+    float unit[NT][2];               // of the scores of heads 2 qc and 2 qc + 1
     float o[NT][DP / 16][4];
-    float m[NT][2], l[NT][2];
-    bool fresh = true;          // the next unit opens a new part or row
-    int part_blk = 0;           // the block it opened with
-    int stage = 0;
-    while (cp.u < end || (CL && fresh)) {
-        const int kvh = cp.v / p.parts, h0 = (cp.v % p.parts) * 16;
-        const int nh = min(16, p.rep - h0);          // query heads of this unit
-        if (fresh) {
-            fresh = false;
-            part_blk = cp.blk;
-            const T* q = static_cast<const T*>(p.q) + cp.b * p.q_row + static_cast<int64_t>(kvh * p.rep + h0) * p.q_head;
+    float base[NT][2], l[NT][2];     // what is taken off the scores: the maximum as it lags, less kLift
+    const uint8_t* mine = smem + warp * 2 * REC;
+
+    // A row's (or part's) beginning: kv head kvh, query heads from h0 on.
+    auto open_row = [&](int kvh, int h0, int nh) {
+        const T* q = static_cast<const T*>(p.q) + cp.b * p.q_row + static_cast<int64_t>(kvh * p.rep + h0) * p.q_head;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                m[t][0] = m[t][1] = -INFINITY;
-                l[t][0] = l[t][1] = 0.0f;
+        for (int t = 0; t < NT; ++t) {
+            base[t][0] = base[t][1] = -INFINITY;
+            l[t][0] = l[t][1] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < DP / 16; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.0f;
-                // a head's columns in units of a power of two: the largest is 2^8 to 2^9
-                const int row = t * 8 + quad;
-                const T* head = q + row * p.q_head + qc * (DP / 4);
-                const bool on = row < nh;
-                uint32_t top = 0;
+            for (int i = 0; i < DP / 16; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.0f;
+            // a head's columns in units of a power of two: the largest is 2^8 to 2^9
+            const int row = t * 8 + quad;
+            const T* head = q + row * p.q_head + qc * (DP / 4);
+            const bool on = row < nh;
+            uint32_t top = 0;
 #pragma unroll
-                for (int d = 0; d < DP / 4; ++d)
-                    if (on && qc * (DP / 4) + d < p.c.head_dim) top = max(top, __float_as_uint(to_f32<T>(head[d])) & 0x7fffffffu);
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int k = min(max(8 - (static_cast<int>(top >> 23) - 127), -110), 110);
-                const float up = __uint_as_float(static_cast<uint32_t>(127 + k) << 23), down = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+            for (int d = 0; d < DP / 4; ++d)
+                if (on && qc * (DP / 4) + d < p.c.head_dim) top = max(top, __float_as_uint(to_f32<T>(head[d])) & 0x7fffffffu);
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int k = min(max(8 - (static_cast<int>(top >> 23) - 127), -110), 110);
+            const float up = __uint_as_float(static_cast<uint32_t>(127 + k) << 23), down = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
 #pragma unroll
-                for (int i = 0; i < DP / 16; ++i)
+            for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int d = i * 4 + j * 2, c = qc * (DP / 4) + d;
-                        const float a = on && c < p.c.head_dim ? to_f32<T>(head[d]) * up : 0.0f;
-                        const float b = on && c + 1 < p.c.head_dim ? to_f32<T>(head[d + 1]) * up : 0.0f;
-                        paged4_halves<TERMS>(a, b, qb[t][i][j]);
+                for (int j = 0; j < 2; ++j) {
+                    const int d = i * 4 + j * 2, c = qc * (DP / 4) + d;
+                    const float a = on && c < p.c.head_dim ? to_f32<T>(head[d]) * up : 0.0f;
+                    const float b = on && c + 1 < p.c.head_dim ? to_f32<T>(head[d + 1]) * up : 0.0f;
+                    paged4_halves<TERMS>(a, b, qb[t][i][j]);
+                }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) unit[t][j] = p.sl2 * __shfl_sync(0xffffffffu, down, (2 * qc + j) * 4);
+        }
+    };
+
+    // The tile in a stage (known at compile time).
+    auto take = [&](int stage) {
+        const uint32_t vis = shows[stage];
+        if (vis == 0u) return;
+        const uint8_t* st = mine + stage * S::kStageBytes;
+        float s[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+        {
+            // this lane's quarter of slots kslot and kslot + 8
+            uint32_t w[2][KW], two[2][(KW + 3) / 4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const uint8_t* slot = st + (kslot + 8 * r) * RB;
+                const uint8_t* scales = st + 16 * RB + (kslot + 8 * r) * (DP / 16);
+                if constexpr (DP == 64) {
+                    const uint2 x = *reinterpret_cast<const uint2*>(slot + qc * 8);
+                    w[r][0] = x.x; w[r][1] = x.y;
+                    two[r][0] = fp8_halves(scales[qc]);
+                } else if constexpr (DP == 128) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(slot + ((qc ^ paged4_turn<DP>(kslot)) << 4));
+                    w[r][0] = x.x; w[r][1] = x.y; w[r][2] = x.z; w[r][3] = x.w;
+                    two[r][0] = fp8_halves(*reinterpret_cast<const uint16_t*>(scales + qc * 2));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(slot + (((2 * qc + i) ^ paged4_turn<DP>(kslot)) << 4));
+                        w[r][4 * i] = x.x; w[r][4 * i + 1] = x.y; w[r][4 * i + 2] = x.z; w[r][4 * i + 3] = x.w;
                     }
-#pragma unroll
-                for (int j = 0; j < 2; ++j) unit[t][j] = p.sl2 * __shfl_sync(0xffffffffu, down, (2 * qc + j) * 4);
+                    const uint32_t sc = *reinterpret_cast<const uint32_t*>(scales + qc * 4);
+                    two[r][0] = fp8_halves(sc);
+                    two[r][1] = fp8_halves(sc >> 16);
+                }
             }
-        }
-        if (ld.u < end) {
-            issue(stage == 0 ? NS - 1 : stage - 1);
-            advance(ld);
-            look = paged_look_at<SEL, true>(p, ld, end, warp, lane);
-        }
-        cp_async_commit();
-        cp_async_wait<NS - 1>();
-        __syncwarp();
-        const uint8_t* st = smem + stage * S::kStageBytes + warp * 2 * REC;
-        const uint32_t vis = cp.u < end ? s_vis[stage * kPdWarps + warp] : 0u;
-        if (vis) {
-            float s[NT][4];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
-            {
-                // this lane's quarter of slots kslot and kslot + 8
-                uint32_t w[2][KW], sc[2];
+            for (int i = 0; i < KW; ++i) {   // 8 columns of both slots: two pieces of 16 in the product's order
+                uint32_t x[2][4];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const uint8_t* slot = st + (kslot + 8 * r) * RB;
-                    const uint8_t* scales = st + 16 * RB + (kslot + 8 * r) * (DP / 16);
-                    if constexpr (DP == 64) {
-                        const uint2 x = *reinterpret_cast<const uint2*>(slot + qc * 8);
-                        w[r][0] = x.x; w[r][1] = x.y;
-                        sc[r] = scales[qc];
-                    } else if constexpr (DP == 128) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(slot + ((qc ^ paged4_turn<DP>(kslot)) << 4));
-                        w[r][0] = x.x; w[r][1] = x.y; w[r][2] = x.z; w[r][3] = x.w;
-                        sc[r] = *reinterpret_cast<const uint16_t*>(scales + qc * 2);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint4 x = *reinterpret_cast<const uint4*>(slot + (((2 * qc + i) ^ paged4_turn<DP>(kslot)) << 4));
-                            w[r][4 * i] = x.x; w[r][4 * i + 1] = x.y; w[r][4 * i + 2] = x.z; w[r][4 * i + 3] = x.w;
-                        }
-                        sc[r] = *reinterpret_cast<const uint32_t*>(scales + qc * 4);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < KW; ++i) {   // 8 columns of both slots: two pieces of 16 in the product's order
-                    uint32_t x[2][4];
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        fp4_halves(w[r][i], x[r]);
-                        const uint32_t two = fp8_halves(sc[r] >> (16 * (i / 4)));
-                        const uint32_t one = __byte_perm(two, two, (i / 2) % 2 == 0 ? 0x1010 : 0x3232);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) x[r][j] = mul_halves(x[r][j], one);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const uint32_t a[4] = {x[0][2 * j], x[1][2 * j], x[0][2 * j + 1], x[1][2 * j + 1]};
-#pragma unroll
-                        for (int t = 0; t < NT; ++t)
-#pragma unroll
-                            for (int e = TERMS - 1; e >= 0; --e)
-                                mma_16816<__half>(s[t], a, qb[t][2 * i + j][0][e], qb[t][2 * i + j][1][e]);
-                    }
-                }
-            }
-            // s[t][0..1]: slot kslot, heads 8t + 2qc, + 1; s[t][2..3]: slot kslot + 8
-            const bool on0 = (vis >> kslot) & 1u, on1 = (vis >> (kslot + 8)) & 1u;
-            bool grow = false;
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s[t][j] = (j < 2 ? on0 : on1) ? s[t][j] * unit[t][j & 1] : -INFINITY;
-                    grow |= s[t][j] > m[t][j & 1] + kGrow;
-                }
-            if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float n = fmaxf(s[t][j], s[t][2 + j]);
-#pragma unroll
-                        for (int x = 4; x < 32; x <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, x));
-                        n = fmaxf(n, m[t][j]);
-                        const float c = n == -INFINITY ? 1.0f : exp2_fast(m[t][j] - n);
-                        m[t][j] = n;
-                        l[t][j] *= c;
-#pragma unroll
-                        for (int i = 0; i < DP / 16; ++i) {
-                            o[t][i][j] *= c;
-                            o[t][i][2 + j] *= c;
-                        }
-                    }
-            }
-            uint32_t pb[NT][2][TERMS];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const float u0 = m[t][0] == -INFINITY ? 0.0f : m[t][0] - kLift, u1 = m[t][1] == -INFINITY ? 0.0f : m[t][1] - kLift;
-                const float a = exp2_fast(s[t][0] - u0), b = exp2_fast(s[t][1] - u1);
-                const float c = exp2_fast(s[t][2] - u0), d = exp2_fast(s[t][3] - u1);
-                l[t][0] += a + c;
-                l[t][1] += b + d;
-                // weights in halves for the second product; the sum keeps fp32
-                uint32_t x[TERMS], y[TERMS];
-                paged4_halves<TERMS>(a, b, x);
-                paged4_halves<TERMS>(c, d, y);
-#pragma unroll
-                for (int e = 0; e < TERMS; ++e) {
-                    pb[t][0][e] = transpose8x8(x[e]);
-                    pb[t][1][e] = transpose8x8(y[e]);
-                }
-            }
-            // this lane's eighth of four slots of V: the products' rows 2 qc, 2 qc + 1 and 8 on
-            uint32_t w[4][VW], sc[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int sl = ((r & 1) ? v1 : v0), at = sl + (r >> 1) * 8;
-                const uint8_t* slot = st + REC + at * RB;
-                const uint8_t* scales = st + REC + 16 * RB + at * (DP / 16);
-                if constexpr (DP == 64) {
-                    w[r][0] = *reinterpret_cast<const uint32_t*>(slot + quad * 4);
-                    sc[r] = scales[quad >> 1];
-                } else if constexpr (DP == 128) {
-                    const uint2 x = *reinterpret_cast<const uint2*>(slot + (((quad >> 1) ^ paged4_turn<DP>(sl)) << 4) + (quad & 1) * 8);
-                    w[r][0] = x.x; w[r][1] = x.y;
-                    sc[r] = scales[quad];
-                } else {
-                    const uint4 x = *reinterpret_cast<const uint4*>(slot + ((quad ^ paged4_turn<DP>(sl)) << 4));
-                    w[r][0] = x.x; w[r][1] = x.y; w[r][2] = x.z; w[r][3] = x.w;
-                    sc[r] = *reinterpret_cast<const uint16_t*>(scales + quad * 2);
-                }
-                sc[r] = fp8_halves(sc[r]);
-                if (vis != 0xffffu && !((vis >> at) & 1u)) sc[r] = 0u;   // what lies behind the length may be anything
-            }
-#pragma unroll
-            for (int i = 0; i < VW; ++i) {
-                uint32_t x[4][4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
                     fp4_halves(w[r][i], x[r]);
-                    const uint32_t one = __byte_perm(sc[r], sc[r], DP < 256 || i < 2 ? 0x1010 : 0x3232);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[r][j] = mul_halves(x[r][j], one);
+                    for (int j = 0; j < 4; ++j)
+                        x[r][j] = (i / 2) % 2 == 0 ? mul_low(x[r][j], two[r][i / 4]) : mul_high(x[r][j], two[r][i / 4]);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {   // columns 2j and 2j + 1 of the word: the rows quad and quad + 8 of a product
-                    const uint32_t a[4] = {__byte_perm(x[0][j], x[1][j], 0x5410), __byte_perm(x[0][j], x[1][j], 0x7632),
-                                           __byte_perm(x[2][j], x[3][j], 0x5410), __byte_perm(x[2][j], x[3][j], 0x7632)};
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t a[4] = {x[0][2 * j], x[1][2 * j], x[0][2 * j + 1], x[1][2 * j + 1]};
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
 #pragma unroll
-                        for (int e = TERMS - 1; e >= 0; --e) mma_16816<__half>(o[t][4 * i + j], a, pb[t][0][e], pb[t][1][e]);
+                        for (int e = TERMS - 1; e >= 0; --e)
+                            mma_16816<__half>(s[t], a, qb[t][2 * i + j][0][e], qb[t][2 * i + j][1][e]);
                 }
             }
         }
-        __syncwarp();   // every lane has read the tile before its stage is filled again
-        stage = stage == NS - 1 ? 0 : stage + 1;
-
-        if (CL ? cp.u + 1 >= end : (cp.blk + 1 == cp.r.nblk || cp.u + 1 == end)) {
-            // the row (or this block's part of it) is complete: join the four warps, 8 heads at a time
-            fresh = !CL;
-            const bool whole = CL ? p.cluster == 1 : part_blk == 0 && cp.blk + 1 == cp.r.nblk;
+        // s[t][0..1]: slot kslot, heads 8t + 2qc, + 1; s[t][2..3]: slot kslot + 8
+        if (vis != 0xffffu) {
+            const bool on0 = (vis >> kslot) & 1u, on1 = (vis >> (kslot + 8)) & 1u;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                if (t * 8 >= nh) break;
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[t][j] = (j < 2 ? on0 : on1) ? s[t][j] : -INFINITY;
+        }
+        // logarithms of the weights; a row's first tile finds base at -inf and grows
+        float x[NT][4];
+        bool grow = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[t][j] = fmaf(s[t][j], unit[t][j & 1], -base[t][j & 1]);
+                grow |= x[t][j] > kGrow + kLift;
+            }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
+                    float n = fmaxf(s[t][j], s[t][2 + j]) * unit[t][j];
 #pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) l[t][j] += __shfl_xor_sync(0xffffffffu, l[t][j], x);
-                    if (quad == 0)
-                        *reinterpret_cast<float2*>(s_ml + (warp * 8 + qc * 2 + j) * 2) = make_float2(m[t][j] - kLift, l[t][j]);
-                    float* dst = s_o + (warp * 8 + qc * 2 + j) * S::kOStride + quad * (DP / 8);
+                    for (int y = 4; y < 32; y <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, y));
+                    n = fmaxf(n - kLift, base[t][j]);
+                    const float c = n == -INFINITY ? 1.0f : exp2_fast(base[t][j] - n);
+                    base[t][j] = n;
+                    l[t][j] *= c;
+                    x[t][j] = n == -INFINITY ? s[t][j] : fmaf(s[t][j], unit[t][j], -n);   // -inf or NaN as it is
+                    x[t][2 + j] = n == -INFINITY ? s[t][2 + j] : fmaf(s[t][2 + j], unit[t][j], -n);
 #pragma unroll
-                    for (int i = 0; i < DP / 16; ++i)
-                        *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[t][i][j], o[t][i][2 + j]);
+                    for (int i = 0; i < DP / 16; ++i) {
+                        o[t][i][j] *= c;
+                        o[t][i][2 + j] *= c;
+                    }
                 }
-                __syncthreads();
-                for (int h = warp; h < 8 && t * 8 + h < nh; h += kPdWarps) {
-                    float M = -INFINITY, L = 0.0f, c[kPdWarps];
+        }
+        uint32_t pb[NT][2][TERMS];
 #pragma unroll
-                    for (int w = 0; w < kPdWarps; ++w) M = fmaxf(M, s_ml[(w * 8 + h) * 2]);
-                    const float u = M == -INFINITY ? 0.0f : M;
+        for (int t = 0; t < NT; ++t) {
+            const float a = exp2_fast(x[t][0]), b = exp2_fast(x[t][1]), c = exp2_fast(x[t][2]), d = exp2_fast(x[t][3]);
+            l[t][0] += a + c;
+            l[t][1] += b + d;
+            // weights in halves for the second product; the sum keeps fp32
+            uint32_t y[TERMS], z[TERMS];
+            paged4_halves<TERMS>(a, b, y);
+            paged4_halves<TERMS>(c, d, z);
+#pragma unroll
+            for (int e = 0; e < TERMS; ++e) {
+                pb[t][0][e] = transpose8x8(y[e]);
+                pb[t][1][e] = transpose8x8(z[e]);
+            }
+        }
+        // this lane's eighth of four slots of V: the products' rows 2 qc, 2 qc + 1 and 8 on
+        uint32_t w[4][VW], sc[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int sl = ((r & 1) ? v1 : v0), at = sl + (r >> 1) * 8;
+            const uint8_t* slot = st + REC + at * RB;
+            const uint8_t* scales = st + REC + 16 * RB + at * (DP / 16);
+            if constexpr (DP == 64) {
+                w[r][0] = *reinterpret_cast<const uint32_t*>(slot + quad * 4);
+                sc[r] = scales[quad >> 1];
+            } else if constexpr (DP == 128) {
+                const uint2 y = *reinterpret_cast<const uint2*>(slot + (((quad >> 1) ^ paged4_turn<DP>(sl)) << 4) + (quad & 1) * 8);
+                w[r][0] = y.x; w[r][1] = y.y;
+                sc[r] = scales[quad];
+            } else {
+                const uint4 y = *reinterpret_cast<const uint4*>(slot + ((quad ^ paged4_turn<DP>(sl)) << 4));
+                w[r][0] = y.x; w[r][1] = y.y; w[r][2] = y.z; w[r][3] = y.w;
+                sc[r] = *reinterpret_cast<const uint16_t*>(scales + quad * 2);
+            }
+        }
+        if (vis != 0xffffu)   // what lies behind the length may be anything
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (!((vis >> (((r & 1) ? v1 : v0) + (r >> 1) * 8)) & 1u)) sc[r] = 0u;
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            uint32_t y[4][4], one[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                fp4_halves(w[r][i], y[r]);
+                // (scale, 0) of the even slots, (0, scale) of the odd ones
+                const uint32_t e = DP < 256 ? sc[r] : i < 2 ? sc[r] & 0xffu : sc[r] >> 8;
+                one[r] = fp8_halves((r & 1) ? e * 256u : e);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {   // columns 2j and 2j + 1 of the word: the rows quad and quad + 8 of a product
+                uint32_t a[4];
+                pair_scaled(y[0][j], y[1][j], one[0], one[1], a[0], a[1]);
+                pair_scaled(y[2][j], y[3][j], one[2], one[3], a[2], a[3]);
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = TERMS - 1; e >= 0; --e) mma_16816<__half>(o[t][4 * i + j], a, pb[t][0][e], pb[t][1][e]);
+            }
+        }
+    };
+
+    // The end of a row (`whole`) or of this block's part of it: join the four warps, 8 heads at a time.
+    auto close_row = [&](int kvh, int h0, int nh, bool whole, bool first) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (t * 8 >= nh) break;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[t][j] += __shfl_xor_sync(0xffffffffu, l[t][j], x);
+                if (quad == 0)
+                    *reinterpret_cast<float2*>(s_ml + (warp * 8 + qc * 2 + j) * 2) = make_float2(base[t][j], l[t][j]);
+                float* dst = s_o + (warp * 8 + qc * 2 + j) * S::kOStride + quad * (DP / 8);
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i)
+                    *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[t][i][j], o[t][i][2 + j]);
+            }
+            __syncthreads();
+            for (int h = warp; h < 8 && t * 8 + h < nh; h += kPdWarps) {
+                float M = -INFINITY, L = 0.0f, c[kPdWarps];
+#pragma unroll
+                for (int w = 0; w < kPdWarps; ++w) M = fmaxf(M, s_ml[(w * 8 + h) * 2]);
+                const float u = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+                for (int w = 0; w < kPdWarps; ++w) {
+                    c[w] = exp2_fast(s_ml[(w * 8 + h) * 2] - u);
+                    L += s_ml[(w * 8 + h) * 2 + 1] * c[w];
+                }
+                const float inv = (whole ? (L > 0.0f ? 1.0f / L : L) : 1.0f) * p.v_scale;
+                const int row = t * 8 + h, qh = kvh * p.rep + h0 + row;
+                const int64_t part = (2 * static_cast<int64_t>(blockIdx.x) + (first ? 1 : 0)) * 16 + row;
+                T* out = static_cast<T*>(p.out) + cp.b * p.out_row + qh * p.out_head;
+                // a cluster's block leaves its part where the copies were (they are all consumed)
+                float* po = CL ? reinterpret_cast<float*>(smem) + row * DP : p.part_o + part * p.part_stride;
+                for (int d = lane * 2; d < DP; d += 64) {
+                    float a = 0.0f, b = 0.0f;
 #pragma unroll
                     for (int w = 0; w < kPdWarps; ++w) {
-                        c[w] = exp2_fast(s_ml[(w * 8 + h) * 2] - u);
-                        L += s_ml[(w * 8 + h) * 2 + 1] * c[w];
+                        const float2 v = *reinterpret_cast<const float2*>(s_o + (w * 8 + h) * S::kOStride + d);
+                        a = fmaf(v.x, c[w], a);
+                        b = fmaf(v.y, c[w], b);
                     }
-                    const float inv = (whole ? (L > 0.0f ? 1.0f / L : L) : 1.0f) * p.v_scale;
-                    const int row = t * 8 + h, head = kvh * p.rep + h0 + row;
-                    const int64_t part = (2 * static_cast<int64_t>(blockIdx.x) + (part_blk == 0 ? 1 : 0)) * 16 + row;
-                    T* out = static_cast<T*>(p.out) + cp.b * p.out_row + head * p.out_head;
-                    // a cluster's block leaves its part where the copies were (they are all consumed)
-                    float* po = CL ? reinterpret_cast<float*>(smem) + row * DP : p.part_o + part * p.part_stride;
-                    for (int d = lane * 2; d < DP; d += 64) {
-                        float a = 0.0f, b = 0.0f;
-#pragma unroll
-                        for (int w = 0; w < kPdWarps; ++w) {
-                            const float2 v = *reinterpret_cast<const float2*>(s_o + (w * 8 + h) * S::kOStride + d);
-                            a = fmaf(v.x, c[w], a);
-                            b = fmaf(v.y, c[w], b);
-                        }
-                        a *= inv;
-                        b *= inv;
-                        if (!whole) {
-                            *reinterpret_cast<float2*>(po + d) = make_float2(a, b);
-                        } else {
-                            if (d < p.c.head_dim) out[d] = from_f32<T>(a);
-                            if (d + 1 < p.c.head_dim) out[d + 1] = from_f32<T>(b);
-                        }
-                    }
-                    if (lane == 0) {
-                        if (!whole) {
-                            float* ml = CL ? reinterpret_cast<float*>(smem) + 16 * DP + row * 2 : p.part_ml + part * 2;
-                            *reinterpret_cast<float2*>(ml) = make_float2(M, L);
-                        } else if (p.lse != nullptr) {
-                            p.lse[static_cast<int64_t>(cp.b) * p.heads + head] = L != 0.0f ? (u + log2f(L)) * kLn2 : -INFINITY;
-                        }
+                    a *= inv;
+                    b *= inv;
+                    if (!whole) {
+                        *reinterpret_cast<float2*>(po + d) = make_float2(a, b);
+                    } else {
+                        if (d < p.c.head_dim) out[d] = from_f32<T>(a);
+                        if (d + 1 < p.c.head_dim) out[d + 1] = from_f32<T>(b);
                     }
                 }
-                if (NT > 1 || !CL) __syncthreads();
+                if (lane == 0) {
+                    if (!whole) {
+                        float* ml = CL ? reinterpret_cast<float*>(smem) + 16 * DP + row * 2 : p.part_ml + part * 2;
+                        *reinterpret_cast<float2*>(ml) = make_float2(M, L);
+                    } else if (p.lse != nullptr) {
+                        p.lse[static_cast<int64_t>(cp.b) * p.heads + qh] = L != 0.0f ? (u + log2f(L)) * kLn2 : -INFINITY;
+                    }
+                }
             }
-            if (CL) break;
+            if (NT > 1 || !CL) __syncthreads();
         }
-        advance(cp);
+    };
+
+    if constexpr (CL) {
+        const int kvh = kv_head(cp.v), h0 = (cp.v - kvh * p.parts) * 16, nh = min(16, p.rep - h0);
+        open_row(kvh, h0, nh);
+        for (int n = 0; n < end; n += NS) {
+#pragma unroll
+            for (int step = 0; step < NS; ++step) {
+                if (n + step >= end) break;
+                issue((step + NS - 1) % NS, 0);
+                cp_async_wait<NS - 1>();
+                __syncwarp();
+                take(step);
+                __syncwarp();   // every lane has read the tile before its stage is filled again
+            }
+        }
+        close_row(kvh, h0, nh, p.cluster == 1, false);
+    } else {
+        static_assert(CL || TILES == NS, "the tiles of a unit are the stages");
+        bool fresh = true;    // the next unit opens a new part or row
+        bool first = false;   // ... the row itself
+        while (cp.u < end) {
+            const int kvh = kv_head(cp.v), h0 = (cp.v - kvh * p.parts) * 16;
+            const int nh = min(16, p.rep - h0);          // query heads of this unit
+            if (fresh) {
+                fresh = false;
+                first = cp.blk == 0;
+                open_row(kvh, h0, nh);
+            }
+#pragma unroll
+            for (int step = 0; step < NS; ++step) {
+                issue((step + NS - 1) % NS, (step + NS - 1) % NS);
+                cp_async_wait<NS - 1>();
+                __syncwarp();
+                take(step);
+                __syncwarp();   // every lane has read the tile before its stage is filled again
+            }
+            const bool last = cp.blk + 1 == cp.r.nblk;
+            if (last || cp.u + 1 == end) {
+                fresh = true;
+                close_row(kvh, h0, nh, first && last, first);
+            }
+            advance(cp);
+        }
     }
     cp_async_wait<0>();
     if constexpr (CL)
         if (p.cluster > 1) {
-            const int kvh = cp.v / p.parts, h0 = (cp.v % p.parts) * 16;
+            const int kvh = kv_head(cp.v), h0 = (cp.v - kvh * p.parts) * 16;
             paged_cluster_join<T>(p, smem, DP, rank, cp.b, kvh * p.rep + h0, min(16, p.rep - h0), warp, lane);
         }
 }

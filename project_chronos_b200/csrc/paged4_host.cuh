@@ -55,6 +55,10 @@ inline int check_packed(const ChronosPagedCache& c, float k_scale, float v_scale
     if (c.page_size % 16) return fail(CHRONOS_ERR_INVALID_ARG, "%s: 4-bit pages need a page_size that is a multiple of 16, got %d", what, c.page_size);
     if (!multiples(16, {c.k_page_stride, c.k_head_stride, c.v_page_stride, c.v_head_stride}) || !aligned(c.k_pages, 16) || !aligned(c.v_pages, 16))
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: 4-bit pages and their strides must be multiples of 16 bytes", what);
+    if (c.k_page_stride < 0 || c.v_page_stride < 0 || c.k_page_stride > UINT32_MAX || c.v_page_stride > UINT32_MAX ||
+        static_cast<int64_t>(c.page_size) * 144 > INT32_MAX)
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: 4-bit pages of %d slots, %lld and %lld bytes apart", what, c.page_size,
+                    static_cast<long long>(c.k_page_stride), static_cast<long long>(c.v_page_stride));
     if (int rc = check_positive("k_scale", k_scale, what)) return rc;
     return check_positive("v_scale", v_scale, what);
 }
