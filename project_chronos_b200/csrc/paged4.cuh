@@ -3,6 +3,8 @@
 // paged.cuh.
 #pragma once
 
+#include <type_traits>
+
 #include "fp4.cuh"
 #include "paged.cuh"
 
@@ -43,6 +45,32 @@ __device__ __forceinline__ void paged4_halves(float a, float b, uint32_t (&r)[TE
         const __half2 l = __floats2half2_rn(x == x ? x : 0.0f, y == y ? y : 0.0f);
         r[1] = *reinterpret_cast<const uint32_t*>(&l);
     }
+}
+
+// Shared memory at an address the compiler keeps in a register (it would work the address out again
+// for every tile), with what is added at compile time in the instruction.
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t (&r)[N], uint32_t at, int off) {
+    if constexpr (N == 1)
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r[0]) : "r"(at + off));
+    else if constexpr (N == 2)
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at + off));
+    else
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at + off));
+}
+// N bytes (1, 2 or 4) with zeros above.
+template <int N>
+__device__ __forceinline__ uint32_t lds_bytes(uint32_t at, int off) {
+    uint32_t r;
+    if constexpr (N == 1) asm volatile("ld.shared.u8 %0, [%1];" : "=r"(r) : "r"(at + off));
+    else if constexpr (N == 2) asm volatile("{\n\t.reg .u16 t;\n\tld.shared.u16 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(r) : "r"(at + off));
+    else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(at + off));
+    return r;
+}
+__device__ __forceinline__ uint32_t kept(uint32_t x) {
+    uint32_t r;
+    asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
 }
 
 // HBM bound as long as the products are fed: 9/8 D bytes per slot and kv head.  Codes become
@@ -185,7 +213,19 @@ __global__ void __launch_bounds__(kPdThreads, Paged4<T, DP, NT>::kBlocksPerSm) p
     float unit[NT][2];               // of the scores of heads 2 qc and 2 qc + 1
     float o[NT][DP / 16][4];
     float base[NT][2], l[NT][2];     // what is taken off the scores: the maximum as it lags, less kLift
-    const uint8_t* mine = smem + warp * 2 * REC;
+    // where this lane finds its parts of a tile (slots + 8: 8 slots on)
+    constexpr int SB = DP / 16;                      // scales of a slot
+    const uint32_t k_at = kept(ring + kslot * RB + (DP == 64 ? qc * 8 : ((DP == 128 ? qc : 2 * qc) ^ paged4_turn<DP>(kslot)) << 4));
+    const uint32_t k_at2 = DP < 256 ? 0u : kept(ring + kslot * RB + (((2 * qc + 1) ^ paged4_turn<DP>(kslot)) << 4));
+    const uint32_t ks_at = kept(ring + 16 * RB + kslot * SB + qc * (SB / 4));
+    uint32_t v_at[2], vs_at[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int sl = r ? v1 : v0;
+        v_at[r] = kept(ring + REC + sl * RB + (DP == 64 ? quad * 4 : DP == 128 ? (((quad >> 1) ^ paged4_turn<DP>(sl)) << 4) + (quad & 1) * 8
+                                                                              : (quad ^ paged4_turn<DP>(sl)) << 4));
+        vs_at[r] = kept(ring + REC + 16 * RB + sl * SB + (DP == 64 ? quad >> 1 : DP == 128 ? quad : quad * 2));
+    }
 
     // A row's (or part's) beginning: kv head kvh, query heads from h0 on.
     auto open_row = [&](int kvh, int h0, int nh) {
@@ -222,36 +262,35 @@ __global__ void __launch_bounds__(kPdThreads, Paged4<T, DP, NT>::kBlocksPerSm) p
         }
     };
 
-    // The tile in a stage (known at compile time).
-    auto take = [&](int stage) {
+    // The tile in a stage.
+    auto take = [&](auto stage_of) {
+        constexpr int stage = decltype(stage_of)::value, at = stage * S::kStageBytes;
         const uint32_t vis = shows[stage];
         if (vis == 0u) return;
-        const uint8_t* st = mine + stage * S::kStageBytes;
         float s[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
         {
             // this lane's quarter of slots kslot and kslot + 8
             uint32_t w[2][KW], two[2][(KW + 3) / 4];
+            if constexpr (DP < 256) {
+                lds_words<KW>(w[0], k_at, at);
+                lds_words<KW>(w[1], k_at, at + 8 * RB);
+                two[0][0] = fp8_halves(lds_bytes<SB / 4>(ks_at, at));
+                two[1][0] = fp8_halves(lds_bytes<SB / 4>(ks_at, at + 8 * SB));
+            } else {
+                uint32_t x[4];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const uint8_t* slot = st + (kslot + 8 * r) * RB;
-                const uint8_t* scales = st + 16 * RB + (kslot + 8 * r) * (DP / 16);
-                if constexpr (DP == 64) {
-                    const uint2 x = *reinterpret_cast<const uint2*>(slot + qc * 8);
-                    w[r][0] = x.x; w[r][1] = x.y;
-                    two[r][0] = fp8_halves(scales[qc]);
-                } else if constexpr (DP == 128) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(slot + ((qc ^ paged4_turn<DP>(kslot)) << 4));
-                    w[r][0] = x.x; w[r][1] = x.y; w[r][2] = x.z; w[r][3] = x.w;
-                    two[r][0] = fp8_halves(*reinterpret_cast<const uint16_t*>(scales + qc * 2));
-                } else {
+                for (int r = 0; r < 2; ++r) {
+                    if (r == 0) lds_words<4>(x, k_at, at);
+                    else lds_words<4>(x, k_at, at + 8 * RB);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(slot + (((2 * qc + i) ^ paged4_turn<DP>(kslot)) << 4));
-                        w[r][4 * i] = x.x; w[r][4 * i + 1] = x.y; w[r][4 * i + 2] = x.z; w[r][4 * i + 3] = x.w;
-                    }
-                    const uint32_t sc = *reinterpret_cast<const uint32_t*>(scales + qc * 4);
+                    for (int i = 0; i < 4; ++i) w[r][i] = x[i];
+                    if (r == 0) lds_words<4>(x, k_at2, at);
+                    else lds_words<4>(x, k_at2, at + 8 * RB);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[r][4 + i] = x[i];
+                    const uint32_t sc = r == 0 ? lds_bytes<4>(ks_at, at) : lds_bytes<4>(ks_at, at + 8 * SB);
                     two[r][0] = fp8_halves(sc);
                     two[r][1] = fp8_halves(sc >> 16);
                 }
@@ -334,24 +373,15 @@ __global__ void __launch_bounds__(kPdThreads, Paged4<T, DP, NT>::kBlocksPerSm) p
         }
         // this lane's eighth of four slots of V: the products' rows 2 qc, 2 qc + 1 and 8 on
         uint32_t w[4][VW], sc[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int sl = ((r & 1) ? v1 : v0), at = sl + (r >> 1) * 8;
-            const uint8_t* slot = st + REC + at * RB;
-            const uint8_t* scales = st + REC + 16 * RB + at * (DP / 16);
-            if constexpr (DP == 64) {
-                w[r][0] = *reinterpret_cast<const uint32_t*>(slot + quad * 4);
-                sc[r] = scales[quad >> 1];
-            } else if constexpr (DP == 128) {
-                const uint2 y = *reinterpret_cast<const uint2*>(slot + (((quad >> 1) ^ paged4_turn<DP>(sl)) << 4) + (quad & 1) * 8);
-                w[r][0] = y.x; w[r][1] = y.y;
-                sc[r] = scales[quad];
-            } else {
-                const uint4 y = *reinterpret_cast<const uint4*>(slot + ((quad ^ paged4_turn<DP>(sl)) << 4));
-                w[r][0] = y.x; w[r][1] = y.y; w[r][2] = y.z; w[r][3] = y.w;
-                sc[r] = *reinterpret_cast<const uint16_t*>(scales + quad * 2);
-            }
-        }
+        constexpr int VB = DP == 256 ? 2 : 1;
+        lds_words<VW>(w[0], v_at[0], at);
+        lds_words<VW>(w[1], v_at[1], at);
+        lds_words<VW>(w[2], v_at[0], at + 8 * RB);
+        lds_words<VW>(w[3], v_at[1], at + 8 * RB);
+        sc[0] = lds_bytes<VB>(vs_at[0], at);
+        sc[1] = lds_bytes<VB>(vs_at[1], at);
+        sc[2] = lds_bytes<VB>(vs_at[0], at + 8 * SB);
+        sc[3] = lds_bytes<VB>(vs_at[1], at + 8 * SB);
         if (vis != 0xffffu)   // what lies behind the length may be anything
 #pragma unroll
             for (int r = 0; r < 4; ++r)
@@ -442,19 +472,23 @@ __global__ void __launch_bounds__(kPdThreads, Paged4<T, DP, NT>::kBlocksPerSm) p
         }
     };
 
+    // The next tile's copies, `tile` of its unit, and the tile in stage `step`.
+    static_assert(NS == 4, "the steps below");
+    auto run = [&](auto step, int tile) {
+        issue((decltype(step)::value + NS - 1) % NS, tile);
+        cp_async_wait<NS - 1>();
+        __syncwarp();
+        take(step);
+        __syncwarp();   // every lane has read the tile before its stage is filled again
+    };
     if constexpr (CL) {
         const int kvh = kv_head(cp.v), h0 = (cp.v - kvh * p.parts) * 16, nh = min(16, p.rep - h0);
         open_row(kvh, h0, nh);
         for (int n = 0; n < end; n += NS) {
-#pragma unroll
-            for (int step = 0; step < NS; ++step) {
-                if (n + step >= end) break;
-                issue((step + NS - 1) % NS, 0);
-                cp_async_wait<NS - 1>();
-                __syncwarp();
-                take(step);
-                __syncwarp();   // every lane has read the tile before its stage is filled again
-            }
+            run(std::integral_constant<int, 0>{}, 0);
+            if (n + 1 < end) run(std::integral_constant<int, 1>{}, 0);
+            if (n + 2 < end) run(std::integral_constant<int, 2>{}, 0);
+            if (n + 3 < end) run(std::integral_constant<int, 3>{}, 0);
         }
         close_row(kvh, h0, nh, p.cluster == 1, false);
     } else {
@@ -469,14 +503,10 @@ __global__ void __launch_bounds__(kPdThreads, Paged4<T, DP, NT>::kBlocksPerSm) p
                 first = cp.blk == 0;
                 open_row(kvh, h0, nh);
             }
-#pragma unroll
-            for (int step = 0; step < NS; ++step) {
-                issue((step + NS - 1) % NS, (step + NS - 1) % NS);
-                cp_async_wait<NS - 1>();
-                __syncwarp();
-                take(step);
-                __syncwarp();   // every lane has read the tile before its stage is filled again
-            }
+            run(std::integral_constant<int, 0>{}, 3);
+            run(std::integral_constant<int, 1>{}, 0);
+            run(std::integral_constant<int, 2>{}, 1);
+            run(std::integral_constant<int, 3>{}, 2);
             const bool last = cp.blk + 1 == cp.r.nblk;
             if (last || cp.u + 1 == end) {
                 fresh = true;
