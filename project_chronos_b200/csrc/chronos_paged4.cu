@@ -293,7 +293,7 @@ extern "C" int chronos_paged_bounds(const ChronosPagedBoundsArgs* a, void* strea
     const int64_t rows = static_cast<int64_t>(c.batch) * c.kv_heads;
     int64_t pages = c.table_width;
     if (!a->full) pages = std::min<int64_t>(pages, a->cu_seqlens == nullptr ? 1 : (a->num_tokens + c.page_size - 1) / c.page_size + 1);
-    pages = std::max<int64_t>(1, std::min<int64_t>(pages, 64 * static_cast<int64_t>(sm_count()) / rows));
+    pages = std::max<int64_t>(1, std::min<int64_t>(pages, 8 * static_cast<int64_t>(sm_count()) / rows));
     const unsigned by = static_cast<unsigned>(std::min<int64_t>(rows, 32768)), bz = static_cast<unsigned>((rows + by - 1) / by);
     const int es = static_cast<int>(elem_bytes(c.dtype));
     const bool vec = c.head_dim % 8 == 0 &&
@@ -354,14 +354,18 @@ extern "C" int chronos_paged_select(const ChronosPagedSelectArgs* a, void* strea
         p.token0 = t0;
         p.tokens = std::min(group, a->num_tokens - t0);
         if (bytes > 0) {
-            const int64_t tiles = (p.tokens + kScoreTokens - 1) / kScoreTokens;
-            // pages per block: 32 at a time; more where blocks abound, to form the queries' sums less often
-            p.chunk = 32;
-            while (p.chunk < 256 && (c.table_width + p.chunk - 1) / p.chunk * tiles * c.kv_heads > 16 * static_cast<int64_t>(sm_count())) p.chunk *= 2;
-            const dim3 grid((c.table_width + p.chunk - 1) / p.chunk, c.kv_heads, static_cast<unsigned>(tiles));
+            // (of a packed call every sequence may have a tile that is not full)
+            const int per = p.cu == nullptr ? 1 : kScoreTokens;
+            const int64_t tiles = p.cu == nullptr ? p.tokens : p.tokens / per + std::min<int64_t>(c.batch, p.tokens);
+            // pages per block: 64 at a time; more once that leaves every SM three blocks
+            p.chunk = 64;
+            while (p.chunk < kScorePages && (c.table_width + p.chunk - 1) / p.chunk * tiles * c.kv_heads > 3 * static_cast<int64_t>(sm_count())) p.chunk *= 2;
+            p.chunks = (c.table_width + p.chunk - 1) / p.chunk;
+            const dim3 grid(static_cast<unsigned>(p.chunks * c.kv_heads * tiles));
             const int rc = by_dtype(c.dtype, [&](auto x) {
                 using T = decltype(x);
-                auto kernel = vec ? paged_score_kernel<T, true> : paged_score_kernel<T, false>;
+                auto kernel = per == 1 ? (vec ? paged_score_kernel<T, true, 1> : paged_score_kernel<T, false, 1>)
+                                       : (vec ? paged_score_kernel<T, true, kScoreTokens> : paged_score_kernel<T, false, kScoreTokens>);
                 CHRONOS_CUDA_CHECK(launch_kernel(kernel, grid, dim3(kScoreThreads), 0, st, false, p));
                 return static_cast<int>(CHRONOS_OK);
             });

@@ -135,7 +135,7 @@ struct PagedSelectParams {
     int max_slots;
     int64_t width;              // keys per token and kv head
     unsigned long long* keys;   // [tokens][kv heads][width]
-    int chunk;                  // pages of a block
+    int chunk, chunks;          // pages of a block, blocks of a row
     int32_t* status;
 };
 
@@ -156,8 +156,8 @@ __device__ __forceinline__ SelectToken select_token(const PagedSelectParams& p, 
     return r;
 }
 
-// A score's place in the order of numbers: -0 as 0, NaN above every number, and room above
-// for the pages that are always in (and 0 for a page that is none).
+// A score's place in the order of numbers: -0 as 0, NaN above every number (and 0 for a page
+// that is none).
 __device__ __forceinline__ unsigned long long select_key(double x) {
     if (x != x) return ~0ull - 1;
     const unsigned long long u = static_cast<unsigned long long>(__double_as_longlong(x + 0.0));
@@ -166,107 +166,150 @@ __device__ __forceinline__ unsigned long long select_key(double x) {
 
 constexpr int kScoreThreads = 256;
 constexpr int kScoreTokens = 8;     // tokens of one sequence that share the reading of a page
+constexpr int kScorePages = 512;    // pages of a block at most
 
-// Bound by reading the bounds.  8 lanes share a page; each takes every eighth group of 8
-// columns of lo and hi, and the partial sums meet in three shuffles.  Block: a chunk of
-// pages, a kv head, up to 8 tokens (split where their sequences differ).
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kScoreThreads) paged_score_kernel(const __grid_constant__ PagedSelectParams p) {
-    constexpr int MAXD = CHRONOS_PAGED_MAX_HEAD_DIM;
-    __shared__ __align__(16) double s_q[kScoreTokens][2][MAXD];   // down, up
-    __shared__ SelectToken s_t[kScoreTokens];
-    const int G = p.c.kv_heads, D = p.c.head_dim, g = blockIdx.y;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t t0 = static_cast<int64_t>(blockIdx.z) * kScoreTokens;
-    const int n = static_cast<int>(min(int64_t{kScoreTokens}, p.tokens - t0));
-    if (warp < n) {
-        const SelectToken r = select_token(p, p.token0 + t0 + warp, lane);
-        if (lane == 0) s_t[warp] = r;
+// Bound by reading the bounds.  8 lanes share a page, two pages at a time (16-bit types), whose loads
+// all go out before the first is used; each lane takes every eighth group of 8 columns of lo and hi, and
+// the partial sums meet in three shuffles.  Block: up to kScorePages pages, a kv head, TOKENS
+// tokens of a sequence (1 where every sequence has one).  The queries' sums lie in shared memory
+// so that the 8 lanes' parts are side by side, the pages' numbers beside them: both are fetched
+// at once.  32 rows of 256 to 512 pages, 8 heads of 128: 52 us with a look-up before every page.
+template <typename T, bool VEC, int TOKENS>
+__global__ void __launch_bounds__(kScoreThreads, TOKENS == 1 ? 3 : 2) paged_score_kernel(const __grid_constant__ PagedSelectParams p) {
+    constexpr int MAXD = CHRONOS_PAGED_MAX_HEAD_DIM, GROUPS = kScoreThreads / 8;
+    constexpr int PAGES = sizeof(T) == 2 && VEC ? 2 : 1, CHUNKS = PAGES;   // pages and 64 columns that are in flight at once
+    __shared__ __align__(16) double2 s_q[TOKENS][2][MAXD / 2];   // down, up; columns 64 c + 8 part + 2 e, + 1 at (4 c + e) * 8 + part
+    __shared__ int s_page[kScorePages];
+    const int G = p.c.kv_heads, D = p.c.head_dim, block = blockIdx.x % p.chunks, g = blockIdx.x / p.chunks % G;
+    const int lane = threadIdx.x & 31;
+    const int j0 = block * p.chunk;
+    // the block's tokens: [t0, t0 + n) of sequence seq, the last of which sees `len` slots
+    int64_t t0 = blockIdx.x / p.chunks / G + p.token0;
+    int seq = static_cast<int>(t0), n = 1;
+    if (p.cu != nullptr) {
+        // tile `tile` of the list of all sequences' tiles of TOKENS tokens (this launch has tokens token0 ..)
+        const int tile = static_cast<int>(blockIdx.x / p.chunks / G);
+        int before = 0;
+        seq = -1;
+        for (int base = 0; base < p.c.batch && seq < 0; base += 32) {
+            const int b = base + lane;
+            int64_t lo = 0, hi = 0;
+            if (b < p.c.batch) {
+                lo = max(static_cast<int64_t>(p.cu[b]), p.token0);
+                hi = min(static_cast<int64_t>(p.cu[b + 1]), p.token0 + p.tokens);
+            }
+            const int mine = hi > lo ? static_cast<int>((hi - lo + TOKENS - 1) / TOKENS) : 0;
+            int inc = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, before + inc > tile);
+            if (past != 0u) {
+                const int l = __ffs(past) - 1;
+                const int in = tile - before - __shfl_sync(0xffffffffu, inc - mine, l);
+                t0 = __shfl_sync(0xffffffffu, lo, l) + static_cast<int64_t>(in) * TOKENS;
+                n = static_cast<int>(min(int64_t{TOKENS}, __shfl_sync(0xffffffffu, hi, l) - t0));
+                seq = base + l;
+            }
+            before += __shfl_sync(0xffffffffu, inc, 31);
+        }
+        if (seq < 0) return;   // more blocks than tiles
     }
-    __syncthreads();
-    const int j0 = blockIdx.x * p.chunk;
-    bool any = false;   // tokens with no more pages than they may take need no scores
-    for (int i = 0; i < n; ++i) any |= s_t[i].pages > p.topk && s_t[i].pages > j0;
-    if (!any) return;
-    const int D8 = (D + 7) & ~7;
-    for (int i = threadIdx.x; i < n * D8; i += kScoreThreads) {
-        const int t = i / D8, d = i % D8;
+    const int raw = min(max(p.c.lens[seq], 0), p.max_slots);
+    // slots at or before the last token, and before that one
+    const int len = p.cu == nullptr ? raw : static_cast<int>(max(int64_t{0}, raw - (static_cast<int64_t>(p.cu[seq + 1]) - (t0 + n))));
+    const int most = (len + p.c.page_size - 1) / p.c.page_size, stop = min(j0 + p.chunk, most);
+    if (most <= p.topk || j0 >= most) return;   // all pages are taken: no scores
+    for (int j = j0 + threadIdx.x; j < stop; j += kScoreThreads) {
+        const int page = p.c.page_table[seq * p.c.page_table_stride + j];
+        const bool none = page < 0 || page >= p.c.num_pages;
+        if (none) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
+        s_page[j - j0] = none ? -1 : page;
+    }
+    const int D64 = (D + 63) & ~63;
+    for (int i = threadIdx.x; i < n * D64; i += kScoreThreads) {
+        const int t = i / D64, d = i % D64;
         double up = 0.0, down = 0.0;
-        if (d < D && s_t[t].pages > p.topk) {
-            const T* q = static_cast<const T*>(p.q) + (p.token0 + t0 + t) * p.q_row + static_cast<int64_t>(g) * p.rep * p.q_head + d;
+        if (d < D) {
+            const T* q = static_cast<const T*>(p.q) + (t0 + t) * p.q_row + static_cast<int64_t>(g) * p.rep * p.q_head + d;
+#pragma unroll 4
             for (int h = 0; h < p.rep; ++h) {
                 const float x = to_f32<T>(q[h * p.q_head]);
                 if (x > 0.0f) up += x;
                 else down += x;   // and NaN
             }
         }
-        s_q[t][0][d] = down;
-        s_q[t][1][d] = up;
+        const int at = 2 * (((d >> 6) * 4 + ((d & 7) >> 1)) * 8 + ((d >> 3) & 7)) + (d & 1);
+        reinterpret_cast<double*>(s_q[t][0])[at] = down;
+        reinterpret_cast<double*>(s_q[t][1])[at] = up;
     }
     __syncthreads();
-    const int part = threadIdx.x & 7;
-    for (int i0 = 0; i0 < n;) {
-        // tokens i0 .. i1 - 1 share a sequence
-        int i1 = i0 + 1;
-        const int seq = s_t[i0].seq;
-        while (i1 < n && s_t[i1].seq == seq) ++i1;
-        const int most = s_t[i1 - 1].pages;   // the last of them sees most
-        if (seq >= 0 && most > p.topk) {
-            const int32_t* table = p.c.page_table + seq * p.c.page_table_stride;
-            for (int j = j0 + (threadIdx.x >> 3); j - static_cast<int>(threadIdx.x >> 3) < min(j0 + p.chunk, most); j += kScoreThreads / 8) {
-                const bool in = j < min(j0 + p.chunk, most);
-                int page = in ? table[j] : -1;
-                if (in && (page < 0 || page >= p.c.num_pages)) {
-                    report_status(p.status, CHRONOS_ERR_INVALID_ARG);
-                    page = -1;
-                }
-                double acc[kScoreTokens];
+    const int part = threadIdx.x & 7, group = threadIdx.x >> 3;
+    unsigned long long* keys = p.keys + ((t0 - p.token0) * G + g) * p.width;
+    for (int base = j0; base < stop; base += PAGES * GROUPS) {
+        double acc[TOKENS][PAGES];
+        int page[PAGES];
 #pragma unroll
-                for (int t = 0; t < kScoreTokens; ++t) acc[t] = 0.0;
-                if (page >= 0) {
-                    const T* lo = static_cast<const T*>(p.bounds) + (static_cast<int64_t>(page) * 2 * G + g) * D;
-                    const T* hi = lo + static_cast<int64_t>(G) * D;
-                    for (int d = part * 8; d < D; d += 64) {
-                        float a[8], c[8];
-                        if constexpr (VEC) {
-                            load8<T>(lo + d, a);
-                            load8<T>(hi + d, c);
-                        } else {
+        for (int k = 0; k < PAGES; ++k) {
+            const int j = base + k * GROUPS + group;
+            page[k] = j < stop ? s_page[j - j0] : -1;
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                a[e] = d + e < D ? to_f32<T>(lo[d + e]) : 0.0f;
-                                c[e] = d + e < D ? to_f32<T>(hi[d + e]) : 0.0f;
-                            }
+            for (int t = 0; t < TOKENS; ++t) acc[t][k] = 0.0;
+        }
+        for (int c0 = 0; c0 * 64 < D; c0 += CHUNKS) {
+            RopeRow<T, VEC> x[PAGES][2][CHUNKS];   // page, lo or hi, 64 columns
+#pragma unroll
+            for (int k = 0; k < PAGES; ++k)
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int c = 0; c < CHUNKS; ++c) {
+                        const int d = (c0 + c) * 64 + part * 8;
+                        const T* row = static_cast<const T*>(p.bounds) + ((static_cast<int64_t>(page[k]) * 2 + w) * G + g) * D;
+                        x[k][w][c].load(row, d, page[k] >= 0 && d < D, D, 0, 0);
+                    }
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) {
+                if ((c0 + c) * 64 >= D) break;
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    float a[PAGES][8];
+#pragma unroll
+                    for (int k = 0; k < PAGES; ++k) x[k][w][c].values(a[k]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        double v[PAGES][2];
+#pragma unroll
+                        for (int k = 0; k < PAGES; ++k) {
+                            v[k][0] = a[k][2 * e];
+                            v[k][1] = a[k][2 * e + 1];
                         }
-                        double wa[8], wc[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            wa[e] = a[e];
-                            wc[e] = c[e];
-                        }
+                        for (int t = 0; t < TOKENS; ++t) {
+                            if (TOKENS > 1 && t >= n) break;
+                            const double2 q = s_q[t][w][((c0 + c) * 4 + e) * 8 + part];
 #pragma unroll
-                        for (int t = 0; t < kScoreTokens; ++t) {
-                            if (i0 + t >= i1) break;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                acc[t] = fma(s_q[i0 + t][0][d + e], wa[e], acc[t]);
-                                acc[t] = fma(s_q[i0 + t][1][d + e], wc[e], acc[t]);
-                            }
+                            for (int k = 0; k < PAGES; ++k) acc[t][k] = fma(q.y, v[k][1], fma(q.x, v[k][0], acc[t][k]));
                         }
                     }
                 }
-#pragma unroll
-                for (int t = 0; t < kScoreTokens; ++t) {
-                    if (i0 + t >= i1) break;
-                    double x = acc[t];
-#pragma unroll
-                    for (int o = 1; o < 8; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-                    if (part == 0 && in && j < s_t[i0 + t].pages)
-                        p.keys[((t0 + i0 + t) * G + g) * p.width + j] = page < 0 ? 0ull : select_key(x);
-                }
             }
         }
-        i0 = i1;
+#pragma unroll
+        for (int t = 0; t < TOKENS; ++t) {
+            if (TOKENS > 1 && t >= n) break;
+            const int pages = TOKENS == 1 ? most : (max(len - (n - 1 - t), 0) + p.c.page_size - 1) / p.c.page_size;
+#pragma unroll
+            for (int k = 0; k < PAGES; ++k) {
+                double x = acc[t][k];
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+                const int j = base + k * GROUPS + group;
+                if (part == 0 && j < stop && j < pages) keys[t * G * p.width + j] = page[k] < 0 ? 0ull : select_key(x);
+            }
+        }
     }
 }
 
@@ -300,12 +343,13 @@ __device__ __forceinline__ int select_scan(int mine, int* x, int warp, int lane,
     return before + inc;
 }
 
-// A block per (token, kv head): the topk-th largest key by radix selection, 11 bits at a time
-// from the highest bit in which the keys differ, then the pages above it and the first of
-// those equal to it, in their order.
+// A block per (token, kv head).  Of the pages that are not always in, the `want`-th largest key
+// by radix selection, 11 bits at a time of what the keys are above the smallest one (scores lie
+// in a few binades: their upper bits alone would tell nothing), then the pages above it and the
+// first of those equal to it, in their order.
 __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __grid_constant__ PagedSelectParams p) {
     extern __shared__ unsigned long long s_keys[];   // [kSelectKeys]
-    __shared__ int s_hist[kSelectBins];
+    __shared__ __align__(16) int s_hist[kSelectBins];
     __shared__ int s_x[kSelectWarps];
     __shared__ unsigned long long s_y[2][kSelectWarps];
     __shared__ int s_digit, s_above, s_same;
@@ -314,6 +358,7 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
     const int64_t t = blockIdx.x / G;   // of this launch
     const int g = blockIdx.x % G;
     const SelectToken tok = select_token(p, p.token0 + t, lane);
+    for (int i = threadIdx.x; i < kSelectBins; i += kSelectThreads) s_hist[i] = 0;
     pdl_wait();
     if (tok.seq < 0) return;
     int32_t* out = p.pages + ((p.token0 + t) * G + g) * p.topk;
@@ -324,49 +369,56 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
         for (int i = threadIdx.x; i < p.topk; i += kSelectThreads) out[i] = i < n ? i : -1;
         return;
     }
-    unsigned long long* mine = p.keys + (t * G + g) * p.width;
-    unsigned long long* keys = n <= kSelectKeys ? s_keys : mine;
-    unsigned long long all = ~0ull, some = 0ull;
-    for (int j = threadIdx.x; j < n; j += kSelectThreads) {
-        const unsigned long long k = j < p.first || j >= n - p.last ? ~0ull : mine[j];
-        keys[j] = k;
-        all &= k;
-        some |= k;
+    // pages [lo, hi) compete for `want` places (first + last <= topk < n: there are some)
+    const int lo = p.first, hi = n - p.last;
+    int want = p.topk - p.first - p.last;
+    const unsigned long long* mine = p.keys + (t * G + g) * p.width;
+    const bool held = n <= kSelectKeys;
+    unsigned long long low = ~0ull, high = 0ull;
+    for (int j = lo + threadIdx.x; j < hi; j += kSelectThreads) {
+        const unsigned long long k = mine[j];
+        if (held) s_keys[j] = k;
+        low = min(low, k);
+        high = max(high, k);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        all &= __shfl_xor_sync(0xffffffffu, all, o);
-        some |= __shfl_xor_sync(0xffffffffu, some, o);
+        low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+        high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
     }
     if (lane == 0) {
-        s_y[0][warp] = all;
-        s_y[1][warp] = some;
+        s_y[0][warp] = low;
+        s_y[1][warp] = high;
     }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kSelectWarps; ++w) {
-        all &= s_y[0][w];
-        some |= s_y[1][w];
+        low = min(low, s_y[0][w]);
+        high = max(high, s_y[1][w]);
     }
-    // bits from `top` on differ somewhere
-    int top = 64 - __clzll(static_cast<long long>(all ^ some));   // 0: all equal
-    unsigned long long known = top == 64 ? 0ull : ~0ull << top, prefix = all & known;
-    int want = p.topk;
-    bool ties = true;   // more keys equal the threshold than are wanted
-    while (top > 0) {
+    auto key = [&](int j) { return (held ? s_keys[j] : mine[j]) - low; };
+    // what the keys are above the smallest has `top` bits
+    int top = 64 - __clzll(static_cast<long long>(high - low));
+    unsigned long long known = top == 64 ? 0ull : ~0ull << top, prefix = 0ull;
+    if (want == 0) prefix = known = ~0ull, top = 0;   // none of them: no key is above or equal (they are below 2^64 - 1)
+    for (bool fresh = true; top > 0; fresh = false) {
         const int shift = max(0, top - kSelectBits), bits = top - shift;
         const unsigned long long mask = (1ull << bits) - 1;
-        for (int i = threadIdx.x; i < kSelectBins; i += kSelectThreads) s_hist[i] = 0;
-        __syncthreads();
-        for (int j = threadIdx.x; j < n; j += kSelectThreads) {
-            const unsigned long long k = keys[j];
+        if (!fresh) {
+            for (int i = threadIdx.x; i < kSelectBins; i += kSelectThreads) s_hist[i] = 0;
+            __syncthreads();
+        }
+        for (int j = lo + threadIdx.x; j < hi; j += kSelectThreads) {
+            const unsigned long long k = key(j);
             if ((k & known) == prefix) atomicAdd(&s_hist[(k >> shift) & mask], 1);
         }
         __syncthreads();
         // thread i holds the digits from kSelectBins - 1 - 4 i down
         int h[4], sum = 0, total;
+        const int4 four = *reinterpret_cast<const int4*>(&s_hist[kSelectBins - 4 - 4 * threadIdx.x]);
+        h[0] = four.w; h[1] = four.z; h[2] = four.y; h[3] = four.x;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += h[i] = s_hist[kSelectBins - 1 - 4 * threadIdx.x - i];
+        for (int i = 0; i < 4; ++i) sum += h[i];
         int above = select_scan(sum, s_x, warp, lane, total) - sum;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -382,28 +434,21 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
         known |= mask << shift;
         want -= s_above;
         top = shift;
-        if (s_same == want) {   // all of them: the bits below do not matter
-            ties = false;
-            break;
-        }
-        __syncthreads();
+        if (s_same == want) break;   // all of them: the bits below do not matter
     }
-    // pages in order: above the threshold, or one of the first `want` equal to it
-    int same = 0, kept = 0;
+    // pages in order: always in, above the threshold, or one of the first `want` equal to it
+    int more = 0, same = 0;   // pages before this round's: taken whatever comes, equal to the threshold
     for (int j0 = 0; j0 < n; j0 += kSelectThreads) {
         const int j = j0 + threadIdx.x;
-        const unsigned long long k = j < n ? keys[j] & known : 0ull;
-        const bool eq = j < n && k == prefix, gt = j < n && k > prefix;
-        bool take = gt || eq;
+        const bool always = j < n && (j < lo || j >= hi);
+        const unsigned long long k = j >= lo && j < hi ? key(j) & known : 0ull;
+        const bool eq = j >= lo && j < hi && k == prefix, gt = always || (j >= lo && j < hi && k > prefix);
         int total;
-        if (ties) {
-            const int at = select_scan(eq ? 1 : 0, s_x, warp, lane, total);
-            take = gt || (eq && same + at <= want);
-            same += total;
-        }
-        const int at = select_scan(take ? 1 : 0, s_x, warp, lane, total);
-        if (take) out[kept + at - 1] = j;
-        kept += total;
+        const int at = select_scan((gt ? 1 << 16 : 0) | (eq ? 1 : 0), s_x, warp, lane, total);
+        const int rank = same + (at & 0xffff);   // among the equal ones, from 1 on
+        if (gt || (eq && rank <= want)) out[more + (at >> 16) + min(rank, want) - 1] = j;
+        more += total >> 16;
+        same += total & 0xffff;
     }
 }
 
