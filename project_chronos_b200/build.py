@@ -1,4 +1,5 @@
-"""Build the sm_100a extension in-tree: project_chronos_b200/libchronos_moe.so.
+"""Build the sm_100a extension in-tree: project_chronos_b200/libchronos_moe.so, and the
+Python module project_chronos_b200/_binding.so that checks tensors and calls it.
 
     python -m project_chronos_b200.build [--force]
 
@@ -14,12 +15,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 LIB = os.path.join(PKG, "libchronos_moe.so")
+BINDING = os.path.join(PKG, "_binding.so")
 OBJ = os.path.join(PKG, "_build")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -46,6 +49,30 @@ def needs_build() -> bool:
     return any(os.path.getmtime(f) > t for f in sources() + headers())
 
 
+def _binding_sources():
+    return [os.path.join(CSRC, "binding.cpp")] + sorted(glob.glob(os.path.join(INCLUDE, "*.h")))
+
+
+def needs_binding() -> bool:
+    if not os.path.exists(BINDING):
+        return True
+    t = os.path.getmtime(BINDING)
+    return any(os.path.getmtime(f) > t for f in _binding_sources())
+
+
+def _binding_command() -> list:
+    """g++ against the headers and libraries of the torch that imports it; the library beside it."""
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(nvcc_path()))
+    return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-I", INCLUDE,
+            "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+            "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(cuda, "include"),
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", os.path.join(CSRC, "binding.cpp"), LIB,
+            "-L", os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN",
+            "-o", BINDING + ".tmp"]
+
+
 def _up_to_date(obj: str) -> bool:
     """Whether the object is newer than every file nvcc read for it (its .d list)."""
     if not (os.path.exists(obj) and os.path.exists(obj + ".d")):
@@ -57,8 +84,18 @@ def _up_to_date(obj: str) -> bool:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and not needs_build():
-        return LIB
+    if force or needs_build():
+        _build_library(force, verbose)
+    if force or needs_binding():
+        cmd = _binding_command()
+        if verbose:
+            print(" ".join(cmd))
+        subprocess.check_call(cmd)
+        os.replace(BINDING + ".tmp", BINDING)
+    return LIB
+
+
+def _build_library(force: bool, verbose: bool) -> None:
     # one object per translation unit, compiled side by side and linked into one library
     flags = [*ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden", "-I", INCLUDE,
              "-I", CSRC, "--expt-relaxed-constexpr", "-cudart", "static"]
@@ -78,9 +115,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
     failed = [cmd for cmd, p in running if p.wait() != 0]
     if failed:
         raise subprocess.CalledProcessError(1, failed[0])
-    subprocess.check_call([nvcc_path(), *ARCH, "--shared", "-cudart", "static", "-o", LIB + ".tmp", *objects])
+    subprocess.check_call([nvcc_path(), *ARCH, "--shared", "-cudart", "static", "-Xlinker", "-soname=" + os.path.basename(LIB),
+                           "-o", LIB + ".tmp", *objects])
     os.replace(LIB + ".tmp", LIB)
-    return LIB
 
 
 if __name__ == "__main__":

@@ -845,43 +845,22 @@ def packed_page_bytes(page_size: int, head_dim: int) -> int:
     return page_size // 16 * 9 * packed_columns(head_dim)
 
 
-def _any_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
-               dt: torch.dtype, d: int, written: bool, dev: torch.device, index: int, grad: bool) -> tuple:
-    """The checked cache part of a call that takes pages of the layer type ``dt`` or, as uint8
-    tensors, of 4-bit values: (cache, packed)."""
-    if k_pages.dtype is not torch.uint8:
-        cache = _paged_cache(k_pages, v_pages, page_table, lens, written, dev, index, grad)
-        if k_pages.dtype is not dt or cache.head_dim != d:
-            raise TypeError(f"pages: {dt} (or uint8) with heads of {d} expected, got {k_pages.dtype} with heads of {cache.head_dim}")
-        return cache, 0
-    code = _DTYPES.get(dt)
-    if code is None:
-        raise TypeError(f"unsupported dtype {dt}")
-    shape = k_pages.shape
-    if len(shape) != 3:
-        raise ValueError(f"4-bit k_pages must be [pages, kv heads, bytes], got {tuple(shape)}")
-    pages, g, nbytes = shape
-    record = 9 * packed_columns(d)
-    if nbytes == 0 or nbytes % record:
-        raise ValueError(f"4-bit pages of heads of {d} have a multiple of {record} bytes, got {nbytes}")
-    ks = _rows("k_pages", k_pages, shape, torch.uint8, index, dev, False)
-    vs = _rows("v_pages", v_pages, shape, torch.uint8, index, dev, False)
-    if written:
-        _written_once("k_pages", shape, ks)
-        _written_once("v_pages", shape, vs)
-    tp, ts, b, width, lp = _table_of(page_table, lens, dev, index)
-    return N.ChronosPagedCache(b, g, d, code, pages, nbytes // record * 16, width, 0, k_pages.data_ptr(), v_pages.data_ptr(),
-                               ks[0], 0, ks[1], vs[0], 0, vs[1], tp, ts, lp), 1
+_native_calls = None
 
 
-def _table_of(page_table: torch.Tensor, lens: torch.Tensor, dev: torch.device, index: int) -> tuple:
-    """(address, row stride, rows, width, address of lens) of a checked page table."""
-    ts = page_table.stride()
-    if page_table.dtype is not torch.int32 or page_table.get_device() != index or len(ts) != 2 \
-            or (ts[1] != 1 and page_table.shape[1] > 1):
-        raise ValueError(f"page_table must be an int32 tensor [B, pages] on {dev} with contiguous rows")
-    b, width = page_table.shape
-    return page_table.data_ptr(), ts[0], b, width, _dense("lens", lens, (b,), torch.int32, index, dev)
+def _calls():
+    """The native module that checks these calls' tensors and makes them (csrc/binding.cpp)."""
+    global _native_calls
+    if _native_calls is None:
+        N.load_library()
+        try:
+            from . import _binding
+        except ImportError as e:
+            raise RuntimeError(f"the native module of the paged calls cannot be loaded ({e}); build it with "
+                               "`python -m project_chronos_b200.build`") from e
+        _binding.init(lambda index: status_word(torch.device("cuda", index)).data_ptr(), N.check)
+        _native_calls = _binding
+    return _native_calls
 
 
 def paged_append_rope(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -906,73 +885,9 @@ def paged_append_rope(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v
     ``paged_append``; a token whose position lies outside the tables is dropped like one
     without a page, and its q and k rows are zeros.  Rows behind the last sequence are left
     as they are."""
-    if not k.is_cuda:
-        _no_cpu(k)
-    dev, index, grad = k.device, k.get_device(), torch.is_grad_enabled()
-    if k.dim() != 3:
-        raise ValueError(f"k must be [tokens, kv heads, head dim], got {tuple(k.shape)}")
-    t, g, d = k.shape
-    dt = k.dtype
-    cache, packed = _any_cache(k_pages, v_pages, page_table, lens, dt, d, True, dev, index, grad)
-    b = cache.batch
-    if cache.kv_heads != g:
-        raise ValueError(f"k has {g} kv heads, the pages {cache.kv_heads}")
-    ks = _rows("k", k, (t, g, d), dt, index, dev, grad)
-    vs = _rows("v", v, (t, g, d), dt, index, dev, grad)
-    h, qs, qo = 0, (0, 0, 1), (0, 0, 1)
-    if q is not None:
-        h = q.shape[1] if q.dim() == 3 else 0
-        if h < 1:
-            raise ValueError(f"q must be [tokens, heads, head dim], got {tuple(q.shape)}")
-        qs = _rows("q", q, (t, h, d), dt, index, dev, grad)
-        if q_out is None:
-            q_out = torch.empty((t, h, d), dtype=dt, device=dev)
-            qo = q_out.stride()
-        else:
-            qo = _rows("q_out", q_out, (t, h, d), dt, index, dev, grad)
-            _written_once("q_out", (t, h, d), qo)
-    elif q_out is not None:
-        raise ValueError("q_out needs q")
-    ko = (0, 0, 1)
-    if k_out is not None:
-        ko = _rows("k_out", k_out, (t, g, d), dt, index, dev, grad)
-        _written_once("k_out", (t, g, d), ko)
-    r, rows, code, cs, ss = 0, 0, 0, (0, 1), (0, 1)
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin go together")
-    if cos is not None:
-        if cos.dim() != 2:
-            raise ValueError(f"cos must be [positions, columns], got {tuple(cos.shape)}")
-        rows, r = cos.shape
-        tt = cos.dtype
-        if tt is not torch.float32 and tt is not dt:
-            raise TypeError(f"cos and sin must be fp32 or {dt}, got {tt}")
-        code = _DTYPES[tt]
-        cs = _rows("cos", cos, (rows, r), tt, index, dev, grad)
-        ss = _rows("sin", sin, (rows, r), tt, index, dev, grad)
-        if seen is None:
-            raise ValueError("the rotation needs seen, the positions of the sequences' next tokens")
-    cap, wp, pp = 0, None, None
-    if weights is not None:
-        cap = weights.shape[-1]
-        wp = _dense("weights", weights, (b, g, cap), torch.float32, index, dev)
-    if positions is not None:
-        if weights is not None and positions.shape[-1] != cap:
-            raise ValueError("weights and positions must have the same number of slots")
-        cap = positions.shape[-1]
-        pp = _dense("positions", positions, (b, g, cap), torch.int32, index, dev)
-    _int32(rope_start=rope_start)
-    args = N.ChronosPagedRopeArgs(
-        cache, packed, h, r, rope_start, rows, code, k_scale, v_scale, t, k.data_ptr(), v.data_ptr(), _ptr(q),
-        None if q is None else q_out.data_ptr(), _ptr(k_out), ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], qo[0], qo[1],
-        ko[0], ko[1], _ptr(cos), _ptr(sin), cs[0], ss[0],
-        None if cu_seqlens is None else _dense("cu_seqlens", cu_seqlens, (b + 1,), torch.int32, index, dev),
-        None if seen is None else _dense("seen", seen, (b,), torch.int32, index, dev), wp, pp, cap,
-        None if lens_out is None else _dense("lens_out", lens_out, (b,), torch.int32, index, dev),
-        None if seen_out is None else _dense("seen_out", seen_out, (b,), torch.int32, index, dev),
-        status_word(dev).data_ptr())
-    _launch(N.load_library().chronos_paged_append_rope, args, index)
-    return q_out
+    return (_native_calls or _calls()).append_rope(
+        k, v, k_pages, v_pages, page_table, lens, seen, cos, sin, q, q_out, k_out, cu_seqlens, rope_start, weights, positions,
+        lens_out, seen_out, k_scale, v_scale)
 
 
 def paged_gather(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
@@ -986,26 +901,7 @@ def paged_gather(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch
     in ``paged_append_rope``.  A slot outside [0, lens[b]) or without a page gives zeros and
     CHRONOS_ERR_INVALID_ARG in the status word; rows behind the last sequence are left as
     they are.  Returns (k_out, v_out)."""
-    if not k_pages.is_cuda:
-        _no_cpu(k_pages)
-    dev, index, grad = k_pages.device, k_pages.get_device(), torch.is_grad_enabled()
-    if k_out.dim() != 3:
-        raise ValueError(f"k_out must be [rows, kv heads, head dim], got {tuple(k_out.shape)}")
-    shape = t, g, d = tuple(k_out.shape)
-    cache, packed = _any_cache(k_pages, v_pages, page_table, lens, k_out.dtype, d, False, dev, index, grad)
-    if cache.kv_heads != g:
-        raise ValueError(f"k_out has {g} kv heads, the pages {cache.kv_heads}")
-    ks = _rows("k_out", k_out, shape, k_out.dtype, index, dev, grad)
-    vs = _rows("v_out", v_out, shape, k_out.dtype, index, dev, grad)
-    _written_once("k_out", shape, ks)
-    _written_once("v_out", shape, vs)
-    b = cache.batch
-    args = N.ChronosPagedGatherArgs(
-        cache, packed, 0, k_scale, v_scale, t, k_out.data_ptr(), v_out.data_ptr(), ks[0], ks[1], vs[0], vs[1],
-        _dense("cu_seqlens", cu_seqlens, (b + 1,), torch.int32, index, dev),
-        None if first is None else _dense("first", first, (b,), torch.int32, index, dev), status_word(dev).data_ptr())
-    _launch(N.load_library().chronos_paged_gather, args, index)
-    return k_out, v_out
+    return (_native_calls or _calls()).gather(k_pages, v_pages, page_table, lens, cu_seqlens, k_out, v_out, first, k_scale, v_scale)
 
 
 def paged_attn_decode4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -1017,39 +913,7 @@ def paged_attn_decode4(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
 
     q [B, heads, D], out [B, heads, D] (may be q) and lse fp32 [B, heads] as there; running sums
     of attention weights are not kept."""
-    if not q.is_cuda:
-        _no_cpu(q)
-    dev, index, grad = q.device, q.get_device(), torch.is_grad_enabled()
-    if q.dim() != 3:
-        raise ValueError(f"q must be [sequences, heads, head dim], got {tuple(q.shape)}")
-    if k_pages.dtype is not torch.uint8:
-        raise TypeError(f"k_pages: uint8 pages of 4-bit values expected, got {k_pages.dtype}")
-    _, h, d = q.shape
-    dt = q.dtype
-    cache, _ = _any_cache(k_pages, v_pages, page_table, lens, dt, d, False, dev, index, grad)
-    shape = (cache.batch, h, d)
-    qs = _rows("q", q, shape, dt, index, dev, grad)
-    out, os = _attention_out(out, q, shape, dt, index, dev, grad)
-    if (window | sinks) >> 31:
-        _int32(window=window, sinks=sinks)
-    args = N.ChronosPagedDecode4Args(
-        cache, h, window, sinks, d ** -0.5 if scale is None else scale, k_scale, v_scale, q.data_ptr(), qs[0], qs[1],
-        out.data_ptr(), os[0], os[1], None if lse is None else _dense("lse", lse, shape[:2], torch.float32, index, dev),
-        None, 0, status_word(dev).data_ptr())
-    lib = N.load_library()
-    ws = _workspace(lib.chronos_paged_decode4_workspace, args, dev, index)  # noqa: F841 (held until the launch)
-    _launch(lib.chronos_paged_decode4, args, index)
-    return out
-
-
-def _attention_out(out, q, shape, dt, index, dev, grad) -> tuple:
-    """The rows that an attention call writes, new or checked, and their strides."""
-    if out is None:
-        out = torch.empty(shape, dtype=dt, device=dev)
-        return out, out.stride()
-    st = _rows("out", out, shape, dt, index, dev, grad)
-    _written_once("out", shape, st)
-    return out, st
+    return (_native_calls or _calls()).decode4(q, k_pages, v_pages, page_table, lens, scale, window, sinks, k_scale, v_scale, out, lse)
 
 
 def paged_bounds(k_pages: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
@@ -1062,30 +926,7 @@ def paged_bounds(k_pages: torch.Tensor, bounds: torch.Tensor, page_table: torch.
     cu_seqlens[b] (``num_tokens``: a bound of how many in all, for the launch; default: no
     bound), lens counting them already.  With ``full`` the pages of all slots, from nothing.
     k_pages as in ``paged_append_rope``.  NaN where a key is.  Returns bounds."""
-    if not k_pages.is_cuda:
-        _no_cpu(k_pages)
-    dev, index, grad = k_pages.device, k_pages.get_device(), torch.is_grad_enabled()
-    if bounds.dim() != 4:
-        raise ValueError(f"bounds must be [pages, 2, kv heads, head dim], got {tuple(bounds.shape)}")
-    d = bounds.shape[3]
-    cache, packed = _any_cache(k_pages, k_pages, page_table, lens, bounds.dtype, d, False, dev, index, grad)
-    at = _bounds_of(bounds, cache, index, dev)
-    if num_tokens is None:
-        num_tokens = cache.batch if cu_seqlens is None else min(cache.batch * cache.table_width * cache.page_size, 0x7FFFFFFF)
-    args = N.ChronosPagedBoundsArgs(
-        cache, packed, 1 if full else 0, k_scale, 0, num_tokens,
-        None if cu_seqlens is None else _dense("cu_seqlens", cu_seqlens, (cache.batch + 1,), torch.int32, index, dev), at,
-        status_word(dev).data_ptr())
-    _launch(N.load_library().chronos_paged_bounds, args, index)
-    return bounds
-
-
-def _bounds_of(bounds: torch.Tensor, cache, index: int, dev: torch.device) -> int:
-    if bounds.dtype not in _DTYPES:
-        raise TypeError(f"unsupported dtype {bounds.dtype}")
-    if bounds.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("forward-only kernels: call under torch.no_grad() or detach the inputs")
-    return _dense("bounds", bounds, (cache.num_pages, 2, cache.kv_heads, cache.head_dim), bounds.dtype, index, dev)
+    return (_native_calls or _calls()).bounds(k_pages, bounds, page_table, lens, cu_seqlens, num_tokens, full, k_scale)
 
 
 def paged_select(q: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, page_size: int,
@@ -1099,40 +940,7 @@ def paged_select(q: torch.Tensor, bounds: torch.Tensor, page_table: torch.Tensor
     The ``first`` pages and the ``last`` (>= 1) up to the token's own are always in, the others
     by the highest sum over the group's heads and columns of max(q lo, q hi), in 64 bits, equal
     ones by the lower page."""
-    if not q.is_cuda:
-        _no_cpu(q)
-    dev, index, grad = q.device, q.get_device(), torch.is_grad_enabled()
-    if q.dim() != 3 or bounds.dim() != 4:
-        raise ValueError(f"q and bounds must be [tokens, heads, head dim] and [pages, 2, kv heads, head dim], "
-                         f"got {tuple(q.shape)} and {tuple(bounds.shape)}")
-    t, h, d = q.shape
-    dt = q.dtype
-    code = _DTYPES.get(dt)
-    if code is None:
-        raise TypeError(f"unsupported dtype {dt}")
-    pages, g = bounds.shape[0], bounds.shape[2]
-    _int32(page_size=page_size, topk=topk, first=first, last=last)
-    tp, ts, b, width, lp = _table_of(page_table, lens, dev, index)
-    cache = N.ChronosPagedCache(b, g, d, code, pages, page_size, width, 0, None, None, 0, 0, 0, 0, 0, 0, tp, ts, lp)
-    if bounds.dtype is not dt:
-        raise TypeError(f"bounds: {dt} expected, got {bounds.dtype}")
-    at = _bounds_of(bounds, cache, index, dev)
-    qs = _rows("q", q, (t, h, d), dt, index, dev, grad)
-    if topk < 1:
-        raise ValueError(f"topk {topk} must be at least 1")
-    if out is None:
-        out = torch.empty((t, g, topk), dtype=torch.int32, device=dev)
-        op = out.data_ptr()
-    else:
-        op = _dense("out", out, (t, g, topk), torch.int32, index, dev)
-    args = N.ChronosPagedSelectArgs(
-        cache, h, topk, first, last, t, q.data_ptr(), qs[0], qs[1], at,
-        None if cu_seqlens is None else _dense("cu_seqlens", cu_seqlens, (b + 1,), torch.int32, index, dev), op, None, 0,
-        status_word(dev).data_ptr())
-    lib = N.load_library()
-    ws = _workspace(lib.chronos_paged_select_workspace, args, dev, index)  # noqa: F841 (held until the launch)
-    _launch(lib.chronos_paged_select, args, index)
-    return out
+    return (_native_calls or _calls()).select(q, bounds, page_table, lens, page_size, topk, first, last, cu_seqlens, out)
 
 
 def paged_attn_sparse(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -1147,26 +955,7 @@ def paged_attn_sparse(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     negative or behind its own page are passed over, one named twice counts twice.  Pages of
     the layer's dtype or of 4-bit values as in ``paged_append_rope``.  Returns out [T, heads, D]
     (zeros where nothing is visible; ``out`` may be q), ``lse`` fp32 [T, heads]."""
-    if not q.is_cuda:
-        _no_cpu(q)
-    dev, index, grad = q.device, q.get_device(), torch.is_grad_enabled()
-    if q.dim() != 3 or pages.dim() != 3:
-        raise ValueError(f"q and pages must be [tokens, heads, head dim] and [tokens, kv heads, n], "
-                         f"got {tuple(q.shape)} and {tuple(pages.shape)}")
-    shape = t, h, d = tuple(q.shape)
-    dt = q.dtype
-    cache, packed = _any_cache(k_pages, v_pages, page_table, lens, dt, d, False, dev, index, grad)
-    qs = _rows("q", q, shape, dt, index, dev, grad)
-    out, os = _attention_out(out, q, shape, dt, index, dev, grad)
-    n = pages.shape[2]
-    args = N.ChronosPagedSparseArgs(
-        cache, packed, h, n, d ** -0.5 if scale is None else scale, k_scale, v_scale, t, q.data_ptr(), qs[0], qs[1],
-        out.data_ptr(), os[0], os[1], None if lse is None else _dense("lse", lse, (t, h), torch.float32, index, dev),
-        _dense("pages", pages, (t, cache.kv_heads, n), torch.int32, index, dev),
-        None if cu_seqlens is None else _dense("cu_seqlens", cu_seqlens, (cache.batch + 1,), torch.int32, index, dev),
-        status_word(dev).data_ptr())
-    _launch(N.load_library().chronos_paged_sparse, args, index)
-    return out
+    return (_native_calls or _calls()).sparse(q, k_pages, v_pages, page_table, lens, pages, cu_seqlens, scale, k_scale, v_scale, out, lse)
 
 
 def profile_begin(max_calls: int) -> None:
