@@ -29,7 +29,7 @@ struct Paged4 {
     static constexpr int kMergeBytes = kPdWarps * 8 * kOStride * 4;
     static constexpr int kSmem = kStages * kStageBytes + kMergeBytes + kPdWarps * 16 * 4;
     static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;      // halves that a query or weight is split into
-    static constexpr int kBlocksPerSm = DP == 256 || (DP == 128 && NT * kTerms > 2) ? 2 : DP == 128 && NT * kTerms > 1 ? 3 : 4;
+    static constexpr int kBlocksPerSm = DP == 256 || (DP == 128 && NT * kTerms > 2) ? 2 : DP == 128 ? 3 : 4;
     static constexpr int kPartBytes = (16 * DP + 32) * 4;      // what a cluster's block leaves for the join
     static_assert(kPartBytes <= kStages * kStageBytes, "the part takes the copies' place");
 };
