@@ -71,6 +71,10 @@ struct RopeRow {
             w[i] = on ? reinterpret_cast<const uint4*>(row + col)[i] : make_uint4(0u, 0u, 0u, 0u);
     }
     __device__ __forceinline__ void values(float (&x)[8]) const { load8<T>(reinterpret_cast<const T*>(w), x); }
+    __device__ __forceinline__ void store(T* row, int col, int) const {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(row + col)[i] = w[i];
+    }
     // Zeros for columns that do not turn.  Whole warps call it.
     __device__ __forceinline__ void partner(float (&x)[8], int lane, bool turns) const {
         RopeRow r;
@@ -100,6 +104,11 @@ struct RopeRow<T, false> {
     __device__ __forceinline__ void values(float (&v)[8]) const {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = x[j];
+    }
+    __device__ __forceinline__ void store(T* row, int col, int D) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (col + j < D) row[col + j] = from_f32<T>(x[j]);
     }
     __device__ __forceinline__ void partner(float (&v)[8], int, bool) const {
 #pragma unroll
@@ -221,35 +230,36 @@ __device__ __forceinline__ uint32_t fp4_block(const float (&y)[8], float top, fl
 template <typename T, typename TT, int LPR, bool VEC, bool PACKED>
 __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) == 4 ? 2 : 3) paged_rope_kernel(const __grid_constant__ PagedRopeParams p) {
     constexpr int RPW = 32 / LPR;                       // rows of a warp at once
-    constexpr int U = sizeof(T) == 2 && VEC && !PACKED ? 4 : 2;    // ... and so many times that in flight
+    constexpr int UK = VEC ? 2 : 1, UQ = sizeof(T) == 2 && VEC ? (PACKED ? 2 : 4) : 1;   // ... and so many times that in flight
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int slice = warp % p.slices;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * (kRopeWarps / p.slices) + warp / p.slices;
+    const int t = static_cast<int>(blockIdx.x) * (kRopeWarps / p.slices) + warp / p.slices;   // (tokens are below 2^28)
     const int G = p.c.kv_heads, D = p.c.head_dim;
     const int sub = lane / LPR, col = lane % LPR * 8;
     const bool on = col < D;
-    // units of RPW rows of one kind: first those of K, then V, then the queries
-    const int uk = (G + RPW - 1) / RPW, units = 2 * uk + (p.heads + RPW - 1) / RPW;
-    const T* src_k = static_cast<const T*>(p.k) + t * p.k_row + sub * p.k_head;
-    const T* src_v = static_cast<const T*>(p.v) + t * p.v_row + sub * p.v_head;
-    const T* src_q = static_cast<const T*>(p.q) + t * p.q_row + sub * p.q_head;
-    auto fetch = [&](RopeRow<T, VEC>& x, int u) {
-        const bool is_k = u < uk, is_q = u >= 2 * uk;
-        const int row = (is_k ? u : is_q ? u - 2 * uk : u - uk) * RPW;
-        const T* src = is_k ? src_k + row * p.k_head : is_q ? src_q + row * p.q_head : src_v + row * p.v_head;
-        x.load(src, col, on && u < units && row + sub < (is_q ? p.heads : G) && t < p.tokens, D, p.start, p.dim);
-    };
-    // the first rows are on their way while the token's place is looked up
-    RopeRow<T, VEC> x[U];
-    int u0 = slice;
+    // rows of one kind, RPW at a time: this warp's begin at `sub + slice * RPW` and lie `step` units apart
+    const int uk = (G + RPW - 1) / RPW, uq = (p.heads + RPW - 1) / RPW, step = p.slices * RPW;
+    const int row0 = slice * RPW + sub;
+    const T* src_k = static_cast<const T*>(p.k) + t * p.k_row + row0 * p.k_head + (VEC ? col : 0);
+    const T* src_v = static_cast<const T*>(p.v) + t * p.v_row + row0 * p.v_head + (VEC ? col : 0);
+    const T* src_q = static_cast<const T*>(p.q) + t * p.q_row + row0 * p.q_head + (VEC ? col : 0);
+    const int at_col = VEC ? 0 : col;
+    // the first rows of every kind are on their way while the token's place is looked up
+    RopeRow<T, VEC> xk[UK], xv[UK], xq[UQ];
+    auto fetch = [&](auto& x, const T* src, int64_t head, int row, int rows) {
 #pragma unroll
-    for (int n = 0; n < U; ++n) fetch(x[n], u0 + n * p.slices);
+        for (int n = 0; n < static_cast<int>(sizeof(x) / sizeof(x[0])); ++n)
+            x[n].load(src + n * step * head, at_col, on && row + n * step < rows && t < p.tokens, D, p.start, p.dim);
+    };
+    fetch(xk, src_k, p.k_head, row0, G);
+    fetch(xv, src_v, p.v_head, row0, G);
+    fetch(xq, src_q, p.q_head, row0, p.heads);
 
     int b = -1, page = -1, in_page = 0;
     int64_t i = 0, slot = 0, at = 0;
     bool placed = false;    // at a position of the tables
     if (t < p.tokens) {
-        b = p.cu == nullptr ? static_cast<int>(t) : paged_sequence(p.cu, p.c.batch, t, lane);
+        b = p.cu == nullptr ? t : paged_sequence(p.cu, p.c.batch, t, lane);
         if (b >= p.c.batch) b = -1;   // a row behind the last sequence
         if (b >= 0 && p.cu != nullptr) {
             i = t - p.cu[b];
@@ -278,7 +288,7 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) =
         }
     }
     if (b < 0) return;
-    if (slice == 0 && page >= 0)
+    if (slice == 0 && page >= 0 && (p.weights != nullptr || p.positions != nullptr))
         for (int g = lane; g < G; g += 32) {
             const int64_t w = (static_cast<int64_t>(b) * G + g) * p.slot_cap + slot;
             if (p.weights != nullptr) p.weights[w] = 0.0f;
@@ -333,22 +343,29 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) =
             y[j] = fmaf(y[j], cs[j], w[j]);
         }
     };
-    // where this lane's codes and (every other lane's) scales of K and V rows lie
+    // where this lane's part of the slot's first row lies
     const int line = in_page & 15;
-    const int64_t rec = static_cast<int64_t>(in_page >> 4) * fp4_record(p.columns);
-    uint8_t* kp = static_cast<uint8_t*>(p.c.k_pages) + page * p.c.k_page_stride + rec + sub * p.c.k_head_stride;
-    uint8_t* vp = static_cast<uint8_t*>(p.c.v_pages) + page * p.c.v_page_stride + rec + sub * p.c.v_head_stride;
-    const int at_codes = line * (p.columns / 2) + col / 2, at_scale = 8 * p.columns + line * (p.columns / 16) + col / 16;
-    auto put4 = [&](uint32_t codes, uint32_t scale, bool is_k, int base) {
-        uint8_t* record = is_k ? kp + base * p.c.k_head_stride : vp + base * p.c.v_head_stride;
-        if (base + sub < G && col < p.columns) {
-            *reinterpret_cast<uint32_t*>(record + at_codes) = codes;
-            if ((col & 8) == 0) record[at_scale] = static_cast<uint8_t>(scale);
+    uint8_t *kp, *vp;   // packed: codes (and `to_scale` on from there the scales); else columns
+    int64_t kh = p.c.k_head_stride, vh = p.c.v_head_stride;
+    const int to_scale = 8 * p.columns + line * (p.columns / 16) + col / 16 - (line * (p.columns / 2) + col / 2);
+    if constexpr (PACKED) {
+        const int64_t in = static_cast<int64_t>(in_page >> 4) * fp4_record(p.columns) + line * (p.columns / 2) + col / 2;
+        kp = static_cast<uint8_t*>(p.c.k_pages) + page * p.c.k_page_stride + in + row0 * kh;
+        vp = static_cast<uint8_t*>(p.c.v_pages) + page * p.c.v_page_stride + in + row0 * vh;
+    } else {
+        kh *= sizeof(T);
+        vh *= sizeof(T);
+        kp = reinterpret_cast<uint8_t*>(static_cast<T*>(p.c.k_pages) + page * p.c.k_page_stride + in_page * p.c.k_slot_stride) + row0 * kh;
+        vp = reinterpret_cast<uint8_t*>(static_cast<T*>(p.c.v_pages) + page * p.c.v_page_stride + in_page * p.c.v_slot_stride) + row0 * vh;
+    }
+    auto put4 = [&](uint32_t codes, uint32_t scale, uint8_t* to, bool has) {
+        if (has && col < p.columns) {
+            *reinterpret_cast<uint32_t*>(to) = codes;
+            if ((col & 8) == 0) to[to_scale] = static_cast<uint8_t>(scale);
         }
     };
-    // rows base.. of K or V into their records; true where one has to be done in 64 bits
-    auto store4 = [&](float (&y)[8], float most, bool turned, bool is_k, int base) {
-        const float unit = is_k ? p.k_unit : p.v_unit;
+    // rows of K or V into their records; true where one has to be done in 64 bits
+    auto store4 = [&](float (&y)[8], float most, bool turned, bool whole, float unit, uint8_t* to, bool has) {
         if (unit != 1.0f) {
             most *= unit;
 #pragma unroll
@@ -358,82 +375,108 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) =
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = max_magnitude(top, y[j]);
         // |x c| + |x' s| <= |y| + 2 |x' s|; fp32 values that are exact need the room of r and the product only
-        const float off = turned || !(is_k ? p.k_exact : p.v_exact) || sizeof(T) == 4 ? fmaf(2.0f, most, top) : 0.0f;
+        const float off = turned || !whole || sizeof(T) == 4 ? fmaf(2.0f, most, top) : 0.0f;
         uint32_t scale;
         bool open;
         const uint32_t codes = fp4_block<T>(y, top, off, scale, open);
-        put4(codes, scale, is_k, base);
-        return __any_sync(0xffffffffu, open && base + sub < G) != 0;
+        put4(codes, scale, to, has);
+        return __any_sync(0xffffffffu, open && has) != 0;
     };
-    for (; u0 < units; u0 += p.slices * U) {
-        if (u0 != slice)
+    // ... which is done here, a warp in some thousand
+    auto again4 = [&](const T* src, bool turned, float factor, uint8_t* to, bool has) {
+        const RopeSource<T, TT> from64{has ? src - (VEC ? col : 0) : nullptr, turned ? cos : nullptr, sin, col, D, p.start, p.dim, factor};
+        uint32_t scale;
+        const uint32_t codes = fp4_block_exact<T, TT>(from64, &scale);
+        put4(codes, scale, to, has);
+    };
+    auto clear = [&](float (&y)[8]) {   // stored nowhere: q_out and k_out are zeros
+        if (!placed)
 #pragma unroll
-            for (int n = 0; n < U; ++n) fetch(x[n], u0 + n * p.slices);
-        __syncwarp();   // q_out may be q, k_out k: a row is read before it is written over
+            for (int j = 0; j < 8; ++j) y[j] = 0.0f;
+    };
+
+    // (a row is read before it is written over: q_out may be q, k_out k)
+    T* k_out = static_cast<T*>(p.k_out) + t * p.ko_row + row0 * p.ko_head;
+    for (int u = slice, row = row0; u < uk; u += p.slices * UK, row += step * UK) {
+        if (u != slice) fetch(xk, src_k, p.k_head, row, G);
+        __syncwarp();
         uint32_t again = 0;
 #pragma unroll
-        for (int n = 0; n < U; ++n) {
-            const int u = u0 + n * p.slices;
-            if (u >= units) break;
+        for (int n = 0; n < UK; ++n) {
+            if (u + n * p.slices >= uk) break;
+            const bool has = row + n * step < G;
             float y[8], most;
-            if (u >= 2 * uk) {
-                const int row = (u - 2 * uk) * RPW + sub;
-                rotate(x[n], y, most);
-                if (!placed)   // stored nowhere: zeros
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) y[j] = 0.0f;
-                if (on && row < p.heads) rope_store<T, VEC>(static_cast<T*>(p.q_out) + t * p.qo_row + row * p.qo_head, y, col, D);
-            } else if (u < uk) {
-                const int row = u * RPW + sub;
-                rotate(x[n], y, most);
-                if (!placed)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) y[j] = 0.0f;
-                T* out = static_cast<T*>(p.k_out) + t * p.ko_row + row * p.ko_head;
-                if constexpr (PACKED) {
+            rotate(xk[n], y, most);
+            if constexpr (PACKED) {
+                if (page >= 0) {
                     float z[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) z[j] = y[j];
-                    if (page >= 0 && store4(z, most, turns, true, u * RPW)) again |= 1u << n;   // k_out may be k: written then
-                    else if (p.k_out != nullptr && on && row < G) rope_store<T, VEC>(out, y, col, D);
-                } else if (on && row < G) {
-                    if (page >= 0)
-                        rope_store<T, VEC>(static_cast<T*>(p.c.k_pages) + page * p.c.k_page_stride + in_page * p.c.k_slot_stride +
-                                               row * p.c.k_head_stride, y, col, D);
-                    if (p.k_out != nullptr) rope_store<T, VEC>(out, y, col, D);
+                    if (store4(z, most, turns, p.k_exact, p.k_unit, kp + n * step * kh, has)) again |= 1u << n;
                 }
-            } else if (page >= 0) {
-                const int row = (u - uk) * RPW + sub;
-                x[n].values(y);
-                if constexpr (PACKED) {
-                    if (store4(y, 0.0f, false, false, (u - uk) * RPW)) again |= 1u << n;
-                } else if (on && row < G) {
-                    rope_store<T, VEC>(static_cast<T*>(p.c.v_pages) + page * p.c.v_page_stride + in_page * p.c.v_slot_stride +
-                                           row * p.c.v_head_stride, y, col, D);
-                }
+            } else if (page >= 0 && on && has) {
+                rope_store<T, VEC>(reinterpret_cast<T*>(kp + n * step * kh), y, col, D);
+            }
+            if (p.k_out != nullptr && ((again >> n) & 1u) == 0u) {
+                clear(y);
+                if (on && has) rope_store<T, VEC>(k_out + n * step * p.ko_head, y, col, D);
             }
         }
-        if constexpr (PACKED) {
-            while (again != 0u) {   // a warp in some thousand
-                const int u = u0 + (__ffs(again) - 1) * p.slices;
-                again &= again - 1;
-                const bool is_k = u < uk;
-                const int row = (is_k ? u : u - uk) * RPW + sub;
-                const RopeSource<T, TT> src{row < G ? (is_k ? src_k + u * RPW * p.k_head : src_v + (u - uk) * RPW * p.v_head) : nullptr,
-                                            is_k && turns ? cos : nullptr, sin, col, D, p.start, p.dim, is_k ? p.k_scale : p.v_scale};
-                uint32_t scale;
-                const uint32_t codes = fp4_block_exact<T, TT>(src, &scale);
-                put4(codes, scale, is_k, row - sub);
-                if (is_k && p.k_out != nullptr) {
-                    RopeRow<T, VEC> r;
-                    fetch(r, u);
+        if constexpr (PACKED)
+            for (; again != 0u; again &= again - 1) {
+                const int n = __ffs(again) - 1;
+                const bool has = row + n * step < G;
+                again4(src_k + n * step * p.k_head, turns, p.k_scale, kp + n * step * kh, has);
+                if (p.k_out != nullptr) {
+                    RopeRow<T, VEC> x;
+                    x.load(src_k + n * step * p.k_head, at_col, on && has, D, p.start, p.dim);
                     __syncwarp();
                     float y[8], most;
-                    rotate(r, y, most);
-                    if (on && row < G) rope_store<T, VEC>(static_cast<T*>(p.k_out) + t * p.ko_row + row * p.ko_head, y, col, D);
+                    rotate(x, y, most);
+                    if (on && has) rope_store<T, VEC>(k_out + n * step * p.ko_head, y, col, D);
                 }
             }
+        src_k += step * UK * p.k_head;
+        kp += step * UK * kh;
+        k_out += step * UK * p.ko_head;
+    }
+    for (int u = slice, row = row0; page >= 0 && u < uk; u += p.slices * UK, row += step * UK) {
+        if (u != slice) fetch(xv, src_v, p.v_head, row, G);
+        uint32_t again = 0;
+#pragma unroll
+        for (int n = 0; n < UK; ++n) {
+            if (u + n * p.slices >= uk) break;
+            const bool has = row + n * step < G;
+            if constexpr (PACKED) {
+                float y[8];
+                xv[n].values(y);
+                if (store4(y, 0.0f, false, p.v_exact, p.v_unit, vp + n * step * vh, has)) again |= 1u << n;
+            } else if (on && has) {
+                xv[n].store(reinterpret_cast<T*>(vp + n * step * vh), col, D);
+            }
         }
+        if constexpr (PACKED)
+            for (; again != 0u; again &= again - 1) {
+                const int n = __ffs(again) - 1;
+                again4(src_v + n * step * p.v_head, false, p.v_scale, vp + n * step * vh, row + n * step < G);
+            }
+        src_v += step * UK * p.v_head;
+        vp += step * UK * vh;
+    }
+    T* q_out = static_cast<T*>(p.q_out) + t * p.qo_row + row0 * p.qo_head;
+    for (int u = slice, row = row0; u < uq; u += p.slices * UQ, row += step * UQ) {
+        if (u != slice) fetch(xq, src_q, p.q_head, row, p.heads);
+        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < UQ; ++n) {
+            if (u + n * p.slices >= uq) break;
+            float y[8], most;
+            rotate(xq[n], y, most);
+            clear(y);
+            if (on && row + n * step < p.heads) rope_store<T, VEC>(q_out + n * step * p.qo_head, y, col, D);
+        }
+        src_q += step * UQ * p.q_head;
+        q_out += step * UQ * p.qo_head;
     }
 }
 

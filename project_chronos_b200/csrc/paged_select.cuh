@@ -135,26 +135,9 @@ struct PagedSelectParams {
     int max_slots;
     int64_t width;              // keys per token and kv head
     unsigned long long* keys;   // [tokens][kv heads][width]
-    int chunk, chunks;          // pages of a block, blocks of a row
+    int cluster;                // blocks per tile and kv head
     int32_t* status;
 };
-
-// A token's sequence (-1: none), the slots at or before it and their pages.
-struct SelectToken {
-    int seq, len, pages;
-};
-__device__ __forceinline__ SelectToken select_token(const PagedSelectParams& p, int64_t t, int lane) {
-    SelectToken r{};
-    r.seq = p.cu == nullptr ? static_cast<int>(t) : paged_sequence(p.cu, p.c.batch, t, lane);
-    if (r.seq >= p.c.batch || (p.cu != nullptr && t < p.cu[r.seq])) {
-        r.seq = -1;
-        return r;
-    }
-    r.len = min(max(p.c.lens[r.seq], 0), p.max_slots);
-    if (p.cu != nullptr) r.len = static_cast<int>(max(int64_t{0}, r.len - (static_cast<int64_t>(p.cu[r.seq + 1]) - 1 - t)));
-    r.pages = (r.len + p.c.page_size - 1) / p.c.page_size;
-    return r;
-}
 
 // A score's place in the order of numbers: -0 as 0, NaN above every number (and 0 for a page
 // that is none).
@@ -164,31 +147,167 @@ __device__ __forceinline__ unsigned long long select_key(double x) {
     return (u >> 63) ? ~u : (u | (1ull << 63));
 }
 
-constexpr int kScoreThreads = 256;
-constexpr int kScoreTokens = 8;     // tokens of one sequence that share the reading of a page
-constexpr int kScorePages = 512;    // pages of a block at most
+constexpr int kSelectThreads = 256;
+constexpr int kSelectWarps = kSelectThreads / 32;
+constexpr int kSelectTokens = 8;    // tokens of one sequence that share the reading of a page
+constexpr int kSelectPages = 512;   // pages whose numbers a block holds at a time
+constexpr int kSelectBits = 11, kSelectBins = 1 << kSelectBits;
+constexpr int kSelectKeys = 6144;   // keys that shared memory holds (48 KB of them)
 
-// Bound by reading the bounds.  8 lanes share a page, two pages at a time (16-bit types), whose loads
-// all go out before the first is used; each lane takes every eighth group of 8 columns of lo and hi, and
-// the partial sums meet in three shuffles.  Block: up to kScorePages pages, a kv head, TOKENS
-// tokens of a sequence (1 where every sequence has one).  The queries' sums lie in shared memory
-// so that the 8 lanes' parts are side by side, the pages' numbers beside them: both are fetched
-// at once.  32 rows of 256 to 512 pages, 8 heads of 128: 52 us with a look-up before every page.
+// Inclusive sum over the block's threads of their counts (x: kSelectWarps ints of shared
+// memory, free before and after); total: of all.
+__device__ __forceinline__ int select_scan(int mine, int* x, int warp, int lane, int& total) {
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+    }
+    __syncthreads();
+    if (lane == 31) x[warp] = inc;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kSelectWarps; ++w) {
+        before += w < warp ? x[w] : 0;
+        total += x[w];
+    }
+    return before + inc;
+}
+
+struct SelectShared {
+    __align__(16) int hist[kSelectBins];
+    int scan[kSelectWarps];
+    unsigned long long ends[2][kSelectWarps];
+    int digit, above, same;
+};
+
+// The pages of one token and kv head, by a block.  Of the pages that are not always in, the
+// `want`-th largest key by radix selection, 11 bits at a time of what the keys are above the
+// smallest one (scores lie in a few binades: their upper bits alone would tell nothing), then the
+// pages above it and the first of those equal to it, in their order.  n: the token's pages.
+__device__ __forceinline__ void select_row(const PagedSelectParams& p, SelectShared& s, unsigned long long* held, const unsigned long long* mine,
+                                           int32_t* out, int n) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (n <= p.topk) {
+        for (int i = threadIdx.x; i < p.topk; i += kSelectThreads) out[i] = i < n ? i : -1;
+        return;
+    }
+    // pages [lo, hi) compete for `want` places (first + last <= topk < n: there are some)
+    const int lo = p.first, hi = n - p.last;
+    int want = p.topk - p.first - p.last;
+    const bool fits = n <= kSelectKeys;
+    for (int i = threadIdx.x; i < kSelectBins; i += kSelectThreads) s.hist[i] = 0;
+    unsigned long long low = ~0ull, high = 0ull;
+#pragma unroll 4
+    for (int j = lo + threadIdx.x; j < hi; j += kSelectThreads) {
+        const unsigned long long k = mine[j];
+        if (fits) held[j] = k;
+        low = min(low, k);
+        high = max(high, k);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+        high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
+    }
+    if (lane == 0) {
+        s.ends[0][warp] = low;
+        s.ends[1][warp] = high;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSelectWarps; ++w) {
+        low = min(low, s.ends[0][w]);
+        high = max(high, s.ends[1][w]);
+    }
+    auto key = [&](int j) { return (fits ? held[j] : mine[j]) - low; };
+    // what the keys are above the smallest has `top` bits
+    int top = 64 - __clzll(static_cast<long long>(high - low));
+    unsigned long long known = top == 64 ? 0ull : ~0ull << top, prefix = 0ull;
+    if (want == 0) prefix = known = ~0ull, top = 0;   // none of them: no key is above or equal (they are below 2^64 - 1)
+    for (bool fresh = true; top > 0; fresh = false) {
+        const int shift = max(0, top - kSelectBits), bits = top - shift;
+        const unsigned long long mask = (1ull << bits) - 1;
+        if (!fresh) {
+            for (int i = threadIdx.x; i < kSelectBins; i += kSelectThreads) s.hist[i] = 0;
+            __syncthreads();
+        }
+        for (int j = lo + threadIdx.x; j < hi; j += kSelectThreads) {
+            const unsigned long long k = key(j);
+            if ((k & known) == prefix) atomicAdd(&s.hist[(k >> shift) & mask], 1);
+        }
+        __syncthreads();
+        // thread i holds the digits from kSelectBins - 1 - PER i down
+        constexpr int PER = kSelectBins / kSelectThreads;
+        static_assert(PER % 4 == 0, "whole vectors");
+        int h[PER], sum = 0, total;
+#pragma unroll
+        for (int i = 0; i < PER / 4; ++i) {
+            const int4 four = *reinterpret_cast<const int4*>(&s.hist[kSelectBins - PER * threadIdx.x - 4 * i - 4]);
+            h[4 * i] = four.w; h[4 * i + 1] = four.z; h[4 * i + 2] = four.y; h[4 * i + 3] = four.x;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) sum += h[i];
+        int above = select_scan(sum, s.scan, warp, lane, total) - sum;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (above < want && above + h[i] >= want) {
+                s.digit = kSelectBins - 1 - PER * threadIdx.x - i;
+                s.above = above;
+                s.same = h[i];
+            }
+            above += h[i];
+        }
+        __syncthreads();
+        prefix |= static_cast<unsigned long long>(s.digit) << shift;
+        known |= mask << shift;
+        want -= s.above;
+        top = shift;
+        if (s.same == want) break;   // all of them: the bits below do not matter
+    }
+    // pages in order: always in, above the threshold, or one of the first `want` equal to it
+    int more = 0, same = 0;   // pages before this round's: taken whatever comes, equal to the threshold
+    for (int j0 = 0; j0 < n; j0 += kSelectThreads) {
+        const int j = j0 + threadIdx.x;
+        const bool inside = j >= lo && j < hi, always = j < n && !inside;
+        const unsigned long long k = inside ? key(j) & known : 0ull;
+        const bool eq = inside && k == prefix, gt = always || (inside && k > prefix);
+        int total;
+        const int at = select_scan((gt ? 1 << 16 : 0) | (eq ? 1 : 0), s.scan, warp, lane, total);
+        const int rank = same + (at & 0xffff);   // among the equal ones, from 1 on
+        if (gt || (eq && rank <= want)) out[more + (at >> 16) + min(rank, want) - 1] = j;
+        more += total >> 16;
+        same += total & 0xffff;
+    }
+}
+
+// Bound by reading the bounds.  A cluster of p.cluster blocks per TOKENS tokens of a sequence (1
+// where every sequence has one) and kv head.  Scores: the blocks share the pages, 8 lanes a
+// page, two pages at a time (16-bit types), whose loads all go out before the first is used; each
+// lane takes every eighth group of 8 columns of lo and hi, and the partial sums meet in three
+// shuffles.  The queries' sums lie in shared memory so that the 8 lanes' parts are side by side,
+// the pages' numbers beside them: both are fetched at once.  Then the blocks share the tokens'
+// selections.  32 rows of 256 to 512 pages, 8 heads of 128: 52 us with a look-up before every
+// page; scores and selection in one kernel save the start of another and its reading.
 template <typename T, bool VEC, int TOKENS>
-__global__ void __launch_bounds__(kScoreThreads, TOKENS == 1 ? 3 : 2) paged_score_kernel(const __grid_constant__ PagedSelectParams p) {
-    constexpr int MAXD = CHRONOS_PAGED_MAX_HEAD_DIM, GROUPS = kScoreThreads / 8;
+__global__ void __launch_bounds__(kSelectThreads, TOKENS == 1 ? 3 : 2) paged_select_kernel(const __grid_constant__ PagedSelectParams p) {
+    constexpr int MAXD = CHRONOS_PAGED_MAX_HEAD_DIM, GROUPS = kSelectThreads / 8;
     constexpr int PAGES = sizeof(T) == 2 && VEC ? 2 : 1, CHUNKS = PAGES;   // pages and 64 columns that are in flight at once
+    constexpr int ROUND = PAGES * GROUPS;                                  // pages of a block at once
+    extern __shared__ unsigned long long s_keys[];                         // [kSelectKeys]
     __shared__ __align__(16) double2 s_q[TOKENS][2][MAXD / 2];   // down, up; columns 64 c + 8 part + 2 e, + 1 at (4 c + e) * 8 + part
-    __shared__ int s_page[kScorePages];
-    const int G = p.c.kv_heads, D = p.c.head_dim, block = blockIdx.x % p.chunks, g = blockIdx.x / p.chunks % G;
+    __shared__ int s_page[kSelectPages];
+    __shared__ SelectShared s_sel;
+    const int G = p.c.kv_heads, D = p.c.head_dim, C = p.cluster;
+    const int rank = blockIdx.x % C, g = blockIdx.x / C % G, tile = blockIdx.x / C / G;
     const int lane = threadIdx.x & 31;
-    const int j0 = block * p.chunk;
-    // the block's tokens: [t0, t0 + n) of sequence seq, the last of which sees `len` slots
-    int64_t t0 = blockIdx.x / p.chunks / G + p.token0;
+    // the tokens: [t0, t0 + n) of sequence seq, the last of which sees `len` slots
+    int64_t t0 = p.token0 + tile;
     int seq = static_cast<int>(t0), n = 1;
     if (p.cu != nullptr) {
-        // tile `tile` of the list of all sequences' tiles of TOKENS tokens (this launch has tokens token0 ..)
-        const int tile = static_cast<int>(blockIdx.x / p.chunks / G);
+        // `tile` of the list of all sequences' tiles of TOKENS tokens (this launch has tokens token0 ..)
         int before = 0;
         seq = -1;
         for (int base = 0; base < p.c.batch && seq < 0; base += 32) {
@@ -215,240 +334,121 @@ __global__ void __launch_bounds__(kScoreThreads, TOKENS == 1 ? 3 : 2) paged_scor
             }
             before += __shfl_sync(0xffffffffu, inc, 31);
         }
-        if (seq < 0) return;   // more blocks than tiles
+        if (seq < 0) return;   // more clusters than tiles
     }
-    const int raw = min(max(p.c.lens[seq], 0), p.max_slots);
-    // slots at or before the last token, and before that one
-    const int len = p.cu == nullptr ? raw : static_cast<int>(max(int64_t{0}, raw - (static_cast<int64_t>(p.cu[seq + 1]) - (t0 + n))));
-    const int most = (len + p.c.page_size - 1) / p.c.page_size, stop = min(j0 + p.chunk, most);
-    if (most <= p.topk || j0 >= most) return;   // all pages are taken: no scores
-    for (int j = j0 + threadIdx.x; j < stop; j += kScoreThreads) {
-        const int page = p.c.page_table[seq * p.c.page_table_stride + j];
-        const bool none = page < 0 || page >= p.c.num_pages;
-        if (none) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
-        s_page[j - j0] = none ? -1 : page;
-    }
-    const int D64 = (D + 63) & ~63;
-    for (int i = threadIdx.x; i < n * D64; i += kScoreThreads) {
-        const int t = i / D64, d = i % D64;
-        double up = 0.0, down = 0.0;
-        if (d < D) {
-            const T* q = static_cast<const T*>(p.q) + (t0 + t) * p.q_row + static_cast<int64_t>(g) * p.rep * p.q_head + d;
+    const int raw = p.c.lens[seq], cut = min(max(raw, 0), p.max_slots);
+    if (raw != cut && blockIdx.x % (C * G) == 0 && threadIdx.x == 0) report_status(p.status, CHRONOS_ERR_INVALID_ARG);
+    const int len = p.cu == nullptr ? cut : static_cast<int>(max(int64_t{0}, cut - (static_cast<int64_t>(p.cu[seq + 1]) - (t0 + n))));
+    const int most = (len + p.c.page_size - 1) / p.c.page_size;
+    unsigned long long* keys = p.keys + ((t0 - p.token0) * G + g) * p.width;   // of token t: t * G * width on
+    auto pages_of = [&](int t) { return TOKENS == 1 ? most : (max(len - (n - 1 - t), 0) + p.c.page_size - 1) / p.c.page_size; };
+    if (most > p.topk) {   // (else all pages are taken: no scores)
+        const int D64 = (D + 63) & ~63;
+        for (int i = threadIdx.x; i < n * D64; i += kSelectThreads) {
+            const int t = i / D64, d = i % D64;
+            double up = 0.0, down = 0.0;
+            if (d < D) {
+                const T* q = static_cast<const T*>(p.q) + (t0 + t) * p.q_row + static_cast<int64_t>(g) * p.rep * p.q_head + d;
 #pragma unroll 4
-            for (int h = 0; h < p.rep; ++h) {
-                const float x = to_f32<T>(q[h * p.q_head]);
-                if (x > 0.0f) up += x;
-                else down += x;   // and NaN
+                for (int h = 0; h < p.rep; ++h) {
+                    const float x = to_f32<T>(q[h * p.q_head]);
+                    if (x > 0.0f) up += x;
+                    else down += x;   // and NaN
+                }
             }
+            const int at = 2 * (((d >> 6) * 4 + ((d & 7) >> 1)) * 8 + ((d >> 3) & 7)) + (d & 1);
+            reinterpret_cast<double*>(s_q[t][0])[at] = down;
+            reinterpret_cast<double*>(s_q[t][1])[at] = up;
         }
-        const int at = 2 * (((d >> 6) * 4 + ((d & 7) >> 1)) * 8 + ((d >> 3) & 7)) + (d & 1);
-        reinterpret_cast<double*>(s_q[t][0])[at] = down;
-        reinterpret_cast<double*>(s_q[t][1])[at] = up;
-    }
-    __syncthreads();
-    const int part = threadIdx.x & 7, group = threadIdx.x >> 3;
-    unsigned long long* keys = p.keys + ((t0 - p.token0) * G + g) * p.width;
-    for (int base = j0; base < stop; base += PAGES * GROUPS) {
-        double acc[TOKENS][PAGES];
-        int page[PAGES];
+        const int part = threadIdx.x & 7, group = threadIdx.x >> 3;
+        // rounds of ROUND pages go to the blocks in turn, kSelectPages / ROUND rounds of this block at a time
+        constexpr int ROUNDS = kSelectPages / ROUND;
+        for (int r0 = 0; (r0 * C + rank) * ROUND < most; r0 += ROUNDS) {
+            if (r0 > 0) __syncthreads();   // the numbers before are read
+            for (int i = threadIdx.x; i < kSelectPages; i += kSelectThreads) {
+                const int64_t j = (static_cast<int64_t>(r0 + i / ROUND) * C + rank) * ROUND + i % ROUND;
+                int page = -1;
+                if (j < most) {
+                    page = p.c.page_table[seq * p.c.page_table_stride + j];
+                    if (page < 0 || page >= p.c.num_pages) {
+                        report_status(p.status, CHRONOS_ERR_INVALID_ARG);
+                        page = -1;
+                    }
+                }
+                s_page[i] = page;
+            }
+            __syncthreads();
+            for (int r = 0; r < ROUNDS && ((r0 + r) * C + rank) * ROUND < most; ++r) {
+                const int j0 = ((r0 + r) * C + rank) * ROUND + group;
+                double acc[TOKENS][PAGES];
+                int page[PAGES];
 #pragma unroll
-        for (int k = 0; k < PAGES; ++k) {
-            const int j = base + k * GROUPS + group;
-            page[k] = j < stop ? s_page[j - j0] : -1;
+                for (int k = 0; k < PAGES; ++k) {
+                    page[k] = s_page[r * ROUND + k * GROUPS + group];
 #pragma unroll
-            for (int t = 0; t < TOKENS; ++t) acc[t][k] = 0.0;
-        }
-        for (int c0 = 0; c0 * 64 < D; c0 += CHUNKS) {
-            RopeRow<T, VEC> x[PAGES][2][CHUNKS];   // page, lo or hi, 64 columns
+                    for (int t = 0; t < TOKENS; ++t) acc[t][k] = 0.0;
+                }
+                for (int c0 = 0; c0 * 64 < D; c0 += CHUNKS) {
+                    RopeRow<T, VEC> x[PAGES][2][CHUNKS];   // page, lo or hi, 64 columns
 #pragma unroll
-            for (int k = 0; k < PAGES; ++k)
+                    for (int k = 0; k < PAGES; ++k)
 #pragma unroll
-                for (int w = 0; w < 2; ++w)
+                        for (int w = 0; w < 2; ++w)
+#pragma unroll
+                            for (int c = 0; c < CHUNKS; ++c) {
+                                const int d = (c0 + c) * 64 + part * 8;
+                                const T* row = static_cast<const T*>(p.bounds) + ((static_cast<int64_t>(page[k]) * 2 + w) * G + g) * D;
+                                x[k][w][c].load(row, d, page[k] >= 0 && d < D, D, 0, 0);
+                            }
 #pragma unroll
                     for (int c = 0; c < CHUNKS; ++c) {
-                        const int d = (c0 + c) * 64 + part * 8;
-                        const T* row = static_cast<const T*>(p.bounds) + ((static_cast<int64_t>(page[k]) * 2 + w) * G + g) * D;
-                        x[k][w][c].load(row, d, page[k] >= 0 && d < D, D, 0, 0);
+                        if ((c0 + c) * 64 >= D) break;
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            float a[PAGES][8];
+#pragma unroll
+                            for (int k = 0; k < PAGES; ++k) x[k][w][c].values(a[k]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                double v[PAGES][2];
+#pragma unroll
+                                for (int k = 0; k < PAGES; ++k) {
+                                    v[k][0] = a[k][2 * e];
+                                    v[k][1] = a[k][2 * e + 1];
+                                }
+#pragma unroll
+                                for (int t = 0; t < TOKENS; ++t) {
+                                    if (TOKENS > 1 && t >= n) break;
+                                    const double2 q = s_q[t][w][((c0 + c) * 4 + e) * 8 + part];
+#pragma unroll
+                                    for (int k = 0; k < PAGES; ++k) acc[t][k] = fma(q.y, v[k][1], fma(q.x, v[k][0], acc[t][k]));
+                                }
+                            }
+                        }
                     }
+                }
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) {
-                if ((c0 + c) * 64 >= D) break;
+                for (int t = 0; t < TOKENS; ++t) {
+                    if (TOKENS > 1 && t >= n) break;
+                    const int pages = pages_of(t);
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    float a[PAGES][8];
+                    for (int k = 0; k < PAGES; ++k) {
+                        double x = acc[t][k];
 #pragma unroll
-                    for (int k = 0; k < PAGES; ++k) x[k][w][c].values(a[k]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        double v[PAGES][2];
-#pragma unroll
-                        for (int k = 0; k < PAGES; ++k) {
-                            v[k][0] = a[k][2 * e];
-                            v[k][1] = a[k][2 * e + 1];
-                        }
-#pragma unroll
-                        for (int t = 0; t < TOKENS; ++t) {
-                            if (TOKENS > 1 && t >= n) break;
-                            const double2 q = s_q[t][w][((c0 + c) * 4 + e) * 8 + part];
-#pragma unroll
-                            for (int k = 0; k < PAGES; ++k) acc[t][k] = fma(q.y, v[k][1], fma(q.x, v[k][0], acc[t][k]));
-                        }
+                        for (int o = 1; o < 8; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+                        const int j = j0 + k * GROUPS;
+                        if (part == 0 && j < pages) keys[t * G * p.width + j] = page[k] < 0 ? 0ull : select_key(x);
                     }
                 }
             }
         }
-#pragma unroll
-        for (int t = 0; t < TOKENS; ++t) {
-            if (TOKENS > 1 && t >= n) break;
-            const int pages = TOKENS == 1 ? most : (max(len - (n - 1 - t), 0) + p.c.page_size - 1) / p.c.page_size;
-#pragma unroll
-            for (int k = 0; k < PAGES; ++k) {
-                double x = acc[t][k];
-#pragma unroll
-                for (int o = 1; o < 8; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-                const int j = base + k * GROUPS + group;
-                if (part == 0 && j < stop && j < pages) keys[t * G * p.width + j] = page[k] < 0 ? 0ull : select_key(x);
-            }
-        }
     }
-}
-
-// ---------------------------------------------------------------------------
-// selection
-// ---------------------------------------------------------------------------
-constexpr int kSelectThreads = 512;
-constexpr int kSelectWarps = kSelectThreads / 32;
-constexpr int kSelectBits = 11, kSelectBins = 1 << kSelectBits;
-constexpr int kSelectKeys = 6144;   // keys that shared memory holds (48 KB of them)
-
-// Inclusive sum over the block's threads of their counts (x: kSelectWarps ints of shared
-// memory, free before and after); total: of all.
-__device__ __forceinline__ int select_scan(int mine, int* x, int warp, int lane, int& total) {
-    int inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-    }
-    __syncthreads();
-    if (lane == 31) x[warp] = inc;
-    __syncthreads();
-    int before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kSelectWarps; ++w) {
-        before += w < warp ? x[w] : 0;
-        total += x[w];
-    }
-    return before + inc;
-}
-
-// A block per (token, kv head).  Of the pages that are not always in, the `want`-th largest key
-// by radix selection, 11 bits at a time of what the keys are above the smallest one (scores lie
-// in a few binades: their upper bits alone would tell nothing), then the pages above it and the
-// first of those equal to it, in their order.
-__global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __grid_constant__ PagedSelectParams p) {
-    extern __shared__ unsigned long long s_keys[];   // [kSelectKeys]
-    __shared__ __align__(16) int s_hist[kSelectBins];
-    __shared__ int s_x[kSelectWarps];
-    __shared__ unsigned long long s_y[2][kSelectWarps];
-    __shared__ int s_digit, s_above, s_same;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int G = p.c.kv_heads;
-    const int64_t t = blockIdx.x / G;   // of this launch
-    const int g = blockIdx.x % G;
-    const SelectToken tok = select_token(p, p.token0 + t, lane);
-    for (int i = threadIdx.x; i < kSelectBins; i += kSelectThreads) s_hist[i] = 0;
-    pdl_wait();
-    if (tok.seq < 0) return;
-    int32_t* out = p.pages + ((p.token0 + t) * G + g) * p.topk;
-    const int n = tok.pages;
-    if (g == 0 && threadIdx.x == 0 && (p.c.lens[tok.seq] < 0 || p.c.lens[tok.seq] > p.max_slots))
-        report_status(p.status, CHRONOS_ERR_INVALID_ARG);
-    if (n <= p.topk) {
-        for (int i = threadIdx.x; i < p.topk; i += kSelectThreads) out[i] = i < n ? i : -1;
-        return;
-    }
-    // pages [lo, hi) compete for `want` places (first + last <= topk < n: there are some)
-    const int lo = p.first, hi = n - p.last;
-    int want = p.topk - p.first - p.last;
-    const unsigned long long* mine = p.keys + (t * G + g) * p.width;
-    const bool held = n <= kSelectKeys;
-    unsigned long long low = ~0ull, high = 0ull;
-    for (int j = lo + threadIdx.x; j < hi; j += kSelectThreads) {
-        const unsigned long long k = mine[j];
-        if (held) s_keys[j] = k;
-        low = min(low, k);
-        high = max(high, k);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
-        high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
-    }
-    if (lane == 0) {
-        s_y[0][warp] = low;
-        s_y[1][warp] = high;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kSelectWarps; ++w) {
-        low = min(low, s_y[0][w]);
-        high = max(high, s_y[1][w]);
-    }
-    auto key = [&](int j) { return (held ? s_keys[j] : mine[j]) - low; };
-    // what the keys are above the smallest has `top` bits
-    int top = 64 - __clzll(static_cast<long long>(high - low));
-    unsigned long long known = top == 64 ? 0ull : ~0ull << top, prefix = 0ull;
-    if (want == 0) prefix = known = ~0ull, top = 0;   // none of them: no key is above or equal (they are below 2^64 - 1)
-    for (bool fresh = true; top > 0; fresh = false) {
-        const int shift = max(0, top - kSelectBits), bits = top - shift;
-        const unsigned long long mask = (1ull << bits) - 1;
-        if (!fresh) {
-            for (int i = threadIdx.x; i < kSelectBins; i += kSelectThreads) s_hist[i] = 0;
-            __syncthreads();
-        }
-        for (int j = lo + threadIdx.x; j < hi; j += kSelectThreads) {
-            const unsigned long long k = key(j);
-            if ((k & known) == prefix) atomicAdd(&s_hist[(k >> shift) & mask], 1);
-        }
-        __syncthreads();
-        // thread i holds the digits from kSelectBins - 1 - 4 i down
-        int h[4], sum = 0, total;
-        const int4 four = *reinterpret_cast<const int4*>(&s_hist[kSelectBins - 4 - 4 * threadIdx.x]);
-        h[0] = four.w; h[1] = four.z; h[2] = four.y; h[3] = four.x;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum += h[i];
-        int above = select_scan(sum, s_x, warp, lane, total) - sum;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (above < want && above + h[i] >= want) {
-                s_digit = kSelectBins - 1 - 4 * threadIdx.x - i;
-                s_above = above;
-                s_same = h[i];
-            }
-            above += h[i];
-        }
-        __syncthreads();
-        prefix |= static_cast<unsigned long long>(s_digit) << shift;
-        known |= mask << shift;
-        want -= s_above;
-        top = shift;
-        if (s_same == want) break;   // all of them: the bits below do not matter
-    }
-    // pages in order: always in, above the threshold, or one of the first `want` equal to it
-    int more = 0, same = 0;   // pages before this round's: taken whatever comes, equal to the threshold
-    for (int j0 = 0; j0 < n; j0 += kSelectThreads) {
-        const int j = j0 + threadIdx.x;
-        const bool always = j < n && (j < lo || j >= hi);
-        const unsigned long long k = j >= lo && j < hi ? key(j) & known : 0ull;
-        const bool eq = j >= lo && j < hi && k == prefix, gt = always || (j >= lo && j < hi && k > prefix);
-        int total;
-        const int at = select_scan((gt ? 1 << 16 : 0) | (eq ? 1 : 0), s_x, warp, lane, total);
-        const int rank = same + (at & 0xffff);   // among the equal ones, from 1 on
-        if (gt || (eq && rank <= want)) out[more + (at >> 16) + min(rank, want) - 1] = j;
-        more += total >> 16;
-        same += total & 0xffff;
+    // every block's keys are written (they are read from global memory, by blocks of this cluster only)
+    if (C > 1) cooperative_groups::this_cluster().sync();
+    else __syncthreads();
+    for (int t = rank; t < n; t += C) {
+        select_row(p, s_sel, s_keys, keys + t * G * p.width, p.pages + ((t0 + t) * G + g) * p.topk, pages_of(t));
+        __syncthreads();   // the next one writes where this one reads
     }
 }
 
