@@ -240,8 +240,10 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) =
     // rows of one kind, RPW at a time: this warp's begin at `sub + slice * RPW` and lie `step` units apart
     const int uk = (G + RPW - 1) / RPW, uq = (p.heads + RPW - 1) / RPW, step = p.slices * RPW;
     const int row0 = slice * RPW + sub;
+    // V's begin half the warps further: where a token's rows of a kind are fewer than its warps, others take them
+    const int slice_v = slice + p.slices / 2 - (slice >= p.slices - p.slices / 2 ? p.slices : 0), row0_v = slice_v * RPW + sub;
     const T* src_k = static_cast<const T*>(p.k) + t * p.k_row + row0 * p.k_head + (VEC ? col : 0);
-    const T* src_v = static_cast<const T*>(p.v) + t * p.v_row + row0 * p.v_head + (VEC ? col : 0);
+    const T* src_v = static_cast<const T*>(p.v) + t * p.v_row + row0_v * p.v_head + (VEC ? col : 0);
     const T* src_q = static_cast<const T*>(p.q) + t * p.q_row + row0 * p.q_head + (VEC ? col : 0);
     const int at_col = VEC ? 0 : col;
     // the first rows of every kind are on their way while the token's place is looked up
@@ -252,7 +254,7 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) =
             x[n].load(src + n * step * head, at_col, on && row + n * step < rows && t < p.tokens, D, p.start, p.dim);
     };
     fetch(xk, src_k, p.k_head, row0, G);
-    fetch(xv, src_v, p.v_head, row0, G);
+    fetch(xv, src_v, p.v_head, row0_v, G);
     fetch(xq, src_q, p.q_head, row0, p.heads);
 
     int b = -1, page = -1, in_page = 0;
@@ -351,12 +353,12 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) =
     if constexpr (PACKED) {
         const int64_t in = static_cast<int64_t>(in_page >> 4) * fp4_record(p.columns) + line * (p.columns / 2) + col / 2;
         kp = static_cast<uint8_t*>(p.c.k_pages) + page * p.c.k_page_stride + in + row0 * kh;
-        vp = static_cast<uint8_t*>(p.c.v_pages) + page * p.c.v_page_stride + in + row0 * vh;
+        vp = static_cast<uint8_t*>(p.c.v_pages) + page * p.c.v_page_stride + in + row0_v * vh;
     } else {
         kh *= sizeof(T);
         vh *= sizeof(T);
         kp = reinterpret_cast<uint8_t*>(static_cast<T*>(p.c.k_pages) + page * p.c.k_page_stride + in_page * p.c.k_slot_stride) + row0 * kh;
-        vp = reinterpret_cast<uint8_t*>(static_cast<T*>(p.c.v_pages) + page * p.c.v_page_stride + in_page * p.c.v_slot_stride) + row0 * vh;
+        vp = reinterpret_cast<uint8_t*>(static_cast<T*>(p.c.v_pages) + page * p.c.v_page_stride + in_page * p.c.v_slot_stride) + row0_v * vh;
     }
     auto put4 = [&](uint32_t codes, uint32_t scale, uint8_t* to, bool has) {
         if (has && col < p.columns) {
@@ -440,8 +442,8 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) =
         kp += step * UK * kh;
         k_out += step * UK * p.ko_head;
     }
-    for (int u = slice, row = row0; page >= 0 && u < uk; u += p.slices * UK, row += step * UK) {
-        if (u != slice) fetch(xv, src_v, p.v_head, row, G);
+    for (int u = slice_v, row = row0_v; page >= 0 && u < uk; u += p.slices * UK, row += step * UK) {
+        if (u != slice_v) fetch(xv, src_v, p.v_head, row, G);
         uint32_t again = 0;
 #pragma unroll
         for (int n = 0; n < UK; ++n) {
