@@ -20,6 +20,8 @@
 
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "chronos_paged.h"
 #include "common.cuh"
 
@@ -494,6 +496,10 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<T, DP>::kBlocksPerSm) pag
     constexpr int RB = S::kRowBytes;
     constexpr int RPI = 32 / CPR;          // rows a warp copies per instruction
     constexpr float kGrow = 8.0f, kLift = WeightLift<T>::value;
+    // bf16 weights of selected pages go through the product with what their rounding leaves: a few
+    // hundred slots do not average 2^-9 each away (8 heads of 2048 slots: 0.0032 off, 0.0016 so, the
+    // result's own rounding), and the copies bound these calls.
+    constexpr bool TWO = SEL && std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ __align__(128) uint8_t smem[];
     float* s_o = reinterpret_cast<float*>(smem + NS * S::kStageBytes);         // [warp][8 heads][kOStride]
     float* s_ml = s_o + S::kMergeBytes / 4;                                    // [warp][8][2]
@@ -738,7 +744,7 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<T, DP>::kBlocksPerSm) pag
                         }
                     }
             }
-            uint32_t pb[NT][2];
+            uint32_t pb[NT][2], rest[TWO ? NT : 1][2];
             Tf32Pair pf[F32 ? 4 : 1];   // [8 slots][2 rows of 4]
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -760,8 +766,13 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<T, DP>::kBlocksPerSm) pag
                     continue;
                 }
                 // weights in T for the second product; the sum keeps fp32
-                pb[t][0] = transpose8x8(pack2<T>(a, b));
-                pb[t][1] = transpose8x8(pack2<T>(c, d));
+                const uint32_t ab = pack2<T>(a, b), cd = pack2<T>(c, d);
+                pb[t][0] = transpose8x8(ab);
+                pb[t][1] = transpose8x8(cd);
+                if constexpr (TWO) {
+                    rest[t][0] = transpose8x8(pack2<T>(a - __uint_as_float(ab << 16), b - __uint_as_float(ab & 0xffff0000u)));
+                    rest[t][1] = transpose8x8(pack2<T>(c - __uint_as_float(cd << 16), d - __uint_as_float(cd & 0xffff0000u)));
+                }
             }
 #pragma unroll
             for (int dd = 0; dd < DP / 16; ++dd) {
@@ -781,7 +792,10 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<T, DP>::kBlocksPerSm) pag
                     uint32_t va[4];
                     ldmatrix_x4<true>(va, st + voff[dd & 3] + (dd >> 2) * 128);
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) mma_16816<T>(o[t][dd], va, pb[t][0], pb[t][1]);
+                    for (int t = 0; t < NT; ++t) {
+                        if constexpr (TWO) mma_16816<T>(o[t][dd], va, rest[t][0], rest[t][1]);
+                        mma_16816<T>(o[t][dd], va, pb[t][0], pb[t][1]);
+                    }
                 }
             }
         }
