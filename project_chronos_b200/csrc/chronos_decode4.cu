@@ -11,8 +11,14 @@
 namespace chronos {
 namespace {
 
-// Blocks of 64 slots that a block of a cluster takes at most (see chronos_paged_decode).
-constexpr int kP4ClusterBlocks = 6, kP4ClusterBlocksFull = 8;
+// Blocks of 64 slots that a block of a cluster takes at most: where the clusters leave half of the
+// grid idle / do not / where the rows alone fill it (clusters of one, also more of them than run at
+// once).  Beyond that the work list, which cuts all rows evenly but costs a second kernel and joins.
+// Heads of 128, list against cluster: 1 row of 4096 slots, 2 kv heads (8 blocks each) 11.8 and 14.4 us;
+// 16 rows up to 1500 slots, 8 kv heads (12 each) 19.1 and 15.9 us, 20 rows up to 4000 (32 each) 29.0 and
+// 35.6 us; 48 rows up to 1500 (24 each) 37.9 and 28.9 us, 128 rows up to 500 57 and 34 us, 100 rows up to
+// 4000 (63 each) 115 and 124 us.
+constexpr int kP4ClusterBlocks = 6, kP4ClusterBlocksFull = 16, kP4RowBlocks = 24;
 // Tiles of 16 slots that a warp takes of a unit of the work list.
 constexpr int kP4ListTiles = 4;
 
@@ -58,8 +64,8 @@ Decode4Plan decode4_plan(const ChronosPagedDecode4Args* a) {
     int size = 1;
     while (size < 8 && size < blocks) size *= 2;
     while (size > 1 && rows * size > room) size /= 2;
-    const int64_t most = 2 * rows * size > room ? kP4ClusterBlocksFull : kP4ClusterBlocks;
-    d.cluster = rows * size <= room && blocks <= most * size ? size : 0;
+    const int64_t most = size == 1 && 2 * rows > room ? kP4RowBlocks : 2 * rows * size > room ? kP4ClusterBlocksFull : kP4ClusterBlocks;
+    d.cluster = blocks <= most * size ? size : 0;
     const size_t slots = d.cluster > 0 ? 0 : 2 * static_cast<size_t>(d.grid) * 16;
     d.o_part_ml = round_up(slots * d.dp * 4, 256);
     d.total = d.cluster > 0 ? 0 : d.o_part_ml + round_up(slots * 8, 256);
@@ -112,7 +118,7 @@ extern "C" int chronos_paged_decode4(const ChronosPagedDecode4Args* a, void* str
     if (a->q == nullptr || a->out == nullptr) return fail(CHRONOS_ERR_INVALID_ARG, "%s: q and out are required", what);
     const Decode4Plan d = decode4_plan(a);
     const int64_t units = (static_cast<int64_t>(d.max_vis) / kPdBlock + 1) * a->cache.batch * a->cache.kv_heads * d.parts;
-    if (units >= (1 << 30) || static_cast<int64_t>(a->cache.batch) * a->heads >= INT32_MAX)
+    if (units >= (1 << 30) || static_cast<int64_t>(a->cache.batch) * a->heads >= INT32_MAX / 8)
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: batch %d * heads * slots %d too large", what, a->cache.batch, d.max_vis);
     if (d.total > 0 && (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < d.total))
         return fail(CHRONOS_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes, %zu (256-byte aligned) needed", what,
