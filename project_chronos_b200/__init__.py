@@ -16,7 +16,10 @@ Public API (mirrors chronos/model/moe_chronos.py of FonaTech/Project_Chronos):
 * ``PagedCache`` (``paged``) and ``ops.paged_append`` / ``paged_attn_decode`` /
   ``paged_evict`` / ``window_attention`` — a paged key-value cache for rows of
   different lengths and the attention that serves prompts and single tokens
-  from it (include/chronos_paged.h);
+  from it (include/chronos_paged.h); with ``ops.paged_append_rope`` /
+  ``paged_attn_decode4`` / ``paged_gather`` / ``paged_bounds`` / ``paged_select`` /
+  ``paged_attn_sparse`` rotation on the way into the pages, pages of 4-bit
+  values and attention over selected pages (include/chronos_paged4.h);
 * ``synthetic`` — seeded workloads of the benchmark configurations.
 
 Importing the package does not load the CUDA library; the first layer call

@@ -29,6 +29,7 @@ struct Paged4 {
     static constexpr int kMergeBytes = kPdWarps * 8 * kOStride * 4;
     static constexpr int kSmem = kStages * kStageBytes + kMergeBytes + kPdWarps * 16 * 4;
     static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;      // halves that a query or weight is split into
+    // four blocks of 128 registers measured 2 to 7 % slower than three for heads of 128
     static constexpr int kBlocksPerSm = DP == 256 || (DP == 128 && NT * kTerms > 2) ? 2 : DP == 128 ? 3 : 4;
     static constexpr int kPartBytes = (16 * DP + 32) * 4;      // what a cluster's block leaves for the join
     static_assert(kPartBytes <= kStages * kStageBytes, "the part takes the copies' place");
@@ -77,7 +78,7 @@ __device__ __forceinline__ uint32_t kept(uint32_t x) {
 // halves, times the scales of their blocks (code * scale has 6 bits: exact), and go through
 // the products of paged.cuh, S^T = K Q^T and O^T = V^T P^T, in fp16 whatever the layer:
 // queries in units of a power of two of their head (all their bits but of columns below
-// 2^-14 of the largest), weights of up to 2^15.  fp32 layers split queries and weights
+// 2^-22 of the largest), weights of up to 2^15.  fp32 layers split queries and weights
 // into two halves each (22 bits).  The order of the columns inside a product is free: a
 // lane takes a contiguous quarter of a K slot and a contiguous eighth of a V slot, so a
 // tile's codes are read by one wide load per slot.  V's halves come in pairs of columns; the
@@ -85,6 +86,12 @@ __device__ __forceinline__ uint32_t kept(uint32_t x) {
 //
 // A warp takes TILES tiles of 16 slots of a unit (4 * TILES tiles), one after the other; its lanes
 // look up the pages of a unit's tiles at once, a unit ahead.
+//
+// Measured, 32 / 8 heads of 128: 4 rows of 100003 to 131072 slots in fp16 138 us, 4.1 TB/s of 4-bit
+// records (the 16-bit cache: 291 to 310 us); 32 ragged rows up to 8192 slots 57 us.  Bound by
+// instructions: 348 per tile, of which 64 conversions, 96 scale products and 16 tensor products are
+// the format's; the heavy FMA pipe and the ALU take two cycles each for theirs, 60 % of issue slots
+// are used.  16 slots per look-up and unit: 206 us.
 template <typename T, int DP, int NT, int TILES, bool CL, bool SEL>
 __global__ void __launch_bounds__(kPdThreads, Paged4<T, DP, NT>::kBlocksPerSm) paged_decode4_kernel(
     const __grid_constant__ PagedDecodeParams p) {

@@ -42,7 +42,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // A block per (sequence, kv head) and page in turn: LPR lanes hold a slot's columns, 8 each,
-// the block's other groups take the next slots; the groups meet in shared memory.
+// the block's other groups take the next slots; the groups meet in shared memory.  One new token
+// per sequence is bound by latency (32 rows of 8 heads 3 us), since older slots are not read again.
 template <typename T, int LPR, bool VEC, bool PACKED>
 __global__ void __launch_bounds__(kBoundThreads) paged_bounds_kernel(const __grid_constant__ PagedBoundsParams p) {
     constexpr int GROUPS = kBoundThreads / LPR;
@@ -290,7 +291,8 @@ __device__ __forceinline__ void select_row(const PagedSelectParams& p, SelectSha
 // shuffles.  The queries' sums lie in shared memory so that the 8 lanes' parts are side by side,
 // the pages' numbers beside them: both are fetched at once.  Then the blocks share the tokens'
 // selections.  32 rows of 256 to 512 pages, 8 heads of 128: 52 us with a look-up before every
-// page; scores and selection in one kernel save the start of another and its reading.
+// page (20 us without, the selection included 21: 67 MB of bounds, 10 us at HBM's rate; the conversions
+// to 64 bits and the selection's rounds of counting are the rest).
 template <typename T, bool VEC, int TOKENS>
 __global__ void __launch_bounds__(kSelectThreads, TOKENS == 1 ? 3 : 2) paged_select_kernel(const __grid_constant__ PagedSelectParams p) {
     constexpr int MAXD = CHRONOS_PAGED_MAX_HEAD_DIM, GROUPS = kSelectThreads / 8;
