@@ -1216,3 +1216,170 @@ def test_calls_follow_the_current_stream():
     for a, b in zip(*res):
         assert torch.equal(a, b)
     ops.check_status(q.device)
+
+
+# ---------------------------------------------------------------------------------------
+# many rows, views, streams, other parts of the cache
+# ---------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("four", [False, True])
+def test_very_many_rows(dt, four):
+    """More rows than a grid's second dimension takes, and than run at once."""
+    from project_chronos_b200 import ops
+    b, h, g, d, size = 70000, 2, 1, 16, 16
+    k, v = _rnd(1, b, g, d, dt=dt), _rnd(2, b, g, d, dt=dt)
+    q = _rnd(3, b, h, d, dt=dt)
+    if four:
+        kp, vp = (torch.zeros(2 * b, g, ops.packed_page_bytes(size, d), dtype=torch.uint8, device="cuda") for _ in range(2))
+    else:
+        kp, vp = (torch.zeros(2 * b, size, g, d, dtype=dt, device="cuda") for _ in range(2))
+    table = torch.randperm(2 * b, generator=_gen(4), device="cuda").to(torch.int32).view(b, 2)
+    ln = torch.full((b,), 15, dtype=torch.int32, device="cuda")
+    ln[1::2] = 16                                          # the second page's first slot
+    ops.paged_append_rope(k, v, kp, vp, table, ln, lens_out=ln)
+    bounds = torch.zeros(2 * b, 2, g, d, dtype=dt, device="cuda")
+    ops.paged_bounds(kp, bounds, table, ln, full=True)
+    pages = ops.paged_select(q, bounds, table, ln, size, 1)
+    want = torch.zeros(b, 1, 1, dtype=torch.int32, device="cuda")
+    want[1::2] = 1                                         # a token's own page
+    assert torch.equal(pages, want)
+    out = ops.paged_attn_sparse(q, kp, vp, table, ln, pages)
+    ops.check_status(out.device)
+    values = _quantise(v.double())[2].to(dt) if four else v
+    # odd rows see their one slot; even ones 15 slots of zeros besides
+    assert torch.allclose(out[1::2].float(), values[1::2].expand(-1, h, -1).float(), rtol=2.0 ** -7, atol=2.0 ** -20)
+    for i in (0, 35000, b - 2):
+        keys = torch.zeros(16, g, d, dtype=torch.float64, device="cuda")
+        vals = keys.clone()
+        keys[15], vals[15] = (_quantise(k[i].double())[2] if four else k[i].double()), values[i].double()
+        _check_attention(out[i], None, q[i], keys, vals, d ** -0.5, dt, four)
+    if four:
+        all_ = ops.paged_attn_decode4(q, kp, vp, table, ln)
+        assert torch.equal(all_[0::2], out[0::2])
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("h, g, b, n", [(4, 2, 300, 700), (8, 1, 150, 1400), (16, 16, 30, 2500), (2, 2, 400, 90)])
+def test_decode4_where_rows_fill_the_grid(dt, h, g, b, n):
+    """A block or a small cluster per row, more rows than run at once."""
+    from project_chronos_b200 import ops
+    d = 64
+    lens = [max(0, n - 7 * i) for i in range(b)]
+    kp, vp, table, ln, rows = _cache4(lens, g, d, 16, 11)
+    q = _rnd(12, b, h, d, dt=dt, scale=2.0)
+    lse = torch.empty(b, h, device="cuda")
+    out = ops.paged_attn_decode4(q, kp, vp, table, ln, lse=lse)
+    ops.check_status(out.device)
+    for i in sorted({0, 1, b // 2, b - 1}):
+        _check_attention(out[i], lse[i], q[i], *rows[i], d ** -0.5, dt, True)
+
+
+@gpu
+@pytest.mark.parametrize("four", [False, True])
+def test_calls_take_views(four):
+    """A part of a wider page table, expanded queries, keys of one head read as several."""
+    from project_chronos_b200 import ops
+    h, g, d, size, dt = 8, 2, 64, 16, BF
+    kp, vp, table, ln, rows = _cache4([100, 50], g, d, size, 3) if four else _cache16([100, 50], g, d, size, dt, 3)
+    wide = torch.full((2, 3 * table.shape[1]), -1, dtype=torch.int32, device="cuda")
+    part = wide[:, 2: 2 + table.shape[1]]
+    part.copy_(table)
+    q = _rnd(1, 1, 1, d, dt=dt).expand(2, h, d)
+    pages = torch.arange(4, dtype=torch.int32, device="cuda").expand(2, g, 4).contiguous()
+    got = ops.paged_attn_sparse(q, kp, vp, part, ln, pages)
+    assert torch.equal(got, ops.paged_attn_sparse(q.contiguous(), kp, vp, table, ln, pages))
+    bounds = torch.zeros(kp.shape[0], 2, g, d, dtype=dt, device="cuda")
+    ops.paged_bounds(kp, bounds, part, ln, full=True)
+    assert torch.equal(ops.paged_select(q, bounds, part, ln, size, 3), ops.paged_select(q.contiguous(), bounds, table, ln, size, 3))
+    if four:
+        assert torch.equal(ops.paged_attn_decode4(q, kp, vp, part, ln), ops.paged_attn_decode4(q.contiguous(), kp, vp, table, ln))
+    cos, sin = _tables(200, d)
+    one = _rnd(2, 2, 1, d, dt=dt)
+    res = []
+    for k, tab in ((one.expand(2, g, d), part), (one.expand(2, g, d).contiguous(), table)):
+        a, b = kp.clone(), vp.clone()
+        qq = ops.paged_append_rope(k, k, a, b, tab, ln, ln, cos[:1].expand(200, d), sin, q=q)
+        res.append((a, b, qq))
+    for x, y in zip(*res):
+        assert torch.equal(x.nan_to_num(9.0) if x.is_floating_point() else x, y.nan_to_num(9.0) if y.is_floating_point() else y)
+    ops.check_status(got.device)
+
+
+@gpu
+def test_two_streams_at_once():
+    """Calls on two streams, each with its own workspace, keep out of each other's way."""
+    from project_chronos_b200 import ops
+    h, g, d, dt = 8, 2, 128, BF
+    caches = [_cache4([9000 + 500 * i, 300], g, d, 16, 5 + i) for i in range(2)]
+    qs = [_rnd(6 + i, 2, h, d, dt=dt, scale=2.0) for i in range(2)]
+    bounds = [torch.zeros(c[0].shape[0], 2, g, d, dtype=dt, device="cuda") for c in caches]
+    for c, b in zip(caches, bounds):
+        ops.paged_bounds(c[0], b, c[2], c[3], full=True)
+    def call(i):
+        kp, vp, table, ln, _ = caches[i]
+        pages = ops.paged_select(qs[i], bounds[i], table, ln, 16, 40, first=1, last=2)
+        return ops.paged_attn_decode4(qs[i], kp, vp, table, ln), pages, ops.paged_attn_sparse(qs[i], kp, vp, table, ln, pages)
+    want = [call(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(x, y) for x, y in zip(r, want[i]))
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_append_rope_in_a_cache_that_evicts(dt):
+    """Rotation on the way into a cache with running sums: positions go on counting tokens after an eviction."""
+    from project_chronos_b200 import PagedCache, ops
+    h, g, d, size = 4, 2, 64, 16
+    c = PagedCache(2, 20, g, d, 10, "cuda", dt, page_size=size, track_weights=True)
+    cos, sin = _tables(400, d)
+    for b in range(2):
+        c.reserve(b, 160)
+    q, k, v = (_rnd(i, 200, x, d, dt=dt) for i, x in ((1, h), (2, g), (3, g)))
+    c.append_rope(q[:180], k[:180], v[:180], cos, sin, cu_seqlens=_i32(0, 120, 180))
+    c.attend(q[:2])
+    c.evict(50, sinks=2, recent=8)
+    assert c.lens.tolist() == [50, 50] and c.seen.tolist() == [120, 60]
+    got = c.append_rope(q[180:182], k[180:182], v[180:182], cos, sin)
+    ops.check_status(got.device)
+    assert c.lens.tolist() == [51, 51] and c.seen.tolist() == [121, 61]
+    for b, at in ((0, 120), (1, 60)):
+        y, m = _rotate(q[180 + b: 181 + b].double(), cos[at: at + 1], sin[at: at + 1], 0)
+        _near(got[b: b + 1], y, m, dt)
+        y, m = _rotate(k[180 + b: 181 + b].double(), cos[at: at + 1], sin[at: at + 1], 0)
+        _near(c.k_pages[c.page_table[b, 3].long(), 2][None], y, m, dt)
+        assert bool((c.positions[b, :, 50] == at).all()) and bool((c.weights[b, :, 50] == 0).all())
+    with pytest.raises(RuntimeError, match="page_bounds"):
+        c.attend_sparse(q[:2], 2)
+
+
+@gpu
+def test_bounds_after_slots_were_given_up():
+    """A draft is taken back: the bounds stay bounds, and are exact again from nothing."""
+    from project_chronos_b200 import PagedCache, ops
+    g, d, size, dt = 2, 64, 16, BF
+    c = PagedCache(1, 8, g, d, 8, "cuda", dt, page_size=size, page_bounds=True)
+    c.reserve(0, 100)
+    k = _rnd(1, 60, g, d, dt=dt)
+    c.append(k[:40], k[:40], _i32(0, 40))
+    c.append(10 * k[40:44], k[40:44], _i32(0, 4))
+    c.lens -= 3
+    c.seen -= 3
+    c.append(k[44:60], k[44:60], _i32(0, 16))
+    rows = torch.cat([k[:40], 10 * k[40:41], k[44:60]])
+    want = _bounds_of(rows, size)
+    got = c.bounds[c.page_table[0, :4].long()]
+    assert torch.equal(got[[0, 1, 3]], want[[0, 1, 3]]) and bool((got[2, 0] <= want[2, 0]).all()) and bool((got[2, 1] >= want[2, 1]).all())
+    ops.paged_bounds(c.k_pages, c.bounds, c.page_table, c.lens, full=True)
+    assert torch.equal(c.bounds[c.page_table[0, :4].long()], want)
