@@ -1383,3 +1383,67 @@ def test_bounds_after_slots_were_given_up():
     assert torch.equal(got[[0, 1, 3]], want[[0, 1, 3]]) and bool((got[2, 0] <= want[2, 0]).all()) and bool((got[2, 1] >= want[2, 1]).all())
     ops.paged_bounds(c.k_pages, c.bounds, c.page_table, c.lens, full=True)
     assert torch.equal(c.bounds[c.page_table[0, :4].long()], want)
+
+
+@gpu
+@pytest.mark.parametrize("four", [False, True])
+def test_offsets_pass_32_bits(four):
+    """Pages, rows and bounds that lie further apart than 32 bits count."""
+    from project_chronos_b200 import ops
+    h, g, d, size, dt = 8, 2, 128, 16, BF
+    far = (1 << 31) + 64
+    def rows(n, *heads):                                   # [n, heads, d] side by side, rows `far` elements apart
+        store = torch.empty((n - 1) * far + sum(heads) * d, dtype=dt, device="cuda")
+        return [store[sum(heads[:i]) * d:].as_strided((n, m, d), (far, d, 1)) for i, m in enumerate(heads)]
+    if four:
+        nbytes, apart = ops.packed_page_bytes(size, d), (1 << 32) - 16
+        store = torch.empty(2 * apart + 2 * g * nbytes, dtype=torch.uint8, device="cuda")
+        kp, vp = (store[i * g * nbytes:].as_strided((3, g, nbytes), (apart, nbytes, 1)) for i in range(2))
+    else:
+        store = torch.empty(2 * far + 2 * size * g * d, dtype=dt, device="cuda")
+        kp, vp = (store[i * size * g * d:].as_strided((3, size, g, d), (far, g * d, d, 1)) for i in range(2))
+    q, k, v = rows(2, h, g, g)
+    for x, seed in ((q, 1), (k, 2), (v, 3)):
+        x.copy_(_rnd(seed, *x.shape, dt=dt))
+    table, ln = _i32(0, 1, 2, 0).view(2, 2), _i32(15, 15)
+    first = _rnd(4, 30, g, d, dt=dt)
+    ops.paged_append_rope(first, -first, kp, vp, table, _i32(0, 0), cu_seqlens=_i32(0, 15, 30))
+    q_out, k_out, v_out = rows(2, h, g, g)
+    ops.paged_append_rope(k, v, kp, vp, table, ln, q=q, q_out=q_out, lens_out=ln)
+    assert torch.equal(q_out, q)
+    ops.paged_gather(kp, vp, table, ln, _i32(0, 1, 2), k_out, v_out)
+    ops.check_status(ln.device)
+    def held(x):
+        return _quantise(x.double())[2] if four else x.double()
+    assert torch.equal(k_out.double(), held(k)) and torch.equal(v_out.double(), held(v))
+    pages = torch.zeros(2, g, 1, dtype=torch.int32, device="cuda")
+    out = rows(2, h)[0]
+    ops.paged_attn_sparse(q, kp, vp, table, ln, pages, out=out)
+    both = [out] + ([ops.paged_attn_decode4(q, kp, vp, table, ln)] if four else [])
+    for i in range(2):
+        keys, vals = (held(torch.cat([s * first[15 * i: 15 * i + 15], x[i: i + 1]])) for s, x in ((1, k), (-1, v)))
+        for o in both:
+            _check_attention(o[i], None, q[i], keys, vals, d ** -0.5, dt, four)
+    bounds = torch.zeros(3, 2, g, d, dtype=dt, device="cuda")
+    ops.paged_bounds(kp, bounds, table, ln, full=True)
+    for i in range(2):
+        keys = held(torch.cat([first[15 * i: 15 * i + 15], k[i: i + 1]])).to(dt)
+        assert torch.equal(bounds[2 * i], _bounds_of(keys, size)[0])
+    ops.check_status(ln.device)
+
+
+@gpu
+def test_select_among_bounds_that_pass_32_bits():
+    from project_chronos_b200 import ops
+    d, dt = 256, BF
+    n = (1 << 31) // (2 * d) + 100                         # pages of a slot each
+    kp = torch.zeros(n, 1, 1, d, dtype=dt, device="cuda")
+    bounds = torch.zeros(n, 2, 1, d, dtype=dt, device="cuda")
+    table, ln = _i32(n - 1, 5, n - 50, n - 2).view(1, 4), _i32(4)
+    k = _rnd(1, 4, 1, d, dt=dt)
+    kp[table[0].long(), 0] = k
+    ops.paged_bounds(kp, bounds, table, ln, full=True)
+    assert torch.equal(bounds[table[0].long()], torch.stack([k, k], 1))
+    q = k[2].expand(1, 1, d)
+    assert ops.paged_select(q, bounds, table, ln, 1, 2).view(-1).tolist() == [2, 3]
+    ops.check_status(ln.device)
