@@ -47,8 +47,10 @@ int launch_rope(PagedRopeParams p, bool packed, bool vec, cudaStream_t st) {
     while (p.slices < kRopeWarps && p.slices * (32 / lanes) < rows && p.tokens * p.slices < 16 * static_cast<int64_t>(sm_count())) p.slices *= 2;
     const int per = kRopeWarps / p.slices;
     auto kernel = packed ? rope_kernel<T, TT, true>(lanes, vec) : rope_kernel<T, TT, false>(lanes, vec);
-    if (p.tokens > 0)
-        CHRONOS_CUDA_CHECK(launch_kernel(kernel, dim3(static_cast<unsigned>((p.tokens + per - 1) / per)), dim3(kRopeThreads), 0, st, false, p));
+    const int smem = vec && sizeof(T) == 2 ? kRopeWarps * kRopeRing * 512 : 0;
+    if (p.tokens > 0) {
+        CHRONOS_CUDA_CHECK(launch_kernel(kernel, dim3(static_cast<unsigned>((p.tokens + per - 1) / per)), dim3(kRopeThreads), smem, st, false, p));
+    }
     if (p.cu != nullptr && (p.lens_out != nullptr || p.seen_out != nullptr))
         CHRONOS_CUDA_CHECK(launch_kernel(paged_rope_advance_kernel, dim3((p.c.batch + kRopeWarps - 1) / kRopeWarps), dim3(kRopeThreads), 0,
                                          st, p.tokens > 0, p));

@@ -5,12 +5,12 @@
 // Bound by HBM for prompts (every row read once, written once) and by latency for one
 // token per sequence.  A warp owns a token, or a slice of its rows where tokens are few:
 // the angles of its columns stay in registers for all heads, a lane holds 8 columns, so a
-// row of 128 takes half a warp.  8 prompts up to 8192 tokens, 32 / 8 heads of 128 in bf16: 162 us,
-// 6.0 TB/s read and written (partner columns by a second load, two rows in flight: 375 us); 32 rows of
-// one token 3.1 us.
+// row of 128 takes half a warp.  8 prompts up to 8192 tokens, 32 / 8 heads of 128 in bf16: 154 us,
+// 6.3 TB/s read and written (partner columns by a second load, two rows in flight: 375 us); 32 rows of
+// one token 3.0 us.
 //
-// 4-bit rows: bound by instructions (250 per 256 values; 8 prompts up to 4096 tokens, 16 / 8 heads of
-// 128 in fp16 85 us for 244 MB).  The code of a value and the scale of a block are decided as exact
+// 4-bit rows: bound by instructions (188 per 256 values of K, V and q; 8 prompts up to 4096 tokens, 16 / 8
+// heads of 128 in fp16 73 us for 244 MB).  The code of a value and the scale of a block are decided as exact
 // arithmetic decides: the fp32 value y is off by at most 2^-22 (|x c| + |x' s|), so a
 // code (scale) is taken where the values that much above and below it give the same
 // one, and computed in 64 bits where they do not (a warp in some thousand).  Values that
@@ -56,6 +56,7 @@ struct PagedRopeParams {
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeWarps = kRopeThreads / 32;
+constexpr int kRopeRing = 8;   // units of rows (512 bytes of 16-bit types) that a warp's ring holds
 
 // Column that column d turns with (d itself where it is not rotated).
 __device__ __forceinline__ int rope_partner(int d, int start, int dim) {
@@ -63,8 +64,8 @@ __device__ __forceinline__ int rope_partner(int d, int start, int dim) {
     return j < 0 || j >= dim ? d : j < dim / 2 ? d + dim / 2 : d - dim / 2;
 }
 
-// A lane's 8 columns of a row as they are loaded.  VEC: 16-byte words (the columns they turn
-// with come from the lane that has them); else numbers, with those columns beside them.
+// A lane's 8 columns of a row as they are loaded.  VEC: 16-byte words; else numbers, with the
+// columns they turn with beside them.
 template <typename T, bool VEC>
 struct RopeRow {
     uint4 w[sizeof(T) / 2];
@@ -78,7 +79,7 @@ struct RopeRow {
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(row + col)[i] = w[i];
     }
-    // Zeros for columns that do not turn.  Whole warps call it.
+    // Columns that lane `lane` has, zeros for those that do not turn.  Whole warps call it.
     __device__ __forceinline__ void partner(float (&x)[8], int lane, bool turns) const {
         RopeRow r;
         auto take = [&](uint32_t v) {
@@ -88,6 +89,11 @@ struct RopeRow {
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.w[i] = make_uint4(take(w[i].x), take(w[i].y), take(w[i].z), take(w[i].w));
         r.values(x);
+    }
+    __device__ __forceinline__ void read(uint32_t at) {   // from shared memory
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w) : "r"(at + i * 16));
     }
 };
 template <typename T>
@@ -112,10 +118,6 @@ struct RopeRow<T, false> {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (col + j < D) row[col + j] = from_f32<T>(x[j]);
-    }
-    __device__ __forceinline__ void partner(float (&v)[8], int, bool) const {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = with[j];
     }
 };
 template <typename T, bool VEC>
@@ -147,17 +149,18 @@ struct RopeSource {
             const double turned = static_cast<double>(to_f32<T>(row[w])) * to_f32<TT>(sin[d - start]);
             v = v * to_f32<TT>(cos[d - start]) + (w > d ? -turned : turned);
         }
-        return v / static_cast<double>(scale);
+        return scale == 1.0f ? v : v / static_cast<double>(scale);
     }
 };
-// Codes and scale in 64 bits.  Whole warps call it.  Not inlined: its registers stay out of
-// the common path.
+// Codes and scale in 64 bits.  Whole warps call it.
 template <typename T, typename TT>
-__device__ __noinline__ uint32_t fp4_block_exact(const RopeSource<T, TT> src, uint32_t* scale) {
-    double t = 0.0;
+__device__ __forceinline__ uint32_t fp4_block_exact(const RopeSource<T, TT>& src, uint32_t& scale) {
+    double x[8], t = 0.0;
     bool bad = false;
+#pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const double d = fabs(src.value(j));
+        x[j] = src.value(j);
+        const double d = fabs(x[j]);
         bad |= !(d < INFINITY);
         t = fmax(t, d);
     }
@@ -165,12 +168,13 @@ __device__ __noinline__ uint32_t fp4_block_exact(const RopeSource<T, TT> src, ui
     bad |= __shfl_xor_sync(0xffffffffu, bad ? 1 : 0, 1) != 0;
     const float t6 = static_cast<float>(t / 6.0);
     const uint32_t e = bad ? kFp8Nan : fp8_scales(t6, t6) & 0xffu;
-    *scale = e;
+    scale = e;
     if (bad || e == 0u) return 0u;
     const double z = fp8_value(e);
     uint32_t c = 0;
+#pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const double d = src.value(j), m = fabs(d);
+        const double d = x[j], m = fabs(d);
         const uint32_t level = (m > 0.25 * z) + (m >= 0.75 * z) + (m > 1.25 * z) + (m >= 1.75 * z) + (m > 2.5 * z) +
                                (m >= 3.5 * z) + (m > 5.0 * z);
         c |= (level | (signbit(d) ? 8u : 0u)) << (4 * j);
@@ -228,37 +232,140 @@ __device__ __forceinline__ uint32_t fp4_block(const float (&y)[8], float top, fl
     return codes;
 }
 
+// Where a slot's codes of the columns from `col` on lie in its record (the first of 16), and their scale.
+__device__ __forceinline__ int fp4_codes_at(int line, int col, int columns) { return line * (columns / 2) + col / 2; }
+__device__ __forceinline__ int fp4_scale_at(int line, int col, int columns) { return 8 * columns + line * (columns / 16) + col / 16; }
+
+// A token's place in the pages and its position.
+struct RopePlace {
+    int t, page, in_page;
+    int64_t at;
+    bool placed;
+};
+// What a warp's rows of 4 bits leave to the end: units (again: bits n % 32 of K's, of V's) with blocks that are
+// decided in 64 bits, and the rows of k_out, which may be k.  Not inlined: its registers stay out of the
+// common path.  Whole warps call it.
+template <typename T, typename TT, int LPR, bool VEC>
+__device__ __noinline__ void rope4_rest(const PagedRopeParams& p, const RopePlace w, int slice, int slice_v, uint32_t again_k, uint32_t again_v) {
+    constexpr int RPW = 32 / LPR;
+    const int lane = threadIdx.x & 31, sub = lane / LPR, col = lane % LPR * 8, G = p.c.kv_heads, D = p.c.head_dim;
+    const int uk = (G + RPW - 1) / RPW;
+    const bool turned = p.dim > 0 && w.placed;
+    const TT* cos = static_cast<const TT*>(p.cos) + w.at * p.cos_row;
+    const TT* sin = static_cast<const TT*>(p.sin) + w.at * p.sin_row;
+    for (int of_v = 0; of_v < 2; ++of_v) {
+        const uint32_t again = of_v ? again_v : again_k;
+        if (again == 0u) continue;
+        const T* src = of_v ? static_cast<const T*>(p.v) + w.t * p.v_row : static_cast<const T*>(p.k) + w.t * p.k_row;
+        uint8_t* to = (of_v ? static_cast<uint8_t*>(p.c.v_pages) + w.page * p.c.v_page_stride : static_cast<uint8_t*>(p.c.k_pages) + w.page * p.c.k_page_stride) +
+                      static_cast<int64_t>(w.in_page >> 4) * fp4_record(p.columns);
+        const int64_t from_head = of_v ? p.v_head : p.k_head, to_head = of_v ? p.c.v_head_stride : p.c.k_head_stride;
+        for (int u = of_v ? slice_v : slice, n = 0; u < uk; u += p.slices, ++n) {
+            if (((again >> (n & 31)) & 1u) == 0u) continue;
+            const int row = u * RPW + sub;
+            const RopeSource<T, TT> exact{row < G ? src + row * from_head : nullptr, turned && !of_v ? cos : nullptr, sin, col, D, p.start, p.dim,
+                                          of_v ? p.v_scale : p.k_scale};
+            uint32_t scale;
+            const uint32_t codes = fp4_block_exact<T, TT>(exact, scale);
+            if (row < G && col < p.columns) {
+                uint8_t* record = to + row * to_head;
+                *reinterpret_cast<uint32_t*>(record + fp4_codes_at(w.in_page & 15, col, p.columns)) = codes;
+                if ((col & 8) == 0) record[fp4_scale_at(w.in_page & 15, col, p.columns)] = static_cast<uint8_t>(scale);
+            }
+        }
+    }
+    if (p.k_out == nullptr) return;
+    __syncwarp();   // the rows are read
+    for (int u = slice; u < uk; u += p.slices) {
+        const int row = u * RPW + sub;
+        const bool has = row < G && col < D;
+        const T* k = static_cast<const T*>(p.k) + w.t * p.k_row + row * p.k_head;
+        T* out = static_cast<T*>(p.k_out) + w.t * p.ko_row + row * p.ko_head;
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            y[j] = 0.0f;
+            const int d = col + j;
+            if (!has || d >= D || !w.placed) continue;
+            y[j] = to_f32<T>(k[d]);
+            const int with = rope_partner(d, p.start, p.dim), r = d - p.start;
+            if (with != d) {
+                const float s = to_f32<TT>(sin[r]);
+                y[j] = fmaf(y[j], to_f32<TT>(cos[r]), to_f32<T>(k[with]) * (with > d ? -s : s));
+            }
+        }
+        __syncwarp();
+        if (has) rope_store<T, VEC>(out, y, col, D);
+    }
+}
+
 // LPR lanes hold a row (8 columns each).  VEC: rows, halves and tables can be read 8
-// columns at a time.
+// columns at a time.  Rows of 16-bit types then come through a ring in shared memory, so that all of a
+// token's are on their way at once (loads next to their uses left warps waiting for memory 43 % of the
+// time: 4-bit prompts and their rows back 112 us for 100); fp32 rows, twice the bytes per unit, come one unit ahead in registers
+// (24 chunks up to 257 tokens: 12.3 us for 14.2 through the ring).
 template <typename T, typename TT, int LPR, bool VEC, bool PACKED>
 __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) == 4 ? 2 : 3) paged_rope_kernel(const __grid_constant__ PagedRopeParams p) {
-    constexpr int RPW = 32 / LPR;                       // rows of a warp at once
-    constexpr int UK = VEC ? 2 : 1, UQ = sizeof(T) == 2 && VEC ? (PACKED ? 2 : 4) : 1;   // ... and so many times that in flight
+    constexpr int RPW = 32 / LPR;                       // rows of a warp at once: a unit
+    constexpr int W = sizeof(T) / 2;                    // 16-byte words of 8 columns (VEC)
+    constexpr int UNIT = W * 512, NS = kRopeRing;
+    constexpr bool RING = VEC && W == 1;
+    extern __shared__ __align__(16) uint4 s_ring[];     // [warp][NS][UNIT / 16]
+    __shared__ uint4 s_zero;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int slice = warp % p.slices;
-    const int t = static_cast<int>(blockIdx.x) * (kRopeWarps / p.slices) + warp / p.slices;   // (tokens are below 2^28)
+    const int slice = warp & (p.slices - 1), shift = __popc(p.slices - 1);
+    const int t = static_cast<int>(blockIdx.x) * (kRopeWarps >> shift) + (warp >> shift);   // (tokens are below 2^28)
     const int G = p.c.kv_heads, D = p.c.head_dim;
     const int sub = lane / LPR, col = lane % LPR * 8;
     const bool on = col < D;
-    // rows of one kind, RPW at a time: this warp's begin at `sub + slice * RPW` and lie `step` units apart
+    // units of one kind: this warp's rows begin at `sub + slice * RPW` and lie `step` apart
     const int uk = (G + RPW - 1) / RPW, uq = (p.heads + RPW - 1) / RPW, step = p.slices * RPW;
     const int row0 = slice * RPW + sub;
     // V's begin half the warps further: where a token's rows of a kind are fewer than its warps, others take them
-    const int slice_v = slice + p.slices / 2 - (slice >= p.slices - p.slices / 2 ? p.slices : 0), row0_v = slice_v * RPW + sub;
-    const T* src_k = static_cast<const T*>(p.k) + t * p.k_row + row0 * p.k_head + (VEC ? col : 0);
-    const T* src_v = static_cast<const T*>(p.v) + t * p.v_row + row0_v * p.v_head + (VEC ? col : 0);
-    const T* src_q = static_cast<const T*>(p.q) + t * p.q_row + row0 * p.q_head + (VEC ? col : 0);
-    const int at_col = VEC ? 0 : col;
-    // the first rows of every kind are on their way while the token's place is looked up
-    RopeRow<T, VEC> xk[UK], xv[UK], xq[UQ];
-    auto fetch = [&](auto& x, const T* src, int64_t head, int row, int rows) {
-#pragma unroll
-        for (int n = 0; n < static_cast<int>(sizeof(x) / sizeof(x[0])); ++n)
-            x[n].load(src + n * step * head, at_col, on && row + n * step < rows && t < p.tokens, D, p.start, p.dim);
+    const int slice_v = (slice + p.slices / 2) & (p.slices - 1), row0_v = slice_v * RPW + sub;
+    const T* src_k = static_cast<const T*>(p.k) + t * p.k_row;
+    const T* src_v = static_cast<const T*>(p.v) + t * p.v_row;
+    const T* src_q = static_cast<const T*>(p.q) + t * p.q_row;
+    // this warp's units: nk of K, then nv of V, then nq of Q (slices is a power of two)
+    const bool some = t < p.tokens;
+    const int nk = some ? (uk - slice + p.slices - 1) >> shift : 0, nv = some ? (uk - slice_v + p.slices - 1) >> shift : 0,
+              nq = some ? (uq - slice + p.slices - 1) >> shift : 0;
+    const uint32_t ring = smem_u32(s_ring) + warp * NS * UNIT, mine = ring + lane * 16;
+    // Where unit m's rows begin for this lane (NULL: it has none of them).
+    auto source = [&](int m) -> const T* {
+        const T* src = src_k;
+        int row = row0, rows = G;
+        int64_t head = p.k_head;
+        if (m >= nk + nv) {
+            m -= nk + nv;
+            src = src_q, row = row0, rows = m < nq ? p.heads : 0, head = p.q_head;
+        } else if (m >= nk) {
+            m -= nk;
+            src = src_v, row = row0_v, head = p.v_head;
+        }
+        row += m * step;
+        return on && row < rows ? src + row * head : nullptr;
     };
-    fetch(xk, src_k, p.k_head, row0, G);
-    fetch(xv, src_v, p.v_head, row0_v, G);
-    fetch(xq, src_q, p.q_head, row0, p.heads);
+    auto issue = [&](int m) {
+        if constexpr (RING) {
+            if (m < nk + nv + nq)
+                if (const T* row = source(m)) cp_async16(mine + (m & (NS - 1)) * UNIT, row + col, true);
+            cp_async_commit();
+        }
+    };
+    // the first rows are on their way while the token's place is looked up
+    RopeRow<T, VEC> ahead;   // fp32: the next unit
+    if constexpr (RING) {
+#pragma unroll
+        for (int m = 0; m < NS - 1; ++m) issue(m);
+        if (!on)   // columns behind the row's end
+#pragma unroll
+            for (int i = 0; i < NS; ++i) s_ring[(warp * NS + i) * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);
+        if (lane == 0) s_zero = make_uint4(0u, 0u, 0u, 0u);   // (every warp writes what it reads)
+    } else if constexpr (VEC) {
+        const T* row = source(0);
+        ahead.load(row, col, row != nullptr, D, 0, 0);
+    }
 
     int b = -1, page = -1, in_page = 0;
     int64_t i = 0, slot = 0, at = 0;
@@ -292,7 +399,10 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) =
             if (p.seen_out != nullptr) p.seen_out[b] = static_cast<int32_t>(at) + (page >= 0 ? 1 : 0);
         }
     }
-    if (b < 0) return;
+    if (b < 0) {
+        cp_async_wait<0>();
+        return;
+    }
     if (slice == 0 && page >= 0 && (p.weights != nullptr || p.positions != nullptr))
         for (int g = lane; g < G; g += 32) {
             const int64_t w = (static_cast<int64_t>(b) * G + g) * p.slot_cap + slot;
@@ -334,12 +444,46 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) =
             }
         }
     }
-    const int from = VEC ? lane - lane % LPR + rope_partner(col, p.start, turns ? p.dim : 0) / 8 : lane;   // the lane that has what these turn with
+    // where the columns these turn with are: in the unit another lane's, zeros for those that do not turn
+    const int other = VEC ? lane - lane % LPR + rope_partner(col, p.start, turns ? p.dim : 0) / 8 : lane;
+    uint32_t from = 0, from_stage = 0;
+    if constexpr (RING) {
+        from = turns ? ring + other * 16 : smem_u32(&s_zero);
+        from_stage = turns ? UNIT : 0;
+    }
 
+    int m = 0;   // units taken
+    // The next unit's rows (has: this lane's is one).
+    auto next = [&](RopeRow<T, VEC>& x, const T* src, bool has) {
+        if constexpr (RING) {
+            __syncwarp();   // every lane has read the unit before
+            issue(m + NS - 1);
+            cp_async_wait<NS - 1>();
+        } else if constexpr (VEC) {
+            x = ahead;
+            const T* row = source(m + 1);
+            ahead.load(row, col, row != nullptr, D, 0, 0);
+        } else {
+            x.load(src, col, on && has, D, p.start, p.dim);
+        }
+        __syncwarp();   // (a row is read before it is written over: q_out may be q, k_out k)
+        if constexpr (RING) x.read(mine + (m & (NS - 1)) * UNIT);
+        ++m;
+    };
+    // ... of the unit taken last
     auto rotate = [&](const RopeRow<T, VEC>& x, float (&y)[8], float& most) {
         float w[8];
         x.values(y);
-        x.partner(w, from, turns);
+        if constexpr (VEC && !RING) {
+            x.partner(w, other, turns);
+        } else if constexpr (RING) {
+            RopeRow<T, true> r;
+            r.read(from + ((m - 1) & (NS - 1)) * from_stage);
+            r.values(w);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = x.with[j];
+        }
         most = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -369,7 +513,7 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) =
             if ((col & 8) == 0) to[to_scale] = static_cast<uint8_t>(scale);
         }
     };
-    // rows of K or V into their records; true where one has to be done in 64 bits
+    // rows of K or V into their records; true where one has to be done in 64 bits (a warp in some thousand)
     auto store4 = [&](float (&y)[8], float most, bool turned, bool whole, float unit, uint8_t* to, bool has) {
         if (unit != 1.0f) {
             most *= unit;
@@ -387,102 +531,56 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) =
         put4(codes, scale, to, has);
         return __any_sync(0xffffffffu, open && has) != 0;
     };
-    // ... which is done here, a warp in some thousand
-    auto again4 = [&](const T* src, bool turned, float factor, uint8_t* to, bool has) {
-        const RopeSource<T, TT> from64{has ? src - (VEC ? col : 0) : nullptr, turned ? cos : nullptr, sin, col, D, p.start, p.dim, factor};
-        uint32_t scale;
-        const uint32_t codes = fp4_block_exact<T, TT>(from64, &scale);
-        put4(codes, scale, to, has);
-    };
     auto clear = [&](float (&y)[8]) {   // stored nowhere: q_out and k_out are zeros
         if (!placed)
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = 0.0f;
     };
 
-    // (a row is read before it is written over: q_out may be q, k_out k)
-    T* k_out = static_cast<T*>(p.k_out) + t * p.ko_row + row0 * p.ko_head;
-    for (int u = slice, row = row0; u < uk; u += p.slices * UK, row += step * UK) {
-        if (u != slice) fetch(xk, src_k, p.k_head, row, G);
-        __syncwarp();
-        uint32_t again = 0;
-#pragma unroll
-        for (int n = 0; n < UK; ++n) {
-            if (u + n * p.slices >= uk) break;
-            const bool has = row + n * step < G;
-            float y[8], most;
-            rotate(xk[n], y, most);
-            if constexpr (PACKED) {
-                if (page >= 0) {
-                    float z[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) z[j] = y[j];
-                    if (store4(z, most, turns, p.k_exact, p.k_unit, kp + n * step * kh, has)) again |= 1u << n;
-                }
-            } else if (page >= 0 && on && has) {
-                rope_store<T, VEC>(reinterpret_cast<T*>(kp + n * step * kh), y, col, D);
-            }
-            if (p.k_out != nullptr && ((again >> n) & 1u) == 0u) {
+    // units with blocks that are left to 64 bits (of 32 and more units some are done that need not)
+    uint32_t again_k = 0, again_v = 0;
+    for (int n = 0, row = row0; n < nk; ++n, row += step) {
+        RopeRow<T, VEC> x;
+        float y[8], most;
+        next(x, src_k + row * p.k_head, row < G);
+        rotate(x, y, most);
+        if constexpr (PACKED) {
+            if (page >= 0 && store4(y, most, turns, p.k_exact, p.k_unit, kp + n * step * kh, row < G)) again_k |= 1u << (n & 31);
+        } else {
+            if (page >= 0 && on && row < G) rope_store<T, VEC>(reinterpret_cast<T*>(kp + n * step * kh), y, col, D);
+            if (p.k_out != nullptr) {
                 clear(y);
-                if (on && has) rope_store<T, VEC>(k_out + n * step * p.ko_head, y, col, D);
+                if (on && row < G) rope_store<T, VEC>(static_cast<T*>(p.k_out) + t * p.ko_row + row * p.ko_head, y, col, D);
             }
         }
-        if constexpr (PACKED)
-            for (; again != 0u; again &= again - 1) {
-                const int n = __ffs(again) - 1;
-                const bool has = row + n * step < G;
-                again4(src_k + n * step * p.k_head, turns, p.k_scale, kp + n * step * kh, has);
-                if (p.k_out != nullptr) {
-                    RopeRow<T, VEC> x;
-                    x.load(src_k + n * step * p.k_head, at_col, on && has, D, p.start, p.dim);
-                    __syncwarp();
-                    float y[8], most;
-                    rotate(x, y, most);
-                    if (on && has) rope_store<T, VEC>(k_out + n * step * p.ko_head, y, col, D);
-                }
-            }
-        src_k += step * UK * p.k_head;
-        kp += step * UK * kh;
-        k_out += step * UK * p.ko_head;
     }
-    for (int u = slice_v, row = row0_v; page >= 0 && u < uk; u += p.slices * UK, row += step * UK) {
-        if (u != slice_v) fetch(xv, src_v, p.v_head, row, G);
-        uint32_t again = 0;
-#pragma unroll
-        for (int n = 0; n < UK; ++n) {
-            if (u + n * p.slices >= uk) break;
-            const bool has = row + n * step < G;
-            if constexpr (PACKED) {
-                float y[8];
-                xv[n].values(y);
-                if (store4(y, 0.0f, false, p.v_exact, p.v_unit, vp + n * step * vh, has)) again |= 1u << n;
-            } else if (on && has) {
-                xv[n].store(reinterpret_cast<T*>(vp + n * step * vh), col, D);
-            }
+    for (int n = 0, row = row0_v; n < nv; ++n, row += step) {
+        const bool has = row < G && page >= 0;
+        RopeRow<T, VEC> x;
+        next(x, src_v + row * p.v_head, has);
+        if constexpr (PACKED) {
+            float y[8];
+            x.values(y);
+            if (store4(y, 0.0f, false, p.v_exact, p.v_unit, vp + n * step * vh, has)) again_v |= 1u << (n & 31);
+        } else if (on && has) {
+            x.store(reinterpret_cast<T*>(vp + n * step * vh), col, D);
         }
-        if constexpr (PACKED)
-            for (; again != 0u; again &= again - 1) {
-                const int n = __ffs(again) - 1;
-                again4(src_v + n * step * p.v_head, false, p.v_scale, vp + n * step * vh, row + n * step < G);
-            }
-        src_v += step * UK * p.v_head;
-        vp += step * UK * vh;
     }
     T* q_out = static_cast<T*>(p.q_out) + t * p.qo_row + row0 * p.qo_head;
-    for (int u = slice, row = row0; u < uq; u += p.slices * UQ, row += step * UQ) {
-        if (u != slice) fetch(xq, src_q, p.q_head, row, p.heads);
-        __syncwarp();
-#pragma unroll
-        for (int n = 0; n < UQ; ++n) {
-            if (u + n * p.slices >= uq) break;
-            float y[8], most;
-            rotate(xq[n], y, most);
-            clear(y);
-            if (on && row + n * step < p.heads) rope_store<T, VEC>(q_out + n * step * p.qo_head, y, col, D);
-        }
-        src_q += step * UQ * p.q_head;
-        q_out += step * UQ * p.qo_head;
+    for (int n = 0, row = row0; n < nq; ++n, row += step) {
+        const bool has = row < p.heads;
+        RopeRow<T, VEC> x;
+        float y[8], most;
+        next(x, src_q + row * p.q_head, has);
+        rotate(x, y, most);
+        clear(y);
+        if (on && has) rope_store<T, VEC>(q_out, y, col, D);
+        q_out += step * p.qo_head;
     }
+    if constexpr (RING) cp_async_wait<0>();
+    if constexpr (PACKED)
+        if ((again_k | again_v) != 0u || p.k_out != nullptr)
+            rope4_rest<T, TT, LPR, VEC>(p, RopePlace{t, page, in_page, at, placed}, slice, slice_v, again_k, again_v);
 }
 
 // The lengths after a packed append, one warp per sequence: its tokens up to the first that
