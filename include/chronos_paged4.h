@@ -138,8 +138,8 @@ typedef struct ChronosPagedBoundsArgs {
  * m = ceil(n / page_size) pages.  For each kv head, pages[t, g, :] = ascending, the pages
  * j < first and j >= m - last, and of the others those with the highest
  *     score_j = sum over the group's heads h and d of max(q_hd bounds[j,0,g,d], q_hd bounds[j,1,g,d])
- * (NaN above every number, equal ones by the lower page), min(topk, m) in all, -1
- * behind.  Scores are sums in 64 bits.  The rows of tokens behind the last sequence are
+ * (0 times infinity and a maximum with NaN are NaN; NaN above every number, equal ones
+ * by the lower page), min(topk, m) in all, -1 behind.  Scores are sums in 64 bits.  The rows of tokens behind the last sequence are
  * left as they are.  A page number that is none ranks last, a lens[b] beyond the table is
  * cut to it; both are reported. */
 typedef struct ChronosPagedSelectArgs {

@@ -6,7 +6,10 @@
 //     score = sum_d up_d hi_d + down_d lo_d,   up = sum_h max(q_h, 0), down = sum_h min(q_h, 0),
 // whatever the number of heads: 2 D products per page for 2 D elements read.  It is summed
 // in 64 bits, whose rate (half of fp32's) the reading does not leave behind: pages that a
-// sum in 32 bits would mix up keep the order that their exact scores have.
+// sum in 32 bits would mix up keep the order that their exact scores have.  That holds for
+// finite bounds and queries: where an infinity meets up or down = 0 (no query of that sign) the
+// product is NaN and the maximum need not be.  Any bound or query that is not finite makes the
+// sum not finite, so those few pages are found by their scores and done again head by head.
 #pragma once
 
 #include "chronos_paged4.h"
@@ -182,6 +185,7 @@ struct SelectShared {
     int scan[kSelectWarps];
     unsigned long long ends[2][kSelectWarps];
     int digit, above, same;
+    int odd;   // a score of the block's pages is not finite
 };
 
 // The pages of one token and kv head, by a block.  Of the pages that are not always in, the
@@ -284,6 +288,76 @@ __device__ __forceinline__ void select_row(const PagedSelectParams& p, SelectSha
     }
 }
 
+// A lane's part of a page's score (8 lanes a page) from the formula as it stands, NaN where a
+// product or a maximum is: columns that are finite are summed as paged_select_kernel sums them, so
+// that equal scores stay equal.
+template <typename T>
+__device__ double select_literal(const PagedSelectParams& p, int64_t token, int g, int page, int part) {
+    const int G = p.c.kv_heads, D = p.c.head_dim;
+    const T* lo_row = static_cast<const T*>(p.bounds) + (static_cast<int64_t>(page) * 2 * G + g) * D;
+    const T* hi_row = lo_row + static_cast<int64_t>(G) * D;
+    double acc = 0.0, odd = 0.0;
+    for (int d0 = part * 8; d0 < D; d0 += 64) {
+        double q[2][8], x[2][8];   // down and up, lo and hi
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            q[0][e] = q[1][e] = x[0][e] = x[1][e] = 0.0;
+            const int d = d0 + e;
+            if (d >= D) continue;
+            const T* head = static_cast<const T*>(p.q) + token * p.q_row + static_cast<int64_t>(g) * p.rep * p.q_head + d;
+            const double lo = to_f32<T>(lo_row[d]), hi = to_f32<T>(hi_row[d]);
+            double sum = 0.0;
+            for (int h = 0; h < p.rep; ++h) {
+                const double v = to_f32<T>(head[h * p.q_head]), a = v * lo, b = v * hi;
+                sum += a != a || a > b ? a : b;   // NaN where one is
+                if (v > 0.0) q[1][e] += v;
+                else q[0][e] += v;
+            }
+            x[0][e] = lo;
+            x[1][e] = hi;
+            if (!(fabs(sum) < INFINITY)) {
+                odd += sum;
+                x[0][e] = x[1][e] = q[0][e] = q[1][e] = 0.0;
+            } else {   // an infinity here is on the side that no query takes
+                if (!(fabs(lo) < INFINITY)) x[0][e] = 0.0;
+                if (!(fabs(hi) < INFINITY)) x[1][e] = 0.0;
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc = fma(q[w][e], x[w][e], acc);
+    }
+    return acc + odd;
+}
+
+// The scores of this block's pages that are not finite, again.  Whole blocks call it; 8 lanes take
+// a page as before.
+template <typename T, int ROUND, int TOKENS>
+__device__ __noinline__ void select_again(const PagedSelectParams& p, unsigned long long* keys, int seq, int64_t t0, int n, int g, int rank, int len) {
+    constexpr int GROUPS = kSelectThreads / 8;
+    const int part = threadIdx.x & 7, group = threadIdx.x >> 3;
+    const uint32_t lanes = 0xffu << (threadIdx.x & 24);
+    const unsigned long long inf = select_key(INFINITY), minus = select_key(-INFINITY);
+    const int most = (len + p.c.page_size - 1) / p.c.page_size;
+    for (int64_t j0 = static_cast<int64_t>(rank) * ROUND; j0 < most; j0 += static_cast<int64_t>(p.cluster) * ROUND)
+        for (int64_t j = j0 + group; j < min(j0 + ROUND, static_cast<int64_t>(most)); j += GROUPS) {
+            const int page = p.c.page_table[seq * p.c.page_table_stride + j];
+            if (page < 0 || page >= p.c.num_pages) continue;
+            for (int t = 0; t < n; ++t) {
+                if (j * p.c.page_size >= max(len - (TOKENS == 1 ? 0 : n - 1 - t), 0)) continue;   // behind the token
+                unsigned long long* key = keys + static_cast<int64_t>(t) * p.c.kv_heads * p.width + j;
+                unsigned long long k = part == 0 ? *key : 0ull;
+                k = __shfl_sync(lanes, k, 0, 8);
+                if (k < inf && k > minus) continue;
+                double x = select_literal<T>(p, t0 + t, g, page, part);
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) x += __shfl_xor_sync(lanes, x, o);
+                if (part == 0) *key = select_key(x);
+            }
+        }
+}
+
 // Bound by reading the bounds.  A cluster of p.cluster blocks per TOKENS tokens of a sequence (1
 // where every sequence has one) and kv head.  Scores: the blocks share the pages, 8 lanes a
 // page, two pages at a time (16-bit types), whose loads all go out before the first is used; each
@@ -344,7 +418,9 @@ __global__ void __launch_bounds__(kSelectThreads, TOKENS == 1 ? 3 : 2) paged_sel
     const int most = (len + p.c.page_size - 1) / p.c.page_size;
     unsigned long long* keys = p.keys + ((t0 - p.token0) * G + g) * p.width;   // of token t: t * G * width on
     auto pages_of = [&](int t) { return TOKENS == 1 ? most : (max(len - (n - 1 - t), 0) + p.c.page_size - 1) / p.c.page_size; };
+    bool again = false;
     if (most > p.topk) {   // (else all pages are taken: no scores)
+        if (threadIdx.x == 0) s_sel.odd = 0;
         const int D64 = (D + 63) & ~63;
         for (int i = threadIdx.x; i < n * D64; i += kSelectThreads) {
             const int t = i / D64, d = i % D64;
@@ -439,15 +515,21 @@ __global__ void __launch_bounds__(kSelectThreads, TOKENS == 1 ? 3 : 2) paged_sel
 #pragma unroll
                         for (int o = 1; o < 8; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
                         const int j = j0 + k * GROUPS;
-                        if (part == 0 && j < pages) keys[t * G * p.width + j] = page[k] < 0 ? 0ull : select_key(x);
+                        if (part == 0 && j < pages) {
+                            keys[t * G * p.width + j] = page[k] < 0 ? 0ull : select_key(x);
+                            if (!(fabs(x) < INFINITY)) s_sel.odd = 1;
+                        }
                     }
                 }
             }
         }
+        __syncthreads();
+        again = s_sel.odd != 0;
+        if (again) select_again<T, ROUND, TOKENS>(p, keys, seq, t0, n, g, rank, len);
     }
     // every block's keys are written (they are read from global memory, by blocks of this cluster only)
     if (C > 1) cooperative_groups::this_cluster().sync();
-    else __syncthreads();
+    else if (again) __syncthreads();
     for (int t = rank; t < n; t += C) {
         select_row(p, s_sel, s_keys, keys + t * G * p.width, p.pages + ((t0 + t) * G + g) * p.topk, pages_of(t));
         __syncthreads();   // the next one writes where this one reads

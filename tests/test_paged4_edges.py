@@ -1,0 +1,104 @@
+"""The paged cache's further operators (include/chronos_paged4.h) at the edges of what they
+take: bounds and queries that are not finite, rows at the ends of their type's range,
+factors with many bits, windows over long rows, results that overlap inputs.
+
+CPU: refusals.  GPU: against the definitions in 64 bits of test_paged4, with its tolerances.
+"""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from test_paged4 import (BF, FP, HF, _cache4, _check_attention, _i32, _native_cache, _page_table, _quantise, _refuses, _rnd, _rotate,
+                         _stored, _visible, gpu, lib)  # noqa: F401
+
+
+# ---------------------------------------------------------------------------------------
+# selection among bounds and queries that are not finite
+# ---------------------------------------------------------------------------------------
+
+def _literal(q, lo, hi, g, topk, first, last):
+    """The pages of one token by the formula as it stands, head by head: q [H, D], lo and hi [m, G, D] -> [G, topk]."""
+    m, h = lo.shape[0], q.shape[0]
+    res = torch.full((g, topk), -1, dtype=torch.int32)
+    for i in range(g):
+        x = q[i * h // g: (i + 1) * h // g, None].double()
+        score = torch.maximum(x * lo[:, i].double(), x * hi[:, i].double()).sum((0, 2)).tolist() if m else []
+
+        def rank(j):
+            if j < first or j >= m - last:
+                return (0, 0.0, j)
+            return (1, 0.0, j) if math.isnan(score[j]) else (2, -score[j], j)
+        best = sorted(sorted(range(m), key=rank)[:topk])
+        res[i, : len(best)] = torch.tensor(best, dtype=torch.int32)
+    return res
+
+
+def _odd_bounds(n, g, d, dt, seed):
+    """Bounds of n pages, most of them ordinary; every tenth page has columns that are infinite on one side, on both,
+    the same infinity twice, or no number."""
+    bounds = _rnd(seed, n, 2, g, d).sort(dim=1).values
+    kinds = [(-math.inf, None), (None, math.inf), (-math.inf, math.inf), (math.inf, math.inf), (-math.inf, -math.inf), (math.nan, math.nan),
+             (-math.inf, None), (None, math.inf)]
+    for i in range(0, n, 10):
+        lo, hi = kinds[i // 10 % len(kinds)]
+        columns = [(i * 7) % d] if i % 20 else [(i * 7) % d, (i * 3 + 1) % d, d - 1]
+        for c in columns:
+            if lo is not None:
+                bounds[i, 0, :, c] = lo
+            if hi is not None:
+                bounds[i, 1, :, c] = hi
+    return bounds.to(dt).contiguous()
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("h, g, d", [(2, 2, 64), (8, 2, 128), (9, 1, 96), (16, 2, 256), (6, 3, 37)])
+@pytest.mark.parametrize("queries", ["up", "down", "mixed", "some zero", "one infinite"])
+@pytest.mark.parametrize("new", [None, [1, 9, 17]])
+def test_select_among_bounds_that_are_not_finite(dt, h, g, d, queries, new):
+    from project_chronos_b200 import ops
+    size, topk, first, last, lens = 4, 60, 1, 2, [700, 1500, 1999]
+    table, n = _page_table(3, 500, 1, 1)
+    bounds = _odd_bounds(n, g, d, dt, 2)
+    t = 3 if new is None else sum(new)
+    q = _rnd(3, t, h, d)
+    if queries == "up":
+        q = q.abs() + 0.01
+    elif queries == "down":
+        q = -q.abs() - 0.01
+    elif queries == "some zero":
+        q = torch.where(torch.rand(q.shape, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda") < 0.3, 0.0, q.abs() + 0.01)
+        q[:, :, :4] = 0.0
+    elif queries == "one infinite":
+        q[::2, 0, 5] = math.inf
+        q[1::2, h - 1, 6] = -math.inf
+    q = q.to(dt)
+    cu = None if new is None else torch.tensor([0] + new, dtype=torch.int32, device="cuda").cumsum(0).to(torch.int32)
+    got = ops.paged_select(q, bounds, table, _i32(*lens), size, topk, first=first, last=last, cu_seqlens=cu)
+    ops.check_status(got.device)
+    row = 0
+    for i in range(3):
+        for j in range(1 if new is None else new[i]):
+            at = lens[i] if new is None else lens[i] - new[i] + 1 + j
+            m = -(-at // size)
+            x = bounds[table[i, :m].long()]
+            assert torch.equal(got[row].cpu(), _literal(q[row], x[:, 0], x[:, 1], g, topk, first, last)), (i, j)
+            row += 1
+
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("odd", [10, 20])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_an_infinite_bound_that_no_query_meets_changes_nothing(dt, odd, sign):
+    """Two equal pages, one of them infinite on the side that the queries never take: the lower page goes first."""
+    from project_chronos_b200 import ops
+    h, g, d, m = 4, 2, 64, 60
+    bounds = torch.zeros(m, 2, g, d, device="cuda")
+    bounds[[10, 20]] = torch.tensor([-1.0, 1.0], device="cuda")[None, :, None, None]
+    bounds[odd, 0 if sign > 0 else 1, :, 7] = -sign * math.inf
+    q = sign * (_rnd(1, 1, h, d).abs() + 0.5)
+    got = ops.paged_select(q.to(dt), bounds.to(dt), torch.arange(m, dtype=torch.int32, device="cuda").view(1, m), _i32(m), 1, 2)
+    assert got[0].tolist() == [[10, 59]] * g
