@@ -184,7 +184,7 @@ __device__ __forceinline__ uint32_t fp4_block_exact(const RopeSource<T, TT>& src
 
 // Codes of a lane's 8 values y (in units of the cache's factor; top: the largest magnitude, NaN
 // where one is) and the scale of its block of 16 (two lanes).  off: no value of the lane is off by more than 2^-22 off; 0 where all are
-// what they are.  open: the block has to be decided in 64 bits.  Whole warps call it.
+// what they are.  open: the block has to be decided in 64 bits (codes and scale are then not).  Whole warps call it.
 template <typename T>
 __device__ __forceinline__ uint32_t fp4_block(const float (&y)[8], float top, float off, uint32_t& scale, bool& open) {
     // here and in what follows: NaN where one of the 16 is
@@ -226,7 +226,9 @@ __device__ __forceinline__ uint32_t fp4_block(const float (&y)[8], float top, fl
         open |= codes != fp4_codes(u);
     }
     scale = two & 0xffu;
-    open &= finite;
+    // NaN and infinities of the inputs, or finite values that pass fp32 on the way (a sum of the
+    // rotation, a quotient by a small factor): 64 bits tell which
+    open |= !finite;
     codes = finite && scale != 0u ? codes : 0u;
     if (!finite) scale = kFp8Nan;
     return codes;

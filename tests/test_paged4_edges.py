@@ -102,3 +102,49 @@ def test_an_infinite_bound_that_no_query_meets_changes_nothing(dt, odd, sign):
     q = sign * (_rnd(1, 1, h, d).abs() + 0.5)
     got = ops.paged_select(q.to(dt), bounds.to(dt), torch.arange(m, dtype=torch.int32, device="cuda").view(1, m), _i32(m), 1, 2)
     assert got[0].tolist() == [[10, 59]] * g
+
+
+# ---------------------------------------------------------------------------------------
+# 4-bit pages: rows at the ends of their type's range
+# ---------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dt, units", [(BF, (1.0, 1.0)), (BF, (0.5, 3.1)), (BF, (1e-30, 2.0 ** -126)), (HF, (1e-36, 2.0 ** -126)), (FP, (1.0, 1.0)),
+                                       (FP, (0.37, 0.25)), (FP, (1e-30, 2.0 ** 126)), (BF, (2.0 ** 126, 1e37))])
+@pytest.mark.parametrize("g, d, r", [(2, 128, 128), (3, 64, 32), (3, 37, 10)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_4bit_pages_of_rows_that_pass_the_range_of_fp32(dt, units, g, d, r, packed):
+    """Values whose rotation or quotient passes fp32 are finite all the same: the largest scale and code.  NaN and
+    infinities stay what they are, blocks of zeros and small values too."""
+    from project_chronos_b200 import ops
+    size, t = 16, 24
+    big = torch.finfo(dt).max
+    def rows(seed):
+        x = _rnd(seed, t, g, d).clamp(-2, 2) / 2 * big
+        m = torch.arange(t, device="cuda") % 6
+        x = torch.where((m == 1)[:, None, None], torch.sign(x) * big, x)
+        x = torch.where((m == 2)[:, None, None], 0.0, x)
+        x = torch.where((m == 3)[:, None, None], x * 1e-30, x)
+        x = x.to(dt)
+        x[4, 0, d // 2], x[10, 0, d // 3], x[16, 0, 0] = math.nan, math.inf, -math.inf
+        return x
+    k, v = rows(1), rows(2)
+    a = torch.linspace(0.0, 6.0, 40 * r // 2, device="cuda", dtype=torch.float64).view(40, r // 2)
+    cos, sin = torch.cat([a.cos(), a.cos()], 1).float(), torch.cat([a.sin(), a.sin()], 1).float()
+    b = 2 if packed else t
+    new = [9, 15] if packed else [1] * t
+    table, n = _page_table(b, 2, 1, 3)
+    kp, vp = (torch.zeros(n, g, ops.packed_page_bytes(size, d), dtype=torch.uint8, device="cuda") for _ in range(2))
+    cu = torch.tensor([0] + new, dtype=torch.int32, device="cuda").cumsum(0).to(torch.int32) if packed else None
+    ops.paged_append_rope(k, v, kp, vp, table, _i32(*[0] * b), _i32(*[5] * b), cos, sin, cu_seqlens=cu, k_scale=units[0], v_scale=units[1])
+    ops.check_status(kp.device)
+    at = 0
+    for i, m in enumerate(new):
+        part = slice(at, at + m)
+        turned, _ = _rotate(k[part].double(), cos[5: 5 + m], sin[5: 5 + m], 0)
+        for pages, x, unit in ((kp, turned, units[0]), (vp, v[part].double(), units[1])):
+            code, scale, _ = _quantise(x, unit)
+            code_, scale_, _ = _stored(pages, table[i], d, size, torch.arange(m, device="cuda"))
+            assert torch.equal(scale_[..., : scale.shape[-1]], scale)
+            assert torch.equal(code_[..., :d], code)
+        at += m
