@@ -19,7 +19,7 @@
  * slot (byte i: column 2i in the low half, 2i + 1 in the high one), then their
  * scales, P / 16 bytes a slot (one for 16 columns).  A code is e2m1 (sign and one of 0,
  * 0.5, 1, 1.5, 2, 3, 4, 6), a scale e4m3 without sign, and
- *     value = code * scale * k_scale (v_scale).
+ *     value = code * scale * k_scale (v_scale; both between 2^-126 and 2^126).
  * Of 16 columns x_i, y_i = x_i / k_scale, the append stores
  *     scale = e4m3(min(fp32(max |y_i| / 6), 448)),  code_i = e2m1(y_i / scale)
  * to the nearest, ties to the even code, as exact arithmetic on the inputs and the
@@ -58,7 +58,7 @@ typedef struct ChronosPagedRopeArgs {
     int32_t rope_start;
     int32_t table_len;         /* rows of cos and sin */
     int32_t table_dtype;       /* fp32, or cache.dtype */
-    float k_scale, v_scale;    /* packed: > 0 */
+    float k_scale, v_scale;    /* packed: 2^-126 to 2^126 */
     int64_t num_tokens;
     const void* k;             /* [num_tokens, G, D] */
     const void* v;
@@ -104,8 +104,8 @@ typedef struct ChronosPagedDecode4Args {
     int32_t heads;
     int32_t window;
     int32_t sinks;
-    float scale;               /* > 0 */
-    float k_scale, v_scale;    /* > 0 */
+    float scale;               /* > 0; scale * k_scale 2^-126 to 2^126 */
+    float k_scale, v_scale;    /* 2^-126 to 2^126 */
     const void* q;             /* [B, H, D] */
     int64_t q_row_stride, q_head_stride;
     void* out;                 /* [B, H, D] */
@@ -169,7 +169,7 @@ typedef struct ChronosPagedSparseArgs {
     int32_t heads;
     int32_t topk;              /* entries of pages per token and kv head */
     float scale;
-    float k_scale, v_scale;
+    float k_scale, v_scale;    /* packed: as in chronos_paged_decode4 */
     int64_t num_tokens;
     const void* q;             /* [num_tokens, H, D] */
     int64_t q_row_stride, q_head_stride;

@@ -35,7 +35,8 @@ int check_decode4(const ChronosPagedDecode4Args* a) {
     if (a->window < 0 || a->sinks < 0)
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: window %d, sinks %d must not be negative", what, a->window, a->sinks);
     if (int rc = check_positive("scale", a->scale, what)) return rc;
-    return check_packed(a->cache, a->k_scale, a->v_scale, what);
+    if (int rc = check_packed(a->cache, a->k_scale, a->v_scale, what)) return rc;
+    return check_scores(a->scale, a->k_scale, what);
 }
 
 template <typename T, int DP, int NT>

@@ -103,8 +103,10 @@ extern "C" int chronos_paged_sparse(const ChronosPagedSparseArgs* a, void* strea
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: topk %d pages of %d slots", what, a->topk, a->cache.page_size);
     if (a->num_tokens * a->heads >= INT32_MAX / 8)
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: %lld tokens of %d heads", what, static_cast<long long>(a->num_tokens), a->heads);
-    if (a->packed)
+    if (a->packed) {
         if (int rc = check_packed(a->cache, a->k_scale, a->v_scale, what)) return rc;
+        if (int rc = check_scores(a->scale, a->k_scale, what)) return rc;
+    }
     if (a->cache.batch == 0 || a->num_tokens == 0) return CHRONOS_OK;
     if (int rc = check_cache_pointers(a->cache, what)) return rc;
     if (a->q == nullptr || a->out == nullptr || (a->topk > 0 && a->pages == nullptr))

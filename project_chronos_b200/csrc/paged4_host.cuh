@@ -24,6 +24,20 @@ inline int check_tokens(int64_t tokens, const int32_t* cu, const ChronosPagedCac
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: %lld rows for %d sequences without cu_seqlens", what, static_cast<long long>(tokens), c.batch);
     return CHRONOS_OK;
 }
+// The factor of a cache: values are multiplied by its reciprocal in fp32, which has to be as exact as
+// any (neither infinite nor with fewer bits).
+inline int check_factor(const char* name, float x, const char* what) {
+    if (!(x >= 0x1p-126f && x <= 0x1p126f))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: %s %g must lie between 2^-126 and 2^126", what, name, x);
+    return CHRONOS_OK;
+}
+// The factor of the scores over 4-bit pages, held in fp32 as well.
+inline int check_scores(float scale, float k_scale, const char* what) {
+    const double x = static_cast<double>(scale) * k_scale;
+    if (!(x >= 0x1p-126 && x <= 0x1p126))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: scale %g * k_scale %g must lie between 2^-126 and 2^126", what, scale, k_scale);
+    return CHRONOS_OK;
+}
 // Rows of heads, strides in bytes.
 struct RowsOf {
     const void* at;
@@ -59,8 +73,8 @@ inline int check_packed(const ChronosPagedCache& c, float k_scale, float v_scale
         static_cast<int64_t>(c.page_size) * 144 > INT32_MAX)
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: 4-bit pages of %d slots, %lld and %lld bytes apart", what, c.page_size,
                     static_cast<long long>(c.k_page_stride), static_cast<long long>(c.v_page_stride));
-    if (int rc = check_positive("k_scale", k_scale, what)) return rc;
-    return check_positive("v_scale", v_scale, what);
+    if (int rc = check_factor("k_scale", k_scale, what)) return rc;
+    return check_factor("v_scale", v_scale, what);
 }
 
 }  // namespace chronos

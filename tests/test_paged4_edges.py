@@ -148,3 +148,36 @@ def test_4bit_pages_of_rows_that_pass_the_range_of_fp32(dt, units, g, d, r, pack
             assert torch.equal(scale_[..., : scale.shape[-1]], scale)
             assert torch.equal(code_[..., :d], code)
         at += m
+
+
+# ---------------------------------------------------------------------------------------
+# factors
+# ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("factor", [1e-45, 1e-39, 1.17e-38, 2.0 ** -126 * (1 - 2.0 ** -23), 2.0 ** 126 * (1 + 2.0 ** -23), 3e38])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+def test_factors_without_a_reciprocal_are_refused(lib, factor, which):  # noqa: F811
+    from project_chronos_b200 import _native as N
+    one = {**dict(k_scale=1.0, v_scale=1.0), which: factor}
+    c = _native_cache(N)
+    _refuses(lib, "append_rope", N.ChronosPagedRopeArgs(cache=c, num_tokens=2, packed=1, **one), which.encode())
+    _refuses(lib, "gather", N.ChronosPagedGatherArgs(cache=c, num_tokens=2, packed=1, **one), which.encode())
+    _refuses(lib, "decode4", N.ChronosPagedDecode4Args(cache=c, heads=2, scale=1.0, **one), which.encode(), workspace=True)
+    _refuses(lib, "sparse", N.ChronosPagedSparseArgs(cache=c, heads=2, scale=1.0, num_tokens=2, packed=1, **one), which.encode())
+    if which == "k_scale":
+        _refuses(lib, "bounds", N.ChronosPagedBoundsArgs(cache=c, packed=1, k_scale=factor), b"k_scale")
+
+
+@pytest.mark.parametrize("factor", [2.0 ** -126, 2.0 ** 126, 0.37])
+def test_factors_with_a_reciprocal_are_taken(lib, factor):  # noqa: F811
+    from project_chronos_b200 import _native as N
+    a = N.ChronosPagedDecode4Args(cache=_native_cache(N, batch=0), heads=2, scale=1.0, k_scale=factor, v_scale=factor)
+    assert lib.chronos_paged_decode4(ctypes.byref(a), None) == N.CHRONOS_OK
+
+
+@pytest.mark.parametrize("scale, factor", [(1e-3, 2.0 ** -126), (4.0, 2.0 ** 126), (1e-30, 1e-30)])
+def test_scores_without_a_factor_in_fp32_are_refused(lib, scale, factor):  # noqa: F811
+    from project_chronos_b200 import _native as N
+    one = dict(heads=2, scale=scale, k_scale=factor, v_scale=1.0)
+    _refuses(lib, "decode4", N.ChronosPagedDecode4Args(cache=_native_cache(N), **one), b"scale", workspace=True)
+    _refuses(lib, "sparse", N.ChronosPagedSparseArgs(cache=_native_cache(N), num_tokens=2, packed=1, **one), b"scale")
