@@ -117,7 +117,8 @@ typedef struct ChronosPagedDecode4Args {
 } ChronosPagedDecode4Args;
 
 /* bounds[page, 0, g, d] and [page, 1, g, d] = smallest and largest key of column d over the
- * page's slots in use, rounded to the layer type; NaN where one of them is.  Brought
+ * page's slots in use (of 4-bit pages, whose values may have more bits than the layer
+ * type, the smallest rounded down and the largest up); NaN where one of them is.  Brought
  * up to date: the pages of the newest tokens (one per sequence, or cu_seqlens[b + 1] -
  * cu_seqlens[b]), whose older slots are in the bounds already; with `full` every page of
  * every sequence, from its slots alone. */

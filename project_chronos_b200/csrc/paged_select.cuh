@@ -44,6 +44,16 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
+// A smallest or largest value of codes and scales as it is stored: times the cache's factor, whose
+// product has more bits than 16-bit types (than fp32, too), rounded outwards, so that no key lies outside.
+template <typename T>
+__device__ __forceinline__ T bound_outwards(float x, float unit, bool largest) {
+    const float y = largest ? __fmul_ru(x, unit) : __fmul_rd(x, unit);
+    if constexpr (std::is_same<T, float>::value) return y;
+    else if constexpr (std::is_same<T, __half>::value) return largest ? __float2half_ru(y) : __float2half_rd(y);
+    else return largest ? __float2bfloat16_ru(y) : __float2bfloat16_rd(y);
+}
+
 // A block per (sequence, kv head) and page in turn: LPR lanes hold a slot's columns, 8 each,
 // the block's other groups take the next slots; the groups meet in shared memory.  One new token
 // per sequence is bound by latency (32 rows of 8 heads 3 us), since older slots are not read again.
@@ -83,7 +93,7 @@ __global__ void __launch_bounds__(kBoundThreads) paged_bounds_kernel(const __gri
                 if constexpr (PACKED) {
                     const uint8_t* record = static_cast<const uint8_t*>(p.c.k_pages) + page * p.c.k_page_stride + g * p.c.k_head_stride +
                                             (i >> 4) * fp4_record(p.columns);
-                    fp4_load8(record, i & 15, col, p.columns, p.k_scale, x);
+                    fp4_load8(record, i & 15, col, p.columns, 1.0f, x);   // (the factor, a positive one, comes last)
                 } else {
                     const T* k = static_cast<const T*>(p.c.k_pages) + page * p.c.k_page_stride + i * p.c.k_slot_stride + g * p.c.k_head_stride;
                     if constexpr (VEC) {
@@ -114,6 +124,7 @@ __global__ void __launch_bounds__(kBoundThreads) paged_bounds_kernel(const __gri
             const int used = min(GROUPS, stop - at);
             for (int k = 1; k < used; ++k) v = which ? max_nan(v, s_x[1][k][d]) : min_nan(v, s_x[0][k][d]);
             T* to = out + static_cast<int64_t>(which) * G * D + d;
+            if constexpr (PACKED) v = to_f32<T>(bound_outwards<T>(v, p.k_scale, which != 0));
             if (at > 0) {   // older slots are in the bounds already
                 const float old = to_f32<T>(*to);
                 v = which ? max_nan(v, old) : min_nan(v, old);

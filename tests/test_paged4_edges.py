@@ -181,3 +181,42 @@ def test_scores_without_a_factor_in_fp32_are_refused(lib, scale, factor):  # noq
     one = dict(heads=2, scale=scale, k_scale=factor, v_scale=1.0)
     _refuses(lib, "decode4", N.ChronosPagedDecode4Args(cache=_native_cache(N), **one), b"scale", workspace=True)
     _refuses(lib, "sparse", N.ChronosPagedSparseArgs(cache=_native_cache(N), num_tokens=2, packed=1, **one), b"scale")
+
+
+# ---------------------------------------------------------------------------------------
+# bounds of 4-bit pages
+# ---------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("factor", [0.37, 3.1, 1.0, 1e-6, 40.0])
+@pytest.mark.parametrize("g, d, size", [(2, 128, 16), (1, 37, 32)])
+def test_no_key_of_a_4bit_page_lies_outside_its_bounds(dt, factor, g, d, size):
+    """A factor with many bits: the keys have more than the bounds' type.  The bounds lie less than a step outside."""
+    from project_chronos_b200 import PagedCache, ops
+    c = PagedCache(2, 20, g, d, 8, "cuda", dt, page_size=size, four_bit=True, page_bounds=True, k_scale=factor)
+    for b in range(2):
+        c.reserve(b, 100)
+    x = factor * _rnd(1, 83, g, d)
+    x[3::7] *= 400.0
+    x = x.to(dt)
+    c.append(x[:70], x[:70], _i32(0, 50, 70))
+    for i in range(70, 83):
+        c.append(x[i: i + 1], x[i: i + 1], _i32(0, 0, 1))
+    ops.check_status(c.lens.device)
+    lens = c.lens.tolist()
+    assert lens == [50, 33]
+    def check():
+        for b in range(2):
+            key = _stored(c.k_pages, c.page_table[b], d, size, torch.arange(lens[b], device="cuda"))[2] * float(torch.tensor(factor))
+            for j, part in enumerate(key.split(size)):
+                low, high = part.amin(0), part.amax(0)
+                got = c.bounds[c.page_table[b, j].long()].double()
+                assert bool((got[0] <= low).all()) and bool((got[1] >= high).all())
+                step = lambda v: torch.finfo(dt).eps * v.abs() + (2.0 ** -24 if dt == HF else 0.0)  # noqa: E731
+                near = high.abs() < torch.finfo(dt).max
+                assert bool((low - got[0] <= step(low))[low.abs() < torch.finfo(dt).max].all()) and bool((got[1] - high <= step(high))[near].all())
+    check()
+    c.bounds.fill_(math.nan)
+    ops.paged_bounds(c.k_pages, c.bounds, c.page_table, c.lens, full=True, k_scale=factor)
+    check()
