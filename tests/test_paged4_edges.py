@@ -220,3 +220,33 @@ def test_no_key_of_a_4bit_page_lies_outside_its_bounds(dt, factor, g, d, size):
     c.bounds.fill_(math.nan)
     ops.paged_bounds(c.k_pages, c.bounds, c.page_table, c.lens, full=True, k_scale=factor)
     check()
+
+
+# ---------------------------------------------------------------------------------------
+# 4-bit attention: windows and first tokens over long rows, heads of 256
+# ---------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("h, g, d", [(8, 2, 64), (24, 1, 128), (4, 2, 128), (12, 2, 256), (20, 1, 256), (10, 2, 80)])
+@pytest.mark.parametrize("lens", [[20011], [6001, 3, 0, 9000, 4100]])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (4097, 0), (5000, 17), (4999, 300), (4096, 4096)])
+def test_decode4_windows_over_long_rows(lib, dt, h, g, d, lens, window, sinks):  # noqa: F811
+    """Rows that are cut evenly over the blocks (the calls that need a workspace)."""
+    from project_chronos_b200 import _native as N
+    from project_chronos_b200 import ops
+    kp, vp, table, ln, rows = _cache4(lens, g, d, 16, h + d)
+    shape = N.ChronosPagedCache(batch=len(lens), kv_heads=g, head_dim=d, dtype=N.DTYPE_BF16 if dt == BF else N.DTYPE_FP32, num_pages=kp.shape[0],
+                                page_size=16, table_width=table.shape[1])
+    a = N.ChronosPagedDecode4Args(cache=shape, heads=h, window=window, sinks=sinks, scale=1.0, k_scale=1.0, v_scale=1.0)
+    assert lib.chronos_paged_decode4_workspace(ctypes.byref(a)) > 0
+    q = _rnd(6, len(lens), h, d, dt=dt, scale=2.0)
+    lse = torch.empty(len(lens), h, device="cuda")
+    out = ops.paged_attn_decode4(q, kp, vp, table, ln, window=window, sinks=sinks, lse=lse)
+    ops.check_status(out.device)
+    for b, (k, v) in enumerate(rows):
+        seen = _visible(lens[b], window, sinks)
+        _check_attention(out[b], lse[b], q[b], k[seen], v[seen], d ** -0.5, dt, True)
+    assert torch.equal(out, ops.paged_attn_decode4(q, kp, vp, table, ln, window=window, sinks=sinks))
+    over = q.clone()
+    assert ops.paged_attn_decode4(over, kp, vp, table, ln, window=window, sinks=sinks, out=over) is over and torch.equal(over, out)
