@@ -11,7 +11,8 @@
  *   chronos_paged_select       the pages that each query's bounds rank highest
  *   chronos_paged_sparse       attention over the slots of selected pages
  *
- * Conventions as in chronos_paged.h.
+ * Conventions as in chronos_paged.h.  Results may not overlap each other, the cache or
+ * another input, but where a call names it: such calls are refused.
  *
  * Packed pages (4-bit values).  With P = head_dim rounded up to 64, 128 or 256 a
  * page of a kv head is page_size / 16 records of 9 P bytes (page_size is a multiple of
@@ -49,7 +50,7 @@ extern "C" {
  * tables is dropped like one without a page (and its rows of q_out and k_out are
  * zeros; those of a token that only lacks a page are rotated all the same).  Rows
  * behind the last sequence are neither read nor written.  q_out may be q and k_out may
- * be k (with the same strides), other overlaps are not allowed. */
+ * be k (with the same strides). */
 typedef struct ChronosPagedRopeArgs {
     ChronosPagedCache cache;   /* lens: before the append */
     int32_t packed;            /* 1: pages of 4-bit values */
@@ -98,7 +99,8 @@ typedef struct ChronosPagedGatherArgs {
     int32_t* status;
 } ChronosPagedGatherArgs;
 
-/* chronos_paged_decode over packed pages, without running sums. */
+/* chronos_paged_decode over packed pages, without running sums.  out may be q (with the
+ * same strides). */
 typedef struct ChronosPagedDecode4Args {
     ChronosPagedCache cache;
     int32_t heads;
@@ -163,7 +165,7 @@ typedef struct ChronosPagedSelectArgs {
 /* Attention of token t (n slots at or before it, as above) over the slots j < n of the
  * pages pages[t, g, :]; entries below 0 or at or beyond m are passed over, a page that is
  * named twice counts twice.  Nothing visible: zeros and lse = -inf.  Rows of tokens behind
- * the last sequence are left as they are. */
+ * the last sequence are left as they are.  out may be q (with the same strides). */
 typedef struct ChronosPagedSparseArgs {
     ChronosPagedCache cache;
     int32_t packed;

@@ -117,6 +117,9 @@ extern "C" int chronos_paged_decode4(const ChronosPagedDecode4Args* a, void* str
     if (a->cache.batch == 0) return CHRONOS_OK;
     if (int rc = check_cache_pointers(a->cache, what)) return rc;
     if (a->q == nullptr || a->out == nullptr) return fail(CHRONOS_ERR_INVALID_ARG, "%s: q and out are required", what);
+    if (int rc = check_results(what, a->cache, true, a->cache.batch, a->heads, a->q, a->q_row_stride, a->q_head_stride, a->out, a->out_row_stride,
+                               a->out_head_stride, a->lse, RowsOf{}, RowsOf{}))
+        return rc;
     const Decode4Plan d = decode4_plan(a);
     const int64_t units = (static_cast<int64_t>(d.max_vis) / kPdBlock + 1) * a->cache.batch * a->cache.kv_heads * d.parts;
     if (units >= (1 << 30) || static_cast<int64_t>(a->cache.batch) * a->heads >= INT32_MAX / 8)

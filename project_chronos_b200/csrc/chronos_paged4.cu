@@ -141,6 +141,20 @@ extern "C" int chronos_paged_append_rope(const ChronosPagedRopeArgs* a, void* st
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: q_out may be q and k_out k, with the same strides; they overlap nothing else", what);
     if (a->packed)
         if (int rc = check_packed(a->cache, a->k_scale, a->v_scale, what)) return rc;
+    {
+        const int64_t es = a->table_dtype == CHRONOS_DTYPE_FP32 ? 4 : 2;
+        const auto table = [&](const void* at, int64_t row) {
+            return RowsOf{at, at == nullptr || a->rope_dim == 0 ? 0 : a->table_len, row * es, 1, 0, a->rope_dim * es};
+        };
+        const RowsOf cos = table(a->cos, a->cos_row_stride), sin = table(a->sin, a->sin_row_stride), cu = array_of(a->cu_seqlens, n + int64_t{1}, 4),
+                     seen = array_of(a->seen, n, 4);
+        if (int rc = check_apart(what, a->cache, a->packed != 0, {qo, ko}, {cos, sin, cu, seen})) return rc;
+        // (lens_out and seen_out among themselves and against lens and seen: above)
+        ChronosPagedCache rest = a->cache;
+        rest.lens = nullptr;
+        for (const void* out : {a->lens_out, a->seen_out})
+            if (int rc = check_apart(what, rest, a->packed != 0, {array_of(out, n, 4)}, {k, v, q, cos, sin, cu, qo, ko})) return rc;
+    }
     const bool counts = a->lens_out != nullptr || a->seen_out != nullptr;
     if (n == 0 || (a->num_tokens == 0 && !counts)) return CHRONOS_OK;
     if (int rc = check_cache_pointers(a->cache, what)) return rc;
@@ -216,21 +230,12 @@ extern "C" int chronos_paged_gather(const ChronosPagedGatherArgs* a, void* strea
     if (int rc = check_cache_pointers(a->cache, what)) return rc;
     if (a->k_out == nullptr || a->v_out == nullptr || a->cu_seqlens == nullptr)
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: k_out, v_out and cu_seqlens are required", what);
-    {
-        const ChronosPagedCache& c = a->cache;
-        const RowsOf k = rows_of(a->k_out, c.dtype, a->num_tokens, a->k_row_stride, c.kv_heads, a->k_head_stride, c.head_dim),
-                     v = rows_of(a->v_out, c.dtype, a->num_tokens, a->v_row_stride, c.kv_heads, a->v_head_stride, c.head_dim);
-        const int64_t es = a->packed ? 1 : static_cast<int64_t>(elem_bytes(c.dtype));
-        const int64_t slots = a->packed ? 1 : c.page_size;
-        const int64_t bytes = a->packed ? static_cast<int64_t>(c.page_size) / 16 * fp4_record(fp4_columns(c.head_dim)) : c.head_dim * es;
-        const auto pages = [&](const void* at, int64_t page, int64_t slot, int64_t head) {   // as one stretch
-            return RowsOf{at, c.num_pages, page * es, 1, 0, ((slots - 1) * slot + (c.kv_heads - 1) * head) * es + bytes};
-        };
-        const RowsOf kp = pages(c.k_pages, c.k_page_stride, c.k_slot_stride, c.k_head_stride),
-                     vp = pages(c.v_pages, c.v_page_stride, c.v_slot_stride, c.v_head_stride);
-        if (rows_meet(k, v) || rows_meet(k, kp) || rows_meet(k, vp) || rows_meet(v, kp) || rows_meet(v, vp))
-            return fail(CHRONOS_ERR_INVALID_ARG, "%s: k_out and v_out overlap each other or the pages", what);
-    }
+    const ChronosPagedCache& c = a->cache;
+    if (int rc = check_apart(what, c, a->packed != 0,
+                             {rows_of(a->k_out, c.dtype, a->num_tokens, a->k_row_stride, c.kv_heads, a->k_head_stride, c.head_dim),
+                              rows_of(a->v_out, c.dtype, a->num_tokens, a->v_row_stride, c.kv_heads, a->v_head_stride, c.head_dim)},
+                             {array_of(a->cu_seqlens, c.batch + int64_t{1}, 4), array_of(a->first, c.batch, 4)}))
+        return rc;
     PagedGatherParams p{};
     p.c = a->cache;
     p.tokens = a->num_tokens;
@@ -280,6 +285,13 @@ extern "C" int chronos_paged_bounds(const ChronosPagedBoundsArgs* a, void* strea
     if (c.batch == 0 || c.table_width == 0 || c.num_pages == 0) return CHRONOS_OK;
     if (c.lens == nullptr || c.page_table == nullptr || c.k_pages == nullptr || a->bounds == nullptr)
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: lens, page_table, k_pages and bounds are required", what);
+    {
+        ChronosPagedCache keys = c;
+        keys.v_pages = nullptr;
+        if (int rc = check_apart(what, keys, a->packed != 0, {array_of(a->bounds, c.num_pages * int64_t{2} * c.kv_heads * c.head_dim, elem_bytes(c.dtype))},
+                                 {array_of(a->cu_seqlens, c.batch + int64_t{1}, 4)}))
+            return rc;
+    }
     PagedBoundsParams p{};
     p.c = c;
     p.packed = a->packed;
@@ -327,6 +339,15 @@ extern "C" int chronos_paged_select(const ChronosPagedSelectArgs* a, void* strea
     if (c.lens == nullptr || a->q == nullptr || a->pages == nullptr ||
         (bytes > 0 && (c.page_table == nullptr || (c.num_pages > 0 && a->bounds == nullptr))))
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: lens, page_table, q, bounds and pages are required", what);
+    {
+        ChronosPagedCache table = c;
+        table.k_pages = table.v_pages = nullptr;
+        if (int rc = check_apart(what, table, false, {array_of(a->pages, a->num_tokens * c.kv_heads * a->topk, 4)},
+                                 {rows_of(a->q, c.dtype, a->num_tokens, a->q_row_stride, a->heads, a->q_head_stride, c.head_dim),
+                                  array_of(a->bounds, c.num_pages * int64_t{2} * c.kv_heads * c.head_dim, elem_bytes(c.dtype)),
+                                  array_of(a->cu_seqlens, c.batch + int64_t{1}, 4)}))
+            return rc;
+    }
     if (bytes > 0 && (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < bytes))
         return fail(CHRONOS_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes, %zu (256-byte aligned) needed", what,
                     a->workspace == nullptr ? size_t{0} : a->workspace_bytes, bytes);

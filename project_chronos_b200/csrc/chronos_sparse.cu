@@ -111,6 +111,10 @@ extern "C" int chronos_paged_sparse(const ChronosPagedSparseArgs* a, void* strea
     if (int rc = check_cache_pointers(a->cache, what)) return rc;
     if (a->q == nullptr || a->out == nullptr || (a->topk > 0 && a->pages == nullptr))
         return fail(CHRONOS_ERR_INVALID_ARG, "%s: q, out and pages are required", what);
+    if (int rc = check_results(what, a->cache, a->packed != 0, a->num_tokens, a->heads, a->q, a->q_row_stride, a->q_head_stride, a->out, a->out_row_stride,
+                               a->out_head_stride, a->lse, array_of(a->pages, a->num_tokens * a->cache.kv_heads * a->topk, 4),
+                               array_of(a->cu_seqlens, a->cache.batch + int64_t{1}, 4)))
+        return rc;
     PagedDecodeParams p{};
     p.c = a->cache;
     p.heads = a->heads;

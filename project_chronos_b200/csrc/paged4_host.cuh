@@ -1,7 +1,10 @@
 // paged4_host.cuh — argument checks that the calls of include/chronos_paged4.h share.
 #pragma once
 
+#include <iterator>
+
 #include "chronos_paged4.h"
+#include "fp4.cuh"
 #include "paged_host.cuh"
 
 namespace chronos {
@@ -61,8 +64,43 @@ inline bool rows_meet(const RowsOf& a, const RowsOf& b) {
     if (a.row == b.row && a.row > 0 && apart(a.row, ea, eb)) return false;
     return !(a.row == b.row && a.head == b.head && a.head > 0 && a.row % a.head == 0 && apart(a.head, a.bytes, b.bytes));
 }
-// Whether rows that are written meet an input other than as the rows that they are made from.
-inline bool rows_same(const RowsOf& a, const RowsOf& b) { return a.at == b.at && a.row == b.row && a.head == b.head; }
+// Whether the two are the same rows.
+inline bool rows_same(const RowsOf& a, const RowsOf& b) {
+    return a.at == b.at && (a.row == b.row || a.rows <= 1) && (a.head == b.head || a.heads <= 1);
+}
+// n numbers of `size` bytes, one after the other.
+inline RowsOf array_of(const void* at, int64_t n, int64_t size) { return RowsOf{at, at == nullptr ? 0 : 1, 0, 1, 0, n * size}; }
+// The pages of K or V, each as one stretch.
+inline RowsOf pages_of(const ChronosPagedCache& c, bool packed, const void* at, int64_t page, int64_t slot, int64_t head) {
+    const int64_t es = packed ? 1 : static_cast<int64_t>(elem_bytes(c.dtype));
+    const int64_t bytes = packed ? static_cast<int64_t>(c.page_size) / 16 * fp4_record(fp4_columns(c.head_dim)) : c.head_dim * es;
+    const int64_t slots = packed ? 0 : (c.page_size - 1) * slot;
+    return RowsOf{at, at == nullptr ? 0 : c.num_pages, page * es, 1, 0, (slots + (c.kv_heads - 1) * head) * es + bytes};
+}
+// A call's results overlap nothing that it reads (`inputs`, the cache) and not each other.
+inline int check_apart(const char* what, const ChronosPagedCache& c, bool packed, std::initializer_list<RowsOf> results,
+                       std::initializer_list<RowsOf> inputs) {
+    const RowsOf cache[] = {pages_of(c, packed, c.k_pages, c.k_page_stride, c.k_slot_stride, c.k_head_stride),
+                            pages_of(c, packed, c.v_pages, c.v_page_stride, c.v_slot_stride, c.v_head_stride),
+                            RowsOf{c.page_table, c.page_table == nullptr ? 0 : c.batch, c.page_table_stride * 4, 1, 0, c.table_width * int64_t{4}},
+                            array_of(c.lens, c.batch, 4)};
+    for (const RowsOf* r = results.begin(); r != results.end(); ++r) {
+        const auto meets = [&](const RowsOf& x) { return rows_meet(*r, x); };
+        if (std::any_of(std::begin(cache), std::end(cache), meets) || std::any_of(inputs.begin(), inputs.end(), meets) ||
+            std::any_of(r + 1, results.end(), meets))
+            return fail(CHRONOS_ERR_INVALID_ARG, "%s: results overlap each other, the cache or other inputs", what);
+    }
+    return CHRONOS_OK;
+}
+// The results of an attention call: `out` may be `q`.
+inline int check_results(const char* what, const ChronosPagedCache& c, bool packed, int64_t rows, int heads, const void* q, int64_t q_row,
+                         int64_t q_head, const void* out, int64_t out_row, int64_t out_head, const float* lse, const RowsOf& list, const RowsOf& cu) {
+    const RowsOf in = rows_of(q, c.dtype, rows, q_row, heads, q_head, c.head_dim), to = rows_of(out, c.dtype, rows, out_row, heads, out_head, c.head_dim),
+                 sums = array_of(lse, rows * heads, 4);
+    if (rows_same(to, in) ? rows_meet(sums, in) : rows_meet(to, in) || rows_meet(sums, in))
+        return fail(CHRONOS_ERR_INVALID_ARG, "%s: out may be q, with the same strides; results overlap no other input", what);
+    return check_apart(what, c, packed, {to, sums}, {list, cu});
+}
 
 // Pages of 4-bit values.
 inline int check_packed(const ChronosPagedCache& c, float k_scale, float v_scale, const char* what) {

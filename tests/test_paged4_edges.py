@@ -250,3 +250,91 @@ def test_decode4_windows_over_long_rows(lib, dt, h, g, d, lens, window, sinks): 
     assert torch.equal(out, ops.paged_attn_decode4(q, kp, vp, table, ln, window=window, sinks=sinks))
     over = q.clone()
     assert ops.paged_attn_decode4(over, kp, vp, table, ln, window=window, sinks=sinks, out=over) is over and torch.equal(over, out)
+
+
+# ---------------------------------------------------------------------------------------
+# results that overlap what a call reads
+# ---------------------------------------------------------------------------------------
+
+KP, VP, TABLE, LENS, Q, OUT, LSE, CU, LIST, BOUNDS = (i << 20 for i in range(1, 11))
+
+
+def _full_cache(N, **kw):
+    """2 sequences of 2 heads of 16 columns in 4 pages of 16 slots; 4-bit pages of 16 * 36 bytes a head."""
+    return _native_cache(N, **{**dict(k_pages=KP, v_pages=VP, k_page_stride=1152, k_slot_stride=32, k_head_stride=576, v_page_stride=1152,
+                                      v_slot_stride=32, v_head_stride=576, page_table=TABLE, page_table_stride=2, lens=LENS), **kw})
+
+
+@pytest.mark.parametrize("change", [
+    dict(out=Q + 64), dict(out=Q, out_row_stride=128), dict(out=KP + 4 * 1152 - 16), dict(out=VP), dict(out=LENS - 64), dict(out=TABLE), dict(lse=OUT),
+    dict(lse=Q + 4), dict(lse=LENS + 4), dict(lse=KP), dict(q=OUT + 254)])
+def test_attention_results_that_overlap_are_refused(lib, change):  # noqa: F811
+    from project_chronos_b200 import _native as N
+    f = dict(heads=4, scale=0.25, k_scale=1.0, v_scale=1.0, q=Q, q_row_stride=64, q_head_stride=16, out=OUT, out_row_stride=64, out_head_stride=16, lse=LSE)
+    _refuses(lib, "decode4", N.ChronosPagedDecode4Args(cache=_full_cache(N), **{**f, **change}), b"overlap")
+    f.update(num_tokens=2, topk=2, pages=LIST, packed=1)
+    _refuses(lib, "sparse", N.ChronosPagedSparseArgs(cache=_full_cache(N), **{**f, **change}), b"overlap")
+
+
+@pytest.mark.parametrize("change", [dict(out=LIST), dict(lse=LIST + 12), dict(out=CU - 250), dict(lse=CU + 8)])
+def test_sparse_results_over_lists_and_offsets_are_refused(lib, change):  # noqa: F811
+    from project_chronos_b200 import _native as N
+    f = dict(heads=4, scale=0.25, k_scale=1.0, v_scale=1.0, q=Q, q_row_stride=64, q_head_stride=16, out=OUT, out_row_stride=64, out_head_stride=16, lse=LSE,
+             num_tokens=2, topk=2, pages=LIST, cu_seqlens=CU)
+    _refuses(lib, "sparse", N.ChronosPagedSparseArgs(cache=_full_cache(N), **{**f, **change}), b"overlap")
+
+
+@pytest.mark.parametrize("pages", [TABLE, LENS + 4, Q, BOUNDS + 256, CU])
+def test_selections_that_overlap_are_refused(lib, pages):  # noqa: F811
+    from project_chronos_b200 import _native as N
+    f = dict(heads=4, topk=3, last=1, num_tokens=2, q=Q, q_row_stride=64, q_head_stride=16, bounds=BOUNDS, cu_seqlens=CU, pages=pages)
+    _refuses(lib, "select", N.ChronosPagedSelectArgs(cache=_full_cache(N), **f), b"overlap")
+
+
+@pytest.mark.parametrize("bounds", [TABLE - 500, LENS, KP, KP + 3 * 1152 * 2, CU])
+def test_bounds_that_overlap_are_refused(lib, bounds):  # noqa: F811
+    from project_chronos_b200 import _native as N
+    _refuses(lib, "bounds", N.ChronosPagedBoundsArgs(cache=_full_cache(N), num_tokens=2, bounds=bounds, cu_seqlens=CU), b"overlap")
+
+
+@pytest.mark.parametrize("change", [
+    dict(q_out=KP), dict(q_out=VP + 4 * 1152 - 32), dict(k_out=KP + 1152), dict(k_out=TABLE), dict(q_out=LENS), dict(q_out=11 << 20), dict(k_out=12 << 20),
+    dict(lens_out=CU), dict(lens_out=TABLE), dict(seen_out=TABLE + 8), dict(seen_out=OUT), dict(q_out=13 << 20)])
+def test_append_results_that_overlap_are_refused(lib, change):  # noqa: F811
+    from project_chronos_b200 import _native as N
+    rows = {f"{x}_{y}_stride": s for x in ("k", "v", "q", "q_out", "k_out") for y, s in (("row", 64), ("head", 16))}
+    f = dict(num_tokens=2, heads=4, rope_dim=4, table_len=10, k=14 << 20, v=15 << 20, q=Q, q_out=OUT, cos=11 << 20, sin=12 << 20, cos_row_stride=4,
+             sin_row_stride=4, cu_seqlens=CU, seen=13 << 20, packed=1, k_scale=1.0, v_scale=1.0, **rows)
+    _refuses(lib, "append_rope", N.ChronosPagedRopeArgs(cache=_full_cache(N), **{**f, **change}), b"overlap")
+
+
+@gpu
+@pytest.mark.parametrize("four", [False, True])
+def test_results_beside_their_inputs_are_taken(four):
+    """In q itself, in other columns of q's array, and with one row in q's place with another stride."""
+    from project_chronos_b200 import ops
+    h, g, d, size = 4, 2, 64, 16
+    kp, vp, table, ln, _ = _cache4([100, 50], g, d, size, 3)
+    if not four:
+        kp, vp = (torch.randn(kp.shape[0], size, g, d, device="cuda").to(BF) for _ in range(2))
+    pages = torch.arange(3, dtype=torch.int32, device="cuda").expand(2, g, 3).contiguous()
+    both = _rnd(4, 2, 2 * h, d, dt=BF)
+    q = both[:, :h]
+    calls = [lambda q, n=2, **kw: ops.paged_attn_sparse(q, kp, vp, table[:n], ln[:n], pages[:n], **kw)]
+    if four:
+        calls.append(lambda q, n=2, **kw: ops.paged_attn_decode4(q, kp, vp, table[:n], ln[:n], **kw))
+    for call in calls:
+        want = call(q)
+        ops.check_status(want.device)
+        assert torch.equal(call(q, out=both[:, h:]), want) and torch.equal(both[:, h:], want)
+        over = both.clone()
+        assert torch.equal(call(over[:, :h], out=over[:, :h]), want)
+        one = q[:1].clone()
+        assert torch.equal(call(one, 1, out=one.as_strided((1, h, d), (7 * d, d, 1))), want[:1])
+        with pytest.raises(RuntimeError, match="overlap"):
+            call(both[:, :h], out=both[:, 1: h + 1])
+        with pytest.raises(RuntimeError, match="overlap"):
+            call(q, lse=kp.view(-1).view(torch.float32)[: 2 * h].view(2, h))
+    bounds = torch.zeros(kp.shape[0], 2, g, d, dtype=BF, device="cuda")
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.paged_select(q, bounds, table, ln, size, 2, out=table.view(-1)[: 2 * g * 2].view(2, g, 2))
