@@ -23,6 +23,7 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 LIB = os.path.join(PKG, "libchronos_moe.so")
 BINDING = os.path.join(PKG, "_binding.so")
+BINDING_STAMP = BINDING + ".txt"   # what it was built against
 OBJ = os.path.join(PKG, "_build")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -53,8 +54,22 @@ def _binding_sources():
     return [os.path.join(CSRC, "binding.cpp")] + sorted(glob.glob(os.path.join(INCLUDE, "*.h")))
 
 
+def binding_target() -> str:
+    """What _binding.so has to fit: the interfaces of this Python and of this torch."""
+    import torch
+    return f"{sysconfig.get_config_var('SOABI')} torch {torch.__version__} abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+
+
+def binding_fits(unknown: bool) -> bool:
+    """Whether _binding.so was built against what runs now; `unknown` where nothing says so."""
+    if not os.path.exists(BINDING_STAMP):
+        return unknown
+    with open(BINDING_STAMP) as f:
+        return f.read() == binding_target()
+
+
 def needs_binding() -> bool:
-    if not os.path.exists(BINDING):
+    if not os.path.exists(BINDING) or not binding_fits(unknown=False):
         return True
     t = os.path.getmtime(BINDING)
     return any(os.path.getmtime(f) > t for f in _binding_sources())
@@ -91,7 +106,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if verbose:
             print(" ".join(cmd))
         subprocess.check_call(cmd)
+        if os.path.exists(BINDING_STAMP):
+            os.remove(BINDING_STAMP)
         os.replace(BINDING + ".tmp", BINDING)
+        with open(BINDING_STAMP, "w") as f:
+            f.write(binding_target())
     return LIB
 
 

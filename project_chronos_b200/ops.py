@@ -853,6 +853,10 @@ def _calls():
     global _native_calls
     if _native_calls is None:
         N.load_library()
+        from . import build
+        if not build.binding_fits(unknown=True):
+            raise RuntimeError("the native module of the paged calls was built against another Python or torch; build it with "
+                               "`python -m project_chronos_b200.build`")
         try:
             from . import _binding
         except ImportError as e:

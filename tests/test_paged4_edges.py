@@ -338,3 +338,29 @@ def test_results_beside_their_inputs_are_taken(four):
     bounds = torch.zeros(kp.shape[0], 2, g, d, dtype=BF, device="cuda")
     with pytest.raises(RuntimeError, match="overlap"):
         ops.paged_select(q, bounds, table, ln, size, 2, out=table.view(-1)[: 2 * g * 2].view(2, g, 2))
+
+
+# ---------------------------------------------------------------------------------------
+# the native module
+# ---------------------------------------------------------------------------------------
+
+def test_a_native_module_of_another_torch_or_python_is_built_again_and_not_loaded(lib, monkeypatch):  # noqa: F811
+    from project_chronos_b200 import build, ops
+    assert build.binding_fits(False) and not build.needs_binding()
+    monkeypatch.setattr(ops, "_native_calls", None)
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    assert not build.binding_fits(False) and build.needs_binding()
+    with pytest.raises(RuntimeError, match="another Python or torch"):
+        ops.paged_gather(*[torch.zeros(1)] * 7)
+    monkeypatch.undo()
+    monkeypatch.setattr(ops, "_native_calls", None)
+    monkeypatch.setattr(build.sysconfig, "get_config_var", lambda name: "cpython-399")
+    assert build.needs_binding()
+    monkeypatch.undo()
+    assert build.binding_fits(False)
+
+
+def test_a_native_module_without_a_record_is_built_again(lib, monkeypatch, tmp_path):  # noqa: F811
+    from project_chronos_b200 import build
+    monkeypatch.setattr(build, "BINDING_STAMP", str(tmp_path / "none"))
+    assert build.needs_binding() and build.binding_fits(True)
