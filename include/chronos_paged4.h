@@ -49,8 +49,8 @@ extern "C" {
  * seen_out as in chronos_paged_append; a token whose position lies outside the
  * tables is dropped like one without a page (and its rows of q_out and k_out are
  * zeros; those of a token that only lacks a page are rotated all the same).  Rows
- * behind the last sequence are neither read nor written.  q_out may be q and k_out may
- * be k (with the same strides). */
+ * behind the last sequence are not written; they may be read, and what they hold does
+ * not matter.  q_out may be q and k_out may be k (with the same strides). */
 typedef struct ChronosPagedRopeArgs {
     ChronosPagedCache cache;   /* lens: before the append */
     int32_t packed;            /* 1: pages of 4-bit values */
