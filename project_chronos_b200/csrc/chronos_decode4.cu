@@ -86,8 +86,8 @@ int launch_decode4(const PagedDecodeParams& p, const Decode4Plan& d, cudaStream_
     auto kernel = paged_decode4_kernel<T, DP, NT, kP4ListTiles, false, false>;
     if (int rc = set_smem(kernel, S::kSmem)) return rc;
     CHRONOS_CUDA_CHECK(launch_kernel(kernel, dim3(p.grid), dim3(kPdThreads), S::kSmem, st, false, p));
-    if (p.join_blocks > 0)   // rows of one unit are never cut: then there is nothing to join
-        CHRONOS_CUDA_CHECK(launch_kernel(paged_join_kernel<T, kP4ListTiles * kPdBlock>, dim3(static_cast<unsigned>(p.join_blocks)), dim3(kPdJoinThreads), 0, st, true, p));
+    // (the list begins at 25 blocks of 64 slots a row: its rows are cut)
+    CHRONOS_CUDA_CHECK(launch_kernel(paged_join_kernel<T, kP4ListTiles * kPdBlock>, dim3(static_cast<unsigned>(p.join_blocks)), dim3(kPdJoinThreads), 0, st, true, p));
     return CHRONOS_OK;
 }
 template <typename T>
@@ -152,7 +152,7 @@ extern "C" int chronos_paged_decode4(const ChronosPagedDecode4Args* a, void* str
     p.part_stride = d.dp;
     p.part_o = reinterpret_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float*>(ws + d.o_part_ml);
-    p.join_blocks = d.max_vis > kP4ListTiles * kPdBlock ? a->cache.batch * a->heads : 0;
+    p.join_blocks = a->cache.batch * a->heads;
     p.status = a->status;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (a->cache.dtype) {
