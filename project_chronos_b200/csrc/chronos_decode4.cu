@@ -86,7 +86,7 @@ int launch_decode4(const PagedDecodeParams& p, const Decode4Plan& d, cudaStream_
     auto kernel = paged_decode4_kernel<T, DP, NT, kP4ListTiles, false, false>;
     if (int rc = set_smem(kernel, S::kSmem)) return rc;
     CHRONOS_CUDA_CHECK(launch_kernel(kernel, dim3(p.grid), dim3(kPdThreads), S::kSmem, st, false, p));
-    // (the list begins at 25 blocks of 64 slots a row: its rows are cut)
+    // (the list begins at 25 blocks of 64 slots a row: there are rows that may be cut)
     CHRONOS_CUDA_CHECK(launch_kernel(paged_join_kernel<T, kP4ListTiles * kPdBlock>, dim3(static_cast<unsigned>(p.join_blocks)), dim3(kPdJoinThreads), 0, st, true, p));
     return CHRONOS_OK;
 }

@@ -385,6 +385,12 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+// ... and back.
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t x) {
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&x));
+    else return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
 // 16 bytes global -> shared, zeros instead where !valid (src is not read then).
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
     const int n = valid ? 16 : 0;
@@ -496,10 +502,11 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<T, DP>::kBlocksPerSm) pag
     constexpr int RB = S::kRowBytes;
     constexpr int RPI = 32 / CPR;          // rows a warp copies per instruction
     constexpr float kGrow = 8.0f, kLift = WeightLift<T>::value;
-    // bf16 weights of selected pages go through the product with what their rounding leaves: a few
-    // hundred slots do not average 2^-9 each away (8 heads of 2048 slots: 0.0032 off, 0.0016 so, the
-    // result's own rounding), and the copies bound these calls.
-    constexpr bool TWO = SEL && std::is_same<T, __nv_bfloat16>::value;
+    // Weights of selected pages go through the product with what their rounding leaves: a few
+    // hundred slots do not average it away (bf16, 8 heads of 2048 slots: 0.0032 off, 0.0016 so, the
+    // result's own rounding; fp16 drafts 2.8e-4 and 2.1e-4), and the copies bound these calls (drafts 72 and 74 us
+    // with their selection).
+    constexpr bool TWO = SEL && sizeof(T) == 2;
     extern __shared__ __align__(128) uint8_t smem[];
     float* s_o = reinterpret_cast<float*>(smem + NS * S::kStageBytes);         // [warp][8 heads][kOStride]
     float* s_ml = s_o + S::kMergeBytes / 4;                                    // [warp][8][2]
@@ -770,8 +777,9 @@ __global__ void __launch_bounds__(kPdThreads, PagedMma<T, DP>::kBlocksPerSm) pag
                 pb[t][0] = transpose8x8(ab);
                 pb[t][1] = transpose8x8(cd);
                 if constexpr (TWO) {
-                    rest[t][0] = transpose8x8(pack2<T>(a - __uint_as_float(ab << 16), b - __uint_as_float(ab & 0xffff0000u)));
-                    rest[t][1] = transpose8x8(pack2<T>(c - __uint_as_float(cd << 16), d - __uint_as_float(cd & 0xffff0000u)));
+                    const float2 x = unpack2<T>(ab), y = unpack2<T>(cd);
+                    rest[t][0] = transpose8x8(pack2<T>(a - x.x, b - x.y));
+                    rest[t][1] = transpose8x8(pack2<T>(c - y.x, d - y.y));
                 }
             }
 #pragma unroll

@@ -28,7 +28,7 @@ struct Paged4 {
     static constexpr int kOStride = DP + 4;
     static constexpr int kMergeBytes = kPdWarps * 8 * kOStride * 4;
     static constexpr int kSmem = kStages * kStageBytes + kMergeBytes + kPdWarps * 16 * 4;
-    static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;      // halves that a query or weight is split into
+    static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;      // halves that a query is split into
     // four blocks of 128 registers measured 2 to 7 % slower than three for heads of 128
     static constexpr int kBlocksPerSm = DP == 256 || (DP == 128 && NT * kTerms > 2) ? 2 : DP == 128 ? 3 : 4;
     static constexpr int kPartBytes = (16 * DP + 32) * 4;      // what a cluster's block leaves for the join
@@ -99,6 +99,12 @@ __global__ void __launch_bounds__(kPdThreads, Paged4<T, DP, NT>::kBlocksPerSm) p
     constexpr int NS = S::kStages, RB = S::kSlotBytes, REC = S::kRecord, TERMS = S::kTerms, BLOCK = TILES * kPdBlock;
     constexpr int KW = DP / 32, VW = DP / 64;                        // words of 8 codes per slot and lane
     constexpr float kGrow = 8.0f, kLift = 7.0f;                      // see WeightLift
+    // Halves that a weight is split into; the sum of weights is fp32 whatever it is.  One is off by up to
+    // 2^-11, an eighth of what a bf16 result's own rounding is, and as much as an fp16 result's: 4 fp16 rows of
+    // 100003 to 131072 slots are 2.4e-4 off with one and 2.1e-4 with two (fp32 weights: 2.1e-4), in
+    // 140 and 160 us, so whole sequences of fp16 layers take one.  Selected pages, few slots whose
+    // look-ups bound the call, take two; so do fp32 layers (22 bits).
+    constexpr int WT = TERMS == 2 || (SEL && std::is_same<T, __half>::value) ? 2 : 1;
     static_assert(!SEL || CL, "selected pages: a cluster per row");
     extern __shared__ __align__(128) uint8_t smem[];
     float* s_o = reinterpret_cast<float*>(smem + NS * S::kStageBytes);   // [warp][8 heads][kOStride]
@@ -362,18 +368,18 @@ __global__ void __launch_bounds__(kPdThreads, Paged4<T, DP, NT>::kBlocksPerSm) p
                     }
                 }
         }
-        uint32_t pb[NT][2][TERMS];
+        uint32_t pb[NT][2][WT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const float a = exp2_fast(x[t][0]), b = exp2_fast(x[t][1]), c = exp2_fast(x[t][2]), d = exp2_fast(x[t][3]);
             l[t][0] += a + c;
             l[t][1] += b + d;
             // weights in halves for the second product; the sum keeps fp32
-            uint32_t y[TERMS], z[TERMS];
-            paged4_halves<TERMS>(a, b, y);
-            paged4_halves<TERMS>(c, d, z);
+            uint32_t y[WT], z[WT];
+            paged4_halves<WT>(a, b, y);
+            paged4_halves<WT>(c, d, z);
 #pragma unroll
-            for (int e = 0; e < TERMS; ++e) {
+            for (int e = 0; e < WT; ++e) {
                 pb[t][0][e] = transpose8x8(y[e]);
                 pb[t][1][e] = transpose8x8(z[e]);
             }
@@ -411,7 +417,7 @@ __global__ void __launch_bounds__(kPdThreads, Paged4<T, DP, NT>::kBlocksPerSm) p
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int e = TERMS - 1; e >= 0; --e) mma_16816<__half>(o[t][4 * i + j], a, pb[t][0][e], pb[t][1][e]);
+                    for (int e = WT - 1; e >= 0; --e) mma_16816<__half>(o[t][4 * i + j], a, pb[t][0][e], pb[t][1][e]);
             }
         }
     };

@@ -10,7 +10,7 @@ import math
 import pytest
 import torch
 
-from test_paged4 import (BF, FP, HF, _cache4, _check_attention, _i32, _native_cache, _page_table, _quantise, _refuses, _rnd, _rotate,
+from test_paged4 import (BF, FP, HF, _attend, _cache4, _check_attention, _i32, _native_cache, _page_table, _quantise, _refuses, _rnd, _rotate,
                          _stored, _visible, gpu, lib)  # noqa: F401
 
 
@@ -364,3 +364,36 @@ def test_a_native_module_without_a_record_is_built_again(lib, monkeypatch, tmp_p
     from project_chronos_b200 import build
     monkeypatch.setattr(build, "BINDING_STAMP", str(tmp_path / "none"))
     assert build.needs_binding() and build.binding_fits(True)
+
+
+# ---------------------------------------------------------------------------------------
+# weights of selected pages
+# ---------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("h, d", [(8, 128), (24, 64), (8, 256)])
+def test_fp16_weights_of_selected_pages_keep_more_than_a_half(four, h, d):
+    """Two slots with values 6 and -6 and nearly equal scores: what is left is the difference of two weights.  Each is off
+    by 2^-22 in two halves (2^-11 in one), the rest is the fp32 part of test_paged4's tolerance."""
+    from project_chronos_b200 import ops
+    g, size, dt = 2, 16, HF
+    k = torch.zeros(2, g, d, dtype=dt, device="cuda")
+    k[:, :, 1], k[0, :, 0] = 6.0, 1.0                      # 4 bits hold them
+    v = torch.full_like(k, 6.0)
+    v[1] = -6.0
+    table = _i32(0).view(1, 1)
+    if four:
+        kp, vp = (torch.zeros(1, g, ops.packed_page_bytes(size, d), dtype=torch.uint8, device="cuda") for _ in range(2))
+    else:
+        kp, vp = (torch.zeros(1, size, g, d, dtype=dt, device="cuda") for _ in range(2))
+    ops.paged_append_rope(k, v, kp, vp, table, _i32(0), cu_seqlens=_i32(0, 2))
+    q = torch.zeros(1, h, d, dtype=dt, device="cuda")
+    q[0, :, 0] = torch.linspace(1e-4, 1e-2, h, device="cuda")
+    out = ops.paged_attn_sparse(q, kp, vp, table, _i32(2), torch.zeros(1, g, 1, dtype=torch.int32, device="cuda"), scale=1.0)[0].double()
+    ops.check_status(kp.device)
+    ref, _, a, s, s2 = _attend(q[0], k, v, 1.0)
+    f = d * 2.0 ** -23 * s + 2 * 2.0 ** -24 + 2.0 ** -20 + (2.0 ** -28 * s2 if four else 0.0)
+    tol = torch.finfo(dt).eps / 2 * ref.abs() + (f[:, None] + 2 * 2.0 ** -23 + 2.0 ** -21) * a + 2.0 ** -25
+    err = (out - ref).abs()
+    assert bool((err <= tol).all()), f"off by {float((err / tol).max()):.2f} of the tolerance"
