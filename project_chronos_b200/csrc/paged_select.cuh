@@ -9,7 +9,7 @@
 // sum in 32 bits would mix up keep the order that their exact scores have.  That holds for
 // finite bounds and queries: where an infinity meets up or down = 0 (no query of that sign) the
 // product is NaN and the maximum need not be.  Any bound or query that is not finite makes the
-// sum not finite, so those few pages are found by their scores and done again head by head.
+// sum infinite or NaN, so those few pages are found by their scores and done again head by head.
 #pragma once
 
 #include "chronos_paged4.h"
@@ -196,15 +196,54 @@ struct SelectShared {
     int scan[kSelectWarps];
     unsigned long long ends[2][kSelectWarps];
     int digit, above, same;
-    int odd;   // a score of the block's pages is not finite
 };
+
+// The scores of a token's pages [lo, hi) that are infinite or NaN, again from the formula as it stands: NaN where
+// a product or a maximum is.  (Only they can be wrong: a sum of minus infinity is an infinite query's, below
+// bounds that are finite.)  What is finite is summed as paged_select_kernel sums it, so that equal
+// scores stay equal.  Whole blocks call it; 8 lanes take a page.  Rare: one column at a time, in few registers.
+template <typename T>
+__device__ __forceinline__ void select_again(const PagedSelectParams& p, unsigned long long* keys, int64_t token, int g, int seq, int lo, int hi) {
+    const uint32_t lanes = 0xffu << (threadIdx.x & 24);
+    const T* q = static_cast<const T*>(p.q) + token * p.q_row + static_cast<int64_t>(g) * p.rep * p.q_head;
+    const int G = p.c.kv_heads, D = p.c.head_dim;
+#pragma unroll 1
+    for (int j = lo + (threadIdx.x >> 3); j < hi; j += kSelectThreads / 8) {
+        if (keys[j] < select_key(INFINITY)) continue;
+        const T* bounds = static_cast<const T*>(p.bounds) + (static_cast<int64_t>(p.c.page_table[seq * p.c.page_table_stride + j]) * 2 * G + g) * D;
+        double x = 0.0, odd = 0.0;
+#pragma unroll 1
+        for (int i = 0; i < 16 * ((D + 63) / 64); ++i) {   // 8 columns' lower, then their upper bounds
+            const bool upper = (i & 8) != 0;
+            const int d = (i >> 4) * 64 + (threadIdx.x & 7) * 8 + (i & 7);
+            if (d >= D) continue;
+            const float low = to_f32<T>(bounds[d]), high = to_f32<T>(bounds[static_cast<int64_t>(G) * D + d]);
+            double sum = 0.0, side = 0.0;   // of the column's maxima, of its queries on this side
+#pragma unroll 1
+            for (int h = 0; h < p.rep; ++h) {
+                const float v = to_f32<T>(q[h * p.q_head + d]);
+                const double a = static_cast<double>(v) * low, b = static_cast<double>(v) * high;
+                sum += a != a || a > b ? a : b;   // NaN where one is
+                if ((v > 0.0f) == upper) side += v;
+            }
+            const float bound = upper ? high : low;
+            if (!(fabs(sum) < INFINITY)) odd += upper ? 0.0 : sum;
+            else if (fabsf(bound) < INFINITY) x = fma(side, static_cast<double>(bound), x);   // (an infinity is on the side that no query takes)
+        }
+        x += odd;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) x += __shfl_xor_sync(lanes, x, o);
+        if ((threadIdx.x & 7) == 0) keys[j] = select_key(x);
+    }
+}
 
 // The pages of one token and kv head, by a block.  Of the pages that are not always in, the
 // `want`-th largest key by radix selection, 11 bits at a time of what the keys are above the
 // smallest one (scores lie in a few binades: their upper bits alone would tell nothing), then the
 // pages above it and the first of those equal to it, in their order.  n: the token's pages.
-__device__ __forceinline__ void select_row(const PagedSelectParams& p, SelectShared& s, unsigned long long* held, const unsigned long long* mine,
-                                           int32_t* out, int n) {
+template <typename T>
+__device__ __forceinline__ void select_row(const PagedSelectParams& p, SelectShared& s, unsigned long long* held, unsigned long long* mine,
+                                           int32_t* out, int n, int64_t token, int g, int seq) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (n <= p.topk) {
         for (int i = threadIdx.x; i < p.topk; i += kSelectThreads) out[i] = i < n ? i : -1;
@@ -215,28 +254,35 @@ __device__ __forceinline__ void select_row(const PagedSelectParams& p, SelectSha
     int want = p.topk - p.first - p.last;
     const bool fits = n <= kSelectKeys;
     for (int i = threadIdx.x; i < kSelectBins; i += kSelectThreads) s.hist[i] = 0;
-    unsigned long long low = ~0ull, high = 0ull;
+    unsigned long long low, high;
+    for (bool again = false;; again = true) {
+        low = ~0ull;
+        high = 0ull;
 #pragma unroll 4
-    for (int j = lo + threadIdx.x; j < hi; j += kSelectThreads) {
-        const unsigned long long k = mine[j];
-        if (fits) held[j] = k;
-        low = min(low, k);
-        high = max(high, k);
-    }
+        for (int j = lo + threadIdx.x; j < hi; j += kSelectThreads) {
+            const unsigned long long k = mine[j];
+            if (fits) held[j] = k;
+            low = min(low, k);
+            high = max(high, k);
+        }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
-        high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
-    }
-    if (lane == 0) {
-        s.ends[0][warp] = low;
-        s.ends[1][warp] = high;
-    }
-    __syncthreads();
+        for (int o = 16; o > 0; o >>= 1) {
+            low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+            high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
+        }
+        if (lane == 0) {
+            s.ends[0][warp] = low;
+            s.ends[1][warp] = high;
+        }
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kSelectWarps; ++w) {
-        low = min(low, s.ends[0][w]);
-        high = max(high, s.ends[1][w]);
+        for (int w = 0; w < kSelectWarps; ++w) {
+            low = min(low, s.ends[0][w]);
+            high = max(high, s.ends[1][w]);
+        }
+        if (again || high < select_key(INFINITY)) break;
+        select_again<T>(p, mine, token, g, seq, lo, hi);
+        __syncthreads();
     }
     auto key = [&](int j) { return (fits ? held[j] : mine[j]) - low; };
     // what the keys are above the smallest has `top` bits
@@ -299,76 +345,6 @@ __device__ __forceinline__ void select_row(const PagedSelectParams& p, SelectSha
     }
 }
 
-// A lane's part of a page's score (8 lanes a page) from the formula as it stands, NaN where a
-// product or a maximum is: columns that are finite are summed as paged_select_kernel sums them, so
-// that equal scores stay equal.
-template <typename T>
-__device__ double select_literal(const PagedSelectParams& p, int64_t token, int g, int page, int part) {
-    const int G = p.c.kv_heads, D = p.c.head_dim;
-    const T* lo_row = static_cast<const T*>(p.bounds) + (static_cast<int64_t>(page) * 2 * G + g) * D;
-    const T* hi_row = lo_row + static_cast<int64_t>(G) * D;
-    double acc = 0.0, odd = 0.0;
-    for (int d0 = part * 8; d0 < D; d0 += 64) {
-        double q[2][8], x[2][8];   // down and up, lo and hi
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            q[0][e] = q[1][e] = x[0][e] = x[1][e] = 0.0;
-            const int d = d0 + e;
-            if (d >= D) continue;
-            const T* head = static_cast<const T*>(p.q) + token * p.q_row + static_cast<int64_t>(g) * p.rep * p.q_head + d;
-            const double lo = to_f32<T>(lo_row[d]), hi = to_f32<T>(hi_row[d]);
-            double sum = 0.0;
-            for (int h = 0; h < p.rep; ++h) {
-                const double v = to_f32<T>(head[h * p.q_head]), a = v * lo, b = v * hi;
-                sum += a != a || a > b ? a : b;   // NaN where one is
-                if (v > 0.0) q[1][e] += v;
-                else q[0][e] += v;
-            }
-            x[0][e] = lo;
-            x[1][e] = hi;
-            if (!(fabs(sum) < INFINITY)) {
-                odd += sum;
-                x[0][e] = x[1][e] = q[0][e] = q[1][e] = 0.0;
-            } else {   // an infinity here is on the side that no query takes
-                if (!(fabs(lo) < INFINITY)) x[0][e] = 0.0;
-                if (!(fabs(hi) < INFINITY)) x[1][e] = 0.0;
-            }
-        }
-#pragma unroll
-        for (int w = 0; w < 2; ++w)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc = fma(q[w][e], x[w][e], acc);
-    }
-    return acc + odd;
-}
-
-// The scores of this block's pages that are not finite, again.  Whole blocks call it; 8 lanes take
-// a page as before.
-template <typename T, int ROUND, int TOKENS>
-__device__ __noinline__ void select_again(const PagedSelectParams& p, unsigned long long* keys, int seq, int64_t t0, int n, int g, int rank, int len) {
-    constexpr int GROUPS = kSelectThreads / 8;
-    const int part = threadIdx.x & 7, group = threadIdx.x >> 3;
-    const uint32_t lanes = 0xffu << (threadIdx.x & 24);
-    const unsigned long long inf = select_key(INFINITY), minus = select_key(-INFINITY);
-    const int most = (len + p.c.page_size - 1) / p.c.page_size;
-    for (int64_t j0 = static_cast<int64_t>(rank) * ROUND; j0 < most; j0 += static_cast<int64_t>(p.cluster) * ROUND)
-        for (int64_t j = j0 + group; j < min(j0 + ROUND, static_cast<int64_t>(most)); j += GROUPS) {
-            const int page = p.c.page_table[seq * p.c.page_table_stride + j];
-            if (page < 0 || page >= p.c.num_pages) continue;
-            for (int t = 0; t < n; ++t) {
-                if (j * p.c.page_size >= max(len - (TOKENS == 1 ? 0 : n - 1 - t), 0)) continue;   // behind the token
-                unsigned long long* key = keys + static_cast<int64_t>(t) * p.c.kv_heads * p.width + j;
-                unsigned long long k = part == 0 ? *key : 0ull;
-                k = __shfl_sync(lanes, k, 0, 8);
-                if (k < inf && k > minus) continue;
-                double x = select_literal<T>(p, t0 + t, g, page, part);
-#pragma unroll
-                for (int o = 1; o < 8; o <<= 1) x += __shfl_xor_sync(lanes, x, o);
-                if (part == 0) *key = select_key(x);
-            }
-        }
-}
-
 // Bound by reading the bounds.  A cluster of p.cluster blocks per TOKENS tokens of a sequence (1
 // where every sequence has one) and kv head.  Scores: the blocks share the pages, 8 lanes a
 // page, two pages at a time (16-bit types), whose loads all go out before the first is used; each
@@ -429,9 +405,7 @@ __global__ void __launch_bounds__(kSelectThreads, TOKENS == 1 ? 3 : 2) paged_sel
     const int most = (len + p.c.page_size - 1) / p.c.page_size;
     unsigned long long* keys = p.keys + ((t0 - p.token0) * G + g) * p.width;   // of token t: t * G * width on
     auto pages_of = [&](int t) { return TOKENS == 1 ? most : (max(len - (n - 1 - t), 0) + p.c.page_size - 1) / p.c.page_size; };
-    bool again = false;
     if (most > p.topk) {   // (else all pages are taken: no scores)
-        if (threadIdx.x == 0) s_sel.odd = 0;
         const int D64 = (D + 63) & ~63;
         for (int i = threadIdx.x; i < n * D64; i += kSelectThreads) {
             const int t = i / D64, d = i % D64;
@@ -526,23 +500,17 @@ __global__ void __launch_bounds__(kSelectThreads, TOKENS == 1 ? 3 : 2) paged_sel
 #pragma unroll
                         for (int o = 1; o < 8; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
                         const int j = j0 + k * GROUPS;
-                        if (part == 0 && j < pages) {
-                            keys[t * G * p.width + j] = page[k] < 0 ? 0ull : select_key(x);
-                            if (!(fabs(x) < INFINITY)) s_sel.odd = 1;
-                        }
+                        if (part == 0 && j < pages) keys[t * G * p.width + j] = page[k] < 0 ? 0ull : select_key(x);
                     }
                 }
             }
         }
-        __syncthreads();
-        again = s_sel.odd != 0;
-        if (again) select_again<T, ROUND, TOKENS>(p, keys, seq, t0, n, g, rank, len);
     }
     // every block's keys are written (they are read from global memory, by blocks of this cluster only)
     if (C > 1) cooperative_groups::this_cluster().sync();
-    else if (again) __syncthreads();
+    else __syncthreads();
     for (int t = rank; t < n; t += C) {
-        select_row(p, s_sel, s_keys, keys + t * G * p.width, p.pages + ((t0 + t) * G + g) * p.topk, pages_of(t));
+        select_row<T>(p, s_sel, s_keys, keys + t * G * p.width, p.pages + ((t0 + t) * G + g) * p.topk, pages_of(t), t0 + t, g, seq);
         __syncthreads();   // the next one writes where this one reads
     }
 }
