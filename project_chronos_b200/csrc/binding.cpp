@@ -10,12 +10,14 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/DynamicTypes.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <array>
 #include <cstdarg>
+#include <cmath>
 #include <cstdint>
-#include <optional>
+#include <exception>
 #include <string>
 
 #include "chronos_paged4.h"
@@ -527,10 +529,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
     try {
         return F(args);
     } catch (const Raised&) {
-    } catch (const c10::Error& e) {
-        if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
-    } catch (const std::exception& e) {
-        if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {   // as torch's own calls raise it: torch.OutOfMemoryError among them
+        if (!PyErr_Occurred()) torch::translate_exception_to_python(std::current_exception());
     }
     return nullptr;
 }

@@ -397,3 +397,15 @@ def test_fp16_weights_of_selected_pages_keep_more_than_a_half(four, h, d):
     tol = torch.finfo(dt).eps / 2 * ref.abs() + (f[:, None] + 2 * 2.0 ** -23 + 2.0 ** -21) * a + 2.0 ** -25
     err = (out - ref).abs()
     assert bool((err <= tol).all()), f"off by {float((err / tol).max()):.2f} of the tolerance"
+
+
+@gpu
+def test_results_that_no_memory_holds_raise_as_torch_does():
+    """A selection of 2^31 - 1 pages for 64 heads: 550 GB."""
+    from project_chronos_b200 import ops
+    q, bounds = _rnd(1, 4, 16, 64, dt=BF), torch.zeros(4, 2, 16, 64, dtype=BF, device="cuda")
+    table, ln = torch.zeros(4, 1, dtype=torch.int32, device="cuda"), _i32(1, 1, 1, 1)
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.paged_select(q, bounds, table, ln, 16, 2 ** 31 - 1)
+    assert ops.paged_select(q, bounds, table, ln, 16, 2).shape == (4, 16, 2)
+    ops.check_status(q.device)
