@@ -88,10 +88,10 @@ __device__ __forceinline__ uint32_t kept(uint32_t x) {
 // look up the pages of a unit's tiles at once, a unit ahead.
 //
 // Measured, 32 / 8 heads of 128: 4 rows of 100003 to 131072 slots in fp16 138 us, 4.1 TB/s of 4-bit
-// records (the 16-bit cache: 291 to 310 us); 32 ragged rows up to 8192 slots 57 us.  Bound by
-// instructions: 348 per tile, of which 64 conversions, 96 scale products and 16 tensor products are
-// the format's; the heavy FMA pipe and the ALU take two cycles each for theirs, 60 % of issue slots
-// are used.  16 slots per look-up and unit: 206 us.
+// records (the 16-bit cache: 291 to 310 us); 32 ragged rows up to 8192 slots 58 us.  348 instructions per
+// tile, of which 64 conversions, 96 scale products and 16 tensor products are the format's.  No unit
+// is full (60 % of issue slots, ALU 43 %, FMA 39 %): a scheduler's three warps each follow one chain of
+// dependent steps per tile.  16 slots per look-up and unit: 206 us.
 template <typename T, int DP, int NT, int TILES, bool CL, bool SEL>
 __global__ void __launch_bounds__(kPdThreads, Paged4<T, DP, NT>::kBlocksPerSm) paged_decode4_kernel(
     const __grid_constant__ PagedDecodeParams p) {

@@ -9,11 +9,12 @@
 // 6.3 TB/s read and written (partner columns by a second load, two rows in flight: 375 us); 32 rows of
 // one token 3.0 us.
 //
-// 4-bit rows: bound by instructions (188 per 256 values of K, V and q; 8 prompts up to 4096 tokens, 16 / 8
-// heads of 128 in fp16 73 us for 244 MB).  The code of a value and the scale of a block are decided as exact
+// 4-bit rows: 193 instructions per 256 values of K, V and q bound them (77 % of issue slots, DRAM 36 % busy;
+// 8 prompts up to 4096 tokens, 16 / 8 heads of 128 in fp16 75 us for 244 MB).  The code of a value and the scale of a block are decided as exact
 // arithmetic decides: the fp32 value y is off by at most 2^-22 (|x c| + |x' s|), so a
 // code (scale) is taken where the values that much above and below it give the same
-// one, and computed in 64 bits where they do not (a warp in some thousand).  Values that
+// one, and computed in 64 bits where they do not (of rotated normal values about one block of 16 in
+// 2000, so about one unit of a warp, 16 blocks, in 125: a step of 128 rows and 8 kv heads has some).  Values that
 // are exact in 16 bits (v, columns that are not rotated) lie on a border or at least 2^-13
 // of a scale away from it: there y / scale is rounded to 2^-17, which restores what lay on it.
 #pragma once
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(kRopeThreads, !VEC ? 1 : PACKED && sizeof(T) =
             if ((col & 8) == 0) to[to_scale] = static_cast<uint8_t>(scale);
         }
     };
-    // rows of K or V into their records; true where one has to be done in 64 bits (a warp in some thousand)
+    // rows of K or V into their records; true where a block has to be done in 64 bits
     auto store4 = [&](float (&y)[8], float most, bool turned, bool whole, float unit, uint8_t* to, bool has) {
         if (unit != 1.0f) {
             most *= unit;
@@ -661,8 +662,9 @@ __device__ __forceinline__ void fp4_load8(const uint8_t* record, int line, int c
 // A block takes p.block consecutive tokens (up to 32): one lane of each warp looks up where a
 // token's slot lies, then the warps take a token's K or V rows in turn, 8 columns per lane and
 // several rows' loads in flight.  Rows that are none are zeros.  19525 tokens of 8 heads of 128 from
-// 4 bits to fp16 26 us (3.9 TB/s read and written, bound by instructions); a warp per token left HBM
-// idle for the chain of look-ups: 40 us.
+// 4 bits to fp16 26 us (3.9 TB/s read and written; 59 % of issue slots, warps wait for loads the rest: no
+// unit is full); a warp per token left HBM idle for the chain of look-ups: 40 us.  From bf16 pages 39049 tokens
+// 58 us (5.5 TB/s).
 constexpr int kGatherTokens = 32;
 
 template <typename T, int LPR, bool VEC, bool PACKED>

@@ -5,7 +5,7 @@
 // heads of a kv head that is one product,
 //     score = sum_d up_d hi_d + down_d lo_d,   up = sum_h max(q_h, 0), down = sum_h min(q_h, 0),
 // whatever the number of heads: 2 D products per page for 2 D elements read.  It is summed
-// in 64 bits, whose rate (half of fp32's) the reading does not leave behind: pages that a
+// in 64 bits, which does not bound it (the FP64 pipe is 9 % busy): pages that a
 // sum in 32 bits would mix up keep the order that their exact scores have.  That holds for
 // finite bounds and queries: where an infinity meets up or down = 0 (no query of that sign) the
 // product is NaN and the maximum need not be.  Any bound or query that is not finite makes the
@@ -352,8 +352,9 @@ __device__ __forceinline__ void select_row(const PagedSelectParams& p, SelectSha
 // shuffles.  The queries' sums lie in shared memory so that the 8 lanes' parts are side by side,
 // the pages' numbers beside them: both are fetched at once.  Then the blocks share the tokens'
 // selections.  32 rows of 256 to 512 pages, 8 heads of 128: 52 us with a look-up before every
-// page (20 us without, the selection included 21: 67 MB of bounds, 10 us at HBM's rate; the conversions
-// to 64 bits and the selection's rounds of counting are the rest).
+// page, 19 without, the selection included (50 MB of bounds, 8 us at HBM's rate; the FP64 pipe is 9 % busy, 34 %
+// of issue slots are used: a block's few warps wait for its rounds of loads, then for the selection's
+// rounds of counting).
 template <typename T, bool VEC, int TOKENS>
 __global__ void __launch_bounds__(kSelectThreads, TOKENS == 1 ? 3 : 2) paged_select_kernel(const __grid_constant__ PagedSelectParams p) {
     constexpr int MAXD = CHRONOS_PAGED_MAX_HEAD_DIM, GROUPS = kSelectThreads / 8;
